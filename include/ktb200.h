@@ -611,6 +611,58 @@ int ktb200_softmax_attn_tiles(int heads, int kv_heads, int maps, int n_tokens, i
 /* whether a tensor-core call runs the 256-row tiles on tcgen05 (csrc/softmax_attn_tc.cuh) */
 int ktb200_softmax_attn_prompt_tiles(const ktb200_softmax_attn_params* params, int n_tokens, int splits);
 
+/* The paged cache in 8 bits (csrc/fp8_cache.cu, csrc/fp8_attn.cu).  A page holds page_size tokens of every key/value head, head by head: k_codes [n_pages][kv_heads][page_size][dim]
+ * and v_codes [n_pages][kv_heads][page_size][vdim] (e4m3), scales [n_pages][kv_heads][2] (fp32, keys then values): a code stands for code * scale of its page and
+ * head.  Scales are powers of two: 2^e, e the smallest number in [-64, 64] with 448 * 2^e >= max |x| over the block's tokens (what is larger saturates, NaN stays NaN).
+ *   ktb200_fp8_cache_append   q [heads*dim] at q_off, k [kv_heads*dim] at k_off, v [kv_heads*vdim] at v_off of proj's rows; q and k head by head: qk_norm 0 nothing, 1
+ *     x / sqrt(mean(x^2) + eps), 3 the same times q_weight / k_weight [dim]; then a turn of the first rot_dims columns (rot_layout as above).  q of all n_tokens tokens to
+ *     q_out [n_tokens][heads][dim]; k, v into the cache.  A portion that begins inside a page keeps the page's earlier tokens (their codes move where the
+ *     scale grows: exactly, but for what becomes subnormal); one that begins at a page's first token starts its blocks anew.  Codes of other rows are left as they were.
+ *   ktb200_fp8_cache_attn     out[t * out_stride + h vdim + c] = out_scale * sum_j w_j v_j / (sum_j w_j + exp(sink[h])), w_j = exp(cap(scale head_scale[h] q.k_j)),
+ *     with the masks, cap and optional pointers of ktb200_softmax_attn.  A row that sees no key is zero.  splits > 1 cuts the key range (workspace:
+ *     ktb200_fp8_cache_attn_workspace bytes, of this call alone); ktb200_fp8_cache_attn_splits: how many a call over up to max_keys keys should take.
+ * seqs: rows (first token's row, token count) of the n_seqs portions, seqs_stride apart.  A portion's tokens stand at consecutive positions from pos[first row], in the pages of table row
+ * slot[first row] (a ring: page p in column p % max_pages); a sequence has one portion in a call, and windows reach back (max_pages - 1) * page_size positions at most.
+ * Rows of tokens in no portion are left as they were, keys in pages outside [0, n_pages) are neither written nor seen.  The stream's device has to be the current one. */
+typedef struct {
+    const void* proj;
+    long proj_stride;
+    int q_off, k_off, v_off, heads, kv_heads, dim, vdim, rot_dims, rot_layout;
+    const double* inv_freq;
+    int qk_norm;
+    const void *q_weight, *k_weight;
+    float eps;
+    const int *pos, *slot, *seqs;
+    int seqs_stride, n_seqs;
+    const int* page_table;
+    int n_slots, max_pages, page_size, n_pages;
+    void *k_codes, *v_codes;
+    float* scales;
+    void* q_out;
+} ktb200_fp8_append_params;
+int ktb200_fp8_cache_append(const ktb200_fp8_append_params* params, int n_tokens, int dtype, void* stream);
+typedef struct {
+    const void* q;
+    int heads, kv_heads, dim, vdim;
+    float scale;
+    const float* head_scale;
+    float softcap;
+    int window, chunk;
+    const float* sink;
+    float out_scale;
+    const int *pos, *slot, *seqs;
+    int seqs_stride, n_seqs;
+    const int* page_table;
+    int n_slots, max_pages, page_size, n_pages;
+    const void *k_codes, *v_codes;
+    const float* scales;
+    void* out;
+    long out_stride;
+} ktb200_fp8_attn_params;
+size_t ktb200_fp8_cache_attn_workspace(int n_tokens, int heads, int vdim, int splits);
+int ktb200_fp8_cache_attn_splits(const ktb200_fp8_attn_params* params, int n_tokens, int max_keys, int dtype, int allow_tensor_cores);
+int ktb200_fp8_cache_attn(const ktb200_fp8_attn_params* params, int n_tokens, int splits, float* workspace, int dtype, int allow_tensor_cores, void* stream);
+
 /* Mamba-2 (csrc/ssd.cu): proj rows hold [x heads*vdim | B groups*state_size | C groups*state_size] at xbc_off and one step logit per head at
  * dt_off; conv_w [channels][taps] (last column = current token), conv_b [channels]; state rows [S heads*state_size*vdim | filter inputs
  * (taps - 1)*channels] fp32, row stride state_stride; portions seqs[0..3][s] and seq_of as for ktb200_delta_prep.

@@ -1,0 +1,240 @@
+// Soft-max attention over grouped key/value heads in the paged e4m3 cache of fp8_cache.cuh (libktb200_seq.so).
+//
+//   ktb200_fp8_cache_attn   o_i = sum_j w_ij v_j / sum_j w_ij over the keys j <= i with i - j < window (window > 0) and floor(j / chunk) == floor(i / chunk) (chunk > 0);
+//                           w_ij = exp(s_ij), s_ij = cap(scale t_h q_i.k_j), cap(s) = c tanh(s / c), c = softcap (softcap <= 0: none), t_h a number per query head
+//                           (optional); exp(sink_h) joins the denominator (optional); o times out_scale.  k_j, v_j: codes times their blocks' scales.  Query head h reads
+//                           key/value head h / (H / G).  The key range is cut into splits for few tokens on long ranges.
+//
+// A portion's tokens stand at consecutive positions from pos[its first token].  Keys in pages that are not there (ids outside the pool) are not seen; a row that sees no key
+// becomes zero.  Rows of tokens that belong to no portion are left as they were.
+#include <cuda_bf16.h>
+
+#include <algorithm>
+
+#include "fp8_cache.cuh"
+
+namespace ktb {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kFp8MaxSplits = 128;
+
+struct Fp8Attn {
+    const void* q;
+    int H, G, d, dv;
+    float scale;
+    const float* head_scale;
+    float softcap;
+    int window, chunk;
+    const float* sink;
+    float out_scale;
+    const int *pos, *slot, *seqs;
+    int seqs_stride, n_seqs, n_tokens;
+    Fp8Pages pages;
+    const uint8_t *k_codes, *v_codes;
+    const float* scales;
+    void* out;
+    long out_stride;
+    float* partial;      // [T][H][splits][dv + 2]: reference maximum, sum, un-normalised weighted values
+    int splits;
+};
+__device__ __forceinline__ int fp8_first_visible(int p, int window, int chunk) {
+    int lo = window > 0 ? max(0, p - window + 1) : 0;
+    if (chunk > 0) lo = max(lo, p - p % chunk);
+    return lo;
+}
+// tokens of portion s (none where its rows are not those of the step)
+__device__ __forceinline__ int fp8_portion(const Fp8Attn& a, int s) {
+    const int start = a.seqs[s], len = a.seqs[a.seqs_stride + s];
+    return len <= 0 || start < 0 || start > a.n_tokens - len || a.pos[start] < 0 ? 0 : len;
+}
+
+// ------------------------------------------------------------------------------------------------ CUDA cores: any head size up to 256, fp32 or bf16
+// grid (tokens, G * head blocks, splits); a warp per query head, the CTA's heads share one key/value head.  Tiles of 32 keys in shared memory as fp32 (code * scale, exact):
+// lane = key for the scores, lane = value column for the weighted sum; running maximum and sum per warp, natural exponentials.
+constexpr int kFgTile = 32, kFgCols = 8;
+template <typename T> __global__ void __launch_bounds__(256) fp8_attn_kernel(const Fp8Attn a) {
+    extern __shared__ __align__(16) float fg_smem[];
+    __shared__ int info[2];
+    const int HB = blockDim.x >> 5, R = a.H / a.G, hblocks = (R + HB - 1) / HB, d = a.d, dv = a.dv, ps = a.pages.page_size;
+    const int g = blockIdx.y / hblocks, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = (blockIdx.y % hblocks) * HB + warp, h = g * R + r;
+    const bool live = r < R;
+    griddep_launch_dependents();
+    griddep_wait();
+    if (warp == 0) {
+        int s, item;
+        const bool found = fp8_find(blockIdx.x, a.n_seqs, [&](int i) { return fp8_portion(a, i); }, s, item);
+        if (lane == 0) { info[0] = found ? s : -1; info[1] = item; }
+    }
+    __syncthreads();
+    if (info[0] < 0) return;
+    const int start = a.seqs[info[0]], p = a.pos[start] + info[1], slot = a.slot[start];
+    const long t = start + info[1];
+    float* qs = fg_smem;
+    float* Ks = qs + HB * d;
+    float* Vs = Ks + kFgTile * (d + 1);
+    float* pw = Vs + kFgTile * dv;
+    const int lo = fp8_first_visible(p, a.window, a.chunk), n_keys = p + 1 - lo;
+    const int per = ((n_keys + a.splits - 1) / a.splits + kFgTile - 1) / kFgTile * kFgTile;
+    const int k_lo = lo + blockIdx.z * per, k_hi = min(p + 1, k_lo + per);
+    float acc[kFgCols];
+#pragma unroll
+    for (int c = 0; c < kFgCols; c++) acc[c] = 0.f;
+    float m = -INFINITY, l = 0.f;
+    if (live) {
+        const float sc = a.head_scale ? a.scale * a.head_scale[h] : a.scale;
+        for (int i = lane; i < d; i += 32) qs[warp * d + i] = to_f(((const T*)a.q)[(t * a.H + h) * d + i]) * sc;
+    }
+    for (int j0 = k_lo; j0 < k_hi; j0 += kFgTile) {
+        __syncthreads();
+        const int nk = min(kFgTile, k_hi - j0);
+        unsigned here = 0;      // keys of the tile whose pages are there
+        for (int j = 0; j < nk; j++) {
+            const int kp = j0 + j, page = a.pages.page(slot, kp / ps);
+            if (page < 0) {
+                for (int i = threadIdx.x; i < dv; i += blockDim.x) Vs[j * dv + i] = 0.f;
+                continue;
+            }
+            here |= 1u << j;
+            const long block = (long)page * a.G + g;
+            const float ks = a.scales[2 * block], vs = a.scales[2 * block + 1];
+            const uint8_t *k = a.k_codes + (block * ps + kp % ps) * d, *v = a.v_codes + (block * ps + kp % ps) * dv;
+            for (int i = threadIdx.x; i < d; i += blockDim.x) Ks[j * (d + 1) + i] = __half2float(__half(__nv_cvt_fp8_to_halfraw(k[i], __NV_E4M3))) * ks;
+            for (int i = threadIdx.x; i < dv; i += blockDim.x) Vs[j * dv + i] = __half2float(__half(__nv_cvt_fp8_to_halfraw(v[i], __NV_E4M3))) * vs;
+        }
+        __syncthreads();
+        if (!live) continue;
+        float s = -INFINITY;
+        if (here >> lane & 1) {
+            float q_k = 0.f;
+            const float *kr = Ks + lane * (d + 1), *qr = qs + warp * d;
+            for (int i = 0; i < d; i++) q_k = fmaf(qr[i], kr[i], q_k);
+            s = a.softcap > 0.f ? a.softcap * tanhf(q_k / a.softcap) : q_k;
+        }
+        const float mn = fmaxf(m, warp_max(s)), u = mn == -INFINITY ? 0.f : mn;
+        const float corr = expf(m - u), pj = expf(s - u);
+        l = l * corr + warp_sum(pj);
+        m = mn;
+        pw[warp * kFgTile + lane] = pj;
+        __syncwarp();
+#pragma unroll
+        for (int c = 0; c < kFgCols; c++) acc[c] *= corr;
+        for (int j = 0; j < nk; j++) {
+            const float wj = pw[warp * kFgTile + j];
+#pragma unroll
+            for (int c = 0; c < kFgCols; c++)
+                if (lane + 32 * c < dv) acc[c] = fmaf(wj, Vs[j * dv + lane + 32 * c], acc[c]);
+        }
+        __syncwarp();
+    }
+    if (!live) return;
+    if (a.partial) {
+        float* o = a.partial + ((t * a.H + h) * a.splits + blockIdx.z) * (dv + 2);
+        if (lane == 0) { o[0] = m; o[1] = l; }
+#pragma unroll
+        for (int c = 0; c < kFgCols; c++)
+            if (lane + 32 * c < dv) o[2 + lane + 32 * c] = acc[c];
+        return;
+    }
+    if (a.sink) {
+        const float mn = fmaxf(m, a.sink[h]), corr = expf(m - mn);
+        l = l * corr + expf(a.sink[h] - mn);
+#pragma unroll
+        for (int c = 0; c < kFgCols; c++) acc[c] *= corr;
+    }
+    const float inv = l > 0.f || l != l ? a.out_scale / l : 0.f;
+    T* out = (T*)a.out + t * a.out_stride + (long)h * dv;
+#pragma unroll
+    for (int c = 0; c < kFgCols; c++)
+        if (lane + 32 * c < dv) out[lane + 32 * c] = from_f<T>(acc[c] * inv);
+}
+
+// The parts of a cut key range, one CTA of 128 threads for each (token, head): the parts' weights once in shared memory (a part without a key has maximum -inf and weighs
+// nothing; the sink joins the sum), then the columns side by side, parts in order.  `unit`: what turns a difference of maxima into a power of two.
+template <typename T> __global__ void __launch_bounds__(128) fp8_merge_kernel(const Fp8Attn a, float unit) {
+    __shared__ float wgt[kFp8MaxSplits], red[4];
+    __shared__ int mine;
+    griddep_launch_dependents();
+    griddep_wait();
+    const long row = blockIdx.x;
+    const int t = (int)(row / a.H), h = (int)(row % a.H), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, splits = a.splits, dv = a.dv;
+    // a token of no portion has no parts
+    if (tid == 0) mine = 0;
+    __syncthreads();
+    for (int s = tid; s < a.n_seqs; s += 128) {
+        const int len = fp8_portion(a, s);
+        if (t >= a.seqs[s] && t - a.seqs[s] < len) mine = 1;
+    }
+    __syncthreads();
+    if (!mine) return;
+    const float* part = a.partial + row * splits * (dv + 2);
+    const float ms = tid < splits ? part[(long)tid * (dv + 2)] : -INFINITY, ls = tid < splits ? part[(long)tid * (dv + 2) + 1] : 0.f;
+    float m = warp_max(ms);
+    if (lane == 0) red[warp] = m;
+    __syncthreads();
+    m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    const float sink = a.sink ? a.sink[h] * (kLog2e / unit) : -INFINITY;
+    m = fmaxf(m, sink);
+    __syncthreads();
+    const float e = ms > -INFINITY ? exp2f((ms - m) * unit) : 0.f;
+    const float part_l = warp_sum(ls * e);
+    if (lane == 0) red[warp] = part_l;
+    __syncthreads();
+    float l = (red[0] + red[1]) + (red[2] + red[3]);
+    if (a.sink) l += exp2f((sink - m) * unit);
+    if (tid < splits) wgt[tid] = l > 0.f || l != l ? e / l : 0.f;
+    __syncthreads();
+    T* out = (T*)a.out + t * a.out_stride + (long)h * dv;
+    for (int c = tid; c < dv; c += 128) {
+        float acc = 0.f;
+#pragma unroll 8
+        for (int s = 0; s < splits; s++) acc = fmaf(wgt[s], part[(long)s * (dv + 2) + 2 + c], acc);
+        out[c] = from_f<T>(acc * a.out_scale);
+    }
+}
+
+}  // namespace ktb
+
+using namespace ktb;
+
+extern "C" size_t ktb200_fp8_cache_attn_workspace(int n_tokens, int heads, int vdim, int splits) {
+    return splits > 1 ? (size_t)n_tokens * heads * splits * (vdim + 2) * sizeof(float) : 0;
+}
+
+// Cut the key range when a small batch would leave most SMs idle on a long one
+extern "C" int ktb200_fp8_cache_attn_splits(const ktb200_fp8_attn_params* c, int n_tokens, int max_keys, int dtype, int allow_tensor_cores) {
+    if (!c || c->heads <= 0 || c->kv_heads <= 0 || n_tokens <= 0) return 1;
+    const int R = c->heads / c->kv_heads;
+    const long ctas = (long)n_tokens * c->kv_heads * ((R + 7) / 8);
+    if (ctas >= 148 || max_keys <= 256) return 1;
+    return (int)std::max<long>(1, std::min<long>({64, max_keys / 128, 592 / ctas}));
+}
+
+extern "C" int ktb200_fp8_cache_attn(const ktb200_fp8_attn_params* c, int n_tokens, int splits, float* workspace, int dtype, int allow_tensor_cores, void* stream) {
+    if (!c || c->heads <= 0 || c->kv_heads <= 0 || c->heads % c->kv_heads || c->dim <= 0 || c->dim > 32 * kFgCols || c->vdim <= 0 || c->vdim > 32 * kFgCols || c->page_size <= 0 ||
+        c->max_pages <= 0 || c->n_pages < 0 || c->n_slots <= 0 || c->n_seqs < 0 || c->window < 0 || c->chunk < 0 || c->out_stride < (long)c->heads * c->vdim) {
+        set_error("fp8_cache_attn: bad argument (head sizes up to %d)", 32 * kFgCols);
+        return KTB200_EINVAL;
+    }
+    if (dtype != KTB200_TYPE_BF16 && dtype != KTB200_TYPE_F32) { set_error("fp8_cache_attn: dtype must be bf16 or f32"); return KTB200_EINVAL; }
+    if (splits < 1 || splits > kFp8MaxSplits) { set_error("fp8_cache_attn: 1 to %d splits", kFp8MaxSplits); return KTB200_EINVAL; }
+    if (n_tokens <= 0 || c->n_seqs == 0) return KTB200_OK;
+    if (!c->q || !c->pos || !c->slot || !c->seqs || !c->page_table || !c->k_codes || !c->v_codes || !c->scales || !c->out) { set_error("fp8_cache_attn: null pointer"); return KTB200_EINVAL; }
+    if (splits > 1 && !workspace) { set_error("fp8_cache_attn: workspace missing"); return KTB200_EINVAL; }
+    const int R = c->heads / c->kv_heads, HB = std::min(R, 8), hblocks = (R + HB - 1) / HB;
+    if ((long)c->kv_heads * hblocks > 65535 || (long)n_tokens * c->heads > 0x7fffffffL) { set_error("fp8_cache_attn: too many heads or tokens"); return KTB200_EINVAL; }
+    const cudaStream_t s = (cudaStream_t)stream;
+    const Fp8Attn a{c->q, c->heads, c->kv_heads, c->dim, c->vdim, c->scale, c->head_scale, c->softcap, c->window, c->chunk, c->sink, c->out_scale, c->pos, c->slot, c->seqs, c->seqs_stride,
+                    c->n_seqs, n_tokens, {c->page_table, c->n_slots, c->max_pages, c->page_size, c->n_pages}, (const uint8_t*)c->k_codes, (const uint8_t*)c->v_codes, c->scales, c->out,
+                    c->out_stride, splits > 1 ? workspace : nullptr, splits};
+    const size_t smem = ((size_t)HB * c->dim + (size_t)kFgTile * (c->dim + 1) + (size_t)kFgTile * c->vdim + (size_t)HB * kFgTile) * sizeof(float);
+    const dim3 grid(n_tokens, c->kv_heads * hblocks, splits);
+    const bool bf16 = dtype == KTB200_TYPE_BF16;
+    KTB_CUDA_CHECK(raise_smem_limit(bf16 ? (const void*)fp8_attn_kernel<__nv_bfloat16> : (const void*)fp8_attn_kernel<float>, smem));
+    KTB_CUDA_CHECK(launch_pdl(bf16 ? fp8_attn_kernel<__nv_bfloat16> : fp8_attn_kernel<float>, grid, dim3(HB * 32), smem, s, a));
+    count_launch();
+    if (splits > 1) {
+        KTB_CUDA_CHECK(launch_pdl(bf16 ? fp8_merge_kernel<__nv_bfloat16> : fp8_merge_kernel<float>, dim3((unsigned)((long)n_tokens * c->heads)), dim3(128), (size_t)0, s, a, kLog2e));
+        count_launch();
+    }
+    return KTB200_OK;
+}

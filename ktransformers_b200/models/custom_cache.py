@@ -104,6 +104,32 @@ class ForwardBatch:
         return self.turns[key]
 
 
+class Fp8CacheLayer:
+    """One cache layer in 8 bits: `k` [pages, kv_heads, page_size, dim] and `v` [pages, kv_heads, page_size, vdim] (float8_e4m3fn), `scales` [pages, kv_heads, 2]
+    (fp32: keys, values).  A code stands for code * scale of its page and head; scales are powers of two.  Written by `operators.attention.fp8_cache_append`, read by
+    `operators.attention.fp8_cache_attention` (csrc/fp8_cache.cu, csrc/fp8_attn.cu)."""
+
+    __slots__ = ("k", "v", "scales")
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, scales: torch.Tensor):
+        if k.dtype != torch.float8_e4m3fn or v.dtype != torch.float8_e4m3fn or scales.dtype != torch.float32:
+            raise ValueError("an 8-bit cache layer has float8_e4m3fn codes and float32 scales")
+        if k.dim() != 4 or v.dim() != 4 or k.shape[:3] != v.shape[:3] or tuple(scales.shape) != (k.shape[0], k.shape[1], 2):
+            raise ValueError(f"an 8-bit cache layer has k, v [pages, heads, page_size, size] and scales [pages, heads, 2], got {tuple(k.shape)}, {tuple(v.shape)}, {tuple(scales.shape)}")
+        if not (k.is_contiguous() and v.is_contiguous() and scales.is_contiguous()):
+            raise ValueError("an 8-bit cache layer's tensors have to be contiguous")
+        self.k, self.v, self.scales = k, v, scales
+
+    @classmethod
+    def empty(cls, pages: int, page_size: int, kv_heads: int, dim: int, vdim: int, device="cuda") -> "Fp8CacheLayer":
+        codes = lambda d: torch.zeros((pages, kv_heads, page_size, d), dtype=torch.float8_e4m3fn, device=device)
+        return cls(codes(dim), codes(vdim), torch.ones((pages, kv_heads, 2), dtype=torch.float32, device=device))
+
+    def dequantize(self) -> Tuple[torch.Tensor, torch.Tensor]:
+        """What the codes stand for: keys and values in fp32."""
+        return self.k.float() * self.scales[:, :, None, None, 0], self.v.float() * self.scales[:, :, None, None, 1]
+
+
 class PagedStateCache:
     """Pages of per-token cache rows plus fixed-size per-sequence state rows, for models whose layers keep a (windowed) latent
     cache and a previous-token row.
@@ -123,19 +149,24 @@ class PagedStateCache:
     batch row; this manager adds allocation, release and the recurrent rows."""
 
     def __init__(self, row_widths, state_width, max_tokens: int, max_slots: int, device, dtype=torch.bfloat16, page_size: int = 64,
-                 window: Optional[int] = None, chunks=None):
+                 window: Optional[int] = None, chunks=None, fp8_heads=None):
         """`row_widths[l]`: cache values per token of cache layer l (0: the layer caches no rows); `state_width`: fp32 state
         values per sequence, one number for all layers or one per layer (0: none).  A model whose layers run several times
         with separate caches counts every run as a cache layer.  `window`: the largest sliding look-back of any caching layer
         (None: unbounded); `chunks`: the chunk lengths of the caching layers when EVERY one of them reads only keys of the
-        query's own chunk (position p sees p - p mod C onwards) — then the pages before the earliest chunk start are given back."""
+        query's own chunk (position p sees p - p mod C onwards) — then the pages before the earliest chunk start are given back.  `fp8_heads[l]`:
+        (key/value heads, key size, value size) of the layers whose rows are held in 8 bits (`Fp8CacheLayer`), None for the others."""
         self.device, self.dtype, self.page_size, self.window = torch.device(device), dtype, int(page_size), window
         self.chunks = sorted({int(c) for c in chunks}) if chunks else None
         self.max_slots = int(max_slots)
         # every live sequence may hold one partly filled page at each end of its range
         self.num_pages = (int(max_tokens) + page_size - 1) // page_size + 2 * self.max_slots
         self.max_pages_per_seq = (int(max_tokens) + page_size - 1) // page_size + 2
-        self.key_cache = [torch.zeros((self.num_pages, page_size, int(w)), dtype=dtype, device=device) for w in row_widths]
+        fp8_heads = list(fp8_heads) if fp8_heads is not None else [None] * len(row_widths)
+        if len(fp8_heads) != len(row_widths):
+            raise ValueError("one entry of fp8_heads per cache layer")
+        self.key_cache = [Fp8CacheLayer.empty(self.num_pages, page_size, *f, device=device) if f is not None else torch.zeros((self.num_pages, page_size, int(w)), dtype=dtype, device=device)
+                          for w, f in zip(row_widths, fp8_heads)]
         state_widths = [int(state_width)] * len(row_widths) if isinstance(state_width, int) else [int(w) for w in state_width]
         if len(state_widths) != len(row_widths):
             raise ValueError("one state width per cache layer")

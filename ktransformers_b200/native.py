@@ -132,6 +132,18 @@ class SoftmaxAttnParams(C.Structure):
                        "p:pos,slot,seqs i:seqs_stride,n_seqs p:page_table i:max_pages,page_size p:cache,out l:out_stride")
 
 
+class Fp8AppendParams(C.Structure):
+    """ktb200_fp8_append_params (include/ktb200.h)"""
+    _fields_ = _fields("p:proj l:proj_stride i:q_off,k_off,v_off,heads,kv_heads,dim,vdim,rot_dims,rot_layout p:inv_freq i:qk_norm p:q_weight,k_weight f:eps p:pos,slot,seqs "
+                       "i:seqs_stride,n_seqs p:page_table i:n_slots,max_pages,page_size,n_pages p:k_codes,v_codes,scales,q_out")
+
+
+class Fp8AttnParams(C.Structure):
+    """ktb200_fp8_attn_params (include/ktb200.h)"""
+    _fields_ = _fields("p:q i:heads,kv_heads,dim,vdim f:scale p:head_scale f:softcap i:window,chunk p:sink f:out_scale p:pos,slot,seqs i:seqs_stride,n_seqs p:page_table "
+                       "i:n_slots,max_pages,page_size,n_pages p:k_codes,v_codes,scales,out l:out_stride")
+
+
 class SsdParams(C.Structure):
     """ktb200_ssd_params (include/ktb200.h)"""
     _fields_ = _fields("p:proj l:proj_stride i:xbc_off,dt_off p:conv_w,conv_b i:taps p:dt_bias,a_log,d_skip i:heads,groups,state_size,vdim p:seq_of,seqs i:seqs_stride,n_seqs p:state "
@@ -206,6 +218,11 @@ SEQ_SYMBOLS = {
     "ktb200_softmax_attn_uses_tensor_cores": (_I, [_I, _I, _I, _I, _I, _I]),
     "ktb200_softmax_attn_tiles": (_I, [_I, _I, _I, _I, _I]),
     "ktb200_softmax_attn_prompt_tiles": (_I, [C.POINTER(SoftmaxAttnParams), _I, _I]),
+    # csrc/fp8_cache.cu, csrc/fp8_attn.cu
+    "ktb200_fp8_cache_append": (_I, [C.POINTER(Fp8AppendParams), _I, _I, _VP]),
+    "ktb200_fp8_cache_attn_workspace": (C.c_size_t, [_I, _I, _I, _I]),
+    "ktb200_fp8_cache_attn_splits": (_I, [C.POINTER(Fp8AttnParams), _I, _I, _I, _I]),
+    "ktb200_fp8_cache_attn": (_I, [C.POINTER(Fp8AttnParams), _I, _I, _VP, _I, _I, _VP]),
     # csrc/retention.cu, csrc/selective_scan.cu
     "ktb200_turn_table": (_I, [_VP, _VP, _I, _VP, _I, _VP]),
     "ktb200_retention_chunk_supported": (_I, [_I, _I, _I]),

@@ -8,6 +8,7 @@ TMEM + TMA, csrc/mla.cu); the cache write is ktb200_mla_kv_write; the projection
 GEMVs over the bf16 halves of kv_b_proj; torch.matmul for other dtypes).  Prefill (q_len > 1 without absorb) is outside this path and raises."""
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import math
 from typing import Optional, Tuple
@@ -20,6 +21,14 @@ from ..models.modeling_deepseek_v3 import DeepseekV3Attention, DeepseekV3RMSNorm
 from ..util.utils import InferenceState
 from .base_operator import BaseInjectedModule
 from .flashinfer_wrapper import MLAWrapper, MLAWrapperSingleton
+
+
+_HERE = contextlib.nullcontext()
+
+
+def _device_of(dev):
+    """`dev` as the current device: kernels are launched on the current one, whatever their stream's"""
+    return _HERE if dev.index is None or dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
 
 
 def _is_plain(module, cls) -> bool:
@@ -506,6 +515,91 @@ def qkv_prep(proj: torch.Tensor, batch, cache, kv: torch.Tensor, heads: int, kv_
                              q_out=q.data_ptr())
     native.check_seq(native.seq_lib().ktb200_qkv_prep(C.byref(a), T, native.GGML_BF16 if dt == torch.bfloat16 else native.GGML_F32, torch.cuda.current_stream(proj.device).cuda_stream))
     return q
+
+
+def _fp8_batch(what: str, rows: torch.Tensor, kv, batch, cache, kv_heads: int, dim: int, vdim: int):
+    """Checks what the 8-bit cache's two calls share; the storage type's code and the stream"""
+    k, v = kv.k, kv.v
+    if not rows.is_cuda:
+        raise ValueError(f"{what}: CUDA tensors only")
+    if rows.dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError(f"{what}: bfloat16 or float32 rows, got {rows.dtype}")
+    if k.shape[1] != kv_heads or k.shape[2] != cache.page_size or k.shape[3] != dim or v.shape[3] != vdim:
+        raise ValueError(f"{what}: the cache layer holds pages of {k.shape[2]} tokens of {k.shape[1]} heads of {k.shape[3]} + {v.shape[3]}, the call has {cache.page_size}, {kv_heads}, {dim} + {vdim}")
+    if batch.seqs is None or batch.seqs.dtype != torch.int32 or batch.pos.dtype != torch.int32 or batch.slot.dtype != torch.int32 or cache.page_table.dtype != torch.int32:
+        raise ValueError(f"{what}: needs int32 pos, slot, seqs and page table")
+    T, dev = rows.shape[0], rows.device
+    if batch.pos.shape[0] < T or batch.slot.shape[0] < T or batch.n_seqs > batch.seqs.shape[1]:
+        raise ValueError(f"{what}: {T} tokens, but {batch.pos.shape[0]} positions, {batch.slot.shape[0]} slots; {batch.n_seqs} portions of {batch.seqs.shape[1]}")
+    if batch.pos.stride(0) != 1 or batch.slot.stride(0) != 1 or batch.seqs.stride(1) != 1 or cache.page_table.stride(1) != 1 or cache.page_table.stride(0) != cache.max_pages_per_seq:
+        raise ValueError(f"{what}: index rows and page table rows have to be contiguous")
+    if not (k.device == batch.pos.device == batch.slot.device == batch.seqs.device == cache.page_table.device == dev):
+        raise ValueError(f"{what}: all tensors have to be on one device")
+    return native.GGML_BF16 if rows.dtype == torch.bfloat16 else native.GGML_F32, torch.cuda.current_stream(dev).cuda_stream
+
+
+def _check_vectors(what: str, dev, **named):
+    """the optional per-head and per-column vectors: (tensor, length, dtype)"""
+    for name, (t, n, dt) in named.items():
+        if t is not None and (t.numel() != n or t.dtype != dt or t.device != dev or not t.is_contiguous()):
+            raise ValueError(f"{what}: {name} has to be {n} contiguous values of {dt} on {dev}")
+
+
+def fp8_cache_append(proj: torch.Tensor, batch, cache, kv, heads: int, kv_heads: int, dim: int, vdim: int, offsets, rot=None, inv_freq: Optional[torch.Tensor] = None, qk_norm: int = 0,
+                     eps: float = 0.0, q_weight: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """`qkv_prep` for a layer held in 8 bits (`kv`: models.custom_cache.Fp8CacheLayer): from a projection's q, k and v columns (`offsets`) to the queries
+    [T, heads, dim] and the layer's codes and scales, one `ktb200_fp8_cache_append` launch (csrc/fp8_cache.cu).  q and k: unit rms per row (qk_norm = 1), or times q_weight /
+    k_weight [dim] ahead of the rotation (qk_norm = 3).  A scale belongs to one page and head: tokens appended to a page whose scale they exceed have its earlier codes moved."""
+    what = "fp8_cache_append"
+    code, st = _fp8_batch(what, proj, kv, batch, cache, kv_heads, dim, vdim)
+    T, dev, dt = proj.shape[0], proj.device, proj.dtype
+    q_off, k_off, v_off = offsets
+    if proj.dim() != 2 or proj.stride(1) != 1 or min(offsets) < 0 or max(q_off + heads * dim, k_off + kv_heads * dim, v_off + kv_heads * vdim) > proj.shape[1]:
+        raise ValueError(f"{what}: rows of proj {tuple(proj.shape)} do not hold q, k and v at {tuple(offsets)}")
+    rot_dims = rot.dims if rot is not None else 0
+    if rot_dims and (inv_freq is None or inv_freq.numel() != rot_dims // 2 or inv_freq.dtype != torch.float64 or inv_freq.device != dev or not inv_freq.is_contiguous()):
+        raise ValueError(f"{what}: inv_freq has to be {rot_dims // 2} contiguous values of torch.float64 on {dev}")
+    if qk_norm == 3:
+        if q_weight is None or k_weight is None:
+            raise ValueError(f"{what}: qk_norm 3 needs both weights")
+        _check_vectors(what, dev, q_weight=(q_weight, dim, dt), k_weight=(k_weight, dim, dt))
+    q = torch.empty((T, heads, dim), dtype=dt, device=dev)
+    table = cache.page_table
+    a = native.Fp8AppendParams(proj.data_ptr(), proj.stride(0), q_off, k_off, v_off, heads, kv_heads, dim, vdim, rot_dims, rot.layout_code if rot_dims else 0,
+                               inv_freq.data_ptr() if rot_dims else None, qk_norm, q_weight.data_ptr() if qk_norm == 3 else None, k_weight.data_ptr() if qk_norm == 3 else None, eps,
+                               batch.pos.data_ptr(), batch.slot.data_ptr(), batch.seqs.data_ptr(), batch.seqs.stride(0), batch.n_seqs, table.data_ptr(), table.shape[0], table.shape[1],
+                               cache.page_size, kv.k.shape[0], kv.k.data_ptr(), kv.v.data_ptr(), kv.scales.data_ptr(), q.data_ptr())
+    with _device_of(dev):
+        native.check_seq(native.seq_lib().ktb200_fp8_cache_append(C.byref(a), T, code, st))
+    return q
+
+
+def fp8_cache_attention(q: torch.Tensor, kv, batch, cache, heads: int, kv_heads: int, dim: int, vdim: int, scale: float, head_scale: Optional[torch.Tensor] = None,
+                        softcap: Optional[float] = None, window: Optional[int] = None, chunk: Optional[int] = None, tensor_cores: bool = True, sink: Optional[torch.Tensor] = None,
+                        out: Optional[torch.Tensor] = None, out_scale: float = 1.0) -> torch.Tensor:
+    """`paged_softmax_attention` over a layer held in 8 bits (`kv`: models.custom_cache.Fp8CacheLayer), with its masks, head scales, cap and sink
+    (`ktb200_fp8_cache_attn`, csrc/fp8_attn.cu): o [T, heads * vdim] of the queries q [T, heads, dim] that `fp8_cache_append` gives, to `out` (a view of any row stride)
+    or a new tensor.  Rows of tokens in none of the batch's portions are left as they were (in a new tensor: as they came)."""
+    what = "fp8_cache_attention"
+    code, st = _fp8_batch(what, q, kv, batch, cache, kv_heads, dim, vdim)
+    T, dev, dt = q.shape[0], q.device, q.dtype
+    if q.numel() != T * heads * dim or not q.is_contiguous():
+        raise ValueError(f"{what}: q has to be contiguous [T, {heads}, {dim}], got {tuple(q.shape)}")
+    _check_vectors(what, dev, head_scale=(head_scale, heads, torch.float32), sink=(sink, heads, torch.float32))
+    if out is None:
+        out = torch.empty((T, heads * vdim), dtype=dt, device=dev)
+    elif tuple(out.shape) != (T, heads * vdim) or out.dtype != dt or out.device != dev or out.stride(1) != 1:
+        raise ValueError(f"{what}: out has to be [{T}, {heads * vdim}] of {dt} on {dev}, columns side by side")
+    table, lib = cache.page_table, native.seq_lib()
+    a = native.Fp8AttnParams(q.data_ptr(), heads, kv_heads, dim, vdim, scale, head_scale.data_ptr() if head_scale is not None else None, softcap or 0.0, window or 0, chunk or 0,
+                             sink.data_ptr() if sink is not None else None, out_scale, batch.pos.data_ptr(), batch.slot.data_ptr(), batch.seqs.data_ptr(), batch.seqs.stride(0),
+                             batch.n_seqs, table.data_ptr(), table.shape[0], table.shape[1], cache.page_size, kv.k.shape[0], kv.k.data_ptr(), kv.v.data_ptr(), kv.scales.data_ptr(),
+                             out.data_ptr(), out.stride(0))
+    with _device_of(dev):
+        splits = lib.ktb200_fp8_cache_attn_splits(C.byref(a), T, batch.max_kv, code, int(tensor_cores))
+        ws = torch.empty(lib.ktb200_fp8_cache_attn_workspace(T, heads, vdim, splits) // 4, dtype=torch.float32, device=dev) if splits > 1 else None
+        native.check_seq(lib.ktb200_fp8_cache_attn(C.byref(a), T, splits, ws.data_ptr() if ws is not None else None, code, int(tensor_cores), st))
+    return out
 
 
 class KCappedWindowAttention(torch.nn.Module):

@@ -1,0 +1,313 @@
+"""The paged e4m3 cache: append (rotation, norms, codes, scales) and attention, against 64-bit forms (fp8_cache_util)."""
+import ctypes as C
+import math
+from types import SimpleNamespace
+
+import pytest
+import torch
+
+import fp8_cache_util as U
+from ktransformers_b200 import native
+from ktransformers_b200.models.custom_cache import Fp8CacheLayer, PagedStateCache
+from ktransformers_b200.operators.attention import fp8_cache_append, fp8_cache_attention
+
+DT = {"bf16": torch.bfloat16, "fp32": torch.float32}
+HALF_STEP = {torch.bfloat16: 2.0 ** -8, torch.float32: 2.0 ** -24}
+ROT = lambda dims, layout: SimpleNamespace(dims=dims, layout_code=layout)
+INV = lambda dims: 10000.0 ** (-torch.arange(0, dims, 2, dtype=torch.float64) / max(dims, 1))
+
+
+def filled(total, G, ps, d, dv, seed, wide=0):
+    """a pool that holds something everywhere; `wide`: scales over so many powers of two"""
+    g = torch.Generator().manual_seed(seed)
+    codes = lambda n: torch.randn((total, G, ps, n), generator=g).mul_(60).to(U.E4M3)
+    return codes(d), codes(dv), torch.exp2(torch.randint(-6 - wide, -5 + wide, (total, G, 2), generator=g).float())
+
+
+def on(x, device="cuda"):
+    if isinstance(x, SimpleNamespace):
+        return SimpleNamespace(**{k: v.to(device) if isinstance(v, torch.Tensor) else v for k, v in vars(x).items()})
+    return x.to(device) if isinstance(x, torch.Tensor) else x
+
+
+# ------------------------------------------------------------------------------------------------------------------------- CPU
+def test_exponent_is_the_smallest_that_reaches():
+    for top in (448.0, 448.0000305, 447.99997, 1.0, 1.75, 1.7500001, 3.5, 1e-30, 1e30, 0.0, 2.0 ** -56 * 448):
+        e = U.exponent(top)
+        assert -64 <= e <= 64
+        if -64 < e < 64:
+            assert 448.0 * 2.0 ** e >= top > 448.0 * 2.0 ** (e - 1)
+
+
+def test_layer_refuses_other_tensors():
+    k, v, s = filled(2, 2, 4, 8, 8, 0)
+    Fp8CacheLayer(k, v, s)
+    for bad in ((k.float(), v, s), (k, v[:, :, :2], s), (k, v, s[:, :, :1]), (k, v, s.double()), (k.transpose(2, 3), v, s), (k[0], v[0], s[0])):
+        with pytest.raises(ValueError):
+            Fp8CacheLayer(*bad)
+    assert [tuple(x.shape) for x in Fp8CacheLayer(k, v, s).dequantize()] == [(2, 2, 4, 8)] * 2
+
+
+def test_cache_manager_holds_layers_in_both_widths():
+    c = PagedStateCache([0, 32, 32], 0, 64, 2, "cpu", page_size=16, fp8_heads=[None, (2, 8, 8), None])
+    assert isinstance(c.key_cache[1], Fp8CacheLayer) and c.key_cache[1].k.shape == (c.num_pages, 2, 16, 8) and c.key_cache[2].shape == (c.num_pages, 16, 32)
+    with pytest.raises(ValueError, match="one entry"):
+        PagedStateCache([32, 32], 0, 64, 2, "cpu", page_size=16, fp8_heads=[None])
+
+
+def test_wrappers_refuse_what_does_not_fit():
+    batch, cache, total = U.batch_of([(5, 1)], 16)
+    kv = Fp8CacheLayer(*filled(total, 2, 16, 32, 32, 0))
+    with pytest.raises(ValueError, match="CUDA tensors only"):
+        fp8_cache_append(torch.zeros(1, 256), batch, cache, kv, 4, 2, 32, 32, (0, 128, 192))
+    with pytest.raises(ValueError, match="CUDA tensors only"):
+        fp8_cache_attention(torch.zeros(1, 4, 32), kv, batch, cache, 4, 2, 32, 32, 0.1)
+
+
+APPEND_OK = dict(proj=16, proj_stride=256, heads=4, kv_heads=2, dim=32, vdim=32, pos=16, slot=16, seqs=16, n_seqs=1, page_table=16, n_slots=1, max_pages=2, page_size=16, n_pages=2, k_codes=16, v_codes=16,
+                 scales=16, q_out=16)
+ATTN_OK = dict(q=16, heads=4, kv_heads=2, dim=32, vdim=32, scale=1.0, out_scale=1.0, pos=16, slot=16, seqs=16, n_seqs=1, page_table=16, n_slots=1, max_pages=2, page_size=16, n_pages=2, k_codes=16,
+               v_codes=16, scales=16, out=16, out_stride=128)
+
+
+@pytest.mark.parametrize("bad", [dict(kv_heads=3), dict(dim=257), dict(dim=0), dict(vdim=300), dict(rot_dims=3), dict(rot_dims=34), dict(rot_dims=8), dict(rot_layout=2), dict(qk_norm=2), dict(qk_norm=3),
+                                 dict(page_size=0), dict(max_pages=0), dict(n_slots=0), dict(n_seqs=-1), dict(proj=None), dict(q_out=None), dict(scales=None), dict(k_codes=None), dict(seqs=None)])
+def test_append_refuses(bad):
+    a = native.Fp8AppendParams(**{**APPEND_OK, **bad})
+    assert native.seq_lib().ktb200_fp8_cache_append(C.byref(a), 1, native.GGML_BF16, None) == native.EINVAL
+    assert b"fp8_cache_append" in native.seq_lib().ktb200_last_error()
+
+
+def test_append_refuses_types_and_takes_no_tokens():
+    lib, a = native.seq_lib(), native.Fp8AppendParams(**APPEND_OK)
+    assert lib.ktb200_fp8_cache_append(C.byref(a), 1, native.GGML_F16, None) == native.EINVAL
+    assert lib.ktb200_fp8_cache_append(None, 1, native.GGML_BF16, None) == native.EINVAL
+    assert lib.ktb200_fp8_cache_append(C.byref(a), 0, native.GGML_BF16, None) == native.OK
+
+
+@pytest.mark.parametrize("bad,splits", [(dict(kv_heads=3), 1), (dict(dim=257), 1), (dict(vdim=0), 1), (dict(page_size=0), 1), (dict(window=-1), 1), (dict(chunk=-4), 1), (dict(out_stride=127), 1),
+                                        (dict(q=None), 1), (dict(out=None), 1), (dict(scales=None), 1), ({}, 0), ({}, 129), ({}, 2)])
+def test_attention_refuses(bad, splits):
+    a = native.Fp8AttnParams(**{**ATTN_OK, **bad})
+    assert native.seq_lib().ktb200_fp8_cache_attn(C.byref(a), 1, splits, None, native.GGML_BF16, 1, None) == native.EINVAL
+    assert b"fp8_cache_attn" in native.seq_lib().ktb200_last_error()
+
+
+def test_attention_takes_no_tokens():
+    lib, a = native.seq_lib(), native.Fp8AttnParams(**ATTN_OK)
+    assert lib.ktb200_fp8_cache_attn(C.byref(a), 0, 1, None, native.GGML_F32, 1, None) == native.OK
+    assert lib.ktb200_fp8_cache_attn(C.byref(a), 1, 1, None, native.GGML_F16, 1, None) == native.EINVAL
+
+
+# ------------------------------------------------------------------------------------------------------------------------- append
+# fp32 against 64 bits: the turn is two products and a sum (3 x 2^-24 of |x| + |y|) with sine and cosine 2^-22 off, a norm 13 roundings of a sum of squares (half of
+# them in the root) and three more: in all below 32 x 2^-24 of a row's largest
+FP32_OFF = 32 * 2.0 ** -24
+
+
+def run_append(lens, ps, H, G, d, dv, dtype, rot=None, norm=0, seed=0, tail=0, gap=0, scale=None, held=None, times=1):
+    """One append on the GPU beside its 64-bit form; checks everything that it returns and what it leaves alone"""
+    g = torch.Generator().manual_seed(seed)
+    batch, cache, total = U.batch_of(lens, ps, seed=seed, tail=tail)
+    T, dt = batch.pos.shape[0], DT[dtype]
+    offs = (gap, gap + H * d + gap, gap + H * d + gap + G * d + gap)
+    proj = torch.randn((T, offs[2] + G * dv + gap), generator=g)
+    if scale is not None:
+        proj = proj * scale(T)
+    proj = proj.to(dt)
+    k, v, s = held or filled(total, G, ps, d, dv, seed)
+    w = [(1 + 0.3 * torch.randn(d, generator=g)).to(dt) for _ in range(2)] if norm == 3 else [None, None]
+    inv = INV(rot.dims) if rot is not None else None
+    q_ref, k_ref, v_ref, s_ref, k_exact, v_exact = U.append(proj, batch, cache, k, v, s, H, G, d, dv, offs, rot, inv, norm, 1e-5, *w)
+    kv = Fp8CacheLayer(*(x.cuda() for x in (k, v, s)))
+    for _ in range(times):
+        q = fp8_cache_append(proj.cuda(), on(batch), on(cache), kv, H, G, d, dv, offs, rot, on(inv), norm, 1e-5, *map(on, w))
+    torch.cuda.synchronize()
+    off = FP32_OFF * q_ref.abs().amax(-1, keepdim=True)
+    assert ((q.cpu().double() - q_ref).abs() <= HALF_STEP[dt] * q_ref.abs() * (1 + 2.0 ** -6) + off).all()
+    assert torch.equal(kv.scales.cpu().double(), s_ref)
+    exact_k = norm == 0 and (rot is None or rot.dims == 0)
+    for got, ahead, slack in ((kv.k, k_exact, 0.0 if exact_k else FP32_OFF), (kv.v, v_exact, 0.0)):
+        got, near = got.cpu().double(), slack * ahead.abs().amax(-1, keepdim=True)
+        lo, hi = U.to_codes(ahead - near), U.to_codes(ahead + near)
+        assert ((got >= lo) & (got <= hi)).all()
+    return kv, (k_ref, v_ref, s_ref)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("lens,ps,H,G,d,dv,rot,norm", [
+    ([(0, 1)], 64, 2, 1, 128, 128, ROT(128, 1), 0),                      # the first token of all
+    ([(63, 1), (64, 1), (65, 1)], 64, 16, 2, 128, 128, ROT(128, 1), 3),    # the last row of a page, the first, the second
+    ([(5, 1)] * 40, 16, 8, 8, 64, 64, ROT(32, 0), 1),                     # more portions than lanes
+    ([(0, 200)], 64, 8, 2, 128, 128, ROT(64, 0), 0),
+    ([(37, 150), (0, 1), (3, 77)], 64, 64, 8, 128, 128, ROT(128, 1), 1),
+    ([(7, 30), (0, 5), (11, 64)], 7, 6, 2, 80, 80, ROT(40, 1), 3),         # odd pages, heads that are no whole vectors
+    ([(1, 33)], 16, 7, 1, 96, 96, ROT(96, 0), 0),
+    ([(10, 20)], 32, 4, 4, 64, 128, ROT(64, 1), 0),                       # values of another size
+    ([(3, 300)], 256, 4, 2, 256, 256, ROT(256, 0), 1),                    # a page's rows do not fit in shared memory
+    ([(2, 9), (0, 3)], 1, 3, 1, 24, 40, None, 0),                        # pages of one token
+    ([(0, 0), (4, 6), (9, 0)], 8, 2, 2, 64, 64, ROT(64, 1), 0),            # portions without tokens
+    ([(100000, 3)], 64, 2, 1, 128, 128, ROT(128, 1), 0),                 # a far position
+])
+def test_append(lens, ps, H, G, d, dv, rot, norm, dtype):
+    run_append(lens, ps, H, G, d, dv, dtype, rot, norm, seed=len(lens) + d)
+
+
+@pytest.mark.gpu
+def test_append_reads_columns_anywhere_and_leaves_other_rows():
+    run_append([(10, 20), (0, 3)], 16, 4, 2, 64, 64, "bf16", ROT(64, 1), 0, seed=3, gap=3, tail=5)      # (columns that begin at no whole vector; tokens of no portion)
+    run_append([(10, 20), (0, 3)], 16, 4, 2, 128, 128, "fp32", ROT(128, 0), 3, seed=4, gap=8, tail=2)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d,ps", [(128, 64), (80, 16), (30, 5)])
+def test_append_moves_the_codes_of_a_page_whose_scale_grows(d, ps):
+    grow = lambda T: torch.logspace(-3, 4, T)[:, None]
+    lens = [(ps - 2, 1), (3, 1), (ps + 1, ps), (ps // 2, 2)]
+    kv, ref = run_append(lens, ps, 4, 2, d, d, "fp32", None, 0, seed=11, scale=grow)
+    # and again: what is there already asks for no larger scale, and the same tokens give the same codes
+    again, _ = run_append(lens, ps, 4, 2, d, d, "fp32", None, 0, seed=11, scale=grow, times=3)
+    assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in ((kv.k, again.k), (kv.v, again.v))) and torch.equal(kv.scales, again.scales)
+
+
+@pytest.mark.gpu
+def test_append_of_nothing_and_of_everything():
+    run_append([(0, 4), (6, 3)], 8, 2, 1, 64, 64, "fp32", ROT(64, 1), 0, scale=lambda T: torch.zeros(T, 1))
+    run_append([(0, 4), (6, 3)], 8, 2, 1, 64, 64, "fp32", None, 0, scale=lambda T: torch.full((T, 1), 1e-30))
+    run_append([(0, 4), (6, 3)], 8, 2, 1, 64, 64, "fp32", None, 0, scale=lambda T: torch.full((T, 1), 1e25))
+
+
+@pytest.mark.gpu
+def test_append_of_infinities_and_nan():
+    batch, cache, total = U.batch_of([(0, 3), (0, 3)], 8)
+    k, v, s = filled(total, 1, 8, 64, 64, 5)
+    proj = torch.randn(6, 192)
+    proj[1, 64], proj[1, 70], proj[1, 130] = math.inf, math.nan, -math.inf      # one key row and one value row of the first sequence
+    kv = Fp8CacheLayer(*(x.cuda() for x in (k, v, s)))
+    fp8_cache_append(proj.cuda(), on(batch), on(cache), kv, 1, 1, 64, 64, (0, 64, 128))
+    _, k_ref, v_ref, s_ref, _, _ = U.append(proj, batch, cache, k, v, s, 1, 1, 64, 64, (0, 64, 128))
+    assert torch.equal(kv.scales.cpu().double(), s_ref)
+    assert torch.equal(kv.k.cpu().double().nan_to_num(1e9), k_ref.nan_to_num(1e9)) and torch.equal(kv.v.cpu().double(), v_ref)
+
+
+@pytest.mark.gpu
+def test_append_leaves_pages_that_are_not_there():
+    batch, cache, total = U.batch_of([(4, 10), (0, 3)], 8)
+    cache.page_table[0, 1], cache.page_table[1, 0] = total + 5, -1      # the first sequence's second page, the second's first
+    k, v, s = filled(total, 2, 8, 64, 64, 6)
+    kv = Fp8CacheLayer(*(x.cuda() for x in (k, v, s)))
+    fp8_cache_append(torch.randn(13, 6 * 64).cuda(), on(batch), on(cache), kv, 2, 2, 64, 64, (0, 128, 256))
+    changed = (kv.k.cpu().view(torch.uint8) != k.view(torch.uint8)).flatten(1).any(1)
+    assert changed.nonzero().flatten().tolist() == [int(cache.page_table[0, 0])]
+
+
+# ------------------------------------------------------------------------------------------------------------------------- attention
+def run_attention(lens, ps, H, G, d, dv, dtype, seed=0, tail=0, wide=0, out_stride=0, tensor_cores=True, break_table=None, big=1.0, **o):
+    g = torch.Generator().manual_seed(seed)
+    batch, cache, total = U.batch_of(lens, ps, seed=seed, tail=tail)
+    k, v, s = filled(total, G, ps, d, dv, seed, wide)
+    live = torch.zeros((total, ps), dtype=torch.bool)      # rows behind a sequence's last token and pages of nobody: NaN
+    for i, (b, n) in enumerate(lens):
+        j = torch.arange(b + n)
+        live[cache.page_table[i].long()[j // ps], j % ps] = True
+    hole = ~live[:, None, :, None]
+    k, v = (torch.where(hole, torch.full((), 0x7f, dtype=torch.uint8), x.view(torch.uint8)).view(U.E4M3) for x in (k, v))
+    if break_table is not None:
+        break_table(cache.page_table, total)
+    T, dt = batch.pos.shape[0], DT[dtype]
+    q = (big * torch.randn((T, H, d), generator=g)).to(dt)
+    scale = d ** -0.5
+    for name in ("head_scale", "sink"):
+        if o.get(name):
+            o[name] = torch.randn(H, generator=g) * (0.3 if name == "head_scale" else 1.0) + (1.0 if name == "head_scale" else 0.0)
+    ref = U.attention(q, k, v, s, batch, cache, H, G, d, dv, scale, **o)
+    kv = Fp8CacheLayer(*(x.cuda() for x in (k, v, s)))
+    wide_out = torch.full((T, H * dv + out_stride), 7.0, dtype=dt, device="cuda")
+    out = fp8_cache_attention(q.cuda(), kv, on(batch), on(cache), H, G, d, dv, scale, tensor_cores=tensor_cores, out=wide_out[:, :H * dv], **{n: on(x) for n, x in o.items()}).cpu().double()
+    assert (wide_out[:, H * dv:] == 7).all()
+    alone = ref.isnan()
+    assert (out[alone] == 7).all()      # tokens of no portion
+    # scores are sums of d products, off by d x 2^-24 of |q||k| in fp32 and twice that on the tensor cores (which cut what a sum does not hold); a score's error e makes its weight's
+    # relative error e, at most 2 e of the weighted mean of values of size V.  Weights rounded to fp16 for the second product: 2^-11 of V
+    K = (k.double().nan_to_num(0.0) * s.double()[:, :, None, None, 0]).norm(dim=-1).max()
+    V = (v.double().nan_to_num(0.0) * s.double()[:, :, None, None, 1]).abs().max()
+    hs = o["head_scale"].abs().max() if o.get("head_scale") is not None else 1.0
+    e = float(q.double().norm(dim=-1).max() * K * scale * hs) * (2 * d + 8) * 2.0 ** -24 + 2.0 ** -20
+    bound = HALF_STEP[dt] * ref.abs() * 1.02 + float(V) * (2 * e + (2.0 ** -11 if dtype == "bf16" else 0.0)) * abs(o.get("out_scale", 1.0))
+    assert ((out - ref).abs() <= bound)[~alone].all(), float(((out - ref).abs() / bound)[~alone].max())
+
+
+SHAPES = [
+    ([(0, 1)], 64, 2, 1, 128, 128),                                   # the first token sees itself alone
+    ([(62, 1), (63, 1), (64, 1), (200, 1)], 64, 16, 2, 128, 128),
+    ([(1500, 1)], 64, 16, 2, 128, 128),                               # one token over a range that is cut
+    ([(333, 1), (5, 1), (90, 1)], 48, 8, 8, 64, 64),                  # pages that are no whole tiles, heads that share nothing
+    ([(100, 3), (0, 5), (17, 1)], 16, 12, 4, 96, 96),
+    ([(100, 3), (0, 5)], 7, 6, 2, 80, 48),
+    ([(70, 2)], 64, 7, 1, 64, 128),
+    ([(30, 2)], 32, 32, 1, 64, 64),
+    ([(40, 4)], 16, 2, 1, 40, 24),                                    # head sizes that no tensor-core tile takes
+    ([(20, 2)], 16, 2, 2, 256, 256),
+    ([(0, 70), (33, 40), (500, 1)], 64, 8, 1, 128, 128),              # prompt portions beside a decoded token
+    ([(10, 100)], 64, 16, 2, 128, 128),
+    ([(3, 0), (9, 20), (0, 0)], 16, 4, 2, 64, 64),                    # portions without tokens
+    ([(6, 40)], 5, 4, 2, 128, 64),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("lens,ps,H,G,d,dv", SHAPES)
+def test_attention(lens, ps, H, G, d, dv, dtype):
+    run_attention(lens, ps, H, G, d, dv, dtype, seed=d + len(lens))
+
+
+MASKS = [dict(window=1), dict(window=50), dict(chunk=16), dict(chunk=33, sink=True), dict(window=20, chunk=64, softcap=20.0), dict(head_scale=True, softcap=5.0), dict(sink=True, out_scale=0.25), dict(out_scale=-2.0)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("options", MASKS, ids=str)
+def test_attention_masks_and_scores(options, dtype):
+    run_attention([(100, 1), (0, 40), (31, 33), (700, 2)], 32, 8, 2, 128, 128, dtype, seed=5, **options)
+    run_attention([(100, 1), (0, 4), (31, 3)], 48, 6, 2, 96, 64, dtype, seed=6, **options)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_attention_blocks_of_very_different_scales(dtype):
+    run_attention([(400, 1), (90, 5)], 16, 4, 1, 64, 64, dtype, seed=8, wide=5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_attention_writes_its_rows_alone(dtype):
+    run_attention([(100, 3), (0, 20)], 16, 4, 2, 64, 64, dtype, seed=9, tail=4, out_stride=24)
+    run_attention([(900, 1)], 16, 4, 2, 64, 64, dtype, seed=9, tail=2, out_stride=8)
+    run_attention([(90, 2)], 16, 4, 2, 64, 64, dtype, seed=9, out_stride=3)      # rows that begin anywhere
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_attention_does_not_see_pages_that_are_not_there(dtype):
+    def break_table(t, total):
+        t[0, 1], t[1, 0] = total, -3
+    run_attention([(100, 2), (0, 3), (60, 40)], 16, 4, 2, 64, 64, dtype, seed=10, break_table=break_table)      # (the second sequence sees nothing at all: zeros)
+    run_attention([(1200, 1)], 64, 4, 2, 128, 128, dtype, seed=10, break_table=lambda t, total: t.__setitem__((0, 3), -1))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_attention_over_a_ring_of_pages(dtype):
+    """positions far beyond the table's width: logical page p stands in column p % max_pages"""
+    batch, cache, total = U.batch_of([(40, 3)], 16)
+    lap = cache.max_pages_per_seq * 16
+    k, v, s = filled(total, 1, 16, 64, 64, 12)
+    q = torch.randn(3, 2, 64).to(DT[dtype])
+    kv = Fp8CacheLayer(*(x.cuda() for x in (k, v, s)))
+    a = fp8_cache_attention(q.cuda(), kv, on(batch), on(cache), 2, 1, 64, 64, 0.125, window=30)
+    batch.pos += 5 * lap
+    batch.max_kv += 5 * lap
+    b = fp8_cache_attention(q.cuda(), kv, on(batch), on(cache), 2, 1, 64, 64, 0.125, window=30)
+    assert torch.allclose(a.float(), b.float(), rtol=0, atol=float(a.float().abs().max()) * (2.0 ** -7 if dtype == "bf16" else 1e-5))
