@@ -52,6 +52,12 @@ class LatentStepParams(C.Structure):
                 + [("workspace_bytes", C.c_size_t)] + [(n, C.c_void_p) for n in ("x", "out", "scratch")] + [("scratch_bytes", C.c_size_t)])
 
 
+class Int8LinearParams(C.Structure):
+    """ktb200_int8_linear_params (include/ktb200.h)"""
+    _fields_ = [("x", C.c_void_p), ("x_stride", C.c_long), ("weight", C.c_void_p), ("weight_stride", C.c_long), ("weight_scale", C.c_void_p), ("bias", C.c_void_p), ("in_features", C.c_int),
+                ("out_features", C.c_int), ("hidden_type", C.c_int), ("y", C.c_void_p), ("y_stride", C.c_long), ("bsz", C.c_void_p)]
+
+
 _lib = None
 _lock = threading.Lock()
 
@@ -74,6 +80,8 @@ SYMBOLS = {
     "ktb200_fp8_linear_create": (_I, [_I, _I, _VP, _VP, _I, _I, C.POINTER(_VP)]),
     "ktb200_fp8_linear_destroy": (None, [_VP]),
     "ktb200_fp8_linear_forward": (_I, [_VP, _I, _VP, _VP, _VP, _VP]),
+    "ktb200_int8_linear_workspace": (C.c_size_t, [_I, _I]),
+    "ktb200_int8_linear": (_I, [C.POINTER(Int8LinearParams), _I, _VP, C.c_size_t, _VP]),
     "ktb200_linear_create": (_I, [_I, _I, _VP, _I, _I, _I, _I, C.POINTER(_VP)]),
     "ktb200_linear_destroy": (None, [_VP]),
     "ktb200_linear_load_weights": (_I, [_VP, _VP]),

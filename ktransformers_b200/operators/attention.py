@@ -8,7 +8,6 @@ TMEM + TMA, csrc/mla.cu); the cache write is ktb200_mla_kv_write; the projection
 GEMVs over the bf16 halves of kv_b_proj; torch.matmul for other dtypes).  Prefill (q_len > 1 without absorb) is outside this path and raises."""
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
 import math
 from typing import Optional, Tuple
@@ -19,16 +18,8 @@ from .. import native
 from ..models.custom_cache import StaticCache
 from ..models.modeling_deepseek_v3 import DeepseekV3Attention, DeepseekV3RMSNorm, DeepseekV3RotaryEmbedding, apply_rotary_pos_emb
 from ..util.utils import InferenceState
-from .base_operator import BaseInjectedModule
+from .base_operator import BaseInjectedModule, device_of
 from .flashinfer_wrapper import MLAWrapper, MLAWrapperSingleton
-
-
-_HERE = contextlib.nullcontext()
-
-
-def _device_of(dev):
-    """`dev` as the current device: kernels are launched on the current one, whatever their stream's"""
-    return _HERE if dev.index is None or dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
 
 
 def _is_plain(module, cls) -> bool:
@@ -569,7 +560,7 @@ def fp8_cache_append(proj: torch.Tensor, batch, cache, kv, heads: int, kv_heads:
                                inv_freq.data_ptr() if rot_dims else None, qk_norm, q_weight.data_ptr() if qk_norm == 3 else None, k_weight.data_ptr() if qk_norm == 3 else None, eps,
                                batch.pos.data_ptr(), batch.slot.data_ptr(), batch.seqs.data_ptr(), batch.seqs.stride(0), batch.n_seqs, table.data_ptr(), table.shape[0], table.shape[1],
                                cache.page_size, kv.k.shape[0], kv.k.data_ptr(), kv.v.data_ptr(), kv.scales.data_ptr(), q.data_ptr())
-    with _device_of(dev):
+    with device_of(dev):
         native.check_seq(native.seq_lib().ktb200_fp8_cache_append(C.byref(a), T, code, st))
     return q
 
@@ -595,7 +586,7 @@ def fp8_cache_attention(q: torch.Tensor, kv, batch, cache, heads: int, kv_heads:
                              sink.data_ptr() if sink is not None else None, out_scale, batch.pos.data_ptr(), batch.slot.data_ptr(), batch.seqs.data_ptr(), batch.seqs.stride(0),
                              batch.n_seqs, table.data_ptr(), table.shape[0], table.shape[1], cache.page_size, kv.k.shape[0], kv.k.data_ptr(), kv.v.data_ptr(), kv.scales.data_ptr(),
                              out.data_ptr(), out.stride(0))
-    with _device_of(dev):
+    with device_of(dev):
         splits = lib.ktb200_fp8_cache_attn_splits(C.byref(a), T, batch.max_kv, code, int(tensor_cores))
         ws = torch.empty(lib.ktb200_fp8_cache_attn_workspace(T, heads, vdim, splits) // 4, dtype=torch.float32, device=dev) if splits > 1 else None
         native.check_seq(lib.ktb200_fp8_cache_attn(C.byref(a), T, splits, ws.data_ptr() if ws is not None else None, code, int(tensor_cores), st))

@@ -4,9 +4,18 @@ Same contract as archive/ktransformers/operators/base_operator.py:12-63: the cto
 found on the wrapper resolve on ``orig_module``, and ``load()`` recurses into children."""
 from __future__ import annotations
 
+import contextlib
 from typing import Any
 
+import torch
 from torch import nn
+
+_HERE = contextlib.nullcontext()
+
+
+def device_of(dev: torch.device):
+    """`dev` as the current device: kernels are launched on the current one, whatever their stream's"""
+    return _HERE if dev.index is None or dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
 
 
 class BaseInjectedModule(nn.Module):

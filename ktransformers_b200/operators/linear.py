@@ -21,7 +21,7 @@ from torch import nn
 from .. import native
 from ..util.custom_gguf import GGML_NAMES, TORCH_TO_GGML_HIDDEN, B200_WEIGHT_TYPES
 from ..util.utils import InferenceState
-from .base_operator import BaseInjectedModule
+from .base_operator import BaseInjectedModule, device_of
 
 _GGML_TO_TORCH = {0: torch.float32, 1: torch.float16, 30: torch.bfloat16}
 
@@ -237,9 +237,97 @@ class KLinearFP8(KLinearBase):
             pass
 
 
+def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor, bias: torch.Tensor | None = None, bsz_tensor: torch.Tensor | None = None) -> torch.Tensor:
+    """y = x W^T + bias with both sides in 8-bit integers: `weight` int8 [out, in] (rows at multiples of 16 bytes) under one fp32 `weight_scale` per output channel, the rows of x (bf16,
+    fp16 or fp32) quantised inside the call under one scale per token, max |x| / 127; exact 32-bit integer sums, scaled and rounded once (`ktb200_int8_linear`,
+    csrc/int8_linear.cu).  Rows at or behind bsz_tensor[0] are left as they come."""
+    K, N = weight.shape[1], weight.shape[0]
+    if not x.is_cuda:
+        raise ValueError("int8_linear: CUDA tensors only")
+    if x.dtype not in _INT8_HIDDEN or weight.dtype != torch.int8 or x.shape[-1] != K:
+        raise ValueError(f"int8_linear: x [.., {K}] of bfloat16, float16 or float32 and an int8 weight, got {x.dtype} {tuple(x.shape)} and {weight.dtype}")
+    if weight.stride(1) != 1 or weight.stride(0) % 16 or weight.data_ptr() % 16:
+        raise ValueError("int8_linear: weight rows have to begin at multiples of 16 bytes")
+    dev = x.device
+    if weight_scale.dtype != torch.float32 or weight_scale.numel() != N or not weight_scale.is_contiguous():
+        raise ValueError(f"int8_linear: weight_scale has to be {N} contiguous float32 values")
+    if bias is not None and (bias.dtype != torch.float32 or bias.numel() != N or not bias.is_contiguous() or bias.device != dev):
+        raise ValueError(f"int8_linear: bias has to be {N} contiguous float32 values on {dev}")
+    if weight.device != dev or weight_scale.device != dev:
+        raise ValueError("int8_linear: all tensors have to be on one device")
+    if bsz_tensor is not None and (bsz_tensor.dtype != torch.int32 or bsz_tensor.device != dev):
+        raise ValueError(f"int8_linear: bsz_tensor has to be int32 on {dev}")
+    x2 = x if x.dim() == 2 else x.reshape(-1, K)
+    if x2.stride(1) != 1 or (x2.shape[0] > 1 and x2.stride(0) < K):
+        x2 = x2.contiguous()
+    T, lib = x2.shape[0], native.lib()
+    y = torch.empty((T, N), dtype=x.dtype, device=dev)
+    if T:
+        nbytes = lib.ktb200_int8_linear_workspace(T, K)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        a = native.Int8LinearParams(x2.data_ptr(), max(x2.stride(0), K), weight.data_ptr(), weight.stride(0), weight_scale.data_ptr(), bias.data_ptr() if bias is not None else None, K, N,
+                                    _INT8_HIDDEN[x.dtype], y.data_ptr(), N, bsz_tensor.data_ptr() if bsz_tensor is not None else None)
+        with device_of(dev):
+            native.check(lib.ktb200_int8_linear(C.byref(a), T, ws.data_ptr(), nbytes, torch.cuda.current_stream(dev).cuda_stream))
+    return y if x.dim() == 2 else y.reshape(*x.shape[:-1], N)
+
+
+_INT8_HIDDEN = {torch.float32: native.GGML_F32, torch.float16: native.GGML_F16, torch.bfloat16: native.GGML_BF16}
+
+
+class KLinearInt8(KLinearBase):
+    """8-bit integer linear (`int8_linear`): symmetric int8 weights with one scale per output channel, activations quantised per token inside the call.  Contract of KLinearFP8:
+    `load(w=(weight int8 [out][in], weight_scale [out] or [out, 1][, bias]))`, a float weight [out][in] (quantised here, row by row, to max |w| / 127), or from a
+    SafeTensorLoader (`<key>.weight` + `<key>.weight_scale`); `forward(x, bsz_tensor)`.  (The reference's linear operators: archive/ktransformers/operators/linear.py.)"""
+
+    def __init__(self, key, gguf_loader, config, orig_module=None, device: str = "cuda", **kwargs):
+        super().__init__(key, gguf_loader, config, orig_module, device, **kwargs)
+        self.weight = self.weight_scale = self.bias = None
+
+    @staticmethod
+    def quantize(weight: torch.Tensor):
+        """(int8 weight, scale per row) of a float weight [out][in]"""
+        w = weight.float()
+        scale = w.abs().amax(1) / 127
+        return torch.round(w / torch.where(scale > 0, scale, torch.ones_like(scale))[:, None]).clamp(-127, 127).to(torch.int8), scale
+
+    def load(self, w=None, device: str | None = None):
+        if self.loaded:
+            return
+        device = device or self.device
+        assert "cuda" in str(device).lower(), "KLinearInt8 can only be loaded on a CUDA device"
+        if w is None:
+            ld = self.gguf_loader
+            if hasattr(ld, "load_tensor"):
+                w = (ld.load_tensor(self.key + ".weight"), ld.load_tensor(self.key + ".weight_scale")) + ((ld.load_tensor(self.key + ".bias"),) if ld.has_tensor(self.key + ".bias") else ())
+            else:
+                w = self.load_weight(device=device)
+        w = tuple(t.data if isinstance(t, nn.Parameter) else t for t in (w if isinstance(w, tuple) else (w,)))
+        if w[0].dtype != torch.int8:      # a float weight[, its bias]
+            w = KLinearInt8.quantize(w[0].to(device).view(self.out_features, self.in_features)) + w[1:]
+        if len(w) not in (2, 3) or tuple(w[0].shape) != (self.out_features, self.in_features) or w[1].numel() != self.out_features or (len(w) == 3 and w[2].numel() != self.out_features):
+            raise ValueError(f"KLinearInt8: weight int8 [{self.out_features}][{self.in_features}], one scale per row and, where there is one, a bias; got {[tuple(t.shape) for t in w]}")
+        pad = -self.in_features % 16      # rows begin at multiples of 16 bytes
+        self.weight = torch.nn.functional.pad(w[0].to(device), (0, pad))[:, :self.in_features] if pad else w[0].to(device).contiguous()
+        self.weight_scale = w[1].to(device=device, dtype=torch.float32).reshape(-1).contiguous()
+        self.has_bias = len(w) == 3
+        self.bias = w[2].to(device=device, dtype=torch.float32).reshape(-1).contiguous() if self.has_bias else None
+        self.loaded = True
+
+    def forward(self, x: torch.Tensor, bsz_tensor: torch.Tensor = None, **kwargs) -> torch.Tensor:
+        if not self.loaded:
+            raise native.KTB200Error("Not Loaded")
+        return int8_linear(x, self.weight, self.weight_scale, self.bias, bsz_tensor)
+
+    def unload(self):
+        self.weight = self.weight_scale = self.bias = None
+        self.loaded = False
+
+
 LINEAR_MAP = {
     "KLinearB200": KLinearB200,
     "KLinearFP8": KLinearFP8,
+    "KLinearInt8": KLinearInt8,
     "KLinearTorch": KLinearTorch,
 }
 
