@@ -193,6 +193,7 @@ template <typename T> __global__ void __launch_bounds__(128) fp8_merge_kernel(co
 }
 
 }  // namespace ktb
+#include "fp8_attn_mma.cuh"
 
 using namespace ktb;
 
@@ -204,6 +205,11 @@ extern "C" size_t ktb200_fp8_cache_attn_workspace(int n_tokens, int heads, int v
 extern "C" int ktb200_fp8_cache_attn_splits(const ktb200_fp8_attn_params* c, int n_tokens, int max_keys, int dtype, int allow_tensor_cores) {
     if (!c || c->heads <= 0 || c->kv_heads <= 0 || n_tokens <= 0) return 1;
     const int R = c->heads / c->kv_heads;
+    if (allow_tensor_cores && fm_takes(c, dtype)) {      // three CTAs an SM; parts of 256 keys or more
+        const long ctas = fm_tiles(c, n_tokens) * c->kv_heads * (R / fm_heads(R));
+        if (ctas >= 296 || max_keys <= 512) return 1;
+        return (int)std::max<long>(1, std::min<long>({kFp8MaxSplits, max_keys / 256, 444 / ctas}));
+    }
     const long ctas = (long)n_tokens * c->kv_heads * ((R + 7) / 8);
     if (ctas >= 148 || max_keys <= 256) return 1;
     return (int)std::max<long>(1, std::min<long>({64, max_keys / 128, 592 / ctas}));
@@ -226,14 +232,20 @@ extern "C" int ktb200_fp8_cache_attn(const ktb200_fp8_attn_params* c, int n_toke
     const Fp8Attn a{c->q, c->heads, c->kv_heads, c->dim, c->vdim, c->scale, c->head_scale, c->softcap, c->window, c->chunk, c->sink, c->out_scale, c->pos, c->slot, c->seqs, c->seqs_stride,
                     c->n_seqs, n_tokens, {c->page_table, c->n_slots, c->max_pages, c->page_size, c->n_pages}, (const uint8_t*)c->k_codes, (const uint8_t*)c->v_codes, c->scales, c->out,
                     c->out_stride, splits > 1 ? workspace : nullptr, splits};
+    const bool bf16 = dtype == KTB200_TYPE_BF16, tiles = allow_tensor_cores && fm_takes(c, dtype);
+    if (tiles) {
+        const int RH = fm_heads(R);
+        const dim3 grid((unsigned)fm_tiles(c, n_tokens), c->kv_heads * (R / RH), splits);
+        KTB_CUDA_CHECK(fm_shared(c, n_tokens) ? fm_launch<true>(a, RH, grid, s) : fm_launch<false>(a, RH, grid, s));
+    } else {
     const size_t smem = ((size_t)HB * c->dim + (size_t)kFgTile * (c->dim + 1) + (size_t)kFgTile * c->vdim + (size_t)HB * kFgTile) * sizeof(float);
     const dim3 grid(n_tokens, c->kv_heads * hblocks, splits);
-    const bool bf16 = dtype == KTB200_TYPE_BF16;
     KTB_CUDA_CHECK(raise_smem_limit(bf16 ? (const void*)fp8_attn_kernel<__nv_bfloat16> : (const void*)fp8_attn_kernel<float>, smem));
     KTB_CUDA_CHECK(launch_pdl(bf16 ? fp8_attn_kernel<__nv_bfloat16> : fp8_attn_kernel<float>, grid, dim3(HB * 32), smem, s, a));
+    }
     count_launch();
     if (splits > 1) {
-        KTB_CUDA_CHECK(launch_pdl(bf16 ? fp8_merge_kernel<__nv_bfloat16> : fp8_merge_kernel<float>, dim3((unsigned)((long)n_tokens * c->heads)), dim3(128), (size_t)0, s, a, kLog2e));
+        KTB_CUDA_CHECK(launch_pdl(bf16 ? fp8_merge_kernel<__nv_bfloat16> : fp8_merge_kernel<float>, dim3((unsigned)((long)n_tokens * c->heads)), dim3(128), (size_t)0, s, a, tiles ? 1.0f : kLog2e));
         count_launch();
     }
     return KTB200_OK;

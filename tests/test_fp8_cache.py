@@ -311,3 +311,83 @@ def test_attention_over_a_ring_of_pages(dtype):
     batch.max_kv += 5 * lap
     b = fp8_cache_attention(q.cuda(), kv, on(batch), on(cache), 2, 1, 64, 64, 0.125, window=30)
     assert torch.allclose(a.float(), b.float(), rtol=0, atol=float(a.float().abs().max()) * (2.0 ** -7 if dtype == "bf16" else 1e-5))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("d,ps,lens,at", [(128, 64, [(0, 90)], 50), (64, 16, [(20, 3)], 21), (96, 48, [(5, 40)], 44), (128, 64, [(200, 300)], 260)])
+def test_attention_keeps_nan_to_the_rows_that_see_it(d, ps, lens, at, dtype):
+    """a token whose key (or value) is NaN: the tokens ahead of it do not see it, those behind it do"""
+    H, G, (b, n) = 4, 2, lens[0]
+    batch, cache, total = U.batch_of(lens, ps)
+    page, row = int(cache.page_table[0, at // ps]), at % ps
+    for what in ("k", "v"):
+        kv = Fp8CacheLayer(*(x.cuda() for x in filled(total, G, ps, d, d, 13)))
+        q = torch.randn((n, H, d), generator=torch.Generator().manual_seed(1)).to(DT[dtype]).cuda()
+        clean = fp8_cache_attention(q, kv, on(batch), on(cache), H, G, d, d, d ** -0.5).view(n, H, d)
+        getattr(kv, what).view(torch.uint8)[page, 1, row, 5] = 0x7f if what == "k" else 0xff      # the second key/value head's
+        out = fp8_cache_attention(q, kv, on(batch), on(cache), H, G, d, d, d ** -0.5).view(n, H, d)
+        first = at - b
+        assert torch.equal(out[:, :2], clean[:, :2]) and torch.equal(out[:first, 2:], clean[:first, 2:])
+        if what == "k":
+            assert out[first:, 2:].isnan().all()
+        else:
+            assert out[first:, 2:, 5].isnan().all() and not out[first:, 2:, 6:].isnan().any()
+
+
+@pytest.mark.gpu
+def test_the_two_calls_as_a_step_uses_them_replayed_on_other_streams():
+    """append, then attention over what was appended, decoded token by token behind a prompt: eagerly, and as one captured graph per step"""
+    H, G, d, ps, steps = 8, 2, 128, 64, 5
+    lens = [(0, 70), (0, 63), (0, 9)]
+    full, cache, total = U.batch_of([(0, n + steps) for _, n in lens], ps)
+    g = torch.Generator().manual_seed(3)
+    rows = [torch.randn((n + steps, (H + 2 * G) * d), generator=g).bfloat16().cuda() for _, n in lens]
+    rot, inv = ROT(d, 1), INV(d).cuda()
+    cache = on(cache)
+
+    def batch_at(done, n):
+        i32 = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")
+        pos = [p for s in range(3) for p in range(done[s], done[s] + n[s])]
+        starts = [sum(n[:s]) for s in range(3)]
+        return SimpleNamespace(pos=i32(pos), slot=i32([s for s in range(3) for _ in range(n[s])]), seqs=i32([starts, n]), n_seqs=3, max_kv=max(x + y for x, y in zip(done, n)))
+
+    def step(kv, b, proj):
+        q = fp8_cache_append(proj, b, cache, kv, H, G, d, d, (0, H * d, (H + G) * d), rot, inv, 1, 1e-6)
+        return fp8_cache_attention(q, kv, b, cache, H, G, d, d, d ** -0.5)
+
+    def serve(captured):
+        kv = Fp8CacheLayer.empty(total, ps, G, d, d)
+        n = [x for _, x in lens]
+        outs = [step(kv, batch_at([0, 0, 0], n), torch.cat([r[:m] for r, m in zip(rows, n)]))]
+        b, proj, graph, side = batch_at(n, [1, 1, 1]), torch.empty_like(rows[0][:3]), None, torch.cuda.Stream()
+        b.max_kv = 64 * ps
+        for i in range(steps):
+            b.pos.copy_(torch.tensor([x + i for x in n], dtype=torch.int32))
+            proj.copy_(torch.stack([r[x + i] for r, x in zip(rows, n)]))
+            if not captured:
+                outs.append(step(kv, b, proj))
+                continue
+            if graph is None:
+                torch.cuda.synchronize()
+                graph = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(graph):
+                    o = step(kv, b, proj)
+            side.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(side):
+                graph.replay()
+            torch.cuda.current_stream().wait_stream(side)
+            outs.append(o.clone())
+        torch.cuda.synchronize()
+        return outs, kv
+
+    (eager, a), (replayed, c) = serve(False), serve(True)
+    assert all(torch.equal(x, y) for x, y in zip(eager, replayed))
+    assert torch.equal(a.k.view(torch.uint8), c.k.view(torch.uint8)) and torch.equal(a.scales, c.scales)
+    # the last decoded tokens against attention over all of a sequence's tokens in 64 bits, over what the cache holds
+    b = batch_at([n + steps - 1 for _, n in lens], [1, 1, 1])
+    proj = torch.stack([r[-1] for r in rows])
+    q, *_ = U.append(proj.cpu(), on(b, "cpu"), on(cache, "cpu"), a.k.cpu(), a.v.cpu(), a.scales.cpu(), H, G, d, d, (0, H * d, (H + G) * d), rot, inv.cpu(), 1, 1e-6)
+    ref = U.attention(q.bfloat16(), a.k.cpu(), a.v.cpu(), a.scales.cpu(), on(b, "cpu"), on(cache, "cpu"), H, G, d, d, d ** -0.5)
+    # queries round as bf16 on both sides (one step apart at most: 2^-7 of a score of size s, s <= 5 here), weights to fp16, results to bf16
+    assert ((eager[-1].cpu().double() - ref).abs() <= 2.0 ** -8 * ref.abs() + (2.0 ** -4 + 2.0 ** -11) * float(a.dequantize()[1].abs().max())).all()
