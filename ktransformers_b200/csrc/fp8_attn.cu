@@ -16,7 +16,7 @@
 namespace ktb {
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kFp8MaxSplits = 128;
+constexpr int kFp8MaxParts = 128, kFp8MinPart = 256;
 
 struct Fp8Attn {
     const void* q;
@@ -34,8 +34,9 @@ struct Fp8Attn {
     const float* scales;
     void* out;
     long out_stride;
-    float* partial;      // [T][H][splits][dv + 2]: reference maximum, sum, un-normalised weighted values
-    int splits;
+    float* partial;      // [T][H][parts][dv + 2]: reference maximum, sum, un-normalised weighted values
+    int part, parts;     // keys of a part (0: the range is not cut), and the most parts of a range
+    int ctoks;           // tokens of a CTA: their range, from the first visible key of the first of them (rounded down to 16) on, is what is cut
 };
 __device__ __forceinline__ int fp8_first_visible(int p, int window, int chunk) {
     int lo = window > 0 ? max(0, p - window + 1) : 0;
@@ -48,34 +49,50 @@ __device__ __forceinline__ int fp8_portion(const Fp8Attn& a, int s) {
     return len <= 0 || start < 0 || start > a.n_tokens - len || a.pos[start] < 0 ? 0 : len;
 }
 
+// Item b of the portions' runs of `toks` tokens (called by a whole warp): info = first token's row, tokens (0: there is no such item), first position, table row
+__device__ __forceinline__ void fp8_find_tokens(const Fp8Attn& a, int b, int toks, int* info) {
+    int s, item, start = 0, len = 0, pos = 0, slot = 0;
+    const bool found = fp8_find(b, a.n_seqs, [&](int i) {
+        start = a.seqs[i];
+        len = a.seqs[a.seqs_stride + i];
+        if (len <= 0 || start < 0 || start > a.n_tokens - len) return 0;
+        pos = a.pos[start];
+        slot = a.slot[start];
+        return pos < 0 ? 0 : (len + toks - 1) / toks;
+    }, s, item);
+    if (found ? (int)(threadIdx.x & 31) == (s & 31) : (threadIdx.x & 31) == 0) {
+        info[0] = start + item * toks;
+        info[1] = found ? min(toks, len - item * toks) : 0;
+        info[2] = pos + item * toks;
+        info[3] = slot;
+    }
+}
+
 // ------------------------------------------------------------------------------------------------ CUDA cores: any head size up to 256, fp32 or bf16
 // grid (tokens, G * head blocks, splits); a warp per query head, the CTA's heads share one key/value head.  Tiles of 32 keys in shared memory as fp32 (code * scale, exact):
 // lane = key for the scores, lane = value column for the weighted sum; running maximum and sum per warp, natural exponentials.
 constexpr int kFgTile = 32, kFgCols = 8;
 template <typename T> __global__ void __launch_bounds__(256) fp8_attn_kernel(const Fp8Attn a) {
     extern __shared__ __align__(16) float fg_smem[];
-    __shared__ int info[2];
+    __shared__ int info[4];
     const int HB = blockDim.x >> 5, R = a.H / a.G, hblocks = (R + HB - 1) / HB, d = a.d, dv = a.dv, ps = a.pages.page_size;
     const int g = blockIdx.y / hblocks, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = (blockIdx.y % hblocks) * HB + warp, h = g * R + r;
     const bool live = r < R;
     griddep_launch_dependents();
     griddep_wait();
-    if (warp == 0) {
-        int s, item;
-        const bool found = fp8_find(blockIdx.x, a.n_seqs, [&](int i) { return fp8_portion(a, i); }, s, item);
-        if (lane == 0) { info[0] = found ? s : -1; info[1] = item; }
-    }
+    if (warp == 0) fp8_find_tokens(a, blockIdx.x, 1, info);
     __syncthreads();
-    if (info[0] < 0) return;
-    const int start = a.seqs[info[0]], p = a.pos[start] + info[1], slot = a.slot[start];
-    const long t = start + info[1];
+    if (info[1] <= 0) return;
+    const int p = info[2], slot = info[3];
+    const long t = info[0];
     float* qs = fg_smem;
     float* Ks = qs + HB * d;
     float* Vs = Ks + kFgTile * (d + 1);
     float* pw = Vs + kFgTile * dv;
-    const int lo = fp8_first_visible(p, a.window, a.chunk), n_keys = p + 1 - lo;
-    const int per = ((n_keys + a.splits - 1) / a.splits + kFgTile - 1) / kFgTile * kFgTile;
-    const int k_lo = lo + blockIdx.z * per, k_hi = min(p + 1, k_lo + per);
+    const int lo = fp8_first_visible(p, a.window, a.chunk), lo16 = lo & ~15;
+    const bool cut = a.part > 0 && p + 1 - lo16 > a.part;
+    const int k_lo = max(lo, lo16 + (int)blockIdx.z * a.part), k_hi = cut ? min(p + 1, lo16 + (int)(blockIdx.z + 1) * a.part) : p + 1;
+    if (blockIdx.z && (!cut || k_lo >= k_hi)) return;
     float acc[kFgCols];
 #pragma unroll
     for (int c = 0; c < kFgCols; c++) acc[c] = 0.f;
@@ -127,8 +144,8 @@ template <typename T> __global__ void __launch_bounds__(256) fp8_attn_kernel(con
         __syncwarp();
     }
     if (!live) return;
-    if (a.partial) {
-        float* o = a.partial + ((t * a.H + h) * a.splits + blockIdx.z) * (dv + 2);
+    if (cut) {
+        float* o = a.partial + ((t * a.H + h) * a.parts + blockIdx.z) * (dv + 2);
         if (lane == 0) { o[0] = m; o[1] = l; }
 #pragma unroll
         for (int c = 0; c < kFgCols; c++)
@@ -151,23 +168,27 @@ template <typename T> __global__ void __launch_bounds__(256) fp8_attn_kernel(con
 // The parts of a cut key range, one CTA of 128 threads for each (token, head): the parts' weights once in shared memory (a part without a key has maximum -inf and weighs
 // nothing; the sink joins the sum), then the columns side by side, parts in order.  `unit`: what turns a difference of maxima into a power of two.
 template <typename T> __global__ void __launch_bounds__(128) fp8_merge_kernel(const Fp8Attn a, float unit) {
-    __shared__ float wgt[kFp8MaxSplits], red[4];
-    __shared__ int mine;
+    __shared__ float wgt[kFp8MaxParts], red[4];
+    __shared__ int count;
     griddep_launch_dependents();
     griddep_wait();
     const long row = blockIdx.x;
-    const int t = (int)(row / a.H), h = (int)(row % a.H), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, splits = a.splits, dv = a.dv;
-    // a token of no portion has no parts
-    if (tid == 0) mine = 0;
+    const int t = (int)(row / a.H), h = (int)(row % a.H), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, dv = a.dv;
+    // the parts of the range that the token's CTA was cut by (none: a token of no portion, or a range in one piece)
+    if (tid == 0) count = 0;
     __syncthreads();
     for (int s = tid; s < a.n_seqs; s += 128) {
-        const int len = fp8_portion(a, s);
-        if (t >= a.seqs[s] && t - a.seqs[s] < len) mine = 1;
+        const int len = fp8_portion(a, s), i = t - a.seqs[s];
+        if (i >= 0 && i < len) {
+            const int i0 = i / a.ctoks * a.ctoks, p0 = a.pos[a.seqs[s]] + i0, lo16 = fp8_first_visible(p0, a.window, a.chunk) & ~15, n = p0 + min(a.ctoks, len - i0) - lo16;
+            if (n > a.part) count = (n + a.part - 1) / a.part;
+        }
     }
     __syncthreads();
-    if (!mine) return;
-    const float* part = a.partial + row * splits * (dv + 2);
-    const float ms = tid < splits ? part[(long)tid * (dv + 2)] : -INFINITY, ls = tid < splits ? part[(long)tid * (dv + 2) + 1] : 0.f;
+    const int parts = min(count, a.parts);
+    if (parts == 0) return;
+    const float* part = a.partial + row * a.parts * (dv + 2);
+    const float ms = tid < parts ? part[(long)tid * (dv + 2)] : -INFINITY, ls = tid < parts ? part[(long)tid * (dv + 2) + 1] : 0.f;
     float m = warp_max(ms);
     if (lane == 0) red[warp] = m;
     __syncthreads();
@@ -181,13 +202,13 @@ template <typename T> __global__ void __launch_bounds__(128) fp8_merge_kernel(co
     __syncthreads();
     float l = (red[0] + red[1]) + (red[2] + red[3]);
     if (a.sink) l += exp2f((sink - m) * unit);
-    if (tid < splits) wgt[tid] = l > 0.f || l != l ? e / l : 0.f;
+    if (tid < parts) wgt[tid] = l > 0.f || l != l ? e / l : 0.f;
     __syncthreads();
     T* out = (T*)a.out + t * a.out_stride + (long)h * dv;
     for (int c = tid; c < dv; c += 128) {
         float acc = 0.f;
 #pragma unroll 8
-        for (int s = 0; s < splits; s++) acc = fmaf(wgt[s], part[(long)s * (dv + 2) + 2 + c], acc);
+        for (int s = 0; s < parts; s++) acc = fmaf(wgt[s], part[(long)s * (dv + 2) + 2 + c], acc);
         out[c] = from_f<T>(acc * a.out_scale);
     }
 }
@@ -197,54 +218,72 @@ template <typename T> __global__ void __launch_bounds__(128) fp8_merge_kernel(co
 
 using namespace ktb;
 
-extern "C" size_t ktb200_fp8_cache_attn_workspace(int n_tokens, int heads, int vdim, int splits) {
-    return splits > 1 ? (size_t)n_tokens * heads * splits * (vdim + 2) * sizeof(float) : 0;
+// the most keys that a CTA's tokens see together, from a multiple of 16 on
+static long fp8_range(const ktb200_fp8_attn_params* c, int max_keys, int ctoks) {
+    long n = max_keys;
+    if (c->window > 0) n = std::min<long>(n, (long)c->window + ctoks);
+    if (c->chunk > 0) n = std::min<long>(n, (long)c->chunk + ctoks);
+    return n + 16;
+}
+static int fp8_ctoks(const ktb200_fp8_attn_params* c, int n_tokens, int dtype, int allow_tensor_cores) { return allow_tensor_cores && fm_takes(c, dtype) ? fm_form(c, n_tokens).toks : 1; }
+static long fp8_tiles(const ktb200_fp8_attn_params* c, int n_tokens, int ctoks) { return std::min<long>(n_tokens, (long)c->n_seqs + n_tokens / ctoks); }
+static bool fp8_sizes_ok(const ktb200_fp8_attn_params* c) { return c && c->heads > 0 && c->kv_heads > 0 && c->heads % c->kv_heads == 0; }
+
+extern "C" size_t ktb200_fp8_cache_attn_workspace(const ktb200_fp8_attn_params* c, int n_tokens, int max_keys, int part, int dtype, int allow_tensor_cores) {
+    if (!fp8_sizes_ok(c) || n_tokens <= 0 || part <= 0) return 0;
+    const long parts = (fp8_range(c, max_keys, fp8_ctoks(c, n_tokens, dtype, allow_tensor_cores)) + part - 1) / part;
+    return parts > 1 ? (size_t)n_tokens * c->heads * parts * (c->vdim + 2) * sizeof(float) : 0;
 }
 
-// Cut the key range when a small batch would leave most SMs idle on a long one
-extern "C" int ktb200_fp8_cache_attn_splits(const ktb200_fp8_attn_params* c, int n_tokens, int max_keys, int dtype, int allow_tensor_cores) {
-    if (!c || c->heads <= 0 || c->kv_heads <= 0 || n_tokens <= 0) return 1;
-    const int R = c->heads / c->kv_heads;
-    if (allow_tensor_cores && fm_takes(c, dtype)) {      // three CTAs an SM; parts of 256 keys or more
-        const long ctas = fm_tiles(c, n_tokens) * c->kv_heads * (R / fm_heads(R));
-        if (ctas >= 296 || max_keys <= 512) return 1;
-        return (int)std::max<long>(1, std::min<long>({kFp8MaxSplits, max_keys / 256, 444 / ctas}));
-    }
-    const long ctas = (long)n_tokens * c->kv_heads * ((R + 7) / 8);
-    if (ctas >= 148 || max_keys <= 256) return 1;
-    return (int)std::max<long>(1, std::min<long>({64, max_keys / 128, 592 / ctas}));
+// Keys of a part: the whole range where the CTAs of uncut ranges fill the SMs' places (three an SM) four times; else so many that one round of CTAs covers the range, and
+// between sequences, whose ranges may have any length, no more than 1024
+extern "C" int ktb200_fp8_cache_attn_part(const ktb200_fp8_attn_params* c, int n_tokens, int max_keys, int dtype, int allow_tensor_cores) {
+    if (!fp8_sizes_ok(c) || n_tokens <= 0) return 0;
+    const int R = c->heads / c->kv_heads, ctoks = fp8_ctoks(c, n_tokens, dtype, allow_tensor_cores);
+    const long tiles = fp8_tiles(c, n_tokens, ctoks), range = fp8_range(c, max_keys, ctoks), places = 3 * 148;
+    const long ctas = tiles * c->kv_heads * (ctoks == 1 && !(allow_tensor_cores && fm_takes(c, dtype)) ? (R + 7) / 8 : R / fm_heads(R));
+    if (ctas >= 4 * places || range <= 2 * kFp8MinPart) return 0;
+    long part = (range * ctas + places - 1) / places;
+    if (c->n_seqs > 1) part = std::min<long>(part, 1024);
+    part = std::max<long>({part, kFp8MinPart, (range + kFp8MaxParts - 1) / kFp8MaxParts});
+    part = (part + 63) / 64 * 64;
+    return part < range ? (int)part : 0;
 }
 
-extern "C" int ktb200_fp8_cache_attn(const ktb200_fp8_attn_params* c, int n_tokens, int splits, float* workspace, int dtype, int allow_tensor_cores, void* stream) {
-    if (!c || c->heads <= 0 || c->kv_heads <= 0 || c->heads % c->kv_heads || c->dim <= 0 || c->dim > 32 * kFgCols || c->vdim <= 0 || c->vdim > 32 * kFgCols || c->page_size <= 0 ||
-        c->max_pages <= 0 || c->n_pages < 0 || c->n_slots <= 0 || c->n_seqs < 0 || c->window < 0 || c->chunk < 0 || c->out_stride < (long)c->heads * c->vdim) {
+extern "C" int ktb200_fp8_cache_attn(const ktb200_fp8_attn_params* c, int n_tokens, int max_keys, int part, float* workspace, size_t workspace_bytes, int dtype, int allow_tensor_cores,
+                                     void* stream) {
+    if (!fp8_sizes_ok(c) || c->dim <= 0 || c->dim > 32 * kFgCols || c->vdim <= 0 || c->vdim > 32 * kFgCols || c->page_size <= 0 || c->max_pages <= 0 || c->n_pages < 0 || c->n_slots <= 0 ||
+        c->n_seqs < 0 || c->window < 0 || c->chunk < 0 || c->out_stride < (long)c->heads * c->vdim) {
         set_error("fp8_cache_attn: bad argument (head sizes up to %d)", 32 * kFgCols);
         return KTB200_EINVAL;
     }
     if (dtype != KTB200_TYPE_BF16 && dtype != KTB200_TYPE_F32) { set_error("fp8_cache_attn: dtype must be bf16 or f32"); return KTB200_EINVAL; }
-    if (splits < 1 || splits > kFp8MaxSplits) { set_error("fp8_cache_attn: 1 to %d splits", kFp8MaxSplits); return KTB200_EINVAL; }
+    if (part < 0 || part % 64 || max_keys < 0) { set_error("fp8_cache_attn: part %d (a multiple of 64 or 0), max_keys %d", part, max_keys); return KTB200_EINVAL; }
     if (n_tokens <= 0 || c->n_seqs == 0) return KTB200_OK;
     if (!c->q || !c->pos || !c->slot || !c->seqs || !c->page_table || !c->k_codes || !c->v_codes || !c->scales || !c->out) { set_error("fp8_cache_attn: null pointer"); return KTB200_EINVAL; }
-    if (splits > 1 && !workspace) { set_error("fp8_cache_attn: workspace missing"); return KTB200_EINVAL; }
-    const int R = c->heads / c->kv_heads, HB = std::min(R, 8), hblocks = (R + HB - 1) / HB;
-    if ((long)c->kv_heads * hblocks > 65535 || (long)n_tokens * c->heads > 0x7fffffffL) { set_error("fp8_cache_attn: too many heads or tokens"); return KTB200_EINVAL; }
+    const bool bf16 = dtype == KTB200_TYPE_BF16, tiles = allow_tensor_cores && fm_takes(c, dtype);
+    const int R = c->heads / c->kv_heads, ctoks = fp8_ctoks(c, n_tokens, dtype, allow_tensor_cores);
+    const long parts = part ? (fp8_range(c, max_keys, ctoks) + part - 1) / part : 1;
+    if (parts > kFp8MaxParts) { set_error("fp8_cache_attn: %ld parts, at most %d", parts, kFp8MaxParts); return KTB200_EINVAL; }
+    const size_t need = ktb200_fp8_cache_attn_workspace(c, n_tokens, max_keys, part, dtype, allow_tensor_cores);
+    if (need && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 7))) { set_error("fp8_cache_attn: workspace missing, too small or not aligned"); return KTB200_EINVAL; }
+    const int HB = std::min(R, 8), hblocks = (R + HB - 1) / HB;
+    if ((long)c->kv_heads * R > 65535 || (long)n_tokens * c->heads > 0x7fffffffL) { set_error("fp8_cache_attn: too many heads or tokens"); return KTB200_EINVAL; }
     const cudaStream_t s = (cudaStream_t)stream;
     const Fp8Attn a{c->q, c->heads, c->kv_heads, c->dim, c->vdim, c->scale, c->head_scale, c->softcap, c->window, c->chunk, c->sink, c->out_scale, c->pos, c->slot, c->seqs, c->seqs_stride,
                     c->n_seqs, n_tokens, {c->page_table, c->n_slots, c->max_pages, c->page_size, c->n_pages}, (const uint8_t*)c->k_codes, (const uint8_t*)c->v_codes, c->scales, c->out,
-                    c->out_stride, splits > 1 ? workspace : nullptr, splits};
-    const bool bf16 = dtype == KTB200_TYPE_BF16, tiles = allow_tensor_cores && fm_takes(c, dtype);
+                    c->out_stride, workspace, parts > 1 ? part : 0, (int)parts, ctoks};
+    const unsigned nt = (unsigned)fp8_tiles(c, n_tokens, ctoks);
     if (tiles) {
-        const int RH = fm_heads(R);
-        const dim3 grid((unsigned)fm_tiles(c, n_tokens), c->kv_heads * (R / RH), splits);
-        KTB_CUDA_CHECK(fm_shared(c, n_tokens) ? fm_launch<true>(a, RH, grid, s) : fm_launch<false>(a, RH, grid, s));
+        const FmForm f = fm_form(c, n_tokens);
+        KTB_CUDA_CHECK(fm_launch(a, f, dim3(nt, c->kv_heads * (R / f.RH), (unsigned)parts), s));
     } else {
-    const size_t smem = ((size_t)HB * c->dim + (size_t)kFgTile * (c->dim + 1) + (size_t)kFgTile * c->vdim + (size_t)HB * kFgTile) * sizeof(float);
-    const dim3 grid(n_tokens, c->kv_heads * hblocks, splits);
-    KTB_CUDA_CHECK(raise_smem_limit(bf16 ? (const void*)fp8_attn_kernel<__nv_bfloat16> : (const void*)fp8_attn_kernel<float>, smem));
-    KTB_CUDA_CHECK(launch_pdl(bf16 ? fp8_attn_kernel<__nv_bfloat16> : fp8_attn_kernel<float>, grid, dim3(HB * 32), smem, s, a));
+        const size_t smem = ((size_t)HB * c->dim + (size_t)kFgTile * (c->dim + 1) + (size_t)kFgTile * c->vdim + (size_t)HB * kFgTile) * sizeof(float);
+        KTB_CUDA_CHECK(raise_smem_limit(bf16 ? (const void*)fp8_attn_kernel<__nv_bfloat16> : (const void*)fp8_attn_kernel<float>, smem));
+        KTB_CUDA_CHECK(launch_pdl(bf16 ? fp8_attn_kernel<__nv_bfloat16> : fp8_attn_kernel<float>, dim3(nt, c->kv_heads * hblocks, (unsigned)parts), dim3(HB * 32), smem, s, a));
     }
     count_launch();
-    if (splits > 1) {
+    if (parts > 1) {
         KTB_CUDA_CHECK(launch_pdl(bf16 ? fp8_merge_kernel<__nv_bfloat16> : fp8_merge_kernel<float>, dim3((unsigned)((long)n_tokens * c->heads)), dim3(128), (size_t)0, s, a, tiles ? 1.0f : kLog2e));
         count_launch();
     }

@@ -1,16 +1,18 @@
-// Attention over the paged e4m3 cache on m16n8k16 fp16 tiles (bf16 queries, head sizes that are multiples of 16 up to 128): decode steps and short portions.
+// Attention over the paged e4m3 cache on the tensor cores' mma tiles (bf16 queries, head sizes that are multiples of 16 up to 128): decode steps and short portions.
 //
-// A warp owns 16 rows = (token, query head) pairs of one portion and one key/value head and takes 16 keys at a time:  S = Q K^T,  t = s log2(e) + log2(value scale),
-// p = 2^(t - m),  O += P V,  l += p / (value scale).  Codes go to the tensor cores as fp16, which holds every e4m3 number exactly (one conversion for two codes); queries
-// as fp16 too, each row first moved by a power of two so that its largest stands below 2^15 (exact for what is within 2^-28 of that); key scales multiply scores.  A block's value scale is
-// a power of two in the weight's exponent, so that O needs no scale at all and the weights of all blocks stand in one range: p <= 2^8 (m is raised only when a row's t
-// outgrows it by 8), rounded to fp16 (2^-12 of a weight).  O / l is the result: 2^m drops out.
+// A warp owns 8 or 16 rows = (token, query head) pairs of one portion and one key/value head and takes 16 keys at a time:  S = Q K^T,  t = s log2(e) + log2(value scale),
+// p = 2^(t - m),  O += P V,  l += p / (value scale).
+//   S   m16n8k32 e4m3: the keys' codes as they are, against each query row as two e4m3 rows, q = q1 + q2 / 16 once the row is moved by a power of two so that its
+//       largest stands in [128, 256): exact for bf16 numbers down to 2^-13 of that largest, 2^-21 of it off below
+//   O   m16n8k16 fp16: codes as fp16, which holds every e4m3 number exactly (one conversion for two), weights rounded to fp16 (2^-11 of a weight)
+// Key scales multiply scores.  A block's value scale is a power of two in the weight's exponent, so that O needs no scale and the weights of all blocks stand in
+// one range: m is raised only when a row's t outgrows it by 8, p <= 2^8.  O / l is the result: 2^m drops out.
 //
-// The order of a product's sum is free, and taken so that no shuffling is needed: of a key's row, the four threads that share it hold 16 neighbouring bytes each (a mma
-// step takes 4 of them), and of a value's row each of the eight column groups has its neighbouring bytes, an output tile's columns being dv / 8 apart.
+// The order of a product's sum is free, and taken so that no shuffling is needed: of a key's row, the four threads that share it hold 16 neighbouring bytes each (an S
+// step takes 8 of them), and of a value's row each of the eight column groups has its neighbouring bytes, an output tile's columns being dv / 8 apart.
 //
-// SHARED = false: the CTA's four warps own the same 16 rows and cut the keys among them, tile by tile (decode: a group's heads fill the rows and one pass over the
-// keys serves all); each has its own cp.async ring, no barrier in the loop; their sums are joined at the end in shared memory.
+// SHARED = false: the CTA's four warps own the same rows and cut the keys among them, tile by tile (decode: a group's heads fill the rows and one pass over the
+// keys serves all); each has its own cp.async ring, no barrier in the loop; their sums are joined at the end in shared memory.  TWO: 16 rows, else 8.
 // SHARED = true: the warps own 64 rows and share each key tile (16 keys brought by each warp), for portions of many tokens.
 #pragma once
 #include "mma_tile.cuh"
@@ -23,6 +25,18 @@ __device__ __forceinline__ void mma_f16_16816(float (&c)[4], const uint32_t (&a)
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// c (16 rows x 8) += a (16 x 32) b (32 x 8), e4m3
+__device__ __forceinline__ void mma_e4m3_16832(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// two numbers as e4m3 codes (the first in the low byte), and as codes 16 times what those leave of them
+__device__ __forceinline__ uint2 split_e4m3(float lo, float hi) {
+    const uint32_t first = __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
+    const float2 got = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)first, __NV_E4M3)));
+    return make_uint2(first, __nv_cvt_float2_to_fp8x2(make_float2((lo - got.x) * 16.f, (hi - got.y) * 16.f), __NV_SATFINITE, __NV_E4M3));
 }
 // two e4m3 codes (the low half of a word) as two fp16 numbers
 __device__ __forceinline__ uint32_t f16_of_codes(uint32_t two) {
@@ -68,118 +82,145 @@ template <int DP, int DVP, bool SHARED> constexpr int fm_smem() {
     return ring > join || SHARED ? ring : join;
 }
 
-template <int DP, int DVP, bool SHARED> __global__ void __launch_bounds__(kFmThreads, 3) fp8_attn_mma_kernel(const Fp8Attn a, int RH) {
-    constexpr int KC = DP / 64, VB = DVP / 8, TILE = fm_tile_bytes<DP, DVP>(), STAGES = fm_stages<SHARED>(), NT = DVP / 8;
+template <int DP, int DVP, bool SHARED, bool TWO> __global__ void __launch_bounds__(kFmThreads, 3) fp8_attn_mma_kernel(const Fp8Attn a, int RH) {
+    constexpr int KC = DP / 64, VB = DVP / 8, TILE = fm_tile_bytes<DP, DVP>(), STAGES = fm_stages<SHARED>(), NT = DVP / 8, ROWS = TWO ? 2 : 1;
     extern __shared__ __align__(16) unsigned char fm_smem_raw[];
-    __shared__ int info[2];
+    __shared__ int info[6];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gq = lane >> 2, tq = lane & 3;
-    const int d = a.d, dv = a.dv, ps = a.pages.page_size, TOKS = 16 / RH, CTOKS = SHARED ? kFmWarps * TOKS : TOKS, R = a.H / a.G, hblocks = R / RH;
+    const int d = a.d, dv = a.dv, ps = a.pages.page_size, TOKS = 8 * ROWS / RH, CTOKS = a.ctoks, R = a.H / a.G, hblocks = R / RH;
     const uint32_t smem = (uint32_t)__cvta_generic_to_shared(fm_smem_raw);
     griddep_launch_dependents();
     griddep_wait();
-    if (warp == 0) {
-        int s, item;
-        const bool found = fp8_find(blockIdx.x, a.n_seqs, [&](int i) { return (fp8_portion(a, i) + CTOKS - 1) / CTOKS; }, s, item);
-        if (lane == 0) { info[0] = found ? s : -1; info[1] = item * CTOKS; }
-    }
+    if (warp == 0) fp8_find_tokens(a, blockIdx.x, CTOKS, info);
     // columns behind a head's last are zeros throughout
     if (d < DP || dv < DVP)
         for (int i = tid; i < kFmWarps * STAGES * TILE / 16; i += kFmThreads) reinterpret_cast<uint4*>(fm_smem_raw)[i] = make_uint4(0, 0, 0, 0);
     __syncthreads();
-    if (info[0] < 0) return;
-    const int start = a.seqs[info[0]], len = a.seqs[a.seqs_stride + info[0]], tok0 = start + info[1], ntok = min(CTOKS, len - info[1]), pos0 = a.pos[start] + info[1], slot = a.slot[start];
+    const int tok0 = info[0], ntok = info[1], pos0 = info[2], slot = info[3];
+    if (ntok <= 0) return;
     const int g = blockIdx.y / hblocks, h0 = g * R + (blockIdx.y % hblocks) * RH, max_pos = pos0 + ntok - 1;
-    // the CTA's key range, cut into this split's part in whole tiles that begin at multiples of 16
-    const int lo = fp8_first_visible(pos0, a.window, a.chunk), lo16 = lo & ~(kFmKeys - 1), n_keys = max_pos + 1 - lo16;
+    // the key range of the CTA's tokens, in parts that begin at multiples of 16
+    const int lo = fp8_first_visible(pos0, a.window, a.chunk), lo16 = lo & ~(kFmKeys - 1);
     constexpr int STEP = kFmWarps * kFmKeys;
-    const int per = ((n_keys + a.splits - 1) / a.splits + STEP - 1) / STEP * STEP;
-    const int k_lo = lo16 + blockIdx.z * per, k_hi = min(max_pos + 1, k_lo + per);
-    // this thread's two rows
+    const bool cut = a.part > 0 && max_pos + 1 - lo16 > a.part;
+    const int k_lo = lo16 + blockIdx.z * a.part, k_hi = cut ? min(max_pos + 1, k_lo + a.part) : max_pos + 1;
+    if (k_lo >= k_hi) return;
+    // this thread's rows
     const int wtok = SHARED ? warp * TOKS : 0, rows = TOKS * RH;
     const int tokA = wtok + gq / RH, tokB = wtok + (gq + 8) / RH, hA = h0 + gq % RH, hB = h0 + (gq + 8) % RH;
-    const bool vA = gq < rows && tokA < ntok, vB = gq + 8 < rows && tokB < ntok;
+    const bool vA = gq < rows && tokA < ntok, vB = TWO && gq + 8 < rows && tokB < ntok;
     const int pA = pos0 + tokA, pB = pos0 + tokB, fA = fp8_first_visible(pA, a.window, a.chunk), fB = fp8_first_visible(pB, a.window, a.chunk);
-    const bool two = rows > 8;      // rows 8 .. 15 carry something
     float O[NT][4];
 #pragma unroll
     for (int n = 0; n < NT; n++)
 #pragma unroll
         for (int e = 0; e < 4; e++) O[n][e] = 0.f;
     float mA = -INFINITY, mB = -INFINITY, lA = 0.f, lB = 0.f;
-    if (k_lo < k_hi) {
+    {
         // ---------------------------------------------------------------- the ring: a tile is 16 keys from a multiple of 16 on
-        const int* pt = a.pages.table + (long)slot * a.pages.max_pages;
         const bool slot_ok = (unsigned)slot < (unsigned)a.pages.slots, whole = ps % kFmKeys == 0;
+        const int* pt = a.pages.table + (slot_ok ? (long)slot * a.pages.max_pages : 0);
         const uint32_t ring = smem + warp * STAGES * TILE;
+        const int piece = lane & 7, r4 = lane >> 3;      // eight neighbouring lanes bring a row's 128 bytes
+        // the page of the tile (or of the lane's row in it) that is brought next, looked up a tile ahead, and the row in that page
+        int page = -1, off = 0, logical = 0, col = 0;
+        auto look = [&](int k0) {
+            const int kp = whole ? k0 : k0 + (lane & 15);
+            page = -1;
+            if (kp >= k_hi || !slot_ok) return;
+            if (!whole) { logical = kp / ps; off = kp - logical * ps; col = logical % a.pages.max_pages; }
+            page = pt[col];
+            if ((unsigned)page >= (unsigned)a.pages.n_pages) page = -1;
+        };
         auto load_tile = [&](int stage, int k0) {      // this warp's 16 keys from k0 on
             if (k0 < k_hi) {
                 const uint32_t kd = ring + stage * TILE, vd = kd + kFmKeys * DP, sd = vd + kFmKeys * DVP;
-                // rows 0 .. 15: a page and a row in it for each (one page for all where pages are whole tiles)
-                int page = -1, off = 0;
-                const int r16 = lane & 15, kp = whole ? k0 : k0 + r16;
-                if (kp < k_hi) {
-                    const int logical = kp / ps;
-                    off = kp - logical * ps;
-                    page = slot_ok ? pt[logical % a.pages.max_pages] : -1;
-                    if ((unsigned)page >= (unsigned)a.pages.n_pages) page = -1;
-                }
-                const long block = (long)page * a.G + g;
-                {
-                    const bool ok = page >= 0 && k0 + r16 < k_hi && k0 + r16 >= lo;
-                    if (lane < 16) cp_async_bytes8(sd + 8 * r16, ok ? a.scales + 2 * block : a.scales, ok);
-                }
-                // eight neighbouring lanes bring the row's 128 bytes
-                const int piece = lane & 7, r4 = lane >> 3;
-                long row_of = block * ps + off;
+                const long block = (long)page * a.G + g, row0 = block * ps + off;
+                // (keys that no row sees may be anything, NaN too: they come as zeros, and so do those of pages that are not there)
+                const bool full = whole && k0 >= lo && k0 + kFmKeys <= k_hi && page >= 0;
+                const int r16 = lane & 15;
+                const bool ok16 = page >= 0 && k0 + r16 < k_hi && k0 + r16 >= lo;
+                if (lane < 16) cp_async_bytes8(sd + 8 * r16, ok16 ? a.scales + 2 * block : a.scales, ok16);
+                // a key row's chunks change halves in odd rows, a value row's by its number: no two of the lanes that read together meet in a bank
+                const uint32_t kx = 16 * (DP == 128 ? piece ^ ((r4 & 1) << 2) : piece);
+                if (full) {
+                    const uint8_t *k = a.k_codes + (row0 + r4) * d + 16 * piece, *v = a.v_codes + (row0 + r4) * dv + 16 * piece;
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int r = 4 * i + r4;
-                    const long row = whole ? row_of + r : __shfl_sync(0xffffffffu, row_of, r);
-                    const bool ok = (whole ? page : __shfl_sync(0xffffffffu, page, r)) >= 0 && k0 + r < k_hi && k0 + r >= lo;      // (keys that no row sees may be anything, NaN too: they come as zeros)
-                    // a key row's chunks change halves in odd rows, a value row's by its number: no two of the lanes that read together meet in a bank
-                    if (16 * piece < d) cp_async_bytes16(kd + r * DP + 16 * (DP == 128 ? piece ^ ((r & 1) << 2) : piece), ok ? a.k_codes + row * d + 16 * piece : a.k_codes, ok);
-                    if (16 * piece < dv) cp_async_bytes16(vd + r * DVP + 16 * (DVP == 128 ? piece ^ (r & 7) : piece ^ ((r >> 1) & 3)), ok ? a.v_codes + row * dv + 16 * piece : a.v_codes, ok);
+                    for (int i = 0; i < 4; i++) {
+                        const int r = 4 * i + r4;
+                        if (16 * piece < d) cp_async_bytes16(kd + r * DP + kx, k + 4 * i * d, true);
+                        if (16 * piece < dv) cp_async_bytes16(vd + r * DVP + 16 * (DVP == 128 ? piece ^ (r & 7) : piece ^ ((r >> 1) & 3)), v + 4 * i * dv, true);
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const int r = 4 * i + r4;
+                        const long row = whole ? row0 + r : __shfl_sync(0xffffffffu, row0, r);
+                        const bool ok = (whole ? page : __shfl_sync(0xffffffffu, page, r)) >= 0 && k0 + r < k_hi && k0 + r >= lo;
+                        if (16 * piece < d) cp_async_bytes16(kd + r * DP + kx, ok ? a.k_codes + row * d + 16 * piece : a.k_codes, ok);
+                        if (16 * piece < dv) cp_async_bytes16(vd + r * DVP + 16 * (DVP == 128 ? piece ^ (r & 7) : piece ^ ((r >> 1) & 3)), ok ? a.v_codes + row * dv + 16 * piece : a.v_codes, ok);
+                    }
                 }
+                if (whole) {
+                    off += STEP;
+                    while (off >= ps) {
+                        off -= ps;
+                        if (++col == a.pages.max_pages) col = 0;
+                    }
+                }
+                look(k0 + STEP);
             }
             cp_async_commit();
         };
+        if (whole) {
+            const int k0 = k_lo + warp * kFmKeys;
+            logical = k0 / ps; off = k0 - logical * ps; col = logical % a.pages.max_pages;
+        }
+        look(k_lo + warp * kFmKeys);
 #pragma unroll
         for (int i = 0; i < STAGES - 1; i++) load_tile(i, k_lo + warp * kFmKeys + i * STEP);
-        // ---------------------------------------------------------------- queries: fp16, row by row below 2^15; the thread's 16 columns of every 64
-        uint32_t Q[4 * KC][4];
-        float fac[2];
-        {
-            uint32_t w[2][8 * KC];
-            const __nv_bfloat16* q = (const __nv_bfloat16*)a.q;
+        // ---------------------------------------------------------------- queries: the thread's 16 columns of every 64, split into two e4m3 rows
+        uint32_t Q[ROWS][2 * KC][4];
+        float fac[ROWS];
 #pragma unroll
-            for (int r = 0; r < 2; r++) {
-                const bool v = r ? vB : vA;
-                const __nv_bfloat16* row = q + ((long)(tok0 + (r ? tokB : tokA)) * a.H + (r ? hB : hA)) * d;
+        for (int r = 0; r < ROWS; r++) {
+            const bool v = r ? vB : vA;
+            const __nv_bfloat16* row = (const __nv_bfloat16*)a.q + ((long)(tok0 + (r ? tokB : tokA)) * a.H + (r ? hB : hA)) * d;
+            uint32_t w[8 * KC];
 #pragma unroll
-                for (int c = 0; c < KC; c++)
+            for (int c = 0; c < KC; c++)
 #pragma unroll
-                    for (int i = 0; i < 2; i++) {
-                        const int col = 64 * c + 16 * tq + 8 * i;
-                        uint4 x = make_uint4(0, 0, 0, 0);
-                        if (v && col < d) x = *reinterpret_cast<const uint4*>(row + col);
-                        w[r][8 * c + 4 * i] = x.x; w[r][8 * c + 4 * i + 1] = x.y; w[r][8 * c + 4 * i + 2] = x.z; w[r][8 * c + 4 * i + 3] = x.w;
-                    }
-                float top = 0.f;
+                for (int i = 0; i < 2; i++) {
+                    const int at = 64 * c + 16 * tq + 8 * i;
+                    uint4 x = make_uint4(0, 0, 0, 0);
+                    if (v && at < d) x = *reinterpret_cast<const uint4*>(row + at);
+                    w[8 * c + 4 * i] = x.x; w[8 * c + 4 * i + 1] = x.y; w[8 * c + 4 * i + 2] = x.z; w[8 * c + 4 * i + 3] = x.w;
+                }
+            float top = 0.f, odd = 0.f;      // odd: NaN as soon as a value is not finite (e4m3 has no infinity)
 #pragma unroll
-                for (int i = 0; i < 8 * KC; i++) top = fmaxf(top, fmaxf(fabsf(__uint_as_float(w[r][i] << 16)), fabsf(__uint_as_float(w[r][i] & 0xffff0000u))));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                // 2^(14 - e) of a largest 1.f 2^e, within what fp32 holds with its inverse
-                const int up = min(126, max(-112, 14 - ((int)(__float_as_uint(top) >> 23) - 127)));
-                const float by = __uint_as_float((uint32_t)(up + 127) << 23);
-                const float hs = v ? (a.head_scale ? a.scale * a.head_scale[r ? hB : hA] : a.scale) : 0.f;
-                fac[r] = hs / by * (a.softcap > 0.f ? 1.f : kLog2e);
-#pragma unroll
-                for (int i = 0; i < 8 * KC; i++) w[r][i] = pack_f16(__uint_as_float(w[r][i] << 16) * by, __uint_as_float(w[r][i] & 0xffff0000u) * by);
+            for (int i = 0; i < 8 * KC; i++) {
+                const float x = __uint_as_float(w[i] << 16), y = __uint_as_float(w[i] & 0xffff0000u);
+                top = fmaxf(top, fmaxf(fabsf(x), fabsf(y)));
+                odd = fmaf(x, 0.f, fmaf(y, 0.f, odd));
             }
-            // word pair (2 s, 2 s + 1) of a 64-column chunk: columns 4 s .. 4 s + 3 of the thread's 16
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            odd += __shfl_xor_sync(0xffffffffu, odd, 1);
+            odd += __shfl_xor_sync(0xffffffffu, odd, 2);
+            // 2^(7 - e) of a largest 1.f 2^e, within what fp32 holds with its inverse
+            const int up = min(126, max(-120, 7 - ((int)(__float_as_uint(top) >> 23) - 127)));
+            const float by = __uint_as_float((uint32_t)(up + 127) << 23);
+            fac[r] = v ? (a.head_scale ? a.scale * a.head_scale[r ? hB : hA] : a.scale) / by * (a.softcap > 0.f ? 1.f : kLog2e) + odd : 0.f;
 #pragma unroll
-            for (int s = 0; s < 4 * KC; s++) { Q[s][0] = w[0][2 * s]; Q[s][1] = w[1][2 * s]; Q[s][2] = w[0][2 * s + 1]; Q[s][3] = w[1][2 * s + 1]; }
+            for (int s = 0; s < 2 * KC; s++)      // columns 8 s .. 8 s + 7 of the thread's
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    const uint32_t u = w[4 * s + 2 * i], x = w[4 * s + 2 * i + 1];
+                    const uint2 lo2 = split_e4m3(__uint_as_float(u << 16) * by, __uint_as_float(u & 0xffff0000u) * by);
+                    const uint2 hi2 = split_e4m3(__uint_as_float(x << 16) * by, __uint_as_float(x & 0xffff0000u) * by);
+                    Q[r][s][2 * i] = lo2.x | hi2.x << 16;
+                    Q[r][s][2 * i + 1] = lo2.y | hi2.y << 16;
+                }
         }
         const float two_over_cap = a.softcap > 0.f ? 2.0f / a.softcap : 0.f;
         const int w_min_pos = pos0 + wtok, w_max_pos = pos0 + min(ntok - 1, wtok + TOKS - 1);
@@ -190,21 +231,33 @@ template <int DP, int DVP, bool SHARED> __global__ void __launch_bounds__(kFmThr
             float S[2][4];
 #pragma unroll
             for (int n = 0; n < 2; n++) {
-#pragma unroll
-                for (int e = 0; e < 4; e++) S[n][e] = 0.f;
                 const int r = 8 * n + gq;
+                float acc[ROWS][4];
+#pragma unroll
+                for (int h = 0; h < ROWS; h++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) acc[h][e] = 0.f;
 #pragma unroll
                 for (int c = 0; c < KC; c++) {
                     const uint4 k = lds16(kd + r * DP + 16 * (DP == 128 ? (4 * c + tq) ^ ((r & 1) << 2) : tq));
-                    const uint32_t kw[4] = {k.x, k.y, k.z, k.w};
 #pragma unroll
-                    for (int s = 0; s < 4; s++) mma_f16_16816(S[n], Q[4 * c + s], f16_of_codes(kw[s]), f16_of_codes(kw[s] >> 16));
+                    for (int h = 0; h < ROWS; h++) {
+                        mma_e4m3_16832(acc[h], Q[h][2 * c][0], Q[h][2 * c][1], Q[h][2 * c][2], Q[h][2 * c][3], k.x, k.y);
+                        mma_e4m3_16832(acc[h], Q[h][2 * c + 1][0], Q[h][2 * c + 1][1], Q[h][2 * c + 1][2], Q[h][2 * c + 1][3], k.z, k.w);
+                    }
                 }
+#pragma unroll
+                for (int h = 0; h < ROWS; h++)
+#pragma unroll
+                    for (int i = 0; i < 2; i++) S[n][2 * h + i] = fmaf(acc[h][2 + i], 0.0625f, acc[h][i]);
+                if (!TWO) S[n][2] = S[n][3] = 0.f;
             }
             // the thread's keys: k0 + 8 n + 2 tq + {0, 1}
             float inv[4];
             const bool plain = k0 + kFmKeys - 1 <= w_min_pos && k0 >= w_last_first && k0 + kFmKeys <= k_hi;
-            float tA = -INFINITY, tB = -INFINITY;
+            float top[ROWS];
+#pragma unroll
+            for (int h = 0; h < ROWS; h++) top[h] = -INFINITY;
 #pragma unroll
             for (int n = 0; n < 2; n++) {
                 const uint4 sc = lds16(sd + 8 * (8 * n + 2 * tq));
@@ -214,53 +267,52 @@ template <int DP, int DVP, bool SHARED> __global__ void __launch_bounds__(kFmThr
                 for (int i = 0; i < 2; i++) {
                     const int key = k0 + 8 * n + 2 * tq + i;
                     const float ve = (float)((int)(vs[i] >> 23) - 127);
-                    inv[2 * n + i] = __uint_as_float((254u << 23) - vs[i]);      // 1 / value scale
-                    float x = S[n][i] * (fac[0] * ks[i]), y = S[n][2 + i] * (fac[1] * ks[i]);
-                    if (a.softcap > 0.f) {
-                        // c tanh(s / c) as c (1 - 2 / (exp(2 s / c) + 1)): absolute error of a few 1e-7 of the cap
-                        x = a.softcap * kLog2e * (1.0f - __fdividef(2.0f, __expf(x * two_over_cap) + 1.0f));
-                        y = a.softcap * kLog2e * (1.0f - __fdividef(2.0f, __expf(y * two_over_cap) + 1.0f));
+                    inv[2 * n + i] = vs[i] ? __uint_as_float((254u << 23) - vs[i]) : 0.f;      // 1 / value scale (a page that is not there: scales of zero)
+#pragma unroll
+                    for (int h = 0; h < ROWS; h++) {
+                        float x = S[n][2 * h + i] * (fac[h] * ks[i]);
+                        if (a.softcap > 0.f) x = a.softcap * kLog2e * (1.0f - __fdividef(2.0f, __expf(x * two_over_cap) + 1.0f));      // c tanh(s / c): a few 1e-7 of the cap off
+                        x += ve;
+                        if (!plain && !((h ? vB : vA) && key <= (h ? pB : pA) && key >= (h ? fB : fA) && key < k_hi)) x = -INFINITY;
+                        if (vs[i] == 0) x = -INFINITY;
+                        S[n][2 * h + i] = x;
+                        top[h] = fmaxf(top[h], x);
                     }
-                    x += ve;
-                    y += ve;
-                    // (a page that is not there: scales of zero)
-                    if (!plain || vs[i] == 0) {
-                        const bool here = vs[i] != 0 && key < k_hi;
-                        if (!(here && vA && key <= pA && key >= fA)) x = -INFINITY;
-                        if (!(here && vB && key <= pB && key >= fB)) y = -INFINITY;
-                        if (vs[i] == 0) inv[2 * n + i] = 0.f;
-                    }
-                    S[n][i] = x;
-                    S[n][2 + i] = y;
-                    tA = fmaxf(tA, x);
-                    tB = fmaxf(tB, y);
                 }
             }
-            tA = fmaxf(tA, __shfl_xor_sync(0xffffffffu, tA, 1));
-            tA = fmaxf(tA, __shfl_xor_sync(0xffffffffu, tA, 2));
-            tB = fmaxf(tB, __shfl_xor_sync(0xffffffffu, tB, 1));
-            tB = fmaxf(tB, __shfl_xor_sync(0xffffffffu, tB, 2));
-            const bool upA = tA > mA + 8.f || (mA == -INFINITY && tA > -INFINITY), upB = tB > mB + 8.f || (mB == -INFINITY && tB > -INFINITY);
-            if (__any_sync(0xffffffffu, upA || upB)) {
-                const float cA = upA ? exp2_approx(mA - tA) : 1.f, cB = upB ? exp2_approx(mB - tB) : 1.f;      // (2^-inf = 0: nothing was summed yet)
-                if (upA) mA = tA;
-                if (upB) mB = tB;
-                lA *= cA;
-                lB *= cB;
+            bool raise[ROWS], any = false;
 #pragma unroll
-                for (int n = 0; n < NT; n++) { O[n][0] *= cA; O[n][1] *= cA; O[n][2] *= cB; O[n][3] *= cB; }
+            for (int h = 0; h < ROWS; h++) {
+                top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
+                top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
+                const float m = h ? mB : mA;
+                raise[h] = top[h] > m + 8.f || (m == -INFINITY && top[h] > -INFINITY);
+                any |= raise[h];
             }
-            const float uA = mA == -INFINITY ? 0.f : mA, uB = mB == -INFINITY ? 0.f : mB;
+            if (__any_sync(0xffffffffu, any)) {
 #pragma unroll
-            for (int n = 0; n < 2; n++)
+                for (int h = 0; h < ROWS; h++) {
+                    float &m = h ? mB : mA, &l = h ? lB : lA;
+                    const float k = raise[h] ? exp2_approx(m - top[h]) : 1.f;      // (2^-inf = 0: nothing was summed yet)
+                    if (raise[h]) m = top[h];
+                    l *= k;
 #pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    S[n][i] = exp2_approx(S[n][i] - uA);
-                    lA = fmaf(S[n][i], inv[2 * n + i], lA);
-                    S[n][2 + i] = exp2_approx(S[n][2 + i] - uB);
-                    lB = fmaf(S[n][2 + i], inv[2 * n + i], lB);
+                    for (int n = 0; n < NT; n++) { O[n][2 * h] *= k; O[n][2 * h + 1] *= k; }
                 }
-            const uint32_t P[4] = {pack_f16(S[0][0], S[0][1]), pack_f16(S[0][2], S[0][3]), pack_f16(S[1][0], S[1][1]), pack_f16(S[1][2], S[1][3])};
+            }
+#pragma unroll
+            for (int h = 0; h < ROWS; h++) {
+                const float m = h ? mB : mA, u = m == -INFINITY ? 0.f : m;
+                float &l = h ? lB : lA;
+#pragma unroll
+                for (int n = 0; n < 2; n++)
+#pragma unroll
+                    for (int i = 0; i < 2; i++) {
+                        S[n][2 * h + i] = exp2_approx(S[n][2 * h + i] - u);
+                        l = fmaf(S[n][2 * h + i], inv[2 * n + i], l);
+                    }
+            }
+            const uint32_t P[4] = {pack_f16(S[0][0], S[0][1]), TWO ? pack_f16(S[0][2], S[0][3]) : 0u, pack_f16(S[1][0], S[1][1]), TWO ? pack_f16(S[1][2], S[1][3]) : 0u};
             // values: rows 2 tq, 2 tq + 1 and 8 more, the VB bytes of column group gq
             uint32_t v[4][VB / 4];
 #pragma unroll
@@ -293,7 +345,7 @@ template <int DP, int DVP, bool SHARED> __global__ void __launch_bounds__(kFmThr
                                 const uint32_t at = vd - smem + r * DVP + (VB == 16 ? 16 * (grp ^ (r & 7)) : 16 * ((grp >> 1) ^ ((r >> 1) & 3)) + 8 * (grp & 1)) + n;
                                 const bool bad = (fm_smem_raw[at] & 0x7f) == 0x7f;
                                 if (bad && seeA) O[n][c] = NAN;
-                                if (bad && seeB) O[n][2 + c] = NAN;
+                                if (TWO && bad && seeB) O[n][2 + c] = NAN;
                             }
                         }
                     }
@@ -344,7 +396,7 @@ template <int DP, int DVP, bool SHARED> __global__ void __launch_bounds__(kFmThr
         constexpr int LD = DVP + 4;
 #pragma unroll
         for (int r = 0; r < 2; r++) {
-            if (r && !two) break;
+            if (r && !TWO) break;
             float* o = join + ((long)warp * 16 + gq + 8 * r) * LD;
             if (tq == 0) { o[0] = r ? mB : mA; o[1] = r ? lB : lA; }
 #pragma unroll
@@ -368,7 +420,7 @@ template <int DP, int DVP, bool SHARED> __global__ void __launch_bounds__(kFmThr
                 l = fmaf(wgt[w], join[(w * 16 + r) * LD + 1], l);
             }
             const long row = (long)(tok0 + tok) * a.H + h;
-            float* part = a.partial ? a.partial + (row * a.splits + blockIdx.z) * (dv + 2) : nullptr;
+            float* part = cut ? a.partial + (row * a.parts + blockIdx.z) * (dv + 2) : nullptr;
             float inv = 1.f;
             if (part) {
                 if ((tid & 7) == 0) { part[0] = m; part[1] = l; }
@@ -412,7 +464,7 @@ template <int DP, int DVP, bool SHARED> __global__ void __launch_bounds__(kFmThr
         const int tok = r ? tokB : tokA, h = r ? hB : hA;
         float m = r ? mB : mA, l = r ? lB : lA, k = 1.f;
         const long row = (long)(tok0 + tok) * a.H + h;
-        float* part = a.partial ? a.partial + (row * a.splits + blockIdx.z) * (dv + 2) : nullptr;
+        float* part = cut ? a.partial + (row * a.parts + blockIdx.z) * (dv + 2) : nullptr;
         if (part) {
             if (tq == 0) { part[0] = m; part[1] = l; }
         } else {
@@ -452,20 +504,27 @@ static bool fm_takes(const ktb200_fp8_attn_params* c, int dtype) {
     return dtype == KTB200_TYPE_BF16 && c->dim % 16 == 0 && c->vdim % 16 == 0 && c->dim <= 128 && c->vdim <= 128 &&
            ((reinterpret_cast<uintptr_t>(c->q) | reinterpret_cast<uintptr_t>(c->k_codes) | reinterpret_cast<uintptr_t>(c->v_codes)) & 15) == 0 && (reinterpret_cast<uintptr_t>(c->scales) & 7) == 0;
 }
-// portions whose tokens fill more than two warps' rows share their key tiles
-static bool fm_shared(const ktb200_fp8_attn_params* c, int n_tokens) { return (long)n_tokens > 2L * c->n_seqs * (16 / fm_heads(c->heads / c->kv_heads)); }
-static long fm_tiles(const ktb200_fp8_attn_params* c, int n_tokens) {
-    const int toks = (fm_shared(c, n_tokens) ? kFmWarps : 1) * (16 / fm_heads(c->heads / c->kv_heads));
-    return std::min<long>(n_tokens, c->n_seqs + (long)n_tokens / toks);
+// Which form: 64 rows that share key tiles where portions have more tokens than two 16-row tiles take; else 8 rows a tile where those hold a portion's tokens, 16 where not
+struct FmForm { int RH, toks; bool shared, two; };
+static FmForm fm_form(const ktb200_fp8_attn_params* c, int n_tokens) {
+    FmForm f;
+    f.RH = fm_heads(c->heads / c->kv_heads);
+    f.shared = (long)n_tokens > 2L * c->n_seqs * (16 / f.RH);
+    f.two = f.shared || f.RH > 8 || (long)n_tokens > (long)c->n_seqs * (8 / f.RH);
+    f.toks = (f.shared ? kFmWarps : 1) * ((f.two ? 16 : 8) / f.RH);
+    return f;
 }
-template <int DP, int DVP, bool SHARED> static cudaError_t fm_launch_as(const Fp8Attn& a, int RH, dim3 grid, cudaStream_t s) {
+template <int DP, int DVP, bool SHARED, bool TWO> static cudaError_t fm_launch_as(const Fp8Attn& a, int RH, dim3 grid, cudaStream_t s) {
     constexpr int smem = fm_smem<DP, DVP, SHARED>();
-    const cudaError_t e = raise_smem_limit((const void*)fp8_attn_mma_kernel<DP, DVP, SHARED>, smem);
-    return e != cudaSuccess ? e : launch_pdl(fp8_attn_mma_kernel<DP, DVP, SHARED>, grid, dim3(kFmThreads), (size_t)smem, s, a, RH);
+    const cudaError_t e = raise_smem_limit((const void*)fp8_attn_mma_kernel<DP, DVP, SHARED, TWO>, smem);
+    return e != cudaSuccess ? e : launch_pdl(fp8_attn_mma_kernel<DP, DVP, SHARED, TWO>, grid, dim3(kFmThreads), (size_t)smem, s, a, RH);
 }
-template <bool SHARED> static cudaError_t fm_launch(const Fp8Attn& a, int RH, dim3 grid, cudaStream_t s) {
-    if (a.d <= 64) return a.dv <= 64 ? fm_launch_as<64, 64, SHARED>(a, RH, grid, s) : fm_launch_as<64, 128, SHARED>(a, RH, grid, s);
-    return a.dv <= 64 ? fm_launch_as<128, 64, SHARED>(a, RH, grid, s) : fm_launch_as<128, 128, SHARED>(a, RH, grid, s);
+template <bool SHARED, bool TWO> static cudaError_t fm_launch_of(const Fp8Attn& a, int RH, dim3 grid, cudaStream_t s) {
+    if (a.d <= 64) return a.dv <= 64 ? fm_launch_as<64, 64, SHARED, TWO>(a, RH, grid, s) : fm_launch_as<64, 128, SHARED, TWO>(a, RH, grid, s);
+    return a.dv <= 64 ? fm_launch_as<128, 64, SHARED, TWO>(a, RH, grid, s) : fm_launch_as<128, 128, SHARED, TWO>(a, RH, grid, s);
+}
+static cudaError_t fm_launch(const Fp8Attn& a, const FmForm& f, dim3 grid, cudaStream_t s) {
+    return f.shared ? fm_launch_of<true, true>(a, f.RH, grid, s) : f.two ? fm_launch_of<false, true>(a, f.RH, grid, s) : fm_launch_of<false, false>(a, f.RH, grid, s);
 }
 
 }  // namespace ktb

@@ -587,9 +587,11 @@ def fp8_cache_attention(q: torch.Tensor, kv, batch, cache, heads: int, kv_heads:
                              batch.n_seqs, table.data_ptr(), table.shape[0], table.shape[1], cache.page_size, kv.k.shape[0], kv.k.data_ptr(), kv.v.data_ptr(), kv.scales.data_ptr(),
                              out.data_ptr(), out.stride(0))
     with device_of(dev):
-        splits = lib.ktb200_fp8_cache_attn_splits(C.byref(a), T, batch.max_kv, code, int(tensor_cores))
-        ws = torch.empty(lib.ktb200_fp8_cache_attn_workspace(T, heads, vdim, splits) // 4, dtype=torch.float32, device=dev) if splits > 1 else None
-        native.check_seq(lib.ktb200_fp8_cache_attn(C.byref(a), T, splits, ws.data_ptr() if ws is not None else None, code, int(tensor_cores), st))
+        ref, tc, n_keys = C.byref(a), int(tensor_cores), batch.max_kv
+        part = lib.ktb200_fp8_cache_attn_part(ref, T, n_keys, code, tc)
+        nbytes = lib.ktb200_fp8_cache_attn_workspace(ref, T, n_keys, part, code, tc) if part else 0
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+        native.check_seq(lib.ktb200_fp8_cache_attn(ref, T, n_keys, part, ws.data_ptr() if nbytes else None, nbytes, code, tc, st))
     return out
 
 

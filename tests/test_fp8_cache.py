@@ -85,18 +85,34 @@ def test_append_refuses_types_and_takes_no_tokens():
     assert lib.ktb200_fp8_cache_append(C.byref(a), 0, native.GGML_BF16, None) == native.OK
 
 
-@pytest.mark.parametrize("bad,splits", [(dict(kv_heads=3), 1), (dict(dim=257), 1), (dict(vdim=0), 1), (dict(page_size=0), 1), (dict(window=-1), 1), (dict(chunk=-4), 1), (dict(out_stride=127), 1),
-                                        (dict(q=None), 1), (dict(out=None), 1), (dict(scales=None), 1), ({}, 0), ({}, 129), ({}, 2)])
-def test_attention_refuses(bad, splits):
+@pytest.mark.parametrize("bad,call", [(dict(kv_heads=3), {}), (dict(dim=257), {}), (dict(vdim=0), {}), (dict(page_size=0), {}), (dict(window=-1), {}), (dict(chunk=-4), {}), (dict(out_stride=127), {}),
+                                      (dict(q=None), {}), (dict(out=None), {}), (dict(scales=None), {}), ({}, dict(part=-64)), ({}, dict(part=100)), ({}, dict(max_keys=-1)),
+                                      ({}, dict(part=64, max_keys=64 * 129)), ({}, dict(part=64, max_keys=1000)), ({}, dict(part=64, max_keys=1000, ws=16, n=100)), ({}, dict(dtype=native.GGML_F16))])
+def test_attention_refuses(bad, call):
     a = native.Fp8AttnParams(**{**ATTN_OK, **bad})
-    assert native.seq_lib().ktb200_fp8_cache_attn(C.byref(a), 1, splits, None, native.GGML_BF16, 1, None) == native.EINVAL
-    assert b"fp8_cache_attn" in native.seq_lib().ktb200_last_error()
+    lib, o = native.seq_lib(), {**dict(max_keys=32, part=0, ws=None, n=0, dtype=native.GGML_BF16), **call}
+    assert lib.ktb200_fp8_cache_attn(C.byref(a), 1, o["max_keys"], o["part"], o["ws"], o["n"], o["dtype"], 1, None) == native.EINVAL
+    assert b"fp8_cache_attn" in lib.ktb200_last_error()
 
 
 def test_attention_takes_no_tokens():
     lib, a = native.seq_lib(), native.Fp8AttnParams(**ATTN_OK)
-    assert lib.ktb200_fp8_cache_attn(C.byref(a), 0, 1, None, native.GGML_F32, 1, None) == native.OK
-    assert lib.ktb200_fp8_cache_attn(C.byref(a), 1, 1, None, native.GGML_F16, 1, None) == native.EINVAL
+    assert lib.ktb200_fp8_cache_attn(C.byref(a), 0, 32, 0, None, 0, native.GGML_F32, 1, None) == native.OK
+
+
+@pytest.mark.parametrize("dtype", [native.GGML_BF16, native.GGML_F32])
+@pytest.mark.parametrize("heads,kv_heads", [(64, 8), (16, 2), (7, 7), (17, 1), (64, 1)])
+@pytest.mark.parametrize("n_seqs,n_tokens", [(1, 1), (3, 3), (200, 200), (2, 50), (1, 3000)])
+def test_attention_parts_cover_any_range(n_seqs, n_tokens, heads, kv_heads, dtype):
+    lib = native.seq_lib()
+    for window, chunk in ((0, 0), (700, 0), (0, 4096)):
+        a = native.Fp8AttnParams(**{**ATTN_OK, **dict(heads=heads, kv_heads=kv_heads, n_seqs=n_seqs, window=window, chunk=chunk)})
+        for keys in (1, 300, 5000, 131072, 1 << 24, 2 ** 31 - 1):
+            part = lib.ktb200_fp8_cache_attn_part(C.byref(a), n_tokens, keys, dtype, 1)
+            need = lib.ktb200_fp8_cache_attn_workspace(C.byref(a), n_tokens, keys, part, dtype, 1)
+            assert part >= 0 and part % 64 == 0 and (need == 0) == (part == 0)
+            parts = need // (n_tokens * heads * 34 * 4)
+            assert parts <= 128 and (part == 0 or parts * part >= min([keys] + [x for x in (window, chunk) if x]))
 
 
 # ------------------------------------------------------------------------------------------------------------------------- append
