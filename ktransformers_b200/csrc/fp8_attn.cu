@@ -36,7 +36,7 @@ struct Fp8Attn {
     long out_stride;
     float* partial;      // [T][H][parts][dv + 2]: reference maximum, sum, un-normalised weighted values
     int part, parts;     // keys of a part (0: the range is not cut), and the most parts of a range
-    int ctoks;           // tokens of a CTA: their range, from the first visible key of the first of them (rounded down to 16) on, is what is cut
+    int ctoks, align;    // tokens of a CTA: their range, from the first visible key of the first of them (rounded down to align) on, is what is cut
 };
 __device__ __forceinline__ int fp8_first_visible(int p, int window, int chunk) {
     int lo = window > 0 ? max(0, p - window + 1) : 0;
@@ -89,7 +89,7 @@ template <typename T> __global__ void __launch_bounds__(256) fp8_attn_kernel(con
     float* Ks = qs + HB * d;
     float* Vs = Ks + kFgTile * (d + 1);
     float* pw = Vs + kFgTile * dv;
-    const int lo = fp8_first_visible(p, a.window, a.chunk), lo16 = lo & ~15;
+    const int lo = fp8_first_visible(p, a.window, a.chunk), lo16 = lo & ~(a.align - 1);
     const bool cut = a.part > 0 && p + 1 - lo16 > a.part;
     const int k_lo = max(lo, lo16 + (int)blockIdx.z * a.part), k_hi = cut ? min(p + 1, lo16 + (int)(blockIdx.z + 1) * a.part) : p + 1;
     if (blockIdx.z && (!cut || k_lo >= k_hi)) return;
@@ -180,7 +180,7 @@ template <typename T> __global__ void __launch_bounds__(128) fp8_merge_kernel(co
     for (int s = tid; s < a.n_seqs; s += 128) {
         const int len = fp8_portion(a, s), i = t - a.seqs[s];
         if (i >= 0 && i < len) {
-            const int i0 = i / a.ctoks * a.ctoks, p0 = a.pos[a.seqs[s]] + i0, lo16 = fp8_first_visible(p0, a.window, a.chunk) & ~15, n = p0 + min(a.ctoks, len - i0) - lo16;
+            const int i0 = i / a.ctoks * a.ctoks, p0 = a.pos[a.seqs[s]] + i0, lo16 = fp8_first_visible(p0, a.window, a.chunk) & ~(a.align - 1), n = p0 + min(a.ctoks, len - i0) - lo16;
             if (n > a.part) count = (n + a.part - 1) / a.part;
         }
     }
@@ -215,38 +215,53 @@ template <typename T> __global__ void __launch_bounds__(128) fp8_merge_kernel(co
 
 }  // namespace ktb
 #include "fp8_attn_mma.cuh"
+#include "fp8_attn_tc.cuh"
 
 using namespace ktb;
 
-// the most keys that a CTA's tokens see together, from a multiple of 16 on
-static long fp8_range(const ktb200_fp8_attn_params* c, int max_keys, int ctoks) {
-    long n = max_keys;
-    if (c->window > 0) n = std::min<long>(n, (long)c->window + ctoks);
-    if (c->chunk > 0) n = std::min<long>(n, (long)c->chunk + ctoks);
-    return n + 16;
+// Which kernel a call takes, the tokens and query heads of its CTAs, how far a range's start is rounded down, and the CTAs that an SM has places for
+struct Fp8Form {
+    enum { kCuda, kMma, kDecode } kernel;
+    FmForm mma;
+    int ctoks, heads, align, places;
+};
+static Fp8Form fp8_form(const ktb200_fp8_attn_params* c, int n_tokens, int dtype, int allow_tensor_cores) {
+    const int R = c->heads / c->kv_heads;
+    if (allow_tensor_cores && fd_takes(c, n_tokens, dtype)) return {Fp8Form::kDecode, {}, 1, fm_heads(R), kFdAlign, 2};
+    if (allow_tensor_cores && fm_takes(c, dtype)) {
+        const FmForm f = fm_form(c, n_tokens);
+        return {Fp8Form::kMma, f, f.toks, f.RH, kFmKeys, 3};
+    }
+    return {Fp8Form::kCuda, {}, 1, std::min(R, 8), 16, 3};
 }
-static int fp8_ctoks(const ktb200_fp8_attn_params* c, int n_tokens, int dtype, int allow_tensor_cores) { return allow_tensor_cores && fm_takes(c, dtype) ? fm_form(c, n_tokens).toks : 1; }
+// the most keys that a CTA's tokens see together, from a multiple of the alignment on
+static long fp8_range(const ktb200_fp8_attn_params* c, int max_keys, const Fp8Form& f) {
+    long n = max_keys;
+    if (c->window > 0) n = std::min<long>(n, (long)c->window + f.ctoks);
+    if (c->chunk > 0) n = std::min<long>(n, (long)c->chunk + f.ctoks);
+    return n + f.align;
+}
 static long fp8_tiles(const ktb200_fp8_attn_params* c, int n_tokens, int ctoks) { return std::min<long>(n_tokens, (long)c->n_seqs + n_tokens / ctoks); }
 static bool fp8_sizes_ok(const ktb200_fp8_attn_params* c) { return c && c->heads > 0 && c->kv_heads > 0 && c->heads % c->kv_heads == 0; }
 
 extern "C" size_t ktb200_fp8_cache_attn_workspace(const ktb200_fp8_attn_params* c, int n_tokens, int max_keys, int part, int dtype, int allow_tensor_cores) {
     if (!fp8_sizes_ok(c) || n_tokens <= 0 || part <= 0) return 0;
-    const long parts = (fp8_range(c, max_keys, fp8_ctoks(c, n_tokens, dtype, allow_tensor_cores)) + part - 1) / part;
+    const long parts = (fp8_range(c, max_keys, fp8_form(c, n_tokens, dtype, allow_tensor_cores)) + part - 1) / part;
     return parts > 1 ? (size_t)n_tokens * c->heads * parts * (c->vdim + 2) * sizeof(float) : 0;
 }
 
-// Keys of a part: the whole range where the CTAs of uncut ranges fill the SMs' places (three an SM) four times; else so many that one round of CTAs covers the range, and
+// Keys of a part: the whole range where the CTAs of uncut ranges fill the SMs' places four times; else so many that one round of CTAs covers the range, and
 // between sequences, whose ranges may have any length, no more than 1024
 extern "C" int ktb200_fp8_cache_attn_part(const ktb200_fp8_attn_params* c, int n_tokens, int max_keys, int dtype, int allow_tensor_cores) {
     if (!fp8_sizes_ok(c) || n_tokens <= 0) return 0;
-    const int R = c->heads / c->kv_heads, ctoks = fp8_ctoks(c, n_tokens, dtype, allow_tensor_cores);
-    const long tiles = fp8_tiles(c, n_tokens, ctoks), range = fp8_range(c, max_keys, ctoks), places = 3 * 148;
-    const long ctas = tiles * c->kv_heads * (ctoks == 1 && !(allow_tensor_cores && fm_takes(c, dtype)) ? (R + 7) / 8 : R / fm_heads(R));
+    const Fp8Form f = fp8_form(c, n_tokens, dtype, allow_tensor_cores);
+    const int R = c->heads / c->kv_heads;
+    const long range = fp8_range(c, max_keys, f), places = f.places * 148, ctas = fp8_tiles(c, n_tokens, f.ctoks) * c->kv_heads * ((R + f.heads - 1) / f.heads);
     if (ctas >= 4 * places || range <= 2 * kFp8MinPart) return 0;
     long part = (range * ctas + places - 1) / places;
     if (c->n_seqs > 1) part = std::min<long>(part, 1024);
     part = std::max<long>({part, kFp8MinPart, (range + kFp8MaxParts - 1) / kFp8MaxParts});
-    part = (part + 63) / 64 * 64;
+    part = (part + 127) / 128 * 128;
     return part < range ? (int)part : 0;
 }
 
@@ -258,33 +273,37 @@ extern "C" int ktb200_fp8_cache_attn(const ktb200_fp8_attn_params* c, int n_toke
         return KTB200_EINVAL;
     }
     if (dtype != KTB200_TYPE_BF16 && dtype != KTB200_TYPE_F32) { set_error("fp8_cache_attn: dtype must be bf16 or f32"); return KTB200_EINVAL; }
-    if (part < 0 || part % 64 || max_keys < 0) { set_error("fp8_cache_attn: part %d (a multiple of 64 or 0), max_keys %d", part, max_keys); return KTB200_EINVAL; }
+    if (part < 0 || part % 128 || max_keys < 0) { set_error("fp8_cache_attn: part %d (a multiple of 128 or 0), max_keys %d", part, max_keys); return KTB200_EINVAL; }
     if (n_tokens <= 0 || c->n_seqs == 0) return KTB200_OK;
     if (!c->q || !c->pos || !c->slot || !c->seqs || !c->page_table || !c->k_codes || !c->v_codes || !c->scales || !c->out) { set_error("fp8_cache_attn: null pointer"); return KTB200_EINVAL; }
-    const bool bf16 = dtype == KTB200_TYPE_BF16, tiles = allow_tensor_cores && fm_takes(c, dtype);
-    const int R = c->heads / c->kv_heads, ctoks = fp8_ctoks(c, n_tokens, dtype, allow_tensor_cores);
-    const long parts = part ? (fp8_range(c, max_keys, ctoks) + part - 1) / part : 1;
+    const bool bf16 = dtype == KTB200_TYPE_BF16;
+    const int R = c->heads / c->kv_heads;
+    const Fp8Form f = fp8_form(c, n_tokens, dtype, allow_tensor_cores);
+    const long parts = part ? (fp8_range(c, max_keys, f) + part - 1) / part : 1;
     if (parts > kFp8MaxParts) { set_error("fp8_cache_attn: %ld parts, at most %d", parts, kFp8MaxParts); return KTB200_EINVAL; }
     const size_t need = ktb200_fp8_cache_attn_workspace(c, n_tokens, max_keys, part, dtype, allow_tensor_cores);
     if (need && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 7))) { set_error("fp8_cache_attn: workspace missing, too small or not aligned"); return KTB200_EINVAL; }
-    const int HB = std::min(R, 8), hblocks = (R + HB - 1) / HB;
     if ((long)c->kv_heads * R > 65535 || (long)n_tokens * c->heads > 0x7fffffffL) { set_error("fp8_cache_attn: too many heads or tokens"); return KTB200_EINVAL; }
     const cudaStream_t s = (cudaStream_t)stream;
     const Fp8Attn a{c->q, c->heads, c->kv_heads, c->dim, c->vdim, c->scale, c->head_scale, c->softcap, c->window, c->chunk, c->sink, c->out_scale, c->pos, c->slot, c->seqs, c->seqs_stride,
                     c->n_seqs, n_tokens, {c->page_table, c->n_slots, c->max_pages, c->page_size, c->n_pages}, (const uint8_t*)c->k_codes, (const uint8_t*)c->v_codes, c->scales, c->out,
-                    c->out_stride, workspace, parts > 1 ? part : 0, (int)parts, ctoks};
-    const unsigned nt = (unsigned)fp8_tiles(c, n_tokens, ctoks);
-    if (tiles) {
-        const FmForm f = fm_form(c, n_tokens);
-        KTB_CUDA_CHECK(fm_launch(a, f, dim3(nt, c->kv_heads * (R / f.RH), (unsigned)parts), s));
+                    c->out_stride, workspace, parts > 1 ? part : 0, (int)parts, f.ctoks, f.align};
+    const dim3 grid((unsigned)fp8_tiles(c, n_tokens, f.ctoks), c->kv_heads * ((R + f.heads - 1) / f.heads), (unsigned)parts);
+    if (f.kernel == Fp8Form::kDecode) {
+        const int rc = fd_launch(a, f.heads, grid, s);
+        if (rc) return rc;
+    } else if (f.kernel == Fp8Form::kMma) {
+        KTB_CUDA_CHECK(fm_launch(a, f.mma, grid, s));
     } else {
+        const int HB = f.heads;
         const size_t smem = ((size_t)HB * c->dim + (size_t)kFgTile * (c->dim + 1) + (size_t)kFgTile * c->vdim + (size_t)HB * kFgTile) * sizeof(float);
         KTB_CUDA_CHECK(raise_smem_limit(bf16 ? (const void*)fp8_attn_kernel<__nv_bfloat16> : (const void*)fp8_attn_kernel<float>, smem));
-        KTB_CUDA_CHECK(launch_pdl(bf16 ? fp8_attn_kernel<__nv_bfloat16> : fp8_attn_kernel<float>, dim3(nt, c->kv_heads * hblocks, (unsigned)parts), dim3(HB * 32), smem, s, a));
+        KTB_CUDA_CHECK(launch_pdl(bf16 ? fp8_attn_kernel<__nv_bfloat16> : fp8_attn_kernel<float>, grid, dim3(HB * 32), smem, s, a));
     }
     count_launch();
     if (parts > 1) {
-        KTB_CUDA_CHECK(launch_pdl(bf16 ? fp8_merge_kernel<__nv_bfloat16> : fp8_merge_kernel<float>, dim3((unsigned)((long)n_tokens * c->heads)), dim3(128), (size_t)0, s, a, tiles ? 1.0f : kLog2e));
+        KTB_CUDA_CHECK(launch_pdl(bf16 ? fp8_merge_kernel<__nv_bfloat16> : fp8_merge_kernel<float>, dim3((unsigned)((long)n_tokens * c->heads)), dim3(128), (size_t)0, s, a,
+                                  f.kernel == Fp8Form::kCuda ? kLog2e : 1.0f));
         count_launch();
     }
     return KTB200_OK;

@@ -1,0 +1,327 @@
+// Attention of single tokens over the paged e4m3 cache on tcgen05 (bf16 queries, heads of 128, up to 16 query heads per key/value head, pages of whole 16 tokens): the decode step.
+//
+// A CTA has one token, one key/value head and its query heads, and a part of the key range in tiles of 128 keys.  The codes are operands as they lie in the cache: nothing is converted.
+//     S^T = K Q^T     128 keys x N, kind::f8f6f4, K the K-major A operand as TMA delivered it
+//     O^T = V^T P^T   128 columns x N, the V tile as an MN-major A operand
+// N = 2 RP columns for RP = 8 or 16 heads: what stands against the codes is split into two e4m3 numbers, the second for 16 times what the first leaves.
+//   queries   a row moved by a power of two so that its largest stands in [128, 256): exact for bf16 numbers down to 2^-13 of that largest, 2^-21 of it off below
+//   weights   p = 2^(t - m), t = s log2(e) + log2(value scale): 2^-8 of a weight off at most (as a bf16 weight is) and 2^-21 of the largest where that is more.  Value scales are
+//             powers of two: in the exponent they cost nothing and O needs none.  m is 7 below a head's largest t, raised when a t outgrows it by 8.75 (2^8.75 < 448)
+// l += p / (value scale), O / l is the result: 2^m drops out.
+//     warp 0      TMA: K and V tiles, three stages; a tile is runs of 16, 32 or 64 keys, each inside one page (runs that no key of the part lies in come as zeros)
+//     warp 1      MMAs: S of the next tile ahead of PV of this one
+//     warps 2-5   a thread owns a key: its scores of all heads are one row of S^T, so that scales and masks are its own; maxima are only needed when one has outgrown its
+//                 reference, which one barrier with a reduction tells.  At the end a thread owns a column of the result
+// TMEM: [S | S | O], N columns each.  Bound by the cache's bytes: a tile is 32 KB, 740 ns of an SM's share of the memory; two CTAs an SM.
+#pragma once
+#include <cuda.h>
+
+#include "umma.cuh"
+
+namespace ktb {
+
+constexpr int kFdThreads = 192, kFdKeys = 128, kFdTile = kFdKeys * 128, kFdStages = 3, kFdAlign = 64;
+constexpr float kFdTop = 7.f, kFdRaise = 8.75f;
+struct FdMisc {
+    unsigned long long k_full[kFdStages], k_free[kFdStages], v_full[kFdStages], v_free[kFdStages], s_full[2], s_free[2], p_full[2], p_free[2], q_ready;
+    float red[4][16], fac[16];
+    uint32_t tmem_base;
+    int info[4];
+};
+template <int RP> constexpr int fd_smem() { return 2 * kFdStages * kFdTile + 3 * 2 * RP * 128 + (int)sizeof(FdMisc) + 1024; }
+
+struct FdMaps { CUtensorMap k, v; };
+
+// Where the byte of key (column) c of row n of a K-major operand with 128-byte rows and 128-byte swizzle lies
+__device__ __forceinline__ uint32_t fd_at(int n, int c) { return (uint32_t)((n >> 3) * 1024 + (n & 7) * 128 + ((((c >> 4) ^ n) & 7) << 4) + (c & 15)); }
+__device__ __forceinline__ bool fd_any(bool p) {      // over the four soft-max warps
+    uint32_t r;
+    asm volatile("{\n.reg .pred a, b;\nsetp.ne.u32 a, %1, 0;\nbarrier.cta.red.or.pred b, 1, 128, a;\nselp.u32 %0, 1, 0, b;\n}" : "=r"(r) : "r"((uint32_t)p) : "memory");
+    return r != 0;
+}
+__device__ __forceinline__ void fd_sync() { asm volatile("barrier.cta.sync 1, 128;" ::: "memory"); }
+
+template <int RP> __global__ void __launch_bounds__(kFdThreads, 2) fp8_attn_decode_kernel(const __grid_constant__ FdMaps maps, const Fp8Attn a, int RH, int run) {
+    using namespace umma;
+    constexpr int N = 2 * RP, OP = N * 128;      // bytes of an operand of N rows
+    extern __shared__ __align__(16) uint8_t fd_smem_raw[];
+    const uint32_t raw = smem_u32(fd_smem_raw), base = (raw + 1023u) & ~1023u;
+    uint8_t* smem = fd_smem_raw + (base - raw);
+    const uint32_t kbase = base, vbase = base + kFdStages * kFdTile, qbase = base + 2 * kFdStages * kFdTile, pbase = qbase + OP;
+    FdMisc& misc = *reinterpret_cast<FdMisc*>(smem + 2 * kFdStages * kFdTile + 3 * OP);
+    const int tid = threadIdx.x, lane = tid & 31, warp = uniform(tid >> 5), ps = a.pages.page_size;
+    griddep_launch_dependents();
+    if (tid == 0) {
+        for (int i = 0; i < kFdStages; i++) { bar_init(smem_u32(&misc.k_full[i]), 1); bar_init(smem_u32(&misc.k_free[i]), 1); bar_init(smem_u32(&misc.v_full[i]), 1); bar_init(smem_u32(&misc.v_free[i]), 1); }
+        for (int i = 0; i < 2; i++) { bar_init(smem_u32(&misc.s_full[i]), 1); bar_init(smem_u32(&misc.s_free[i]), 4); bar_init(smem_u32(&misc.p_full[i]), 4); bar_init(smem_u32(&misc.p_free[i]), 1); }
+        bar_init(smem_u32(&misc.q_ready), 4);
+        bar_fence_init();
+        tma_prefetch_desc(&maps.k);
+        tma_prefetch_desc(&maps.v);
+    }
+    griddep_wait();
+    if (warp == 2) fp8_find_tokens(a, blockIdx.x, 1, misc.info);
+    __syncthreads();
+    const int t = misc.info[0], p = misc.info[2], slot = misc.info[3], R = a.H / a.G, hblocks = R / RH;
+    if (misc.info[1] <= 0) return;
+    const int g = blockIdx.y / hblocks, h0 = g * R + (blockIdx.y % hblocks) * RH;
+    const int lo = fp8_first_visible(p, a.window, a.chunk), lo_al = lo & ~(kFdAlign - 1);
+    const bool cut = a.part > 0 && p + 1 - lo_al > a.part;
+    const int k_lo = lo_al + blockIdx.z * a.part, k_hi = cut ? min(p + 1, k_lo + a.part) : p + 1;
+    if (k_lo >= k_hi) return;
+    const int tiles = (k_hi - k_lo + kFdKeys - 1) / kFdKeys;
+    if (warp == 1) tmem_alloc(smem_u32(&misc.tmem_base), 128);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = uniform(misc.tmem_base), tmem_o = tmem + 2 * N;
+    const bool slot_ok = (unsigned)slot < (unsigned)a.pages.slots;
+    const int* pt = a.pages.table + (slot_ok ? (long)slot * a.pages.max_pages : 0);
+    auto page_of = [&](int key) {      // -1: not there
+        const int page = pt[(key / ps) % a.pages.max_pages];
+        return (unsigned)page < (unsigned)a.pages.n_pages ? page : -1;
+    };
+
+    if (warp == 0) {
+        // ================================================================ copies
+        const int runs = kFdKeys / run, ahead = 32 / runs, none = a.pages.n_pages * a.G * ps;      // (rows from `none` on are outside the maps: zeros)
+        int row = none;
+        for (int j = 0; j < tiles; j++) {
+            if (j % ahead == 0) {      // a lane looks one run's page up, for as many tiles as the lanes reach
+                const int kp = k_lo + j * kFdKeys + lane * run, page = slot_ok && kp < k_hi && kp + run > lo ? page_of(kp) : -1;
+                row = page < 0 ? none : (page * a.G + g) * ps + kp % ps;
+            }
+            const int st = j % kFdStages, ph = ((j / kFdStages) & 1) ^ 1;
+            const uint32_t kf = smem_u32(&misc.k_full[st]), vf = smem_u32(&misc.v_full[st]);
+            if (lane == 0) {
+                bar_wait(smem_u32(&misc.k_free[st]), ph);
+                bar_expect_tx(kf, kFdTile);
+            }
+            for (int i = 0; i < runs; i++) {
+                const int r = __shfl_sync(0xffffffffu, row, (j % ahead) * runs + i);
+                if (lane == 0) tma_load_2d(kbase + st * kFdTile + i * run * 128, &maps.k, kf, 0, r);
+            }
+            if (lane == 0) {
+                bar_wait(smem_u32(&misc.v_free[st]), ph);
+                bar_expect_tx(vf, kFdTile);
+            }
+            for (int i = 0; i < runs; i++) {
+                const int r = __shfl_sync(0xffffffffu, row, (j % ahead) * runs + i);
+                if (lane == 0) tma_load_2d(vbase + st * kFdTile + i * run * 128, &maps.v, vf, 0, r);
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        // ================================================================ products (converged warp)
+        constexpr uint32_t idesc_s = instr_desc(1, 0, 0, 0, 0, 128, N), idesc_o = instr_desc(1, 0, 0, 1, 0, 128, N);
+        bar_wait(smem_u32(&misc.q_ready), 0);
+        for (int j = 0; j <= tiles; j++) {
+            if (j < tiles) {
+                const int st = j % kFdStages, buf = j & 1;
+                bar_wait(smem_u32(&misc.k_full[st]), (j / kFdStages) & 1);
+                bar_wait(smem_u32(&misc.s_free[buf]), ((j >> 1) & 1) ^ 1);
+                tc_fence_after();
+                mma_f8_x4(tmem + buf * N, smem_desc(kbase + st * kFdTile, 16, 1024, kLayoutSw128), smem_desc(qbase, 16, 1024, kLayoutSw128), idesc_s, 0, smem_u32(&misc.s_full[buf]),
+                          smem_u32(&misc.k_free[st]));
+            }
+            if (j > 0) {
+                const int i = j - 1, st = i % kFdStages, buf = i & 1;
+                bar_wait(smem_u32(&misc.v_full[st]), (i / kFdStages) & 1);
+                bar_wait(smem_u32(&misc.p_full[buf]), (i >> 1) & 1);
+                tc_fence_after();
+                // 32 keys a step: 32 rows of V, 32 bytes of P's rows
+                mma_f8_x4<256, 2>(tmem_o, smem_desc(vbase + st * kFdTile, 16, 1024, kLayoutSw128), smem_desc(pbase + buf * OP, 16, 1024, kLayoutSw128), idesc_o, i > 0, smem_u32(&misc.p_free[buf]),
+                                  smem_u32(&misc.v_free[st]));
+            }
+        }
+    } else {
+        // ================================================================ queries, soft-max, result
+        const int sp = warp & 3, r = 32 * sp + lane, w4 = warp - 2;
+        const uint32_t lanes = (uint32_t)(32 * sp) << 16;
+        {      // a warp a head: lane has columns 4 lane ..
+            for (int h = w4; h < RP; h += 4) {
+                float x[4] = {0.f, 0.f, 0.f, 0.f}, odd = 0.f;
+                if (h < RH) {
+                    const uint2 v = *reinterpret_cast<const uint2*>((const __nv_bfloat16*)a.q + ((long)t * a.H + h0 + h) * 128 + 4 * lane);
+                    x[0] = __uint_as_float(v.x << 16); x[1] = __uint_as_float(v.x & 0xffff0000u); x[2] = __uint_as_float(v.y << 16); x[3] = __uint_as_float(v.y & 0xffff0000u);
+                }
+                float top = 0.f;
+#pragma unroll
+                for (int i = 0; i < 4; i++) { top = fmaxf(top, fabsf(x[i])); odd = fmaf(x[i], 0.f, odd); }
+                top = warp_max(top);
+                odd = warp_sum(odd);      // NaN where a value is not finite (e4m3 has no infinity)
+                const int up = min(126, max(-120, 7 - ((int)(__float_as_uint(top) >> 23) - 127)));      // 2^(7 - e) of a largest 1.f 2^e, within what fp32 holds with its inverse
+                const float by = __uint_as_float((uint32_t)(up + 127) << 23);
+                const uint2 lo2 = split_e4m3(x[0] * by, x[1] * by), hi2 = split_e4m3(x[2] * by, x[3] * by);
+                *reinterpret_cast<uint32_t*>(smem + (qbase - base) + fd_at(h, 4 * lane)) = lo2.x | hi2.x << 16;
+                *reinterpret_cast<uint32_t*>(smem + (qbase - base) + fd_at(RP + h, 4 * lane)) = lo2.y | hi2.y << 16;
+                if (lane == 0) misc.fac[h] = h < RH ? (a.head_scale ? a.scale * a.head_scale[h0 + h] : a.scale) / by * (a.softcap > 0.f ? 1.f : kLog2e) + odd : 0.f;
+            }
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) bar_arrive(smem_u32(&misc.q_ready));
+            fd_sync();      // (the factors)
+        }
+        float fac[RP], m[RP], l[RP];
+#pragma unroll
+        for (int h = 0; h < RP; h++) { fac[h] = misc.fac[h]; m[h] = -INFINITY; l[h] = 0.f; }
+        const float two_over_cap = a.softcap > 0.f ? 2.0f / a.softcap : 0.f, cap = a.softcap * kLog2e;
+        // the scales of the thread's key, a tile ahead, and its page, two ahead
+        auto see = [&](int j) { const int key = k_lo + j * kFdKeys + r; return slot_ok && key >= lo && key < k_hi; };
+        auto look = [&](int j) { return see(j) ? page_of(k_lo + j * kFdKeys + r) : -1; };
+        auto scales_of = [&](int page) { return page < 0 ? make_float2(0.f, 0.f) : *reinterpret_cast<const float2*>(a.scales + 2 * ((long)page * a.G + g)); };
+        float2 sc = scales_of(look(0));
+        int page1 = look(1);
+        for (int j = 0; j < tiles; j++) {
+            const int buf = j & 1;
+            const float2 next = scales_of(page1);
+            page1 = look(j + 2);
+            const bool here = sc.y > 0.f;      // (scales of a key that is not seen are zero)
+            bar_wait(smem_u32(&misc.s_full[buf]), (j >> 1) & 1);
+            tc_fence_after();
+            uint32_t s[N];
+            if constexpr (N == 16) tmem_ld16(tmem + lanes + buf * N, s); else tmem_ld32(tmem + lanes + buf * N, s);
+            tmem_wait_ld();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) bar_arrive(smem_u32(&misc.s_free[buf]));
+            const float ve = (float)((int)(__float_as_uint(sc.y) >> 23) - 127), inv = here ? __uint_as_float((254u << 23) - __float_as_uint(sc.y)) : 0.f;
+            float x[RP];
+            bool up = false;
+#pragma unroll
+            for (int h = 0; h < RP; h++) x[h] = fmaf(__uint_as_float(s[RP + h]), 0.0625f, __uint_as_float(s[h])) * (fac[h] * sc.x);
+            if (a.softcap > 0.f) {
+#pragma unroll
+                for (int h = 0; h < RP; h++) x[h] = cap * (1.0f - __fdividef(2.0f, __expf(x[h] * two_over_cap) + 1.0f));      // c tanh(s / c): a few 1e-7 of the cap off
+            }
+#pragma unroll
+            for (int h = 0; h < RP; h++) {
+                x[h] = here ? x[h] + ve : -INFINITY;
+                up |= x[h] > m[h] + kFdRaise;
+            }
+            if (fd_any(up)) {      // (always in the first tile that has a key)
+#pragma unroll
+                for (int h = 0; h < RP; h++) {
+                    const float top = warp_max(x[h]);
+                    if (lane == 0) misc.red[w4][h] = top;
+                }
+                fd_sync();
+                float k[RP];
+#pragma unroll
+                for (int h = 0; h < RP; h++) {
+                    const float top = fmaxf(fmaxf(misc.red[0][h], misc.red[1][h]), fmaxf(misc.red[2][h], misc.red[3][h]));
+                    k[h] = 1.f;
+                    if (top > m[h] + kFdRaise) {
+                        k[h] = exp2_approx(m[h] - (top - kFdTop));      // (2^-inf = 0: nothing was summed yet)
+                        m[h] = top - kFdTop;
+                        l[h] *= k[h];
+                    }
+                }
+                if (j > 0) {
+                    bar_wait(smem_u32(&misc.p_free[buf ^ 1]), ((j - 1) >> 1) & 1);      // PV of the tile before this one is complete
+                    tc_fence_after();
+                    uint32_t o[N];
+                    if constexpr (N == 16) tmem_ld16(tmem_o + lanes, o); else tmem_ld32(tmem_o + lanes, o);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int h = 0; h < RP; h++) { o[h] = __float_as_uint(__uint_as_float(o[h]) * k[h]); o[RP + h] = __float_as_uint(__uint_as_float(o[RP + h]) * k[h]); }
+                    if constexpr (N == 16) tmem_st16(tmem_o + lanes, o); else tmem_st32(tmem_o + lanes, o);
+                    tmem_wait_st();
+                    tc_fence_before();
+                }
+            }
+            if (j > 1) bar_wait(smem_u32(&misc.p_free[buf]), ((j - 2) >> 1) & 1);
+            uint8_t* P = smem + (pbase - base) + buf * OP;
+#pragma unroll
+            for (int h = 0; h < RP; h += 2) {
+                const float u0 = m[h] == -INFINITY ? 0.f : m[h], u1 = m[h + 1] == -INFINITY ? 0.f : m[h + 1];
+                const float p0 = exp2_approx(x[h] - u0), p1 = exp2_approx(x[h + 1] - u1);
+                l[h] = fmaf(p0, inv, l[h]);
+                l[h + 1] = fmaf(p1, inv, l[h + 1]);
+                const uint2 c = split_e4m3(p0, p1);
+                P[fd_at(h, r)] = (uint8_t)c.x;
+                P[fd_at(h + 1, r)] = (uint8_t)(c.x >> 8);
+                P[fd_at(RP + h, r)] = (uint8_t)c.y;
+                P[fd_at(RP + h + 1, r)] = (uint8_t)(c.y >> 8);
+            }
+            const int k0 = k_lo + j * kFdKeys;
+            if (k0 < lo || k0 + kFdKeys > k_hi) {      // the first and last tiles: values of keys that are not seen may be anything (0 x NaN)
+                const int st = j % kFdStages;
+                bar_wait(smem_u32(&misc.v_full[st]), (j / kFdStages) & 1);
+                if (k0 + r < lo || k0 + r >= k_hi) {
+#pragma unroll
+                    for (int i = 0; i < 8; i++) *reinterpret_cast<uint4*>(smem + (vbase - base) + st * kFdTile + r * 128 + 16 * i) = make_uint4(0, 0, 0, 0);
+                }
+            }
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) bar_arrive(smem_u32(&misc.p_full[buf]));
+            sc = next;
+        }
+        // sums over the keys' threads (the last tile's maxima have been read by all)
+        fd_sync();
+#pragma unroll
+        for (int h = 0; h < RP; h++) {
+            const float sum = warp_sum(l[h]);
+            if (lane == 0) misc.red[w4][h] = sum;
+        }
+        bar_wait(smem_u32(&misc.p_free[(tiles - 1) & 1]), ((tiles - 1) >> 1) & 1);
+        tc_fence_after();
+        uint32_t o[N];
+        if constexpr (N == 16) tmem_ld16(tmem_o + lanes, o); else tmem_ld32(tmem_o + lanes, o);
+        tmem_wait_ld();
+        fd_sync();
+#pragma unroll
+        for (int h = 0; h < RP; h++) {
+            if (h >= RH) break;
+            float sum = (misc.red[0][h] + misc.red[1][h]) + (misc.red[2][h] + misc.red[3][h]), v = fmaf(__uint_as_float(o[RP + h]), 0.0625f, __uint_as_float(o[h]));
+            const long row = (long)t * a.H + h0 + h;
+            if (cut) {
+                float* part = a.partial + (row * a.parts + blockIdx.z) * 130;
+                if (r == 0) { part[0] = m[h]; part[1] = sum; }
+                part[2 + r] = v;
+            } else {
+                if (a.sink) {
+                    const float sk = a.sink[h0 + h] * kLog2e, mn = fmaxf(m[h], sk), k = m[h] == -INFINITY ? 0.f : exp2_approx(m[h] - mn);
+                    sum = sum * k + exp2_approx(sk - mn);
+                    v *= k;
+                }
+                v = sum > 0.f || sum != sum ? v * (a.out_scale / sum) : 0.f;
+                ((__nv_bfloat16*)a.out)[(long)t * a.out_stride + (long)(h0 + h) * 128 + r] = __float2bfloat16_rn(v);
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 128);
+    }
+}
+
+// heads of a group that one CTA takes: the largest divisor of the group up to 16
+static bool fd_takes(const ktb200_fp8_attn_params* c, int n_tokens, int dtype) {
+    return fm_takes(c, dtype) && c->dim == 128 && c->vdim == 128 && c->page_size % 16 == 0 && (long)n_tokens <= 2L * c->n_seqs && (long)c->n_pages * c->kv_heads * c->page_size < (1L << 31) &&
+           c->n_pages > 0;
+}
+template <int RP> static cudaError_t fd_launch_as(const FdMaps& maps, const Fp8Attn& a, int RH, int run, dim3 grid, cudaStream_t s) {
+    const cudaError_t e = raise_smem_limit((const void*)fp8_attn_decode_kernel<RP>, fd_smem<RP>());
+    return e != cudaSuccess ? e : launch_pdl(fp8_attn_decode_kernel<RP>, grid, dim3(kFdThreads), (size_t)fd_smem<RP>(), s, maps, a, RH, run);
+}
+static int fd_launch(const Fp8Attn& a, int RH, dim3 grid, cudaStream_t s) {
+    const umma::EncodeTiledFn enc = umma::encode_tiled();
+    if (!enc) { set_error("fp8_cache_attn: cuTensorMapEncodeTiled is not available from this driver"); return KTB200_ECUDA; }
+    const int ps = a.pages.page_size, run = ps % 64 == 0 ? 64 : ps % 32 == 0 ? 32 : 16;
+    const cuuint64_t dims[2] = {128, (cuuint64_t)a.pages.n_pages * a.G * ps}, strides[1] = {128};
+    const cuuint32_t box[2] = {128, (cuuint32_t)run}, estr[2] = {1, 1};
+    FdMaps maps;
+    for (int i = 0; i < 2; i++) {
+        const CUresult cr = enc(i ? &maps.v : &maps.k, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t*>(i ? a.v_codes : a.k_codes), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+        if (cr != CUDA_SUCCESS) { set_error("fp8_cache_attn: cuTensorMapEncodeTiled failed (%d)", (int)cr); return KTB200_ECUDA; }
+    }
+    KTB_CUDA_CHECK(RH <= 8 ? fd_launch_as<8>(maps, a, RH, run, grid, s) : fd_launch_as<16>(maps, a, RH, run, grid, s));
+    return KTB200_OK;
+}
+
+}  // namespace ktb

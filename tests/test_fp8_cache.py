@@ -87,7 +87,7 @@ def test_append_refuses_types_and_takes_no_tokens():
 
 @pytest.mark.parametrize("bad,call", [(dict(kv_heads=3), {}), (dict(dim=257), {}), (dict(vdim=0), {}), (dict(page_size=0), {}), (dict(window=-1), {}), (dict(chunk=-4), {}), (dict(out_stride=127), {}),
                                       (dict(q=None), {}), (dict(out=None), {}), (dict(scales=None), {}), ({}, dict(part=-64)), ({}, dict(part=100)), ({}, dict(max_keys=-1)),
-                                      ({}, dict(part=64, max_keys=64 * 129)), ({}, dict(part=64, max_keys=1000)), ({}, dict(part=64, max_keys=1000, ws=16, n=100)), ({}, dict(dtype=native.GGML_F16))])
+                                      ({}, dict(part=128, max_keys=128 * 129)), ({}, dict(part=128, max_keys=1000)), ({}, dict(part=128, max_keys=1000, ws=16, n=100)), ({}, dict(dtype=native.GGML_F16))])
 def test_attention_refuses(bad, call):
     a = native.Fp8AttnParams(**{**ATTN_OK, **bad})
     lib, o = native.seq_lib(), {**dict(max_keys=32, part=0, ws=None, n=0, dtype=native.GGML_BF16), **call}
@@ -110,7 +110,7 @@ def test_attention_parts_cover_any_range(n_seqs, n_tokens, heads, kv_heads, dtyp
         for keys in (1, 300, 5000, 131072, 1 << 24, 2 ** 31 - 1):
             part = lib.ktb200_fp8_cache_attn_part(C.byref(a), n_tokens, keys, dtype, 1)
             need = lib.ktb200_fp8_cache_attn_workspace(C.byref(a), n_tokens, keys, part, dtype, 1)
-            assert part >= 0 and part % 64 == 0 and (need == 0) == (part == 0)
+            assert part >= 0 and part % 128 == 0 and (need == 0) == (part == 0)
             parts = need // (n_tokens * heads * 34 * 4)
             assert parts <= 128 and (part == 0 or parts * part >= min([keys] + [x for x in (window, chunk) if x]))
 
