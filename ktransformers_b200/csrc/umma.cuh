@@ -292,6 +292,9 @@ template <int DA = 2, int DB = 2, int DD = 0>
 __device__ __forceinline__ void mma_f8_x4(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate, uint32_t bar0 = 0, uint32_t bar1 = 0) { KTB_MMA_SS4("f8f6f4"); }
 template <int DA = 2, int DB = 2, int DD = 0>
 __device__ __forceinline__ void mma_f16_x4(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate, uint32_t bar0 = 0, uint32_t bar1 = 0) { KTB_MMA_SS4("f16"); }
+// 8-bit integers, 32-bit integer sums: K = 32 per product
+template <int DA = 2, int DB = 2, int DD = 0>
+__device__ __forceinline__ void mma_i8_x4(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate, uint32_t bar0 = 0, uint32_t bar1 = 0) { KTB_MMA_SS4("i8"); }
 #undef KTB_MMA_SS4
 
 }  // namespace umma
