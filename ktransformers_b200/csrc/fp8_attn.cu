@@ -216,18 +216,20 @@ template <typename T> __global__ void __launch_bounds__(128) fp8_merge_kernel(co
 }  // namespace ktb
 #include "fp8_attn_mma.cuh"
 #include "fp8_attn_tc.cuh"
+#include "fp8_attn_prompt.cuh"
 
 using namespace ktb;
 
 // Which kernel a call takes, the tokens and query heads of its CTAs, how far a range's start is rounded down, and the CTAs that an SM has places for
 struct Fp8Form {
-    enum { kCuda, kMma, kDecode } kernel;
+    enum { kCuda, kMma, kDecode, kPrompt } kernel;
     FmForm mma;
     int ctoks, heads, align, places;
 };
 static Fp8Form fp8_form(const ktb200_fp8_attn_params* c, int n_tokens, int dtype, int allow_tensor_cores) {
     const int R = c->heads / c->kv_heads;
     if (allow_tensor_cores && fd_takes(c, n_tokens, dtype)) return {Fp8Form::kDecode, {}, 1, fm_heads(R), kFdAlign, 2};
+    if (allow_tensor_cores && fp_takes(c, n_tokens, dtype)) return {Fp8Form::kPrompt, {}, 2 * (128 / fm_heads(R)), fm_heads(R), kFpKeys, 1};
     if (allow_tensor_cores && fm_takes(c, dtype)) {
         const FmForm f = fm_form(c, n_tokens);
         return {Fp8Form::kMma, f, f.toks, f.RH, kFmKeys, 3};
@@ -251,7 +253,7 @@ extern "C" size_t ktb200_fp8_cache_attn_workspace(const ktb200_fp8_attn_params* 
 }
 
 // Keys of a part: the whole range where the CTAs of uncut ranges fill the SMs' places four times; else so many that one round of CTAs covers the range, and
-// between sequences, whose ranges may have any length, no more than 1024
+// between sequences that decode, whose ranges may have any length, no more than 1024
 extern "C" int ktb200_fp8_cache_attn_part(const ktb200_fp8_attn_params* c, int n_tokens, int max_keys, int dtype, int allow_tensor_cores) {
     if (!fp8_sizes_ok(c) || n_tokens <= 0) return 0;
     const Fp8Form f = fp8_form(c, n_tokens, dtype, allow_tensor_cores);
@@ -259,7 +261,7 @@ extern "C" int ktb200_fp8_cache_attn_part(const ktb200_fp8_attn_params* c, int n
     const long range = fp8_range(c, max_keys, f), places = f.places * 148, ctas = fp8_tiles(c, n_tokens, f.ctoks) * c->kv_heads * ((R + f.heads - 1) / f.heads);
     if (ctas >= 4 * places || range <= 2 * kFp8MinPart) return 0;
     long part = (range * ctas + places - 1) / places;
-    if (c->n_seqs > 1) part = std::min<long>(part, 1024);
+    if (c->n_seqs > 1 && f.kernel != Fp8Form::kPrompt) part = std::min<long>(part, 1024);
     part = std::max<long>({part, kFp8MinPart, (range + kFp8MaxParts - 1) / kFp8MaxParts});
     part = (part + 127) / 128 * 128;
     return part < range ? (int)part : 0;
@@ -291,6 +293,9 @@ extern "C" int ktb200_fp8_cache_attn(const ktb200_fp8_attn_params* c, int n_toke
     const dim3 grid((unsigned)fp8_tiles(c, n_tokens, f.ctoks), c->kv_heads * ((R + f.heads - 1) / f.heads), (unsigned)parts);
     if (f.kernel == Fp8Form::kDecode) {
         const int rc = fd_launch(a, f.heads, grid, s);
+        if (rc) return rc;
+    } else if (f.kernel == Fp8Form::kPrompt) {
+        const int rc = fp_launch(a, f.heads, grid, s);
         if (rc) return rc;
     } else if (f.kernel == Fp8Form::kMma) {
         KTB_CUDA_CHECK(fm_launch(a, f.mma, grid, s));

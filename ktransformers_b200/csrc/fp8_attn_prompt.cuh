@@ -1,0 +1,410 @@
+// Attention of prompt portions over the paged e4m3 cache on tcgen05 (bf16 queries, heads of 128, pages of whole 64 tokens).
+//
+// A CTA owns 256 rows = (token, query head) pairs of one sequence portion and one key/value head as two tiles of 128 (RH heads of 128 / RH consecutive tokens each); keys run in
+// tiles of 128 from a multiple of 128 on.
+//     warps 0, 2, 3   codes to fp16, which holds every e4m3 number exactly: TMA brings a tile's codes, the warps turn them into the swizzled operands (a conversion for two codes)
+//     warp 1          MMAs: S = Q K^T from shared memory, O += P V with P in tensor memory.  The tiles take turns, S of the next key tile right behind PV of this one, so that one
+//                     tile's soft-max runs beside the other's products
+//     warps 4-7       soft-max of the first tile, 8-11 of the second: a thread owns a row.  First it makes its row of Q: fp16 of the row moved by a power of two so that its largest
+//                     stands in [2^13, 2^14) (exact for what is within 2^-28 of that).  t = s log2(e) + log2(value scale), p = 2^(t - m), l += p / (value scale): scales are one number a
+//                     page and head, so that of 64 scores at a time they change the factor and the offset of an fma that is there anyway, and O needs none.  P (fp16, 2^-11 of a
+//                     weight off at most) replaces its S in tensor memory; m is raised, and O scaled in tensor memory, only when a row's t outgrows it by 8
+// TMEM: [S0 | O0 | S1 | O1], 128 columns each.  Shared memory: Q 64 KB, K and V 2 x 32 KB each as fp16, 16 KB each as codes.
+#pragma once
+#include <cuda.h>
+
+#include "umma.cuh"
+
+namespace ktb {
+
+constexpr int kFpThreads = 384, kFpKeys = 128, kFpTile = 128 * 128 * 2, kFpCodes = 128 * 128, kFpBad = 64;
+struct FpMisc {
+    unsigned long long q_full, k8_full, v8_full, k_full[2], k_free[2], v_full[2], v_free[2], s_full[2], p_full[2], o_done[2];
+    float2 scales[4][2];      // of a tile's two runs of 64 keys (zeros: not there)
+    uint32_t tmem_base;
+    int info[4], n_bad, bad_lo, bad_hi;
+    int2 bad[kFpBad];      // values that are NaN in tiles that not every row sees whole: (key, run of 16 columns << 16 | which of them)
+};
+constexpr int kFpSmem = 6 * kFpTile + 2 * kFpCodes + (int)sizeof(FpMisc) + 1024;
+static_assert(kFpSmem <= 232448, "shared memory budget");
+
+__global__ void __launch_bounds__(kFpThreads, 1) fp8_attn_prompt_kernel(const __grid_constant__ FdMaps maps, const Fp8Attn a, int RH) {
+    using namespace umma;
+    extern __shared__ __align__(16) uint8_t fp_smem_raw[];
+    const uint32_t raw = smem_u32(fp_smem_raw), base = (raw + 1023u) & ~1023u;
+    uint8_t* smem = fp_smem_raw + (base - raw);
+    const uint32_t kbase = base + 2 * kFpTile, vbase = base + 4 * kFpTile, k8base = base + 6 * kFpTile, v8base = k8base + kFpCodes;
+    FpMisc& misc = *reinterpret_cast<FpMisc*>(smem + 6 * kFpTile + 2 * kFpCodes);
+    const int tid = threadIdx.x, lane = tid & 31, warp = uniform(tid >> 5), ps = a.pages.page_size, TOKS = 128 / RH, R = a.H / a.G, hblocks = R / RH;
+    griddep_launch_dependents();
+    if (tid == 0) {
+        bar_init(smem_u32(&misc.q_full), 8);
+        bar_init(smem_u32(&misc.k8_full), 1);
+        bar_init(smem_u32(&misc.v8_full), 1);
+        for (int i = 0; i < 2; i++) {
+            bar_init(smem_u32(&misc.k_full[i]), 3); bar_init(smem_u32(&misc.k_free[i]), 1); bar_init(smem_u32(&misc.v_full[i]), 3); bar_init(smem_u32(&misc.v_free[i]), 1);
+            bar_init(smem_u32(&misc.s_full[i]), 1); bar_init(smem_u32(&misc.p_full[i]), 4); bar_init(smem_u32(&misc.o_done[i]), 1);
+        }
+        bar_fence_init();
+        misc.n_bad = 0;
+        misc.bad_lo = 0x7fffffff;
+        misc.bad_hi = -1;
+        tma_prefetch_desc(&maps.k);
+        tma_prefetch_desc(&maps.v);
+    }
+    griddep_wait();
+    if (warp == 1) fp8_find_tokens(a, gridDim.x - 1 - blockIdx.x, 2 * TOKS, misc.info);      // the last tokens, which see most keys, first
+    __syncthreads();
+    const int tok0 = misc.info[0], ntok = misc.info[1], pos0 = misc.info[2], slot = misc.info[3];
+    if (ntok <= 0) return;
+    const int g = blockIdx.y / hblocks, h0 = g * R + (blockIdx.y % hblocks) * RH;
+    const int max_pos = pos0 + ntok - 1, lo = fp8_first_visible(pos0, a.window, a.chunk), lo_al = lo & ~(kFpKeys - 1);
+    const bool cut = a.part > 0 && max_pos + 1 - lo_al > a.part;
+    const int k_lo = lo_al + blockIdx.z * a.part, k_hi = cut ? min(max_pos + 1, k_lo + a.part) : max_pos + 1;
+    if (k_lo >= k_hi) return;
+    const int n = (k_hi - k_lo + kFpKeys - 1) / kFpKeys;
+    if (warp == 1) tmem_alloc(smem_u32(&misc.tmem_base), 512);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = uniform(misc.tmem_base);
+
+    // registers: 168 a thread at launch; a soft-max thread holds a row of 128 scores (2 x 208 + 88 = 3 x 168)
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+        if (warp == 1) {
+            // ================================================================ products (converged warp)
+            constexpr uint32_t idesc_qk = instr_desc(1, 0, 0, 0, 0, 128, 128), idesc_pv = instr_desc(1, 0, 0, 0, 1, 128, 128);      // V [key][column]: B MN-major
+            auto scores = [&](int t, int j) {
+                const uint32_t qb = base + t * kFpTile, kb = kbase + (j & 1) * kFpTile;
+#pragma unroll
+                for (int k = 0; k < 2; k++)
+                    mma_f16_x4(tmem + t * 256, smem_desc(qb + k * (kFpTile / 2), 16, 1024, kLayoutSw128), smem_desc(kb + k * (kFpTile / 2), 16, 1024, kLayoutSw128), idesc_qk, k != 0,
+                               k ? smem_u32(&misc.s_full[t]) : 0);
+            };
+            bar_wait(smem_u32(&misc.q_full), 0);
+            bar_wait(smem_u32(&misc.k_full[0]), 0);
+            tc_fence_after();
+            scores(0, 0);
+            scores(1, 0);
+            mma_commit(smem_u32(&misc.k_free[0]));
+            for (int j = 0; j < n; j++) {
+                const int st = j & 1;
+                const uint32_t vb = vbase + st * kFpTile;
+                bar_wait(smem_u32(&misc.v_full[st]), (j >> 1) & 1);
+                if (j + 1 < n) bar_wait(smem_u32(&misc.k_full[st ^ 1]), ((j + 1) >> 1) & 1);
+#pragma unroll 1
+                for (int t = 0; t < 2; t++) {
+                    bar_wait(smem_u32(&misc.p_full[t]), j & 1);
+                    tc_fence_after();
+#pragma unroll
+                    for (int k = 0; k < 8; k++)
+                        mma_f16_ta(tmem + t * 256 + 128, tmem + t * 256 + 8 * k, smem_desc(vb + k * 2048, kFpTile / 2, 1024, kLayoutSw128), idesc_pv, (j | k) != 0);
+                    if (t == 1) mma_commit(smem_u32(&misc.v_free[st]));
+                    if (j + 1 < n) {
+                        scores(t, j + 1);
+                        if (t == 1) mma_commit(smem_u32(&misc.k_free[st ^ 1]));
+                    } else {
+                        mma_commit(smem_u32(&misc.o_done[t]));
+                    }
+                }
+            }
+        } else {
+            // ================================================================ codes to fp16
+            const int cw = warp == 0 ? 0 : warp - 1, piece = lane & 7, r4 = lane >> 3, none = a.pages.n_pages * a.G * ps;      // (rows from `none` on are outside the maps: zeros)
+            const bool slot_ok = (unsigned)slot < (unsigned)a.pages.slots;
+            const int* pt = a.pages.table + (slot_ok ? (long)slot * a.pages.max_pages : 0);
+            const int last_first = fp8_first_visible(max_pos, a.window, a.chunk);
+            auto row_of = [&](int key) {      // of a run of 64 keys; `none`: not there, or nobody sees it
+                if (!slot_ok || key >= k_hi || key + 64 <= lo) return none;
+                const int page = pt[(key / ps) % a.pages.max_pages];
+                return (unsigned)page < (unsigned)a.pages.n_pages ? (page * a.G + g) * ps + key % ps : none;
+            };
+            auto bring = [&](uint32_t dst, const CUtensorMap* map, unsigned long long* bar, int r0, int r1) {
+                bar_expect_tx(smem_u32(bar), kFpCodes);
+                tma_load_2d(dst, map, smem_u32(bar), 0, r0);
+                tma_load_2d(dst + kFpCodes / 2, map, smem_u32(bar), 0, r1);
+            };
+            // rows 4 i + r4 of the tile, 16 codes a lane, into the 128-byte-swizzled operand: two blocks of 64 columns, rows of 128 bytes
+            auto turn = [&](uint32_t src, uint32_t dst, bool values, int k0) {
+                const bool partial = values && !(k0 >= last_first && k0 + kFpKeys - 1 <= pos0), edge = values && (k0 < lo || k0 + kFpKeys > k_hi);
+#pragma unroll 4
+                for (int i = cw; i < 32; i += 3) {
+                    const int r = 4 * i + r4;
+                    const uint4 v = lds16(src + r * 128 + piece * 16);
+                    uint32_t w[4] = {v.x, v.y, v.z, v.w};
+                    if (edge && (k0 + r < lo || k0 + r >= k_hi)) w[0] = w[1] = w[2] = w[3] = 0;      // values that no row sees may be anything (0 x NaN)
+                    if (partial) {      // a value that is NaN belongs to the rows that see it: they are told at the end
+                        uint32_t mask = 0;
+#pragma unroll
+                        for (int q = 0; q < 4; q++) {
+                            const uint32_t odd = (((w[q] & 0x7f7f7f7fu) + 0x01010101u) >> 7) & 0x01010101u;
+                            mask |= ((odd * 0x10204080u) >> 28) << (4 * q);      // byte b's bit to bit b
+                            w[q] &= ~(odd * 0xffu);
+                        }
+                        if (mask) {
+                            const int at = atomicAdd(&misc.n_bad, 1);
+                            if (at < kFpBad) misc.bad[at] = make_int2(k0 + r, piece << 16 | (int)mask);
+                            atomicMin(&misc.bad_lo, k0 + r);
+                            atomicMax(&misc.bad_hi, k0 + r);
+                        }
+                    }
+                    uint32_t f[8];
+#pragma unroll
+                    for (int q = 0; q < 4; q++) { f[2 * q] = f16_of_codes(w[q]); f[2 * q + 1] = f16_of_codes(w[q] >> 16); }
+                    const uint32_t at = dst + (piece >> 2) * (kFpTile / 2) + r * 128;
+                    const int c = 2 * (piece & 3);
+                    // (the second block's lanes begin with their second half: no two lanes meet in a bank)
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        const int h = e ^ (piece >> 2);
+                        const uint32_t to = at + (((c + h) ^ (r & 7)) << 4);
+                        const uint32_t x0 = h ? f[4] : f[0], x1 = h ? f[5] : f[1], x2 = h ? f[6] : f[2], x3 = h ? f[7] : f[3];
+                        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(x0), "r"(x1), "r"(x2), "r"(x3) : "memory");
+                    }
+                }
+                fence_async_smem();
+            };
+            auto together = [] { asm volatile("barrier.cta.sync 2, 96;" ::: "memory"); };
+            int r0 = row_of(k_lo), r1 = row_of(k_lo + 64);
+            if (warp == 0 && lane == 0) {
+                bring(k8base, &maps.k, &misc.k8_full, r0, r1);
+                bring(v8base, &maps.v, &misc.v8_full, r0, r1);
+            }
+            for (int j = 0; j < n; j++) {
+                const int st = j & 1, ph = ((j >> 1) & 1) ^ 1, k0 = k_lo + j * kFpKeys;
+                if (warp == 2 && lane < 2) {      // the runs' scales
+                    const int row = lane ? r1 : r0;
+                    misc.scales[j & 3][lane] = row == none ? make_float2(0.f, 0.f) : *reinterpret_cast<const float2*>(a.scales + 2 * (long)(row / ps));
+                }
+                r0 = row_of(k0 + kFpKeys);
+                r1 = row_of(k0 + kFpKeys + 64);
+                bar_wait(smem_u32(&misc.k8_full), j & 1);
+                bar_wait(smem_u32(&misc.k_free[st]), ph);
+                turn(k8base, kbase + st * kFpTile, false, k0);
+                together();
+                if (lane == 0) {
+                    bar_arrive(smem_u32(&misc.k_full[st]));
+                    if (warp == 0 && j + 1 < n) bring(k8base, &maps.k, &misc.k8_full, r0, r1);
+                }
+                __syncwarp();
+                bar_wait(smem_u32(&misc.v8_full), j & 1);
+                bar_wait(smem_u32(&misc.v_free[st]), ph);
+                turn(v8base, vbase + st * kFpTile, true, k0);
+                together();
+                if (lane == 0) {
+                    bar_arrive(smem_u32(&misc.v_full[st]));
+                    if (warp == 0 && j + 1 < n) bring(v8base, &maps.v, &misc.v8_full, r0, r1);
+                }
+                __syncwarp();
+            }
+        }
+    } else {
+        // ================================================================ soft-max
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+        const int t = (warp - 4) >> 2, sp = warp & 3, r = 32 * sp + lane;
+        const uint32_t ts = tmem + ((uint32_t)(32 * sp) << 16) + t * 256, to = ts + 128;
+        const int tok = t * TOKS + r / RH, h = h0 + r % RH;
+        const bool valid = r < TOKS * RH && tok < ntok;
+        const int p = pos0 + tok, first = fp8_first_visible(p, a.window, a.chunk);
+        float fac;
+        {      // the row of Q
+            uint32_t w[64];
+            const uint4* row = reinterpret_cast<const uint4*>((const __nv_bfloat16*)a.q + ((long)(tok0 + tok) * a.H + h) * 128);
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                const uint4 v = valid ? row[i] : make_uint4(0, 0, 0, 0);
+                w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
+            }
+            float top = 0.f;
+#pragma unroll
+            for (int i = 0; i < 64; i++) top = fmaxf(top, fmaxf(fabsf(__uint_as_float(w[i] << 16)), fabsf(__uint_as_float(w[i] & 0xffff0000u))));
+            const int up = min(126, max(-112, 13 - ((int)(__float_as_uint(top) >> 23) - 127)));      // (an infinity stays one)
+            const float by = __uint_as_float((uint32_t)(up + 127) << 23);
+            fac = valid ? (a.head_scale ? a.scale * a.head_scale[h] : a.scale) / by : 0.f;
+#pragma unroll
+            for (int c = 0; c < 16; c++) {
+                uint32_t f[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) f[i] = pack_f16(__uint_as_float(w[4 * c + i] << 16) * by, __uint_as_float(w[4 * c + i] & 0xffff0000u) * by);
+                *reinterpret_cast<uint4*>(smem + t * kFpTile + (c >> 3) * (kFpTile / 2) + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = make_uint4(f[0], f[1], f[2], f[3]);
+            }
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) bar_arrive(smem_u32(&misc.q_full));
+        }
+        const float softcap = a.softcap, two_over_cap = softcap > 0.f ? 2.0f / softcap : 0.f;
+        // scores that are only scaled (by a positive number) go to the exponential as they are
+        const bool direct = __all_sync(0xffffffffu, softcap <= 0.f && (fac > 0.f || !valid));
+        const int w_tok0 = t * TOKS + 32 * sp / RH, w_tok1 = t * TOKS + min(TOKS - 1, (32 * sp + 31) / RH);      // the warp's first and last token
+        const bool w_full = w_tok1 < ntok;
+        const int w_last_first = fp8_first_visible(pos0 + w_tok1, a.window, a.chunk);
+        float m_ref = -INFINITY, l = 0.f;
+        for (int j = 0; j < n; j++) {
+            const int k0 = k_lo + j * kFpKeys;
+            bar_wait(smem_u32(&misc.s_full[t]), j & 1);      // (also: PV of the tile before this one is complete)
+            tc_fence_after();
+            float s[kFpKeys];
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                uint32_t v[32];
+                tmem_ld32(ts + 32 * q, v);
+#pragma unroll
+                for (int i = 0; i < 32; i++) s[32 * q + i] = __uint_as_float(v[i]);
+            }
+            float c[2], ve[2], inv[2];
+            bool there = true;
+#pragma unroll
+            for (int q = 0; q < 2; q++) {
+                const float2 sc = misc.scales[j & 3][q];
+                const uint32_t vb = __float_as_uint(sc.y);
+                c[q] = direct ? fmaxf(fac * sc.x * kLog2e, 1.2e-38f) : fac * sc.x;      // (above zero: -inf times it stays that)
+                ve[q] = (float)((int)(vb >> 23) - 127);
+                inv[q] = vb ? __uint_as_float((254u << 23) - vb) : 0.f;
+                there &= vb != 0;
+            }
+            tmem_wait_ld();
+            // (the loads above are in registers only now)
+#pragma unroll
+            for (int i = 0; i < kFpKeys; i++) asm volatile("" : "+f"(s[i]));
+            if (!direct) {
+#pragma unroll
+                for (int i = 0; i < kFpKeys; i++) {
+                    float x = s[i] * c[i >> 6];
+                    if (softcap > 0.f) x = softcap * (1.0f - __fdividef(2.0f, __expf(x * two_over_cap) + 1.0f));      // c tanh(s / c): a few 1e-7 of the cap off
+                    s[i] = x * kLog2e;
+                }
+                c[0] = c[1] = 1.f;
+            }
+            if (!(there && w_full && k0 + kFpKeys <= k_hi && k0 + kFpKeys - 1 <= pos0 + w_tok0 && k0 >= w_last_first)) {
+                const int i0 = first - k0, i1 = valid ? min(p, k_hi - 1) - k0 : -1;
+#pragma unroll
+                for (int i = 0; i < kFpKeys; i++)
+                    if (i < i0 || i > i1 || inv[i >> 6] == 0.f) s[i] = -INFINITY;
+            }
+            float mx[4] = {s[0], s[1], s[64], s[65]};
+#pragma unroll
+            for (int i = 2; i < 64; i += 2) {
+                mx[0] = fmaxf(mx[0], s[i]);
+                mx[1] = fmaxf(mx[1], s[i + 1]);
+                mx[2] = fmaxf(mx[2], s[64 + i]);
+                mx[3] = fmaxf(mx[3], s[64 + i + 1]);
+            }
+            const float m_new = fmaxf(fmaf(fmaxf(mx[0], mx[1]), c[0], ve[0]), fmaf(fmaxf(mx[2], mx[3]), c[1], ve[1]));
+            const bool raise = m_new > m_ref + 8.f || (m_ref == -INFINITY && m_new > -INFINITY);
+            if (__any_sync(0xffffffffu, raise)) {
+                const float alpha = raise ? exp2_approx(m_ref - m_new) : 1.f;      // (2^-inf = 0: nothing was summed yet)
+                if (raise) { m_ref = m_new; l *= alpha; }
+                if (j > 0) {
+#pragma unroll 1
+                    for (int q = 0; q < 4; q++) {
+                        uint32_t v[32];
+                        tmem_ld32(to + 32 * q, v);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 32; i++) v[i] = __float_as_uint(__uint_as_float(v[i]) * alpha);
+                        tmem_st32(to + 32 * q, v);
+                    }
+                }
+            }
+            const float u = m_ref == -INFINITY ? 0.f : m_ref;
+#pragma unroll
+            for (int q = 0; q < 2; q++) {
+                const f32x2 c2 = pack2(c[q], c[q]), o2 = pack2(ve[q] - u, ve[q] - u);
+                f32x2 sum[2] = {0, 0};
+                uint32_t pk[32];
+#pragma unroll
+                for (int i = 0; i < 32; i++) {
+                    float e0, e1;
+                    unpack2(fma2(pack2(s[64 * q + 2 * i], s[64 * q + 2 * i + 1]), c2, o2), e0, e1);
+                    e0 = exp2_approx(e0);
+                    e1 = exp2_approx(e1);
+                    pk[i] = pack_f16(e0, e1);
+                    sum[i & 1] = add2(sum[i & 1], pack2(e0, e1));
+                }
+                tmem_st32(ts + 32 * q, pk);
+                float a0, a1, a2, a3;
+                unpack2(sum[0], a0, a1);
+                unpack2(sum[1], a2, a3);
+                l = fmaf((a0 + a1) + (a2 + a3), inv[q], l);
+            }
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) bar_arrive(smem_u32(&misc.p_full[t]));
+        }
+        bar_wait(smem_u32(&misc.o_done[t]), 0);
+        tc_fence_after();
+        const long row = (long)(tok0 + tok) * a.H + h;
+        float* part = cut ? a.partial + (row * a.parts + blockIdx.z) * 130 : nullptr;
+        float k = 1.f;
+        if (cut) {
+            if (valid) *reinterpret_cast<float2*>(part) = make_float2(m_ref, l);
+        } else {
+            if (a.sink) {
+                const float sk = a.sink[h] * kLog2e, mn = fmaxf(m_ref, sk);
+                k = m_ref == -INFINITY ? 0.f : exp2_approx(m_ref - mn);
+                l = l * k + exp2_approx(sk - mn);
+            }
+            k = l > 0.f || l != l ? k * a.out_scale / l : 0.f;
+        }
+        __nv_bfloat16* out = (__nv_bfloat16*)a.out + (long)(tok0 + tok) * a.out_stride + (long)h * 128;
+        const bool vec = (reinterpret_cast<uintptr_t>(out) & 15) == 0;
+        const int bad = min(misc.n_bad, kFpBad);
+#pragma unroll 1
+        for (int q = 0; q < 4; q++) {
+            uint32_t v[32];
+            tmem_ld32(to + 32 * q, v);
+            tmem_wait_ld();
+            if (!valid) continue;
+            if (bad > 0) {
+                const bool whole = misc.n_bad > kFpBad && misc.bad_lo <= p && misc.bad_hi >= first;      // (more than the list holds: rows that see keys between the first and the last)
+                for (int b = 0; b < bad; b++) {
+                    const int2 e = misc.bad[b];
+                    const int run = e.y >> 16;
+                    const uint32_t mask = e.x >= first && e.x <= p && (run >> 1) == q ? (uint32_t)(e.y & 0xffff) << (16 * (run & 1)) : 0u;
+#pragma unroll
+                    for (int i = 0; i < 32; i++)
+                        if (whole || (mask >> i & 1)) v[i] = 0x7fffffffu;
+                }
+            }
+            if (cut) {
+#pragma unroll
+                for (int i = 0; i < 16; i++) *reinterpret_cast<float2*>(part + 2 + 32 * q + 2 * i) = make_float2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
+                continue;
+            }
+            uint32_t o[16];
+#pragma unroll
+            for (int i = 0; i < 16; i++) o[i] = pack_bf16(__uint_as_float(v[2 * i]) * k, __uint_as_float(v[2 * i + 1]) * k);
+            if (vec) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) *reinterpret_cast<uint4*>(out + 32 * q + 8 * i) = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 32; i++) reinterpret_cast<uint16_t*>(out)[32 * q + i] = (uint16_t)(o[i >> 1] >> (16 * (i & 1)));
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+// whether these tiles take the call: portions of half a row tile's tokens on average
+static bool fp_takes(const ktb200_fp8_attn_params* c, int n_tokens, int dtype) {
+    return fm_takes(c, dtype) && c->dim == 128 && c->vdim == 128 && c->page_size % 64 == 0 && c->n_pages > 0 && (long)c->n_pages * c->kv_heads * c->page_size < (1L << 31) &&
+           (long)n_tokens * fm_heads(c->heads / c->kv_heads) >= 64L * c->n_seqs;
+}
+static int fp_launch(const Fp8Attn& a, int RH, dim3 grid, cudaStream_t s) {
+    FdMaps maps;
+    const int rc = fd_maps(maps, a, 64, CU_TENSOR_MAP_SWIZZLE_NONE);
+    if (rc) return rc;
+    KTB_CUDA_CHECK(raise_smem_limit((const void*)fp8_attn_prompt_kernel, kFpSmem));
+    KTB_CUDA_CHECK(launch_pdl(fp8_attn_prompt_kernel, grid, dim3(kFpThreads), (size_t)kFpSmem, s, maps, a, RH));
+    return KTB200_OK;
+}
+
+}  // namespace ktb

@@ -269,6 +269,11 @@ SHAPES = [
     ([(10, 100)], 64, 16, 2, 128, 128),
     ([(3, 0), (9, 20), (0, 0)], 16, 4, 2, 64, 64),                    # portions without tokens
     ([(6, 40)], 5, 4, 2, 128, 64),
+    ([(130, 200)], 64, 3, 1, 128, 128),                               # rows that a tile's tokens do not fill
+    ([(2000, 20)], 64, 16, 1, 128, 128),                              # a short portion over a range that is cut
+    ([(9, 150), (0, 64)], 128, 2, 2, 128, 128),
+    ([(500, 1), (3, 1), (129, 1)], 16, 12, 2, 128, 128),
+    ([(500, 1), (3, 1)], 48, 34, 2, 128, 128),                        # a group that no run of 16 heads divides
 ]
 
 
@@ -288,12 +293,16 @@ MASKS = [dict(window=1), dict(window=50), dict(chunk=16), dict(chunk=33, sink=Tr
 def test_attention_masks_and_scores(options, dtype):
     run_attention([(100, 1), (0, 40), (31, 33), (700, 2)], 32, 8, 2, 128, 128, dtype, seed=5, **options)
     run_attention([(100, 1), (0, 4), (31, 3)], 48, 6, 2, 96, 64, dtype, seed=6, **options)
+    run_attention([(150, 40), (0, 140), (600, 3)], 64, 8, 2, 128, 128, dtype, seed=7, **options)
+    run_attention([(200, 1), (0, 1), (1300, 1)], 64, 16, 1, 128, 128, dtype, seed=7, **options)
 
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["bf16", "fp32"])
 def test_attention_blocks_of_very_different_scales(dtype):
     run_attention([(400, 1), (90, 5)], 16, 4, 1, 64, 64, dtype, seed=8, wide=5)
+    run_attention([(700, 1), (300, 1)], 64, 4, 1, 128, 128, dtype, seed=8, wide=5)
+    run_attention([(300, 40)], 64, 4, 1, 128, 128, dtype, seed=8, wide=5)
 
 
 @pytest.mark.gpu
@@ -302,6 +311,8 @@ def test_attention_writes_its_rows_alone(dtype):
     run_attention([(100, 3), (0, 20)], 16, 4, 2, 64, 64, dtype, seed=9, tail=4, out_stride=24)
     run_attention([(900, 1)], 16, 4, 2, 64, 64, dtype, seed=9, tail=2, out_stride=8)
     run_attention([(90, 2)], 16, 4, 2, 64, 64, dtype, seed=9, out_stride=3)      # rows that begin anywhere
+    run_attention([(90, 70)], 64, 4, 2, 128, 128, dtype, seed=9, tail=3, out_stride=3)
+    run_attention([(990, 1)], 64, 4, 2, 128, 128, dtype, seed=9, tail=1, out_stride=5)
 
 
 @pytest.mark.gpu
@@ -331,7 +342,7 @@ def test_attention_over_a_ring_of_pages(dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["bf16", "fp32"])
-@pytest.mark.parametrize("d,ps,lens,at", [(128, 64, [(0, 90)], 50), (64, 16, [(20, 3)], 21), (96, 48, [(5, 40)], 44), (128, 64, [(200, 300)], 260)])
+@pytest.mark.parametrize("d,ps,lens,at", [(128, 64, [(0, 90)], 50), (128, 64, [(0, 20)], 11), (64, 16, [(20, 3)], 21), (96, 48, [(5, 40)], 44), (128, 64, [(200, 300)], 260)])
 def test_attention_keeps_nan_to_the_rows_that_see_it(d, ps, lens, at, dtype):
     """a token whose key (or value) is NaN: the tokens ahead of it do not see it, those behind it do"""
     H, G, (b, n) = 4, 2, lens[0]
@@ -349,6 +360,10 @@ def test_attention_keeps_nan_to_the_rows_that_see_it(d, ps, lens, at, dtype):
             assert out[first:, 2:].isnan().all()
         else:
             assert out[first:, 2:, 5].isnan().all() and not out[first:, 2:, 6:].isnan().any()
+            for more in range(at, min(at + 9, b + n), 2):      # whole tokens of them
+                kv.v.view(torch.uint8)[int(cache.page_table[0, more // ps]), 1, more % ps] = 0x7f
+            out = fp8_cache_attention(q, kv, on(batch), on(cache), H, G, d, d, d ** -0.5).view(n, H, d)
+            assert torch.equal(out[:first, 2:], clean[:first, 2:]) and out[first:, 2:].isnan().all()
 
 
 @pytest.mark.gpu
