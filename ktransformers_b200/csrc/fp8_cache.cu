@@ -4,10 +4,11 @@
 //                             column (3); then a turn of the first rot_dims columns (pairs of either layout, angle pos * inv_freq[i]).  q to q_out; k and v as
 //                             e4m3 codes under one scale per page and head.
 //
-// The tokens of a portion that fall into one page are appended by one CTA per key/value head, which finds their largest |k| and |v|, makes the block's scales, moves
-// the codes of the tokens that the page held before where a scale has grown, and writes the new codes: no other CTA touches the block, so there is nothing to
-// order and nothing to add up atomically.  A portion that begins at a page's first token starts its blocks anew (whatever the page held).
-// Rotation, norms and scaling are fp32; angles are reduced in fp64.
+// The tokens of a portion that fall into one page are appended by one CTA per key/value head for the keys and one for the values, which finds their largest magnitude, makes
+// the block's scale, moves the codes of the tokens that the page held before where the scale has grown, and writes the new codes: no other CTA touches the block, so there
+// is nothing to order and nothing to add up atomically.  A portion that begins at a page's first token starts its blocks anew (whatever the page held).
+// Queries are turned and normed in fp32.  Keys are in fp64 up to their one rounding to fp32 ahead of the codes (the GPU does half as many fp64 operations as fp32 ones in a cycle, and a
+// step's keys are few): their codes are those of the exact numbers, whatever the order of a sum.  Angles are fp64 in both.
 #include <cuda_bf16.h>
 
 #include <algorithm>
@@ -16,7 +17,7 @@
 
 namespace ktb {
 
-constexpr int kAppThreads = 256, kAppWarps = kAppThreads / 32, kAppCols = 8 /* columns of a lane: head sizes up to 256 */, kAppKeep = 96 * 1024;
+constexpr int kAppCols = 8 /* columns of a lane: head sizes up to 256 */, kAppKeep = 48 * 1024 /* bytes of rows that a CTA keeps between the search for their largest and their codes */;
 
 struct Fp8Append {
     const void* proj;
@@ -32,100 +33,161 @@ struct Fp8Append {
     uint8_t *k_codes, *v_codes;
     float* scales;
     void* q_out;
-    int kv_ctas, keep, q_tokens, q_heads, q_blocks;
+    int kv_ctas, q_heads, q_blocks, keep;      // CTAs of keys and values; query heads of a warp, warps of a token; rows of a page that fit in kAppKeep
 };
 
-// (cos, sin) of pos * freq: the angle and its remainder in 64 bits, sine and cosine of the remainder's fp32 part, corrected by what that left
-__device__ __forceinline__ float2 app_turn(int pos, double freq) {
-    const double angle = (double)pos * freq, rest = fma(-rint(angle * 0.15915494309189535), 6.283185307179586, angle);
-    const float hi = (float)rest, lo = (float)(rest - (double)hi);
-    float sn, cs;
-    sincosf(hi, &sn, &cs);
-    return make_float2(fmaf(-lo, sn, cs), fmaf(lo, cs, sn));
+template <typename F> struct AppTurn { F c, s; };
+// (cos, sin) of pos * freq: the angle less a multiple of pi / 2, within pi / 4 of zero, and the first terms of both series (2e-14 and 1e-15 off)
+template <typename F> __device__ __forceinline__ AppTurn<F> app_turn(int pos, double freq) {
+    const double angle = (double)pos * freq, k = rint(angle * 0.63661977236758134), r = fma(-k, 6.123233995736766e-17, fma(-k, 1.5707963267948966, angle)), x = r * r;
+    double s = fma(x, 1.0 / 6227020800.0, -1.0 / 39916800.0), c = fma(x, -1.0 / 87178291200.0, 1.0 / 479001600.0);
+    s = fma(x, s, 1.0 / 362880.0);
+    c = fma(x, c, -1.0 / 3628800.0);
+    s = fma(x, s, -1.0 / 5040.0);
+    c = fma(x, c, 1.0 / 40320.0);
+    s = fma(x, s, 1.0 / 120.0);
+    c = fma(x, c, -1.0 / 720.0);
+    s = fma(x, s, -1.0 / 6.0);
+    c = fma(x, c, 1.0 / 24.0);
+    s = fma(r * x, s, r);
+    c = fma(x, fma(x, c, -0.5), 1.0);
+    const int quarter = (int)k;
+    const double u = quarter & 1 ? s : c, v = quarter & 1 ? c : s;      // cos and sin of the angle but for their signs
+    return {(F)((quarter + 1) & 2 ? -u : u), (F)(quarter & 2 ? -v : v)};
 }
+template <typename F> __device__ __forceinline__ F app_sum(F v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+__device__ __forceinline__ float app_inv_root(float x) { return 1.0f / sqrtf(x); }
+__device__ __forceinline__ double app_inv_root(double x) { return 1.0 / sqrt(x); }
 
 // One head's columns of one token, as a warp holds them.  PER > 0: heads of 32 PER columns, a lane's PER of them side by side; PER = 0: any size, columns lane, lane + 32, ..
 template <typename T, int PER> struct AppRow {
     static constexpr int N = PER ? PER : kAppCols;
     float x[N];
     __device__ __forceinline__ static int col(int e) { const int lane = threadIdx.x & 31; return PER ? lane * PER + e : lane + 32 * e; }
+    static constexpr int W = PER ? PER * (int)sizeof(T) / 4 : 1;      // words of a lane's columns as they are stored
+    __device__ __forceinline__ static void fetch(uint32_t (&w)[W], const T* row) {
+        const void* from = row + col(0);
+        if constexpr (W == 1) w[0] = *reinterpret_cast<const uint32_t*>(from);
+        else if constexpr (W == 2) { const uint2 v = *reinterpret_cast<const uint2*>(from); w[0] = v.x; w[1] = v.y; }
+        else {
+#pragma unroll
+            for (int i = 0; i < W; i += 4) { const uint4 v = reinterpret_cast<const uint4*>(from)[i / 4]; w[i] = v.x; w[i + 1] = v.y; w[i + 2] = v.z; w[i + 3] = v.w; }
+        }
+    }
+    __device__ __forceinline__ void unpack(const uint32_t (&w)[W]) {
+#pragma unroll
+        for (int i = 0; i < W; i++) {
+            if constexpr (sizeof(T) == 4) x[i] = __uint_as_float(w[i]);
+            else { x[2 * i] = __uint_as_float(w[i] << 16); x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+        }
+    }
+    // a lane's columns on their way to shared memory (the lane reads them there itself)
+    __device__ __forceinline__ static void bring(T* to, const T* row) {
+        constexpr int B = W * 4 < 16 ? W * 4 : 16;
+        const uint32_t dst = (uint32_t)__cvta_generic_to_shared(to + col(0));
+        const char* src = reinterpret_cast<const char*>(row + col(0));
+#pragma unroll
+        for (int i = 0; i < W * 4; i += B) asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst + i), "l"(src + i), "n"(B) : "memory");
+    }
     __device__ __forceinline__ void load(const T* row, int n) {
         if constexpr (PER == 0) {
 #pragma unroll
             for (int e = 0; e < N; e++) x[e] = col(e) < n ? to_f(row[col(e)]) : 0.f;
-        } else if constexpr (sizeof(T) == 4) {
-            if constexpr (PER == 2) {
-                const float2 v = *reinterpret_cast<const float2*>(row + col(0));
-                x[0] = v.x; x[1] = v.y;
-            } else {
-#pragma unroll
-                for (int e = 0; e < N; e += 4) {
-                    const float4 v = *reinterpret_cast<const float4*>(row + col(e));
-                    x[e] = v.x; x[e + 1] = v.y; x[e + 2] = v.z; x[e + 3] = v.w;
-                }
-            }
         } else {
-            uint32_t w[PER / 2];
-            if constexpr (PER == 2) w[0] = *reinterpret_cast<const uint32_t*>(row + col(0));
-            else if constexpr (PER == 4) { const uint2 v = *reinterpret_cast<const uint2*>(row + col(0)); w[0] = v.x; w[1] = v.y; }
-            else { const uint4 v = *reinterpret_cast<const uint4*>(row + col(0)); w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w; }
-#pragma unroll
-            for (int e = 0; e < PER / 2; e++) { x[2 * e] = __uint_as_float(w[e] << 16); x[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u); }
+            uint32_t w[W];
+            fetch(w, row);
+            unpack(w);
         }
     }
-    // norm and turn; `turn(i)`: (cos, sin) of pair i
-    template <typename Turn> __device__ __forceinline__ void prepare(const T* row, const Fp8Append& a, const T* w, Turn turn) {
-        const int lane = threadIdx.x & 31, half = a.rot_dims >> 1;
-        float inv = 1.f;
-        if (a.qk_norm) {
-            float ss = 0.f;
+    // The turns of a lane's columns at a position.  Two columns share each: two neighbours of a lane, or (halves) one of this lane and one of its partner, of which each makes half
+    template <typename F> __device__ __forceinline__ static void turns(const Fp8Append& a, int pos, AppTurn<F> (&t)[N]) {
+        const int half = a.rot_dims >> 1, lane = threadIdx.x & 31;
+        if constexpr (PER == 0) {
 #pragma unroll
-            for (int e = 0; e < N; e++) ss = fmaf(x[e], x[e], ss);
-            inv = 1.0f / sqrtf(warp_sum(ss) / (float)a.d + a.eps);
-#pragma unroll
-            for (int e = 0; e < N; e++)
-                if (PER || col(e) < a.d) x[e] = a.qk_norm == 3 ? x[e] * inv * to_f(w[col(e)]) : x[e] * inv;
-        }
-        if (a.rot_dims == 0) return;
-        if (a.rot_layout == kRotInterleaved && PER) {
+            for (int e = 0; e < N; e++) {
+                const int c = col(e);
+                t[e] = {F(1), F(0)};
+                if (c < a.rot_dims) t[e] = app_turn<F>(pos, a.inv_freq[a.rot_layout == kRotHalves ? (c >= half ? c - half : c) : c >> 1]);
+            }
+        } else if (a.rot_layout == kRotInterleaved) {
 #pragma unroll
             for (int e = 0; e < N; e += 2) {
                 const int c = col(e);
-                if (c < a.rot_dims) {
-                    const float2 t = turn(c >> 1);
-                    const float u = x[e], v = x[e + 1];
-                    x[e] = u * t.x - v * t.y;
-                    x[e + 1] = v * t.x + u * t.y;
-                }
-            }
-        } else if (PER) {      // halves: the partner's lane is half / PER lanes away
-            const int step = half / (PER ? PER : 1);
-#pragma unroll
-            for (int e = 0; e < N; e++) {
-                const int c = col(e);
-                const bool second = c >= half;
-                const float other = __shfl_sync(0xffffffffu, x[e], second ? lane - step : lane + step);
-                if (c < a.rot_dims) {
-                    const float2 t = turn(second ? c - half : c);
-                    x[e] = second ? x[e] * t.x + other * t.y : x[e] * t.x - other * t.y;
-                }
+                t[e] = {F(1), F(0)};
+                if (c < a.rot_dims) t[e] = app_turn<F>(pos, a.inv_freq[c >> 1]);
+                t[e + 1] = t[e];
             }
         } else {
+            const int step = half / (PER ? PER : 1);
+            const bool second = col(0) >= half, in = col(0) < a.rot_dims;
+            const int partner = second ? lane - step : lane + step;
 #pragma unroll
-            for (int e = 0; e < N; e++) {
-                const int c = col(e);
-                if (c < a.rot_dims) {
-                    const int o = rot_partner(c, a.rot_dims, a.rot_layout);
-                    const bool second = a.rot_layout == kRotHalves ? c >= half : (c & 1);
-                    const float2 t = turn(a.rot_layout == kRotHalves ? (second ? c - half : c) : (c >> 1));
-                    float other = to_f(row[o]) * inv;
-                    if (a.qk_norm == 3) other *= to_f(w[o]);
-                    x[e] = second ? x[e] * t.x + other * t.y : x[e] * t.x - other * t.y;
-                }
+            for (int e = 0; e < N / 2; e++) {
+                AppTurn<F> own{F(1), F(0)};
+                if (in) own = app_turn<F>(pos, a.inv_freq[col(second ? e + N / 2 : e) - (second ? half : 0)]);
+                const AppTurn<F> other{__shfl_sync(0xffffffffu, own.c, partner), __shfl_sync(0xffffffffu, own.s, partner)};
+                t[e] = second && in ? other : own;
+                t[e + N / 2] = second && in ? own : other;
+            }
+            if (!in) {
+#pragma unroll
+                for (int e = 0; e < N; e++) t[e] = {F(1), F(0)};
             }
         }
     }
-    __device__ __forceinline__ float top(int n) const {
+    // norm and turn, in F, then back to fp32
+    template <typename F> __device__ __forceinline__ void prepare(const T* row, const Fp8Append& a, const T* w, const AppTurn<F> (&t)[N]) {
+        const int lane = threadIdx.x & 31, half = a.rot_dims >> 1;
+        F y[N], inv = F(1);
+#pragma unroll
+        for (int e = 0; e < N; e++) y[e] = (F)x[e];
+        if (a.qk_norm) {
+            F ss = F(0);
+#pragma unroll
+            for (int e = 0; e < N; e++) ss = fma(y[e], y[e], ss);
+            inv = app_inv_root(app_sum(ss) / (F)a.d + (F)a.eps);
+#pragma unroll
+            for (int e = 0; e < N; e++)
+                if (PER || col(e) < a.d) y[e] = a.qk_norm == 3 ? y[e] * inv * (F)to_f(w[col(e)]) : y[e] * inv;
+        }
+        if (a.rot_dims) {
+            if (a.rot_layout == kRotInterleaved && PER) {
+#pragma unroll
+                for (int e = 0; e < N; e += 2) {
+                    const F u = y[e], v = y[e + 1];
+                    y[e] = u * t[e].c - v * t[e].s;
+                    y[e + 1] = v * t[e].c + u * t[e].s;
+                }
+            } else if (PER) {      // halves: the partner's lane is half / PER lanes away
+                const int step = half / (PER ? PER : 1);
+#pragma unroll
+                for (int e = 0; e < N; e++) {
+                    const int c = col(e);
+                    const F other = __shfl_sync(0xffffffffu, y[e], c >= half ? lane - step : lane + step);
+                    if (c < a.rot_dims) y[e] = c >= half ? y[e] * t[e].c + other * t[e].s : y[e] * t[e].c - other * t[e].s;
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < N; e++) {
+                    const int c = col(e);
+                    if (c < a.rot_dims) {
+                        const int o = rot_partner(c, a.rot_dims, a.rot_layout);
+                        const bool second = a.rot_layout == kRotHalves ? c >= half : (c & 1);
+                        F other = (F)to_f(row[o]) * inv;
+                        if (a.qk_norm == 3) other *= (F)to_f(w[o]);
+                        y[e] = second ? y[e] * t[e].c + other * t[e].s : y[e] * t[e].c - other * t[e].s;
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < N; e++) x[e] = (float)y[e];
+    }
+    __device__ __forceinline__ float top() const {
         float m = 0.f;
 #pragma unroll
         for (int e = 0; e < N; e++) m = fmaxf(m, fabsf(x[e]));      // (columns behind a head's last are zero)
@@ -172,7 +234,7 @@ __device__ __forceinline__ float fp8_power(int e) { return __uint_as_float((uint
 // The codes of `bytes` bytes at p times f (a power of two below one)
 __device__ __forceinline__ void fp8_move(uint8_t* p, long bytes, float f) {
     if (((reinterpret_cast<uintptr_t>(p) | bytes) & 3) == 0) {
-        for (long i = 4 * (long)threadIdx.x; i < bytes; i += 4 * kAppThreads) {
+        for (long i = 4 * (long)threadIdx.x; i < bytes; i += 4 * blockDim.x) {
             uint32_t w = *reinterpret_cast<uint32_t*>(p + i), r = 0;
 #pragma unroll
             for (int h = 0; h < 2; h++) {
@@ -183,124 +245,151 @@ __device__ __forceinline__ void fp8_move(uint8_t* p, long bytes, float f) {
             *reinterpret_cast<uint32_t*>(p + i) = r;
         }
     } else {
-        for (long i = threadIdx.x; i < bytes; i += kAppThreads) {
+        for (long i = threadIdx.x; i < bytes; i += blockDim.x) {
             const float x = __half2float(__half(__nv_cvt_fp8_to_halfraw(p[i], __NV_E4M3)));
             p[i] = (uint8_t)__nv_cvt_float_to_fp8(x * f, __NV_SATFINITE, __NV_E4M3);
         }
     }
 }
 
-// Blocks [0, kv_ctas): one page's tokens of one portion for one key/value head (the portions' pages in order, heads fastest); the blocks behind them: q_tokens tokens
-// times q_heads query heads.
-template <typename T, int PER> __global__ void __launch_bounds__(kAppThreads) fp8_append_kernel(const Fp8Append a) {
+// Blocks [0, kv_ctas): the keys or the values of one page's tokens of one portion for one key/value head (the portions' pages in order, then heads, keys ahead of values); the
+// blocks behind them: a warp has q_heads query heads of one token, whose turns it makes once.
+// Bound by the bytes of proj, q and the codes: what counts is rows in flight, eight a warp of queries, a CTA's whole page of keys or values.
+template <typename T, int PER> __global__ void __launch_bounds__(256, PER == 8 || PER == 0 ? 2 : 3) fp8_append_kernel(const Fp8Append a) {
     using Row = AppRow<T, PER>;
-    extern __shared__ __align__(16) float app_smem[];
-    __shared__ float tops[2][kAppWarps];
-    __shared__ int info[4];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, ps = a.pages.page_size;
+    extern __shared__ __align__(16) unsigned char app_smem[];
+    __shared__ float tops[8];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5, ps = a.pages.page_size;
     const T* proj = (const T*)a.proj;
     griddep_launch_dependents();
     griddep_wait();
     if ((int)blockIdx.x >= a.kv_ctas) {
-        const int b = blockIdx.x - a.kv_ctas, t0 = (b / a.q_blocks) * a.q_tokens, h0 = (b % a.q_blocks) * a.q_heads, half = a.rot_dims >> 1;
-        const int nt = min(a.q_tokens, a.n_tokens - t0), nh = min(a.q_heads, a.H - h0);
-        float2* table = reinterpret_cast<float2*>(app_smem);
-        for (int i = threadIdx.x; i < nt * half; i += kAppThreads) table[i] = app_turn(a.pos[t0 + i / half], a.inv_freq[i % half]);
-        __syncthreads();
-        constexpr int U = PER ? 4 : 1;      // units whose loads are in flight together
-        for (int u0 = warp * U; u0 < nt * nh; u0 += kAppWarps * U) {
-            Row r[U];
+        const long unit = (long)(blockIdx.x - a.kv_ctas) * nw + warp;
+        const int t = (int)(unit / a.q_blocks), h0 = (int)(unit % a.q_blocks) * a.q_heads, h1 = min(a.H, h0 + a.q_heads);
+        if (t >= a.n_tokens) return;
+        const T* row = proj + (long)t * a.proj_stride + a.q_off;
+        T* out = (T*)a.q_out + (long)t * a.H * a.d;
+        AppTurn<float> turn[Row::N];
+        if constexpr (PER == 0) {
+            Row::turns(a, a.pos[t], turn);
+            for (int h = h0; h < h1; h++) {
+                Row r;
+                r.load(row + (long)h * a.d, a.d);
+                r.prepare(row + (long)h * a.d, a, (const T*)a.q_w, turn);
+                r.store(out + (long)h * a.d, a.d);
+            }
+        } else {
+            constexpr int U = Row::W <= 4 ? 8 : 4;
+            uint32_t w[U][Row::W];
+            auto fetch = [&](int h) {
 #pragma unroll
-            for (int u = 0; u < U; u++)
-                if (u0 + u < nt * nh) r[u].load(proj + (long)(t0 + (u0 + u) / nh) * a.proj_stride + a.q_off + (long)(h0 + (u0 + u) % nh) * a.d, a.d);
+                for (int u = 0; u < U; u++)
+                    if (h + u < h1) Row::fetch(w[u], row + (long)(h + u) * a.d);
+            };
+            fetch(h0);
+            Row::turns(a, a.pos[t], turn);
+            for (int h = h0; h < h1; h += U) {
 #pragma unroll
-            for (int u = 0; u < U; u++)
-                if (u0 + u < nt * nh) {
-                    const int t = (u0 + u) / nh, h = h0 + (u0 + u) % nh;
-                    r[u].prepare(proj + (long)(t0 + t) * a.proj_stride + a.q_off + (long)h * a.d, a, (const T*)a.q_w, [&](int i) { return table[t * half + i]; });
-                    r[u].store((T*)a.q_out + ((long)(t0 + t) * a.H + h) * a.d, a.d);
-                }
+                for (int u = 0; u < U; u++)
+                    if (h + u < h1) {
+                        Row r;
+                        r.unpack(w[u]);
+                        r.prepare(row + (long)(h + u) * a.d, a, (const T*)a.q_w, turn);
+                        r.store(out + (long)(h + u) * a.d, a.d);
+                    }
+                fetch(h + U);
+            }
         }
         return;
     }
-    const int g = blockIdx.x % a.G;
-    if (warp == 0) {
-        int s, item;
-        const bool found = fp8_find(blockIdx.x / a.G, a.n_seqs, [&](int i) {
-            const int start = a.seqs[i], len = a.seqs[a.seqs_stride + i];
-            if (len <= 0 || start < 0 || start > a.n_tokens - len) return 0;
-            const int p = a.pos[start];
-            return p < 0 ? 0 : (p + len - 1) / ps - p / ps + 1;
-        }, s, item);
-        if (lane == 0) {
-            info[0] = -1;
-            if (found) {
-                const int start = a.seqs[s], len = a.seqs[a.seqs_stride + s], p = a.pos[start], logical = p / ps + item;
-                const int first = item ? logical * ps - p : 0, last = min(len, (logical + 1) * ps - p);      // the portion's tokens in this page
-                info[0] = a.pages.page(a.slot[start], logical);
-                info[1] = start + first;
-                info[2] = last - first;
-                info[3] = p + first;
-            }
+    const bool is_v = blockIdx.x & 1;
+    const int g = (blockIdx.x >> 1) % a.G;
+    int s, item, start = 0, len = 0, pos = 0, slot = 0;
+    const bool found = fp8_find((blockIdx.x >> 1) / a.G, a.n_seqs, [&](int i) {
+        start = a.seqs[i];
+        len = a.seqs[a.seqs_stride + i];
+        if (len <= 0 || start < 0 || start > a.n_tokens - len) return 0;
+        pos = a.pos[start];
+        slot = a.slot[start];
+        return pos < 0 ? 0 : (pos + len - 1) / ps - pos / ps + 1;
+    }, s, item);
+    if (!found) return;
+    start = __shfl_sync(0xffffffffu, start, s & 31);
+    len = __shfl_sync(0xffffffffu, len, s & 31);
+    pos = __shfl_sync(0xffffffffu, pos, s & 31);
+    slot = __shfl_sync(0xffffffffu, slot, s & 31);
+    const int logical = pos / ps + item, first = item ? logical * ps - pos : 0, n = min(len, (logical + 1) * ps - pos) - first;      // the portion's tokens in this page
+    const int t0 = start + first, p0 = pos + first, begun = p0 % ps, page = a.pages.page(slot, logical), width = is_v ? a.dv : a.d;
+    const T* rows = proj + (long)t0 * a.proj_stride + (is_v ? a.v_off + (long)g * a.dv : a.k_off + (long)g * a.d);
+    // A warp has rows warp, warp + nw, ..: of a.keep at a time the columns as they came (PER > 0) and, of keys that were turned or normed, the results
+    T* raw = reinterpret_cast<T*>(app_smem);
+    float* done = reinterpret_cast<float*>(app_smem + (PER ? (size_t)a.keep * max(a.d, a.dv) * sizeof(T) : 0));
+    const bool work = !is_v && (a.rot_dims || a.qk_norm), kept = n <= a.keep;
+    float top = 0.f;
+    auto make = [&](int base) {
+        const int end = min(n, base + a.keep);
+        if constexpr (PER > 0) {
+            for (int t = base + warp; t < end; t += nw) Row::bring(raw + (long)(t - base) * width, rows + (long)t * a.proj_stride);
+            asm volatile("cp.async.commit_group;\ncp.async.wait_group 0;" ::: "memory");
         }
-    }
-    __syncthreads();
-    const int page = info[0], t0 = info[1], n = info[2], p0 = info[3], begun = p0 % ps;
+#pragma unroll 1
+        for (int t = base + warp; t < end; t += nw) {
+            Row r;
+            const T* row = rows + (long)t * a.proj_stride;
+            r.load(PER ? raw + (long)(t - base) * width : row, width);
+            if (work) {
+                AppTurn<double> turn[Row::N];
+                if (a.rot_dims) Row::turns(a, p0 + t, turn);
+                r.prepare(row, a, (const T*)a.k_w, turn);
+            }
+            if (work || PER == 0) {
+#pragma unroll
+                for (int e = 0; e < Row::N; e++)
+                    if (PER || Row::col(e) < width) done[(long)(t - base) * width + Row::col(e)] = r.x[e];
+            }
+            top = fmaxf(top, r.top());
+        }
+    };
+    auto codes_of = [&](int base, uint8_t* codes, float inv) {
+        const int end = min(n, base + a.keep);
+        for (int t = base + warp; t < end; t += nw) {
+            Row r;
+            if (work || PER == 0) {
+#pragma unroll
+                for (int e = 0; e < Row::N; e++) r.x[e] = PER || Row::col(e) < width ? done[(long)(t - base) * width + Row::col(e)] : 0.f;
+            } else {
+                r.load(raw + (long)(t - base) * width, width);
+            }
+            r.store_codes(codes + (long)(begun + t) * width, width, inv);
+        }
+    };
+    for (int base = 0; base < n; base += a.keep) make(base);
     if (page < 0) return;
     const long block = (long)page * a.G + g;
-    uint8_t *kc = a.k_codes + block * ps * a.d, *vc = a.v_codes + block * ps * a.dv;
-    const int width = max(a.d, a.dv);
-    const float old_k = begun ? a.scales[2 * block] : 0.f, old_v = begun ? a.scales[2 * block + 1] : 0.f;
-    // rows 0 .. n - 1: keys, n .. 2 n - 1: values
-    auto make = [&](Row& r, int u) {
-        const bool is_v = u >= n;
-        const int t = is_v ? u - n : u;
-        const T* row = proj + (long)(t0 + t) * a.proj_stride + (is_v ? a.v_off + (long)g * a.dv : a.k_off + (long)g * a.d);
-        r.load(row, is_v ? a.dv : a.d);
-        if (!is_v) r.prepare(row, a, (const T*)a.k_w, [&](int i) { return app_turn(p0 + t, a.inv_freq[i]); });
-    };
-    float top_k = 0.f, top_v = 0.f;
-    for (int u = warp; u < 2 * n; u += kAppWarps) {
-        Row r;
-        make(r, u);
-        const float m = r.top(0);
-        if (u >= n) top_v = fmaxf(top_v, m); else top_k = fmaxf(top_k, m);
-        if (a.keep) {
-#pragma unroll
-            for (int e = 0; e < Row::N; e++)
-                if (PER || Row::col(e) < width) app_smem[(long)u * width + Row::col(e)] = r.x[e];
-        }
-    }
-    top_k = warp_max(top_k);
-    top_v = warp_max(top_v);
-    if (lane == 0) { tops[0][warp] = top_k; tops[1][warp] = top_v; }
+    uint8_t* codes = (is_v ? a.v_codes : a.k_codes) + block * ps * width;
+    float* scale = a.scales + 2 * block + is_v;
+    const float old = begun ? *scale : 0.f;
+    top = warp_max(top);
+    if (lane == 0) tops[warp] = top;
     __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kAppWarps; w++) { top_k = fmaxf(top_k, tops[0][w]); top_v = fmaxf(top_v, tops[1][w]); }
-    const float now_k = fmaxf(old_k, fp8_power(fp8_exponent(top_k))), now_v = fmaxf(old_v, fp8_power(fp8_exponent(top_v)));
-    if (threadIdx.x == 0) { a.scales[2 * block] = now_k; a.scales[2 * block + 1] = now_v; }      // (every thread read the old ones ahead of the barrier)
-    if (begun && now_k > old_k) fp8_move(kc, (long)begun * a.d, old_k / now_k);
-    if (begun && now_v > old_v) fp8_move(vc, (long)begun * a.dv, old_v / now_v);
-    const float inv_k = 1.0f / now_k, inv_v = 1.0f / now_v;
-    for (int u = warp; u < 2 * n; u += kAppWarps) {
-        Row r;
-        if (a.keep) {
-#pragma unroll
-            for (int e = 0; e < Row::N; e++) r.x[e] = PER || Row::col(e) < width ? app_smem[(long)u * width + Row::col(e)] : 0.f;
-        } else {
-            make(r, u);
+    for (int w = 0; w < nw; w++) top = fmaxf(top, tops[w]);
+    const float now = fmaxf(old, fp8_power(fp8_exponent(top))), inv = 1.0f / now;
+    if (threadIdx.x == 0) *scale = now;      // (every thread read the old one ahead of the barrier)
+    if (begun && now > old) fp8_move(codes, (long)begun * width, old / now);
+    if (kept) {
+        codes_of(0, codes, inv);
+    } else {
+        for (int base = 0; base < n; base += a.keep) {      // (more rows than the CTA keeps: once more)
+            make(base);
+            codes_of(base, codes, inv);
         }
-        if (u >= n) r.store_codes(vc + (long)(begun + u - n) * a.dv, a.dv, inv_v);
-        else r.store_codes(kc + (long)(begun + u) * a.d, a.d, inv_k);
     }
 }
 
-template <typename T, int PER> static cudaError_t launch_append(const Fp8Append& a, unsigned grid, size_t smem, cudaStream_t s) {
-    const cudaError_t e = raise_smem_limit((const void*)fp8_append_kernel<T, PER>, smem);
-    return e != cudaSuccess ? e : launch_pdl(fp8_append_kernel<T, PER>, dim3(grid), dim3(kAppThreads), smem, s, a);
-}
-template <typename T> static cudaError_t launch_append_of(const Fp8Append& a, int per, unsigned grid, size_t smem, cudaStream_t s) {
-    return per == 2 ? launch_append<T, 2>(a, grid, smem, s) : per == 4 ? launch_append<T, 4>(a, grid, smem, s) : per == 8 ? launch_append<T, 8>(a, grid, smem, s) : launch_append<T, 0>(a, grid, smem, s);
+template <typename T> static cudaError_t launch_append(const Fp8Append& a, int per, unsigned grid, int threads, size_t smem, cudaStream_t s) {
+    const auto kernel = per == 2 ? fp8_append_kernel<T, 2> : per == 4 ? fp8_append_kernel<T, 4> : per == 8 ? fp8_append_kernel<T, 8> : fp8_append_kernel<T, 0>;
+    const cudaError_t e = raise_smem_limit((const void*)kernel, smem);
+    return e != cudaSuccess ? e : launch_pdl(kernel, dim3(grid), dim3(threads), smem, s, a);
 }
 
 }  // namespace ktb
@@ -321,7 +410,7 @@ extern "C" int ktb200_fp8_cache_append(const ktb200_fp8_append_params* c, int n_
     if (!c->proj || !c->pos || !c->slot || !c->seqs || !c->page_table || !c->k_codes || !c->v_codes || !c->scales || !c->q_out) { set_error("fp8_cache_append: null pointer"); return KTB200_EINVAL; }
     Fp8Append a{c->proj, c->proj_stride, c->q_off, c->k_off, c->v_off, c->heads, c->kv_heads, c->dim, c->vdim, c->rot_dims, c->rot_layout, c->inv_freq, c->qk_norm, c->q_weight, c->k_weight, c->eps,
                 c->pos, c->slot, c->seqs, c->seqs_stride, c->n_seqs, n_tokens, {c->page_table, c->n_slots, c->max_pages, c->page_size, c->n_pages}, (uint8_t*)c->k_codes, (uint8_t*)c->v_codes,
-                c->scales, c->q_out, 0, 0, 0, 0, 0};
+                c->scales, c->q_out, 0, 0, 0, 0};
     // a portion of n tokens meets n / page_size + 2 pages at most, and no more than n
     const long pages = c->n_seqs ? std::min<long>(n_tokens, n_tokens / c->page_size + 2L * c->n_seqs) : 0;
     // whole vectors of a lane's columns
@@ -334,20 +423,19 @@ extern "C" int ktb200_fp8_cache_append(const ktb200_fp8_append_params* c, int n_
             (reinterpret_cast<uintptr_t>(c->v_codes) & (per - 1)) || (c->rot_layout == kRotHalves ? (c->rot_dims / 2) % per : 0))
             per = 0;
     }
-    // queries: a token's heads share its table of angles; eight units (one a warp) a CTA until the SMs are full, then four tokens with all their heads
-    const bool many = (long)n_tokens * c->heads > 8 * 148 * 8;
-    a.q_tokens = many ? 4 : 1;
-    a.q_heads = many ? std::min(c->heads, 64) : std::min(c->heads, kAppWarps);
+    // decode steps bring one row to most blocks: two warps a CTA; prompts eight
+    const int threads = (long)n_tokens <= 4L * c->n_seqs ? 64 : 256, nw = threads / 32;
+    // query heads of a warp: as many as leave about 32 warps an SM
+    a.q_heads = (int)std::max<long>(1, std::min<long>({32, c->heads, (long)n_tokens * c->heads / (148 * 32)}));
     a.q_blocks = (c->heads + a.q_heads - 1) / a.q_heads;
-    const long q_ctas = ((long)n_tokens + a.q_tokens - 1) / a.q_tokens * a.q_blocks, kv_ctas = pages * c->kv_heads;
+    const long q_ctas = ((long)n_tokens * a.q_blocks + nw - 1) / nw, kv_ctas = 2 * pages * c->kv_heads;
     if (q_ctas + kv_ctas > 0x7fffffffL) { set_error("fp8_cache_append: too many tokens"); return KTB200_EINVAL; }
     a.kv_ctas = (int)kv_ctas;
-    // a page's rows stay in shared memory between the search for their largest and their codes where they fit
-    const size_t rows = (size_t)2 * std::min(c->page_size, n_tokens) * std::max(c->dim, c->vdim) * sizeof(float);
-    a.keep = rows <= kAppKeep;
-    const size_t smem = std::max(a.keep ? rows : 0, (size_t)a.q_tokens * (c->rot_dims / 2) * sizeof(float2));
-    KTB_CUDA_CHECK(dtype == KTB200_TYPE_BF16 ? launch_append_of<__nv_bfloat16>(a, per, (unsigned)(q_ctas + kv_ctas), smem, (cudaStream_t)stream)
-                                             : launch_append_of<float>(a, per, (unsigned)(q_ctas + kv_ctas), smem, (cudaStream_t)stream));
+    const size_t row_bytes = (size_t)std::max(c->dim, c->vdim) * ((per ? esz : 0) + sizeof(float));
+    a.keep = (int)std::min<size_t>(std::min(c->page_size, n_tokens), kAppKeep / row_bytes);
+    const size_t smem = a.keep * row_bytes;
+    KTB_CUDA_CHECK(dtype == KTB200_TYPE_BF16 ? launch_append<__nv_bfloat16>(a, per, (unsigned)(q_ctas + kv_ctas), threads, smem, (cudaStream_t)stream)
+                                             : launch_append<float>(a, per, (unsigned)(q_ctas + kv_ctas), threads, smem, (cudaStream_t)stream));
     count_launch();
     return KTB200_OK;
 }
