@@ -60,11 +60,11 @@ template <typename F> __device__ __forceinline__ F app_sum(F v) {
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
 }
-__device__ __forceinline__ float app_inv_root(float x) { return 1.0f / sqrtf(x); }
-__device__ __forceinline__ double app_inv_root(double x) { return 1.0 / sqrt(x); }
+__device__ __forceinline__ float app_inv_root(float x) { return rsqrtf(x); }      // (2 ulp; a correctly rounded root and quotient are 20 instructions a row)
+__device__ __forceinline__ double app_inv_root(double x) { return rsqrt(x); }
 
 // One head's columns of one token, as a warp holds them.  PER > 0: heads of 32 PER columns, a lane's PER of them side by side; PER = 0: any size, columns lane, lane + 32, ..
-template <typename T, int PER> struct AppRow {
+template <typename T, int PER, bool HALVES> struct AppRow {
     static constexpr int N = PER ? PER : kAppCols;
     float x[N];
     __device__ __forceinline__ static int col(int e) { const int lane = threadIdx.x & 31; return PER ? lane * PER + e : lane + 32 * e; }
@@ -113,7 +113,7 @@ template <typename T, int PER> struct AppRow {
                 t[e] = {F(1), F(0)};
                 if (c < a.rot_dims) t[e] = app_turn<F>(pos, a.inv_freq[a.rot_layout == kRotHalves ? (c >= half ? c - half : c) : c >> 1]);
             }
-        } else if (a.rot_layout == kRotInterleaved) {
+        } else if constexpr (!HALVES) {
 #pragma unroll
             for (int e = 0; e < N; e += 2) {
                 const int c = col(e);
@@ -139,8 +139,13 @@ template <typename T, int PER> struct AppRow {
             }
         }
     }
-    // norm and turn, in F, then back to fp32
-    template <typename F> __device__ __forceinline__ void prepare(const T* row, const Fp8Append& a, const T* w, const AppTurn<F> (&t)[N]) {
+    // the weights of a lane's columns (qk_norm 3; one elsewhere)
+    __device__ __forceinline__ static void weights(const Fp8Append& a, const T* w, float (&to)[N]) {
+#pragma unroll
+        for (int e = 0; e < N; e++) to[e] = a.qk_norm == 3 && (PER || col(e) < a.d) ? to_f(w[col(e)]) : 1.f;
+    }
+    // norm and turn, in F, then back to fp32 (row, w: what PER = 0 reads its partners from)
+    template <typename F> __device__ __forceinline__ void prepare(const T* row, const Fp8Append& a, const T* w, const float (&wv)[N], const AppTurn<F> (&t)[N]) {
         const int lane = threadIdx.x & 31, half = a.rot_dims >> 1;
         F y[N], inv = F(1);
 #pragma unroll
@@ -151,36 +156,33 @@ template <typename T, int PER> struct AppRow {
             for (int e = 0; e < N; e++) ss = fma(y[e], y[e], ss);
             inv = app_inv_root(app_sum(ss) / (F)a.d + (F)a.eps);
 #pragma unroll
-            for (int e = 0; e < N; e++)
-                if (PER || col(e) < a.d) y[e] = a.qk_norm == 3 ? y[e] * inv * (F)to_f(w[col(e)]) : y[e] * inv;
+            for (int e = 0; e < N; e++) y[e] = y[e] * inv * (F)wv[e];
         }
-        if (a.rot_dims) {
-            if (a.rot_layout == kRotInterleaved && PER) {
+        if constexpr (PER > 0 && !HALVES) {
 #pragma unroll
-                for (int e = 0; e < N; e += 2) {
-                    const F u = y[e], v = y[e + 1];
-                    y[e] = u * t[e].c - v * t[e].s;
-                    y[e + 1] = v * t[e].c + u * t[e].s;
-                }
-            } else if (PER) {      // halves: the partner's lane is half / PER lanes away
-                const int step = half / (PER ? PER : 1);
+            for (int e = 0; e < N; e += 2) {
+                const F u = y[e], v = y[e + 1];
+                y[e] = u * t[e].c - v * t[e].s;
+                y[e + 1] = v * t[e].c + u * t[e].s;
+            }
+        } else if constexpr (PER > 0) {      // halves: the partner's lane is half / PER lanes away; the signs of the sines are in s (columns that do not turn: 0)
+            const int step = half / PER, c = col(0), partner = c >= half ? lane - step : lane + step;
+            const F sign = c >= half ? F(1) : F(-1);
 #pragma unroll
-                for (int e = 0; e < N; e++) {
-                    const int c = col(e);
-                    const F other = __shfl_sync(0xffffffffu, y[e], c >= half ? lane - step : lane + step);
-                    if (c < a.rot_dims) y[e] = c >= half ? y[e] * t[e].c + other * t[e].s : y[e] * t[e].c - other * t[e].s;
-                }
-            } else {
+            for (int e = 0; e < N; e++) {
+                const F other = __shfl_sync(0xffffffffu, y[e], partner);
+                y[e] = y[e] * t[e].c + other * (sign * t[e].s);
+            }
+        } else if (a.rot_dims) {
 #pragma unroll
-                for (int e = 0; e < N; e++) {
-                    const int c = col(e);
-                    if (c < a.rot_dims) {
-                        const int o = rot_partner(c, a.rot_dims, a.rot_layout);
-                        const bool second = a.rot_layout == kRotHalves ? c >= half : (c & 1);
-                        F other = (F)to_f(row[o]) * inv;
-                        if (a.qk_norm == 3) other *= (F)to_f(w[o]);
-                        y[e] = second ? y[e] * t[e].c + other * t[e].s : y[e] * t[e].c - other * t[e].s;
-                    }
+            for (int e = 0; e < N; e++) {
+                const int c = col(e);
+                if (c < a.rot_dims) {
+                    const int o = rot_partner(c, a.rot_dims, a.rot_layout);
+                    const bool second = a.rot_layout == kRotHalves ? c >= half : (c & 1);
+                    F other = (F)to_f(row[o]) * inv;
+                    if (a.qk_norm == 3) other *= (F)to_f(w[o]);
+                    y[e] = second ? y[e] * t[e].c + other * t[e].s : y[e] * t[e].c - other * t[e].s;
                 }
             }
         }
@@ -255,8 +257,8 @@ __device__ __forceinline__ void fp8_move(uint8_t* p, long bytes, float f) {
 // Blocks [0, kv_ctas): the keys or the values of one page's tokens of one portion for one key/value head (the portions' pages in order, then heads, keys ahead of values); the
 // blocks behind them: a warp has q_heads query heads of one token, whose turns it makes once.
 // Bound by the bytes of proj, q and the codes: what counts is rows in flight, eight a warp of queries, a CTA's whole page of keys or values.
-template <typename T, int PER> __global__ void __launch_bounds__(256, PER == 8 || PER == 0 ? 2 : 3) fp8_append_kernel(const Fp8Append a) {
-    using Row = AppRow<T, PER>;
+template <typename T, int PER, bool HALVES> __global__ void __launch_bounds__(256, PER == 8 || PER == 0 ? 2 : 3) fp8_append_kernel(const Fp8Append a) {
+    using Row = AppRow<T, PER, HALVES>;
     extern __shared__ __align__(16) unsigned char app_smem[];
     __shared__ float tops[8];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5, ps = a.pages.page_size;
@@ -269,36 +271,41 @@ template <typename T, int PER> __global__ void __launch_bounds__(256, PER == 8 |
         if (t >= a.n_tokens) return;
         const T* row = proj + (long)t * a.proj_stride + a.q_off;
         T* out = (T*)a.q_out + (long)t * a.H * a.d;
+        row += (long)h0 * a.d;
+        out += (long)h0 * a.d;
+        int left = h1 - h0;
         AppTurn<float> turn[Row::N];
-        if constexpr (PER == 0) {
-            Row::turns(a, a.pos[t], turn);
-            for (int h = h0; h < h1; h++) {
-                Row r;
-                r.load(row + (long)h * a.d, a.d);
-                r.prepare(row + (long)h * a.d, a, (const T*)a.q_w, turn);
-                r.store(out + (long)h * a.d, a.d);
-            }
-        } else {
-            constexpr int U = Row::W <= 4 ? 8 : 4;
-            uint32_t w[U][Row::W];
-            auto fetch = [&](int h) {
+        float wv[Row::N];
+        constexpr int U = PER == 0 ? 1 : Row::W <= 4 ? 8 : 4;
+        uint32_t w[U][Row::W];
+        if constexpr (PER > 0) {
+            if (left >= U) {
 #pragma unroll
-                for (int u = 0; u < U; u++)
-                    if (h + u < h1) Row::fetch(w[u], row + (long)(h + u) * a.d);
-            };
-            fetch(h0);
-            Row::turns(a, a.pos[t], turn);
-            for (int h = h0; h < h1; h += U) {
-#pragma unroll
-                for (int u = 0; u < U; u++)
-                    if (h + u < h1) {
-                        Row r;
-                        r.unpack(w[u]);
-                        r.prepare(row + (long)(h + u) * a.d, a, (const T*)a.q_w, turn);
-                        r.store(out + (long)(h + u) * a.d, a.d);
-                    }
-                fetch(h + U);
+                for (int u = 0; u < U; u++) Row::fetch(w[u], row + u * a.d);
             }
+        }
+        Row::turns(a, a.pos[t], turn);
+        Row::weights(a, (const T*)a.q_w, wv);
+        if constexpr (PER > 0) {
+            while (left >= U) {
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    Row r;
+                    r.unpack(w[u]);
+                    if (left >= U + U) Row::fetch(w[u], row + (U + u) * a.d);
+                    r.prepare(row, a, (const T*)a.q_w, wv, turn);
+                    r.store(out + u * a.d, a.d);
+                }
+                left -= U;
+                row += U * a.d;
+                out += U * a.d;
+            }
+        }
+        for (; left > 0; left--, row += a.d, out += a.d) {
+            Row r;
+            r.load(row, a.d);
+            r.prepare(row, a, (const T*)a.q_w, wv, turn);
+            r.store(out, a.d);
         }
         return;
     }
@@ -325,7 +332,8 @@ template <typename T, int PER> __global__ void __launch_bounds__(256, PER == 8 |
     T* raw = reinterpret_cast<T*>(app_smem);
     float* done = reinterpret_cast<float*>(app_smem + (PER ? (size_t)a.keep * max(a.d, a.dv) * sizeof(T) : 0));
     const bool work = !is_v && (a.rot_dims || a.qk_norm), kept = n <= a.keep;
-    float top = 0.f;
+    float top = 0.f, wv[Row::N];
+    if (work) Row::weights(a, (const T*)a.k_w, wv);
     auto make = [&](int base) {
         const int end = min(n, base + a.keep);
         if constexpr (PER > 0) {
@@ -339,8 +347,8 @@ template <typename T, int PER> __global__ void __launch_bounds__(256, PER == 8 |
             r.load(PER ? raw + (long)(t - base) * width : row, width);
             if (work) {
                 AppTurn<double> turn[Row::N];
-                if (a.rot_dims) Row::turns(a, p0 + t, turn);
-                r.prepare(row, a, (const T*)a.k_w, turn);
+                Row::turns(a, p0 + t, turn);
+                r.prepare(row, a, (const T*)a.k_w, wv, turn);
             }
             if (work || PER == 0) {
 #pragma unroll
@@ -387,7 +395,11 @@ template <typename T, int PER> __global__ void __launch_bounds__(256, PER == 8 |
 }
 
 template <typename T> static cudaError_t launch_append(const Fp8Append& a, int per, unsigned grid, int threads, size_t smem, cudaStream_t s) {
-    const auto kernel = per == 2 ? fp8_append_kernel<T, 2> : per == 4 ? fp8_append_kernel<T, 4> : per == 8 ? fp8_append_kernel<T, 8> : fp8_append_kernel<T, 0>;
+    const bool halves = a.rot_layout == kRotHalves;
+    const auto kernel = per == 2   ? (halves ? fp8_append_kernel<T, 2, true> : fp8_append_kernel<T, 2, false>)
+                        : per == 4 ? (halves ? fp8_append_kernel<T, 4, true> : fp8_append_kernel<T, 4, false>)
+                        : per == 8 ? (halves ? fp8_append_kernel<T, 8, true> : fp8_append_kernel<T, 8, false>)
+                                   : fp8_append_kernel<T, 0, false>;
     const cudaError_t e = raise_smem_limit((const void*)kernel, smem);
     return e != cudaSuccess ? e : launch_pdl(kernel, dim3(grid), dim3(threads), smem, s, a);
 }
@@ -432,7 +444,7 @@ extern "C" int ktb200_fp8_cache_append(const ktb200_fp8_append_params* c, int n_
     if (q_ctas + kv_ctas > 0x7fffffffL) { set_error("fp8_cache_append: too many tokens"); return KTB200_EINVAL; }
     a.kv_ctas = (int)kv_ctas;
     const size_t row_bytes = (size_t)std::max(c->dim, c->vdim) * ((per ? esz : 0) + sizeof(float));
-    a.keep = (int)std::min<size_t>(std::min(c->page_size, n_tokens), kAppKeep / row_bytes);
+    a.keep = (int)std::min<size_t>(threads == 64 ? 8 : std::min(c->page_size, n_tokens), kAppKeep / row_bytes);      // (decode: little shared memory, many CTAs)
     const size_t smem = a.keep * row_bytes;
     KTB_CUDA_CHECK(dtype == KTB200_TYPE_BF16 ? launch_append<__nv_bfloat16>(a, per, (unsigned)(q_ctas + kv_ctas), threads, smem, (cudaStream_t)stream)
                                              : launch_append<float>(a, per, (unsigned)(q_ctas + kv_ctas), threads, smem, (cudaStream_t)stream));
