@@ -55,98 +55,88 @@ template <typename F> __device__ __forceinline__ AppTurn<F> app_turn(int pos, do
     const double u = quarter & 1 ? s : c, v = quarter & 1 ? c : s;      // cos and sin of the angle but for their signs
     return {(F)((quarter + 1) & 2 ? -u : u), (F)(quarter & 2 ? -v : v)};
 }
-template <typename F> __device__ __forceinline__ F app_sum(F v) {
+template <int LANES, typename F> __device__ __forceinline__ F app_sum(F v) {      // over groups of LANES lanes
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    for (int o = LANES / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
 }
 __device__ __forceinline__ float app_inv_root(float x) { return rsqrtf(x); }      // (2 ulp; a correctly rounded root and quotient are 20 instructions a row)
 __device__ __forceinline__ double app_inv_root(double x) { return rsqrt(x); }
 
-// One head's columns of one token, as a warp holds them.  PER > 0: heads of 32 PER columns, a lane's PER of them side by side; PER = 0: any size, columns lane, lane + 32, ..
-template <typename T, int PER, bool HALVES> struct AppRow {
-    static constexpr int N = PER ? PER : kAppCols;
+// One head's columns of one token: LPR lanes have eight each (head sizes 64, 128 and 256), so that a warp has 32 / LPR rows at a time; LPR = 0: any size, the whole warp one row, columns
+// lane, lane + 32, ..  A lane's eight are two runs of four at c0 and c1.  HALVES: a turned lane's runs are rot_dims / 2 apart, so that pairs meet in a lane; every other lane's are
+// side by side.
+template <typename T, int LPR, bool HALVES> struct AppRow {
+    static constexpr int N = kAppCols, PAIRS = LPR ? 4 : N, LANES = LPR ? LPR : 32, ROWS = 32 / LANES, W = LPR ? (int)sizeof(T) : 1;      // W: words of four columns, twice
     float x[N];
-    __device__ __forceinline__ static int col(int e) { const int lane = threadIdx.x & 31; return PER ? lane * PER + e : lane + 32 * e; }
-    static constexpr int W = PER ? PER * (int)sizeof(T) / 4 : 1;      // words of a lane's columns as they are stored
-    __device__ __forceinline__ static void fetch(uint32_t (&w)[W], const T* row) {
-        const void* from = row + col(0);
-        if constexpr (W == 1) w[0] = *reinterpret_cast<const uint32_t*>(from);
-        else if constexpr (W == 2) { const uint2 v = *reinterpret_cast<const uint2*>(from); w[0] = v.x; w[1] = v.y; }
-        else {
-#pragma unroll
-            for (int i = 0; i < W; i += 4) { const uint4 v = reinterpret_cast<const uint4*>(from)[i / 4]; w[i] = v.x; w[i + 1] = v.y; w[i + 2] = v.z; w[i + 3] = v.w; }
+    struct Place { int c0, c1, pair; };      // pair: the first of a lane's four (neighbours or halves), or -1: not turned
+    __device__ __forceinline__ static Place place(const Fp8Append& a, int lane_in_row, bool turned) {
+        const int r = turned ? a.rot_dims : 0;
+        if (HALVES && 8 * lane_in_row < r) return {4 * lane_in_row, r / 2 + 4 * lane_in_row, 4 * lane_in_row};
+        return {8 * lane_in_row, 8 * lane_in_row + 4, 8 * lane_in_row < r ? 4 * lane_in_row : -1};
+    }
+    __device__ __forceinline__ static int col(int e) { return (threadIdx.x & 31) + 32 * e; }      // (LPR = 0)
+    __device__ __forceinline__ static void fetch(uint32_t (&w)[2 * W], const T* row, const Place& p) {
+        if constexpr (W == 2) {
+            const uint2 u = *reinterpret_cast<const uint2*>(row + p.c0), v = *reinterpret_cast<const uint2*>(row + p.c1);
+            w[0] = u.x; w[1] = u.y; w[2] = v.x; w[3] = v.y;
+        } else if constexpr (W == 4) {
+            const uint4 u = *reinterpret_cast<const uint4*>(row + p.c0), v = *reinterpret_cast<const uint4*>(row + p.c1);
+            w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w; w[4] = v.x; w[5] = v.y; w[6] = v.z; w[7] = v.w;
         }
     }
-    __device__ __forceinline__ void unpack(const uint32_t (&w)[W]) {
+    __device__ __forceinline__ void unpack(const uint32_t (&w)[2 * W]) {
+        if constexpr (LPR > 0) {
 #pragma unroll
-        for (int i = 0; i < W; i++) {
-            if constexpr (sizeof(T) == 4) x[i] = __uint_as_float(w[i]);
-            else { x[2 * i] = __uint_as_float(w[i] << 16); x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+            for (int i = 0; i < 2 * W; i++) {
+                if constexpr (sizeof(T) == 4) x[i] = __uint_as_float(w[i]);
+                else { x[2 * i] = __uint_as_float(w[i] << 16); x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+            }
         }
     }
     // a lane's columns on their way to shared memory (the lane reads them there itself)
-    __device__ __forceinline__ static void bring(T* to, const T* row) {
-        constexpr int B = W * 4 < 16 ? W * 4 : 16;
-        const uint32_t dst = (uint32_t)__cvta_generic_to_shared(to + col(0));
-        const char* src = reinterpret_cast<const char*>(row + col(0));
+    __device__ __forceinline__ static void bring(T* to, const T* row, const Place& p) {
+        constexpr int B = 4 * sizeof(T);
 #pragma unroll
-        for (int i = 0; i < W * 4; i += B) asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst + i), "l"(src + i), "n"(B) : "memory");
+        for (int i = 0; i < 2; i++) {
+            const int c = i ? p.c1 : p.c0;
+            asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"((uint32_t)__cvta_generic_to_shared(to + c)), "l"(row + c), "n"(B) : "memory");
+        }
     }
-    __device__ __forceinline__ void load(const T* row, int n) {
-        if constexpr (PER == 0) {
+    __device__ __forceinline__ void load(const T* row, int n, const Place& p) {
+        if constexpr (LPR == 0) {
 #pragma unroll
             for (int e = 0; e < N; e++) x[e] = col(e) < n ? to_f(row[col(e)]) : 0.f;
         } else {
-            uint32_t w[W];
-            fetch(w, row);
+            uint32_t w[2 * W];
+            fetch(w, row, p);
             unpack(w);
         }
     }
-    // The turns of a lane's columns at a position.  Two columns share each: two neighbours of a lane, or (halves) one of this lane and one of its partner, of which each makes half
-    template <typename F> __device__ __forceinline__ static void turns(const Fp8Append& a, int pos, AppTurn<F> (&t)[N]) {
-        const int half = a.rot_dims >> 1, lane = threadIdx.x & 31;
-        if constexpr (PER == 0) {
+    // the turns of a lane's pairs (LPR = 0: of its columns) at a position
+    template <typename F> __device__ __forceinline__ static void turns(const Fp8Append& a, int pos, const Place& p, AppTurn<F> (&t)[PAIRS]) {
+        const int half = a.rot_dims >> 1;
 #pragma unroll
-            for (int e = 0; e < N; e++) {
+        for (int e = 0; e < PAIRS; e++) {
+            t[e] = {F(1), F(0)};
+            if constexpr (LPR > 0) {
+                if (p.pair >= 0) t[e] = app_turn<F>(pos, a.inv_freq[p.pair + e]);
+            } else {
                 const int c = col(e);
-                t[e] = {F(1), F(0)};
                 if (c < a.rot_dims) t[e] = app_turn<F>(pos, a.inv_freq[a.rot_layout == kRotHalves ? (c >= half ? c - half : c) : c >> 1]);
-            }
-        } else if constexpr (!HALVES) {
-#pragma unroll
-            for (int e = 0; e < N; e += 2) {
-                const int c = col(e);
-                t[e] = {F(1), F(0)};
-                if (c < a.rot_dims) t[e] = app_turn<F>(pos, a.inv_freq[c >> 1]);
-                t[e + 1] = t[e];
-            }
-        } else {
-            const int step = half / (PER ? PER : 1);
-            const bool second = col(0) >= half, in = col(0) < a.rot_dims;
-            const int partner = second ? lane - step : lane + step;
-#pragma unroll
-            for (int e = 0; e < N / 2; e++) {
-                AppTurn<F> own{F(1), F(0)};
-                if (in) own = app_turn<F>(pos, a.inv_freq[col(second ? e + N / 2 : e) - (second ? half : 0)]);
-                const AppTurn<F> other{__shfl_sync(0xffffffffu, own.c, partner), __shfl_sync(0xffffffffu, own.s, partner)};
-                t[e] = second && in ? other : own;
-                t[e + N / 2] = second && in ? own : other;
-            }
-            if (!in) {
-#pragma unroll
-                for (int e = 0; e < N; e++) t[e] = {F(1), F(0)};
             }
         }
     }
     // the weights of a lane's columns (qk_norm 3; one elsewhere)
-    __device__ __forceinline__ static void weights(const Fp8Append& a, const T* w, float (&to)[N]) {
+    __device__ __forceinline__ static void weights(const Fp8Append& a, const T* w, const Place& p, float (&to)[N]) {
 #pragma unroll
-        for (int e = 0; e < N; e++) to[e] = a.qk_norm == 3 && (PER || col(e) < a.d) ? to_f(w[col(e)]) : 1.f;
+        for (int e = 0; e < N; e++) {
+            const int c = LPR ? (e < 4 ? p.c0 + e : p.c1 + e - 4) : col(e);
+            to[e] = a.qk_norm == 3 && c < a.d ? to_f(w[c]) : 1.f;
+        }
     }
-    // norm and turn, in F, then back to fp32 (row, w: what PER = 0 reads its partners from)
-    template <typename F> __device__ __forceinline__ void prepare(const T* row, const Fp8Append& a, const T* w, const float (&wv)[N], const AppTurn<F> (&t)[N]) {
-        const int lane = threadIdx.x & 31, half = a.rot_dims >> 1;
+    // norm and turn, in F, then back to fp32 (row, w: what LPR = 0 reads its partners from)
+    template <typename F> __device__ __forceinline__ void prepare(const T* row, const Fp8Append& a, const T* w, const float (&wv)[N], const AppTurn<F> (&t)[PAIRS]) {
         F y[N], inv = F(1);
 #pragma unroll
         for (int e = 0; e < N; e++) y[e] = (F)x[e];
@@ -154,26 +144,20 @@ template <typename T, int PER, bool HALVES> struct AppRow {
             F ss = F(0);
 #pragma unroll
             for (int e = 0; e < N; e++) ss = fma(y[e], y[e], ss);
-            inv = app_inv_root(app_sum(ss) / (F)a.d + (F)a.eps);
+            inv = app_inv_root(app_sum<LANES>(ss) / (F)a.d + (F)a.eps);
 #pragma unroll
             for (int e = 0; e < N; e++) y[e] = y[e] * inv * (F)wv[e];
         }
-        if constexpr (PER > 0 && !HALVES) {
+        if constexpr (LPR > 0) {
 #pragma unroll
-            for (int e = 0; e < N; e += 2) {
-                const F u = y[e], v = y[e + 1];
-                y[e] = u * t[e].c - v * t[e].s;
-                y[e + 1] = v * t[e].c + u * t[e].s;
-            }
-        } else if constexpr (PER > 0) {      // halves: the partner's lane is half / PER lanes away; the signs of the sines are in s (columns that do not turn: 0)
-            const int step = half / PER, c = col(0), partner = c >= half ? lane - step : lane + step;
-            const F sign = c >= half ? F(1) : F(-1);
-#pragma unroll
-            for (int e = 0; e < N; e++) {
-                const F other = __shfl_sync(0xffffffffu, y[e], partner);
-                y[e] = y[e] * t[e].c + other * (sign * t[e].s);
+            for (int i = 0; i < 4; i++) {
+                const int e = HALVES ? i : 2 * i, o = HALVES ? i + 4 : 2 * i + 1;
+                const F u = y[e], v = y[o];
+                y[e] = u * t[i].c - v * t[i].s;
+                y[o] = v * t[i].c + u * t[i].s;
             }
         } else if (a.rot_dims) {
+            const int half = a.rot_dims >> 1;
 #pragma unroll
             for (int e = 0; e < N; e++) {
                 const int c = col(e);
@@ -195,32 +179,37 @@ template <typename T, int PER, bool HALVES> struct AppRow {
         for (int e = 0; e < N; e++) m = fmaxf(m, fabsf(x[e]));      // (columns behind a head's last are zero)
         return m;
     }
-    __device__ __forceinline__ void store(T* row, int n) const {
-        if constexpr (PER == 0) {
+    template <typename D> __device__ __forceinline__ void store(D* row, int n, const Place& p) const {
+        if constexpr (LPR == 0) {
 #pragma unroll
             for (int e = 0; e < N; e++)
-                if (col(e) < n) row[col(e)] = from_f<T>(x[e]);
-        } else if constexpr (PER == 2) {
-            if constexpr (sizeof(T) == 4) *reinterpret_cast<float2*>(row + col(0)) = make_float2(x[0], x[1]);
-            else { const __nv_bfloat162 v = __floats2bfloat162_rn(x[0], x[1]); *reinterpret_cast<__nv_bfloat162*>(row + col(0)) = v; }
+                if (col(e) < n) row[col(e)] = from_f<D>(x[e]);
         } else {
-#pragma unroll
-            for (int e = 0; e < N; e += 4) store4(row + col(e), make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]));
+            store4(row + p.c0, make_float4(x[0], x[1], x[2], x[3]));
+            store4(row + p.c1, make_float4(x[4], x[5], x[6], x[7]));
         }
     }
-    __device__ __forceinline__ void store_codes(uint8_t* row, int n, float inv_scale) const {
-        if constexpr (PER == 0) {
+    __device__ __forceinline__ void load_done(const float* row, int n, const Place& p) {
+        if constexpr (LPR == 0) {
+#pragma unroll
+            for (int e = 0; e < N; e++) x[e] = col(e) < n ? row[col(e)] : 0.f;
+        } else {
+            const float4 u = load4(row + p.c0), v = load4(row + p.c1);
+            x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w; x[4] = v.x; x[5] = v.y; x[6] = v.z; x[7] = v.w;
+        }
+    }
+    __device__ __forceinline__ void store_codes(uint8_t* row, int n, float inv_scale, const Place& p) const {
+        if constexpr (LPR == 0) {
 #pragma unroll
             for (int e = 0; e < N; e++)
                 if (col(e) < n) row[col(e)] = (uint8_t)__nv_cvt_float_to_fp8(x[e] * inv_scale, __NV_SATFINITE, __NV_E4M3);
         } else {
-            uint32_t w[(PER + 3) / 4] = {};
 #pragma unroll
-            for (int e = 0; e < N; e += 2)
-                w[e / 4] |= (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(x[e] * inv_scale, x[e + 1] * inv_scale), __NV_SATFINITE, __NV_E4M3) << (8 * (e & 3));
-            if constexpr (PER == 2) *reinterpret_cast<uint16_t*>(row + col(0)) = (uint16_t)w[0];
-            else if constexpr (PER == 4) *reinterpret_cast<uint32_t*>(row + col(0)) = w[0];
-            else *reinterpret_cast<uint2*>(row + col(0)) = make_uint2(w[0], w[1]);
+            for (int i = 0; i < 2; i++) {
+                const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(x[4 * i] * inv_scale, x[4 * i + 1] * inv_scale), __NV_SATFINITE, __NV_E4M3);
+                const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(x[4 * i + 2] * inv_scale, x[4 * i + 3] * inv_scale), __NV_SATFINITE, __NV_E4M3);
+                *reinterpret_cast<uint32_t*>(row + (i ? p.c1 : p.c0)) = lo | hi << 16;
+            }
         }
     }
 };
@@ -256,56 +245,56 @@ __device__ __forceinline__ void fp8_move(uint8_t* p, long bytes, float f) {
 
 // Blocks [0, kv_ctas): the keys or the values of one page's tokens of one portion for one key/value head (the portions' pages in order, then heads, keys ahead of values); the
 // blocks behind them: a warp has q_heads query heads of one token, whose turns it makes once.
-// Bound by the bytes of proj, q and the codes: what counts is rows in flight, eight a warp of queries, a CTA's whole page of keys or values.
-template <typename T, int PER, bool HALVES> __global__ void __launch_bounds__(256, PER == 8 || PER == 0 ? 2 : 3) fp8_append_kernel(const Fp8Append a) {
-    using Row = AppRow<T, PER, HALVES>;
+// Bound by the bytes of proj, q and the codes: what counts is rows in flight, and instructions a row: two rows of 128 columns a warp and no exchange between lanes but for a norm's sum.
+template <typename T, int LPR, bool HALVES> __global__ void __launch_bounds__(256, LPR == 0 ? 2 : 3) fp8_append_kernel(const Fp8Append a) {
+    using Row = AppRow<T, LPR, HALVES>;
     extern __shared__ __align__(16) unsigned char app_smem[];
     __shared__ float tops[8];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5, ps = a.pages.page_size;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5, ps = a.pages.page_size, sub = lane / Row::LANES, in_row = lane % Row::LANES;
     const T* proj = (const T*)a.proj;
     griddep_launch_dependents();
     griddep_wait();
     if ((int)blockIdx.x >= a.kv_ctas) {
         const long unit = (long)(blockIdx.x - a.kv_ctas) * nw + warp;
-        const int t = (int)(unit / a.q_blocks), h0 = (int)(unit % a.q_blocks) * a.q_heads, h1 = min(a.H, h0 + a.q_heads);
+        const int t = (int)(unit / a.q_blocks), h0 = (int)(unit % a.q_blocks) * a.q_heads, n = min(a.H - h0, a.q_heads);
         if (t >= a.n_tokens) return;
-        const T* row = proj + (long)t * a.proj_stride + a.q_off;
-        T* out = (T*)a.q_out + (long)t * a.H * a.d;
-        row += (long)h0 * a.d;
-        out += (long)h0 * a.d;
-        int left = h1 - h0;
-        AppTurn<float> turn[Row::N];
+        const typename Row::Place p = Row::place(a, in_row, true);
+        const T* row = proj + (long)t * a.proj_stride + a.q_off + (long)h0 * a.d;
+        T* out = (T*)a.q_out + ((long)t * a.H + h0) * a.d;
+        AppTurn<float> turn[Row::PAIRS];
         float wv[Row::N];
-        constexpr int U = PER == 0 ? 1 : Row::W <= 4 ? 8 : 4;
-        uint32_t w[U][Row::W];
-        if constexpr (PER > 0) {
-            if (left >= U) {
+        constexpr int U = LPR == 0 ? 1 : 4, STEP = U * Row::ROWS;      // U groups of a warp's rows on their way at once
+        uint32_t w[U][2 * Row::W];
+        int h = 0;
+        if constexpr (LPR > 0) {
+            if (STEP <= n) {
 #pragma unroll
-                for (int u = 0; u < U; u++) Row::fetch(w[u], row + u * a.d);
+                for (int u = 0; u < U; u++) Row::fetch(w[u], row + (long)(u * Row::ROWS + sub) * a.d, p);
             }
         }
-        Row::turns(a, a.pos[t], turn);
-        Row::weights(a, (const T*)a.q_w, wv);
-        if constexpr (PER > 0) {
-            while (left >= U) {
+        Row::turns(a, a.pos[t], p, turn);
+        Row::weights(a, (const T*)a.q_w, p, wv);
+        if constexpr (LPR > 0) {
+            for (; h + STEP <= n; h += STEP) {
+                const bool more = h + 2 * STEP <= n;
 #pragma unroll
                 for (int u = 0; u < U; u++) {
+                    const long at = (long)(h + u * Row::ROWS + sub) * a.d;
                     Row r;
                     r.unpack(w[u]);
-                    if (left >= U + U) Row::fetch(w[u], row + (U + u) * a.d);
+                    if (more) Row::fetch(w[u], row + at + (long)STEP * a.d, p);
                     r.prepare(row, a, (const T*)a.q_w, wv, turn);
-                    r.store(out + u * a.d, a.d);
+                    r.store(out + at, a.d, p);
                 }
-                left -= U;
-                row += U * a.d;
-                out += U * a.d;
             }
         }
-        for (; left > 0; left--, row += a.d, out += a.d) {
+        for (; h < n; h += Row::ROWS) {
+            const bool mine = h + sub < n;
+            const long at = (long)(mine ? h + sub : h) * a.d;
             Row r;
-            r.load(row, a.d);
-            r.prepare(row, a, (const T*)a.q_w, wv, turn);
-            r.store(out, a.d);
+            r.load(row + at, a.d, p);
+            r.prepare(row + at, a, (const T*)a.q_w, wv, turn);
+            if (mine) r.store(out + at, a.d, p);
         }
         return;
     }
@@ -328,47 +317,43 @@ template <typename T, int PER, bool HALVES> __global__ void __launch_bounds__(25
     const int logical = pos / ps + item, first = item ? logical * ps - pos : 0, n = min(len, (logical + 1) * ps - pos) - first;      // the portion's tokens in this page
     const int t0 = start + first, p0 = pos + first, begun = p0 % ps, page = a.pages.page(slot, logical), width = is_v ? a.dv : a.d;
     const T* rows = proj + (long)t0 * a.proj_stride + (is_v ? a.v_off + (long)g * a.dv : a.k_off + (long)g * a.d);
-    // A warp has rows warp, warp + nw, ..: of a.keep at a time the columns as they came (PER > 0) and, of keys that were turned or normed, the results
-    T* raw = reinterpret_cast<T*>(app_smem);
-    float* done = reinterpret_cast<float*>(app_smem + (PER ? (size_t)a.keep * max(a.d, a.dv) * sizeof(T) : 0));
+    // A warp has groups of its rows, nw groups apart: of a.keep rows at a time the columns as they came (LPR > 0) and, of keys that were turned or normed, the results
     const bool work = !is_v && (a.rot_dims || a.qk_norm), kept = n <= a.keep;
+    const typename Row::Place place = Row::place(a, in_row, work);
+    T* raw = reinterpret_cast<T*>(app_smem);
+    float* done = reinterpret_cast<float*>(app_smem + (LPR ? (size_t)a.keep * a.d * sizeof(T) : 0));
     float top = 0.f, wv[Row::N];
-    if (work) Row::weights(a, (const T*)a.k_w, wv);
+    if (work) Row::weights(a, (const T*)a.k_w, place, wv);
     auto make = [&](int base) {
         const int end = min(n, base + a.keep);
-        if constexpr (PER > 0) {
-            for (int t = base + warp; t < end; t += nw) Row::bring(raw + (long)(t - base) * width, rows + (long)t * a.proj_stride);
+        if constexpr (LPR > 0) {
+            for (int t = base + warp * Row::ROWS + sub; t < end; t += nw * Row::ROWS) Row::bring(raw + (long)(t - base) * width, rows + (long)t * a.proj_stride, place);
             asm volatile("cp.async.commit_group;\ncp.async.wait_group 0;" ::: "memory");
         }
 #pragma unroll 1
-        for (int t = base + warp; t < end; t += nw) {
+        for (int t0 = base + warp * Row::ROWS; t0 < end; t0 += nw * Row::ROWS) {
+            const bool mine = t0 + sub < end;
+            const int t = mine ? t0 + sub : t0;      // (a row that is not there: the group's first once more, whose columns another lane brought)
+            __syncwarp();
             Row r;
             const T* row = rows + (long)t * a.proj_stride;
-            r.load(PER ? raw + (long)(t - base) * width : row, width);
+            r.load(LPR ? raw + (long)(t - base) * width : row, width, place);
             if (work) {
-                AppTurn<double> turn[Row::N];
-                Row::turns(a, p0 + t, turn);
+                AppTurn<double> turn[Row::PAIRS];
+                Row::turns(a, p0 + t, place, turn);
                 r.prepare(row, a, (const T*)a.k_w, wv, turn);
             }
-            if (work || PER == 0) {
-#pragma unroll
-                for (int e = 0; e < Row::N; e++)
-                    if (PER || Row::col(e) < width) done[(long)(t - base) * width + Row::col(e)] = r.x[e];
-            }
+            if ((work || LPR == 0) && mine) r.store(done + (long)(t - base) * width, width, place);
             top = fmaxf(top, r.top());
         }
     };
     auto codes_of = [&](int base, uint8_t* codes, float inv) {
         const int end = min(n, base + a.keep);
-        for (int t = base + warp; t < end; t += nw) {
+        for (int t = base + warp * Row::ROWS + sub; t < end; t += nw * Row::ROWS) {
             Row r;
-            if (work || PER == 0) {
-#pragma unroll
-                for (int e = 0; e < Row::N; e++) r.x[e] = PER || Row::col(e) < width ? done[(long)(t - base) * width + Row::col(e)] : 0.f;
-            } else {
-                r.load(raw + (long)(t - base) * width, width);
-            }
-            r.store_codes(codes + (long)(begun + t) * width, width, inv);
+            if (work || LPR == 0) r.load_done(done + (long)(t - base) * width, width, place);
+            else r.load(raw + (long)(t - base) * width, width, place);
+            r.store_codes(codes + (long)(begun + t) * width, width, inv, place);
         }
     };
     for (int base = 0; base < n; base += a.keep) make(base);
@@ -394,12 +379,12 @@ template <typename T, int PER, bool HALVES> __global__ void __launch_bounds__(25
     }
 }
 
-template <typename T> static cudaError_t launch_append(const Fp8Append& a, int per, unsigned grid, int threads, size_t smem, cudaStream_t s) {
+template <typename T> static cudaError_t launch_append(const Fp8Append& a, int lanes, unsigned grid, int threads, size_t smem, cudaStream_t s) {
     const bool halves = a.rot_layout == kRotHalves;
-    const auto kernel = per == 2   ? (halves ? fp8_append_kernel<T, 2, true> : fp8_append_kernel<T, 2, false>)
-                        : per == 4 ? (halves ? fp8_append_kernel<T, 4, true> : fp8_append_kernel<T, 4, false>)
-                        : per == 8 ? (halves ? fp8_append_kernel<T, 8, true> : fp8_append_kernel<T, 8, false>)
-                                   : fp8_append_kernel<T, 0, false>;
+    const auto kernel = lanes == 8    ? (halves ? fp8_append_kernel<T, 8, true> : fp8_append_kernel<T, 8, false>)
+                        : lanes == 16 ? (halves ? fp8_append_kernel<T, 16, true> : fp8_append_kernel<T, 16, false>)
+                        : lanes == 32 ? (halves ? fp8_append_kernel<T, 32, true> : fp8_append_kernel<T, 32, false>)
+                                      : fp8_append_kernel<T, 0, false>;
     const cudaError_t e = raise_smem_limit((const void*)kernel, smem);
     return e != cudaSuccess ? e : launch_pdl(kernel, dim3(grid), dim3(threads), smem, s, a);
 }
@@ -425,29 +410,27 @@ extern "C" int ktb200_fp8_cache_append(const ktb200_fp8_append_params* c, int n_
                 c->scales, c->q_out, 0, 0, 0, 0};
     // a portion of n tokens meets n / page_size + 2 pages at most, and no more than n
     const long pages = c->n_seqs ? std::min<long>(n_tokens, n_tokens / c->page_size + 2L * c->n_seqs) : 0;
-    // whole vectors of a lane's columns
+    // eight columns a lane, four at a time
     const size_t esz = dtype == KTB200_TYPE_BF16 ? 2 : 4;
-    int per = c->dim == c->vdim && (c->dim == 64 || c->dim == 128 || c->dim == 256) ? c->dim / 32 : 0;
-    if (per) {
-        const size_t lane_bytes = std::min<size_t>(16, per * esz);
-        auto whole = [&](const void* p) { return (reinterpret_cast<uintptr_t>(p) & (lane_bytes - 1)) == 0; };
-        if (c->q_off % per || c->k_off % per || c->v_off % per || c->proj_stride % per || !whole(c->proj) || !whole(c->q_out) || (reinterpret_cast<uintptr_t>(c->k_codes) & (per - 1)) ||
-            (reinterpret_cast<uintptr_t>(c->v_codes) & (per - 1)) || (c->rot_layout == kRotHalves ? (c->rot_dims / 2) % per : 0))
-            per = 0;
+    int lanes = c->dim == c->vdim && (c->dim == 64 || c->dim == 128 || c->dim == 256) && c->rot_dims % 8 == 0 ? c->dim / 8 : 0;
+    if (lanes) {
+        auto whole = [&](const void* p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; };
+        if (c->q_off % 4 || c->k_off % 4 || c->v_off % 4 || c->proj_stride % 4 || !whole(c->proj, 4 * esz) || !whole(c->q_out, 4 * esz) || !whole(c->k_codes, 4) || !whole(c->v_codes, 4)) lanes = 0;
     }
     // decode steps bring one row to most blocks: two warps a CTA; prompts eight
     const int threads = (long)n_tokens <= 4L * c->n_seqs ? 64 : 256, nw = threads / 32;
-    // query heads of a warp: as many as leave about 32 warps an SM
-    a.q_heads = (int)std::max<long>(1, std::min<long>({32, c->heads, (long)n_tokens * c->heads / (148 * 32)}));
+    // query heads of a warp: as many as leave about 32 warps an SM, whole groups of its rows
+    const long group = lanes ? 32 / lanes : 1, want = (long)n_tokens * c->heads / (148 * 32);
+    a.q_heads = (int)std::min<long>(32, std::max(group, want / group * group));
     a.q_blocks = (c->heads + a.q_heads - 1) / a.q_heads;
     const long q_ctas = ((long)n_tokens * a.q_blocks + nw - 1) / nw, kv_ctas = 2 * pages * c->kv_heads;
     if (q_ctas + kv_ctas > 0x7fffffffL) { set_error("fp8_cache_append: too many tokens"); return KTB200_EINVAL; }
     a.kv_ctas = (int)kv_ctas;
-    const size_t row_bytes = (size_t)std::max(c->dim, c->vdim) * ((per ? esz : 0) + sizeof(float));
+    const size_t row_bytes = (size_t)std::max(c->dim, c->vdim) * ((lanes ? esz : 0) + sizeof(float));
     a.keep = (int)std::min<size_t>(threads == 64 ? 8 : std::min(c->page_size, n_tokens), kAppKeep / row_bytes);      // (decode: little shared memory, many CTAs)
     const size_t smem = a.keep * row_bytes;
-    KTB_CUDA_CHECK(dtype == KTB200_TYPE_BF16 ? launch_append<__nv_bfloat16>(a, per, (unsigned)(q_ctas + kv_ctas), threads, smem, (cudaStream_t)stream)
-                                             : launch_append<float>(a, per, (unsigned)(q_ctas + kv_ctas), threads, smem, (cudaStream_t)stream));
+    KTB_CUDA_CHECK(dtype == KTB200_TYPE_BF16 ? launch_append<__nv_bfloat16>(a, lanes, (unsigned)(q_ctas + kv_ctas), threads, smem, (cudaStream_t)stream)
+                                             : launch_append<float>(a, lanes, (unsigned)(q_ctas + kv_ctas), threads, smem, (cudaStream_t)stream));
     count_launch();
     return KTB200_OK;
 }
