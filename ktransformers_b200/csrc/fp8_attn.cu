@@ -246,17 +246,9 @@ static long fp8_range(const ktb200_fp8_attn_params* c, int max_keys, const Fp8Fo
 static long fp8_tiles(const ktb200_fp8_attn_params* c, int n_tokens, int ctoks) { return std::min<long>(n_tokens, (long)c->n_seqs + n_tokens / ctoks); }
 static bool fp8_sizes_ok(const ktb200_fp8_attn_params* c) { return c && c->heads > 0 && c->kv_heads > 0 && c->heads % c->kv_heads == 0; }
 
-extern "C" size_t ktb200_fp8_cache_attn_workspace(const ktb200_fp8_attn_params* c, int n_tokens, int max_keys, int part, int dtype, int allow_tensor_cores) {
-    if (!fp8_sizes_ok(c) || n_tokens <= 0 || part <= 0) return 0;
-    const long parts = (fp8_range(c, max_keys, fp8_form(c, n_tokens, dtype, allow_tensor_cores)) + part - 1) / part;
-    return parts > 1 ? (size_t)n_tokens * c->heads * parts * (c->vdim + 2) * sizeof(float) : 0;
-}
-
 // Keys of a part: the whole range where the CTAs of uncut ranges fill the SMs' places four times; else so many that one round of CTAs covers the range, and
 // between sequences that decode, whose ranges may have any length, no more than 1024
-extern "C" int ktb200_fp8_cache_attn_part(const ktb200_fp8_attn_params* c, int n_tokens, int max_keys, int dtype, int allow_tensor_cores) {
-    if (!fp8_sizes_ok(c) || n_tokens <= 0) return 0;
-    const Fp8Form f = fp8_form(c, n_tokens, dtype, allow_tensor_cores);
+static int fp8_part(const ktb200_fp8_attn_params* c, int n_tokens, int max_keys, const Fp8Form& f) {
     const int R = c->heads / c->kv_heads;
     const long range = fp8_range(c, max_keys, f), places = f.places * 148, ctas = fp8_tiles(c, n_tokens, f.ctoks) * c->kv_heads * ((R + f.heads - 1) / f.heads);
     if (ctas >= 4 * places || range <= 2 * kFp8MinPart) return 0;
@@ -267,6 +259,21 @@ extern "C" int ktb200_fp8_cache_attn_part(const ktb200_fp8_attn_params* c, int n
     return part < range ? (int)part : 0;
 }
 
+extern "C" int ktb200_fp8_cache_attn_part(const ktb200_fp8_attn_params* c, int n_tokens, int max_keys, int dtype, int allow_tensor_cores) {
+    return fp8_sizes_ok(c) && n_tokens > 0 ? fp8_part(c, n_tokens, max_keys, fp8_form(c, n_tokens, dtype, allow_tensor_cores)) : 0;
+}
+
+static size_t fp8_workspace(const ktb200_fp8_attn_params* c, int n_tokens, int max_keys, int part, const Fp8Form& f) {
+    const long parts = part > 0 ? (fp8_range(c, max_keys, f) + part - 1) / part : 1;
+    return parts > 1 ? (size_t)n_tokens * c->heads * parts * (c->vdim + 2) * sizeof(float) : 0;
+}
+
+extern "C" size_t ktb200_fp8_cache_attn_workspace(const ktb200_fp8_attn_params* c, int n_tokens, int max_keys, int part, int dtype, int allow_tensor_cores) {
+    if (!fp8_sizes_ok(c) || n_tokens <= 0) return 0;
+    const Fp8Form f = fp8_form(c, n_tokens, dtype, allow_tensor_cores);
+    return fp8_workspace(c, n_tokens, max_keys, part < 0 ? fp8_part(c, n_tokens, max_keys, f) : part, f);
+}
+
 extern "C" int ktb200_fp8_cache_attn(const ktb200_fp8_attn_params* c, int n_tokens, int max_keys, int part, float* workspace, size_t workspace_bytes, int dtype, int allow_tensor_cores,
                                      void* stream) {
     if (!fp8_sizes_ok(c) || c->dim <= 0 || c->dim > 32 * kFgCols || c->vdim <= 0 || c->vdim > 32 * kFgCols || c->page_size <= 0 || c->max_pages <= 0 || c->n_pages < 0 || c->n_slots <= 0 ||
@@ -275,15 +282,16 @@ extern "C" int ktb200_fp8_cache_attn(const ktb200_fp8_attn_params* c, int n_toke
         return KTB200_EINVAL;
     }
     if (dtype != KTB200_TYPE_BF16 && dtype != KTB200_TYPE_F32) { set_error("fp8_cache_attn: dtype must be bf16 or f32"); return KTB200_EINVAL; }
-    if (part < 0 || part % 128 || max_keys < 0) { set_error("fp8_cache_attn: part %d (a multiple of 128 or 0), max_keys %d", part, max_keys); return KTB200_EINVAL; }
+    if (part < -1 || (part > 0 && part % 128) || max_keys < 0) { set_error("fp8_cache_attn: part %d (a multiple of 128, 0 or -1), max_keys %d", part, max_keys); return KTB200_EINVAL; }
     if (n_tokens <= 0 || c->n_seqs == 0) return KTB200_OK;
     if (!c->q || !c->pos || !c->slot || !c->seqs || !c->page_table || !c->k_codes || !c->v_codes || !c->scales || !c->out) { set_error("fp8_cache_attn: null pointer"); return KTB200_EINVAL; }
     const bool bf16 = dtype == KTB200_TYPE_BF16;
     const int R = c->heads / c->kv_heads;
     const Fp8Form f = fp8_form(c, n_tokens, dtype, allow_tensor_cores);
+    if (part < 0) part = fp8_part(c, n_tokens, max_keys, f);
     const long parts = part ? (fp8_range(c, max_keys, f) + part - 1) / part : 1;
     if (parts > kFp8MaxParts) { set_error("fp8_cache_attn: %ld parts, at most %d", parts, kFp8MaxParts); return KTB200_EINVAL; }
-    const size_t need = ktb200_fp8_cache_attn_workspace(c, n_tokens, max_keys, part, dtype, allow_tensor_cores);
+    const size_t need = fp8_workspace(c, n_tokens, max_keys, part, f);
     if (need && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 7))) { set_error("fp8_cache_attn: workspace missing, too small or not aligned"); return KTB200_EINVAL; }
     if ((long)c->kv_heads * R > 65535 || (long)n_tokens * c->heads > 0x7fffffffL) { set_error("fp8_cache_attn: too many heads or tokens"); return KTB200_EINVAL; }
     const cudaStream_t s = (cudaStream_t)stream;

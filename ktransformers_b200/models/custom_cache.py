@@ -112,9 +112,10 @@ class Fp8CacheLayer:
     __slots__ = ("k", "v", "scales")
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, scales: torch.Tensor):
-        if k.dtype != torch.float8_e4m3fn or v.dtype != torch.float8_e4m3fn or scales.dtype != torch.float32:
+        if not (k.dtype is v.dtype is torch.float8_e4m3fn and scales.dtype is torch.float32):
             raise ValueError("an 8-bit cache layer has float8_e4m3fn codes and float32 scales")
-        if k.dim() != 4 or v.dim() != 4 or k.shape[:3] != v.shape[:3] or tuple(scales.shape) != (k.shape[0], k.shape[1], 2):
+        shape = k.shape
+        if len(shape) != 4 or v.dim() != 4 or shape[:3] != v.shape[:3] or tuple(scales.shape) != (shape[0], shape[1], 2):
             raise ValueError(f"an 8-bit cache layer has k, v [pages, heads, page_size, size] and scales [pages, heads, 2], got {tuple(k.shape)}, {tuple(v.shape)}, {tuple(scales.shape)}")
         if not (k.is_contiguous() and v.is_contiguous() and scales.is_contiguous()):
             raise ValueError("an 8-bit cache layer's tensors have to be contiguous")

@@ -18,7 +18,7 @@ from .. import native
 from ..models.custom_cache import StaticCache
 from ..models.modeling_deepseek_v3 import DeepseekV3Attention, DeepseekV3RMSNorm, DeepseekV3RotaryEmbedding, apply_rotary_pos_emb
 from ..util.utils import InferenceState
-from .base_operator import BaseInjectedModule, device_of
+from .base_operator import BaseInjectedModule, device_of, stream_of
 from .flashinfer_wrapper import MLAWrapper, MLAWrapperSingleton
 
 
@@ -508,32 +508,36 @@ def qkv_prep(proj: torch.Tensor, batch, cache, kv: torch.Tensor, heads: int, kv_
     return q
 
 
+_FP8_ROWS = {torch.bfloat16: native.GGML_BF16, torch.float32: native.GGML_F32}
+
+
 def _fp8_batch(what: str, rows: torch.Tensor, kv, batch, cache, kv_heads: int, dim: int, vdim: int):
-    """Checks what the 8-bit cache's two calls share; the storage type's code and the stream"""
-    k, v = kv.k, kv.v
-    if not rows.is_cuda:
-        raise ValueError(f"{what}: CUDA tensors only")
-    if rows.dtype not in (torch.bfloat16, torch.float32):
-        raise ValueError(f"{what}: bfloat16 or float32 rows, got {rows.dtype}")
-    if k.shape[1] != kv_heads or k.shape[2] != cache.page_size or k.shape[3] != dim or v.shape[3] != vdim:
-        raise ValueError(f"{what}: the cache layer holds pages of {k.shape[2]} tokens of {k.shape[1]} heads of {k.shape[3]} + {v.shape[3]}, the call has {cache.page_size}, {kv_heads}, {dim} + {vdim}")
-    if batch.seqs is None or batch.seqs.dtype != torch.int32 or batch.pos.dtype != torch.int32 or batch.slot.dtype != torch.int32 or cache.page_table.dtype != torch.int32:
+    """Checks what the 8-bit cache's two calls share; their arguments from `pos` to the codes and scales, the storage type's code and the device"""
+    k, v, pos, slot, seqs, table, page_size, dev = kv.k, kv.v, batch.pos, batch.slot, batch.seqs, cache.page_table, cache.page_size, rows.device
+    code, T, n_seqs = _FP8_ROWS.get(rows.dtype), rows.shape[0], batch.n_seqs
+    if code is None or dev.type != "cuda":
+        raise ValueError(f"{what}: CUDA tensors only, bfloat16 or float32 rows; got {rows.dtype} on {dev}")
+    pages, heads, ps, d = k.shape
+    if heads != kv_heads or ps != page_size or d != dim or v.shape[3] != vdim:
+        raise ValueError(f"{what}: the cache layer holds pages of {ps} tokens of {heads} heads of {d} + {v.shape[3]}, the call has {page_size}, {kv_heads}, {dim} + {vdim}")
+    if seqs is None or not (seqs.dtype is pos.dtype is slot.dtype is table.dtype is torch.int32):
         raise ValueError(f"{what}: needs int32 pos, slot, seqs and page table")
-    T, dev = rows.shape[0], rows.device
-    if batch.pos.shape[0] < T or batch.slot.shape[0] < T or batch.n_seqs > batch.seqs.shape[1]:
-        raise ValueError(f"{what}: {T} tokens, but {batch.pos.shape[0]} positions, {batch.slot.shape[0]} slots; {batch.n_seqs} portions of {batch.seqs.shape[1]}")
-    if batch.pos.stride(0) != 1 or batch.slot.stride(0) != 1 or batch.seqs.stride(1) != 1 or cache.page_table.stride(1) != 1 or cache.page_table.stride(0) != cache.max_pages_per_seq:
-        raise ValueError(f"{what}: index rows and page table rows have to be contiguous")
-    if not (k.device == batch.pos.device == batch.slot.device == batch.seqs.device == cache.page_table.device == dev):
+    if pos.shape[0] < T or slot.shape[0] < T or n_seqs > seqs.shape[1]:
+        raise ValueError(f"{what}: {T} tokens, but {pos.shape[0]} positions, {slot.shape[0]} slots; {n_seqs} portions of {seqs.shape[1]}")
+    seqs_stride, columns = seqs.stride(), table.shape[1]
+    if pos.stride(0) != 1 or slot.stride(0) != 1 or seqs_stride[1] != 1 or table.stride() != (columns, 1) or columns != cache.max_pages_per_seq:
+        raise ValueError(f"{what}: index rows and page table rows have to be contiguous, max_pages_per_seq = {cache.max_pages_per_seq} of them")
+    if not (k.device == pos.device == slot.device == seqs.device == table.device == dev):
         raise ValueError(f"{what}: all tensors have to be on one device")
-    return native.GGML_BF16 if rows.dtype == torch.bfloat16 else native.GGML_F32, torch.cuda.current_stream(dev).cuda_stream
+    return (pos.data_ptr(), slot.data_ptr(), seqs.data_ptr(), seqs_stride[0], n_seqs, table.data_ptr(), table.shape[0], columns, page_size, pages, k.data_ptr(), v.data_ptr(),
+            kv.scales.data_ptr()), code, dev
 
 
-def _check_vectors(what: str, dev, **named):
-    """the optional per-head and per-column vectors: (tensor, length, dtype)"""
-    for name, (t, n, dt) in named.items():
-        if t is not None and (t.numel() != n or t.dtype != dt or t.device != dev or not t.is_contiguous()):
-            raise ValueError(f"{what}: {name} has to be {n} contiguous values of {dt} on {dev}")
+def _check_vector(what: str, name: str, t: torch.Tensor, n: int, dtype, dev):
+    """the optional per-head and per-column vectors"""
+    if t.numel() != n or t.dtype is not dtype or t.device != dev or not t.is_contiguous():
+        raise ValueError(f"{what}: {name} has to be {n} contiguous values of {dtype} on {dev}")
+    return t.data_ptr()
 
 
 def fp8_cache_append(proj: torch.Tensor, batch, cache, kv, heads: int, kv_heads: int, dim: int, vdim: int, offsets, rot=None, inv_freq: Optional[torch.Tensor] = None, qk_norm: int = 0,
@@ -542,26 +546,23 @@ def fp8_cache_append(proj: torch.Tensor, batch, cache, kv, heads: int, kv_heads:
     [T, heads, dim] and the layer's codes and scales, one `ktb200_fp8_cache_append` launch (csrc/fp8_cache.cu).  q and k: unit rms per row (qk_norm = 1), or times q_weight /
     k_weight [dim] ahead of the rotation (qk_norm = 3).  A scale belongs to one page and head: tokens appended to a page whose scale they exceed have its earlier codes moved."""
     what = "fp8_cache_append"
-    code, st = _fp8_batch(what, proj, kv, batch, cache, kv_heads, dim, vdim)
-    T, dev, dt = proj.shape[0], proj.device, proj.dtype
-    q_off, k_off, v_off = offsets
+    args, code, dev = _fp8_batch(what, proj, kv, batch, cache, kv_heads, dim, vdim)
+    T, dt, (q_off, k_off, v_off) = proj.shape[0], proj.dtype, offsets
     if proj.dim() != 2 or proj.stride(1) != 1 or min(offsets) < 0 or max(q_off + heads * dim, k_off + kv_heads * dim, v_off + kv_heads * vdim) > proj.shape[1]:
         raise ValueError(f"{what}: rows of proj {tuple(proj.shape)} do not hold q, k and v at {tuple(offsets)}")
-    rot_dims = rot.dims if rot is not None else 0
-    if rot_dims and (inv_freq is None or inv_freq.numel() != rot_dims // 2 or inv_freq.dtype != torch.float64 or inv_freq.device != dev or not inv_freq.is_contiguous()):
-        raise ValueError(f"{what}: inv_freq has to be {rot_dims // 2} contiguous values of torch.float64 on {dev}")
+    rot_dims, layout, freq, qw, kw = 0, 0, None, None, None
+    if rot is not None and rot.dims:
+        if inv_freq is None:
+            raise ValueError(f"{what}: a rotation needs inv_freq")
+        rot_dims, layout, freq = rot.dims, rot.layout_code, _check_vector(what, "inv_freq", inv_freq, rot.dims // 2, torch.float64, dev)
     if qk_norm == 3:
         if q_weight is None or k_weight is None:
             raise ValueError(f"{what}: qk_norm 3 needs both weights")
-        _check_vectors(what, dev, q_weight=(q_weight, dim, dt), k_weight=(k_weight, dim, dt))
-    q = torch.empty((T, heads, dim), dtype=dt, device=dev)
-    table = cache.page_table
-    a = native.Fp8AppendParams(proj.data_ptr(), proj.stride(0), q_off, k_off, v_off, heads, kv_heads, dim, vdim, rot_dims, rot.layout_code if rot_dims else 0,
-                               inv_freq.data_ptr() if rot_dims else None, qk_norm, q_weight.data_ptr() if qk_norm == 3 else None, k_weight.data_ptr() if qk_norm == 3 else None, eps,
-                               batch.pos.data_ptr(), batch.slot.data_ptr(), batch.seqs.data_ptr(), batch.seqs.stride(0), batch.n_seqs, table.data_ptr(), table.shape[0], table.shape[1],
-                               cache.page_size, kv.k.shape[0], kv.k.data_ptr(), kv.v.data_ptr(), kv.scales.data_ptr(), q.data_ptr())
+        qw, kw = _check_vector(what, "q_weight", q_weight, dim, dt, dev), _check_vector(what, "k_weight", k_weight, dim, dt, dev)
+    q = proj.new_empty((T, heads, dim))
+    a = native.Fp8AppendParams(proj.data_ptr(), proj.stride(0), q_off, k_off, v_off, heads, kv_heads, dim, vdim, rot_dims, layout, freq, qk_norm, qw, kw, eps, *args, q.data_ptr())
     with device_of(dev):
-        native.check_seq(native.seq_lib().ktb200_fp8_cache_append(C.byref(a), T, code, st))
+        native.check_seq(native.seq_lib().ktb200_fp8_cache_append(C.byref(a), T, code, stream_of(dev)))
     return q
 
 
@@ -572,26 +573,22 @@ def fp8_cache_attention(q: torch.Tensor, kv, batch, cache, heads: int, kv_heads:
     (`ktb200_fp8_cache_attn`, csrc/fp8_attn.cu): o [T, heads * vdim] of the queries q [T, heads, dim] that `fp8_cache_append` gives, to `out` (a view of any row stride)
     or a new tensor.  Rows of tokens in none of the batch's portions are left as they were (in a new tensor: as they came)."""
     what = "fp8_cache_attention"
-    code, st = _fp8_batch(what, q, kv, batch, cache, kv_heads, dim, vdim)
-    T, dev, dt = q.shape[0], q.device, q.dtype
+    args, code, dev = _fp8_batch(what, q, kv, batch, cache, kv_heads, dim, vdim)
+    T, n_out = q.shape[0], heads * vdim
     if q.numel() != T * heads * dim or not q.is_contiguous():
         raise ValueError(f"{what}: q has to be contiguous [T, {heads}, {dim}], got {tuple(q.shape)}")
-    _check_vectors(what, dev, head_scale=(head_scale, heads, torch.float32), sink=(sink, heads, torch.float32))
+    hs = _check_vector(what, "head_scale", head_scale, heads, torch.float32, dev) if head_scale is not None else None
+    sk = _check_vector(what, "sink", sink, heads, torch.float32, dev) if sink is not None else None
     if out is None:
-        out = torch.empty((T, heads * vdim), dtype=dt, device=dev)
-    elif tuple(out.shape) != (T, heads * vdim) or out.dtype != dt or out.device != dev or out.stride(1) != 1:
-        raise ValueError(f"{what}: out has to be [{T}, {heads * vdim}] of {dt} on {dev}, columns side by side")
-    table, lib = cache.page_table, native.seq_lib()
-    a = native.Fp8AttnParams(q.data_ptr(), heads, kv_heads, dim, vdim, scale, head_scale.data_ptr() if head_scale is not None else None, softcap or 0.0, window or 0, chunk or 0,
-                             sink.data_ptr() if sink is not None else None, out_scale, batch.pos.data_ptr(), batch.slot.data_ptr(), batch.seqs.data_ptr(), batch.seqs.stride(0),
-                             batch.n_seqs, table.data_ptr(), table.shape[0], table.shape[1], cache.page_size, kv.k.shape[0], kv.k.data_ptr(), kv.v.data_ptr(), kv.scales.data_ptr(),
-                             out.data_ptr(), out.stride(0))
+        out = q.new_empty((T, n_out))
+    elif tuple(out.shape) != (T, n_out) or out.dtype is not q.dtype or out.device != dev or out.stride(1) != 1:
+        raise ValueError(f"{what}: out has to be [{T}, {n_out}] of {q.dtype} on {dev}, columns side by side")
+    a = native.Fp8AttnParams(q.data_ptr(), heads, kv_heads, dim, vdim, scale, hs, softcap or 0.0, window or 0, chunk or 0, sk, out_scale, *args, out.data_ptr(), out.stride(0))
+    lib, ref, tc, keys = native.seq_lib(), C.byref(a), int(tensor_cores), batch.max_kv
+    nbytes = lib.ktb200_fp8_cache_attn_workspace(ref, T, keys, -1, code, tc)
+    ws = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
     with device_of(dev):
-        ref, tc, n_keys = C.byref(a), int(tensor_cores), batch.max_kv
-        part = lib.ktb200_fp8_cache_attn_part(ref, T, n_keys, code, tc)
-        nbytes = lib.ktb200_fp8_cache_attn_workspace(ref, T, n_keys, part, code, tc) if part else 0
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-        native.check_seq(lib.ktb200_fp8_cache_attn(ref, T, n_keys, part, ws.data_ptr() if nbytes else None, nbytes, code, tc, st))
+        native.check_seq(lib.ktb200_fp8_cache_attn(ref, T, keys, -1, ws.data_ptr() if nbytes else None, nbytes, code, tc, stream_of(dev)))
     return out
 
 

@@ -13,6 +13,11 @@ from torch import nn
 _HERE = contextlib.nullcontext()
 
 
+def stream_of(dev: torch.device) -> int:
+    """the current stream of a CUDA device as the C-ABI takes it (a fifteenth of the time of torch.cuda.current_stream(dev).cuda_stream, which makes a Stream)"""
+    return torch._C._cuda_getCurrentRawStream(dev.index)
+
+
 def device_of(dev: torch.device):
     """`dev` as the current device: kernels are launched on the current one, whatever their stream's"""
     return _HERE if dev.index is None or dev.index == torch.cuda.current_device() else torch.cuda.device(dev)

@@ -21,7 +21,7 @@ from torch import nn
 from .. import native
 from ..util.custom_gguf import GGML_NAMES, TORCH_TO_GGML_HIDDEN, B200_WEIGHT_TYPES
 from ..util.utils import InferenceState
-from .base_operator import BaseInjectedModule, device_of
+from .base_operator import BaseInjectedModule, device_of, stream_of
 
 _GGML_TO_TORCH = {0: torch.float32, 1: torch.float16, 30: torch.bfloat16}
 
@@ -241,35 +241,36 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
     """y = x W^T + bias with both sides in 8-bit integers: `weight` int8 [out, in] (rows at multiples of 16 bytes) under one fp32 `weight_scale` per output channel, the rows of x (bf16,
     fp16 or fp32) quantised inside the call under one scale per token, max |x| / 127; exact 32-bit integer sums, scaled and rounded once (`ktb200_int8_linear`,
     csrc/int8_linear.cu).  Rows at or behind bsz_tensor[0] are left as they come."""
-    K, N = weight.shape[1], weight.shape[0]
-    if not x.is_cuda:
+    (N, K), dev, shape, hidden = weight.shape, x.device, x.shape, _INT8_HIDDEN.get(x.dtype)
+    if dev.type != "cuda":
         raise ValueError("int8_linear: CUDA tensors only")
-    if x.dtype not in _INT8_HIDDEN or weight.dtype != torch.int8 or x.shape[-1] != K:
+    if hidden is None or weight.dtype is not torch.int8 or shape[-1] != K:
         raise ValueError(f"int8_linear: x [.., {K}] of bfloat16, float16 or float32 and an int8 weight, got {x.dtype} {tuple(x.shape)} and {weight.dtype}")
-    if weight.stride(1) != 1 or weight.stride(0) % 16 or weight.data_ptr() % 16:
+    w_stride, w_ptr = weight.stride(), weight.data_ptr()
+    if w_stride[1] != 1 or w_stride[0] % 16 or w_ptr % 16:
         raise ValueError("int8_linear: weight rows have to begin at multiples of 16 bytes")
-    dev = x.device
-    if weight_scale.dtype != torch.float32 or weight_scale.numel() != N or not weight_scale.is_contiguous():
+    if weight_scale.dtype is not torch.float32 or weight_scale.numel() != N or not weight_scale.is_contiguous():
         raise ValueError(f"int8_linear: weight_scale has to be {N} contiguous float32 values")
-    if bias is not None and (bias.dtype != torch.float32 or bias.numel() != N or not bias.is_contiguous() or bias.device != dev):
+    if bias is not None and (bias.dtype is not torch.float32 or bias.numel() != N or not bias.is_contiguous() or bias.device != dev):
         raise ValueError(f"int8_linear: bias has to be {N} contiguous float32 values on {dev}")
-    if weight.device != dev or weight_scale.device != dev:
+    if not (weight.device == weight_scale.device == dev):
         raise ValueError("int8_linear: all tensors have to be on one device")
-    if bsz_tensor is not None and (bsz_tensor.dtype != torch.int32 or bsz_tensor.device != dev):
+    if bsz_tensor is not None and (bsz_tensor.dtype is not torch.int32 or bsz_tensor.device != dev):
         raise ValueError(f"int8_linear: bsz_tensor has to be int32 on {dev}")
-    x2 = x if x.dim() == 2 else x.reshape(-1, K)
-    if x2.stride(1) != 1 or (x2.shape[0] > 1 and x2.stride(0) < K):
-        x2 = x2.contiguous()
-    T, lib = x2.shape[0], native.lib()
-    y = torch.empty((T, N), dtype=x.dtype, device=dev)
+    x2 = x if len(shape) == 2 else x.reshape(-1, K)
+    T, (x_stride, one) = x2.shape[0], x2.stride()
+    if one != 1 or (T > 1 and x_stride < K):
+        x2, x_stride = x2.contiguous(), K
+    y = x.new_empty((T, N))
     if T:
+        lib = native.lib()
         nbytes = lib.ktb200_int8_linear_workspace(T, K)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        a = native.Int8LinearParams(x2.data_ptr(), max(x2.stride(0), K), weight.data_ptr(), weight.stride(0), weight_scale.data_ptr(), bias.data_ptr() if bias is not None else None, K, N,
-                                    _INT8_HIDDEN[x.dtype], y.data_ptr(), N, bsz_tensor.data_ptr() if bsz_tensor is not None else None)
+        ws = x.new_empty(nbytes, dtype=torch.uint8)
+        a = native.Int8LinearParams(x2.data_ptr(), max(x_stride, K), w_ptr, w_stride[0], weight_scale.data_ptr(), bias.data_ptr() if bias is not None else None, K, N, hidden, y.data_ptr(), N,
+                                    bsz_tensor.data_ptr() if bsz_tensor is not None else None)
         with device_of(dev):
-            native.check(lib.ktb200_int8_linear(C.byref(a), T, ws.data_ptr(), nbytes, torch.cuda.current_stream(dev).cuda_stream))
-    return y if x.dim() == 2 else y.reshape(*x.shape[:-1], N)
+            native.check(lib.ktb200_int8_linear(C.byref(a), T, ws.data_ptr(), nbytes, stream_of(dev)))
+    return y if len(shape) == 2 else y.reshape(*shape[:-1], N)
 
 
 _INT8_HIDDEN = {torch.float32: native.GGML_F32, torch.float16: native.GGML_F16, torch.bfloat16: native.GGML_BF16}

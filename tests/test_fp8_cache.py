@@ -86,7 +86,7 @@ def test_append_refuses_types_and_takes_no_tokens():
 
 
 @pytest.mark.parametrize("bad,call", [(dict(kv_heads=3), {}), (dict(dim=257), {}), (dict(vdim=0), {}), (dict(page_size=0), {}), (dict(window=-1), {}), (dict(chunk=-4), {}), (dict(out_stride=127), {}),
-                                      (dict(q=None), {}), (dict(out=None), {}), (dict(scales=None), {}), ({}, dict(part=-64)), ({}, dict(part=100)), ({}, dict(max_keys=-1)),
+                                      (dict(q=None), {}), (dict(out=None), {}), (dict(scales=None), {}), ({}, dict(part=-128)), ({}, dict(part=100)), ({}, dict(max_keys=-1)),
                                       ({}, dict(part=128, max_keys=128 * 129)), ({}, dict(part=128, max_keys=1000)), ({}, dict(part=128, max_keys=1000, ws=16, n=100)), ({}, dict(dtype=native.GGML_F16))])
 def test_attention_refuses(bad, call):
     a = native.Fp8AttnParams(**{**ATTN_OK, **bad})
