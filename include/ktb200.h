@@ -638,8 +638,8 @@ int ktb200_softmax_attn_prompt_tiles(const ktb200_softmax_attn_params* params, i
  *     scale grows: exactly, but for what becomes subnormal); one that begins at a page's first token starts its blocks anew.  Codes of other rows are left as they were.
  *   ktb200_fp8_cache_attn     out[t * out_stride + h vdim + c] = out_scale * sum_j w_j v_j / (sum_j w_j + exp(sink[h])), w_j = exp(cap(scale head_scale[h] q.k_j)),
  *     with the masks, cap and optional pointers of ktb200_softmax_attn.  A row that sees no key is zero.  max_keys: no sequence has more tokens, this
- *     call's included.  part > 0 (a multiple of 128) cuts longer key ranges into parts of so many, 128 at most (workspace: ktb200_fp8_cache_attn_workspace bytes, of this call
- *     alone); ktb200_fp8_cache_attn_part: the part that such a call should take, and takes where part is -1 (it reads the struct's sizes, counts and pointers' alignment).
+ *     call's included.  part: -1, the library cuts long key ranges among CTAs as it sees fit; 0, it does not; more (a multiple of 128), in parts of so many keys, 128 of them at most.
+ *     workspace: ktb200_fp8_cache_attn_workspace bytes, of this call alone (that function reads the struct's sizes, counts and the pointers' alignment).
  * seqs: rows (first token's row, token count) of the n_seqs portions, seqs_stride apart.  A portion's tokens stand at consecutive positions from pos[first row], in the pages of table row
  * slot[first row] (a ring: page p in column p % max_pages); a sequence has one portion in a call, and windows reach back (max_pages - 1) * page_size positions at most.
  * Rows of tokens in no portion are left as they were, keys in pages outside [0, n_pages) are neither written nor seen.  The stream's device has to be the current one. */
@@ -679,7 +679,6 @@ typedef struct {
     long out_stride;
 } ktb200_fp8_attn_params;
 size_t ktb200_fp8_cache_attn_workspace(const ktb200_fp8_attn_params* params, int n_tokens, int max_keys, int part, int dtype, int allow_tensor_cores);
-int ktb200_fp8_cache_attn_part(const ktb200_fp8_attn_params* params, int n_tokens, int max_keys, int dtype, int allow_tensor_cores);
 int ktb200_fp8_cache_attn(const ktb200_fp8_attn_params* params, int n_tokens, int max_keys, int part, float* workspace, size_t workspace_bytes, int dtype, int allow_tensor_cores, void* stream);
 
 /* Mamba-2 (csrc/ssd.cu): proj rows hold [x heads*vdim | B groups*state_size | C groups*state_size] at xbc_off and one step logit per head at

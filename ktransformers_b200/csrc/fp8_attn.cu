@@ -36,6 +36,7 @@ struct Fp8Attn {
     long out_stride;
     float* partial;      // [T][H][parts][dv + 2]: reference maximum, sum, un-normalised weighted values
     int part, parts;     // keys of a part (0: the range is not cut), and the most parts of a range
+    int even;            // or: into so many parts of about the same length, one cluster's (0: not)
     int ctoks, align;    // tokens of a CTA: their range, from the first visible key of the first of them (rounded down to align) on, is what is cut
 };
 __device__ __forceinline__ int fp8_first_visible(int p, int window, int chunk) {
@@ -228,7 +229,7 @@ struct Fp8Form {
 };
 static Fp8Form fp8_form(const ktb200_fp8_attn_params* c, int n_tokens, int dtype, int allow_tensor_cores) {
     const int R = c->heads / c->kv_heads;
-    if (allow_tensor_cores && fd_takes(c, n_tokens, dtype)) return {Fp8Form::kDecode, {}, 1, fm_heads(R), kFdAlign, 2};
+    if (allow_tensor_cores && fd_takes(c, n_tokens, dtype)) return {Fp8Form::kDecode, {}, 1, fm_heads(R), kFdAlign, 3};
     if (allow_tensor_cores && fp_takes(c, n_tokens, dtype)) return {Fp8Form::kPrompt, {}, 2 * (128 / fm_heads(R)), fm_heads(R), kFpKeys, 1};
     if (allow_tensor_cores && fm_takes(c, dtype)) {
         const FmForm f = fm_form(c, n_tokens);
@@ -246,21 +247,21 @@ static long fp8_range(const ktb200_fp8_attn_params* c, int max_keys, const Fp8Fo
 static long fp8_tiles(const ktb200_fp8_attn_params* c, int n_tokens, int ctoks) { return std::min<long>(n_tokens, (long)c->n_seqs + n_tokens / ctoks); }
 static bool fp8_sizes_ok(const ktb200_fp8_attn_params* c) { return c && c->heads > 0 && c->kv_heads > 0 && c->heads % c->kv_heads == 0; }
 
-// Keys of a part: the whole range where the CTAs of uncut ranges fill the SMs' places four times; else so many that one round of CTAs covers the range, and
-// between sequences that decode, whose ranges may have any length, no more than 1024
-static int fp8_part(const ktb200_fp8_attn_params* c, int n_tokens, int max_keys, const Fp8Form& f) {
+// How a call's ranges are cut: `even` CTAs of a cluster for each, or parts of `part` keys, or (0, 0) not at all.  Not where the CTAs of uncut ranges fill the SMs' places four times.  A
+// cluster where eight CTAs a range fill the places once, or leave them 1024 keys at most: as many as fill the places four times and still have 256 keys each.  Else parts of such a length
+// that one round of CTAs covers the ranges, between sequences that decode (whose ranges may have any length) no more than 2048
+struct Fp8Cut { int even, part; };
+static Fp8Cut fp8_cut(const ktb200_fp8_attn_params* c, int n_tokens, int max_keys, const Fp8Form& f) {
     const int R = c->heads / c->kv_heads;
     const long range = fp8_range(c, max_keys, f), places = f.places * 148, ctas = fp8_tiles(c, n_tokens, f.ctoks) * c->kv_heads * ((R + f.heads - 1) / f.heads);
-    if (ctas >= 4 * places || range <= 2 * kFp8MinPart) return 0;
+    if (ctas >= 4 * places || range <= 2 * kFp8MinPart) return {0, 0};
+    if (f.kernel == Fp8Form::kDecode && (ctas * kFdCluster >= places || range <= 1024 * kFdCluster))
+        return {(int)std::min<long>({kFdCluster, (4 * places + ctas - 1) / ctas, (range + kFp8MinPart - 1) / kFp8MinPart}), 0};
     long part = (range * ctas + places - 1) / places;
-    if (c->n_seqs > 1 && f.kernel != Fp8Form::kPrompt) part = std::min<long>(part, 1024);
+    if (c->n_seqs > 1 && f.kernel != Fp8Form::kPrompt) part = std::min<long>(part, 2048);
     part = std::max<long>({part, kFp8MinPart, (range + kFp8MaxParts - 1) / kFp8MaxParts});
     part = (part + 127) / 128 * 128;
-    return part < range ? (int)part : 0;
-}
-
-extern "C" int ktb200_fp8_cache_attn_part(const ktb200_fp8_attn_params* c, int n_tokens, int max_keys, int dtype, int allow_tensor_cores) {
-    return fp8_sizes_ok(c) && n_tokens > 0 ? fp8_part(c, n_tokens, max_keys, fp8_form(c, n_tokens, dtype, allow_tensor_cores)) : 0;
+    return {0, part < range ? (int)part : 0};
 }
 
 static size_t fp8_workspace(const ktb200_fp8_attn_params* c, int n_tokens, int max_keys, int part, const Fp8Form& f) {
@@ -271,7 +272,7 @@ static size_t fp8_workspace(const ktb200_fp8_attn_params* c, int n_tokens, int m
 extern "C" size_t ktb200_fp8_cache_attn_workspace(const ktb200_fp8_attn_params* c, int n_tokens, int max_keys, int part, int dtype, int allow_tensor_cores) {
     if (!fp8_sizes_ok(c) || n_tokens <= 0) return 0;
     const Fp8Form f = fp8_form(c, n_tokens, dtype, allow_tensor_cores);
-    return fp8_workspace(c, n_tokens, max_keys, part < 0 ? fp8_part(c, n_tokens, max_keys, f) : part, f);
+    return fp8_workspace(c, n_tokens, max_keys, part < 0 ? fp8_cut(c, n_tokens, max_keys, f).part : part, f);
 }
 
 extern "C" int ktb200_fp8_cache_attn(const ktb200_fp8_attn_params* c, int n_tokens, int max_keys, int part, float* workspace, size_t workspace_bytes, int dtype, int allow_tensor_cores,
@@ -288,7 +289,8 @@ extern "C" int ktb200_fp8_cache_attn(const ktb200_fp8_attn_params* c, int n_toke
     const bool bf16 = dtype == KTB200_TYPE_BF16;
     const int R = c->heads / c->kv_heads;
     const Fp8Form f = fp8_form(c, n_tokens, dtype, allow_tensor_cores);
-    if (part < 0) part = fp8_part(c, n_tokens, max_keys, f);
+    const Fp8Cut own = part < 0 ? fp8_cut(c, n_tokens, max_keys, f) : Fp8Cut{0, part};
+    part = own.part;
     const long parts = part ? (fp8_range(c, max_keys, f) + part - 1) / part : 1;
     if (parts > kFp8MaxParts) { set_error("fp8_cache_attn: %ld parts, at most %d", parts, kFp8MaxParts); return KTB200_EINVAL; }
     const size_t need = fp8_workspace(c, n_tokens, max_keys, part, f);
@@ -297,8 +299,8 @@ extern "C" int ktb200_fp8_cache_attn(const ktb200_fp8_attn_params* c, int n_toke
     const cudaStream_t s = (cudaStream_t)stream;
     const Fp8Attn a{c->q, c->heads, c->kv_heads, c->dim, c->vdim, c->scale, c->head_scale, c->softcap, c->window, c->chunk, c->sink, c->out_scale, c->pos, c->slot, c->seqs, c->seqs_stride,
                     c->n_seqs, n_tokens, {c->page_table, c->n_slots, c->max_pages, c->page_size, c->n_pages}, (const uint8_t*)c->k_codes, (const uint8_t*)c->v_codes, c->scales, c->out,
-                    c->out_stride, workspace, parts > 1 ? part : 0, (int)parts, f.ctoks, f.align};
-    const dim3 grid((unsigned)fp8_tiles(c, n_tokens, f.ctoks), c->kv_heads * ((R + f.heads - 1) / f.heads), (unsigned)parts);
+                    c->out_stride, workspace, parts > 1 ? part : 0, (int)parts, own.even > 1 ? own.even : 0, f.ctoks, f.align};
+    const dim3 grid((unsigned)fp8_tiles(c, n_tokens, f.ctoks), c->kv_heads * ((R + f.heads - 1) / f.heads), own.even > 1 ? (unsigned)own.even : (unsigned)parts);
     if (f.kernel == Fp8Form::kDecode) {
         const int rc = fd_launch(a, f.heads, grid, s);
         if (rc) return rc;

@@ -8,11 +8,14 @@
 //   weights   p = 2^(t - m), t = s log2(e) + log2(value scale): 2^-8 of a weight off at most (as a bf16 weight is) and 2^-21 of the largest where that is more.  Value scales are
 //             powers of two: in the exponent they cost nothing and O needs none.  m is 7 below a head's largest t, raised when a t outgrows it by 8.75 (2^8.75 < 448)
 // l += p / (value scale), O / l is the result: 2^m drops out.
-//     warp 0      TMA: K and V tiles, three stages; a tile is runs of 16, 32 or 64 keys, each inside one page (runs that no key of the part lies in come as zeros)
+//     warp 0      TMA: K and V tiles, two stages; a tile is runs of 16, 32 or 64 keys, each inside one page (runs that no key of the part lies in come as zeros)
 //     warp 1      MMAs: S of the next tile ahead of PV of this one
 //     warps 2-5   a thread owns a key: its scores of all heads are one row of S^T, so that scales and masks are its own; maxima are only needed when one has outgrown its
 //                 reference, which one barrier with a reduction tells.  At the end a thread owns a column of the result
-// TMEM: [S | S | O], N columns each.  Bound by the cache's bytes: a tile is 32 KB, 740 ns of an SM's share of the memory; two CTAs an SM.
+// A range that is cut for up to eight CTAs is cut evenly, sequence by sequence, and its CTAs are a cluster: each leaves its sums in its shared memory and joins some of the heads from
+// all of them, so that there is neither a workspace nor a second launch.  Longer ranges of few sequences go in parts of one length, joined by fp8_merge_kernel.
+// TMEM: [S | S | O], N columns each.  Bound by the cache's bytes: a tile is 32 KB, 740 ns of an SM's share of the memory; three CTAs an SM (two for 16 heads), so that what a CTA
+// spends ahead of its first tile and between a tile's steps is another's time.
 #pragma once
 #include <cuda.h>
 
@@ -20,7 +23,7 @@
 
 namespace ktb {
 
-constexpr int kFdThreads = 192, kFdKeys = 128, kFdTile = kFdKeys * 128, kFdStages = 3, kFdAlign = 64;
+constexpr int kFdThreads = 192, kFdKeys = 128, kFdTile = kFdKeys * 128, kFdStages = 2, kFdAlign = 64;
 constexpr float kFdTop = 7.f, kFdRaise = 8.75f;
 struct FdMisc {
     unsigned long long k_full[kFdStages], k_free[kFdStages], v_full[kFdStages], v_free[kFdStages], s_full[2], s_free[2], p_full[2], p_free[2], q_ready;
@@ -31,6 +34,16 @@ struct FdMisc {
 template <int RP> constexpr int fd_smem() { return 2 * kFdStages * kFdTile + 3 * 2 * RP * 128 + (int)sizeof(FdMisc) + 1024; }
 
 struct FdMaps { CUtensorMap k, v; };
+constexpr int kFdCluster = 8;
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ float cluster_load(uint32_t addr, uint32_t rank) {      // a word of another CTA's shared memory
+    uint32_t at;
+    float v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(addr), "r"(rank));
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+    return v;
+}
 
 // Where the byte of key (column) c of row n of a K-major operand with 128-byte rows and 128-byte swizzle lies
 __device__ __forceinline__ uint32_t fd_at(int n, int c) { return (uint32_t)((n >> 3) * 1024 + (n & 7) * 128 + ((((c >> 4) ^ n) & 7) << 4) + (c & 15)); }
@@ -41,7 +54,7 @@ __device__ __forceinline__ bool fd_any(bool p) {      // over the four soft-max 
 }
 __device__ __forceinline__ void fd_sync() { asm volatile("barrier.cta.sync 1, 128;" ::: "memory"); }
 
-template <int RP> __global__ void __launch_bounds__(kFdThreads, 2) fp8_attn_decode_kernel(const __grid_constant__ FdMaps maps, const Fp8Attn a, int RH, int run) {
+template <int RP> __global__ void __launch_bounds__(kFdThreads, RP == 8 ? 3 : 2) fp8_attn_decode_kernel(const __grid_constant__ FdMaps maps, const Fp8Attn a, int RH, int run) {
     using namespace umma;
     constexpr int N = 2 * RP, OP = N * 128;      // bytes of an operand of N rows
     extern __shared__ __align__(16) uint8_t fd_smem_raw[];
@@ -66,9 +79,19 @@ template <int RP> __global__ void __launch_bounds__(kFdThreads, 2) fp8_attn_deco
     if (misc.info[1] <= 0) return;
     const int g = blockIdx.y / hblocks, h0 = g * R + (blockIdx.y % hblocks) * RH;
     const int lo = fp8_first_visible(p, a.window, a.chunk), lo_al = lo & ~(kFdAlign - 1);
-    const bool cut = a.part > 0 && p + 1 - lo_al > a.part;
-    const int k_lo = lo_al + blockIdx.z * a.part, k_hi = cut ? min(p + 1, k_lo + a.part) : p + 1;
-    if (k_lo >= k_hi) return;
+    const int even = a.even, part = even ? ((p + 1 - lo_al + kFdKeys - 1) / kFdKeys + even - 1) / even * kFdKeys : a.part;
+    const bool cut = !even && part > 0 && p + 1 - lo_al > part;
+    const int k_lo = lo_al + blockIdx.z * part, k_hi = cut || even ? min(p + 1, k_lo + part) : p + 1;
+    float* join = reinterpret_cast<float*>(smem);      // a cluster's CTA: (reference, sum) of RP heads, then RP rows of 128 columns, over the ring
+    if (k_lo >= k_hi) {
+        if (even) {      // nothing to add: the cluster's barriers only
+            cluster_arrive();
+            cluster_wait();
+            cluster_arrive();
+            cluster_wait();
+        }
+        return;
+    }
     const int tiles = (k_hi - k_lo + kFdKeys - 1) / kFdKeys;
     if (warp == 1) tmem_alloc(smem_u32(&misc.tmem_base), 128);
     tc_fence_before();
@@ -276,7 +299,10 @@ template <int RP> __global__ void __launch_bounds__(kFdThreads, 2) fp8_attn_deco
             if (h >= RH) break;
             float sum = (misc.red[0][h] + misc.red[1][h]) + (misc.red[2][h] + misc.red[3][h]), v = fmaf(__uint_as_float(o[RP + h]), 0.0625f, __uint_as_float(o[h]));
             const long row = (long)t * a.H + h0 + h;
-            if (cut) {
+            if (even) {
+                if (r == 0) { join[2 * h] = m[h]; join[2 * h + 1] = sum; }
+                join[2 * RP + 128 * h + r] = v;
+            } else if (cut) {
                 float* part = a.partial + (row * a.parts + blockIdx.z) * 130;
                 if (r == 0) { part[0] = m[h]; part[1] = sum; }
                 part[2 + r] = v;
@@ -292,7 +318,40 @@ template <int RP> __global__ void __launch_bounds__(kFdThreads, 2) fp8_attn_deco
         }
     }
     tc_fence_before();
-    __syncthreads();
+    if (even) {
+        __syncwarp();
+        cluster_arrive();
+        cluster_wait();
+        if (warp >= 2) {
+            const int c = tid - 64, cuts = (p + 1 - lo_al + part - 1) / part;      // the CTAs that have keys
+            for (int h = blockIdx.z; h < RH; h += cuts) {
+                float mk[kFdCluster], lk[kFdCluster], vk[kFdCluster], top = a.sink ? a.sink[h0 + h] * kLog2e : -INFINITY;
+#pragma unroll
+                for (int k = 0; k < kFdCluster; k++)
+                    if (k < cuts) {
+                        mk[k] = cluster_load(base + 8 * h, k);
+                        lk[k] = cluster_load(base + 8 * h + 4, k);
+                        vk[k] = mk[k] > -INFINITY ? cluster_load(base + 8 * RP + 512 * h + 4 * c, k) : 0.f;
+                        top = fmaxf(top, mk[k]);
+                    }
+                float sum = a.sink ? exp2_approx(a.sink[h0 + h] * kLog2e - top) : 0.f, v = 0.f;
+#pragma unroll
+                for (int k = 0; k < kFdCluster; k++)
+                    if (k < cuts) {
+                        const float w = mk[k] > -INFINITY ? exp2_approx(mk[k] - top) : lk[k];      // (nothing seen: 0; scores of NaN have a sum of NaN and no reference)
+                        sum = fmaf(lk[k], mk[k] > -INFINITY ? w : 1.f, sum);
+                        v = fmaf(vk[k], w, v);
+                    }
+                v = sum > 0.f || sum != sum ? v * (a.out_scale / sum) : 0.f;
+                ((__nv_bfloat16*)a.out)[(long)t * a.out_stride + (long)(h0 + h) * 128 + c] = __float2bfloat16_rn(v);
+            }
+        }
+        __syncwarp();
+        cluster_arrive();      // nobody leaves while its shared memory is read
+        cluster_wait();
+    } else {
+        __syncthreads();
+    }
     if (warp == 1) {
         tc_fence_after();
         tmem_dealloc(tmem, 128);
@@ -306,7 +365,22 @@ static bool fd_takes(const ktb200_fp8_attn_params* c, int n_tokens, int dtype) {
 }
 template <int RP> static cudaError_t fd_launch_as(const FdMaps& maps, const Fp8Attn& a, int RH, int run, dim3 grid, cudaStream_t s) {
     const cudaError_t e = raise_smem_limit((const void*)fp8_attn_decode_kernel<RP>, fd_smem<RP>());
-    return e != cudaSuccess ? e : launch_pdl(fp8_attn_decode_kernel<RP>, grid, dim3(kFdThreads), (size_t)fd_smem<RP>(), s, maps, a, RH, run);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t lc{};
+    lc.gridDim = grid; lc.blockDim = dim3(kFdThreads); lc.dynamicSmemBytes = fd_smem<RP>(); lc.stream = s;
+    cudaLaunchAttribute at[2];
+    int n = 0;
+    if (pdl_enabled()) {
+        at[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        at[n++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    if (a.even) {
+        at[n].id = cudaLaunchAttributeClusterDimension;
+        at[n].val.clusterDim.x = 1; at[n].val.clusterDim.y = 1; at[n++].val.clusterDim.z = a.even;
+    }
+    lc.attrs = at;
+    lc.numAttrs = n;
+    return cudaLaunchKernelEx(&lc, fp8_attn_decode_kernel<RP>, maps, a, RH, run);
 }
 // the codes as rows of 128 bytes, boxes of `run` rows
 static int fd_maps(FdMaps& maps, const Fp8Attn& a, int run, CUtensorMapSwizzle swizzle) {

@@ -229,7 +229,6 @@ SEQ_SYMBOLS = {
     # csrc/fp8_cache.cu, csrc/fp8_attn.cu
     "ktb200_fp8_cache_append": (_I, [C.POINTER(Fp8AppendParams), _I, _I, _VP]),
     "ktb200_fp8_cache_attn_workspace": (C.c_size_t, [C.POINTER(Fp8AttnParams), _I, _I, _I, _I, _I]),
-    "ktb200_fp8_cache_attn_part": (_I, [C.POINTER(Fp8AttnParams), _I, _I, _I, _I]),
     "ktb200_fp8_cache_attn": (_I, [C.POINTER(Fp8AttnParams), _I, _I, _I, _VP, C.c_size_t, _I, _I, _VP]),
     # csrc/retention.cu, csrc/selective_scan.cu
     "ktb200_turn_table": (_I, [_VP, _VP, _I, _VP, _I, _VP]),

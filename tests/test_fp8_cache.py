@@ -103,16 +103,14 @@ def test_attention_takes_no_tokens():
 @pytest.mark.parametrize("dtype", [native.GGML_BF16, native.GGML_F32])
 @pytest.mark.parametrize("heads,kv_heads", [(64, 8), (16, 2), (7, 7), (17, 1), (64, 1)])
 @pytest.mark.parametrize("n_seqs,n_tokens", [(1, 1), (3, 3), (200, 200), (2, 50), (1, 3000)])
-def test_attention_parts_cover_any_range(n_seqs, n_tokens, heads, kv_heads, dtype):
+def test_attention_parts_of_any_range_are_few(n_seqs, n_tokens, heads, kv_heads, dtype):
     lib = native.seq_lib()
     for window, chunk in ((0, 0), (700, 0), (0, 4096)):
         a = native.Fp8AttnParams(**{**ATTN_OK, **dict(heads=heads, kv_heads=kv_heads, n_seqs=n_seqs, window=window, chunk=chunk)})
         for keys in (1, 300, 5000, 131072, 1 << 24, 2 ** 31 - 1):
-            part = lib.ktb200_fp8_cache_attn_part(C.byref(a), n_tokens, keys, dtype, 1)
-            need = lib.ktb200_fp8_cache_attn_workspace(C.byref(a), n_tokens, keys, part, dtype, 1)
-            assert part >= 0 and part % 128 == 0 and (need == 0) == (part == 0)
-            parts = need // (n_tokens * heads * 34 * 4)
-            assert parts <= 128 and (part == 0 or parts * part >= min([keys] + [x for x in (window, chunk) if x]))
+            need = lib.ktb200_fp8_cache_attn_workspace(C.byref(a), n_tokens, keys, -1, dtype, 1)
+            assert need % (n_tokens * heads * 34 * 4) == 0 and need // (n_tokens * heads * 34 * 4) <= 128
+            assert lib.ktb200_fp8_cache_attn_workspace(C.byref(a), n_tokens, keys, 0, dtype, 1) == 0
 
 
 # ------------------------------------------------------------------------------------------------------------------------- append
@@ -273,6 +271,8 @@ SHAPES = [
     ([(2000, 20)], 64, 16, 1, 128, 128),                              # a short portion over a range that is cut
     ([(9, 150), (0, 64)], 128, 2, 2, 128, 128),
     ([(500, 1), (3, 1), (129, 1)], 16, 12, 2, 128, 128),
+    ([(1400, 1), (900, 1), (0, 1), (300, 1), (511, 1)], 64, 4, 2, 128, 128),
+    ([(9000, 1)], 64, 2, 1, 128, 128),
     ([(500, 1), (3, 1)], 48, 34, 2, 128, 128),                        # a group that no run of 16 heads divides
 ]
 
@@ -322,6 +322,27 @@ def test_attention_does_not_see_pages_that_are_not_there(dtype):
         t[0, 1], t[1, 0] = total, -3
     run_attention([(100, 2), (0, 3), (60, 40)], 16, 4, 2, 64, 64, dtype, seed=10, break_table=break_table)      # (the second sequence sees nothing at all: zeros)
     run_attention([(1200, 1)], 64, 4, 2, 128, 128, dtype, seed=10, break_table=lambda t, total: t.__setitem__((0, 3), -1))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d,lens", [(128, [(1500, 1), (300, 1)]), (64, [(1500, 1), (300, 1)]), (128, [(700, 40), (0, 90)])])
+def test_attention_cut_and_uncut_agree(d, lens):
+    """the caller's parts, the library's own cut, and none"""
+    H, G, lib = 8, 2, native.seq_lib()
+    batch, cache, total = U.batch_of(lens, 64, seed=2)
+    batch, cache, T = on(batch), on(cache), batch.pos.shape[0]
+    kv = Fp8CacheLayer(*(x.cuda() for x in filled(total, G, 64, d, d, 2)))
+    q, outs = torch.randn((T, H, d), generator=torch.Generator().manual_seed(2)).bfloat16().cuda(), []
+    for part in (-1, 0, 128, 384, 1024):
+        out = torch.zeros((T, H * d), dtype=torch.bfloat16, device="cuda")
+        a = native.Fp8AttnParams(q.data_ptr(), H, G, d, d, d ** -0.5, None, 0.0, 0, 0, None, 1.0, batch.pos.data_ptr(), batch.slot.data_ptr(), batch.seqs.data_ptr(), batch.seqs.stride(0), batch.n_seqs,
+                                 cache.page_table.data_ptr(), cache.page_table.shape[0], cache.page_table.shape[1], 64, total, kv.k.data_ptr(), kv.v.data_ptr(), kv.scales.data_ptr(), out.data_ptr(), H * d)
+        n = lib.ktb200_fp8_cache_attn_workspace(C.byref(a), T, batch.max_kv, part, native.GGML_BF16, 1)
+        ws = torch.empty(n, dtype=torch.uint8, device="cuda")
+        native.check_seq(lib.ktb200_fp8_cache_attn(C.byref(a), T, batch.max_kv, part, ws.data_ptr() if n else None, n, native.GGML_BF16, 1, torch.cuda.current_stream().cuda_stream))
+        outs.append(out.float())
+    # weights and results round to 8 bits on either way (2^-8 of a value each)
+    assert all(((o - outs[1]).abs() <= 2.0 ** -7 * outs[1].abs() + 2.0 ** -8 * float(kv.dequantize()[1].abs().max())).all() for o in outs) and outs[1].abs().max() > 0
 
 
 @pytest.mark.gpu
