@@ -166,22 +166,24 @@ template <typename T> __global__ void __launch_bounds__(256) fp8_attn_kernel(con
         if (lane + 32 * c < dv) out[lane + 32 * c] = from_f<T>(acc[c] * inv);
 }
 
-// The parts of a cut key range, one CTA of 128 threads for each (token, head): the parts' weights once in shared memory (a part without a key has maximum -inf and weighs
-// nothing; the sink joins the sum), then the columns side by side, parts in order.  `unit`: what turns a difference of maxima into a power of two.
-template <typename T> __global__ void __launch_bounds__(128) fp8_merge_kernel(const Fp8Attn a, float unit) {
-    __shared__ float wgt[kFp8MaxParts], red[4];
+// The parts of a cut key range, one CTA for each (token, head): the parts' weights once in shared memory (a part without a key has maximum -inf and weighs nothing; the sink joins
+// the sum), then 128 columns side by side and the parts dealt among kMergeGroups groups of threads, so that the loads of a long range's parts are all under way at once; the groups' sums are
+// added in order.  `unit`: what turns a difference of maxima into a power of two.
+constexpr int kMergeGroups = 4;
+template <typename T> __global__ void __launch_bounds__(128 * kMergeGroups) fp8_merge_kernel(const Fp8Attn a, float unit) {
+    __shared__ float wgt[kFp8MaxParts], red[4], sums[kMergeGroups][128];
     __shared__ int count;
-    griddep_launch_dependents();
-    griddep_wait();
     const long row = blockIdx.x;
-    const int t = (int)(row / a.H), h = (int)(row % a.H), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, dv = a.dv;
-    // the parts of the range that the token's CTA was cut by (none: a token of no portion, or a range in one piece)
+    const int t = (int)(row / a.H), h = (int)(row % a.H), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, dv = a.dv, column = tid & 127, group = tid >> 7;
     if (tid == 0) count = 0;
     __syncthreads();
-    for (int s = tid; s < a.n_seqs; s += 128) {
+    griddep_launch_dependents();
+    griddep_wait();
+    // the parts of the range that the token's CTA was cut by (none: a token of no portion, or a range in one piece)
+    for (int s = tid; s < a.n_seqs; s += blockDim.x) {
         const int len = fp8_portion(a, s), i = t - a.seqs[s];
         if (i >= 0 && i < len) {
-            const int i0 = i / a.ctoks * a.ctoks, p0 = a.pos[a.seqs[s]] + i0, lo16 = fp8_first_visible(p0, a.window, a.chunk) & ~(a.align - 1), n = p0 + min(a.ctoks, len - i0) - lo16;
+            const int i0 = i / a.ctoks * a.ctoks, p0 = a.pos[a.seqs[s]] + i0, first = fp8_first_visible(p0, a.window, a.chunk) & ~(a.align - 1), n = p0 + min(a.ctoks, len - i0) - first;
             if (n > a.part) count = (n + a.part - 1) / a.part;
         }
     }
@@ -189,28 +191,37 @@ template <typename T> __global__ void __launch_bounds__(128) fp8_merge_kernel(co
     const int parts = min(count, a.parts);
     if (parts == 0) return;
     const float* part = a.partial + row * a.parts * (dv + 2);
-    const float ms = tid < parts ? part[(long)tid * (dv + 2)] : -INFINITY, ls = tid < parts ? part[(long)tid * (dv + 2) + 1] : 0.f;
-    float m = warp_max(ms);
-    if (lane == 0) red[warp] = m;
-    __syncthreads();
-    m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-    const float sink = a.sink ? a.sink[h] * (kLog2e / unit) : -INFINITY;
-    m = fmaxf(m, sink);
-    __syncthreads();
-    const float e = ms > -INFINITY ? exp2f((ms - m) * unit) : 0.f;
-    const float part_l = warp_sum(ls * e);
-    if (lane == 0) red[warp] = part_l;
-    __syncthreads();
-    float l = (red[0] + red[1]) + (red[2] + red[3]);
-    if (a.sink) l += exp2f((sink - m) * unit);
-    if (tid < parts) wgt[tid] = l > 0.f || l != l ? e / l : 0.f;
+    if (group == 0) {      // (four warps)
+        const float ms = tid < parts ? part[(long)tid * (dv + 2)] : -INFINITY, ls = tid < parts ? part[(long)tid * (dv + 2) + 1] : 0.f;
+        const float top = warp_max(ms);
+        if (lane == 0) red[warp] = top;
+        asm volatile("barrier.cta.sync 1, 128;" ::: "memory");
+        const float sink = a.sink ? a.sink[h] * (kLog2e / unit) : -INFINITY, m = fmaxf(fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])), sink);
+        asm volatile("barrier.cta.sync 1, 128;" ::: "memory");
+        const float e = ms > -INFINITY ? exp2f((ms - m) * unit) : 0.f, part_l = warp_sum(ms > -INFINITY ? ls * e : ls);      // (scores of NaN have a sum of NaN and no maximum)
+        if (lane == 0) red[warp] = part_l;
+        asm volatile("barrier.cta.sync 1, 128;" ::: "memory");
+        float l = (red[0] + red[1]) + (red[2] + red[3]);
+        if (a.sink) l += exp2f((sink - m) * unit);
+        if (tid < parts) wgt[tid] = l > 0.f || l != l ? e / l : 0.f;
+        if (l != l && tid < parts) wgt[tid] = l;
+    }
     __syncthreads();
     T* out = (T*)a.out + t * a.out_stride + (long)h * dv;
-    for (int c = tid; c < dv; c += 128) {
+    for (int c0 = 0; c0 < dv; c0 += 128) {
+        const int c = c0 + column;
         float acc = 0.f;
-#pragma unroll 8
-        for (int s = 0; s < parts; s++) acc = fmaf(wgt[s], part[(long)s * (dv + 2) + 2 + c], acc);
-        out[c] = from_f<T>(acc * a.out_scale);
+        if (c < dv) {
+#pragma unroll 16
+            for (int s = group; s < parts; s += kMergeGroups) acc = fmaf(wgt[s], part[(long)s * (dv + 2) + 2 + c], acc);
+        }
+        sums[group][column] = acc;
+        __syncthreads();
+        if (group == 0 && c < dv) {
+            acc = (sums[0][column] + sums[1][column]) + (sums[2][column] + sums[3][column]);
+            out[c] = from_f<T>(acc * a.out_scale);
+        }
+        __syncthreads();
     }
 }
 
@@ -248,7 +259,7 @@ static long fp8_tiles(const ktb200_fp8_attn_params* c, int n_tokens, int ctoks) 
 static bool fp8_sizes_ok(const ktb200_fp8_attn_params* c) { return c && c->heads > 0 && c->kv_heads > 0 && c->heads % c->kv_heads == 0; }
 
 // How a call's ranges are cut: `even` CTAs of a cluster for each, or parts of `part` keys, or (0, 0) not at all.  Not where the CTAs of uncut ranges fill the SMs' places four times.  A
-// cluster where eight CTAs a range fill the places once, or leave them 1024 keys at most: as many as fill the places four times and still have 256 keys each.  Else parts of such a length
+// cluster where eight CTAs a range fill the places once, or leave them 1024 keys at most: as many as fill the places twice and still have 256 keys each (64 contexts of 4095 to 8190: two CTAs a range 151 us, three 154, four 158).  Else parts of such a length
 // that one round of CTAs covers the ranges, between sequences that decode (whose ranges may have any length) no more than 2048
 struct Fp8Cut { int even, part; };
 static Fp8Cut fp8_cut(const ktb200_fp8_attn_params* c, int n_tokens, int max_keys, const Fp8Form& f) {
@@ -256,7 +267,7 @@ static Fp8Cut fp8_cut(const ktb200_fp8_attn_params* c, int n_tokens, int max_key
     const long range = fp8_range(c, max_keys, f), places = f.places * 148, ctas = fp8_tiles(c, n_tokens, f.ctoks) * c->kv_heads * ((R + f.heads - 1) / f.heads);
     if (ctas >= 4 * places || range <= 2 * kFp8MinPart) return {0, 0};
     if (f.kernel == Fp8Form::kDecode && (ctas * kFdCluster >= places || range <= 1024 * kFdCluster))
-        return {(int)std::min<long>({kFdCluster, (4 * places + ctas - 1) / ctas, (range + kFp8MinPart - 1) / kFp8MinPart}), 0};
+        return {(int)std::min<long>({kFdCluster, (2 * places + ctas - 1) / ctas, (range + kFp8MinPart - 1) / kFp8MinPart}), 0};
     long part = (range * ctas + places - 1) / places;
     if (c->n_seqs > 1 && f.kernel != Fp8Form::kPrompt) part = std::min<long>(part, 2048);
     part = std::max<long>({part, kFp8MinPart, (range + kFp8MaxParts - 1) / kFp8MaxParts});
@@ -317,7 +328,7 @@ extern "C" int ktb200_fp8_cache_attn(const ktb200_fp8_attn_params* c, int n_toke
     }
     count_launch();
     if (parts > 1) {
-        KTB_CUDA_CHECK(launch_pdl(bf16 ? fp8_merge_kernel<__nv_bfloat16> : fp8_merge_kernel<float>, dim3((unsigned)((long)n_tokens * c->heads)), dim3(128), (size_t)0, s, a,
+        KTB_CUDA_CHECK(launch_pdl(bf16 ? fp8_merge_kernel<__nv_bfloat16> : fp8_merge_kernel<float>, dim3((unsigned)((long)n_tokens * c->heads)), dim3(128 * kMergeGroups), (size_t)0, s, a,
                                   f.kernel == Fp8Form::kCuda ? kLog2e : 1.0f));
         count_launch();
     }

@@ -29,7 +29,7 @@ struct FdMisc {
     unsigned long long k_full[kFdStages], k_free[kFdStages], v_full[kFdStages], v_free[kFdStages], s_full[2], s_free[2], p_full[2], p_free[2], q_ready;
     float red[4][16], fac[16];
     uint32_t tmem_base;
-    int info[4];
+    int found;
 };
 template <int RP> constexpr int fd_smem() { return 2 * kFdStages * kFdTile + 3 * 2 * RP * 128 + (int)sizeof(FdMisc) + 1024; }
 
@@ -73,11 +73,27 @@ template <int RP> __global__ void __launch_bounds__(kFdThreads, RP == 8 ? 3 : 2)
         tma_prefetch_desc(&maps.v);
     }
     griddep_wait();
-    if (warp == 2) fp8_find_tokens(a, blockIdx.x, 1, misc.info);
+    // What a CTA needs ahead of its first copy, loaded side by side: the token's position and table row, whether a portion has the token, and the token's queries
+    const int t = blockIdx.x, R = a.H / a.G, hblocks = R / RH, g = blockIdx.y / hblocks, h0 = g * R + (blockIdx.y % hblocks) * RH;
+    const int p = a.pos[t], slot = a.slot[t];
+    uint2 q_row[RP / 4];
+    if (warp >= 2) {      // a warp a head: a lane has columns 4 lane ..
+#pragma unroll
+        for (int i = 0; i < RP / 4; i++) {
+            const int h = warp - 2 + 4 * i;
+            q_row[i] = h < RH ? *reinterpret_cast<const uint2*>((const __nv_bfloat16*)a.q + ((long)t * a.H + h0 + h) * 128 + 4 * lane) : make_uint2(0, 0);
+        }
+    } else if (warp == 0) {
+        bool mine = false;
+        for (int s = lane; s < a.n_seqs; s += 32) {
+            const int start = a.seqs[s], len = a.seqs[a.seqs_stride + s];
+            mine |= start >= 0 && start <= a.n_tokens - len && t >= start && t - start < len;
+        }
+        const bool found = __any_sync(0xffffffffu, mine);
+        if (lane == 0) misc.found = found && p >= 0;
+    }
     __syncthreads();
-    const int t = misc.info[0], p = misc.info[2], slot = misc.info[3], R = a.H / a.G, hblocks = R / RH;
-    if (misc.info[1] <= 0) return;
-    const int g = blockIdx.y / hblocks, h0 = g * R + (blockIdx.y % hblocks) * RH;
+    if (!misc.found) return;
     const int lo = fp8_first_visible(p, a.window, a.chunk), lo_al = lo & ~(kFdAlign - 1);
     const int even = a.even, part = even ? ((p + 1 - lo_al + kFdKeys - 1) / kFdKeys + even - 1) / even * kFdKeys : a.part;
     const bool cut = !even && part > 0 && p + 1 - lo_al > part;
@@ -161,16 +177,16 @@ template <int RP> __global__ void __launch_bounds__(kFdThreads, RP == 8 ? 3 : 2)
         // ================================================================ queries, soft-max, result
         const int sp = warp & 3, r = 32 * sp + lane, w4 = warp - 2;
         const uint32_t lanes = (uint32_t)(32 * sp) << 16;
-        {      // a warp a head: lane has columns 4 lane ..
-            for (int h = w4; h < RP; h += 4) {
-                float x[4] = {0.f, 0.f, 0.f, 0.f}, odd = 0.f;
-                if (h < RH) {
-                    const uint2 v = *reinterpret_cast<const uint2*>((const __nv_bfloat16*)a.q + ((long)t * a.H + h0 + h) * 128 + 4 * lane);
-                    x[0] = __uint_as_float(v.x << 16); x[1] = __uint_as_float(v.x & 0xffff0000u); x[2] = __uint_as_float(v.y << 16); x[3] = __uint_as_float(v.y & 0xffff0000u);
-                }
+        {
+#pragma unroll
+            for (int i = 0; i < RP / 4; i++) {
+                const int h = w4 + 4 * i;
+                const uint2 v = q_row[i];
+                const float x[4] = {__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u), __uint_as_float(v.y << 16), __uint_as_float(v.y & 0xffff0000u)};
+                float odd = 0.f;
                 float top = 0.f;
 #pragma unroll
-                for (int i = 0; i < 4; i++) { top = fmaxf(top, fabsf(x[i])); odd = fmaf(x[i], 0.f, odd); }
+                for (int k = 0; k < 4; k++) { top = fmaxf(top, fabsf(x[k])); odd = fmaf(x[k], 0.f, odd); }
                 top = warp_max(top);
                 odd = warp_sum(odd);      // NaN where a value is not finite (e4m3 has no infinity)
                 const int up = min(126, max(-120, 7 - ((int)(__float_as_uint(top) >> 23) - 127)));      // 2^(7 - e) of a largest 1.f 2^e, within what fp32 holds with its inverse
