@@ -8,7 +8,7 @@
 //   int8_rows_kernel   weight rows on the MMA's 128 rows, 16 to 128 tokens on its columns: a decode step reads the weights once.  K is split over the CTAs of a cluster, which add their
 //                      parts through distributed shared memory: no workspace to clear, no second launch.  Weight boxes are under way before the codes are there (the launch is
 //                      a programmatic dependent of the quantiser's).
-//   int8_gemm_kernel   prompts: 128 tokens x BN outputs a tile, persistent, two accumulators in tensor memory
+//   int8_gemm_kernel   prompts: 256 tokens x up to 256 outputs a tile of two CTAs, persistent, two accumulators in tensor memory
 #include <cuda.h>
 
 #include <algorithm>
@@ -238,97 +238,145 @@ template <int NT> __global__ void __launch_bounds__(kI8RowsThreads, 2) int8_rows
 }
 
 // ------------------------------------------------------------------------------------------------ many tokens
-// Persistent: a tile is 128 tokens x BN outputs; warp 0 TMA ring (192 KB), warp 1 products, warps 4-19 results (a thread one token and a quarter of the tile's columns).  Tiles run
-// token tile fastest inside groups of kI8Group, so that the CTAs of a wave share the weight rows and the tokens through L2.
-constexpr int kI8GemmThreads = 640, kI8Group = 16, kI8Ring = 192 * 1024, kI8Turn = 16 * 33;
+// Persistent pairs of CTAs (cta_group::2): a pair's tile is 256 tokens x bn outputs, each CTA has 128 of the tokens and brings half of the outputs' weight rows, which both tensor
+// cores read: a K block of 128 costs a CTA 16 KB + 64 bn bytes of shared memory each way where one CTA alone would need 16 KB + 128 bn (single CTAs with 256 columns were bound by
+// that: 735 cycles a block against 524 of the products).  bn is any multiple of 32: the one whose rounds of tiles take least.
+//     warp 0 TMA ring (192 KB) of its own half, whose bytes are counted by the first CTA's barriers; warp 1 of the first CTA the pair's products; warps 4-19 results (a thread one token,
+//     every fourth run of 16 columns).  Two accumulators of bn columns.
+// Tiles run token tile fastest inside groups of kI8Group, so that the CTAs of a wave share the weight rows and the tokens through L2.
+constexpr int kI8GemmThreads = 640, kI8Group = 8, kI8Ring = 192 * 1024, kI8Turn = 16 * 33;
 struct Int8GemmMisc {
     unsigned long long full[8], free[8], d_full[2], d_free[2];
     uint32_t tmem_base;
 };
 constexpr int kI8GemmSmem = kI8Ring + (int)sizeof(Int8GemmMisc) + 1024, kI8GemmSmemTurn = kI8GemmSmem + 16 * kI8Turn * 4;
 static_assert(kI8GemmSmemTurn <= 232448, "shared memory budget");
+__host__ __device__ constexpr int i8_gemm_stage(int bn) { return 128 * 128 + bn / 2 * 128; }
+__host__ __device__ constexpr int i8_gemm_stages(int bn) { return kI8Ring / i8_gemm_stage(bn) < 8 ? kI8Ring / i8_gemm_stage(bn) : 8; }
+
+__device__ __forceinline__ uint32_t cluster_at(uint32_t addr, uint32_t rank) {
+    uint32_t at;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(addr), "r"(rank));
+    return at;
+}
+// a box into this CTA's shared memory, counted by a barrier of either CTA of the pair
+__device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap* m, uint32_t bar, int c0, int c1) {
+    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst), "l"(m), "r"(bar), "r"(c0), "r"(c1) : "memory");
+}
+// Four products of the pair on consecutive K-steps of 32 bytes, and the barriers (of both CTAs) that complete when all so far have (0: not asked for); called by a converged warp
+__device__ __forceinline__ void mma_i8_pair_x4(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate, uint32_t bar0, uint32_t bar1) {
+    asm volatile(
+        "{\n"
+        ".reg .pred p, q, c, e, t;\n"
+        ".reg .b32 r;\n"
+        ".reg .b64 a, b;\n"
+        ".reg .b16 both;\n"
+        "mov.b16 both, 3;\n"
+        "elect.sync r|q, 0xffffffff;\n"
+        "setp.ne.b32 p, %4, 0;\n"
+        "setp.eq.b32 t, %4, %4;\n"
+        "setp.ne.and.b32 c, %5, 0, q;\n"
+        "setp.ne.and.b32 e, %6, 0, q;\n"
+        "@q tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n"
+        "add.u64 a, %1, 2;\n"
+        "add.u64 b, %2, 2;\n"
+        "@q tcgen05.mma.cta_group::2.kind::i8 [%0], a, b, %3, t;\n"
+        "add.u64 a, a, 2;\n"
+        "add.u64 b, b, 2;\n"
+        "@q tcgen05.mma.cta_group::2.kind::i8 [%0], a, b, %3, t;\n"
+        "add.u64 a, a, 2;\n"
+        "add.u64 b, b, 2;\n"
+        "@q tcgen05.mma.cta_group::2.kind::i8 [%0], a, b, %3, t;\n"
+        "@c tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%5], both;\n"
+        "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%6], both;\n"
+        "}\n" ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate), "r"(bar0), "r"(bar1) : "memory");
+}
 
 // TURN: rows of y that do not begin at 32 bytes.  A thread's columns of its token would be scattered values; the warp turns 16 columns of its 32 tokens around in shared memory, and
 // 16 threads write 16 columns of one row
-template <int BN, bool TURN> __global__ void __launch_bounds__(kI8GemmThreads, 1) int8_gemm_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap, const Int8Out o,
-                                                                                                  int mt, int nt) {
-    constexpr int STAGE = 128 * 128 + BN * 128, STAGES = kI8Ring / STAGE < 8 ? kI8Ring / STAGE : 8, COLS = 2 * BN;
+template <bool TURN> __global__ void __launch_bounds__(kI8GemmThreads, 1) __cluster_dims__(2, 1, 1)
+    int8_gemm_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap, const Int8Out o, int bn, int mt, int nt) {
     extern __shared__ __align__(16) uint8_t i8_smem_raw[];
     const uint32_t raw = smem_u32(i8_smem_raw), base = (raw + 1023u) & ~1023u;
     Int8GemmMisc& misc = *reinterpret_cast<Int8GemmMisc*>(i8_smem_raw + (base - raw) + kI8Ring);
-    const int tid = threadIdx.x, lane = tid & 31, warp = uniform(tid >> 5);
+    const int tid = threadIdx.x, lane = tid & 31, warp = uniform(tid >> 5), rank = blockIdx.x & 1, pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+    const int stage = i8_gemm_stage(bn), stages = i8_gemm_stages(bn), tiles = mt * nt;
     griddep_launch_dependents();
     if (tid == 0) {
-        for (int s = 0; s < STAGES; s++) { bar_init(smem_u32(&misc.full[s]), 1); bar_init(smem_u32(&misc.free[s]), 1); }
-        for (int b = 0; b < 2; b++) { bar_init(smem_u32(&misc.d_full[b]), 1); bar_init(smem_u32(&misc.d_free[b]), 16); }
+        for (int s = 0; s < 8; s++) { bar_init(smem_u32(&misc.full[s]), 1); bar_init(smem_u32(&misc.free[s]), 1); }
+        for (int b = 0; b < 2; b++) { bar_init(smem_u32(&misc.d_full[b]), 1); bar_init(smem_u32(&misc.d_free[b]), 32); }
         bar_fence_init();
         tma_prefetch_desc(&xmap);
         tma_prefetch_desc(&wmap);
     }
-    if (warp == 1) tmem_alloc(smem_u32(&misc.tmem_base), COLS);
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&misc.tmem_base)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
     tc_fence_before();
     __syncthreads();
+    cluster_arrive();      // (the pair's barriers and tensor memory are there)
+    cluster_wait();
     tc_fence_after();
     const uint32_t tmem = uniform(misc.tmem_base);
-    const int tiles = mt * nt;
     auto place = [&](int tile, int& m0, int& n0) {
         const int per = kI8Group * nt, g = tile / per, r = tile - g * per, gm = min(kI8Group, mt - g * kI8Group);
-        n0 = (r / gm) * BN;
-        m0 = (g * kI8Group + r % gm) * 128;
+        n0 = (r / gm) * bn;
+        m0 = (g * kI8Group + r % gm) * 256 + rank * 128;
     };
     griddep_wait();
     if (warp == 0) {
         if (lane == 0) {
             int s = 0, ph = 1;
-            for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+            for (int tile = pair; tile < tiles; tile += pairs) {
                 int m0, n0;
                 place(tile, m0, n0);
                 for (int kb = 0; kb < o.nkb; kb++) {
                     bar_wait(smem_u32(&misc.free[s]), ph);
-                    const uint32_t bar = smem_u32(&misc.full[s]), dst = base + s * STAGE;
-                    bar_expect_tx(bar, STAGE);
-                    tma_load_2d(dst, &xmap, bar, kb * 128, m0);
-                    tma_load_2d(dst + 128 * 128, &wmap, bar, kb * 128, n0);
-                    if (++s == STAGES) { s = 0; ph ^= 1; }
+                    const uint32_t dst = base + s * stage, bar = cluster_at(smem_u32(&misc.full[s]), 0);
+                    if (rank == 0) bar_expect_tx(smem_u32(&misc.full[s]), 2 * stage);
+                    tma_load_pair(dst, &xmap, bar, kb * 128, m0);
+                    tma_load_pair(dst + 128 * 128, &wmap, bar, kb * 128, n0 + rank * (bn / 2));
+                    if (++s == stages) { s = 0; ph ^= 1; }
                 }
             }
         }
         __syncwarp();
-    } else if (warp == 1) {
-        constexpr uint32_t idesc = instr_desc(2, 1, 1, 0, 0, 128, BN);
+    } else if (warp == 1 && rank == 0) {
+        const uint32_t idesc = instr_desc(2, 1, 1, 0, 0, 256, 0) | ((uint32_t)(bn >> 3) << 17);
         int s = 0, ph = 0, it = 0;
-        for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, it++) {
+        for (int tile = pair; tile < tiles; tile += pairs, it++) {
             const int buf = it & 1;
             bar_wait(smem_u32(&misc.d_free[buf]), ((it >> 1) & 1) ^ 1);
             tc_fence_after();
             for (int kb = 0; kb < o.nkb; kb++) {
                 bar_wait(smem_u32(&misc.full[s]), ph);
                 tc_fence_after();
-                const uint32_t a = base + s * STAGE, b = a + 128 * 128;
-                mma_i8_x4(tmem + buf * BN, smem_desc(a, 16, 1024, kLayoutSw128), smem_desc(b, 16, 1024, kLayoutSw128), idesc, kb > 0, smem_u32(&misc.free[s]),
-                          kb + 1 == o.nkb ? smem_u32(&misc.d_full[buf]) : 0);
-                if (++s == STAGES) { s = 0; ph ^= 1; }
+                const uint32_t a = base + s * stage, b = a + 128 * 128;
+                mma_i8_pair_x4(tmem + buf * 256, smem_desc(a, 16, 1024, kLayoutSw128), smem_desc(b, 16, 1024, kLayoutSw128), idesc, kb > 0, smem_u32(&misc.free[s]),
+                               kb + 1 == o.nkb ? smem_u32(&misc.d_full[buf]) : 0);
+                if (++s == stages) { s = 0; ph ^= 1; }
             }
         }
     } else if (warp >= 4) {
-        constexpr int PART = BN / 4;
         const int sp = warp & 3, ch = (warp - 4) >> 2, live = o.bsz ? max(0, min(o.T, *o.bsz)) : o.T;
-        const uint32_t tcol = tmem + ((uint32_t)(32 * sp) << 16) + ch * PART;
         float* turn = reinterpret_cast<float*>(i8_smem_raw + (base - raw) + kI8Ring + sizeof(Int8GemmMisc)) + (warp - 4) * kI8Turn;
         int it = 0;
-        for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, it++) {
+        for (int tile = pair; tile < tiles; tile += pairs, it++) {
             int m0, n0;
             place(tile, m0, n0);
-            const int buf = it & 1, t = m0 + 32 * sp + lane, nb = n0 + ch * PART;
+            const int buf = it & 1, t = m0 + 32 * sp + lane;
+            const uint32_t tcol = tmem + ((uint32_t)(32 * sp) << 16) + buf * 256;
             const float xs = t < o.T ? __ldg(o.xs + t) : 0.f;
             bar_wait(smem_u32(&misc.d_full[buf]), (it >> 1) & 1);
             tc_fence_after();
 #pragma unroll 1
-            for (int c = 0; c < PART; c += 16) {
+            for (int c = 16 * ch; c < bn; c += 64) {
                 uint32_t v[16];
-                tmem_ld16(tcol + buf * BN + c, v);
+                tmem_ld16(tcol + c, v);
                 tmem_wait_ld();
-                const int n = nb + c;
+                const int n = n0 + c;
+                if (n >= o.N) break;
                 float f[16];
 #pragma unroll
                 for (int i = 0; i < 16; i++) f[i] = n + i < o.N ? i8_result((int)v[i], xs, __ldg(o.ws + n + i), o.bias ? __ldg(o.bias + n + i) : 0.f) : 0.f;
@@ -366,14 +414,16 @@ template <int BN, bool TURN> __global__ void __launch_bounds__(kI8GemmThreads, 1
             }
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) bar_arrive(smem_u32(&misc.d_free[buf]));
+            if (lane == 0) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_at(smem_u32(&misc.d_free[buf]), 0)) : "memory");
         }
     }
     tc_fence_before();
     __syncthreads();
+    cluster_arrive();      // nobody leaves while the other's copies and products reach for its barriers
+    cluster_wait();
     if (warp == 1) {
         tc_fence_after();
-        tmem_dealloc(tmem, COLS);
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
     }
 }
 
@@ -425,17 +475,31 @@ template <int NT> static int i8_launch_rows(const void* w, long w_stride, const 
     count_launch();
     return KTB200_OK;
 }
-template <int BN> static int i8_launch_gemm(const void* w, long w_stride, const int8_t* codes, int K, int Kp, const Int8Out& o, int sms, cudaStream_t s) {
+// Columns of a pair's tile: the multiple of 32 whose rounds take least.  A K block of bn columns takes the larger of its products' time and the shared memory's, in 128 x bn: bn, and about
+// 128 + bn / 2; kI8Fixed is what a tile costs beside its blocks, in blocks
+constexpr int kI8Fixed = 4;
+static int i8_columns(int mt, int N, int nkb, int pairs, long* cost_out = nullptr) {
+    int best = 256;
+    long least = LONG_MAX;
+    for (int bn = 256; bn >= 32; bn -= 32) {
+        const long rounds = ((long)mt * ((N + bn - 1) / bn) + pairs - 1) / pairs, cost = rounds * (nkb + kI8Fixed) * std::max(bn, 128 + bn / 2);
+        if (cost < least) { least = cost; best = bn; }
+    }
+    if (cost_out) *cost_out = least;
+    return best;
+}
+static int i8_launch_gemm(const void* w, long w_stride, const int8_t* codes, int K, int Kp, const Int8Out& o, int sms, cudaStream_t s) {
+    const int pairs = sms / 2, mt = (o.T + 255) / 256, bn = i8_columns(mt, o.N, o.nkb, pairs), nt = (o.N + bn - 1) / bn;
     CUtensorMap wmap, xmap;
-    int rc = i8_map(&wmap, w, K, w_stride, o.N, BN);
+    int rc = i8_map(&wmap, w, K, w_stride, o.N, bn / 2);
     if (rc == KTB200_OK) rc = i8_map(&xmap, codes, K, Kp, o.T, 128);
     if (rc) return rc;
     const size_t es = type_size(o.type);
     const bool turn = (uintptr_t)o.y % 32 || o.y_stride * es % 32;
-    const int mt = (o.T + 127) / 128, nt = (o.N + BN - 1) / BN, smem = turn ? kI8GemmSmemTurn : kI8GemmSmem;
-    const auto kernel = turn ? int8_gemm_kernel<BN, true> : int8_gemm_kernel<BN, false>;
+    const int smem = turn ? kI8GemmSmemTurn : kI8GemmSmem;
+    const auto kernel = turn ? int8_gemm_kernel<true> : int8_gemm_kernel<false>;
     KTB_CUDA_CHECK(raise_smem_limit((const void*)kernel, smem));
-    KTB_CUDA_CHECK(launch_pdl(kernel, dim3((unsigned)std::min<long>((long)mt * nt, sms)), dim3(kI8GemmThreads), (size_t)smem, s, xmap, wmap, o, mt, nt));
+    KTB_CUDA_CHECK(launch_pdl(kernel, dim3((unsigned)(2 * std::min<long>((long)mt * nt, pairs))), dim3(kI8GemmThreads), (size_t)smem, s, xmap, wmap, o, bn, mt, nt));
     count_launch();
     return KTB200_OK;
 }
@@ -475,14 +539,10 @@ extern "C" int ktb200_int8_linear(const ktb200_int8_linear_params* c, int n_toke
     count_launch();
     const Int8Out o{scales, c->weight_scale, c->bias, c->y, c->y_stride, c->bsz, c->hidden_type, T, N, (K + 127) / 128};
     auto rows = [&](auto nt) { return i8_launch_rows<decltype(nt)::value>(c->weight, c->weight_stride, codes, K, Kp, o, sms, s); };
-    auto gemm = [&](auto bn) { return i8_launch_gemm<decltype(bn)::value>(c->weight, c->weight_stride, codes, K, Kp, o, sms, s); };
     if (T <= 16) return rows(std::integral_constant<int, 16>());
     if (T <= 32) return rows(std::integral_constant<int, 32>());
     if (T <= 64) return rows(std::integral_constant<int, 64>());
-    // the widest tile that still gives every SM one; where even the narrowest does not, row tiles whose K is split
-    const long mt = (T + 127) / 128;
-    if (T <= 128 || mt * ((N + 63) / 64) < sms) return rows(std::integral_constant<int, 128>());
-    if (mt * ((N + 255) / 256) >= sms) return gemm(std::integral_constant<int, 256>());
-    if (mt * ((N + 127) / 128) >= sms) return gemm(std::integral_constant<int, 128>());
-    return gemm(std::integral_constant<int, 64>());
+    // row tiles whose K is split where the GEMM's narrowest tiles would leave most pairs without one
+    if (T <= 128 || (long)((T + 255) / 256) * ((N + 63) / 64) < sms / 2) return rows(std::integral_constant<int, 128>());
+    return i8_launch_gemm(c->weight, c->weight_stride, codes, K, Kp, o, sms, s);
 }
