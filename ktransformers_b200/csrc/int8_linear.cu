@@ -22,8 +22,12 @@ using namespace umma;
 
 // ------------------------------------------------------------------------------------------------ codes
 // A row per CTA: the largest magnitude, then the codes; codes behind column K (up to Kp) are zeros.  VEC: rows of whole 16-byte vectors, of which a thread keeps kI8Keep in registers between
-// the two (what does not fit is read again, from L2).  Bound by the bytes of x and of the codes.
+// the two (what does not fit is read again, from L2).  Bound by the bytes of x and of the codes, and by little: nine instructions a value.
+//   - magnitudes are compared as their bits (two 16-bit ones at a time); infinities and NaN are the largest of all
+//   - a code is rint of the fp32 quotient x / s.  x times 1 / s is within 2e-5 of that, so its nearest integer (an addition of 1.5 2^23) is the code unless it stands so close to the middle
+//     of two; a vector with such a value, one in some thousand, is divided.  (Divided throughout 4000 rows of 18432 took 130 us.)
 constexpr int kI8Keep = 6;
+constexpr float kI8Magic = 12582912.f;      // 1.5 2^23: the low byte of magic + k is k's
 template <int TYPE> __device__ __forceinline__ void i8_unpack(uint4 w, float (&v)[TYPE == KTB200_TYPE_F32 ? 4 : 8]) {
     const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
@@ -34,17 +38,31 @@ template <int TYPE> __device__ __forceinline__ void i8_unpack(uint4 w, float (&v
     }
 }
 __device__ __forceinline__ uint32_t i8_code(float x, float s) { return (uint32_t)(int)fminf(fmaxf(rintf(__fdiv_rn(x, s)), -127.f), 127.f) & 0xffu; }
+// the magnitude of a value of the type, from its bits
+template <int TYPE> __device__ __forceinline__ float i8_magnitude(uint32_t bits) {
+    return TYPE == KTB200_TYPE_F32 ? __uint_as_float(bits) : TYPE == KTB200_TYPE_BF16 ? __uint_as_float(bits << 16) : fp16_bits_to_f32((uint16_t)bits);
+}
+template <int TYPE> __device__ __forceinline__ uint32_t i8_bits(const uint8_t* row, int k) {
+    if constexpr (TYPE == KTB200_TYPE_F32) return reinterpret_cast<const uint32_t*>(row)[k] & 0x7fffffffu;
+    else return reinterpret_cast<const uint16_t*>(row)[k] & 0x7fffu;
+}
 
 template <int TYPE, bool VEC> __global__ void __launch_bounds__(512) int8_quant_kernel(const void* x, long x_stride, int K, int Kp, int8_t* codes, float* scales) {
     constexpr int E = TYPE == KTB200_TYPE_F32 ? 4 : 8, ESZ = 16 / E;
-    __shared__ float red[16];
+    constexpr uint32_t kInf = TYPE == KTB200_TYPE_F32 ? 0x7f800000u : TYPE == KTB200_TYPE_BF16 ? 0x7f80u : 0x7c00u;
+    __shared__ uint32_t red[16];
     const long t = blockIdx.x;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
     griddep_launch_dependents();
     griddep_wait();
-    float top = 0.f, odd = 0.f;      // odd: NaN as soon as a value is not finite
+    uint32_t top = 0;      // 16-bit types: of the even and of the odd values
     uint4 keep[VEC ? kI8Keep : 1];
     const uint8_t* row = reinterpret_cast<const uint8_t*>(x) + t * x_stride * ESZ;
+    auto largest = [&](uint4 w) {
+        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++) top = TYPE == KTB200_TYPE_F32 ? max(top, u[i] & 0x7fffffffu) : __vmaxu2(top, u[i] & 0x7fff7fffu);
+    };
     if constexpr (VEC) {
         const int n = K / E;
 #pragma unroll
@@ -53,44 +71,42 @@ template <int TYPE, bool VEC> __global__ void __launch_bounds__(512) int8_quant_
             keep[i] = at < n ? *reinterpret_cast<const uint4*>(row + 16 * (long)at) : make_uint4(0, 0, 0, 0);
         }
 #pragma unroll
-        for (int i = 0; i < kI8Keep; i++) {
-            float v[E];
-            i8_unpack<TYPE>(keep[i], v);
-#pragma unroll
-            for (int e = 0; e < E; e++) { top = fmaxf(top, fabsf(v[e])); odd = fmaf(v[e], 0.f, odd); }
-        }
-        for (int at = threadIdx.x + kI8Keep * blockDim.x; at < n; at += blockDim.x) {
-            float v[E];
-            i8_unpack<TYPE>(*reinterpret_cast<const uint4*>(row + 16 * (long)at), v);
-#pragma unroll
-            for (int e = 0; e < E; e++) { top = fmaxf(top, fabsf(v[e])); odd = fmaf(v[e], 0.f, odd); }
-        }
+        for (int i = 0; i < kI8Keep; i++) largest(keep[i]);
+        for (int at = threadIdx.x + kI8Keep * blockDim.x; at < n; at += blockDim.x) largest(*reinterpret_cast<const uint4*>(row + 16 * (long)at));
+        if constexpr (TYPE != KTB200_TYPE_F32) top = max(top & 0xffffu, top >> 16);
     } else {
-        for (int k = threadIdx.x; k < K; k += blockDim.x) {
-            const float v = load_hidden(row, k, TYPE);
-            top = fmaxf(top, fabsf(v));
-            odd = fmaf(v, 0.f, odd);
-        }
+        for (int k = threadIdx.x; k < K; k += blockDim.x) top = max(top, i8_bits<TYPE>(row, k));
     }
-    if (odd != odd) top = INFINITY;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    top = __reduce_max_sync(0xffffffffu, top);
     if (lane == 0) red[warp] = top;
     __syncthreads();
     top = red[0];
-    for (int w = 1; w < nw; w++) top = fmaxf(top, red[w]);
-    const float s = top == INFINITY ? NAN : __fdiv_rn(top, 127.f);
+    for (int w = 1; w < nw; w++) top = max(top, red[w]);
+    const float s = top >= kInf ? NAN : __fdiv_rn(i8_magnitude<TYPE>(top), 127.f);
     const bool some = s > 0.f;
     if (threadIdx.x == 0) scales[t] = s;
     int8_t* out = codes + t * Kp;
     if constexpr (VEC) {
+        const float inv = s > 1e-37f ? __fdiv_rn(1.0f, s) : 0.f;      // (0: scales whose inverse fp32 does not hold; their rows are divided)
         auto store = [&](int at, uint4 w) {
-            float v[E];
+            float v[E], far = inv > 0.f ? 0.f : 1.f;
             i8_unpack<TYPE>(w, v);
-            uint32_t c[E / 4] = {};
-            if (some) {
+            uint32_t c[E / 4] = {}, r[E];
 #pragma unroll
-                for (int e = 0; e < E; e++) c[e / 4] |= i8_code(v[e], s) << (8 * (e & 3));
+            for (int e = 0; e < E; e++) {
+                const float m = fmaf(v[e], inv, kI8Magic);
+                far = fmaxf(far, fabsf(fmaf(v[e], inv, kI8Magic - m)));
+                r[e] = __float_as_uint(m);
+            }
+#pragma unroll
+            for (int i = 0; i < E / 4; i++) c[i] = __byte_perm(__byte_perm(r[4 * i], r[4 * i + 1], 0x0040), __byte_perm(r[4 * i + 2], r[4 * i + 3], 0x0040), 0x5410);
+            if (far > 0.4999f) {
+#pragma unroll
+                for (int i = 0; i < E / 4; i++) c[i] = 0;
+                if (some) {
+#pragma unroll
+                    for (int e = 0; e < E; e++) c[e / 4] |= i8_code(v[e], s) << (8 * (e & 3));
+                }
             }
             if constexpr (E == 4) *reinterpret_cast<uint32_t*>(out + 4 * (long)at) = c[0];
             else *reinterpret_cast<uint2*>(out + 8 * (long)at) = make_uint2(c[0], c[1]);
@@ -120,7 +136,7 @@ __device__ __forceinline__ float i8_result(int acc, float xs, float ws, float bi
 // ------------------------------------------------------------------------------------------------ few tokens
 // grid (row tiles of 128, K splits = the cluster, token tiles of NT); 192 threads: warp 0 copies, warp 1 products, warps 2-5 results.  A stage of the ring is 128 bytes of K: a box of
 // 128 weight rows and one of NT tokens.
-constexpr int kI8RowsThreads = 192;
+constexpr int kI8RowsThreads = 192, kI8MaxSplits = 8;
 template <int NT> constexpr int i8_rows_stage() { return 128 * 128 + NT * 128; }
 template <int NT> constexpr int i8_rows_stages() { return NT == 16 ? 6 : NT == 32 ? 5 : NT == 64 ? 4 : 3; }      // about 100 KB: two CTAs an SM
 struct Int8RowsMisc {
@@ -134,7 +150,7 @@ __device__ __forceinline__ int cluster_load(uint32_t addr, uint32_t rank) {     
     uint32_t at;
     int v;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(addr), "r"(rank));
-    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(at));      // (ordered by the cluster's barriers)
     return v;
 }
 
@@ -219,10 +235,21 @@ template <int NT> __global__ void __launch_bounds__(kI8RowsThreads, 2) int8_rows
         if (warp >= 2) {
             const int mine = o.bsz ? min(live, *o.bsz - t0) : live;
             const float ws = n < o.N ? o.ws[n] : 0.f, bias = n < o.N && o.bias ? o.bias[n] : 0.f;
-            for (int t = blockIdx.y; t < mine; t += splits) {
-                int acc = 0;
-                for (int k = 0; k < splits; k++) acc += cluster_load(base + (t * 128 + r) * 4, k);
-                if (n < o.N) store_hidden(o.y, (long)(t0 + t) * o.y_stride + n, o.type, i8_result(acc, __ldg(o.xs + t0 + t), ws, bias));
+            // four tokens at a time, so that the loads from all CTAs of the cluster are on their way together
+            for (int t0c = blockIdx.y; t0c < mine; t0c += 4 * splits) {
+                int v[4][kI8MaxSplits];
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+#pragma unroll
+                    for (int k = 0; k < kI8MaxSplits; k++) v[i][k] = k < splits && t0c + i * splits < mine ? cluster_load(base + ((t0c + i * splits) * 128 + r) * 4, k) : 0;
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int t = t0c + i * splits;
+                    int acc = 0;
+#pragma unroll
+                    for (int k = 0; k < kI8MaxSplits; k++) acc += v[i][k];
+                    if (t < mine && n < o.N) store_hidden(o.y, (long)(t0 + t) * o.y_stride + n, o.type, i8_result(acc, __ldg(o.xs + t0 + t), ws, bias));
+                }
             }
         }
         __syncwarp();
@@ -439,7 +466,7 @@ static int i8_map(CUtensorMap* map, const void* ptr, int K, long stride, int n, 
     return KTB200_OK;
 }
 // K splits of int8_rows_kernel: those whose CTAs, two an SM, take least one after the other; kI8Round is what a CTA costs beside its blocks, in blocks
-constexpr int kI8Round = 8, kI8MaxSplits = 8;
+constexpr int kI8Round = 8;
 static int i8_splits(long tiles, int nkb, int sms, long* cost_out = nullptr) {
     int best = 1;
     long least = LONG_MAX;
