@@ -32,11 +32,11 @@ __device__ __forceinline__ void mma_e4m3_16832(float (&c)[4], uint32_t a0, uint3
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// two numbers as e4m3 codes (the first in the low byte), and as codes 16 times what those leave of them
-__device__ __forceinline__ uint2 split_e4m3(float lo, float hi) {
+// two numbers as e4m3 codes (the first in the low byte), and as codes TIMES times what those leave of them
+template <int TIMES = 16> __device__ __forceinline__ uint2 split_e4m3(float lo, float hi) {
     const uint32_t first = __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
     const float2 got = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)first, __NV_E4M3)));
-    return make_uint2(first, __nv_cvt_float2_to_fp8x2(make_float2((lo - got.x) * 16.f, (hi - got.y) * 16.f), __NV_SATFINITE, __NV_E4M3));
+    return make_uint2(first, __nv_cvt_float2_to_fp8x2(make_float2((lo - got.x) * TIMES, (hi - got.y) * TIMES), __NV_SATFINITE, __NV_E4M3));
 }
 // two e4m3 codes (the low half of a word) as two fp16 numbers
 __device__ __forceinline__ uint32_t f16_of_codes(uint32_t two) {

@@ -2,14 +2,17 @@
 //
 // A CTA owns 256 rows = (token, query head) pairs of one sequence portion and one key/value head as two tiles of 128 (RH heads of 128 / RH consecutive tokens each); keys run in
 // tiles of 128 from a multiple of 128 on.
-//     warps 0, 2, 3   codes to fp16, which holds every e4m3 number exactly: TMA brings a tile's codes, the warps turn them into the swizzled operands (a conversion for two codes)
-//     warp 1          MMAs: S = Q K^T from shared memory, O += P V with P in tensor memory.  The tiles take turns, S of the next key tile right behind PV of this one, so that one
-//                     tile's soft-max runs beside the other's products
-//     warps 4-7       soft-max of the first tile, 8-11 of the second: a thread owns a row.  First it makes its row of Q: fp16 of the row moved by a power of two so that its largest
-//                     stands in [2^13, 2^14) (exact for what is within 2^-28 of that).  t = s log2(e) + log2(value scale), p = 2^(t - m), l += p / (value scale): scales are one number a
-//                     page and head, so that of 64 scores at a time they change the factor and the offset of an fma that is there anyway, and O needs none.  P (fp16, 2^-11 of a
-//                     weight off at most) replaces its S in tensor memory; m is raised, and O scaled in tensor memory, only when a row's t outgrows it by 8
-// TMEM: [S0 | O0 | S1 | O1], 128 columns each.  Shared memory: Q 64 KB, K and V 2 x 32 KB each as fp16, 16 KB each as codes.
+//     warps 0, 2, 3   values: TMA brings a tile's codes, the warps turn them into swizzled fp16 operands, which hold every e4m3 number exactly (a conversion for two codes).  Keys need none:
+//                     warp 0 has their codes brought as operands
+//     warp 1          MMAs: S = Q K^T (kind::f8f6f4) from shared memory, O += P V (kind::f16) with P in tensor memory.  The tiles take turns, S of the next key tile right behind PV of this
+//                     one, so that one tile's soft-max runs beside the other's products
+//     warps 4-7       soft-max of the first tile, 8-11 of the second: a thread owns a row.  First it makes its row of Q: moved by a power of two so that its largest stands in [128, 256) and
+//                     split into two e4m3 numbers, q = q1 + q2, whose products add up in one sum: exact for bf16 numbers down to 2^-9 of the largest, 2^-17 of it off below.
+//                     t = s log2(e) + log2(value scale), p = 2^(t - m), l += p / (value scale): scales are one number a page and head, so that of 64 scores at a time they change the
+//                     factor and the offset of an fma that is there anyway, and O needs none.  P (fp16, 2^-11 of a weight off at most) replaces its S in tensor memory; m is raised,
+//                     and O scaled in tensor memory, only when a row's t outgrows it by 8
+// TMEM: [S0 | O0 | S1 | O1], 128 columns each.  Shared memory: Q 64 KB, K 3 x 16 KB, V 2 x 32 KB as fp16 and 2 x 16 KB as codes.
+// (With keys turned into fp16 as well the three warps were the bound: 2048 tokens behind 2001 took 318 us, 228 with their work left out.)
 #pragma once
 #include <cuda.h>
 
@@ -17,15 +20,15 @@
 
 namespace ktb {
 
-constexpr int kFpThreads = 384, kFpKeys = 128, kFpTile = 128 * 128 * 2, kFpCodes = 128 * 128, kFpBad = 64;
+constexpr int kFpThreads = 384, kFpKeys = 128, kFpTile = 128 * 128 * 2, kFpCodes = 128 * 128, kFpKStages = 3, kFpBad = 64;
 struct FpMisc {
-    unsigned long long q_full, k8_full, v8_full, k_full[2], k_free[2], v_full[2], v_free[2], s_full[2], p_full[2], o_done[2];
+    unsigned long long q_full, v8_full[2], k_full[kFpKStages], k_free[kFpKStages], v_full[2], v_free[2], s_full[2], p_full[2], o_done[2];
     float2 scales[4][2];      // of a tile's two runs of 64 keys (zeros: not there)
     uint32_t tmem_base;
     int info[4], n_bad, bad_lo, bad_hi;
     int2 bad[kFpBad];      // values that are NaN in tiles that not every row sees whole: (key, run of 16 columns << 16 | which of them)
 };
-constexpr int kFpSmem = 6 * kFpTile + 2 * kFpCodes + (int)sizeof(FpMisc) + 1024;
+constexpr int kFpSmem = 4 * kFpTile + (kFpKStages + 2) * kFpCodes + (int)sizeof(FpMisc) + 1024;
 static_assert(kFpSmem <= 232448, "shared memory budget");
 
 __global__ void __launch_bounds__(kFpThreads, 1) fp8_attn_prompt_kernel(const __grid_constant__ FdMaps maps, const Fp8Attn a, int RH) {
@@ -33,16 +36,15 @@ __global__ void __launch_bounds__(kFpThreads, 1) fp8_attn_prompt_kernel(const __
     extern __shared__ __align__(16) uint8_t fp_smem_raw[];
     const uint32_t raw = smem_u32(fp_smem_raw), base = (raw + 1023u) & ~1023u;
     uint8_t* smem = fp_smem_raw + (base - raw);
-    const uint32_t kbase = base + 2 * kFpTile, vbase = base + 4 * kFpTile, k8base = base + 6 * kFpTile, v8base = k8base + kFpCodes;
-    FpMisc& misc = *reinterpret_cast<FpMisc*>(smem + 6 * kFpTile + 2 * kFpCodes);
+    const uint32_t vbase = base + 2 * kFpTile, kbase = base + 4 * kFpTile, v8base = kbase + kFpKStages * kFpCodes;
+    FpMisc& misc = *reinterpret_cast<FpMisc*>(smem + 4 * kFpTile + (kFpKStages + 2) * kFpCodes);
     const int tid = threadIdx.x, lane = tid & 31, warp = uniform(tid >> 5), ps = a.pages.page_size, TOKS = 128 / RH, R = a.H / a.G, hblocks = R / RH;
     griddep_launch_dependents();
     if (tid == 0) {
-        bar_init(smem_u32(&misc.q_full), 8);
-        bar_init(smem_u32(&misc.k8_full), 1);
-        bar_init(smem_u32(&misc.v8_full), 1);
+        bar_init(smem_u32(&misc.q_full), 9);
+        for (int i = 0; i < kFpKStages; i++) { bar_init(smem_u32(&misc.k_full[i]), 1); bar_init(smem_u32(&misc.k_free[i]), 1); }
         for (int i = 0; i < 2; i++) {
-            bar_init(smem_u32(&misc.k_full[i]), 3); bar_init(smem_u32(&misc.k_free[i]), 1); bar_init(smem_u32(&misc.v_full[i]), 3); bar_init(smem_u32(&misc.v_free[i]), 1);
+            bar_init(smem_u32(&misc.v8_full[i]), 1); bar_init(smem_u32(&misc.v_full[i]), 3); bar_init(smem_u32(&misc.v_free[i]), 1);
             bar_init(smem_u32(&misc.s_full[i]), 1); bar_init(smem_u32(&misc.p_full[i]), 4); bar_init(smem_u32(&misc.o_done[i]), 1);
         }
         bar_fence_init();
@@ -75,24 +77,24 @@ __global__ void __launch_bounds__(kFpThreads, 1) fp8_attn_prompt_kernel(const __
         if (warp == 1) {
             // ================================================================ products (converged warp)
             constexpr uint32_t idesc_qk = instr_desc(1, 0, 0, 0, 0, 128, 128), idesc_pv = instr_desc(1, 0, 0, 0, 1, 128, 128);      // V [key][column]: B MN-major
-            auto scores = [&](int t, int j) {
-                const uint32_t qb = base + t * kFpTile, kb = kbase + (j & 1) * kFpTile;
-#pragma unroll
-                for (int k = 0; k < 2; k++)
-                    mma_f16_x4(tmem + t * 256, smem_desc(qb + k * (kFpTile / 2), 16, 1024, kLayoutSw128), smem_desc(kb + k * (kFpTile / 2), 16, 1024, kLayoutSw128), idesc_qk, k != 0,
-                               k ? smem_u32(&misc.s_full[t]) : 0);
+            auto scores = [&](int t, int kst) {
+                const uint32_t qb = base + t * kFpTile;
+                const uint64_t k = smem_desc(kbase + kst * kFpCodes, 16, 1024, kLayoutSw128);
+                mma_f8_x4(tmem + t * 256, smem_desc(qb, 16, 1024, kLayoutSw128), k, idesc_qk, 0);
+                mma_f8_x4(tmem + t * 256, smem_desc(qb + kFpCodes, 16, 1024, kLayoutSw128), k, idesc_qk, 1, smem_u32(&misc.s_full[t]), t ? smem_u32(&misc.k_free[kst]) : 0);
             };
             bar_wait(smem_u32(&misc.q_full), 0);
             bar_wait(smem_u32(&misc.k_full[0]), 0);
             tc_fence_after();
             scores(0, 0);
             scores(1, 0);
-            mma_commit(smem_u32(&misc.k_free[0]));
+            int kst = 0, kph = 0;
             for (int j = 0; j < n; j++) {
                 const int st = j & 1;
                 const uint32_t vb = vbase + st * kFpTile;
                 bar_wait(smem_u32(&misc.v_full[st]), (j >> 1) & 1);
-                if (j + 1 < n) bar_wait(smem_u32(&misc.k_full[st ^ 1]), ((j + 1) >> 1) & 1);
+                if (++kst == kFpKStages) { kst = 0; kph ^= 1; }
+                if (j + 1 < n) bar_wait(smem_u32(&misc.k_full[kst]), kph);
 #pragma unroll 1
                 for (int t = 0; t < 2; t++) {
                     bar_wait(smem_u32(&misc.p_full[t]), j & 1);
@@ -102,15 +104,14 @@ __global__ void __launch_bounds__(kFpThreads, 1) fp8_attn_prompt_kernel(const __
                         mma_f16_ta(tmem + t * 256 + 128, tmem + t * 256 + 8 * k, smem_desc(vb + k * 2048, kFpTile / 2, 1024, kLayoutSw128), idesc_pv, (j | k) != 0);
                     if (t == 1) mma_commit(smem_u32(&misc.v_free[st]));
                     if (j + 1 < n) {
-                        scores(t, j + 1);
-                        if (t == 1) mma_commit(smem_u32(&misc.k_free[st ^ 1]));
+                        scores(t, kst);
                     } else {
                         mma_commit(smem_u32(&misc.o_done[t]));
                     }
                 }
             }
         } else {
-            // ================================================================ codes to fp16
+            // ================================================================ copies, and values' codes to fp16
             const int cw = warp == 0 ? 0 : warp - 1, piece = lane & 7, r4 = lane >> 3, none = a.pages.n_pages * a.G * ps;      // (rows from `none` on are outside the maps: zeros)
             const bool slot_ok = (unsigned)slot < (unsigned)a.pages.slots;
             const int* pt = a.pages.table + (slot_ok ? (long)slot * a.pages.max_pages : 0);
@@ -126,8 +127,8 @@ __global__ void __launch_bounds__(kFpThreads, 1) fp8_attn_prompt_kernel(const __
                 tma_load_2d(dst + kFpCodes / 2, map, smem_u32(bar), 0, r1);
             };
             // rows 4 i + r4 of the tile, 16 codes a lane, into the 128-byte-swizzled operand: two blocks of 64 columns, rows of 128 bytes
-            auto turn = [&](uint32_t src, uint32_t dst, bool values, int k0) {
-                const bool partial = values && !(k0 >= last_first && k0 + kFpKeys - 1 <= pos0), edge = values && (k0 < lo || k0 + kFpKeys > k_hi);
+            auto turn = [&](uint32_t src, uint32_t dst, int k0) {
+                const bool partial = !(k0 >= last_first && k0 + kFpKeys - 1 <= pos0), edge = k0 < lo || k0 + kFpKeys > k_hi;
 #pragma unroll 4
                 for (int i = cw; i < 32; i += 3) {
                     const int r = 4 * i + r4;
@@ -166,37 +167,45 @@ __global__ void __launch_bounds__(kFpThreads, 1) fp8_attn_prompt_kernel(const __
                 fence_async_smem();
             };
             auto together = [] { asm volatile("barrier.cta.sync 2, 96;" ::: "memory"); };
-            int r0 = row_of(k_lo), r1 = row_of(k_lo + 64);
+            const int r0 = row_of(k_lo), r1 = row_of(k_lo + 64);
+            int n0 = row_of(k_lo + 128), n1 = row_of(k_lo + 192);      // the next tile's runs
             if (warp == 0 && lane == 0) {
-                bring(k8base, &maps.k, &misc.k8_full, r0, r1);
-                bring(v8base, &maps.v, &misc.v8_full, r0, r1);
+                bring(kbase, &maps.k, &misc.k_full[0], r0, r1);
+                bring(v8base, &maps.v, &misc.v8_full[0], r0, r1);
+                if (n > 1) {
+                    bring(kbase + kFpCodes, &maps.k, &misc.k_full[1], n0, n1);
+                    bring(v8base + kFpCodes, &maps.v, &misc.v8_full[1], n0, n1);
+                }
             }
-            for (int j = 0; j < n; j++) {
-                const int st = j & 1, ph = ((j >> 1) & 1) ^ 1, k0 = k_lo + j * kFpKeys;
-                if (warp == 2 && lane < 2) {      // the runs' scales
-                    const int row = lane ? r1 : r0;
+            auto scales_of = [&](int j, int a0, int a1) {      // a tile's runs'
+                if (warp == 2 && lane < 2) {
+                    const int row = lane ? a1 : a0;
                     misc.scales[j & 3][lane] = row == none ? make_float2(0.f, 0.f) : *reinterpret_cast<const float2*>(a.scales + 2 * (long)(row / ps));
                 }
-                r0 = row_of(k0 + kFpKeys);
-                r1 = row_of(k0 + kFpKeys + 64);
-                bar_wait(smem_u32(&misc.k8_full), j & 1);
-                bar_wait(smem_u32(&misc.k_free[st]), ph);
-                turn(k8base, kbase + st * kFpTile, false, k0);
-                together();
-                if (lane == 0) {
-                    bar_arrive(smem_u32(&misc.k_full[st]));
-                    if (warp == 0 && j + 1 < n) bring(k8base, &maps.k, &misc.k8_full, r0, r1);
+            };
+            scales_of(0, r0, r1);
+            __syncwarp();
+            if (warp == 2 && lane == 0) bar_arrive(smem_u32(&misc.q_full));      // (S of the first tile waits for its scales too)
+            for (int j = 0; j < n; j++) {
+                const int st = j & 1, k0 = k_lo + j * kFpKeys, l0 = row_of(k0 + 2 * kFpKeys), l1 = row_of(k0 + 2 * kFpKeys + 64);      // (the tile after the next)
+                if (j + 1 < n) scales_of(j + 1, n0, n1);      // (S of that tile waits for this one's values)
+                if (warp == 0 && lane == 0 && j + 2 < n) {      // (its stage was tile j - 1's)
+                    const int kst = (j + 2) % kFpKStages;
+                    bar_wait(smem_u32(&misc.k_free[kst]), (((j + 2) / kFpKStages) & 1) ^ 1);
+                    bring(kbase + kst * kFpCodes, &maps.k, &misc.k_full[kst], l0, l1);
                 }
                 __syncwarp();
-                bar_wait(smem_u32(&misc.v8_full), j & 1);
-                bar_wait(smem_u32(&misc.v_free[st]), ph);
-                turn(v8base, vbase + st * kFpTile, true, k0);
+                bar_wait(smem_u32(&misc.v8_full[st]), (j >> 1) & 1);
+                bar_wait(smem_u32(&misc.v_free[st]), ((j >> 1) & 1) ^ 1);
+                turn(v8base + st * kFpCodes, vbase + st * kFpTile, k0);
                 together();
                 if (lane == 0) {
                     bar_arrive(smem_u32(&misc.v_full[st]));
-                    if (warp == 0 && j + 1 < n) bring(v8base, &maps.v, &misc.v8_full, r0, r1);
+                    if (warp == 0 && j + 2 < n) bring(v8base + st * kFpCodes, &maps.v, &misc.v8_full[st], l0, l1);
                 }
                 __syncwarp();
+                n0 = l0;
+                n1 = l1;
             }
         }
     } else {
@@ -216,18 +225,29 @@ __global__ void __launch_bounds__(kFpThreads, 1) fp8_attn_prompt_kernel(const __
                 const uint4 v = valid ? row[i] : make_uint4(0, 0, 0, 0);
                 w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
             }
-            float top = 0.f;
+            float top = 0.f, odd = 0.f;      // odd: NaN as soon as a value is not finite (e4m3 has no infinity)
 #pragma unroll
-            for (int i = 0; i < 64; i++) top = fmaxf(top, fmaxf(fabsf(__uint_as_float(w[i] << 16)), fabsf(__uint_as_float(w[i] & 0xffff0000u))));
-            const int up = min(126, max(-112, 13 - ((int)(__float_as_uint(top) >> 23) - 127)));      // (an infinity stays one)
+            for (int i = 0; i < 64; i++) {
+                const float x = __uint_as_float(w[i] << 16), y = __uint_as_float(w[i] & 0xffff0000u);
+                top = fmaxf(top, fmaxf(fabsf(x), fabsf(y)));
+                odd = fmaf(x, 0.f, fmaf(y, 0.f, odd));
+            }
+            const int up = min(126, max(-120, 7 - ((int)(__float_as_uint(top) >> 23) - 127)));
             const float by = __uint_as_float((uint32_t)(up + 127) << 23);
-            fac = valid ? (a.head_scale ? a.scale * a.head_scale[h] : a.scale) / by : 0.f;
+            fac = valid ? (a.head_scale ? a.scale * a.head_scale[h] : a.scale) / by + odd : 0.f;
+            uint8_t* to = smem + t * kFpTile + r * 128;
 #pragma unroll
-            for (int c = 0; c < 16; c++) {
-                uint32_t f[4];
+            for (int c = 0; c < 8; c++) {      // 16 columns, both terms
+                uint32_t f[4], e[4];
 #pragma unroll
-                for (int i = 0; i < 4; i++) f[i] = pack_f16(__uint_as_float(w[4 * c + i] << 16) * by, __uint_as_float(w[4 * c + i] & 0xffff0000u) * by);
-                *reinterpret_cast<uint4*>(smem + t * kFpTile + (c >> 3) * (kFpTile / 2) + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = make_uint4(f[0], f[1], f[2], f[3]);
+                for (int i = 0; i < 4; i++) {
+                    const uint32_t u = w[8 * c + 2 * i], v = w[8 * c + 2 * i + 1];
+                    const uint2 lo2 = split_e4m3<1>(__uint_as_float(u << 16) * by, __uint_as_float(u & 0xffff0000u) * by), hi2 = split_e4m3<1>(__uint_as_float(v << 16) * by, __uint_as_float(v & 0xffff0000u) * by);
+                    f[i] = lo2.x | hi2.x << 16;
+                    e[i] = lo2.y | hi2.y << 16;
+                }
+                *reinterpret_cast<uint4*>(to + ((c ^ (r & 7)) << 4)) = make_uint4(f[0], f[1], f[2], f[3]);
+                *reinterpret_cast<uint4*>(to + kFpCodes + ((c ^ (r & 7)) << 4)) = make_uint4(e[0], e[1], e[2], e[3]);
             }
             fence_async_smem();
             __syncwarp();
@@ -400,7 +420,7 @@ static bool fp_takes(const ktb200_fp8_attn_params* c, int n_tokens, int dtype) {
 }
 static int fp_launch(const Fp8Attn& a, int RH, dim3 grid, cudaStream_t s) {
     FdMaps maps;
-    const int rc = fd_maps(maps, a, 64, CU_TENSOR_MAP_SWIZZLE_NONE);
+    const int rc = fd_maps(maps, a, 64, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_SWIZZLE_NONE);
     if (rc) return rc;
     KTB_CUDA_CHECK(raise_smem_limit((const void*)fp8_attn_prompt_kernel, kFpSmem));
     KTB_CUDA_CHECK(launch_pdl(fp8_attn_prompt_kernel, grid, dim3(kFpThreads), (size_t)kFpSmem, s, maps, a, RH));
