@@ -112,7 +112,7 @@ __global__ void __launch_bounds__(kFpThreads, 1) fp8_attn_prompt_kernel(const __
             }
         } else {
             // ================================================================ copies, and values' codes to fp16
-            const int cw = warp == 0 ? 0 : warp - 1, piece = lane & 7, r4 = lane >> 3, none = a.pages.n_pages * a.G * ps;      // (rows from `none` on are outside the maps: zeros)
+            const int cw = warp == 0 ? 0 : warp - 1, none = a.pages.n_pages * a.G * ps;      // (rows from `none` on are outside the maps: zeros)
             const bool slot_ok = (unsigned)slot < (unsigned)a.pages.slots;
             const int* pt = a.pages.table + (slot_ok ? (long)slot * a.pages.max_pages : 0);
             const int last_first = fp8_first_visible(max_pos, a.window, a.chunk);
@@ -126,13 +126,14 @@ __global__ void __launch_bounds__(kFpThreads, 1) fp8_attn_prompt_kernel(const __
                 tma_load_2d(dst, map, smem_u32(bar), 0, r0);
                 tma_load_2d(dst + kFpCodes / 2, map, smem_u32(bar), 0, r1);
             };
-            // rows 4 i + r4 of the tile, 16 codes a lane, into the 128-byte-swizzled operand: two blocks of 64 columns, rows of 128 bytes
+            // 8 rows and 4 of their 8 pieces of 16 codes at a time, into the operand: two blocks of 64 columns, rows of 128 bytes.  Both sides are 128-byte-swizzled, so that no two of the lanes
+            // that read or write together meet in a bank
             auto turn = [&](uint32_t src, uint32_t dst, int k0) {
                 const bool partial = !(k0 >= last_first && k0 + kFpKeys - 1 <= pos0), edge = k0 < lo || k0 + kFpKeys > k_hi;
 #pragma unroll 4
                 for (int i = cw; i < 32; i += 3) {
-                    const int r = 4 * i + r4;
-                    const uint4 v = lds16(src + r * 128 + piece * 16);
+                    const int r = 8 * (i >> 1) + (lane & 7), piece = 4 * (i & 1) + (lane >> 3);
+                    const uint4 v = lds16(src + r * 128 + ((piece ^ (lane & 7)) << 4));
                     uint32_t w[4] = {v.x, v.y, v.z, v.w};
                     if (edge && (k0 + r < lo || k0 + r >= k_hi)) w[0] = w[1] = w[2] = w[3] = 0;      // values that no row sees may be anything (0 x NaN)
                     if (partial) {      // a value that is NaN belongs to the rows that see it: they are told at the end
@@ -153,16 +154,10 @@ __global__ void __launch_bounds__(kFpThreads, 1) fp8_attn_prompt_kernel(const __
                     uint32_t f[8];
 #pragma unroll
                     for (int q = 0; q < 4; q++) { f[2 * q] = f16_of_codes(w[q]); f[2 * q + 1] = f16_of_codes(w[q] >> 16); }
-                    const uint32_t at = dst + (piece >> 2) * (kFpTile / 2) + r * 128;
-                    const int c = 2 * (piece & 3);
-                    // (the second block's lanes begin with their second half: no two lanes meet in a bank)
+                    const uint32_t at = dst + (i & 1) * (kFpTile / 2) + r * 128;
 #pragma unroll
-                    for (int e = 0; e < 2; e++) {
-                        const int h = e ^ (piece >> 2);
-                        const uint32_t to = at + (((c + h) ^ (r & 7)) << 4);
-                        const uint32_t x0 = h ? f[4] : f[0], x1 = h ? f[5] : f[1], x2 = h ? f[6] : f[2], x3 = h ? f[7] : f[3];
-                        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(x0), "r"(x1), "r"(x2), "r"(x3) : "memory");
-                    }
+                    for (int e = 0; e < 2; e++)
+                        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at + (((2 * (piece & 3) + e) ^ (lane & 7)) << 4)), "r"(f[4 * e]), "r"(f[4 * e + 1]), "r"(f[4 * e + 2]), "r"(f[4 * e + 3]) : "memory");
                 }
                 fence_async_smem();
             };
@@ -420,7 +415,7 @@ static bool fp_takes(const ktb200_fp8_attn_params* c, int n_tokens, int dtype) {
 }
 static int fp_launch(const Fp8Attn& a, int RH, dim3 grid, cudaStream_t s) {
     FdMaps maps;
-    const int rc = fd_maps(maps, a, 64, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_SWIZZLE_NONE);
+    const int rc = fd_maps(maps, a, 64);
     if (rc) return rc;
     KTB_CUDA_CHECK(raise_smem_limit((const void*)fp8_attn_prompt_kernel, kFpSmem));
     KTB_CUDA_CHECK(launch_pdl(fp8_attn_prompt_kernel, grid, dim3(kFpThreads), (size_t)kFpSmem, s, maps, a, RH));

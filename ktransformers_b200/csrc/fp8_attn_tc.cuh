@@ -398,15 +398,15 @@ template <int RP> static cudaError_t fd_launch_as(const FdMaps& maps, const Fp8A
     lc.numAttrs = n;
     return cudaLaunchKernelEx(&lc, fp8_attn_decode_kernel<RP>, maps, a, RH, run);
 }
-// the codes as rows of 128 bytes, boxes of `run` rows
-static int fd_maps(FdMaps& maps, const Fp8Attn& a, int run, CUtensorMapSwizzle k_swizzle, CUtensorMapSwizzle v_swizzle) {
+// the codes as rows of 128 bytes, boxes of `run` rows, 128-byte-swizzled
+static int fd_maps(FdMaps& maps, const Fp8Attn& a, int run) {
     const umma::EncodeTiledFn enc = umma::encode_tiled();
     if (!enc) { set_error("fp8_cache_attn: cuTensorMapEncodeTiled is not available from this driver"); return KTB200_ECUDA; }
     const cuuint64_t dims[2] = {128, (cuuint64_t)a.pages.n_pages * a.G * a.pages.page_size}, strides[1] = {128};
     const cuuint32_t box[2] = {128, (cuuint32_t)run}, estr[2] = {1, 1};
     for (int i = 0; i < 2; i++) {
         const CUresult cr = enc(i ? &maps.v : &maps.k, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t*>(i ? a.v_codes : a.k_codes), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                                i ? v_swizzle : k_swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
         if (cr != CUDA_SUCCESS) { set_error("fp8_cache_attn: cuTensorMapEncodeTiled failed (%d)", (int)cr); return KTB200_ECUDA; }
     }
     return KTB200_OK;
@@ -414,7 +414,7 @@ static int fd_maps(FdMaps& maps, const Fp8Attn& a, int run, CUtensorMapSwizzle k
 static int fd_launch(const Fp8Attn& a, int RH, dim3 grid, cudaStream_t s) {
     const int ps = a.pages.page_size, run = ps % 64 == 0 ? 64 : ps % 32 == 0 ? 32 : 16;
     FdMaps maps;
-    const int rc = fd_maps(maps, a, run, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_SWIZZLE_128B);
+    const int rc = fd_maps(maps, a, run);
     if (rc) return rc;
     KTB_CUDA_CHECK(RH <= 8 ? fd_launch_as<8>(maps, a, RH, run, grid, s) : fd_launch_as<16>(maps, a, RH, run, grid, s));
     return KTB200_OK;
