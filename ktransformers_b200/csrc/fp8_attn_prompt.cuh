@@ -4,14 +4,14 @@
 // tiles of 128 from a multiple of 128 on.
 //     warps 0, 2, 3   values: TMA brings a tile's codes, the warps turn them into swizzled fp16 operands, which hold every e4m3 number exactly (a conversion for two codes).  Keys need none:
 //                     warp 0 has their codes brought as operands
-//     warp 1          MMAs: S = Q K^T (kind::f8f6f4) from shared memory, O += P V (kind::f16) with P in tensor memory.  The tiles take turns, S of the next key tile right behind PV of this
-//                     one, so that one tile's soft-max runs beside the other's products
+//     warp 1          MMAs of 64 keys at a time: S = Q K^T (kind::f8f6f4) from shared memory, O += P V (kind::f16) with P in tensor memory.  A row tile has two buffers of 64 scores: S of the
+//                     next 64 keys is there before the soft-max of these is done, which so never waits for a product
 //     warps 4-7       soft-max of the first tile, 8-11 of the second: a thread owns a row.  First it makes its row of Q: moved by a power of two so that its largest stands in [128, 256) and
 //                     split into two e4m3 numbers, q = q1 + q2, whose products add up in one sum: exact for bf16 numbers down to 2^-9 of the largest, 2^-17 of it off below.
 //                     t = s log2(e) + log2(value scale), p = 2^(t - m), l += p / (value scale): scales are one number a page and head, so that of 64 scores at a time they change the
 //                     factor and the offset of an fma that is there anyway, and O needs none.  P (fp16, 2^-11 of a weight off at most) replaces its S in tensor memory; m is raised,
 //                     and O scaled in tensor memory, only when a row's t outgrows it by 8
-// TMEM: [S0 | O0 | S1 | O1], 128 columns each.  Shared memory: Q 64 KB, K 3 x 16 KB, V 2 x 32 KB as fp16 and 2 x 16 KB as codes.
+// TMEM: [S0 | O0 | S1 | O1], 128 columns each (S: two buffers of 64).  Shared memory: Q 64 KB, K 3 x 16 KB, V 2 x 32 KB as fp16 and 2 x 16 KB as codes.
 // (With keys turned into fp16 as well the three warps were the bound: 2048 tokens behind 2001 took 318 us, 228 with their work left out.)
 #pragma once
 #include <cuda.h>
@@ -22,7 +22,7 @@ namespace ktb {
 
 constexpr int kFpThreads = 384, kFpKeys = 128, kFpTile = 128 * 128 * 2, kFpCodes = 128 * 128, kFpKStages = 3, kFpBad = 64;
 struct FpMisc {
-    unsigned long long q_full, v8_full[2], k_full[kFpKStages], k_free[kFpKStages], v_full[2], v_free[2], s_full[2], p_full[2], o_done[2];
+    unsigned long long q_full, v8_full[2], k_full[kFpKStages], k_free[kFpKStages], v_full[2], v_free[2], s_full[2][2], p_full[2][2], pv_done[2];      // [row tile][buffer]
     float2 scales[4][2];      // of a tile's two runs of 64 keys (zeros: not there)
     uint32_t tmem_base;
     int info[4], n_bad, bad_lo, bad_hi;
@@ -45,7 +45,8 @@ __global__ void __launch_bounds__(kFpThreads, 1) fp8_attn_prompt_kernel(const __
         for (int i = 0; i < kFpKStages; i++) { bar_init(smem_u32(&misc.k_full[i]), 1); bar_init(smem_u32(&misc.k_free[i]), 1); }
         for (int i = 0; i < 2; i++) {
             bar_init(smem_u32(&misc.v8_full[i]), 1); bar_init(smem_u32(&misc.v_full[i]), 3); bar_init(smem_u32(&misc.v_free[i]), 1);
-            bar_init(smem_u32(&misc.s_full[i]), 1); bar_init(smem_u32(&misc.p_full[i]), 4); bar_init(smem_u32(&misc.o_done[i]), 1);
+            bar_init(smem_u32(&misc.pv_done[i]), 1);
+            for (int b = 0; b < 2; b++) { bar_init(smem_u32(&misc.s_full[i][b]), 1); bar_init(smem_u32(&misc.p_full[i][b]), 4); }
         }
         bar_fence_init();
         misc.n_bad = 0;
@@ -76,38 +77,38 @@ __global__ void __launch_bounds__(kFpThreads, 1) fp8_attn_prompt_kernel(const __
         asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
         if (warp == 1) {
             // ================================================================ products (converged warp)
-            constexpr uint32_t idesc_qk = instr_desc(1, 0, 0, 0, 0, 128, 128), idesc_pv = instr_desc(1, 0, 0, 0, 1, 128, 128);      // V [key][column]: B MN-major
-            auto scores = [&](int t, int kst) {
+            constexpr uint32_t idesc_qk = instr_desc(1, 0, 0, 0, 0, 128, 64), idesc_pv = instr_desc(1, 0, 0, 0, 1, 128, 128);      // V [key][column]: B MN-major
+            int kst = 0, kph = 0;      // the stage and phase of the keys that S takes next
+            auto scores = [&](int t, int i) {      // of the i-th 64 keys
                 const uint32_t qb = base + t * kFpTile;
-                const uint64_t k = smem_desc(kbase + kst * kFpCodes, 16, 1024, kLayoutSw128);
-                mma_f8_x4(tmem + t * 256, smem_desc(qb, 16, 1024, kLayoutSw128), k, idesc_qk, 0);
-                mma_f8_x4(tmem + t * 256, smem_desc(qb + kFpCodes, 16, 1024, kLayoutSw128), k, idesc_qk, 1, smem_u32(&misc.s_full[t]), t ? smem_u32(&misc.k_free[kst]) : 0);
+                const uint64_t k = smem_desc(kbase + kst * kFpCodes + (i & 1) * (kFpCodes / 2), 16, 1024, kLayoutSw128);
+                const uint32_t d = tmem + t * 256 + (i & 1) * 64;
+                mma_f8_x4(d, smem_desc(qb, 16, 1024, kLayoutSw128), k, idesc_qk, 0);
+                mma_f8_x4(d, smem_desc(qb + kFpCodes, 16, 1024, kLayoutSw128), k, idesc_qk, 1, smem_u32(&misc.s_full[t][i & 1]), t && (i & 1) ? smem_u32(&misc.k_free[kst]) : 0);
             };
             bar_wait(smem_u32(&misc.q_full), 0);
             bar_wait(smem_u32(&misc.k_full[0]), 0);
             tc_fence_after();
-            scores(0, 0);
-            scores(1, 0);
-            int kst = 0, kph = 0;
-            for (int j = 0; j < n; j++) {
-                const int st = j & 1;
-                const uint32_t vb = vbase + st * kFpTile;
-                bar_wait(smem_u32(&misc.v_full[st]), (j >> 1) & 1);
-                if (++kst == kFpKStages) { kst = 0; kph ^= 1; }
-                if (j + 1 < n) bar_wait(smem_u32(&misc.k_full[kst]), kph);
+#pragma unroll 1
+            for (int i = 0; i < 4; i++) scores(i & 1, i >> 1);
+            for (int i = 0; i < 2 * n; i++) {
+                const int j = i >> 1, st = j & 1, buf = i & 1;
+                const uint32_t vb = vbase + st * kFpTile + buf * 4 * 2048;
+                if (buf == 0) {
+                    bar_wait(smem_u32(&misc.v_full[st]), (j >> 1) & 1);
+                    if (++kst == kFpKStages) { kst = 0; kph ^= 1; }
+                    if (j + 1 < n) bar_wait(smem_u32(&misc.k_full[kst]), kph);
+                }
 #pragma unroll 1
                 for (int t = 0; t < 2; t++) {
-                    bar_wait(smem_u32(&misc.p_full[t]), j & 1);
+                    bar_wait(smem_u32(&misc.p_full[t][buf]), j & 1);
                     tc_fence_after();
 #pragma unroll
-                    for (int k = 0; k < 8; k++)
-                        mma_f16_ta(tmem + t * 256 + 128, tmem + t * 256 + 8 * k, smem_desc(vb + k * 2048, kFpTile / 2, 1024, kLayoutSw128), idesc_pv, (j | k) != 0);
-                    if (t == 1) mma_commit(smem_u32(&misc.v_free[st]));
-                    if (j + 1 < n) {
-                        scores(t, kst);
-                    } else {
-                        mma_commit(smem_u32(&misc.o_done[t]));
-                    }
+                    for (int k = 0; k < 4; k++)
+                        mma_f16_ta(tmem + t * 256 + 128, tmem + t * 256 + buf * 64 + 8 * k, smem_desc(vb + k * 2048, kFpTile / 2, 1024, kLayoutSw128), idesc_pv, (i | k) != 0);
+                    mma_commit(smem_u32(&misc.pv_done[t]));
+                    if (t == 1 && buf == 1) mma_commit(smem_u32(&misc.v_free[st]));
+                    if (j + 1 < n) scores(t, i);      // (of 128 keys on)
                 }
             }
         } else {
@@ -255,62 +256,55 @@ __global__ void __launch_bounds__(kFpThreads, 1) fp8_attn_prompt_kernel(const __
         const bool w_full = w_tok1 < ntok;
         const int w_last_first = fp8_first_visible(pos0 + w_tok1, a.window, a.chunk);
         float m_ref = -INFINITY, l = 0.f;
-        for (int j = 0; j < n; j++) {
-            const int k0 = k_lo + j * kFpKeys;
-            bar_wait(smem_u32(&misc.s_full[t]), j & 1);      // (also: PV of the tile before this one is complete)
+        for (int i64 = 0; i64 < 2 * n; i64++) {
+            const int k0 = k_lo + 64 * i64, buf = i64 & 1;
+            const uint32_t tb = ts + 64 * buf;
+            bar_wait(smem_u32(&misc.s_full[t][buf]), (i64 >> 1) & 1);
             tc_fence_after();
-            float s[kFpKeys];
+            float s[64];
 #pragma unroll
-            for (int q = 0; q < 4; q++) {
+            for (int q = 0; q < 2; q++) {
                 uint32_t v[32];
-                tmem_ld32(ts + 32 * q, v);
+                tmem_ld32(tb + 32 * q, v);
 #pragma unroll
                 for (int i = 0; i < 32; i++) s[32 * q + i] = __uint_as_float(v[i]);
             }
-            float c[2], ve[2], inv[2];
-            bool there = true;
-#pragma unroll
-            for (int q = 0; q < 2; q++) {
-                const float2 sc = misc.scales[j & 3][q];
-                const uint32_t vb = __float_as_uint(sc.y);
-                c[q] = direct ? fmaxf(fac * sc.x * kLog2e, 1.2e-38f) : fac * sc.x;      // (above zero: -inf times it stays that)
-                ve[q] = (float)((int)(vb >> 23) - 127);
-                inv[q] = vb ? __uint_as_float((254u << 23) - vb) : 0.f;
-                there &= vb != 0;
-            }
+            const float2 sc = misc.scales[(i64 >> 1) & 3][buf];
+            const uint32_t vbits = __float_as_uint(sc.y);
+            float c = direct ? fmaxf(fac * sc.x * kLog2e, 1.2e-38f) : fac * sc.x;      // (above zero: -inf times it stays that)
+            const float ve = (float)((int)(vbits >> 23) - 127), inv = vbits ? __uint_as_float((254u << 23) - vbits) : 0.f;
             tmem_wait_ld();
             // (the loads above are in registers only now)
 #pragma unroll
-            for (int i = 0; i < kFpKeys; i++) asm volatile("" : "+f"(s[i]));
+            for (int i = 0; i < 64; i++) asm volatile("" : "+f"(s[i]));
             if (!direct) {
 #pragma unroll
-                for (int i = 0; i < kFpKeys; i++) {
-                    float x = s[i] * c[i >> 6];
+                for (int i = 0; i < 64; i++) {
+                    float x = s[i] * c;
                     if (softcap > 0.f) x = softcap * (1.0f - __fdividef(2.0f, __expf(x * two_over_cap) + 1.0f));      // c tanh(s / c): a few 1e-7 of the cap off
                     s[i] = x * kLog2e;
                 }
-                c[0] = c[1] = 1.f;
+                c = 1.f;
             }
-            if (!(there && w_full && k0 + kFpKeys <= k_hi && k0 + kFpKeys - 1 <= pos0 + w_tok0 && k0 >= w_last_first)) {
-                const int i0 = first - k0, i1 = valid ? min(p, k_hi - 1) - k0 : -1;
+            if (!(vbits && w_full && k0 + 64 <= k_hi && k0 + 63 <= pos0 + w_tok0 && k0 >= w_last_first)) {
+                const int i0 = first - k0, i1 = valid && vbits ? min(p, k_hi - 1) - k0 : -1;
 #pragma unroll
-                for (int i = 0; i < kFpKeys; i++)
-                    if (i < i0 || i > i1 || inv[i >> 6] == 0.f) s[i] = -INFINITY;
+                for (int i = 0; i < 64; i++)
+                    if (i < i0 || i > i1) s[i] = -INFINITY;
             }
-            float mx[4] = {s[0], s[1], s[64], s[65]};
+            float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-            for (int i = 2; i < 64; i += 2) {
-                mx[0] = fmaxf(mx[0], s[i]);
-                mx[1] = fmaxf(mx[1], s[i + 1]);
-                mx[2] = fmaxf(mx[2], s[64 + i]);
-                mx[3] = fmaxf(mx[3], s[64 + i + 1]);
-            }
-            const float m_new = fmaxf(fmaf(fmaxf(mx[0], mx[1]), c[0], ve[0]), fmaf(fmaxf(mx[2], mx[3]), c[1], ve[1]));
+            for (int i = 4; i < 64; i += 4)
+#pragma unroll
+                for (int q = 0; q < 4; q++) mx[q] = fmaxf(mx[q], s[i + q]);
+            const float m_new = fmaf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), c, ve);
             const bool raise = m_new > m_ref + 8.f || (m_ref == -INFINITY && m_new > -INFINITY);
             if (__any_sync(0xffffffffu, raise)) {
                 const float alpha = raise ? exp2_approx(m_ref - m_new) : 1.f;      // (2^-inf = 0: nothing was summed yet)
                 if (raise) { m_ref = m_new; l *= alpha; }
-                if (j > 0) {
+                if (i64 > 0) {
+                    bar_wait(smem_u32(&misc.pv_done[t]), (i64 - 1) & 1);
+                    tc_fence_after();
 #pragma unroll 1
                     for (int q = 0; q < 4; q++) {
                         uint32_t v[32];
@@ -323,32 +317,31 @@ __global__ void __launch_bounds__(kFpThreads, 1) fp8_attn_prompt_kernel(const __
                 }
             }
             const float u = m_ref == -INFINITY ? 0.f : m_ref;
+            const f32x2 c2 = pack2(c, c), o2 = pack2(ve - u, ve - u);
+            f32x2 sum[2] = {0, 0};
+            uint32_t pk[32];
 #pragma unroll
-            for (int q = 0; q < 2; q++) {
-                const f32x2 c2 = pack2(c[q], c[q]), o2 = pack2(ve[q] - u, ve[q] - u);
-                f32x2 sum[2] = {0, 0};
-                uint32_t pk[32];
-#pragma unroll
-                for (int i = 0; i < 32; i++) {
-                    float e0, e1;
-                    unpack2(fma2(pack2(s[64 * q + 2 * i], s[64 * q + 2 * i + 1]), c2, o2), e0, e1);
-                    e0 = exp2_approx(e0);
-                    e1 = exp2_approx(e1);
-                    pk[i] = pack_f16(e0, e1);
-                    sum[i & 1] = add2(sum[i & 1], pack2(e0, e1));
-                }
-                tmem_st32(ts + 32 * q, pk);
-                float a0, a1, a2, a3;
-                unpack2(sum[0], a0, a1);
-                unpack2(sum[1], a2, a3);
-                l = fmaf((a0 + a1) + (a2 + a3), inv[q], l);
+            for (int i = 0; i < 32; i++) {
+                float e0, e1;
+                unpack2(fma2(pack2(s[2 * i], s[2 * i + 1]), c2, o2), e0, e1);
+                e0 = exp2_approx(e0);
+                e1 = exp2_approx(e1);
+                pk[i] = pack_f16(e0, e1);
+                sum[i & 1] = add2(sum[i & 1], pack2(e0, e1));
             }
+            tmem_st32(tb, pk);
             tmem_wait_st();
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) bar_arrive(smem_u32(&misc.p_full[t]));
+            if (lane == 0) bar_arrive(smem_u32(&misc.p_full[t][buf]));
+            float a0, a1, a2, a3;
+            unpack2(sum[0], a0, a1);
+            unpack2(sum[1], a2, a3);
+            l = fmaf((a0 + a1) + (a2 + a3), inv, l);
         }
-        bar_wait(smem_u32(&misc.o_done[t]), 0);
+        // the last two of an even number of products (the scores that the loop waited for last were behind all others)
+        bar_wait(smem_u32(&misc.pv_done[t]), 0);
+        bar_wait(smem_u32(&misc.pv_done[t]), 1);
         tc_fence_after();
         const long row = (long)(tok0 + tok) * a.H + h;
         float* part = cut ? a.partial + (row * a.parts + blockIdx.z) * 130 : nullptr;
