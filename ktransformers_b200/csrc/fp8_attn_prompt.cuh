@@ -56,11 +56,11 @@ __global__ void __launch_bounds__(kFpThreads, 1) fp8_attn_prompt_kernel(const __
         tma_prefetch_desc(&maps.v);
     }
     griddep_wait();
-    if (warp == 1) fp8_find_tokens(a, gridDim.x - 1 - blockIdx.x, 2 * TOKS, misc.info);      // the last tokens, which see most keys, first
+    if (warp == 1) fp8_find_tokens(a, gridDim.y - 1 - blockIdx.y, 2 * TOKS, misc.info);      // the last tokens, which see most keys, first
     __syncthreads();
     const int tok0 = misc.info[0], ntok = misc.info[1], pos0 = misc.info[2], slot = misc.info[3];
     if (ntok <= 0) return;
-    const int g = blockIdx.y / hblocks, h0 = g * R + (blockIdx.y % hblocks) * RH;
+    const int g = blockIdx.x / hblocks, h0 = g * R + (blockIdx.x % hblocks) * RH;
     const int max_pos = pos0 + ntok - 1, lo = fp8_first_visible(pos0, a.window, a.chunk), lo_al = lo & ~(kFpKeys - 1);
     const bool cut = a.part > 0 && max_pos + 1 - lo_al > a.part;
     const int k_lo = lo_al + blockIdx.z * a.part, k_hi = cut ? min(max_pos + 1, k_lo + a.part) : max_pos + 1;
@@ -411,7 +411,8 @@ static int fp_launch(const Fp8Attn& a, int RH, dim3 grid, cudaStream_t s) {
     const int rc = fd_maps(maps, a, 64);
     if (rc) return rc;
     KTB_CUDA_CHECK(raise_smem_limit((const void*)fp8_attn_prompt_kernel, kFpSmem));
-    KTB_CUDA_CHECK(launch_pdl(fp8_attn_prompt_kernel, grid, dim3(kFpThreads), (size_t)kFpSmem, s, maps, a, RH));
+    if (grid.x > 65535) { set_error("fp8_cache_attn: too many tokens"); return KTB200_EINVAL; }
+    KTB_CUDA_CHECK(launch_pdl(fp8_attn_prompt_kernel, dim3(grid.y, grid.x, grid.z), dim3(kFpThreads), (size_t)kFpSmem, s, maps, a, RH));
     return KTB200_OK;
 }
 
