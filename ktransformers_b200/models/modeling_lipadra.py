@@ -72,9 +72,15 @@ class LipadraForCausalLM(nn.Module):
             layer.load(loader, f"l{i}.")
         self.final_norm.load(loader, "final.norm")
 
-    def make_cache(self, max_tokens: int, max_slots: int = 8, page_size: int = 64) -> PagedStateCache:
+    kv_cache_kinds = ("fp8",)      # what `make_cache` holds attention rows in besides the model's own type
+
+    def make_cache(self, max_tokens: int, max_slots: int = 8, page_size: int = 64, kv_cache: Optional[str] = None) -> PagedStateCache:
+        """`kv_cache` = "fp8": the attention layers' keys and values as e4m3 codes with a scale per page and head (custom_cache.Fp8CacheLayer), half the bytes of bf16."""
+        if kv_cache is not None and kv_cache not in self.kv_cache_kinds:
+            raise ValueError(f"Lipadra: no {kv_cache!r} cache, only {self.kv_cache_kinds}")
         c = self.config
-        return PagedStateCache(c.cache_row_widths(), c.state_widths(), max_tokens, max_slots, self.device, dtype=self.dtype, page_size=page_size, window=None, chunks=c.chunks())
+        fp8 = [(l.mixer.kv_heads, l.mixer.dim, l.mixer.vdim) if l.type == "attention" else None for l in c.layers] if kv_cache == "fp8" else None
+        return PagedStateCache(c.cache_row_widths(), c.state_widths(), max_tokens, max_slots, self.device, dtype=self.dtype, page_size=page_size, window=None, chunks=c.chunks(), fp8_heads=fp8)
 
     def decode_is_capturable(self, max_batch: int = 47) -> bool:
         """Whether a decode step of up to `max_batch` sequences makes no host read (then the engine may replay it as a CUDA graph)."""

@@ -15,7 +15,7 @@ from typing import Optional, Tuple
 import torch
 
 from .. import native
-from ..models.custom_cache import StaticCache
+from ..models.custom_cache import Fp8CacheLayer, StaticCache
 from ..models.modeling_deepseek_v3 import DeepseekV3Attention, DeepseekV3RMSNorm, DeepseekV3RotaryEmbedding, apply_rotary_pos_emb
 from ..util.utils import InferenceState
 from .base_operator import BaseInjectedModule, device_of, stream_of
@@ -463,7 +463,13 @@ def paged_softmax_attention(q: torch.Tensor, kv: torch.Tensor, batch, cache, hea
     scale * head_scale[h] * q.k, squashed to c tanh(s / c) with c = softcap, less r1[h] ln(1 + r2[h] (i - j)) with dist_bias = (r1, r2); exp(sink[h])
     joins the denominator; fp32 scores and weights.  maps = 2: two attentions per head over the same values, combined as
     unit rms of (first - lam[0] second), `rms_eps` inside the root.  The result times out_scale times sigmoid(gate), element by element
-    (gate [T, heads * vdim], a view of any row stride), goes to `out` (a view of any row stride) or a new tensor."""
+    (gate [T, heads * vdim], a view of any row stride), goes to `out` (a view of any row stride) or a new tensor.  A layer held in 8 bits (models.custom_cache.Fp8CacheLayer) goes to
+    `fp8_cache_attention`, which has no second map, distance bias or gate."""
+    if isinstance(kv, Fp8CacheLayer):
+        if maps != 1 or dist_bias is not None or gate is not None:
+            raise ValueError("paged_softmax_attention: a cache layer in 8 bits takes one map, no distance bias and no gate")
+        return fp8_cache_attention(q, kv, batch, cache, heads, kv_heads, dim, vdim, scale, head_scale=head_scale, softcap=softcap, window=window, chunk=chunk, tensor_cores=tensor_cores, sink=sink,
+                                   out=out, out_scale=out_scale)
     T, dev, dt = q.shape[0], q.device, q.dtype
     lib, code, st = native.seq_lib(), native.GGML_BF16 if dt == torch.bfloat16 else native.GGML_F32, torch.cuda.current_stream(dev).cuda_stream
     o = torch.empty((T, heads * vdim), dtype=dt, device=dev) if out is None else out
@@ -492,7 +498,11 @@ def qkv_prep(proj: torch.Tensor, batch, cache, kv: torch.Tensor, heads: int, kv_
     """From a projection's q, k and v columns (`offsets`) to the queries [T, heads, maps * dim] and the [k | v] rows of cache layer `kv`, one
     `ktb200_qkv_prep` launch (csrc/softmax_attn.cu): a short causal filter on every channel (conv_w [channels, taps]; its last inputs per
     sequence live at the front of the `state` rows), the rotation, unit rms per row (qk_norm = 1; qk_norm = 3: per row, times q_weight / k_weight
-    [dim], ahead of the rotation)."""
+    [dim], ahead of the rotation).  A layer held in 8 bits (models.custom_cache.Fp8CacheLayer) goes to `fp8_cache_append`, which has one map, no filter and no row-wide norm."""
+    if isinstance(kv, Fp8CacheLayer):
+        if maps != 1 or conv_w is not None:
+            raise ValueError("qkv_prep: a cache layer in 8 bits takes one map and no filter")
+        return fp8_cache_append(proj, batch, cache, kv, heads, kv_heads, dim, vdim, offsets, rot=rot, inv_freq=inv_freq, qk_norm=qk_norm, eps=eps, q_weight=q_weight, k_weight=k_weight)
     T, dt = proj.shape[0], proj.dtype
     q = torch.empty((T, heads, maps * dim), dtype=dt, device=proj.device)
     ptr = lambda t: t.data_ptr() if t is not None else None

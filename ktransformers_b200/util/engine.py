@@ -68,9 +68,13 @@ class Engine:
 
     graph_max_batch = 47        # below the experts' and the router's switch to their prompt-sized paths
 
-    def __init__(self, model, max_tokens: int = 8192, max_slots: int = 8, page_size: int = 64, max_step_tokens: int = 2048, cuda_graphs: bool = True):
+    def __init__(self, model, max_tokens: int = 8192, max_slots: int = 8, page_size: int = 64, max_step_tokens: int = 2048, cuda_graphs: bool = True,
+                 kv_cache: Optional[str] = None):
+        """`kv_cache`: what the attention layers' rows are held in; None, the model's own type; "fp8", 8 bits with a scale per page and head, for models that say so in `kv_cache_kinds`."""
+        if kv_cache is not None and kv_cache not in getattr(model, "kv_cache_kinds", ()):
+            raise ValueError(f"{type(model).__name__} has no {kv_cache!r} cache")
         self.model = model
-        self.cache = model.make_cache(max_tokens, max_slots=max_slots, page_size=page_size)
+        self.cache = model.make_cache(max_tokens, max_slots=max_slots, page_size=page_size, **({"kv_cache": kv_cache} if kv_cache is not None else {}))
         self.scheduler = Scheduler(self.cache, max_step_tokens=max_step_tokens)
         self.cuda_graphs = cuda_graphs and self.cache.device.type == "cuda" and getattr(model, "decode_is_capturable", lambda n: True)(self.graph_max_batch)
         self._captured, self._seen = {}, {}

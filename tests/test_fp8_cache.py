@@ -113,6 +113,35 @@ def test_attention_parts_of_any_range_are_few(n_seqs, n_tokens, heads, kv_heads,
             assert lib.ktb200_fp8_cache_attn_workspace(C.byref(a), n_tokens, keys, 0, dtype, 1) == 0
 
 
+def test_engine_refuses_an_8_bit_cache_where_there_is_none():
+    from ktransformers_b200.util.engine import Engine
+    model = SimpleNamespace(make_cache=lambda *a, **k: None)
+    with pytest.raises(ValueError, match="has no 'fp8' cache"):
+        Engine(model, kv_cache="fp8")
+
+
+def test_lipadra_keeps_its_attention_rows_in_8_bits_where_asked():
+    import lipadra_util as LU
+    from ktransformers_b200.models.configuration_lipadra import LipadraConfig
+    from ktransformers_b200.models.modeling_lipadra import LipadraForCausalLM
+    cfg = LipadraConfig.from_dict(LU.config([(LU.attention(dim=16, vdim=16), None), (LU.retention(), None)]))
+    model = LipadraForCausalLM(cfg, device="cpu")
+    c = model.make_cache(64, max_slots=2, page_size=16, kv_cache="fp8")
+    assert isinstance(c.key_cache[0], Fp8CacheLayer) and c.key_cache[0].k.shape[1:] == (2, 16, 16) and not isinstance(c.key_cache[1], Fp8CacheLayer)
+    with pytest.raises(ValueError, match="no 'int4' cache"):
+        model.make_cache(64, kv_cache="int4")
+
+
+def test_prep_and_attention_refuse_what_8_bit_layers_do_not_have():
+    from ktransformers_b200.operators.attention import paged_softmax_attention, qkv_prep
+    batch, cache, total = U.batch_of([(5, 1)], 16)
+    kv = Fp8CacheLayer(*filled(total, 2, 16, 32, 32, 0))
+    with pytest.raises(ValueError, match="8 bits"):
+        qkv_prep(torch.zeros(1, 256), batch, cache, kv, 4, 2, 32, 32, (0, 128, 192), maps=2)
+    with pytest.raises(ValueError, match="8 bits"):
+        paged_softmax_attention(torch.zeros(1, 4, 32), kv, batch, cache, 4, 2, 32, 32, 0.1, gate=torch.zeros(1, 128))
+
+
 # ------------------------------------------------------------------------------------------------------------------------- append
 # fp32 against 64 bits: the turn is two products and a sum (3 x 2^-24 of |x| + |y|) with sine and cosine 2^-22 off, a norm 13 roundings of a sum of squares (half of
 # them in the root) and three more: in all below 32 x 2^-24 of a row's largest
@@ -443,3 +472,61 @@ def test_the_two_calls_as_a_step_uses_them_replayed_on_other_streams():
     ref = U.attention(q.bfloat16(), a.k.cpu(), a.v.cpu(), a.scales.cpu(), on(b, "cpu"), on(cache, "cpu"), H, G, d, d, d ** -0.5)
     # queries round as bf16 on both sides (one step apart at most: 2^-7 of a score of size s, s <= 5 here), weights to fp16, results to bf16
     assert ((eager[-1].cpu().double() - ref).abs() <= 2.0 ** -8 * ref.abs() + (2.0 ** -4 + 2.0 ** -11) * float(a.dequantize()[1].abs().max())).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("dim,page,chunk", [(128, 64, 4096), (32, 16, 40)])
+def test_an_attention_layer_on_an_8_bit_cache(dim, page, chunk, dtype):
+    """KPlusOneAttention through the cache manager, a prompt in portions and decoded tokens, against the 64-bit forms on the same projections"""
+    from ktransformers_b200.models.configuration_lipadra import PlusOneAttentionSpec
+    from ktransformers_b200.operators.attention import KPlusOneAttention
+    H, G, dt = 4, 2, DT[dtype]
+    spec = PlusOneAttentionSpec.from_dict({"heads": H, "kv_heads": G, "dim": dim, "vdim": dim, "mask": {"size": chunk}, "rot": {"base": 1000.0, "dims": dim}})
+    width, g = H * dim, torch.Generator().manual_seed(4)
+    layer = KPlusOneAttention(width, spec, 1e-5, dtype=dt, device="cuda")
+    rn = lambda *shape: torch.randn(shape, generator=g)
+    layer.w_in.data.copy_(rn(*layer.w_in.shape) / width ** 0.5)
+    layer.b_in.data.copy_(0.1 * rn(layer.n_in))
+    layer.q_norm.data.copy_(1 + 0.2 * rn(dim))
+    layer.k_norm.data.copy_(1 + 0.2 * rn(dim))
+    layer.o.data.copy_(torch.eye(width))      # (the layer's result is then the attention's)
+    c = PagedStateCache([spec.cache_row_width()], 0, 512, 2, "cuda", dtype=dt, page_size=page, chunks=[chunk], fp8_heads=[(G, dim, dim)])
+    held = c.key_cache[0]
+    k, v, s = (x.cpu() for x in (held.k, held.v, held.scales))
+    offs = (0, H * dim, (H + G) * dim)
+    for step in ([("a", 70), ("b", 9)], [("a", 33), ("b", 1)], [("a", 1), ("b", 1)], [("b", 40)], [("a", 1), ("b", 1)]):
+        batch = c.build_batch([(name, [0] * n, []) for name, n in step])
+        h = rn(batch.n_tokens, width).to(dt).cuda()
+        out = layer(h, batch, c, 0).cpu().double()
+        c.commit()
+        proj = torch.nn.functional.linear(h, layer.w_in, layer.b_in).cpu()
+        cpu = SimpleNamespace(pos=batch.pos.cpu(), slot=batch.slot.cpu(), seqs=batch.seqs.cpu(), n_seqs=batch.n_seqs)
+        table = SimpleNamespace(page_table=c.page_table.cpu(), max_pages_per_seq=c.max_pages_per_seq, page_size=page)
+        inv = layer.inv_freq.cpu()
+        q, *_ = U.append(proj, cpu, table, k, v, s, H, G, dim, dim, offs, spec.rot, inv, 3, 1e-5, layer.q_norm.cpu(), layer.k_norm.cpu())
+        k, v, s = held.k.cpu(), held.v.cpu(), held.scales.cpu()      # (what the cache holds is tested with the append)
+        ref = U.attention(q.to(dt), k, v, s, cpu, table, H, G, dim, dim, spec.scale, chunk=chunk, sink=torch.zeros(H))
+        # queries may round to the other side (a step of 2^-7 in bf16, 2^-20 for the fp32 rotation and norm) in scores below 32; weights to fp16; the result and the product with one to the type
+        top = float((v.double() * s.double()[:, :, None, None, 1]).nan_to_num(0.0).abs().max())
+        off = {"bf16": 2 * (2.0 ** -7 * 6 + 2.0 ** -11), "fp32": 2 * 32 * 2.0 ** -18}[dtype]
+        assert ((out - ref).abs() <= 2 * HALF_STEP[dt] * ref.abs() * 1.02 + off * top).all()
+
+
+@pytest.mark.gpu
+def test_a_model_served_from_an_8_bit_cache(tmp_path):
+    """the engine's prompt portions, decode steps and captured decode steps on an 8-bit cache: the same tokens whichever way"""
+    import lipadra_util as LU
+    from ktransformers_b200.models import load_model
+    from ktransformers_b200.util.engine import Engine
+    cfg = LU.config([(LU.attention(heads=4, kv_heads=2, dim=128, vdim=128, chunk=256, dims=128), LU.moe()), (LU.retention(), None), (LU.attention(heads=4, kv_heads=2, dim=16, vdim=16, chunk=32, dims=16), None)])
+    path = LU.save(tmp_path / "m", cfg, LU.weights(cfg, dtype=torch.bfloat16))
+    model = load_model(path, "bfloat16")
+    prompts = [[(7 * i + j) % 50 for j in range(n)] for i, n in enumerate((90, 3, 41))]
+    outs = [Engine(model, max_tokens=1024, page_size=64, max_step_tokens=step, cuda_graphs=graphs, kv_cache="fp8").generate(prompts, 12) for step, graphs in ((2048, False), (2048, True))]
+    assert outs[0] == outs[1] and all(len(o) == 12 for o in outs[0])
+    eng = Engine(model, max_tokens=1024, page_size=64, kv_cache="fp8")
+    assert isinstance(eng.cache.key_cache[0], Fp8CacheLayer) and isinstance(eng.cache.key_cache[2], Fp8CacheLayer)
+    logits = eng.step([("x", prompts[0], [89])])
+    plain = Engine(model, max_tokens=1024, page_size=64).step([("x", prompts[0], [89])])
+    assert logits.shape == plain.shape and torch.isfinite(logits).all()
