@@ -16,7 +16,7 @@
 namespace ktb {
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kFp8MaxParts = 128, kFp8MinPart = 256;
+constexpr int kFp8MaxParts = 128, kFp8MinPart = 256, kFp8MaxDim = 256;
 
 struct Fp8Attn {
     const void* q;
@@ -70,100 +70,216 @@ __device__ __forceinline__ void fp8_find_tokens(const Fp8Attn& a, int b, int tok
 }
 
 // ------------------------------------------------------------------------------------------------ CUDA cores: any head size up to 256, fp32 or bf16
-// grid (tokens, G * head blocks, splits); a warp per query head, the CTA's heads share one key/value head.  Tiles of 32 keys in shared memory as fp32 (code * scale, exact):
-// lane = key for the scores, lane = value column for the weighted sum; running maximum and sum per warp, natural exponentials.
-constexpr int kFgTile = 32, kFgCols = 8;
-template <typename T> __global__ void __launch_bounds__(256) fp8_attn_kernel(const Fp8Attn a) {
-    extern __shared__ __align__(16) float fg_smem[];
-    __shared__ int info[4];
-    const int HB = blockDim.x >> 5, R = a.H / a.G, hblocks = (R + HB - 1) / HB, d = a.d, dv = a.dv, ps = a.pages.page_size;
-    const int g = blockIdx.y / hblocks, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = (blockIdx.y % hblocks) * HB + warp, h = g * R + r;
-    const bool live = r < R;
+// A CTA of 8 warps owns up to 32 rows = (token, query head) pairs of one portion and one key/value head, a warp four of them, so that a key or value read from shared memory serves four
+// rows.  Tiles of 32 keys in shared memory as fp32 (code * scale, exact), the next tile's codes on their way in registers meanwhile (VEC: head sizes of whole 16 codes): lane = key for the
+// scores, lane = value column for the weighted sum; a running maximum per row, natural exponentials, sums kept by lanes until the end.
+// Bound by fp32 products: 2 d FMAs a key and row, 5 shared-memory loads of 16 bytes for 16 of them.
+constexpr int kFgTile = 32, kFgRows = 4, kFgWarps = 8, kFgPieces = 4;
+struct FgMisc { int info[4], bad[2]; };
+__host__ __device__ inline int fg_heads(int R) {      // heads of a group that one CTA's rows take: the largest divisor of the group up to 32
+    for (int h = R < 32 ? R : 32; h > 1; h--)
+        if (R % h == 0) return h;
+    return 1;
+}
+__host__ __device__ inline int fg_pitch(int d) { return d % 4 ? d | 1 : d + 4; }      // floats of a key's row: neighbouring rows meet in no bank
+static size_t fg_smem(int d, int dv) { return ((size_t)kFgTile * fg_pitch(d) + (size_t)kFgTile * dv + (size_t)kFgRows * kFgWarps * ((d + 3) / 4 * 4 + kFgTile)) * sizeof(float); }
+
+template <typename T, int NC, bool VEC> __global__ void __launch_bounds__(256, 2) fp8_attn_kernel(const Fp8Attn a, int RH) {
+    extern __shared__ __align__(16) float fg_smem_raw[];
+    __shared__ FgMisc misc;
+    const int d = a.d, dv = a.dv, ps = a.pages.page_size, R = a.H / a.G, hblocks = R / RH, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, pitch = fg_pitch(d), qp = (d + 3) / 4 * 4;
+    const int g = blockIdx.y / hblocks, h0 = g * R + (blockIdx.y % hblocks) * RH;
     griddep_launch_dependents();
     griddep_wait();
-    if (warp == 0) fp8_find_tokens(a, blockIdx.x, 1, info);
+    if (warp == 0) fp8_find_tokens(a, blockIdx.x, a.ctoks, misc.info);
+    if (threadIdx.x < 2) misc.bad[threadIdx.x] = 0;
     __syncthreads();
-    if (info[1] <= 0) return;
-    const int p = info[2], slot = info[3];
-    const long t = info[0];
-    float* qs = fg_smem;
-    float* Ks = qs + HB * d;
-    float* Vs = Ks + kFgTile * (d + 1);
-    float* pw = Vs + kFgTile * dv;
-    const int lo = fp8_first_visible(p, a.window, a.chunk), lo16 = lo & ~(a.align - 1);
-    const bool cut = a.part > 0 && p + 1 - lo16 > a.part;
-    const int k_lo = max(lo, lo16 + (int)blockIdx.z * a.part), k_hi = cut ? min(p + 1, lo16 + (int)(blockIdx.z + 1) * a.part) : p + 1;
+    const int tok0 = misc.info[0], ntok = misc.info[1], pos0 = misc.info[2], slot = misc.info[3], max_pos = pos0 + ntok - 1;
+    if (ntok <= 0) return;
+    const int lo = fp8_first_visible(pos0, a.window, a.chunk), lo_al = lo & ~(a.align - 1);
+    const bool cut = a.part > 0 && max_pos + 1 - lo_al > a.part;
+    const int k_lo = max(lo, lo_al + (int)blockIdx.z * a.part), k_hi = cut ? min(max_pos + 1, lo_al + (int)(blockIdx.z + 1) * a.part) : max_pos + 1;
     if (blockIdx.z && (!cut || k_lo >= k_hi)) return;
-    float acc[kFgCols];
+    float* Ks = fg_smem_raw;
+    float* Vs = Ks + kFgTile * pitch;
+    float* qs = Vs + kFgTile * dv + warp * kFgRows * qp;      // the warp's four rows of queries, then their weights
+    float* pw = Vs + kFgTile * dv + kFgWarps * kFgRows * qp + warp * kFgRows * kFgTile;
+    // the warp's rows
+    const int rows = ntok * RH;
+    int row_pos[kFgRows], row_first[kFgRows];
 #pragma unroll
-    for (int c = 0; c < kFgCols; c++) acc[c] = 0.f;
-    float m = -INFINITY, l = 0.f;
-    if (live) {
-        const float sc = a.head_scale ? a.scale * a.head_scale[h] : a.scale;
-        for (int i = lane; i < d; i += 32) qs[warp * d + i] = to_f(((const T*)a.q)[(t * a.H + h) * d + i]) * sc;
+    for (int r = 0; r < kFgRows; r++) {
+        const int i = warp * kFgRows + r, tok = i / RH, h = h0 + i % RH;
+        const bool live = i < rows;
+        row_pos[r] = live ? pos0 + tok : -1;
+        row_first[r] = live ? fp8_first_visible(pos0 + tok, a.window, a.chunk) : 0;
+        const float sc = live ? (a.head_scale ? a.scale * a.head_scale[h] : a.scale) : 0.f;
+        for (int c = lane; c < qp; c += 32) qs[r * qp + c] = live && c < d ? to_f(((const T*)a.q)[((long)(tok0 + tok) * a.H + h) * d + c]) * sc : 0.f;
     }
-    for (int j0 = k_lo; j0 < k_hi; j0 += kFgTile) {
-        __syncthreads();
-        const int nk = min(kFgTile, k_hi - j0);
-        unsigned here = 0;      // keys of the tile whose pages are there
-        for (int j = 0; j < nk; j++) {
-            const int kp = j0 + j, page = a.pages.page(slot, kp / ps);
-            if (page < 0) {
-                for (int i = threadIdx.x; i < dv; i += blockDim.x) Vs[j * dv + i] = 0.f;
-                continue;
-            }
-            here |= 1u << j;
+    __syncwarp();
+    // a tile's pieces of 16 codes: first the keys' (d / 16 a key), then the values'
+    const int kp = d / 16, vp = dv / 16, pieces = kFgTile * (kp + vp);
+    uint4 codes[kFgPieces];
+    float scale[kFgPieces];
+    auto fetch = [&](int j0) {
+#pragma unroll
+        for (int i = 0; i < kFgPieces; i++) {
+            const int at = threadIdx.x + 256 * i;
+            scale[i] = 0.f;
+            codes[i] = make_uint4(0, 0, 0, 0);
+            if (at >= pieces) continue;
+            const bool is_v = at >= kFgTile * kp;
+            const int per = is_v ? vp : kp, u = is_v ? at - kFgTile * kp : at, key = j0 + u / per, piece = u % per;
+            const int page = key < k_hi ? a.pages.page(slot, key / ps) : -1;
+            if (page < 0) continue;
             const long block = (long)page * a.G + g;
-            const float ks = a.scales[2 * block], vs = a.scales[2 * block + 1];
-            const uint8_t *k = a.k_codes + (block * ps + kp % ps) * d, *v = a.v_codes + (block * ps + kp % ps) * dv;
-            for (int i = threadIdx.x; i < d; i += blockDim.x) Ks[j * (d + 1) + i] = __half2float(__half(__nv_cvt_fp8_to_halfraw(k[i], __NV_E4M3))) * ks;
-            for (int i = threadIdx.x; i < dv; i += blockDim.x) Vs[j * dv + i] = __half2float(__half(__nv_cvt_fp8_to_halfraw(v[i], __NV_E4M3))) * vs;
+            scale[i] = a.scales[2 * block + is_v];
+            codes[i] = *reinterpret_cast<const uint4*>((is_v ? a.v_codes + (block * ps + key % ps) * dv : a.k_codes + (block * ps + key % ps) * d) + 16 * piece);
         }
+    };
+    auto spread = [&](int buf) {      // to shared memory, and whether a value is NaN
+#pragma unroll
+        for (int i = 0; i < kFgPieces; i++) {
+            const int at = threadIdx.x + 256 * i;
+            if (at >= pieces) continue;
+            const bool is_v = at >= kFgTile * kp;
+            const int per = is_v ? vp : kp, u = is_v ? at - kFgTile * kp : at, key = u / per, piece = u % per;
+            float* to = (is_v ? Vs + key * dv : Ks + key * pitch) + 16 * piece;
+            const uint32_t w[4] = {codes[i].x, codes[i].y, codes[i].z, codes[i].w};
+            uint32_t odd = 0;
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                odd |= (w[q] & 0x7f7f7f7fu) + 0x01010101u;
+                const float2 x = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)w[q], __NV_E4M3)));
+                const float2 y = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w[q] >> 16), __NV_E4M3)));
+                *reinterpret_cast<float4*>(to + 4 * q) = make_float4(x.x * scale[i], x.y * scale[i], y.x * scale[i], y.y * scale[i]);
+            }
+            if (is_v && (odd & 0x80808080u)) misc.bad[buf] = 1;
+        }
+    };
+    auto bring = [&](int j0, int buf) {      // head sizes of any number of codes
+        for (int at = threadIdx.x; at < kFgTile * (d + dv); at += 256) {
+            const bool is_v = at >= kFgTile * d;
+            const int per = is_v ? dv : d, u = is_v ? at - kFgTile * d : at, k = u / per, c = u % per, key = j0 + k;
+            const int page = key < k_hi ? a.pages.page(slot, key / ps) : -1;
+            float v = 0.f;
+            if (page >= 0) {
+                const long block = (long)page * a.G + g;
+                v = __half2float(__half(__nv_cvt_fp8_to_halfraw((is_v ? a.v_codes : a.k_codes)[(block * ps + key % ps) * per + c], __NV_E4M3))) * a.scales[2 * block + is_v];
+            }
+            (is_v ? Vs + k * dv : Ks + k * pitch)[c] = v;
+            if (is_v && v != v) misc.bad[buf] = 1;
+        }
+    };
+    float acc[kFgRows][NC], m[kFgRows], l[kFgRows];
+#pragma unroll
+    for (int r = 0; r < kFgRows; r++) {
+        m[r] = -INFINITY;
+        l[r] = 0.f;
+#pragma unroll
+        for (int c = 0; c < NC; c++) acc[r][c] = 0.f;
+    }
+    if (VEC && k_lo < k_hi) fetch(k_lo);
+    for (int j0 = k_lo, buf = 0; j0 < k_hi; j0 += kFgTile, buf ^= 1) {
+        __syncthreads();      // (the tile before this one has been read)
+        if (threadIdx.x == 0) misc.bad[buf ^ 1] = 0;
+        if (VEC) spread(buf); else bring(j0, buf);
         __syncthreads();
-        if (!live) continue;
-        float s = -INFINITY;
-        if (here >> lane & 1) {
-            float q_k = 0.f;
-            const float *kr = Ks + lane * (d + 1), *qr = qs + warp * d;
-            for (int i = 0; i < d; i++) q_k = fmaf(qr[i], kr[i], q_k);
-            s = a.softcap > 0.f ? a.softcap * tanhf(q_k / a.softcap) : q_k;
+        const bool bad = misc.bad[buf];
+        if (VEC && j0 + kFgTile < k_hi) fetch(j0 + kFgTile);
+        if (warp * kFgRows >= rows) continue;
+        const int key = j0 + lane;
+        const bool here = key < k_hi && a.pages.page(slot, key / ps) >= 0;
+        float s[kFgRows];
+#pragma unroll
+        for (int r = 0; r < kFgRows; r++) s[r] = 0.f;
+        const float* kr = Ks + lane * pitch;
+        if (d % 4 == 0) {
+#pragma unroll 4
+            for (int c = 0; c < d; c += 4) {
+                const float4 k = *reinterpret_cast<const float4*>(kr + c);
+#pragma unroll
+                for (int r = 0; r < kFgRows; r++) {
+                    const float4 q = *reinterpret_cast<const float4*>(qs + r * qp + c);
+                    s[r] = fmaf(q.x, k.x, s[r]);
+                    s[r] = fmaf(q.y, k.y, s[r]);
+                    s[r] = fmaf(q.z, k.z, s[r]);
+                    s[r] = fmaf(q.w, k.w, s[r]);
+                }
+            }
+        } else {
+            for (int c = 0; c < d; c++)
+#pragma unroll
+                for (int r = 0; r < kFgRows; r++) s[r] = fmaf(qs[r * qp + c], kr[c], s[r]);
         }
-        const float mn = fmaxf(m, warp_max(s)), u = mn == -INFINITY ? 0.f : mn;
-        const float corr = expf(m - u), pj = expf(s - u);
-        l = l * corr + warp_sum(pj);
-        m = mn;
-        pw[warp * kFgTile + lane] = pj;
+#pragma unroll
+        for (int r = 0; r < kFgRows; r++) {
+            if (a.softcap > 0.f) s[r] = a.softcap * tanhf(s[r] / a.softcap);
+            if (!(here && key <= row_pos[r] && key >= row_first[r])) s[r] = -INFINITY;
+            const float mn = fmaxf(m[r], warp_max(s[r])), u = mn == -INFINITY ? 0.f : mn, corr = expf(m[r] - u), p = expf(s[r] - u);
+            m[r] = mn;
+            l[r] = fmaf(l[r], corr, p);
+            pw[r * kFgTile + lane] = p;
+            if (corr != 1.f) {
+#pragma unroll
+                for (int c = 0; c < NC; c++) acc[r][c] *= corr;
+            }
+        }
         __syncwarp();
+        if (!bad) {
+#pragma unroll 2
+            for (int j = 0; j < kFgTile; j += 4) {
+                float4 w[kFgRows];
 #pragma unroll
-        for (int c = 0; c < kFgCols; c++) acc[c] *= corr;
-        for (int j = 0; j < nk; j++) {
-            const float wj = pw[warp * kFgTile + j];
+                for (int r = 0; r < kFgRows; r++) w[r] = *reinterpret_cast<const float4*>(pw + r * kFgTile + j);
 #pragma unroll
-            for (int c = 0; c < kFgCols; c++)
-                if (lane + 32 * c < dv) acc[c] = fmaf(wj, Vs[j * dv + lane + 32 * c], acc[c]);
+                for (int c = 0; c < NC; c++) {
+                    if (lane + 32 * c < dv) {
+                        const float* v = Vs + j * dv + lane + 32 * c;
+                        const float v0 = v[0], v1 = v[dv], v2 = v[2 * dv], v3 = v[3 * dv];
+#pragma unroll
+                        for (int r = 0; r < kFgRows; r++) acc[r][c] = fmaf(w[r].w, v3, fmaf(w[r].z, v2, fmaf(w[r].y, v1, fmaf(w[r].x, v0, acc[r][c]))));
+                    }
+                }
+            }
+        } else {      // a value that is NaN belongs to the rows that weigh it
+            for (int j = 0; j < kFgTile; j++)
+#pragma unroll
+                for (int r = 0; r < kFgRows; r++) {
+                    const float w = pw[r * kFgTile + j];
+#pragma unroll
+                    for (int c = 0; c < NC; c++)
+                        if (w != 0.f && lane + 32 * c < dv) acc[r][c] = fmaf(w, Vs[j * dv + lane + 32 * c], acc[r][c]);
+                }
         }
         __syncwarp();
     }
-    if (!live) return;
-    if (cut) {
-        float* o = a.partial + ((t * a.H + h) * a.parts + blockIdx.z) * (dv + 2);
-        if (lane == 0) { o[0] = m; o[1] = l; }
 #pragma unroll
-        for (int c = 0; c < kFgCols; c++)
-            if (lane + 32 * c < dv) o[2 + lane + 32 * c] = acc[c];
-        return;
+    for (int r = 0; r < kFgRows; r++) {
+        const int i = warp * kFgRows + r, tok = i / RH, h = h0 + i % RH;
+        if (i >= rows) break;
+        float sum = warp_sum(l[r]);
+        const long t = tok0 + tok;
+        if (cut) {
+            float* o = a.partial + ((t * a.H + h) * a.parts + blockIdx.z) * (dv + 2);
+            if (lane == 0) { o[0] = m[r]; o[1] = sum; }
+#pragma unroll
+            for (int c = 0; c < NC; c++)
+                if (lane + 32 * c < dv) o[2 + lane + 32 * c] = acc[r][c];
+            continue;
+        }
+        float corr = 1.f;
+        if (a.sink) {
+            const float mn = fmaxf(m[r], a.sink[h]);
+            corr = expf(m[r] - mn);
+            sum = sum * corr + expf(a.sink[h] - mn);
+        }
+        const float inv = sum > 0.f || sum != sum ? corr * a.out_scale / sum : 0.f;
+        T* out = (T*)a.out + t * a.out_stride + (long)h * dv;
+#pragma unroll
+        for (int c = 0; c < NC; c++)
+            if (lane + 32 * c < dv) out[lane + 32 * c] = from_f<T>(acc[r][c] * inv);
     }
-    if (a.sink) {
-        const float mn = fmaxf(m, a.sink[h]), corr = expf(m - mn);
-        l = l * corr + expf(a.sink[h] - mn);
-#pragma unroll
-        for (int c = 0; c < kFgCols; c++) acc[c] *= corr;
-    }
-    const float inv = l > 0.f || l != l ? a.out_scale / l : 0.f;
-    T* out = (T*)a.out + t * a.out_stride + (long)h * dv;
-#pragma unroll
-    for (int c = 0; c < kFgCols; c++)
-        if (lane + 32 * c < dv) out[lane + 32 * c] = from_f<T>(acc[c] * inv);
 }
 
 // The parts of a cut key range, one CTA for each (token, head): the parts' weights once in shared memory (a part without a key has maximum -inf and weighs nothing; the sink joins
@@ -246,7 +362,7 @@ static Fp8Form fp8_form(const ktb200_fp8_attn_params* c, int n_tokens, int dtype
         const FmForm f = fm_form(c, n_tokens);
         return {Fp8Form::kMma, f, f.toks, f.RH, kFmKeys, 3};
     }
-    return {Fp8Form::kCuda, {}, 1, std::min(R, 8), 16, 3};
+    return {Fp8Form::kCuda, {}, 32 / fg_heads(R), fg_heads(R), 16, 2};
 }
 // the most keys that a CTA's tokens see together, from a multiple of the alignment on
 static long fp8_range(const ktb200_fp8_attn_params* c, int max_keys, const Fp8Form& f) {
@@ -288,9 +404,9 @@ extern "C" size_t ktb200_fp8_cache_attn_workspace(const ktb200_fp8_attn_params* 
 
 extern "C" int ktb200_fp8_cache_attn(const ktb200_fp8_attn_params* c, int n_tokens, int max_keys, int part, float* workspace, size_t workspace_bytes, int dtype, int allow_tensor_cores,
                                      void* stream) {
-    if (!fp8_sizes_ok(c) || c->dim <= 0 || c->dim > 32 * kFgCols || c->vdim <= 0 || c->vdim > 32 * kFgCols || c->page_size <= 0 || c->max_pages <= 0 || c->n_pages < 0 || c->n_slots <= 0 ||
+    if (!fp8_sizes_ok(c) || c->dim <= 0 || c->dim > kFp8MaxDim || c->vdim <= 0 || c->vdim > kFp8MaxDim || c->page_size <= 0 || c->max_pages <= 0 || c->n_pages < 0 || c->n_slots <= 0 ||
         c->n_seqs < 0 || c->window < 0 || c->chunk < 0 || c->out_stride < (long)c->heads * c->vdim) {
-        set_error("fp8_cache_attn: bad argument (head sizes up to %d)", 32 * kFgCols);
+        set_error("fp8_cache_attn: bad argument (head sizes up to %d)", kFp8MaxDim);
         return KTB200_EINVAL;
     }
     if (dtype != KTB200_TYPE_BF16 && dtype != KTB200_TYPE_F32) { set_error("fp8_cache_attn: dtype must be bf16 or f32"); return KTB200_EINVAL; }
@@ -321,10 +437,15 @@ extern "C" int ktb200_fp8_cache_attn(const ktb200_fp8_attn_params* c, int n_toke
     } else if (f.kernel == Fp8Form::kMma) {
         KTB_CUDA_CHECK(fm_launch(a, f.mma, grid, s));
     } else {
-        const int HB = f.heads;
-        const size_t smem = ((size_t)HB * c->dim + (size_t)kFgTile * (c->dim + 1) + (size_t)kFgTile * c->vdim + (size_t)HB * kFgTile) * sizeof(float);
-        KTB_CUDA_CHECK(raise_smem_limit(bf16 ? (const void*)fp8_attn_kernel<__nv_bfloat16> : (const void*)fp8_attn_kernel<float>, smem));
-        KTB_CUDA_CHECK(launch_pdl(bf16 ? fp8_attn_kernel<__nv_bfloat16> : fp8_attn_kernel<float>, grid, dim3(HB * 32), smem, s, a));
+        const size_t smem = fg_smem(c->dim, c->vdim);
+        const bool vec = c->dim % 16 == 0 && c->vdim % 16 == 0 && !((reinterpret_cast<uintptr_t>(c->k_codes) | reinterpret_cast<uintptr_t>(c->v_codes)) & 15);
+        const int cols = (c->vdim + 31) / 32;
+#define FG_OF(T, NC) (vec ? fp8_attn_kernel<T, NC, true> : fp8_attn_kernel<T, NC, false>)
+        const auto kernel = bf16 ? (cols <= 2 ? FG_OF(__nv_bfloat16, 2) : cols <= 4 ? FG_OF(__nv_bfloat16, 4) : FG_OF(__nv_bfloat16, 8))
+                                 : (cols <= 2 ? FG_OF(float, 2) : cols <= 4 ? FG_OF(float, 4) : FG_OF(float, 8));
+#undef FG_OF
+        KTB_CUDA_CHECK(raise_smem_limit((const void*)kernel, smem));
+        KTB_CUDA_CHECK(launch_pdl(kernel, grid, dim3(kFgWarps * 32), smem, s, a, f.heads));
     }
     count_launch();
     if (parts > 1) {
