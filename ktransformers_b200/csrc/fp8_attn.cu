@@ -70,11 +70,11 @@ __device__ __forceinline__ void fp8_find_tokens(const Fp8Attn& a, int b, int tok
 }
 
 // ------------------------------------------------------------------------------------------------ CUDA cores: any head size up to 256, fp32 or bf16
-// A CTA of 8 warps owns up to 32 rows = (token, query head) pairs of one portion and one key/value head, a warp four of them, so that a key or value read from shared memory serves four
-// rows.  Tiles of 32 keys in shared memory as fp32 (code * scale, exact), the next tile's codes on their way in registers meanwhile (VEC: head sizes of whole 16 codes): lane = key for the
+// A CTA of 8 warps owns up to 32 rows = (token, query head) pairs of one portion and one key/value head, a warp up to four of them, so that a key or value read from shared memory serves
+// them all; a decode step's few rows go to as many warps (ROWS 1 or 2 a warp).  Tiles of 32 keys in shared memory as fp32 (code * scale, exact), the next tile's codes on their way in registers meanwhile (VEC: head sizes of whole 16 codes): lane = key for the
 // scores, lane = value column for the weighted sum; a running maximum per row, natural exponentials, sums kept by lanes until the end.
 // Bound by fp32 products: 2 d FMAs a key and row, 5 shared-memory loads of 16 bytes for 16 of them.
-constexpr int kFgTile = 32, kFgRows = 4, kFgWarps = 8, kFgPieces = 4;
+constexpr int kFgTile = 32, kFgWarps = 8, kFgPieces = 4;
 struct FgMisc { int info[4], bad[2]; };
 __host__ __device__ inline int fg_heads(int R) {      // heads of a group that one CTA's rows take: the largest divisor of the group up to 32
     for (int h = R < 32 ? R : 32; h > 1; h--)
@@ -82,9 +82,9 @@ __host__ __device__ inline int fg_heads(int R) {      // heads of a group that o
     return 1;
 }
 __host__ __device__ inline int fg_pitch(int d) { return d % 4 ? d | 1 : d + 4; }      // floats of a key's row: neighbouring rows meet in no bank
-static size_t fg_smem(int d, int dv) { return ((size_t)kFgTile * fg_pitch(d) + (size_t)kFgTile * dv + (size_t)kFgRows * kFgWarps * ((d + 3) / 4 * 4 + kFgTile)) * sizeof(float); }
+static size_t fg_smem(int d, int dv, int rows) { return ((size_t)kFgTile * fg_pitch(d) + (size_t)kFgTile * dv + (size_t)rows * kFgWarps * ((d + 3) / 4 * 4 + kFgTile)) * sizeof(float); }
 
-template <typename T, int NC, bool VEC> __global__ void __launch_bounds__(256, 2) fp8_attn_kernel(const Fp8Attn a, int RH) {
+template <typename T, int NC, bool VEC, int ROWS> __global__ void __launch_bounds__(256, 2) fp8_attn_kernel(const Fp8Attn a, int RH) {
     extern __shared__ __align__(16) float fg_smem_raw[];
     __shared__ FgMisc misc;
     const int d = a.d, dv = a.dv, ps = a.pages.page_size, R = a.H / a.G, hblocks = R / RH, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, pitch = fg_pitch(d), qp = (d + 3) / 4 * 4;
@@ -102,14 +102,14 @@ template <typename T, int NC, bool VEC> __global__ void __launch_bounds__(256, 2
     if (blockIdx.z && (!cut || k_lo >= k_hi)) return;
     float* Ks = fg_smem_raw;
     float* Vs = Ks + kFgTile * pitch;
-    float* qs = Vs + kFgTile * dv + warp * kFgRows * qp;      // the warp's four rows of queries, then their weights
-    float* pw = Vs + kFgTile * dv + kFgWarps * kFgRows * qp + warp * kFgRows * kFgTile;
+    float* qs = Vs + kFgTile * dv + warp * ROWS * qp;      // the warp's four rows of queries, then their weights
+    float* pw = Vs + kFgTile * dv + kFgWarps * ROWS * qp + warp * ROWS * kFgTile;
     // the warp's rows
     const int rows = ntok * RH;
-    int row_pos[kFgRows], row_first[kFgRows];
+    int row_pos[ROWS], row_first[ROWS];
 #pragma unroll
-    for (int r = 0; r < kFgRows; r++) {
-        const int i = warp * kFgRows + r, tok = i / RH, h = h0 + i % RH;
+    for (int r = 0; r < ROWS; r++) {
+        const int i = warp * ROWS + r, tok = i / RH, h = h0 + i % RH;
         const bool live = i < rows;
         row_pos[r] = live ? pos0 + tok : -1;
         row_first[r] = live ? fp8_first_visible(pos0 + tok, a.window, a.chunk) : 0;
@@ -171,9 +171,9 @@ template <typename T, int NC, bool VEC> __global__ void __launch_bounds__(256, 2
             if (is_v && v != v) misc.bad[buf] = 1;
         }
     };
-    float acc[kFgRows][NC], m[kFgRows], l[kFgRows];
+    float acc[ROWS][NC], m[ROWS], l[ROWS];
 #pragma unroll
-    for (int r = 0; r < kFgRows; r++) {
+    for (int r = 0; r < ROWS; r++) {
         m[r] = -INFINITY;
         l[r] = 0.f;
 #pragma unroll
@@ -187,19 +187,19 @@ template <typename T, int NC, bool VEC> __global__ void __launch_bounds__(256, 2
         __syncthreads();
         const bool bad = misc.bad[buf];
         if (VEC && j0 + kFgTile < k_hi) fetch(j0 + kFgTile);
-        if (warp * kFgRows >= rows) continue;
+        if (warp * ROWS >= rows) continue;
         const int key = j0 + lane;
         const bool here = key < k_hi && a.pages.page(slot, key / ps) >= 0;
-        float s[kFgRows];
+        float s[ROWS];
 #pragma unroll
-        for (int r = 0; r < kFgRows; r++) s[r] = 0.f;
+        for (int r = 0; r < ROWS; r++) s[r] = 0.f;
         const float* kr = Ks + lane * pitch;
         if (d % 4 == 0) {
 #pragma unroll 4
             for (int c = 0; c < d; c += 4) {
                 const float4 k = *reinterpret_cast<const float4*>(kr + c);
 #pragma unroll
-                for (int r = 0; r < kFgRows; r++) {
+                for (int r = 0; r < ROWS; r++) {
                     const float4 q = *reinterpret_cast<const float4*>(qs + r * qp + c);
                     s[r] = fmaf(q.x, k.x, s[r]);
                     s[r] = fmaf(q.y, k.y, s[r]);
@@ -210,10 +210,10 @@ template <typename T, int NC, bool VEC> __global__ void __launch_bounds__(256, 2
         } else {
             for (int c = 0; c < d; c++)
 #pragma unroll
-                for (int r = 0; r < kFgRows; r++) s[r] = fmaf(qs[r * qp + c], kr[c], s[r]);
+                for (int r = 0; r < ROWS; r++) s[r] = fmaf(qs[r * qp + c], kr[c], s[r]);
         }
 #pragma unroll
-        for (int r = 0; r < kFgRows; r++) {
+        for (int r = 0; r < ROWS; r++) {
             if (a.softcap > 0.f) s[r] = a.softcap * tanhf(s[r] / a.softcap);
             if (!(here && key <= row_pos[r] && key >= row_first[r])) s[r] = -INFINITY;
             const float mn = fmaxf(m[r], warp_max(s[r])), u = mn == -INFINITY ? 0.f : mn, corr = expf(m[r] - u), p = expf(s[r] - u);
@@ -229,23 +229,23 @@ template <typename T, int NC, bool VEC> __global__ void __launch_bounds__(256, 2
         if (!bad) {
 #pragma unroll 2
             for (int j = 0; j < kFgTile; j += 4) {
-                float4 w[kFgRows];
+                float4 w[ROWS];
 #pragma unroll
-                for (int r = 0; r < kFgRows; r++) w[r] = *reinterpret_cast<const float4*>(pw + r * kFgTile + j);
+                for (int r = 0; r < ROWS; r++) w[r] = *reinterpret_cast<const float4*>(pw + r * kFgTile + j);
 #pragma unroll
                 for (int c = 0; c < NC; c++) {
                     if (lane + 32 * c < dv) {
                         const float* v = Vs + j * dv + lane + 32 * c;
                         const float v0 = v[0], v1 = v[dv], v2 = v[2 * dv], v3 = v[3 * dv];
 #pragma unroll
-                        for (int r = 0; r < kFgRows; r++) acc[r][c] = fmaf(w[r].w, v3, fmaf(w[r].z, v2, fmaf(w[r].y, v1, fmaf(w[r].x, v0, acc[r][c]))));
+                        for (int r = 0; r < ROWS; r++) acc[r][c] = fmaf(w[r].w, v3, fmaf(w[r].z, v2, fmaf(w[r].y, v1, fmaf(w[r].x, v0, acc[r][c]))));
                     }
                 }
             }
         } else {      // a value that is NaN belongs to the rows that weigh it
             for (int j = 0; j < kFgTile; j++)
 #pragma unroll
-                for (int r = 0; r < kFgRows; r++) {
+                for (int r = 0; r < ROWS; r++) {
                     const float w = pw[r * kFgTile + j];
 #pragma unroll
                     for (int c = 0; c < NC; c++)
@@ -255,8 +255,8 @@ template <typename T, int NC, bool VEC> __global__ void __launch_bounds__(256, 2
         __syncwarp();
     }
 #pragma unroll
-    for (int r = 0; r < kFgRows; r++) {
-        const int i = warp * kFgRows + r, tok = i / RH, h = h0 + i % RH;
+    for (int r = 0; r < ROWS; r++) {
+        const int i = warp * ROWS + r, tok = i / RH, h = h0 + i % RH;
         if (i >= rows) break;
         float sum = warp_sum(l[r]);
         const long t = tok0 + tok;
@@ -352,17 +352,21 @@ using namespace ktb;
 struct Fp8Form {
     enum { kCuda, kMma, kDecode, kPrompt } kernel;
     FmForm mma;
-    int ctoks, heads, align, places;
+    int ctoks, heads, align, places, rows;      // (rows of a warp: kCuda)
 };
+static bool fg_vec(const ktb200_fp8_attn_params* c) {      // whole pieces of 16 codes
+    return c->dim % 16 == 0 && c->vdim % 16 == 0 && !((reinterpret_cast<uintptr_t>(c->k_codes) | reinterpret_cast<uintptr_t>(c->v_codes)) & 15);
+}
 static Fp8Form fp8_form(const ktb200_fp8_attn_params* c, int n_tokens, int dtype, int allow_tensor_cores) {
     const int R = c->heads / c->kv_heads;
     if (allow_tensor_cores && fd_takes(c, n_tokens, dtype)) return {Fp8Form::kDecode, {}, 1, fm_heads(R), kFdAlign, 3};
-    if (allow_tensor_cores && fp_takes(c, n_tokens, dtype)) return {Fp8Form::kPrompt, {}, 2 * (128 / fm_heads(R)), fm_heads(R), kFpKeys, 1};
+    if (allow_tensor_cores && fp_takes(c, n_tokens, dtype)) return {Fp8Form::kPrompt, {}, 2 * (128 / fm_heads(R)), fm_heads(R), kFpKeys, 1, 0};
     if (allow_tensor_cores && fm_takes(c, dtype)) {
         const FmForm f = fm_form(c, n_tokens);
-        return {Fp8Form::kMma, f, f.toks, f.RH, kFmKeys, 3};
+        return {Fp8Form::kMma, f, f.toks, f.RH, kFmKeys, 3, 0};
     }
-    return {Fp8Form::kCuda, {}, 32 / fg_heads(R), fg_heads(R), 16, 2};
+    const int RH = fg_heads(R), rows = n_tokens > c->n_seqs || RH > 16 || !fg_vec(c) ? 4 : RH > 8 ? 2 : 1;
+    return {Fp8Form::kCuda, {}, kFgWarps * rows / RH, RH, 16, 2, rows};
 }
 // the most keys that a CTA's tokens see together, from a multiple of the alignment on
 static long fp8_range(const ktb200_fp8_attn_params* c, int max_keys, const Fp8Form& f) {
@@ -437,10 +441,9 @@ extern "C" int ktb200_fp8_cache_attn(const ktb200_fp8_attn_params* c, int n_toke
     } else if (f.kernel == Fp8Form::kMma) {
         KTB_CUDA_CHECK(fm_launch(a, f.mma, grid, s));
     } else {
-        const size_t smem = fg_smem(c->dim, c->vdim);
-        const bool vec = c->dim % 16 == 0 && c->vdim % 16 == 0 && !((reinterpret_cast<uintptr_t>(c->k_codes) | reinterpret_cast<uintptr_t>(c->v_codes)) & 15);
+        const size_t smem = fg_smem(c->dim, c->vdim, f.rows);
         const int cols = (c->vdim + 31) / 32;
-#define FG_OF(T, NC) (vec ? fp8_attn_kernel<T, NC, true> : fp8_attn_kernel<T, NC, false>)
+#define FG_OF(T, NC) (f.rows == 1 ? fp8_attn_kernel<T, NC, true, 1> : f.rows == 2 ? fp8_attn_kernel<T, NC, true, 2> : fg_vec(c) ? fp8_attn_kernel<T, NC, true, 4> : fp8_attn_kernel<T, NC, false, 4>)
         const auto kernel = bf16 ? (cols <= 2 ? FG_OF(__nv_bfloat16, 2) : cols <= 4 ? FG_OF(__nv_bfloat16, 4) : FG_OF(__nv_bfloat16, 8))
                                  : (cols <= 2 ? FG_OF(float, 2) : cols <= 4 ? FG_OF(float, 4) : FG_OF(float, 8));
 #undef FG_OF
