@@ -2,14 +2,14 @@
 //
 // A warp owns 8 or 16 rows = (token, query head) pairs of one portion and one key/value head and takes 16 keys at a time:  S = Q K^T,  t = s log2(e) + log2(value scale),
 // p = 2^(t - m),  O += P V,  l += p / (value scale).
-//   S   m16n8k32 e4m3: the keys' codes as they are, against each query row as two e4m3 rows, q = q1 + q2 / 16 once the row is moved by a power of two so that its
-//       largest stands in [128, 256): exact for bf16 numbers down to 2^-13 of that largest, 2^-21 of it off below
-//   O   m16n8k16 fp16: codes as fp16, which holds every e4m3 number exactly (one conversion for two), weights rounded to fp16 (2^-11 of a weight)
+// Codes go to m16n8k16 fp16 products as fp16, which holds every e4m3 number exactly (one conversion for two codes), against queries as fp16 too, each row first moved by a power of two so
+// that its largest stands below 2^15 (exact for what is within 2^-28 of that), and weights rounded to fp16 (2^-11 of a weight).  (m16n8k32 e4m3 products took more instructions: they
+// count as two fp16 ones each, with the conversions of both operands.)
 // Key scales multiply scores.  A block's value scale is a power of two in the weight's exponent, so that O needs no scale and the weights of all blocks stand in
 // one range: m is raised only when a row's t outgrows it by 8, p <= 2^8.  O / l is the result: 2^m drops out.
 //
 // The order of a product's sum is free, and taken so that no shuffling is needed: of a key's row, the four threads that share it hold 16 neighbouring bytes each (an S
-// step takes 8 of them), and of a value's row each of the eight column groups has its neighbouring bytes, an output tile's columns being dv / 8 apart.
+// step takes 4 of them), and of a value's row each of the eight column groups has its neighbouring bytes, an output tile's columns being dv / 8 apart.
 //
 // SHARED = false: the CTA's four warps own the same rows and cut the keys among them, tile by tile (decode: a group's heads fill the rows and one pass over the
 // keys serves all); each has its own cp.async ring, no barrier in the loop; their sums are joined at the end in shared memory.  TWO: 16 rows, else 8.
@@ -25,12 +25,6 @@ __device__ __forceinline__ void mma_f16_16816(float (&c)[4], const uint32_t (&a)
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-// c (16 rows x 8) += a (16 x 32) b (32 x 8), e4m3
-__device__ __forceinline__ void mma_e4m3_16832(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 // two numbers as e4m3 codes (the first in the low byte), and as codes TIMES times what those leave of them
 template <int TIMES = 16> __device__ __forceinline__ uint2 split_e4m3(float lo, float hi) {
@@ -179,14 +173,14 @@ template <int DP, int DVP, bool SHARED, bool TWO> __global__ void __launch_bound
         look(k_lo + warp * kFmKeys);
 #pragma unroll
         for (int i = 0; i < STAGES - 1; i++) load_tile(i, k_lo + warp * kFmKeys + i * STEP);
-        // ---------------------------------------------------------------- queries: the thread's 16 columns of every 64, split into two e4m3 rows
-        uint32_t Q[ROWS][2 * KC][4];
+        // ---------------------------------------------------------------- queries: the thread's 16 columns of every 64
+        uint32_t Q[ROWS][8 * KC];
         float fac[ROWS];
 #pragma unroll
         for (int r = 0; r < ROWS; r++) {
             const bool v = r ? vB : vA;
             const __nv_bfloat16* row = (const __nv_bfloat16*)a.q + ((long)(tok0 + (r ? tokB : tokA)) * a.H + (r ? hB : hA)) * d;
-            uint32_t w[8 * KC];
+            uint32_t(&w)[8 * KC] = Q[r];
 #pragma unroll
             for (int c = 0; c < KC; c++)
 #pragma unroll
@@ -196,31 +190,17 @@ template <int DP, int DVP, bool SHARED, bool TWO> __global__ void __launch_bound
                     if (v && at < d) x = *reinterpret_cast<const uint4*>(row + at);
                     w[8 * c + 4 * i] = x.x; w[8 * c + 4 * i + 1] = x.y; w[8 * c + 4 * i + 2] = x.z; w[8 * c + 4 * i + 3] = x.w;
                 }
-            float top = 0.f, odd = 0.f;      // odd: NaN as soon as a value is not finite (e4m3 has no infinity)
+            float top = 0.f;
 #pragma unroll
-            for (int i = 0; i < 8 * KC; i++) {
-                const float x = __uint_as_float(w[i] << 16), y = __uint_as_float(w[i] & 0xffff0000u);
-                top = fmaxf(top, fmaxf(fabsf(x), fabsf(y)));
-                odd = fmaf(x, 0.f, fmaf(y, 0.f, odd));
-            }
+            for (int i = 0; i < 8 * KC; i++) top = fmaxf(top, fmaxf(fabsf(__uint_as_float(w[i] << 16)), fabsf(__uint_as_float(w[i] & 0xffff0000u))));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            odd += __shfl_xor_sync(0xffffffffu, odd, 1);
-            odd += __shfl_xor_sync(0xffffffffu, odd, 2);
-            // 2^(7 - e) of a largest 1.f 2^e, within what fp32 holds with its inverse
-            const int up = min(126, max(-120, 7 - ((int)(__float_as_uint(top) >> 23) - 127)));
+            // 2^(14 - e) of a largest 1.f 2^e, within what fp32 holds with its inverse (an infinity stays one)
+            const int up = min(126, max(-112, 14 - ((int)(__float_as_uint(top) >> 23) - 127)));
             const float by = __uint_as_float((uint32_t)(up + 127) << 23);
-            fac[r] = v ? (a.head_scale ? a.scale * a.head_scale[r ? hB : hA] : a.scale) / by * (a.softcap > 0.f ? 1.f : kLog2e) + odd : 0.f;
+            fac[r] = v ? (a.head_scale ? a.scale * a.head_scale[r ? hB : hA] : a.scale) / by * (a.softcap > 0.f ? 1.f : kLog2e) : 0.f;
 #pragma unroll
-            for (int s = 0; s < 2 * KC; s++)      // columns 8 s .. 8 s + 7 of the thread's
-#pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    const uint32_t u = w[4 * s + 2 * i], x = w[4 * s + 2 * i + 1];
-                    const uint2 lo2 = split_e4m3(__uint_as_float(u << 16) * by, __uint_as_float(u & 0xffff0000u) * by);
-                    const uint2 hi2 = split_e4m3(__uint_as_float(x << 16) * by, __uint_as_float(x & 0xffff0000u) * by);
-                    Q[r][s][2 * i] = lo2.x | hi2.x << 16;
-                    Q[r][s][2 * i + 1] = lo2.y | hi2.y << 16;
-                }
+            for (int i = 0; i < 8 * KC; i++) w[i] = pack_f16(__uint_as_float(w[i] << 16) * by, __uint_as_float(w[i] & 0xffff0000u) * by);
         }
         const float two_over_cap = a.softcap > 0.f ? 2.0f / a.softcap : 0.f;
         const int w_min_pos = pos0 + wtok, w_max_pos = pos0 + min(ntok - 1, wtok + TOKS - 1);
@@ -232,25 +212,19 @@ template <int DP, int DVP, bool SHARED, bool TWO> __global__ void __launch_bound
 #pragma unroll
             for (int n = 0; n < 2; n++) {
                 const int r = 8 * n + gq;
-                float acc[ROWS][4];
 #pragma unroll
-                for (int h = 0; h < ROWS; h++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) acc[h][e] = 0.f;
+                for (int e = 0; e < 4; e++) S[n][e] = 0.f;
 #pragma unroll
                 for (int c = 0; c < KC; c++) {
                     const uint4 k = lds16(kd + r * DP + 16 * (DP == 128 ? (4 * c + tq) ^ ((r & 1) << 2) : tq));
+                    const uint32_t kw[4] = {k.x, k.y, k.z, k.w};
 #pragma unroll
-                    for (int h = 0; h < ROWS; h++) {
-                        mma_e4m3_16832(acc[h], Q[h][2 * c][0], Q[h][2 * c][1], Q[h][2 * c][2], Q[h][2 * c][3], k.x, k.y);
-                        mma_e4m3_16832(acc[h], Q[h][2 * c + 1][0], Q[h][2 * c + 1][1], Q[h][2 * c + 1][2], Q[h][2 * c + 1][3], k.z, k.w);
+                    for (int s = 0; s < 4; s++) {      // columns 4 s .. 4 s + 3 of the thread's 16
+                        const int at = 8 * c + 2 * s;
+                        const uint32_t q[4] = {Q[0][at], TWO ? Q[ROWS - 1][at] : 0u, Q[0][at + 1], TWO ? Q[ROWS - 1][at + 1] : 0u};
+                        mma_f16_16816(S[n], q, f16_of_codes(kw[s]), f16_of_codes(kw[s] >> 16));
                     }
                 }
-#pragma unroll
-                for (int h = 0; h < ROWS; h++)
-#pragma unroll
-                    for (int i = 0; i < 2; i++) S[n][2 * h + i] = fmaf(acc[h][2 + i], 0.0625f, acc[h][i]);
-                if (!TWO) S[n][2] = S[n][3] = 0.f;
             }
             // the thread's keys: k0 + 8 n + 2 tq + {0, 1}
             float inv[4];
