@@ -359,7 +359,10 @@ static bool fg_vec(const ktb200_fp8_attn_params* c) {      // whole pieces of 16
 }
 static Fp8Form fp8_form(const ktb200_fp8_attn_params* c, int n_tokens, int dtype, int allow_tensor_cores) {
     const int R = c->heads / c->kv_heads;
-    if (allow_tensor_cores && fd_takes(c, n_tokens, dtype)) return {Fp8Form::kDecode, {}, 1, fm_heads(R), kFdAlign, 3};
+    if (allow_tensor_cores && fd_takes(c, n_tokens, dtype)) {
+        const int RH = fd_heads(R, c->dim);
+        return {Fp8Form::kDecode, {}, 1, RH, c->dim == 64 ? 128 : 64, RH <= 8 && c->dim == 128 ? 3 : 2, 0};
+    }
     if (allow_tensor_cores && fp_takes(c, n_tokens, dtype)) return {Fp8Form::kPrompt, {}, 2 * (128 / fm_heads(R)), fm_heads(R), kFpKeys, 1, 0};
     if (allow_tensor_cores && fm_takes(c, dtype)) {
         const FmForm f = fm_form(c, n_tokens);

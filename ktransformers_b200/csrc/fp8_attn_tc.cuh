@@ -1,4 +1,4 @@
-// Attention of single tokens over the paged e4m3 cache on tcgen05 (bf16 queries, heads of 128, up to 16 query heads per key/value head, pages of whole 16 tokens): the decode step.
+// Attention of single tokens over the paged e4m3 cache on tcgen05 (bf16 queries, heads of 128 or 64, pages of whole 16 tokens): the decode step.
 //
 // A CTA has one token, one key/value head and its query heads, and a part of the key range in tiles of 128 keys.  The codes are operands as they lie in the cache: nothing is converted.
 //     S^T = K Q^T     128 keys x N, kind::f8f6f4, K the K-major A operand as TMA delivered it
@@ -8,6 +8,9 @@
 //   weights   p = 2^(t - m), t = s log2(e) + log2(value scale): 2^-8 of a weight off at most (as a bf16 weight is) and 2^-21 of the largest where that is more.  Value scales are
 //             powers of two: in the exponent they cost nothing and O needs none.  m is 7 below a head's largest t, raised when a t outgrows it by 8.75 (2^8.75 < 448)
 // l += p / (value scale), O / l is the result: 2^m drops out.
+// Heads of 64 (PAIR = 2): a row of 128 bytes is two neighbouring keys.  Queries and weights then have rows of their own for the first and for the second of a pair, zero where the other's
+// columns are; of the products, twice as many as needed, the mixed ones are not looked at.  What bounds is the bytes all the same: 30 tokens over 2000 to 4000 keys, 64 heads over 8, take
+// 43 us where fp16 mma tiles take 56, one over 60000 keys 24 us against 33.
 //     warp 0      TMA: K and V tiles, two stages; a tile is runs of 16, 32 or 64 keys, each inside one page (runs that no key of the part lies in come as zeros)
 //     warp 1      MMAs: S of the next tile ahead of PV of this one
 //     warps 2-5   a thread owns a key: its scores of all heads are one row of S^T, so that scales and masks are its own; maxima are only needed when one has outgrown its
@@ -23,7 +26,7 @@
 
 namespace ktb {
 
-constexpr int kFdThreads = 192, kFdKeys = 128, kFdTile = kFdKeys * 128, kFdStages = 2, kFdAlign = 64;
+constexpr int kFdThreads = 192, kFdRows = 128, kFdTile = kFdRows * 128, kFdStages = 2;
 constexpr float kFdTop = 7.f, kFdRaise = 8.75f;
 struct FdMisc {
     unsigned long long k_full[kFdStages], k_free[kFdStages], v_full[kFdStages], v_free[kFdStages], s_full[2], s_free[2], p_full[2], p_free[2], q_ready;
@@ -31,7 +34,7 @@ struct FdMisc {
     uint32_t tmem_base;
     int found;
 };
-template <int RP> constexpr int fd_smem() { return 2 * kFdStages * kFdTile + 3 * 2 * RP * 128 + (int)sizeof(FdMisc) + 1024; }
+template <int RP, int PAIR> constexpr int fd_smem() { return 2 * kFdStages * kFdTile + 3 * 2 * RP * PAIR * 128 + (int)sizeof(FdMisc) + 1024; }
 
 struct FdMaps { CUtensorMap k, v; };
 constexpr int kFdCluster = 8;
@@ -54,9 +57,9 @@ __device__ __forceinline__ bool fd_any(bool p) {      // over the four soft-max 
 }
 __device__ __forceinline__ void fd_sync() { asm volatile("barrier.cta.sync 1, 128;" ::: "memory"); }
 
-template <int RP> __global__ void __launch_bounds__(kFdThreads, RP == 8 ? 3 : 2) fp8_attn_decode_kernel(const __grid_constant__ FdMaps maps, const Fp8Attn a, int RH, int run) {
+template <int RP, int PAIR> __global__ void __launch_bounds__(kFdThreads, RP * PAIR == 8 ? 3 : 2) fp8_attn_decode_kernel(const __grid_constant__ FdMaps maps, const Fp8Attn a, int RH, int run) {
     using namespace umma;
-    constexpr int N = 2 * RP, OP = N * 128;      // bytes of an operand of N rows
+    constexpr int N = 2 * RP * PAIR, OP = N * 128, D = 128 / PAIR, KEYS = kFdRows * PAIR;      // OP: bytes of an operand of N rows
     extern __shared__ __align__(16) uint8_t fd_smem_raw[];
     const uint32_t raw = smem_u32(fd_smem_raw), base = (raw + 1023u) & ~1023u;
     uint8_t* smem = fd_smem_raw + (base - raw);
@@ -77,11 +80,12 @@ template <int RP> __global__ void __launch_bounds__(kFdThreads, RP == 8 ? 3 : 2)
     const int t = blockIdx.x, R = a.H / a.G, hblocks = R / RH, g = blockIdx.y / hblocks, h0 = g * R + (blockIdx.y % hblocks) * RH;
     const int p = a.pos[t], slot = a.slot[t];
     uint2 q_row[RP / 4];
-    if (warp >= 2) {      // a warp a head: a lane has columns 4 lane ..
+    if (warp >= 2) {      // a warp a head: a lane has columns 4 lane .. (2 lane ..)
 #pragma unroll
         for (int i = 0; i < RP / 4; i++) {
             const int h = warp - 2 + 4 * i;
-            q_row[i] = h < RH ? *reinterpret_cast<const uint2*>((const __nv_bfloat16*)a.q + ((long)t * a.H + h0 + h) * 128 + 4 * lane) : make_uint2(0, 0);
+            const __nv_bfloat16* row = (const __nv_bfloat16*)a.q + ((long)t * a.H + h0 + h) * D + 4 / PAIR * lane;
+            q_row[i] = h >= RH ? make_uint2(0, 0) : PAIR == 1 ? *reinterpret_cast<const uint2*>(row) : make_uint2(*reinterpret_cast<const uint32_t*>(row), 0);
         }
     } else if (warp == 0) {
         bool mine = false;
@@ -94,8 +98,8 @@ template <int RP> __global__ void __launch_bounds__(kFdThreads, RP == 8 ? 3 : 2)
     }
     __syncthreads();
     if (!misc.found) return;
-    const int lo = fp8_first_visible(p, a.window, a.chunk), lo_al = lo & ~(kFdAlign - 1);
-    const int even = a.even, part = even ? ((p + 1 - lo_al + kFdKeys - 1) / kFdKeys + even - 1) / even * kFdKeys : a.part;
+    const int lo = fp8_first_visible(p, a.window, a.chunk), lo_al = lo & ~(a.align - 1);
+    const int even = a.even, part = even ? ((p + 1 - lo_al + KEYS - 1) / KEYS + even - 1) / even * KEYS : a.part;
     const bool cut = !even && part > 0 && p + 1 - lo_al > part;
     const int k_lo = lo_al + blockIdx.z * part, k_hi = cut || even ? min(p + 1, k_lo + part) : p + 1;
     float* join = reinterpret_cast<float*>(smem);      // a cluster's CTA: (reference, sum) of RP heads, then RP rows of 128 columns, over the ring
@@ -108,7 +112,7 @@ template <int RP> __global__ void __launch_bounds__(kFdThreads, RP == 8 ? 3 : 2)
         }
         return;
     }
-    const int tiles = (k_hi - k_lo + kFdKeys - 1) / kFdKeys;
+    const int tiles = (k_hi - k_lo + KEYS - 1) / KEYS;
     if (warp == 1) tmem_alloc(smem_u32(&misc.tmem_base), 128);
     tc_fence_before();
     __syncthreads();
@@ -123,12 +127,12 @@ template <int RP> __global__ void __launch_bounds__(kFdThreads, RP == 8 ? 3 : 2)
 
     if (warp == 0) {
         // ================================================================ copies
-        const int runs = kFdKeys / run, ahead = 32 / runs, none = a.pages.n_pages * a.G * ps;      // (rows from `none` on are outside the maps: zeros)
+        const int runs = kFdRows / run, ahead = 32 / runs, none = a.pages.n_pages * a.G * (ps / PAIR);      // (rows from `none` on are outside the maps: zeros)
         int row = none;
         for (int j = 0; j < tiles; j++) {
             if (j % ahead == 0) {      // a lane looks one run's page up, for as many tiles as the lanes reach
-                const int kp = k_lo + j * kFdKeys + lane * run, page = slot_ok && kp < k_hi && kp + run > lo ? page_of(kp) : -1;
-                row = page < 0 ? none : (page * a.G + g) * ps + kp % ps;
+                const int kp = k_lo + j * KEYS + lane * run * PAIR, page = slot_ok && kp < k_hi && kp + run * PAIR > lo ? page_of(kp) : -1;
+                row = page < 0 ? none : (page * a.G + g) * (ps / PAIR) + kp % ps / PAIR;
             }
             const int st = j % kFdStages, ph = ((j / kFdStages) & 1) ^ 1;
             const uint32_t kf = smem_u32(&misc.k_full[st]), vf = smem_u32(&misc.v_full[st]);
@@ -158,6 +162,15 @@ template <int RP> __global__ void __launch_bounds__(kFdThreads, RP == 8 ? 3 : 2)
             if (j < tiles) {
                 const int st = j % kFdStages, buf = j & 1;
                 bar_wait(smem_u32(&misc.k_full[st]), (j / kFdStages) & 1);
+                const int k0 = k_lo + j * KEYS;
+                if (PAIR == 2 && (k0 < lo || k0 + KEYS > k_hi)) {      // the first and last tiles: a key that is not seen may be anything, and stands in a row with one that is (0 x NaN)
+                    for (int i = lane; i < kFdRows * 8; i += 32) {
+                        const int row = i >> 3, c = i & 7, key = k0 + 2 * row + (c >> 2);
+                        if (key < lo || key >= k_hi) *reinterpret_cast<uint4*>(smem + (kbase - base) + st * kFdTile + row * 128 + ((c ^ (row & 7)) << 4)) = make_uint4(0, 0, 0, 0);
+                    }
+                    fence_async_smem();
+                    __syncwarp();
+                }
                 bar_wait(smem_u32(&misc.s_free[buf]), ((j >> 1) & 1) ^ 1);
                 tc_fence_after();
                 mma_f8_x4(tmem + buf * N, smem_desc(kbase + st * kFdTile, 16, 1024, kLayoutSw128), smem_desc(qbase, 16, 1024, kLayoutSw128), idesc_s, 0, smem_u32(&misc.s_full[buf]),
@@ -192,8 +205,19 @@ template <int RP> __global__ void __launch_bounds__(kFdThreads, RP == 8 ? 3 : 2)
                 const int up = min(126, max(-120, 7 - ((int)(__float_as_uint(top) >> 23) - 127)));      // 2^(7 - e) of a largest 1.f 2^e, within what fp32 holds with its inverse
                 const float by = __uint_as_float((uint32_t)(up + 127) << 23);
                 const uint2 lo2 = split_e4m3(x[0] * by, x[1] * by), hi2 = split_e4m3(x[2] * by, x[3] * by);
-                *reinterpret_cast<uint32_t*>(smem + (qbase - base) + fd_at(h, 4 * lane)) = lo2.x | hi2.x << 16;
-                *reinterpret_cast<uint32_t*>(smem + (qbase - base) + fd_at(RP + h, 4 * lane)) = lo2.y | hi2.y << 16;
+                uint8_t* Q = smem + (qbase - base);
+                if constexpr (PAIR == 1) {
+                    *reinterpret_cast<uint32_t*>(Q + fd_at(h, 4 * lane)) = lo2.x | hi2.x << 16;
+                    *reinterpret_cast<uint32_t*>(Q + fd_at(RP + h, 4 * lane)) = lo2.y | hi2.y << 16;
+                } else {
+#pragma unroll
+                    for (int u = 0; u < 2; u++)
+#pragma unroll
+                        for (int k = 0; k < 2; k++) {      // row 2 RP u + h (+ RP): key u of a pair
+                            *reinterpret_cast<uint16_t*>(Q + fd_at(2 * RP * u + h, 64 * k + 2 * lane)) = u == k ? (uint16_t)lo2.x : (uint16_t)0;
+                            *reinterpret_cast<uint16_t*>(Q + fd_at(2 * RP * u + RP + h, 64 * k + 2 * lane)) = u == k ? (uint16_t)lo2.y : (uint16_t)0;
+                        }
+                }
                 if (lane == 0) misc.fac[h] = h < RH ? (a.head_scale ? a.scale * a.head_scale[h0 + h] : a.scale) / by * (a.softcap > 0.f ? 1.f : kLog2e) + odd : 0.f;
             }
             fence_async_smem();
@@ -205,9 +229,8 @@ template <int RP> __global__ void __launch_bounds__(kFdThreads, RP == 8 ? 3 : 2)
 #pragma unroll
         for (int h = 0; h < RP; h++) { fac[h] = misc.fac[h]; m[h] = -INFINITY; l[h] = 0.f; }
         const float two_over_cap = a.softcap > 0.f ? 2.0f / a.softcap : 0.f, cap = a.softcap * kLog2e;
-        // the scales of the thread's key, a tile ahead, and its page, two ahead
-        auto see = [&](int j) { const int key = k_lo + j * kFdKeys + r; return slot_ok && key >= lo && key < k_hi; };
-        auto look = [&](int j) { return see(j) ? page_of(k_lo + j * kFdKeys + r) : -1; };
+        // the scales of the thread's keys (which share a page), a tile ahead, and their page, two ahead
+        auto look = [&](int j) { const int key = k_lo + j * KEYS + PAIR * r; return slot_ok && key + PAIR > lo && key < k_hi ? page_of(key) : -1; };
         auto scales_of = [&](int page) { return page < 0 ? make_float2(0.f, 0.f) : *reinterpret_cast<const float2*>(a.scales + 2 * ((long)page * a.G + g)); };
         float2 sc = scales_of(look(0));
         int page1 = look(1);
@@ -215,7 +238,8 @@ template <int RP> __global__ void __launch_bounds__(kFdThreads, RP == 8 ? 3 : 2)
             const int buf = j & 1;
             const float2 next = scales_of(page1);
             page1 = look(j + 2);
-            const bool here = sc.y > 0.f;      // (scales of a key that is not seen are zero)
+            const int key0 = k_lo + j * KEYS + PAIR * r;
+            const bool there = sc.y > 0.f;      // (scales of keys that are not seen are zero)
             bar_wait(smem_u32(&misc.s_full[buf]), (j >> 1) & 1);
             tc_fence_after();
             uint32_t s[N];
@@ -224,24 +248,27 @@ template <int RP> __global__ void __launch_bounds__(kFdThreads, RP == 8 ? 3 : 2)
             tc_fence_before();
             __syncwarp();
             if (lane == 0) bar_arrive(smem_u32(&misc.s_free[buf]));
-            const float ve = (float)((int)(__float_as_uint(sc.y) >> 23) - 127), inv = here ? __uint_as_float((254u << 23) - __float_as_uint(sc.y)) : 0.f;
-            float x[RP];
+            const float ve = (float)((int)(__float_as_uint(sc.y) >> 23) - 127), inv = there ? __uint_as_float((254u << 23) - __float_as_uint(sc.y)) : 0.f;
+            float x[PAIR * RP];
             bool up = false;
 #pragma unroll
-            for (int h = 0; h < RP; h++) x[h] = fmaf(__uint_as_float(s[RP + h]), 0.0625f, __uint_as_float(s[h])) * (fac[h] * sc.x);
+            for (int i = 0; i < PAIR * RP; i++) {
+                const int u = i / RP, h = i % RP;
+                x[i] = fmaf(__uint_as_float(s[2 * RP * u + RP + h]), 0.0625f, __uint_as_float(s[2 * RP * u + h])) * (fac[h] * sc.x);
+            }
             if (a.softcap > 0.f) {
 #pragma unroll
-                for (int h = 0; h < RP; h++) x[h] = cap * (1.0f - __fdividef(2.0f, __expf(x[h] * two_over_cap) + 1.0f));      // c tanh(s / c): a few 1e-7 of the cap off
+                for (int i = 0; i < PAIR * RP; i++) x[i] = cap * (1.0f - __fdividef(2.0f, __expf(x[i] * two_over_cap) + 1.0f));      // c tanh(s / c): a few 1e-7 of the cap off
             }
 #pragma unroll
-            for (int h = 0; h < RP; h++) {
-                x[h] = here ? x[h] + ve : -INFINITY;
-                up |= x[h] > m[h] + kFdRaise;
+            for (int i = 0; i < PAIR * RP; i++) {
+                x[i] = there && key0 + i / RP >= lo && key0 + i / RP < k_hi ? x[i] + ve : -INFINITY;
+                up |= x[i] > m[i % RP] + kFdRaise;
             }
             if (fd_any(up)) {      // (always in the first tile that has a key)
 #pragma unroll
                 for (int h = 0; h < RP; h++) {
-                    const float top = warp_max(x[h]);
+                    const float top = warp_max(PAIR == 1 ? x[h] : fmaxf(x[h], x[PAIR * RP - RP + h]));
                     if (lane == 0) misc.red[w4][h] = top;
                 }
                 fd_sync();
@@ -263,7 +290,7 @@ template <int RP> __global__ void __launch_bounds__(kFdThreads, RP == 8 ? 3 : 2)
                     if constexpr (N == 16) tmem_ld16(tmem_o + lanes, o); else tmem_ld32(tmem_o + lanes, o);
                     tmem_wait_ld();
 #pragma unroll
-                    for (int h = 0; h < RP; h++) { o[h] = __float_as_uint(__uint_as_float(o[h]) * k[h]); o[RP + h] = __float_as_uint(__uint_as_float(o[RP + h]) * k[h]); }
+                    for (int i = 0; i < N; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * k[i % RP]);
                     if constexpr (N == 16) tmem_st16(tmem_o + lanes, o); else tmem_st32(tmem_o + lanes, o);
                     tmem_wait_st();
                     tc_fence_before();
@@ -272,25 +299,29 @@ template <int RP> __global__ void __launch_bounds__(kFdThreads, RP == 8 ? 3 : 2)
             if (j > 1) bar_wait(smem_u32(&misc.p_free[buf]), ((j - 2) >> 1) & 1);
             uint8_t* P = smem + (pbase - base) + buf * OP;
 #pragma unroll
-            for (int h = 0; h < RP; h += 2) {
+            for (int i = 0; i < PAIR * RP; i += 2) {
+                const int h = i % RP, n = i / RP * 2 * RP + h;
                 const float u0 = m[h] == -INFINITY ? 0.f : m[h], u1 = m[h + 1] == -INFINITY ? 0.f : m[h + 1];
-                const float p0 = exp2_approx(x[h] - u0), p1 = exp2_approx(x[h + 1] - u1);
+                const float p0 = exp2_approx(x[i] - u0), p1 = exp2_approx(x[i + 1] - u1);
                 l[h] = fmaf(p0, inv, l[h]);
                 l[h + 1] = fmaf(p1, inv, l[h + 1]);
                 const uint2 c = split_e4m3(p0, p1);
-                P[fd_at(h, r)] = (uint8_t)c.x;
-                P[fd_at(h + 1, r)] = (uint8_t)(c.x >> 8);
-                P[fd_at(RP + h, r)] = (uint8_t)c.y;
-                P[fd_at(RP + h + 1, r)] = (uint8_t)(c.y >> 8);
+                P[fd_at(n, r)] = (uint8_t)c.x;
+                P[fd_at(n + 1, r)] = (uint8_t)(c.x >> 8);
+                P[fd_at(n + RP, r)] = (uint8_t)c.y;
+                P[fd_at(n + RP + 1, r)] = (uint8_t)(c.y >> 8);
             }
-            const int k0 = k_lo + j * kFdKeys;
-            if (k0 < lo || k0 + kFdKeys > k_hi) {      // the first and last tiles: values of keys that are not seen may be anything (0 x NaN)
+            const int k0 = k_lo + j * KEYS;
+            if (k0 < lo || k0 + KEYS > k_hi) {      // the first and last tiles: values of keys that are not seen may be anything (0 x NaN)
                 const int st = j % kFdStages;
                 bar_wait(smem_u32(&misc.v_full[st]), (j / kFdStages) & 1);
-                if (k0 + r < lo || k0 + r >= k_hi) {
 #pragma unroll
-                    for (int i = 0; i < 8; i++) *reinterpret_cast<uint4*>(smem + (vbase - base) + st * kFdTile + r * 128 + 16 * i) = make_uint4(0, 0, 0, 0);
-                }
+                for (int u = 0; u < PAIR; u++)
+                    if (key0 + u < lo || key0 + u >= k_hi) {
+#pragma unroll
+                        for (int i = 0; i < 8 / PAIR; i++)
+                            *reinterpret_cast<uint4*>(smem + (vbase - base) + st * kFdTile + r * 128 + (((8 / PAIR * u + i) ^ (r & 7)) << 4)) = make_uint4(0, 0, 0, 0);
+                    }
             }
             fence_async_smem();
             __syncwarp();
@@ -309,27 +340,43 @@ template <int RP> __global__ void __launch_bounds__(kFdThreads, RP == 8 ? 3 : 2)
         uint32_t o[N];
         if constexpr (N == 16) tmem_ld16(tmem_o + lanes, o); else tmem_ld32(tmem_o + lanes, o);
         tmem_wait_ld();
+        float v[RP];      // of column r; heads of 64: what the first keys of pairs give it, and from thread r + 64 what the second ones do
+        if constexpr (PAIR == 1) {
+#pragma unroll
+            for (int h = 0; h < RP; h++) v[h] = fmaf(__uint_as_float(o[RP + h]), 0.0625f, __uint_as_float(o[h]));
+        } else {
+            float* other = join + 2 * RP + 128 * RP;
+#pragma unroll
+            for (int h = 0; h < RP; h++) {
+                v[h] = r < 64 ? fmaf(__uint_as_float(o[RP + h]), 0.0625f, __uint_as_float(o[h])) : fmaf(__uint_as_float(o[N - RP + h]), 0.0625f, __uint_as_float(o[N - 2 * RP + h]));
+                if (r >= 64) other[64 * h + r - 64] = v[h];
+            }
+            fd_sync();
+            if (r < 64) {
+#pragma unroll
+                for (int h = 0; h < RP; h++) v[h] += other[64 * h + r];
+            }
+        }
         fd_sync();
 #pragma unroll
         for (int h = 0; h < RP; h++) {
-            if (h >= RH) break;
-            float sum = (misc.red[0][h] + misc.red[1][h]) + (misc.red[2][h] + misc.red[3][h]), v = fmaf(__uint_as_float(o[RP + h]), 0.0625f, __uint_as_float(o[h]));
+            if (h >= RH || r >= D) break;
+            float sum = (misc.red[0][h] + misc.red[1][h]) + (misc.red[2][h] + misc.red[3][h]);
             const long row = (long)t * a.H + h0 + h;
             if (even) {
                 if (r == 0) { join[2 * h] = m[h]; join[2 * h + 1] = sum; }
-                join[2 * RP + 128 * h + r] = v;
+                join[2 * RP + 128 * h + r] = v[h];
             } else if (cut) {
-                float* part = a.partial + (row * a.parts + blockIdx.z) * 130;
+                float* part = a.partial + (row * a.parts + blockIdx.z) * (D + 2);
                 if (r == 0) { part[0] = m[h]; part[1] = sum; }
-                part[2 + r] = v;
+                part[2 + r] = v[h];
             } else {
                 if (a.sink) {
                     const float sk = a.sink[h0 + h] * kLog2e, mn = fmaxf(m[h], sk), k = m[h] == -INFINITY ? 0.f : exp2_approx(m[h] - mn);
                     sum = sum * k + exp2_approx(sk - mn);
-                    v *= k;
+                    v[h] *= k;
                 }
-                v = sum > 0.f || sum != sum ? v * (a.out_scale / sum) : 0.f;
-                ((__nv_bfloat16*)a.out)[(long)t * a.out_stride + (long)(h0 + h) * 128 + r] = __float2bfloat16_rn(v);
+                ((__nv_bfloat16*)a.out)[(long)t * a.out_stride + (long)(h0 + h) * D + r] = __float2bfloat16_rn(sum > 0.f || sum != sum ? v[h] * (a.out_scale / sum) : 0.f);
             }
         }
     }
@@ -340,7 +387,7 @@ template <int RP> __global__ void __launch_bounds__(kFdThreads, RP == 8 ? 3 : 2)
         cluster_wait();
         if (warp >= 2) {
             const int c = tid - 64, cuts = (p + 1 - lo_al + part - 1) / part;      // the CTAs that have keys
-            for (int h = blockIdx.z; h < RH; h += cuts) {
+            for (int h = blockIdx.z; h < RH && c < D; h += cuts) {
                 float mk[kFdCluster], lk[kFdCluster], vk[kFdCluster], top = a.sink ? a.sink[h0 + h] * kLog2e : -INFINITY;
 #pragma unroll
                 for (int k = 0; k < kFdCluster; k++)
@@ -359,7 +406,7 @@ template <int RP> __global__ void __launch_bounds__(kFdThreads, RP == 8 ? 3 : 2)
                         v = fmaf(vk[k], w, v);
                     }
                 v = sum > 0.f || sum != sum ? v * (a.out_scale / sum) : 0.f;
-                ((__nv_bfloat16*)a.out)[(long)t * a.out_stride + (long)(h0 + h) * 128 + c] = __float2bfloat16_rn(v);
+                ((__nv_bfloat16*)a.out)[(long)t * a.out_stride + (long)(h0 + h) * D + c] = __float2bfloat16_rn(v);
             }
         }
         __syncwarp();
@@ -374,16 +421,22 @@ template <int RP> __global__ void __launch_bounds__(kFdThreads, RP == 8 ? 3 : 2)
     }
 }
 
-// heads of a group that one CTA takes: the largest divisor of the group up to 16
 static bool fd_takes(const ktb200_fp8_attn_params* c, int n_tokens, int dtype) {
-    return fm_takes(c, dtype) && c->dim == 128 && c->vdim == 128 && c->page_size % 16 == 0 && (long)n_tokens <= 2L * c->n_seqs && (long)c->n_pages * c->kv_heads * c->page_size < (1L << 31) &&
-           c->n_pages > 0;
+    return fm_takes(c, dtype) && c->dim == c->vdim && (c->dim == 128 || c->dim == 64) && c->page_size % 16 == 0 && (long)n_tokens <= 2L * c->n_seqs &&
+           (long)c->n_pages * c->kv_heads * c->page_size < (1L << 31) && c->n_pages > 0;
 }
-template <int RP> static cudaError_t fd_launch_as(const FdMaps& maps, const Fp8Attn& a, int RH, int run, dim3 grid, cudaStream_t s) {
-    const cudaError_t e = raise_smem_limit((const void*)fp8_attn_decode_kernel<RP>, fd_smem<RP>());
+// heads of a group that one CTA takes: 16 at most, 8 for heads of 64
+static int fd_heads(int R, int dim) {
+    int h = fm_heads(R);
+    if (dim == 64 && h > 8)
+        for (h = 8; R % h; h--) {}
+    return h;
+}
+template <int RP, int PAIR> static cudaError_t fd_launch_as(const FdMaps& maps, const Fp8Attn& a, int RH, int run, dim3 grid, cudaStream_t s) {
+    const cudaError_t e = raise_smem_limit((const void*)fp8_attn_decode_kernel<RP, PAIR>, fd_smem<RP, PAIR>());
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t lc{};
-    lc.gridDim = grid; lc.blockDim = dim3(kFdThreads); lc.dynamicSmemBytes = fd_smem<RP>(); lc.stream = s;
+    lc.gridDim = grid; lc.blockDim = dim3(kFdThreads); lc.dynamicSmemBytes = fd_smem<RP, PAIR>(); lc.stream = s;
     cudaLaunchAttribute at[2];
     int n = 0;
     if (pdl_enabled()) {
@@ -396,13 +449,13 @@ template <int RP> static cudaError_t fd_launch_as(const FdMaps& maps, const Fp8A
     }
     lc.attrs = at;
     lc.numAttrs = n;
-    return cudaLaunchKernelEx(&lc, fp8_attn_decode_kernel<RP>, maps, a, RH, run);
+    return cudaLaunchKernelEx(&lc, fp8_attn_decode_kernel<RP, PAIR>, maps, a, RH, run);
 }
 // the codes as rows of 128 bytes, boxes of `run` rows, 128-byte-swizzled
 static int fd_maps(FdMaps& maps, const Fp8Attn& a, int run) {
     const umma::EncodeTiledFn enc = umma::encode_tiled();
     if (!enc) { set_error("fp8_cache_attn: cuTensorMapEncodeTiled is not available from this driver"); return KTB200_ECUDA; }
-    const cuuint64_t dims[2] = {128, (cuuint64_t)a.pages.n_pages * a.G * a.pages.page_size}, strides[1] = {128};
+    const cuuint64_t dims[2] = {128, (cuuint64_t)a.pages.n_pages * a.G * a.pages.page_size * a.d / 128}, strides[1] = {128};
     const cuuint32_t box[2] = {128, (cuuint32_t)run}, estr[2] = {1, 1};
     for (int i = 0; i < 2; i++) {
         const CUresult cr = enc(i ? &maps.v : &maps.k, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t*>(i ? a.v_codes : a.k_codes), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
@@ -412,11 +465,14 @@ static int fd_maps(FdMaps& maps, const Fp8Attn& a, int run) {
     return KTB200_OK;
 }
 static int fd_launch(const Fp8Attn& a, int RH, dim3 grid, cudaStream_t s) {
-    const int ps = a.pages.page_size, run = ps % 64 == 0 ? 64 : ps % 32 == 0 ? 32 : 16;
+    const int pair = 128 / a.d;
+    int run = 64;      // rows of a box: whole boxes in a page
+    while (a.pages.page_size % (run * pair)) run >>= 1;
     FdMaps maps;
     const int rc = fd_maps(maps, a, run);
     if (rc) return rc;
-    KTB_CUDA_CHECK(RH <= 8 ? fd_launch_as<8>(maps, a, RH, run, grid, s) : fd_launch_as<16>(maps, a, RH, run, grid, s));
+    const auto launch = pair == 2 ? fd_launch_as<8, 2> : RH <= 8 ? fd_launch_as<8, 1> : fd_launch_as<16, 1>;
+    KTB_CUDA_CHECK(launch(maps, a, RH, run, grid, s));
     return KTB200_OK;
 }
 

@@ -302,6 +302,9 @@ SHAPES = [
     ([(500, 1), (3, 1), (129, 1)], 16, 12, 2, 128, 128),
     ([(1400, 1), (900, 1), (0, 1), (300, 1), (511, 1)], 64, 4, 2, 128, 128),
     ([(9000, 1)], 64, 2, 1, 128, 128),
+    ([(1400, 1), (901, 1), (0, 1), (300, 1), (511, 1)], 32, 16, 1, 64, 64),
+    ([(9001, 1)], 16, 2, 1, 64, 64),
+    ([(700, 1), (33, 1)], 80, 12, 1, 64, 64),
     ([(500, 1), (3, 1)], 48, 34, 2, 128, 128),                        # a group that no run of 16 heads divides
 ]
 
@@ -324,6 +327,7 @@ def test_attention_masks_and_scores(options, dtype):
     run_attention([(100, 1), (0, 4), (31, 3)], 48, 6, 2, 96, 64, dtype, seed=6, **options)
     run_attention([(150, 40), (0, 140), (600, 3)], 64, 8, 2, 128, 128, dtype, seed=7, **options)
     run_attention([(200, 1), (0, 1), (1300, 1)], 64, 16, 1, 128, 128, dtype, seed=7, **options)
+    run_attention([(201, 1), (0, 1), (1300, 1)], 64, 8, 1, 64, 64, dtype, seed=7, **options)
 
 
 @pytest.mark.gpu
@@ -331,6 +335,7 @@ def test_attention_masks_and_scores(options, dtype):
 def test_attention_blocks_of_very_different_scales(dtype):
     run_attention([(400, 1), (90, 5)], 16, 4, 1, 64, 64, dtype, seed=8, wide=5)
     run_attention([(700, 1), (300, 1)], 64, 4, 1, 128, 128, dtype, seed=8, wide=5)
+    run_attention([(700, 1), (301, 1)], 64, 4, 1, 64, 64, dtype, seed=8, wide=5)
     run_attention([(300, 40)], 64, 4, 1, 128, 128, dtype, seed=8, wide=5)
 
 
@@ -351,6 +356,7 @@ def test_attention_does_not_see_pages_that_are_not_there(dtype):
         t[0, 1], t[1, 0] = total, -3
     run_attention([(100, 2), (0, 3), (60, 40)], 16, 4, 2, 64, 64, dtype, seed=10, break_table=break_table)      # (the second sequence sees nothing at all: zeros)
     run_attention([(1200, 1)], 64, 4, 2, 128, 128, dtype, seed=10, break_table=lambda t, total: t.__setitem__((0, 3), -1))
+    run_attention([(1200, 1)], 16, 4, 2, 64, 64, dtype, seed=10, break_table=lambda t, total: t.__setitem__((0, 3), -1))
 
 
 @pytest.mark.gpu
@@ -530,3 +536,22 @@ def test_a_model_served_from_an_8_bit_cache(tmp_path):
     logits = eng.step([("x", prompts[0], [89])])
     plain = Engine(model, max_tokens=1024, page_size=64).step([("x", prompts[0], [89])])
     assert logits.shape == plain.shape and torch.isfinite(logits).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("d,ps,base,window", [(128, 64, 300, 0), (128, 64, 300, 77), (64, 16, 301, 0), (64, 16, 300, 0), (64, 64, 300, 78), (64, 64, 1300, 77), (96, 16, 300, 77)])
+def test_attention_of_one_token_is_free_of_what_it_does_not_see(d, ps, base, window, dtype):
+    """NaN in all codes ahead of a window and behind the token, the seen keys' neighbours among them: the same result"""
+    H, G = 4, 2
+    batch, cache, total = U.batch_of([(base, 1)], ps)
+    kv = Fp8CacheLayer(*(x.cuda() for x in filled(total, G, ps, d, d, 14)))
+    q = torch.randn((1, H, d), generator=torch.Generator().manual_seed(3)).to(DT[dtype]).cuda()
+    clean = fp8_cache_attention(q, kv, on(batch), on(cache), H, G, d, d, d ** -0.5, window=window)
+    keep = torch.zeros((total, ps), dtype=torch.bool)
+    for key in range(max(0, base + 1 - window) if window else 0, base + 1):
+        keep[int(cache.page_table[0, key // ps]), key % ps] = True
+    for x in (kv.k, kv.v):
+        x.view(torch.uint8)[(~keep).cuda()[:, None, :, None].expand(total, G, ps, d)] = 0x7f
+    out = fp8_cache_attention(q, kv, on(batch), on(cache), H, G, d, d, d ** -0.5, window=window)
+    assert torch.equal(out, clean) and clean.isfinite().all() and float(clean.abs().max()) > 0

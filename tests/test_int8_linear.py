@@ -99,7 +99,7 @@ def test_linear_refuses_weights_that_do_not_fit():
 # ------------------------------------------------------------------------------------------------------------------------- GPU
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
-@pytest.mark.parametrize("T,K,N", [(1, 16, 1), (1, 2048, 2048), (1, 5000, 129), (2, 7168, 576), (3, 33, 7), (5, 128, 128), (8, 1536, 1000), (16, 640, 333), (17, 4096, 130), (31, 272, 2112),
+@pytest.mark.parametrize("T,K,N", [(1, 16, 1), (1, 1, 1), (3, 7, 130), (140, 1, 9500), (1, 2048, 2048), (1, 5000, 129), (2, 7168, 576), (3, 33, 7), (5, 128, 128), (8, 1536, 1000), (16, 640, 333), (17, 4096, 130), (31, 272, 2112),
                                    (64, 1024, 257), (65, 144, 512), (100, 2000, 384), (128, 512, 2000), (129, 256, 128), (257, 1040, 1025), (500, 130, 260), (1200, 384, 777)])
 def test_int8_linear(T, K, N, dtype):
     x, w, ws, bias = inputs(T, K, N, dtype, seed=T + K, bias=T % 2 == 1)
