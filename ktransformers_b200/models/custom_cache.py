@@ -119,6 +119,8 @@ class Fp8CacheLayer:
             raise ValueError(f"an 8-bit cache layer has k, v [pages, heads, page_size, size] and scales [pages, heads, 2], got {tuple(k.shape)}, {tuple(v.shape)}, {tuple(scales.shape)}")
         if not (k.is_contiguous() and v.is_contiguous() and scales.is_contiguous()):
             raise ValueError("an 8-bit cache layer's tensors have to be contiguous")
+        if not (k.device == v.device == scales.device):
+            raise ValueError("an 8-bit cache layer's tensors have to be on one device")
         self.k, self.v, self.scales = k, v, scales
 
     @classmethod

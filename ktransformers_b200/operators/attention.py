@@ -532,8 +532,8 @@ def _fp8_batch(what: str, rows: torch.Tensor, kv, batch, cache, kv_heads: int, d
         raise ValueError(f"{what}: the cache layer holds pages of {ps} tokens of {heads} heads of {d} + {v.shape[3]}, the call has {page_size}, {kv_heads}, {dim} + {vdim}")
     if seqs is None or not (seqs.dtype is pos.dtype is slot.dtype is table.dtype is torch.int32):
         raise ValueError(f"{what}: needs int32 pos, slot, seqs and page table")
-    if pos.shape[0] < T or slot.shape[0] < T or n_seqs > seqs.shape[1]:
-        raise ValueError(f"{what}: {T} tokens, but {pos.shape[0]} positions, {slot.shape[0]} slots; {n_seqs} portions of {seqs.shape[1]}")
+    if pos.shape[0] < T or slot.shape[0] < T or seqs.shape[0] < 2 or n_seqs > seqs.shape[1]:
+        raise ValueError(f"{what}: {T} tokens, but {pos.shape[0]} positions, {slot.shape[0]} slots; {n_seqs} portions of {tuple(seqs.shape)}")
     seqs_stride, columns = seqs.stride(), table.shape[1]
     if pos.stride(0) != 1 or slot.stride(0) != 1 or seqs_stride[1] != 1 or table.stride() != (columns, 1) or columns != cache.max_pages_per_seq:
         raise ValueError(f"{what}: index rows and page table rows have to be contiguous, max_pages_per_seq = {cache.max_pages_per_seq} of them")

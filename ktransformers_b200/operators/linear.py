@@ -255,8 +255,8 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
         raise ValueError(f"int8_linear: bias has to be {N} contiguous float32 values on {dev}")
     if not (weight.device == weight_scale.device == dev):
         raise ValueError("int8_linear: all tensors have to be on one device")
-    if bsz_tensor is not None and (bsz_tensor.dtype is not torch.int32 or bsz_tensor.device != dev):
-        raise ValueError(f"int8_linear: bsz_tensor has to be int32 on {dev}")
+    if bsz_tensor is not None and (bsz_tensor.dtype is not torch.int32 or bsz_tensor.device != dev or not bsz_tensor.numel()):
+        raise ValueError(f"int8_linear: bsz_tensor has to be int32 on {dev}, one value at least")
     x2 = x if len(shape) == 2 else x.reshape(-1, K)
     T, (x_stride, one) = x2.shape[0], x2.stride()
     if one != 1 or (T > 1 and x_stride < K):

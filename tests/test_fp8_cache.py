@@ -42,7 +42,7 @@ def test_exponent_is_the_smallest_that_reaches():
 def test_layer_refuses_other_tensors():
     k, v, s = filled(2, 2, 4, 8, 8, 0)
     Fp8CacheLayer(k, v, s)
-    for bad in ((k.float(), v, s), (k, v[:, :, :2], s), (k, v, s[:, :, :1]), (k, v, s.double()), (k.transpose(2, 3), v, s), (k[0], v[0], s[0])):
+    for bad in ((k.float(), v, s), (k, v[:, :, :2], s), (k, v, s[:, :, :1]), (k, v, s.double()), (k.transpose(2, 3), v, s), (k[0], v[0], s[0]), (k, v.to("meta"), s)):
         with pytest.raises(ValueError):
             Fp8CacheLayer(*bad)
     assert [tuple(x.shape) for x in Fp8CacheLayer(k, v, s).dequantize()] == [(2, 2, 4, 8)] * 2
@@ -55,6 +55,10 @@ def test_cache_manager_holds_layers_in_both_widths():
         PagedStateCache([32, 32], 0, 64, 2, "cpu", page_size=16, fp8_heads=[None])
 
 
+RotDims = lambda dims: SimpleNamespace(dims=dims, layout_code=0)
+
+
+@pytest.mark.gpu
 def test_wrappers_refuse_what_does_not_fit():
     batch, cache, total = U.batch_of([(5, 1)], 16)
     kv = Fp8CacheLayer(*filled(total, 2, 16, 32, 32, 0))
@@ -555,3 +559,37 @@ def test_attention_of_one_token_is_free_of_what_it_does_not_see(d, ps, base, win
         x.view(torch.uint8)[(~keep).cuda()[:, None, :, None].expand(total, G, ps, d)] = 0x7f
     out = fp8_cache_attention(q, kv, on(batch), on(cache), H, G, d, d, d ** -0.5, window=window)
     assert torch.equal(out, clean) and clean.isfinite().all() and float(clean.abs().max()) > 0
+
+
+RotDims = lambda dims: SimpleNamespace(dims=dims, layout_code=0)
+
+
+@pytest.mark.gpu
+def test_wrappers_refuse_what_does_not_fit():
+    H, G, d, ps = 4, 2, 64, 16
+    batch, cache, total = U.batch_of([(20, 3)], ps)
+    batch, cache = on(batch), on(cache)
+    kv = Fp8CacheLayer.empty(total, ps, G, d, d, "cuda")
+    proj, q = torch.zeros(3, (H + 2 * G) * d, device="cuda"), torch.zeros(3, H, d, device="cuda")
+    n, offsets = H * d, (0, H * d, (H + G) * d)
+    append = lambda rows=proj, b=batch, c=cache, layer=kv, at=offsets, kv_heads=G, **o: fp8_cache_append(rows, b, c, layer, H, kv_heads, d, d, at, **o)
+    attend = lambda rows=q, b=batch, c=cache, layer=kv, kv_heads=G, dim=d, **o: fp8_cache_attention(rows, layer, b, c, H, kv_heads, dim, d, 1.0, **o)
+    assert append().shape == (3, H, d) and attend().shape == (3, n)
+    swap = lambda x, **o: SimpleNamespace(**{**{k: getattr(x, k) for k in ("pos", "slot", "seqs", "n_seqs", "max_kv", "page_table", "page_size", "max_pages_per_seq") if hasattr(x, k)}, **o})
+    for f in (append, attend):
+        for o in (dict(kv_heads=1), dict(layer=Fp8CacheLayer.empty(total, 2 * ps, G, d, d, "cuda")), dict(layer=Fp8CacheLayer.empty(total, ps, G, 32, d, "cuda")),
+                  dict(layer=Fp8CacheLayer.empty(total, ps, G, d, d, "cpu")), dict(b=swap(batch, pos=batch.pos.long())), dict(b=swap(batch, pos=batch.pos[:2])), dict(b=swap(batch, slot=batch.slot[:1])),
+                  dict(b=swap(batch, seqs=None)), dict(b=swap(batch, seqs=batch.seqs[:1])), dict(b=swap(batch, n_seqs=batch.seqs.shape[1] + 1)), dict(b=swap(batch, pos=batch.pos.cpu())),
+                  dict(c=swap(cache, page_table=cache.page_table.long())), dict(c=swap(cache, max_pages_per_seq=cache.max_pages_per_seq + 1))):
+            with pytest.raises(ValueError, match="fp8_cache"):
+                f(**o)
+    freq = torch.ones(4, dtype=torch.float64, device="cuda")
+    for o in (dict(at=(0, n, n + 1 + G * d)), dict(at=(-1, n, n + G * d)), dict(rows=proj.half()), dict(rows=proj.t()), dict(rot=RotDims(8)), dict(rot=RotDims(8), inv_freq=freq[:3]),
+              dict(rot=RotDims(8), inv_freq=freq.float()), dict(qk_norm=3), dict(qk_norm=3, q_weight=q[0, 0], k_weight=q[0, 0, :5])):
+        with pytest.raises(ValueError, match="fp8_cache_append"):
+            append(**o)
+    row = torch.zeros(H, device="cuda")
+    for o in (dict(rows=q[:, :2]), dict(rows=q.transpose(1, 2)), dict(rows=q.half()), dict(head_scale=row[:3]), dict(head_scale=row.double()), dict(sink=row.cpu()),
+              dict(out=torch.zeros(3, n - 1, device="cuda")), dict(out=torch.zeros(3, n, device="cuda").half()), dict(out=torch.zeros(n, 3, device="cuda").t())):
+        with pytest.raises(ValueError, match="fp8_cache_attention"):
+            attend(**o)

@@ -193,3 +193,14 @@ def test_klinear_int8_through_the_linear_module():
     codes, scale = KLinearInt8.quantize(wf)
     check(lin(x.cuda()).reshape(6, 24), reference(x.reshape(6, 40), codes, scale, torch.arange(24.0)), x.reshape(6, 40), codes, scale, torch.arange(24.0))
     lin.load(mode=InferenceState.UNLOAD)
+
+
+@pytest.mark.gpu
+def test_wrapper_refuses_what_does_not_fit():
+    x, w, s = torch.zeros(2, 32, device="cuda"), torch.zeros(4, 32, dtype=torch.int8, device="cuda"), torch.ones(4, device="cuda")
+    limit = torch.ones(1, dtype=torch.int32, device="cuda")
+    assert int8_linear(x, w, s, s, limit).shape == (2, 4)
+    for call in ((x[:, :31], w, s), (x.double(), w, s), (x, w.float(), s), (x, w.t().contiguous().t(), s), (x, w[:, 1:], s), (x, w, s[:3]), (x, w, s.half()), (x, w, s.cpu()), (x, w, s, s[:3]), (x, w, s, s.half()),
+                 (x, w, s, s.cpu()), (x, w, s, None, limit.long()), (x, w, s, None, limit.cpu()), (x, w, s, None, limit[:0]), (x, torch.zeros(4, 40, dtype=torch.int8, device="cuda")[:, :32], s)):
+        with pytest.raises(ValueError, match="int8_linear"):
+            int8_linear(*call)
