@@ -134,7 +134,7 @@ int ktb200_fp8_linear_create(int in_features, int out_features, const void* weig
 void ktb200_fp8_linear_destroy(ktb200_fp8_linear* l);
 int ktb200_fp8_linear_forward(ktb200_fp8_linear* l, int qlen, const void* x, void* y, const int* bsz, void* stream);
 
-/* Linear with 8-bit integers (csrc/int8_linear.cu): y[t][n] = (sum_k c[t][k] weight[n][k]) * (s[t] weight_scale[n]) + bias[n], where s[t] = max_k |x[t][k]| / 127 in fp32 and
+/* Linear with 8-bit integers (csrc/int8_linear.cu): y[t][n] = (sum_k c[t][k] weight[n][k]) * (s[t] weight_scale[n]) + bias[n], where s[t] = max_k |x[t][k]| * (1 / 127) in fp32 and
  * c[t][k] = rint(x[t][k] / s[t]) (0 in a row of zeros); the sum is exact.  A row of x with an infinity or NaN becomes NaN.  x and y of hidden_type (F32, F16, BF16), rows x_stride /
  * y_stride elements apart; weight int8 [out_features][weight_stride], weight_stride and the address multiples of 16; bias fp32 or NULL; rows of y at or behind *bsz (NULL: none) are left
  * as they were.  workspace: ktb200_int8_linear_workspace bytes on 16, of this call alone.  The stream's device has to be the current one. */

@@ -1,5 +1,5 @@
 // Linear with 8-bit integers: a scale per token for the activations, a scale per output channel for the weights.
-//     s[t] = max_k |x[t][k]| / 127 (fp32),   c[t][k] = rint(x[t][k] / s[t])                     (IEEE quotient; 0 where the row is zero)
+//     s[t] = max_k |x[t][k]| * (1 / 127) (fp32),  c[t][k] = rint(x[t][k] / s[t])                     (IEEE quotient; 0 where the row is zero)
 //     y[t][n] = cast(float(sum_k c[t][k] w[n][k]) * (s[t] w_scale[n]) + bias[n])                 (the sum in 32-bit integers, exact)
 // A row of x with an infinity or NaN has no scale: its results are NaN.
 //
@@ -82,7 +82,7 @@ template <int TYPE, bool VEC> __global__ void __launch_bounds__(512) int8_quant_
     __syncthreads();
     top = red[0];
     for (int w = 1; w < nw; w++) top = max(top, red[w]);
-    const float s = top >= kInf ? NAN : __fdiv_rn(i8_magnitude<TYPE>(top), 127.f);
+    const float s = top >= kInf ? NAN : i8_magnitude<TYPE>(top) * (1.0f / 127.0f);      // (by the rounded inverse, as tensor arithmetic on the GPU divides by a number: the codes are the same as there)
     const bool some = s > 0.f;
     if (threadIdx.x == 0) scales[t] = s;
     int8_t* out = codes + t * Kp;

@@ -239,7 +239,7 @@ class KLinearFP8(KLinearBase):
 
 def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor, bias: torch.Tensor | None = None, bsz_tensor: torch.Tensor | None = None) -> torch.Tensor:
     """y = x W^T + bias with both sides in 8-bit integers: `weight` int8 [out, in] (rows at multiples of 16 bytes) under one fp32 `weight_scale` per output channel, the rows of x (bf16,
-    fp16 or fp32) quantised inside the call under one scale per token, max |x| / 127; exact 32-bit integer sums, scaled and rounded once (`ktb200_int8_linear`,
+    fp16 or fp32) quantised inside the call under one scale per token, max |x| * (1 / 127) in fp32; exact 32-bit integer sums, scaled and rounded once (`ktb200_int8_linear`,
     csrc/int8_linear.cu).  Rows at or behind bsz_tensor[0] are left as they come."""
     (N, K), dev, shape, hidden = weight.shape, x.device, x.shape, _INT8_HIDDEN.get(x.dtype)
     if dev.type != "cuda":

@@ -17,7 +17,7 @@ HALF_STEP = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11, torch.float32
 def codes_of(x):
     """(codes, scales) of rows, as the format defines them: the scale and the quotient are numbers of 32 bits"""
     x = x.float()
-    s = x.abs().amax(1) / 127
+    s = x.abs().amax(1) * (torch.ones(()) / 127)      # (times the rounded inverse)
     return torch.where(s[:, None] > 0, torch.round(x / s[:, None]), torch.zeros(())).clamp(-127, 127).to(torch.int64), s
 
 
