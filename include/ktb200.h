@@ -641,7 +641,8 @@ int ktb200_softmax_attn_prompt_tiles(const ktb200_softmax_attn_params* params, i
  *     call's included.  part: -1, the library cuts long key ranges among CTAs as it sees fit; 0, it does not; more (a multiple of 128), in parts of so many keys, 128 of them at most.
  *     workspace: ktb200_fp8_cache_attn_workspace bytes, of this call alone (that function reads the struct's sizes, counts and the pointers' alignment).
  * seqs: rows (first token's row, token count) of the n_seqs portions, seqs_stride apart.  A portion's tokens stand at consecutive positions from pos[first row], in the pages of table row
- * slot[first row] (a ring: page p in column p % max_pages); a sequence has one portion in a call, and windows reach back (max_pages - 1) * page_size positions at most.
+ * slot[first row] (a ring: page p in column p % max_pages); a sequence has one portion in a call, and windows reach back (max_pages - 1) * page_size positions at most;
+ * of a portion that is longer than the ring, the tokens whose pages it writes again are left out.
  * Rows of tokens in no portion are left as they were, keys in pages outside [0, n_pages) are neither written nor seen.  The stream's device has to be the current one. */
 typedef struct {
     const void* proj;

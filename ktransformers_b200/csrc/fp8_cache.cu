@@ -314,7 +314,9 @@ template <typename T, int LPR, bool HALVES> __global__ void __launch_bounds__(25
     len = __shfl_sync(0xffffffffu, len, s & 31);
     pos = __shfl_sync(0xffffffffu, pos, s & 31);
     slot = __shfl_sync(0xffffffffu, slot, s & 31);
-    const int logical = pos / ps + item, first = item ? logical * ps - pos : 0, n = min(len, (logical + 1) * ps - pos) - first;      // the portion's tokens in this page
+    const int logical = pos / ps + item;
+    if ((pos + len - 1) / ps - logical >= a.pages.max_pages) return;      // the portion itself goes once round the ring and writes the page again
+    const int first = item ? logical * ps - pos : 0, n = min(len, (logical + 1) * ps - pos) - first;      // the portion's tokens in this page
     const int t0 = start + first, p0 = pos + first, begun = p0 % ps, page = a.pages.page(slot, logical), width = is_v ? a.dv : a.d;
     const T* rows = proj + (long)t0 * a.proj_stride + (is_v ? a.v_off + (long)g * a.dv : a.k_off + (long)g * a.d);
     // A warp has groups of its rows, nw groups apart: of a.keep rows at a time the columns as they came (LPR > 0) and, of keys that were turned or normed, the results
@@ -326,6 +328,7 @@ template <typename T, int LPR, bool HALVES> __global__ void __launch_bounds__(25
     if (work) Row::weights(a, (const T*)a.k_w, place, wv);
     auto make = [&](int base) {
         const int end = min(n, base + a.keep);
+        __syncwarp();      // (of the pass before, all lanes have read the columns)
         if constexpr (LPR > 0) {
             for (int t = base + warp * Row::ROWS + sub; t < end; t += nw * Row::ROWS) Row::bring(raw + (long)(t - base) * width, rows + (long)t * a.proj_stride, place);
             asm volatile("cp.async.commit_group;\ncp.async.wait_group 0;" ::: "memory");

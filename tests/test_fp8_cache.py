@@ -593,3 +593,27 @@ def test_wrappers_refuse_what_does_not_fit():
               dict(out=torch.zeros(3, n - 1, device="cuda")), dict(out=torch.zeros(3, n, device="cuda").half()), dict(out=torch.zeros(n, 3, device="cuda").t())):
         with pytest.raises(ValueError, match="fp8_cache_attention"):
             attend(**o)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,d", [("bf16", 128), ("fp32", 64), ("bf16", 48)])
+@pytest.mark.parametrize("before,n", [(20, 100), (0, 65), (63, 300)])
+def test_append_of_a_portion_longer_than_the_ring(before, n, dtype, d):
+    """its last pages are what stays, each time"""
+    H, G, ps, columns = 4, 2, 16, 4
+    pool = filled(columns + 1, G, ps, d, d, 3)
+    proj = torch.randn((n, (H + 2 * G) * d), generator=torch.Generator().manual_seed(n)).to(DT[dtype]).cuda()
+    cache = on(SimpleNamespace(page_table=torch.tensor([[3, 0, 4, 1]], dtype=torch.int32), max_pages_per_seq=columns, page_size=ps))
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32)
+
+    def append(start):      # the portion's tokens from row `start` on
+        m = n - start
+        batch = on(SimpleNamespace(pos=torch.arange(before, before + n, dtype=torch.int32), slot=i32([0] * n), seqs=i32([[start], [m], [0], [0]]), n_seqs=1, max_kv=before + n))
+        kv = Fp8CacheLayer(*(x.cuda() for x in pool))
+        q = fp8_cache_append(proj, batch, cache, kv, H, G, d, d, (0, H * d, (H + G) * d), qk_norm=1)
+        return [q] + [x.view(torch.uint8) if x.dtype is U.E4M3 else x for x in (kv.k, kv.v, kv.scales)]
+    first = ((before + n - 1) // ps - columns + 1) * ps - before      # the row at which the last pages begin
+    assert first > 0
+    want = append(first)
+    for _ in range(5):
+        assert all(torch.equal(x, y) for x, y in zip(append(0), want))
