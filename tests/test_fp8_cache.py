@@ -617,3 +617,23 @@ def test_append_of_a_portion_longer_than_the_ring(before, n, dtype, d):
     want = append(first)
     for _ in range(5):
         assert all(torch.equal(x, y) for x, y in zip(append(0), want))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,d,lens", [("bf16", 128, [(900, 1), (70, 1)]), ("bf16", 64, [(900, 1)]), ("bf16", 128, [(300, 90)]), ("bf16", 96, [(300, 5)]), ("fp32", 128, [(300, 5)])])
+def test_both_calls_beyond_four_gigabytes(dtype, d, lens):
+    """the same blocks at the end of a pool whose offsets pass 32 bits: the same results"""
+    H, G, ps = 8, 2, 64
+    batch, cache, total = U.batch_of(lens, ps, seed=4)
+    far = (1 << 32) // (G * ps * d) + 5
+    T = batch.pos.shape[0]
+    proj = torch.randn((T, (H + 2 * G) * d), generator=torch.Generator().manual_seed(5)).to(DT[dtype]).cuda()
+    near = Fp8CacheLayer(*(x.cuda() for x in filled(total, G, ps, d, d, 15)))
+    codes = lambda x: torch.cat([torch.empty((far, G, ps, d), dtype=torch.uint8, device="cuda"), x.view(torch.uint8)]).view(U.E4M3)
+    away = Fp8CacheLayer(codes(near.k), codes(near.v), torch.cat([torch.ones((far, G, 2), device="cuda"), near.scales]))
+    there = SimpleNamespace(**{**vars(cache), "page_table": cache.page_table + far})
+    outs = []
+    for kv, c in ((near, cache), (away, there)):
+        q = fp8_cache_append(proj, on(batch), on(c), kv, H, G, d, d, (0, H * d, (H + G) * d), qk_norm=1)
+        outs.append([q, fp8_cache_attention(q, kv, on(batch), on(c), H, G, d, d, d ** -0.5)] + [x[-total:].view(torch.uint8) for x in (kv.k, kv.v)] + [kv.scales[-total:]])
+    assert all(torch.equal(x, y) for x, y in zip(*outs)) and outs[0][1].isfinite().all()
