@@ -22,7 +22,7 @@ namespace ktb {
 
 constexpr int kFpThreads = 384, kFpKeys = 128, kFpTile = 128 * 128 * 2, kFpCodes = 128 * 128, kFpKStages = 3, kFpBad = 64;
 struct FpMisc {
-    unsigned long long q_full, v8_full[2], k_full[kFpKStages], k_free[kFpKStages], v_full[2], v_free[2], s_full[2][2], p_full[2][2], pv_done[2];      // [row tile][buffer]
+    unsigned long long q_full, v8_full[2], k_full[kFpKStages], k_free[kFpKStages], v_full[2], v_free[2], s_full[2][2], p_full[2][2], pv_done[2][2];      // [row tile][buffer]
     float2 scales[4][2];      // of a tile's two runs of 64 keys (zeros: not there)
     uint32_t tmem_base;
     int info[4], n_bad, bad_lo, bad_hi;
@@ -45,8 +45,7 @@ __global__ void __launch_bounds__(kFpThreads, 1) fp8_attn_prompt_kernel(const __
         for (int i = 0; i < kFpKStages; i++) { bar_init(smem_u32(&misc.k_full[i]), 1); bar_init(smem_u32(&misc.k_free[i]), 1); }
         for (int i = 0; i < 2; i++) {
             bar_init(smem_u32(&misc.v8_full[i]), 1); bar_init(smem_u32(&misc.v_full[i]), 3); bar_init(smem_u32(&misc.v_free[i]), 1);
-            bar_init(smem_u32(&misc.pv_done[i]), 1);
-            for (int b = 0; b < 2; b++) { bar_init(smem_u32(&misc.s_full[i][b]), 1); bar_init(smem_u32(&misc.p_full[i][b]), 4); }
+            for (int b = 0; b < 2; b++) { bar_init(smem_u32(&misc.s_full[i][b]), 1); bar_init(smem_u32(&misc.p_full[i][b]), 4); bar_init(smem_u32(&misc.pv_done[i][b]), 1); }
         }
         bar_fence_init();
         misc.n_bad = 0;
@@ -106,7 +105,7 @@ __global__ void __launch_bounds__(kFpThreads, 1) fp8_attn_prompt_kernel(const __
 #pragma unroll
                     for (int k = 0; k < 4; k++)
                         mma_f16_ta(tmem + t * 256 + 128, tmem + t * 256 + buf * 64 + 8 * k, smem_desc(vb + k * 2048, kFpTile / 2, 1024, kLayoutSw128), idesc_pv, (i | k) != 0);
-                    mma_commit(smem_u32(&misc.pv_done[t]));
+                    mma_commit(smem_u32(&misc.pv_done[t][buf]));
                     if (t == 1 && buf == 1) mma_commit(smem_u32(&misc.v_free[st]));
                     if (j + 1 < n) scores(t, i);      // (of 128 keys on)
                 }
@@ -303,7 +302,7 @@ __global__ void __launch_bounds__(kFpThreads, 1) fp8_attn_prompt_kernel(const __
                 const float alpha = raise ? exp2_approx(m_ref - m_new) : 1.f;      // (2^-inf = 0: nothing was summed yet)
                 if (raise) { m_ref = m_new; l *= alpha; }
                 if (i64 > 0) {
-                    bar_wait(smem_u32(&misc.pv_done[t]), (i64 - 1) & 1);
+                    bar_wait(smem_u32(&misc.pv_done[t][buf ^ 1]), ((i64 - 1) >> 1) & 1);
                     tc_fence_after();
 #pragma unroll 1
                     for (int q = 0; q < 4; q++) {
@@ -339,9 +338,10 @@ __global__ void __launch_bounds__(kFpThreads, 1) fp8_attn_prompt_kernel(const __
             unpack2(sum[1], a2, a3);
             l = fmaf((a0 + a1) + (a2 + a3), inv, l);
         }
-        // the last two of an even number of products (the scores that the loop waited for last were behind all others)
-        bar_wait(smem_u32(&misc.pv_done[t]), 0);
-        bar_wait(smem_u32(&misc.pv_done[t]), 1);
+        // the last product of each buffer: its n-th.  (The (n - 1)-th of both are complete, the scores that the loop waited for last are behind them; a barrier for both buffers would stand
+        // one phase or two behind what is known, and a wait for a phase that is two back never ends)
+        bar_wait(smem_u32(&misc.pv_done[t][0]), (n - 1) & 1);
+        bar_wait(smem_u32(&misc.pv_done[t][1]), (n - 1) & 1);
         tc_fence_after();
         const long row = (long)(tok0 + tok) * a.H + h;
         float* part = cut ? a.partial + (row * a.parts + blockIdx.z) * 130 : nullptr;
