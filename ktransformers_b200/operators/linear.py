@@ -278,8 +278,9 @@ _INT8_HIDDEN = {torch.float32: native.GGML_F32, torch.float16: native.GGML_F16, 
 
 class KLinearInt8(KLinearBase):
     """8-bit integer linear (`int8_linear`): symmetric int8 weights with one scale per output channel, activations quantised per token inside the call.  Contract of KLinearFP8:
-    `load(w=(weight int8 [out][in], weight_scale [out] or [out, 1][, bias]))`, a float weight [out][in] (quantised here, row by row, to max |w| / 127), or from a
-    SafeTensorLoader (`<key>.weight` + `<key>.weight_scale`); `forward(x, bsz_tensor)`.  (The reference's linear operators: archive/ktransformers/operators/linear.py.)"""
+    `load(w=(weight int8 [out][in], weight_scale [out] or [out, 1][, bias]))`, a float weight [out][in] of 16 bits or more or (weight, bias [out]) (quantised here, row by row, to
+    max |w| / 127), or from a SafeTensorLoader (`<key>.weight` in int8 + `<key>.weight_scale`, or a float `<key>.weight` alone, and `<key>.bias` where there is one; other weights, and float
+    ones that come with scales, are refused); `forward(x, bsz_tensor)`.  (The reference's linear operators: archive/ktransformers/operators/linear.py.)"""
 
     def __init__(self, key, gguf_loader, config, orig_module=None, device: str = "cuda", **kwargs):
         super().__init__(key, gguf_loader, config, orig_module, device, **kwargs)
@@ -292,6 +293,16 @@ class KLinearInt8(KLinearBase):
         scale = w.abs().amax(1) / 127
         return torch.round(w / torch.where(scale > 0, scale, torch.ones_like(scale))[:, None]).clamp(-127, 127).to(torch.int8), scale
 
+    def _from_safetensors(self, ld):
+        weight = ld.load_tensor(self.key + ".weight")
+        bias = (ld.load_tensor(self.key + ".bias"),) if ld.has_tensor(self.key + ".bias") else ()
+        if weight.dtype == torch.int8:
+            return (weight, ld.load_tensor(self.key + ".weight_scale")) + bias
+        scales = [name for name in (".weight_scale", ".weight_scale_inv") if ld.has_tensor(self.key + name)]
+        if scales:      # (what such a weight stands for is another format's to say)
+            raise ValueError(f"KLinearInt8: {self.key}{scales[0]} belongs to an int8 weight, {self.key}.weight is {weight.dtype}")
+        return (weight,) + bias
+
     def load(self, w=None, device: str | None = None):
         if self.loaded:
             return
@@ -299,15 +310,17 @@ class KLinearInt8(KLinearBase):
         assert "cuda" in str(device).lower(), "KLinearInt8 can only be loaded on a CUDA device"
         if w is None:
             ld = self.gguf_loader
-            if hasattr(ld, "load_tensor"):
-                w = (ld.load_tensor(self.key + ".weight"), ld.load_tensor(self.key + ".weight_scale")) + ((ld.load_tensor(self.key + ".bias"),) if ld.has_tensor(self.key + ".bias") else ())
-            else:
-                w = self.load_weight(device=device)
+            w = self._from_safetensors(ld) if hasattr(ld, "load_tensor") else self.load_weight(device=device)
         w = tuple(t.data if isinstance(t, nn.Parameter) else t for t in (w if isinstance(w, tuple) else (w,)))
-        if w[0].dtype != torch.int8:      # a float weight[, its bias]
-            w = KLinearInt8.quantize(w[0].to(device).view(self.out_features, self.in_features)) + w[1:]
-        if len(w) not in (2, 3) or tuple(w[0].shape) != (self.out_features, self.in_features) or w[1].numel() != self.out_features or (len(w) == 3 and w[2].numel() != self.out_features):
-            raise ValueError(f"KLinearInt8: weight int8 [{self.out_features}][{self.in_features}], one scale per row and, where there is one, a bias; got {[tuple(t.shape) for t in w]}")
+        n, shapes = self.out_features, [tuple(t.shape) for t in w]
+        if w[0].is_floating_point() and w[0].element_size() > 1:      # a float weight[, its bias]
+            if len(w) > 2 or shapes[0] not in ((n, self.in_features), (n * self.in_features,)) or shapes[1:] not in ([], [(n,)]):
+                raise ValueError(f"KLinearInt8: a float weight [{n}][{self.in_features}] and, where there is one, a bias [{n}]; got {shapes}")
+            w = KLinearInt8.quantize(w[0].to(device).view(n, self.in_features)) + w[1:]
+        elif w[0].dtype != torch.int8:
+            raise ValueError(f"KLinearInt8: weights of int8 with a scale per row, or floats of 16 bits or more; got {w[0].dtype}")
+        elif len(w) not in (2, 3) or shapes[0] != (n, self.in_features) or w[1].numel() != n or (len(w) == 3 and w[2].numel() != n):
+            raise ValueError(f"KLinearInt8: weight int8 [{n}][{self.in_features}], one scale per row and, where there is one, a bias; got {shapes}")
         pad = -self.in_features % 16      # rows begin at multiples of 16 bytes
         self.weight = torch.nn.functional.pad(w[0].to(device), (0, pad))[:, :self.in_features] if pad else w[0].to(device).contiguous()
         self.weight_scale = w[1].to(device=device, dtype=torch.float32).reshape(-1).contiguous()
