@@ -7,7 +7,7 @@
 // any order (so that splits of K join without rounding):
 //   int8_rows_kernel   weight rows on the MMA's 128 rows, 16 to 128 tokens on its columns: a decode step reads the weights once.  K is split over the CTAs of a cluster, which add their
 //                      parts through distributed shared memory: no workspace to clear, no second launch.  Weight boxes are under way before the codes are there (the launch is
-//                      a programmatic dependent of the quantiser's).
+//                      a programmatic dependent of the quantiser's, which lets it start once all work ahead of the call is complete).
 //   int8_gemm_kernel   prompts: 256 tokens x up to 256 outputs a tile of two CTAs, persistent, two accumulators in tensor memory
 #include <cuda.h>
 
@@ -53,8 +53,8 @@ template <int TYPE, bool VEC> __global__ void __launch_bounds__(512) int8_quant_
     __shared__ uint32_t red[16];
     const long t = blockIdx.x;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
-    griddep_launch_dependents();
     griddep_wait();
+    griddep_launch_dependents();      // (behind the wait: the rows kernel asks for weights as soon as it starts, and what is ahead of this kernel in the stream may have made them)
     uint32_t top = 0;      // 16-bit types: of the even and of the odd values
     uint4 keep[VEC ? kI8Keep : 1];
     const uint8_t* row = reinterpret_cast<const uint8_t*>(x) + t * x_stride * ESZ;
@@ -175,7 +175,7 @@ template <int NT> __global__ void __launch_bounds__(kI8RowsThreads, 2) int8_rows
     const uint32_t tmem = uniform(misc.tmem_base);
     if (warp == 0) {
         if (lane == 0) {
-            // the ring's first weights do not wait for the codes
+            // the ring's first weights do not wait for the codes (what was ahead of the quantiser is complete: it lets this kernel start behind its own wait)
             for (int i = 0; i < nk && i < STAGES; i++) {
                 const uint32_t bar = smem_u32(&misc.full[i]);
                 bar_expect_tx(bar, STAGE);

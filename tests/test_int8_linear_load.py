@@ -4,7 +4,7 @@ from types import SimpleNamespace
 import pytest
 import torch
 
-from ktransformers_b200.operators.linear import KLinearInt8, KTransformersLinear
+from ktransformers_b200.operators.linear import KLinearInt8, KTransformersLinear, int8_linear
 from ktransformers_b200.util.custom_loader import SafeTensorLoader
 from ktransformers_b200.util.utils import InferenceState
 
@@ -76,3 +76,23 @@ def test_a_checkpoint_stands_for_its_weights(tmp_path, kind, bias):
     x_half = xd.abs().amax(1, keepdim=True) / 254
     bound = 1.01 * (xd.abs().sum(1, keepdim=True) * half + x_half * (w.abs().sum(1) + K * half)) + 2.0 ** -20 * (ref.abs() + 1)
     assert ((y - ref).abs() <= bound).all() and lin.generate_linear.has_bias == bias
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,T", [(64, 1), (2000, 5), (7168, 20), (2000, 200)])
+def test_weights_made_on_the_stream_just_ahead(rows, T):
+    """The int8 weight is the bytes of another integer linear's result, whose kernel lets its dependents start before it is done; then bytes that are copied over them"""
+    g = torch.Generator().manual_seed(rows)
+    rn = lambda *shape: torch.randn(shape, generator=g).cuda()
+    many, scale, x = [rn(rows, 512) for _ in range(4)], torch.ones(rows, device="cuda"), rn(T, 1024).bfloat16()
+    w1, s1 = KLinearInt8.quantize(rn(512, 512))
+    made = [int8_linear(m.bfloat16(), w1, s1).view(torch.int8) for m in many]      # [rows, 1024]: bytes of bf16 numbers
+    torch.cuda.synchronize()
+    want = [int8_linear(x, w, scale) for w in made]
+    torch.cuda.synchronize()
+    got = [int8_linear(x, int8_linear(m.bfloat16(), w1, s1).view(torch.int8), scale) for m in many]
+    weight, copied = torch.empty_like(made[0]), []
+    for w in made:
+        weight.copy_(w)
+        copied.append(int8_linear(x, weight, scale))
+    assert all(torch.equal(a, b) for a, b in zip(got + copied, want + want)) and not torch.equal(want[0], want[1])
