@@ -3,10 +3,12 @@
 // A CTA has one token, one key/value head and its query heads, and a part of the key range in tiles of 128 keys.  The codes are operands as they lie in the cache: nothing is converted.
 //     S^T = K Q^T     128 keys x N, kind::f8f6f4, K the K-major A operand as TMA delivered it
 //     O^T = V^T P^T   128 columns x N, the V tile as an MN-major A operand
-// N = 2 RP columns for RP = 8 or 16 heads: what stands against the codes is split into two e4m3 numbers, the second for 16 times what the first leaves.
+// N = 2 RP columns of S^T, NO = 4 RP of O^T, for RP = 8 or 16 heads: what stands against the codes is split into two e4m3 numbers, the second for 16 times what the first leaves.
 //   queries   a row moved by a power of two so that its largest stands in [128, 256): exact for bf16 numbers down to 2^-13 of that largest, 2^-21 of it off below
-//   weights   p = 2^(t - m), t = s log2(e) + log2(value scale): 2^-8 of a weight off at most (as a bf16 weight is) and 2^-21 of the largest where that is more.  Value scales are
-//             powers of two: in the exponent they cost nothing and O needs none.  m is 7 below a head's largest t, raised when a t outgrows it by 8.75 (2^8.75 < 448)
+//   weights   p = 2^(t - m), t = s log2(e) + log2(value scale).  Value scales are powers of two: in the exponent they cost nothing and O needs none.  m is 7 below a head's largest t,
+//             raised when a t outgrows it by 8.75 (2^8.75 < 448).  The two numbers are within 2^-8 of a weight from 2^-6 on (as a bf16 weight is).  A long context behind one key that has
+//             most of the weight lies below that, so a smaller weight stands in two more columns, 2^14 times itself: within 2^-8 of it down to 2^-20, and 2^-28 off below, 2^-35 of the
+//             largest.  They are zeros, and not written, as long as a warp has no such weight (64 contexts of 4095 to 8190 keys: 148 us without any, 152 with some in every tile)
 // l += p / (value scale), O / l is the result: 2^m drops out.
 // Heads of 64 (PAIR = 2): a row of 128 bytes is two neighbouring keys.  Queries and weights then have rows of their own for the first and for the second of a pair, zero where the other's
 // columns are; of the products, twice as many as needed, the mixed ones are not looked at.  What bounds is the bytes all the same: 30 tokens over 2000 to 4000 keys, 64 heads over 8, take
@@ -17,7 +19,7 @@
 //                 reference, which one barrier with a reduction tells.  At the end a thread owns a column of the result
 // A range that is cut for up to eight CTAs is cut evenly, sequence by sequence, and its CTAs are a cluster: each leaves its sums in its shared memory and joins some of the heads from
 // all of them, so that there is neither a workspace nor a second launch.  Longer ranges of few sequences go in parts of one length, joined by fp8_merge_kernel.
-// TMEM: [S | S | O], N columns each.  Bound by the cache's bytes: a tile is 32 KB, 740 ns of an SM's share of the memory; three CTAs an SM (two for 16 heads), so that what a CTA
+// TMEM: [S | S | O], N, N and NO columns.  Bound by the cache's bytes: a tile is 32 KB, 740 ns of an SM's share of the memory; three CTAs an SM (two for 16 heads), so that what a CTA
 // spends ahead of its first tile and between a tile's steps is another's time.
 #pragma once
 #include <cuda.h>
@@ -28,13 +30,16 @@ namespace ktb {
 
 constexpr int kFdThreads = 192, kFdRows = 128, kFdTile = kFdRows * 128, kFdStages = 2;
 constexpr float kFdTop = 7.f, kFdRaise = 8.75f;
-struct FdMisc {
+constexpr float kFdSmall = 0.015625f, kFdLift = 16384.f, kFdNone = 3.7252903e-9f;      // weights below 2^-6 stand as 2^14 times themselves; 2^-28: and what becomes zero there
+template <int RP> struct FdMisc {
     unsigned long long k_full[kFdStages], k_free[kFdStages], v_full[kFdStages], v_free[kFdStages], s_full[2], s_free[2], p_full[2], p_free[2], q_ready;
-    float red[4][16], fac[16];
+    float red[4][RP], fac[RP];
     uint32_t tmem_base;
     int found;
 };
-template <int RP, int PAIR> constexpr int fd_smem() { return 2 * kFdStages * kFdTile + 3 * 2 * RP * PAIR * 128 + (int)sizeof(FdMisc) + 1024; }
+// the ring, the queries (2 RP rows, twice for pairs), two buffers of weights (4 RP rows)
+template <int RP, int PAIR> constexpr int fd_smem() { return 2 * kFdStages * kFdTile + (2 + 2 * 4) * RP * PAIR * 128 + (int)sizeof(FdMisc<RP>); }
+static_assert(3 * (fd_smem<8, 1>() + 1024) <= 228 * 1024, "three CTAs an SM");
 
 struct FdMaps { CUtensorMap k, v; };
 constexpr int kFdCluster = 8;
@@ -59,12 +64,12 @@ __device__ __forceinline__ void fd_sync() { asm volatile("barrier.cta.sync 1, 12
 
 template <int RP, int PAIR> __global__ void __launch_bounds__(kFdThreads, RP * PAIR == 8 ? 3 : 2) fp8_attn_decode_kernel(const __grid_constant__ FdMaps maps, const Fp8Attn a, int RH, int run) {
     using namespace umma;
-    constexpr int N = 2 * RP * PAIR, OP = N * 128, D = 128 / PAIR, KEYS = kFdRows * PAIR;      // OP: bytes of an operand of N rows
-    extern __shared__ __align__(16) uint8_t fd_smem_raw[];
-    const uint32_t raw = smem_u32(fd_smem_raw), base = (raw + 1023u) & ~1023u;
+    constexpr int N = 2 * RP * PAIR, NO = 2 * N, QP = N * 128, OP = NO * 128, D = 128 / PAIR, KEYS = kFdRows * PAIR;      // QP, OP: bytes of the queries and of a buffer of weights
+    extern __shared__ __align__(1024) uint8_t fd_smem_raw[];
+    const uint32_t raw = smem_u32(fd_smem_raw), base = (raw + 1023u) & ~1023u;      // (the same number; with raw itself, whose value is known, a call over 1500 keys took 9.6 us, and takes 9.1)
     uint8_t* smem = fd_smem_raw + (base - raw);
-    const uint32_t kbase = base, vbase = base + kFdStages * kFdTile, qbase = base + 2 * kFdStages * kFdTile, pbase = qbase + OP;
-    FdMisc& misc = *reinterpret_cast<FdMisc*>(smem + 2 * kFdStages * kFdTile + 3 * OP);
+    const uint32_t kbase = base, vbase = base + kFdStages * kFdTile, qbase = base + 2 * kFdStages * kFdTile, pbase = qbase + QP;
+    FdMisc<RP>& misc = *reinterpret_cast<FdMisc<RP>*>(smem + 2 * kFdStages * kFdTile + QP + 2 * OP);
     const int tid = threadIdx.x, lane = tid & 31, warp = uniform(tid >> 5), ps = a.pages.page_size;
     griddep_launch_dependents();
     if (tid == 0) {
@@ -156,7 +161,7 @@ template <int RP, int PAIR> __global__ void __launch_bounds__(kFdThreads, RP * P
         __syncwarp();
     } else if (warp == 1) {
         // ================================================================ products (converged warp)
-        constexpr uint32_t idesc_s = instr_desc(1, 0, 0, 0, 0, 128, N), idesc_o = instr_desc(1, 0, 0, 1, 0, 128, N);
+        constexpr uint32_t idesc_s = instr_desc(1, 0, 0, 0, 0, 128, N), idesc_o = instr_desc(1, 0, 0, 1, 0, 128, NO);
         bar_wait(smem_u32(&misc.q_ready), 0);
         for (int j = 0; j <= tiles; j++) {
             if (j < tiles) {
@@ -220,10 +225,12 @@ template <int RP, int PAIR> __global__ void __launch_bounds__(kFdThreads, RP * P
                 }
                 if (lane == 0) misc.fac[h] = h < RH ? (a.head_scale ? a.scale * a.head_scale[h0 + h] : a.scale) / by * (a.softcap > 0.f ? 1.f : kLog2e) + odd : 0.f;
             }
+            for (int i = tid - 64; i < 2 * PAIR * 2 * RP * 8; i += 128)      // no small weights: rows 2 RP .. 4 RP - 1 (of either key of pairs)
+                *reinterpret_cast<uint4*>(smem + (pbase - base) + (2 * (i / (16 * RP)) + 1) * 2 * RP * 128 + i % (16 * RP) * 16) = make_uint4(0, 0, 0, 0);
             fence_async_smem();
             __syncwarp();
             if (lane == 0) bar_arrive(smem_u32(&misc.q_ready));
-            fd_sync();      // (the factors)
+            fd_sync();      // (the factors and the zeros)
         }
         float fac[RP], m[RP], l[RP];
 #pragma unroll
@@ -234,6 +241,7 @@ template <int RP, int PAIR> __global__ void __launch_bounds__(kFdThreads, RP * P
         auto scales_of = [&](int page) { return page < 0 ? make_float2(0.f, 0.f) : *reinterpret_cast<const float2*>(a.scales + 2 * ((long)page * a.G + g)); };
         float2 sc = scales_of(look(0));
         int page1 = look(1);
+        uint32_t lifted = 0;      // the buffers whose columns of small weights this warp has written
         for (int j = 0; j < tiles; j++) {
             const int buf = j & 1;
             const float2 next = scales_of(page1);
@@ -286,30 +294,48 @@ template <int RP, int PAIR> __global__ void __launch_bounds__(kFdThreads, RP * P
                 if (j > 0) {
                     bar_wait(smem_u32(&misc.p_free[buf ^ 1]), ((j - 1) >> 1) & 1);      // PV of the tile before this one is complete
                     tc_fence_after();
-                    uint32_t o[N];
-                    if constexpr (N == 16) tmem_ld16(tmem_o + lanes, o); else tmem_ld32(tmem_o + lanes, o);
-                    tmem_wait_ld();
+#pragma unroll 1
+                    for (int c = 0; c < NO; c += 32) {
+                        uint32_t o[32];
+                        tmem_ld32(tmem_o + lanes + c, o);
+                        tmem_wait_ld();
 #pragma unroll
-                    for (int i = 0; i < N; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * k[i % RP]);
-                    if constexpr (N == 16) tmem_st16(tmem_o + lanes, o); else tmem_st32(tmem_o + lanes, o);
+                        for (int i = 0; i < 32; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * k[i % RP]);
+                        tmem_st32(tmem_o + lanes + c, o);
+                    }
                     tmem_wait_st();
                     tc_fence_before();
                 }
             }
             if (j > 1) bar_wait(smem_u32(&misc.p_free[buf]), ((j - 2) >> 1) & 1);
-            uint8_t* P = smem + (pbase - base) + buf * OP;
+            bool small = false;
 #pragma unroll
-            for (int i = 0; i < PAIR * RP; i += 2) {
-                const int h = i % RP, n = i / RP * 2 * RP + h;
-                const float u0 = m[h] == -INFINITY ? 0.f : m[h], u1 = m[h + 1] == -INFINITY ? 0.f : m[h + 1];
-                const float p0 = exp2_approx(x[i] - u0), p1 = exp2_approx(x[i + 1] - u1);
-                l[h] = fmaf(p0, inv, l[h]);
-                l[h + 1] = fmaf(p1, inv, l[h + 1]);
-                const uint2 c = split_e4m3(p0, p1);
+            for (int i = 0; i < PAIR * RP; i++) {
+                const int h = i % RP;
+                x[i] = exp2_approx(x[i] - (m[h] == -INFINITY ? 0.f : m[h]));
+                l[h] = fmaf(x[i], inv, l[h]);
+                small |= x[i] < kFdSmall && x[i] > kFdNone;
+            }
+            uint8_t* P = smem + (pbase - base) + buf * OP;
+            auto put = [&](int n, uint2 c) {      // rows n, n + 1 of both terms
                 P[fd_at(n, r)] = (uint8_t)c.x;
                 P[fd_at(n + 1, r)] = (uint8_t)(c.x >> 8);
                 P[fd_at(n + RP, r)] = (uint8_t)c.y;
                 P[fd_at(n + RP + 1, r)] = (uint8_t)(c.y >> 8);
+            };
+            small = __any_sync(0xffffffffu, small);
+            if (small || (lifted >> buf & 1)) {
+#pragma unroll
+                for (int i = 0; i < PAIR * RP; i += 2) {
+                    const int n = i / RP * 4 * RP + i % RP;
+                    const bool s0 = x[i] < kFdSmall, s1 = x[i + 1] < kFdSmall;
+                    put(n, split_e4m3(s0 ? 0.f : x[i], s1 ? 0.f : x[i + 1]));
+                    put(n + 2 * RP, split_e4m3(s0 ? x[i] * kFdLift : 0.f, s1 ? x[i + 1] * kFdLift : 0.f));
+                }
+                lifted ^= ((lifted >> buf & 1) ^ (uint32_t)small) << buf;
+            } else {
+#pragma unroll
+                for (int i = 0; i < PAIR * RP; i += 2) put(i / RP * 4 * RP + i % RP, split_e4m3(x[i], x[i + 1]));
             }
             const int k0 = k_lo + j * KEYS;
             if (k0 < lo || k0 + KEYS > k_hi) {      // the first and last tiles: values of keys that are not seen may be anything (0 x NaN)
@@ -337,19 +363,25 @@ template <int RP, int PAIR> __global__ void __launch_bounds__(kFdThreads, RP * P
         }
         bar_wait(smem_u32(&misc.p_free[(tiles - 1) & 1]), ((tiles - 1) >> 1) & 1);
         tc_fence_after();
-        uint32_t o[N];
-        if constexpr (N == 16) tmem_ld16(tmem_o + lanes, o); else tmem_ld32(tmem_o + lanes, o);
-        tmem_wait_ld();
         float v[RP];      // of column r; heads of 64: what the first keys of pairs give it, and from thread r + 64 what the second ones do
-        if constexpr (PAIR == 1) {
 #pragma unroll
-            for (int h = 0; h < RP; h++) v[h] = fmaf(__uint_as_float(o[RP + h]), 0.0625f, __uint_as_float(o[h]));
-        } else {
+        for (int h = 0; h < RP; h++) v[h] = 0.f;
+#pragma unroll
+        for (int c = 4 * RP - 32; c >= 0; c -= 32) {      // small weights first
+            uint32_t o[32];
+            tmem_ld32(tmem_o + lanes + (PAIR == 2 && sp >= 2 ? 4 * RP : 0) + c, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 31; i >= 0; i--) {
+                const int term = (c + i) / RP;
+                v[i % RP] = fmaf(__uint_as_float(o[i]), (term & 1 ? 0.0625f : 1.f) * (term & 2 ? 1.f / kFdLift : 1.f), v[i % RP]);
+            }
+        }
+        if constexpr (PAIR == 2) {
             float* other = join + 2 * RP + 128 * RP;
+            if (r >= 64) {
 #pragma unroll
-            for (int h = 0; h < RP; h++) {
-                v[h] = r < 64 ? fmaf(__uint_as_float(o[RP + h]), 0.0625f, __uint_as_float(o[h])) : fmaf(__uint_as_float(o[N - RP + h]), 0.0625f, __uint_as_float(o[N - 2 * RP + h]));
-                if (r >= 64) other[64 * h + r - 64] = v[h];
+                for (int h = 0; h < RP; h++) other[64 * h + r - 64] = v[h];
             }
             fd_sync();
             if (r < 64) {

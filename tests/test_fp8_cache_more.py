@@ -42,3 +42,66 @@ def test_prompt_attention_never_waits_for_a_phase_that_has_gone(lens, H, G):
         torch.cuda.synchronize()
         assert begin.elapsed_time(end) < 15.0
         assert all(torch.equal(first, o) for o in outs)
+
+
+def run_dominant(lens, ps, H, G, d, dtype, gap, at, equal, wide=0, weight=2.0 ** -8, floor=2.0 ** -35, seed=0):
+    """One key with most of every row's weight and a value of zero: what is left is the sum of all the others' small weights, compared with 64 bits relative to that sum.
+    at: the key, a share of the first token's range.  gap: by how many nats its score is above the others' mean, about.  equal: the others have one score.  wide: 2^wide is the value
+    scale of its page, beside one for the others.  weight, floor: how far a weight may be off, of itself, and of the row's largest"""
+    g = torch.Generator().manual_seed(seed)
+    batch, cache, total = U.batch_of(lens, ps, seed=seed)
+    T, dt, scale = batch.pos.shape[0], {"bf16": torch.bfloat16, "fp32": torch.float32}[dtype], d ** -0.5
+    q = torch.randn((T, H, d), generator=g).to(dt)
+    codes = lambda x: x.clamp(-448, 448).to(U.E4M3)
+    k = codes(torch.zeros((total, G, ps, d)) if equal else 16 * torch.randn((total, G, ps, d), generator=g))
+    v = codes(16 + 4 * torch.randn((total, G, ps, d), generator=g))
+    s = torch.full((total, G, 2), 2.0 ** -4)
+    for i, (b, n) in enumerate(lens):
+        key, rows = int(at * b), q[int(batch.seqs[0, i]):int(batch.seqs[0, i]) + n].double().reshape(n, G, H // G, d)
+        page = int(cache.page_table[i, key // ps])
+        # along the first token's queries of the group: each head's score is about its own |q|^2 of it
+        k[page, :, key % ps] = codes((16 * gap / d ** 0.5 * rows[0].sum(1)).float())
+        v[page, :, key % ps] = codes(torch.zeros(G, d))
+        s[page, :, 1] *= 2.0 ** wide
+    kv = Fp8CacheLayer(k.cuda(), v.cuda(), s.cuda())
+    out = fp8_cache_attention(q.cuda(), kv, on(batch), on(cache), H, G, d, d, scale).cpu().double().reshape(T, H, d)
+    half, worst, seen = {"bf16": 2.0 ** -8, "fp32": 2.0 ** -24}[dtype], 0.0, []
+    for i, (b, n) in enumerate(lens):
+        j = torch.arange(b + n)
+        page = cache.page_table[i].long()[j // ps]
+        for h in range(G):
+            K, V = (x[page, h, j % ps].double() * s[page, h, c, None].double() for c, x in ((0, k), (1, v)))
+            for t in range(n):
+                at_t, rows = b + t + 1, q[int(batch.seqs[0, i]) + t].double().reshape(G, H // G, d)[h]
+                z = rows @ K[:at_t].T * scale
+                w = torch.softmax(z, 1)
+                ref, spread = w @ V[:at_t], w @ V[:at_t].abs()
+                # scores are fp32 sums of d products of queries that are 2^-21 of a row's largest off at most; an error e of them makes weights 2 e off
+                e = float(rows.norm(dim=1).max() * K[:at_t].norm(dim=1).max() * scale) * (2 * d + 8) * 2.0 ** -24 + float(rows.abs().max() * K[:at_t].abs().sum(1).max()) * scale * 2.0 ** -21 + 2.0 ** -20
+                bound = half * ref.abs() * 1.02 + (weight + 2 * e) * spread * 1.02 + floor * w.amax(1, keepdim=True) * 2.0 ** max(0, wide) * V[:at_t].abs().sum(0)
+                got = out[int(batch.seqs[0, i]) + t].reshape(G, H // G, d)[h]
+                worst = max(worst, float(((got - ref).abs() / bound).max()))
+                seen.append(float(w.amax(1).max()))
+    assert max(seen) > 0.9      # (the key does have most of the weight)
+    assert worst <= 1, worst
+
+
+DOMINANT = [
+    ([(15999, 1)], 64, 16, 2, 128, 12), ([(60000, 1)], 64, 4, 1, 128, 14), ([(15999, 1)], 16, 4, 1, 64, 12), ([(59999, 1)], 64, 4, 1, 64, 14), ([(8000, 1)], 32, 16, 1, 128, 14),
+    ([(700, 1), (90, 1), (64, 1)], 64, 8, 1, 128, 8), ([(700, 1), (90, 1), (64, 1)], 16, 8, 1, 64, 8), ([(2000, 1)] * 3, 64, 16, 1, 128, 18),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("equal", [False, True])
+@pytest.mark.parametrize("at", [0.0, 0.5, 1.0])
+@pytest.mark.parametrize("lens,ps,H,G,d,gap", DOMINANT)
+def test_single_tokens_keep_the_weights_beside_a_dominant_key(lens, ps, H, G, d, gap, at, equal):
+    run_dominant(lens, ps, H, G, d, "bf16", gap, at, equal)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d", [64, 128])
+def test_single_tokens_keep_the_weights_beside_a_dominant_key_of_a_page_of_large_values(d):
+    run_dominant([(15999, 1)], 64, 4, 1, d, "bf16", 14, 0.0, True, wide=5)
+    run_dominant([(500, 1), (2000, 1)], 64, 4, 1, d, "bf16", 8, 1.0, False, wide=5)
