@@ -6,7 +6,8 @@
 // that its largest stands below 2^15 (exact for what is within 2^-28 of that), and weights rounded to fp16 (2^-11 of a weight).  (m16n8k32 e4m3 products took more instructions: they
 // count as two fp16 ones each, with the conversions of both operands.)
 // Key scales multiply scores.  A block's value scale is a power of two in the weight's exponent, so that O needs no scale and the weights of all blocks stand in
-// one range: m is raised only when a row's t outgrows it by 8, p <= 2^8.  O / l is the result: 2^m drops out.
+// one range: m is 7 below a row's largest t and raised only when a t outgrows it by 15, p <= 2^15.  (With m at that largest the weights beside one key that has most of the weight stood
+// among fp16's subnormal numbers: so they are 2^-11 of themselves off down to 2^-21 of the largest, and 2^-32 of that below.)  O / l is the result: 2^m drops out.
 //
 // The order of a product's sum is free, and taken so that no shuffling is needed: of a key's row, the four threads that share it hold 16 neighbouring bytes each (an S
 // step takes 4 of them), and of a value's row each of the eight column groups has its neighbouring bytes, an output tile's columns being dv / 8 apart.
@@ -20,6 +21,7 @@
 namespace ktb {
 
 constexpr int kFmThreads = 128, kFmWarps = 4, kFmKeys = 16;
+constexpr float kFmTop = 7.f, kFmRaise = 15.f;      // a row's largest weight stands between 2^7 and 2^15 (fp16 holds 2^16 - 2^5)
 
 __device__ __forceinline__ void mma_f16_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -260,15 +262,15 @@ template <int DP, int DVP, bool SHARED, bool TWO> __global__ void __launch_bound
                 top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
                 top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
                 const float m = h ? mB : mA;
-                raise[h] = top[h] > m + 8.f || (m == -INFINITY && top[h] > -INFINITY);
+                raise[h] = top[h] > m + kFmRaise || (m == -INFINITY && top[h] > -INFINITY);
                 any |= raise[h];
             }
             if (__any_sync(0xffffffffu, any)) {
 #pragma unroll
                 for (int h = 0; h < ROWS; h++) {
                     float &m = h ? mB : mA, &l = h ? lB : lA;
-                    const float k = raise[h] ? exp2_approx(m - top[h]) : 1.f;      // (2^-inf = 0: nothing was summed yet)
-                    if (raise[h]) m = top[h];
+                    const float k = raise[h] ? exp2_approx(m - (top[h] - kFmTop)) : 1.f;      // (2^-inf = 0: nothing was summed yet)
+                    if (raise[h]) m = top[h] - kFmTop;
                     l *= k;
 #pragma unroll
                     for (int n = 0; n < NT; n++) { O[n][2 * h] *= k; O[n][2 * h + 1] *= k; }

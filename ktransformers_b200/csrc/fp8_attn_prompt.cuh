@@ -9,8 +9,8 @@
 //     warps 4-7       soft-max of the first tile, 8-11 of the second: a thread owns a row.  First it makes its row of Q: moved by a power of two so that its largest stands in [128, 256) and
 //                     split into two e4m3 numbers, q = q1 + q2, whose products add up in one sum: exact for bf16 numbers down to 2^-9 of the largest, 2^-17 of it off below.
 //                     t = s log2(e) + log2(value scale), p = 2^(t - m), l += p / (value scale): scales are one number a page and head, so that of 64 scores at a time they change the
-//                     factor and the offset of an fma that is there anyway, and O needs none.  P (fp16, 2^-11 of a weight off at most) replaces its S in tensor memory; m is raised,
-//                     and O scaled in tensor memory, only when a row's t outgrows it by 8
+//                     factor and the offset of an fma that is there anyway, and O needs none.  P (fp16) replaces its S in tensor memory; m is 7 below a row's largest t and raised, and
+//                     O scaled in tensor memory, only when a t outgrows it by 15: weights are 2^-11 of themselves off down to 2^-21 of the largest, and 2^-32 of that below
 // TMEM: [S0 | O0 | S1 | O1], 128 columns each (S: two buffers of 64).  Shared memory: Q 64 KB, K 3 x 16 KB, V 2 x 32 KB as fp16 and 2 x 16 KB as codes.
 // (With keys turned into fp16 as well the three warps were the bound: 2048 tokens behind 2001 took 318 us, 228 with their work left out.)
 #pragma once
@@ -297,10 +297,10 @@ __global__ void __launch_bounds__(kFpThreads, 1) fp8_attn_prompt_kernel(const __
 #pragma unroll
                 for (int q = 0; q < 4; q++) mx[q] = fmaxf(mx[q], s[i + q]);
             const float m_new = fmaf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), c, ve);
-            const bool raise = m_new > m_ref + 8.f || (m_ref == -INFINITY && m_new > -INFINITY);
+            const bool raise = m_new > m_ref + kFmRaise || (m_ref == -INFINITY && m_new > -INFINITY);
             if (__any_sync(0xffffffffu, raise)) {
-                const float alpha = raise ? exp2_approx(m_ref - m_new) : 1.f;      // (2^-inf = 0: nothing was summed yet)
-                if (raise) { m_ref = m_new; l *= alpha; }
+                const float alpha = raise ? exp2_approx(m_ref - (m_new - kFmTop)) : 1.f;      // (2^-inf = 0: nothing was summed yet)
+                if (raise) { m_ref = m_new - kFmTop; l *= alpha; }
                 if (i64 > 0) {
                     bar_wait(smem_u32(&misc.pv_done[t][buf ^ 1]), ((i64 - 1) >> 1) & 1);
                     tc_fence_after();

@@ -44,14 +44,19 @@ def test_prompt_attention_never_waits_for_a_phase_that_has_gone(lens, H, G):
         assert all(torch.equal(first, o) for o in outs)
 
 
-def run_dominant(lens, ps, H, G, d, dtype, gap, at, equal, wide=0, weight=2.0 ** -8, floor=2.0 ** -35, seed=0):
+def run_dominant(lens, ps, H, G, d, dtype, gap, at, equal, wide=0, weight=2.0 ** -8, floor=2.0 ** -35, query=2.0 ** -21, seed=0):
     """One key with most of every row's weight and a value of zero: what is left is the sum of all the others' small weights, compared with 64 bits relative to that sum.
     at: the key, a share of the first token's range.  gap: by how many nats its score is above the others' mean, about.  equal: the others have one score.  wide: 2^wide is the value
-    scale of its page, beside one for the others.  weight, floor: how far a weight may be off, of itself, and of the row's largest"""
+    scale of its page, beside one for the others.  weight, floor: how far a weight may be off, of itself, and of the row's largest;
+    query: how far a query's column, of the row's largest"""
     g = torch.Generator().manual_seed(seed)
     batch, cache, total = U.batch_of(lens, ps, seed=seed)
     T, dt, scale = batch.pos.shape[0], {"bf16": torch.bfloat16, "fp32": torch.float32}[dtype], d ** -0.5
     q = torch.randn((T, H, d), generator=g).to(dt)
+    for i, (_, n) in enumerate(lens):      # a portion's tokens look the same way
+        if n > 1:
+            t = int(batch.seqs[0, i])
+            q[t + 1:t + n] = q[t] + (0.1 * q[t + 1:t + n].float()).to(dt)
     codes = lambda x: x.clamp(-448, 448).to(U.E4M3)
     k = codes(torch.zeros((total, G, ps, d)) if equal else 16 * torch.randn((total, G, ps, d), generator=g))
     v = codes(16 + 4 * torch.randn((total, G, ps, d), generator=g))
@@ -76,8 +81,8 @@ def run_dominant(lens, ps, H, G, d, dtype, gap, at, equal, wide=0, weight=2.0 **
                 z = rows @ K[:at_t].T * scale
                 w = torch.softmax(z, 1)
                 ref, spread = w @ V[:at_t], w @ V[:at_t].abs()
-                # scores are fp32 sums of d products of queries that are 2^-21 of a row's largest off at most; an error e of them makes weights 2 e off
-                e = float(rows.norm(dim=1).max() * K[:at_t].norm(dim=1).max() * scale) * (2 * d + 8) * 2.0 ** -24 + float(rows.abs().max() * K[:at_t].abs().sum(1).max()) * scale * 2.0 ** -21 + 2.0 ** -20
+                # scores are fp32 sums of d products of queries that are `query` of a row's largest off at most; an error e of them makes weights 2 e off
+                e = float(rows.norm(dim=1).max() * K[:at_t].norm(dim=1).max() * scale) * (2 * d + 8) * 2.0 ** -24 + float(rows.abs().max() * K[:at_t].abs().sum(1).max()) * scale * query + 2.0 ** -20
                 bound = half * ref.abs() * 1.02 + (weight + 2 * e) * spread * 1.02 + floor * w.amax(1, keepdim=True) * 2.0 ** max(0, wide) * V[:at_t].abs().sum(0)
                 got = out[int(batch.seqs[0, i]) + t].reshape(G, H // G, d)[h]
                 worst = max(worst, float(((got - ref).abs() / bound).max()))
@@ -105,3 +110,18 @@ def test_single_tokens_keep_the_weights_beside_a_dominant_key(lens, ps, H, G, d,
 def test_single_tokens_keep_the_weights_beside_a_dominant_key_of_a_page_of_large_values(d):
     run_dominant([(15999, 1)], 64, 4, 1, d, "bf16", 14, 0.0, True, wide=5)
     run_dominant([(500, 1), (2000, 1)], 64, 4, 1, d, "bf16", 8, 1.0, False, wide=5)
+
+
+# fp16 weights: a step of 2^-24 beside a largest of 2^7 at least.  Prompt queries are two numbers of one scale, 2^-17 of a row's largest off
+SEVERAL = [
+    ([(15999, 1)], 64, 8, 2, 96, "bf16", 12), ([(12000, 2)], 20, 4, 1, 80, "bf16", 14), ([(15998, 4)], 64, 8, 2, 128, "bf16", 14), ([(3000, 40)], 32, 4, 1, 128, "bf16", 12), ([(700, 1), (90, 2)], 48, 6, 2, 96, "bf16", 9),
+    ([(8000, 40)], 64, 8, 2, 128, "bf16", 13), ([(4000, 130)], 64, 16, 1, 128, "bf16", 14), ([(64, 64), (900, 70)], 64, 8, 1, 128, "bf16", 9), ([(15999, 2)], 64, 4, 1, 128, "fp32", 14), ([(6000, 1)], 20, 4, 1, 80, "fp32", 12),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("equal", [False, True])
+@pytest.mark.parametrize("at", [0.0, 0.5, 1.0])
+@pytest.mark.parametrize("lens,ps,H,G,d,dtype,gap", SEVERAL)
+def test_other_calls_keep_the_weights_beside_a_dominant_key(lens, ps, H, G, d, dtype, gap, at, equal):
+    run_dominant(lens, ps, H, G, d, dtype, gap, at, equal, weight=2.0 ** -11 if dtype == "bf16" else 2.0 ** -22, floor=2.0 ** -32 if dtype == "bf16" else 0.0, query=2.0 ** -17 if dtype == "bf16" else 0.0)
