@@ -637,7 +637,7 @@ int ktb200_softmax_attn_prompt_tiles(const ktb200_softmax_attn_params* params, i
  *     q_out [n_tokens][heads][dim]; k, v into the cache.  A portion that begins inside a page keeps the page's earlier tokens (their codes move where the
  *     scale grows: exactly, but for what becomes subnormal); one that begins at a page's first token starts its blocks anew.  Codes of other rows are left as they were.
  *   ktb200_fp8_cache_attn     out[t * out_stride + h vdim + c] = out_scale * sum_j w_j v_j / (sum_j w_j + exp(sink[h])), w_j = exp(cap(scale head_scale[h] q.k_j)),
- *     with the masks, cap and optional pointers of ktb200_softmax_attn.  A row that sees no key is zero.  max_keys: no sequence has more tokens, this
+ *     with the masks, cap and optional pointers of ktb200_softmax_attn.  A row that sees no key is zero, beside any sink (an infinite one, or one that overflows: nothing or everything).  max_keys: no sequence has more tokens, this
  *     call's included.  part: -1, the library cuts long key ranges among CTAs as it sees fit; 0, it does not; more (a multiple of 128), in parts of so many keys, 128 of them at most.
  *     workspace: ktb200_fp8_cache_attn_workspace bytes, of this call alone (that function reads the struct's sizes, counts and the pointers' alignment).
  * seqs: rows (first token's row, token count) of the n_seqs portions, seqs_stride apart.  A portion's tokens stand at consecutive positions from pos[first row], in the pages of table row

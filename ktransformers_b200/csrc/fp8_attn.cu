@@ -44,6 +44,13 @@ __device__ __forceinline__ int fp8_first_visible(int p, int window, int chunk) {
     if (chunk > 0) lo = max(lo, p - p % chunk);
     return lo;
 }
+// The sink's term in a row's sum l over the reference m (both, and the sink, as exponents of two); returns what the row's other sums are multiplied by.  An infinite sink takes all (+) or
+// nothing (-), and a row that sees no key stays at zero beside either
+__device__ __forceinline__ float fp8_sink(float sink, float m, float& l) {
+    const float sk = sink * kLog2e, mn = fmaxf(m, sk), k = m == -INFINITY ? 0.f : exp2_approx(m - mn);
+    l = l * k + (sk == mn ? 1.f : exp2_approx(sk - mn));
+    return k;
+}
 // tokens of portion s (none where its rows are not those of the step)
 __device__ __forceinline__ int fp8_portion(const Fp8Attn& a, int s) {
     const int start = a.seqs[s], len = a.seqs[a.seqs_stride + s];
@@ -271,8 +278,8 @@ template <typename T, int NC, bool VEC, int ROWS> __global__ void __launch_bound
         float corr = 1.f;
         if (a.sink) {
             const float mn = fmaxf(m[r], a.sink[h]);
-            corr = expf(m[r] - mn);
-            sum = sum * corr + expf(a.sink[h] - mn);
+            corr = m[r] == -INFINITY ? 0.f : expf(m[r] - mn);
+            sum = sum * corr + (a.sink[h] == mn ? 1.f : expf(a.sink[h] - mn));
         }
         const float inv = sum > 0.f || sum != sum ? corr * a.out_scale / sum : 0.f;
         T* out = (T*)a.out + t * a.out_stride + (long)h * dv;
@@ -318,7 +325,7 @@ template <typename T> __global__ void __launch_bounds__(128 * kMergeGroups) fp8_
         if (lane == 0) red[warp] = part_l;
         asm volatile("barrier.cta.sync 1, 128;" ::: "memory");
         float l = (red[0] + red[1]) + (red[2] + red[3]);
-        if (a.sink) l += exp2f((sink - m) * unit);
+        if (a.sink) l += sink == m ? 1.f : exp2f((sink - m) * unit);      // (an infinite one too)
         if (tid < parts) wgt[tid] = l > 0.f || l != l ? e / l : 0.f;
         if (l != l && tid < parts) wgt[tid] = l;
     }

@@ -402,8 +402,7 @@ template <int DP, int DVP, bool SHARED, bool TWO> __global__ void __launch_bound
                 if ((tid & 7) == 0) { part[0] = m; part[1] = l; }
             } else {
                 if (a.sink) {
-                    const float sk = a.sink[h] * kLog2e, mn = fmaxf(m, sk), k = m == -INFINITY ? 0.f : exp2_approx(m - mn);
-                    l = l * k + exp2_approx(sk - mn);
+                    const float k = fp8_sink(a.sink[h], m, l);
 #pragma unroll
                     for (int w = 0; w < kFmWarps; w++) wgt[w] *= k;
                 }
@@ -444,11 +443,7 @@ template <int DP, int DVP, bool SHARED, bool TWO> __global__ void __launch_bound
         if (part) {
             if (tq == 0) { part[0] = m; part[1] = l; }
         } else {
-            if (a.sink) {
-                const float sk = a.sink[h] * kLog2e, mn = fmaxf(m, sk);
-                k = m == -INFINITY ? 0.f : exp2_approx(m - mn);
-                l = l * k + exp2_approx(sk - mn);
-            }
+            if (a.sink) k = fp8_sink(a.sink[h], m, l);
             k = l > 0.f || l != l ? k * a.out_scale / l : 0.f;
         }
         __nv_bfloat16* out = (__nv_bfloat16*)a.out + (long)(tok0 + tok) * a.out_stride + (long)h * dv;

@@ -349,11 +349,7 @@ __global__ void __launch_bounds__(kFpThreads, 1) fp8_attn_prompt_kernel(const __
         if (cut) {
             if (valid) *reinterpret_cast<float2*>(part) = make_float2(m_ref, l);
         } else {
-            if (a.sink) {
-                const float sk = a.sink[h] * kLog2e, mn = fmaxf(m_ref, sk);
-                k = m_ref == -INFINITY ? 0.f : exp2_approx(m_ref - mn);
-                l = l * k + exp2_approx(sk - mn);
-            }
+            if (a.sink) k = fp8_sink(a.sink[h], m_ref, l);
             k = l > 0.f || l != l ? k * a.out_scale / l : 0.f;
         }
         __nv_bfloat16* out = (__nv_bfloat16*)a.out + (long)(tok0 + tok) * a.out_stride + (long)h * 128;

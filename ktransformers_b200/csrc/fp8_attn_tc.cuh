@@ -403,11 +403,7 @@ template <int RP, int PAIR> __global__ void __launch_bounds__(kFdThreads, RP * P
                 if (r == 0) { part[0] = m[h]; part[1] = sum; }
                 part[2 + r] = v[h];
             } else {
-                if (a.sink) {
-                    const float sk = a.sink[h0 + h] * kLog2e, mn = fmaxf(m[h], sk), k = m[h] == -INFINITY ? 0.f : exp2_approx(m[h] - mn);
-                    sum = sum * k + exp2_approx(sk - mn);
-                    v[h] *= k;
-                }
+                if (a.sink) v[h] *= fp8_sink(a.sink[h0 + h], m[h], sum);
                 ((__nv_bfloat16*)a.out)[(long)t * a.out_stride + (long)(h0 + h) * D + r] = __float2bfloat16_rn(sum > 0.f || sum != sum ? v[h] * (a.out_scale / sum) : 0.f);
             }
         }
@@ -420,7 +416,8 @@ template <int RP, int PAIR> __global__ void __launch_bounds__(kFdThreads, RP * P
         if (warp >= 2) {
             const int c = tid - 64, cuts = (p + 1 - lo_al + part - 1) / part;      // the CTAs that have keys
             for (int h = blockIdx.z; h < RH && c < D; h += cuts) {
-                float mk[kFdCluster], lk[kFdCluster], vk[kFdCluster], top = a.sink ? a.sink[h0 + h] * kLog2e : -INFINITY;
+                const float sink = a.sink ? a.sink[h0 + h] * kLog2e : -INFINITY;
+                float mk[kFdCluster], lk[kFdCluster], vk[kFdCluster], top = sink;
 #pragma unroll
                 for (int k = 0; k < kFdCluster; k++)
                     if (k < cuts) {
@@ -429,7 +426,7 @@ template <int RP, int PAIR> __global__ void __launch_bounds__(kFdThreads, RP * P
                         vk[k] = mk[k] > -INFINITY ? cluster_load(base + 8 * RP + 512 * h + 4 * c, k) : 0.f;
                         top = fmaxf(top, mk[k]);
                     }
-                float sum = a.sink ? exp2_approx(a.sink[h0 + h] * kLog2e - top) : 0.f, v = 0.f;
+                float sum = !a.sink ? 0.f : sink == top ? 1.f : exp2_approx(sink - top), v = 0.f;
 #pragma unroll
                 for (int k = 0; k < kFdCluster; k++)
                     if (k < cuts) {

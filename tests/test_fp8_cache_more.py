@@ -125,3 +125,25 @@ SEVERAL = [
 @pytest.mark.parametrize("lens,ps,H,G,d,dtype,gap", SEVERAL)
 def test_other_calls_keep_the_weights_beside_a_dominant_key(lens, ps, H, G, d, dtype, gap, at, equal):
     run_dominant(lens, ps, H, G, d, dtype, gap, at, equal, weight=2.0 ** -11 if dtype == "bf16" else 2.0 ** -22, floor=2.0 ** -32 if dtype == "bf16" else 0.0, query=2.0 ** -17 if dtype == "bf16" else 0.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("lens,ps,H,G,d", [
+    ([(200, 1), (40, 1)], 64, 8, 1, 128), ([(3000, 1), (40, 1)], 64, 16, 1, 128), ([(60000, 1), (40, 1)], 64, 4, 1, 128), ([(900, 1), (40, 1)], 16, 8, 1, 64), ([(100, 3), (40, 2)], 48, 6, 2, 96),
+    ([(3000, 1), (40, 1)], 64, 6, 2, 96), ([(100, 40), (10, 40)], 32, 4, 1, 128), ([(700, 90), (10, 90)], 64, 4, 1, 128), ([(5000, 64), (10, 64)], 64, 2, 1, 128), ([(30, 2), (3, 2)], 16, 2, 1, 40),
+])
+def test_sinks_of_nothing_and_of_everything(lens, ps, H, G, d, dtype):
+    """exp(-inf) adds nothing, exp(+inf) leaves nothing of the keys, and the second sequence, none of whose pages is there, is zero beside either"""
+    batch, cache, total = U.batch_of(lens, ps, seed=3)
+    cache.page_table[1] = -1
+    kv, T = layer(total, G, ps, d, 3), batch.pos.shape[0]
+    q = torch.randn((T, H, d), generator=torch.Generator().manual_seed(4)).to(torch.bfloat16 if dtype == "bf16" else torch.float32).cuda()
+    run = lambda sink: fp8_cache_attention(q, kv, on(batch), on(cache), H, G, d, d, d ** -0.5, sink=sink)
+    row, none, first = torch.ones(H, device="cuda"), run(None), lens[0][1]
+    assert none.isfinite().all() and (none[:first] != 0).any() and (none[first:] == 0).all()
+    for low in (-math.inf, -3.4028234663852886e38):
+        assert torch.equal(run(low * row), none)
+    assert (run(row)[first:] == 0).all()
+    for high in (math.inf, 3.4028234663852886e38):
+        assert (run(high * row) == 0).all()
