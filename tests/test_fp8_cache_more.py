@@ -147,3 +147,12 @@ def test_sinks_of_nothing_and_of_everything(lens, ps, H, G, d, dtype):
     assert (run(row)[first:] == 0).all()
     for high in (math.inf, 3.4028234663852886e38):
         assert (run(high * row) == 0).all()
+
+
+def test_both_calls_refuse_cpu_tensors():
+    batch, cache, total = U.batch_of([(5, 1)], 16)
+    kv = layer(total, 2, 16, 32, 0, "cpu")
+    with pytest.raises(ValueError, match="fp8_cache_append: CUDA tensors only"):
+        fp8_cache_append(torch.zeros(1, 256), batch, cache, kv, 4, 2, 32, 32, (0, 128, 192))
+    with pytest.raises(ValueError, match="fp8_cache_attention: CUDA tensors only"):
+        fp8_cache_attention(torch.zeros(1, 4, 32), kv, batch, cache, 4, 2, 32, 32, 0.1)
