@@ -467,7 +467,7 @@ static int i8_map(CUtensorMap* map, const void* ptr, int K, long stride, int n, 
 }
 // K splits of int8_rows_kernel: those whose CTAs, two an SM, take least one after the other; kI8Round is what a CTA costs beside its blocks, in blocks
 constexpr int kI8Round = 8;
-static int i8_splits(long tiles, int nkb, int sms, long* cost_out = nullptr) {
+static int i8_splits(long tiles, int nkb, int sms) {
     int best = 1;
     long least = LONG_MAX;
     for (int s = 1; s <= std::min(kI8MaxSplits, nkb); s++) {
@@ -476,7 +476,6 @@ static int i8_splits(long tiles, int nkb, int sms, long* cost_out = nullptr) {
         const long cost = ((tiles * s + 2 * sms - 1) / (2 * sms)) * (per + kI8Round);
         if (cost < least) { least = cost; best = s; }
     }
-    if (cost_out) *cost_out = least;
     return best;
 }
 template <int NT> static int i8_launch_rows(const void* w, long w_stride, const int8_t* codes, int K, int Kp, const Int8Out& o, int sms, cudaStream_t s) {
@@ -505,14 +504,13 @@ template <int NT> static int i8_launch_rows(const void* w, long w_stride, const 
 // Columns of a pair's tile: the multiple of 32 whose rounds take least.  A K block of bn columns takes the larger of its products' time and the shared memory's, in 128 x bn: bn, and about
 // 128 + bn / 2; kI8Fixed is what a tile costs beside its blocks, in blocks
 constexpr int kI8Fixed = 4;
-static int i8_columns(int mt, int N, int nkb, int pairs, long* cost_out = nullptr) {
+static int i8_columns(int mt, int N, int nkb, int pairs) {
     int best = 256;
     long least = LONG_MAX;
     for (int bn = 256; bn >= 32; bn -= 32) {
         const long rounds = ((long)mt * ((N + bn - 1) / bn) + pairs - 1) / pairs, cost = rounds * (nkb + kI8Fixed) * std::max(bn, 128 + bn / 2);
         if (cost < least) { least = cost; best = bn; }
     }
-    if (cost_out) *cost_out = least;
     return best;
 }
 static int i8_launch_gemm(const void* w, long w_stride, const int8_t* codes, int K, int Kp, const Int8Out& o, int sms, cudaStream_t s) {
