@@ -8,7 +8,7 @@
 //   weights   p = 2^(t - m), t = s log2(e) + log2(value scale).  Value scales are powers of two: in the exponent they cost nothing and O needs none.  m is 7 below a head's largest t,
 //             raised when a t outgrows it by 8.75 (2^8.75 < 448).  The two numbers are within 2^-8 of a weight from 2^-6 on (as a bf16 weight is).  A long context behind one key that has
 //             most of the weight lies below that, so a smaller weight stands in two more columns, 2^14 times itself: within 2^-8 of it down to 2^-20, and 2^-28 off below, 2^-35 of the
-//             largest.  They are zeros, and not written, as long as a warp has no such weight (64 contexts of 4095 to 8190 keys: 148 us without any, 152 with some in every tile)
+//             largest.  They are zeros, and not written, as long as a warp has no such weight (64 contexts of 4095 to 8190 keys: 148 us with few, 152 with some in every tile)
 // l += p / (value scale), O / l is the result: 2^m drops out.
 // Heads of 64 (PAIR = 2): a row of 128 bytes is two neighbouring keys.  Queries and weights then have rows of their own for the first and for the second of a pair, zero where the other's
 // columns are; of the products, twice as many as needed, the mixed ones are not looked at.  What bounds is the bytes all the same: 30 tokens over 2000 to 4000 keys, 64 heads over 8, take
@@ -30,7 +30,7 @@ namespace ktb {
 
 constexpr int kFdThreads = 192, kFdRows = 128, kFdTile = kFdRows * 128, kFdStages = 2;
 constexpr float kFdTop = 7.f, kFdRaise = 8.75f;
-constexpr float kFdSmall = 0.015625f, kFdLift = 16384.f, kFdNone = 3.7252903e-9f;      // weights below 2^-6 stand as 2^14 times themselves; 2^-28: and what becomes zero there
+constexpr float kFdSmall = -6.f, kFdLift = 16384.f, kFdNone = -28.f;      // weights below 2^-6 stand as 2^14 times themselves; those below 2^-28 become zero there
 template <int RP> struct FdMisc {
     unsigned long long k_full[kFdStages], k_free[kFdStages], v_full[kFdStages], v_free[kFdStages], s_full[2], s_free[2], p_full[2], p_free[2], q_ready;
     float red[4][RP], fac[RP];
@@ -311,32 +311,34 @@ template <int RP, int PAIR> __global__ void __launch_bounds__(kFdThreads, RP * P
             bool small = false;
 #pragma unroll
             for (int i = 0; i < PAIR * RP; i++) {
-                const int h = i % RP;
-                x[i] = exp2_approx(x[i] - (m[h] == -INFINITY ? 0.f : m[h]));
-                l[h] = fmaf(x[i], inv, l[h]);
+                x[i] -= m[i % RP] == -INFINITY ? 0.f : m[i % RP];
                 small |= x[i] < kFdSmall && x[i] > kFdNone;
             }
+            small = __any_sync(0xffffffffu, small);
+            const bool wide = small || (lifted >> buf & 1);      // (what the warp wrote there two tiles ago is taken back)
             uint8_t* P = smem + (pbase - base) + buf * OP;
-            auto put = [&](int n, uint2 c) {      // rows n, n + 1 of both terms
+            auto put = [&](int n, float p0, float p1) {      // rows n, n + 1 of both terms
+                const uint2 c = split_e4m3(p0, p1);
                 P[fd_at(n, r)] = (uint8_t)c.x;
                 P[fd_at(n + 1, r)] = (uint8_t)(c.x >> 8);
                 P[fd_at(n + RP, r)] = (uint8_t)c.y;
                 P[fd_at(n + RP + 1, r)] = (uint8_t)(c.y >> 8);
             };
-            small = __any_sync(0xffffffffu, small);
-            if (small || (lifted >> buf & 1)) {
 #pragma unroll
-                for (int i = 0; i < PAIR * RP; i += 2) {
-                    const int n = i / RP * 4 * RP + i % RP;
+            for (int i = 0; i < PAIR * RP; i += 2) {
+                const int h = i % RP, n = i / RP * 4 * RP + h;
+                float p0 = exp2_approx(x[i]), p1 = exp2_approx(x[i + 1]);
+                l[h] = fmaf(p0, inv, l[h]);
+                l[h + 1] = fmaf(p1, inv, l[h + 1]);
+                if (wide) {
                     const bool s0 = x[i] < kFdSmall, s1 = x[i + 1] < kFdSmall;
-                    put(n, split_e4m3(s0 ? 0.f : x[i], s1 ? 0.f : x[i + 1]));
-                    put(n + 2 * RP, split_e4m3(s0 ? x[i] * kFdLift : 0.f, s1 ? x[i + 1] * kFdLift : 0.f));
+                    put(n + 2 * RP, s0 ? p0 * kFdLift : 0.f, s1 ? p1 * kFdLift : 0.f);
+                    p0 = s0 ? 0.f : p0;
+                    p1 = s1 ? 0.f : p1;
                 }
-                lifted ^= ((lifted >> buf & 1) ^ (uint32_t)small) << buf;
-            } else {
-#pragma unroll
-                for (int i = 0; i < PAIR * RP; i += 2) put(i / RP * 4 * RP + i % RP, split_e4m3(x[i], x[i + 1]));
+                put(n, p0, p1);
             }
+            lifted = (lifted & ~(1u << buf)) | (uint32_t)small << buf;
             const int k0 = k_lo + j * KEYS;
             if (k0 < lo || k0 + KEYS > k_hi) {      // the first and last tiles: values of keys that are not seen may be anything (0 x NaN)
                 const int st = j % kFdStages;
