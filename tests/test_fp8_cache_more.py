@@ -44,11 +44,32 @@ def test_prompt_attention_never_waits_for_a_phase_that_has_gone(lens, H, G):
         assert all(torch.equal(first, o) for o in outs)
 
 
+def farthest(out, q, k, v, s, batch, cache, lens, scale, weight, floor, query, wide=1.0):
+    """(largest distance of out [T, H, d] from attention in 64 bits, in bounds; the rows' largest weights); all on the CPU.  weight, floor: how far a weight may be off, of itself, and of the
+    row's largest; query: how far a query's column, of the row's largest; wide: the largest value scale over the smallest"""
+    half, worst, seen, (_, G, ps, d), H = {torch.bfloat16: 2.0 ** -8, torch.float32: 2.0 ** -24}[q.dtype], 0.0, [], k.shape, q.shape[1]
+    for i, (b, n) in enumerate(lens):
+        j = torch.arange(b + n)
+        page = cache.page_table[i].long()[j // ps]
+        for h in range(G):
+            K, V = (x[page, h, j % ps].double() * s[page, h, c, None].double() for c, x in ((0, k), (1, v)))
+            for t in range(n):
+                at_t, rows = b + t + 1, q[int(batch.seqs[0, i]) + t].double().reshape(G, H // G, d)[h]
+                w = torch.softmax(rows @ K[:at_t].T * scale, 1)
+                ref, spread = w @ V[:at_t], w @ V[:at_t].abs()
+                # scores are fp32 sums of d products of queries that are `query` of a row's largest off at most; an error e of them makes weights 2 e off
+                e = float(rows.norm(dim=1).max() * K[:at_t].norm(dim=1).max() * scale) * (2 * d + 8) * 2.0 ** -24 + float(rows.abs().max() * K[:at_t].abs().sum(1).max()) * scale * query + 2.0 ** -20
+                bound = half * ref.abs() * 1.02 + (weight + 2 * e) * spread * 1.02 + floor * w.amax(1, keepdim=True) * wide * V[:at_t].abs().sum(0)
+                got = out[int(batch.seqs[0, i]) + t].reshape(G, H // G, d)[h]
+                worst = max(worst, float(((got - ref).abs() / bound).max()))
+                seen.append(float(w.amax(1).max()))
+    return worst, seen
+
+
 def run_dominant(lens, ps, H, G, d, dtype, gap, at, equal, wide=0, weight=2.0 ** -8, floor=2.0 ** -35, query=2.0 ** -21, big=1.0, seed=0):
     """One key (gap: None, no such key) with most of every row's weight and a value of zero: what is left is the sum of all the others' small weights, compared with 64 bits relative to that sum.
     at: the key, a share of the first token's range.  gap: by how many nats its score is above the others' mean, about.  equal: the others have one score.  wide: 2^wide is the value
-    scale of its page, beside one for the others.  weight, floor: how far a weight may be off, of itself, and of the row's largest;
-    query: how far a query's column, of the row's largest.  big: the size of the queries"""
+    scale of its page, beside one for the others.  weight, floor, query: as in `farthest`.  big: the size of the queries"""
     g = torch.Generator().manual_seed(seed)
     batch, cache, total = U.batch_of(lens, ps, seed=seed)
     T, dt, scale = batch.pos.shape[0], {"bf16": torch.bfloat16, "fp32": torch.float32}[dtype], d ** -0.5
@@ -70,23 +91,7 @@ def run_dominant(lens, ps, H, G, d, dtype, gap, at, equal, wide=0, weight=2.0 **
         s[page, :, 1] *= 2.0 ** wide
     kv = Fp8CacheLayer(k.cuda(), v.cuda(), s.cuda())
     out = fp8_cache_attention(q.cuda(), kv, on(batch), on(cache), H, G, d, d, scale).cpu().double().reshape(T, H, d)
-    half, worst, seen = {"bf16": 2.0 ** -8, "fp32": 2.0 ** -24}[dtype], 0.0, []
-    for i, (b, n) in enumerate(lens):
-        j = torch.arange(b + n)
-        page = cache.page_table[i].long()[j // ps]
-        for h in range(G):
-            K, V = (x[page, h, j % ps].double() * s[page, h, c, None].double() for c, x in ((0, k), (1, v)))
-            for t in range(n):
-                at_t, rows = b + t + 1, q[int(batch.seqs[0, i]) + t].double().reshape(G, H // G, d)[h]
-                z = rows @ K[:at_t].T * scale
-                w = torch.softmax(z, 1)
-                ref, spread = w @ V[:at_t], w @ V[:at_t].abs()
-                # scores are fp32 sums of d products of queries that are `query` of a row's largest off at most; an error e of them makes weights 2 e off
-                e = float(rows.norm(dim=1).max() * K[:at_t].norm(dim=1).max() * scale) * (2 * d + 8) * 2.0 ** -24 + float(rows.abs().max() * K[:at_t].abs().sum(1).max()) * scale * query + 2.0 ** -20
-                bound = half * ref.abs() * 1.02 + (weight + 2 * e) * spread * 1.02 + floor * w.amax(1, keepdim=True) * 2.0 ** max(0, wide) * V[:at_t].abs().sum(0)
-                got = out[int(batch.seqs[0, i]) + t].reshape(G, H // G, d)[h]
-                worst = max(worst, float(((got - ref).abs() / bound).max()))
-                seen.append(float(w.amax(1).max()))
+    worst, seen = farthest(out, q, k, v, s, batch, cache, lens, scale, weight, floor, query, 2.0 ** max(0, wide))
     assert gap is None or max(seen) > 0.9      # (the key does have most of the weight)
     assert worst <= 1, worst
 
@@ -201,3 +206,27 @@ def test_scores_of_any_size(lens, ps, H, G, d, dtype, big):
     single = dtype == "bf16" and d in (64, 128) and ps % 16 == 0 and all(n == 1 for _, n in lens)
     weight, floor, query = (2.0 ** -22, 0.0, 0.0) if dtype == "fp32" else (2.0 ** -8, 2.0 ** -35, 2.0 ** -21) if single else (2.0 ** -11, 2.0 ** -32, 2.0 ** -17)
     run_dominant(lens, ps, H, G, d, dtype, None, 0.0, False, weight=weight, floor=floor, query=query, big=big)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d,ps,dtype", [(128, 64, "bf16"), (64, 16, "bf16"), (96, 48, "bf16"), (128, 64, "fp32")])
+def test_steps_read_what_they_appended(d, ps, dtype):
+    """Prompt portions, steps of portions beside decoded tokens, and decoded tokens: each step's attention against 64 bits over what the cache holds then, of the queries that the append gave"""
+    H, G, g, dt = 8, 2, torch.Generator().manual_seed(d), {"bf16": torch.bfloat16, "fp32": torch.float32}[dtype]
+    rot, inv, done = SimpleNamespace(dims=d, layout_code=1), 1000.0 ** (-torch.arange(0, d, 2, dtype=torch.float64) / d), [0, 0, 0]
+    _, cache, total = U.batch_of([(0, 400)] * 3, ps)
+    kv, i32 = Fp8CacheLayer.empty(total, ps, G, d, d), lambda v: torch.tensor(v, dtype=torch.int32)
+    for step in ((200, 70, 0), (90, 1, 1), (1, 150, 1), (1, 1, 1), (2, 1, 3), (1, 1, 1)):
+        lens = list(zip(done, step))
+        starts = [sum(step[:i]) for i in range(3)]
+        batch = SimpleNamespace(pos=i32([p for b, n in lens for p in range(b, b + n)]), slot=i32([i for i, n in enumerate(step) for _ in range(n)]), seqs=i32([starts, step]), n_seqs=3,
+                                max_kv=max(b + n for b, n in lens))
+        proj = (1 + 3 * (torch.rand((H + 2 * G) * d, generator=g) > 0.97)) * torch.randn((sum(step), (H + 2 * G) * d), generator=g)
+        q = fp8_cache_append(proj.to(dt).cuda(), on(batch), on(cache), kv, H, G, d, d, (0, H * d, (H + G) * d), rot, inv.cuda(), 1, 1e-6)
+        out = fp8_cache_attention(q, kv, on(batch), on(cache), H, G, d, d, 2 * d ** -0.5).cpu().double().reshape(-1, H, d)
+        k, v, s = (x.cpu() for x in (kv.k, kv.v, kv.scales))
+        spread = float(s[..., 1].max() / s[..., 1].min())
+        weight, floor, query = (2.0 ** -22, 0.0, 0.0) if dtype == "fp32" else (2.0 ** -8, 2.0 ** -32, 2.0 ** -17)      # (whichever kernel a step takes)
+        worst, _ = farthest(out, q.cpu(), k, v, s, batch, cache, lens, 2 * d ** -0.5, weight, floor, query, spread)
+        assert worst <= 1, (step, worst)
+        done = [b + n for b, n in lens]
