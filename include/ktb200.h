@@ -631,7 +631,8 @@ int ktb200_softmax_attn_prompt_tiles(const ktb200_softmax_attn_params* params, i
 
 /* The paged cache in 8 bits (csrc/fp8_cache.cu, csrc/fp8_attn.cu).  A page holds page_size tokens of every key/value head, head by head: k_codes [n_pages][kv_heads][page_size][dim]
  * and v_codes [n_pages][kv_heads][page_size][vdim] (e4m3), scales [n_pages][kv_heads][2] (fp32, keys then values): a code stands for code * scale of its page and
- * head.  Scales are powers of two: 2^e, e the smallest number in [-64, 64] with 448 * 2^e >= max |x| over the block's tokens (what is larger saturates, NaN stays NaN).
+ * head.  Scales are powers of two: 2^e, e the smallest number in [-64, 64] with 448 * 2^e >= max |x| over the block's tokens (what is larger saturates, NaN stays NaN; an infinity makes it
+ * 2^64, under which the block's other values become zero).  A page is written by one portion of a call: two that append to the same one race.
  *   ktb200_fp8_cache_append   q [heads*dim] at q_off, k [kv_heads*dim] at k_off, v [kv_heads*vdim] at v_off of proj's rows; q and k head by head: qk_norm 0 nothing, 1
  *     x / sqrt(mean(x^2) + eps), 3 the same times q_weight / k_weight [dim]; then a turn of the first rot_dims columns (rot_layout as above).  q of all n_tokens tokens to
  *     q_out [n_tokens][heads][dim]; k, v into the cache.  A portion that begins inside a page keeps the page's earlier tokens (their codes move where the

@@ -389,7 +389,7 @@ static long fp8_tiles(const ktb200_fp8_attn_params* c, int n_tokens, int ctoks) 
 static bool fp8_sizes_ok(const ktb200_fp8_attn_params* c) { return c && c->heads > 0 && c->kv_heads > 0 && c->heads % c->kv_heads == 0; }
 
 // How a call's ranges are cut: `even` CTAs of a cluster for each, or parts of `part` keys, or (0, 0) not at all.  Not where the CTAs of uncut ranges fill the SMs' places four times.  A
-// cluster where eight CTAs a range fill the places once, or leave them 1024 keys at most: as many as fill the places twice and still have 256 keys each (64 contexts of 4095 to 8190: two CTAs a range 151 us, three 154, four 158).  Else parts of such a length
+// cluster where eight CTAs a range fill the places once, or leave them 1024 keys at most: as many as fill the places twice and still have 256 keys each (64 contexts of 4095 to 8190: two CTAs a range 148 us; when that was 151, three took 154 and four 158).  Else parts of such a length
 // that one round of CTAs covers the ranges, between sequences that decode (whose ranges may have any length) no more than 2048
 struct Fp8Cut { int even, part; };
 static Fp8Cut fp8_cut(const ktb200_fp8_attn_params* c, int n_tokens, int max_keys, const Fp8Form& f) {

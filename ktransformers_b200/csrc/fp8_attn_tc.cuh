@@ -11,8 +11,8 @@
 //             largest.  They are zeros, and not written, as long as a warp has no such weight (64 contexts of 4095 to 8190 keys: 148 us with few, 152 with some in every tile)
 // l += p / (value scale), O / l is the result: 2^m drops out.
 // Heads of 64 (PAIR = 2): a row of 128 bytes is two neighbouring keys.  Queries and weights then have rows of their own for the first and for the second of a pair, zero where the other's
-// columns are; of the products, twice as many as needed, the mixed ones are not looked at.  What bounds is the bytes all the same: 30 tokens over 2000 to 4000 keys, 64 heads over 8, take
-// 43 us where fp16 mma tiles take 56, one over 60000 keys 24 us against 33.
+// columns are; of the products, twice as many as needed, the mixed ones are not looked at.  Bound by the soft-max threads, which write twice the bytes of weights for one of codes: 30 tokens
+// over 2000 to 4000 keys, 64 heads over 8, take 45 us (53 with small weights in every tile; the cache's bytes 14) where fp16 mma tiles take 56, one over 60000 keys 25 (29; 9) against 33.
 //     warp 0      TMA: K and V tiles, two stages; a tile is runs of 16, 32 or 64 keys, each inside one page (runs that no key of the part lies in come as zeros)
 //     warp 1      MMAs: S of the next tile ahead of PV of this one
 //     warps 2-5   a thread owns a key: its scores of all heads are one row of S^T, so that scales and masks are its own; maxima are only needed when one has outgrown its

@@ -554,7 +554,8 @@ def fp8_cache_append(proj: torch.Tensor, batch, cache, kv, heads: int, kv_heads:
                      eps: float = 0.0, q_weight: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None) -> torch.Tensor:
     """`qkv_prep` for a layer held in 8 bits (`kv`: models.custom_cache.Fp8CacheLayer): from a projection's q, k and v columns (`offsets`) to the queries
     [T, heads, dim] and the layer's codes and scales, one `ktb200_fp8_cache_append` launch (csrc/fp8_cache.cu).  q and k: unit rms per row (qk_norm = 1), or times q_weight /
-    k_weight [dim] ahead of the rotation (qk_norm = 3).  A scale belongs to one page and head: tokens appended to a page whose scale they exceed have its earlier codes moved."""
+    k_weight [dim] ahead of the rotation (qk_norm = 3).  A scale belongs to one page and head: tokens appended to a page whose scale they exceed have its earlier codes moved
+    (a page belongs to one sequence of the batch)."""
     what = "fp8_cache_append"
     args, code, dev = _fp8_batch(what, proj, kv, batch, cache, kv_heads, dim, vdim)
     T, dt, (q_off, k_off, v_off) = proj.shape[0], proj.dtype, offsets
