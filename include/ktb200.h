@@ -405,6 +405,42 @@ size_t ktb200_latent_step_bytes(int batch, int heads, int nope_dim, int v_dim, i
 int ktb200_latent_step(const ktb200_latent_step_params* p, void* stream);
 
 
+/* ------------------------------------------------------------------------------------------
+ * Latent attention beyond one decoded token (bf16): the append to the paged latent cache and the attention of any number of new tokens a sequence over it
+ * (archive/ktransformers/operators/attention.py:140-344, the prefill branches; operators/RoPE.py:222-326, the scaled rotation).
+ * Token t of a call belongs to sequence slot[t] (a row of page_table, n_slots x max_pages, a ring over logical pages) at position pos[t]; portion s is the tokens seqs[s] ..
+ * seqs[s] + seqs[seqs_stride + s] - 1, at consecutive positions.  cache: [n_pages][page_size][kv_rank + rot_dim], [latent | rotated key part].  What slots, pages or portions that are not
+ * there would hold is neither read nor written, and rows of tokens in no portion stay as they were.
+ *
+ * ktb200_latent_append: q row = heads x [nope_dim | rot_dim], kva row = [latent | key part | ...].  q_rot[t][h][:] and the cache row's key part: pairs of the first rot_dims columns turned
+ *   by pos * inv_freq[i] (fp64; angle_pos[t] in pos's place where given), cosines and sines times rot_gain.  rot_layout 0: columns 2 i and 2 i + 1 are a pair, 1: i and i + rot_dims / 2;
+ *   rot_split: pairs of layout 0 come out in layout 1, as DeepSeek's caches hold them.  Latent: x / sqrt(mean x^2 + eps) * norm_weight, rounded once.
+ * ktb200_latent_attn: out[t][h][:] = soft-max attention of [q_nope | q_rot] over the sequence's keys [W_K,h c_j | k_j], values W_V,h c_j, j <= pos[t]; w [heads][nope_dim + vdim][512] holds
+ *   W_K,h above W_V,h (kv_b_proj).  Latents of 512 + 64, nope_dim and vdim 64 or 128, scale > 0.  form 1 (absorbed): the queries go to the latents and sums of latents to the values; 2 (expanded):
+ *   keys and values are made of the latents once a call; 0: the one that takes less (ktb200_latent_attn_form).  max_kv: no position of the call is max_kv or more.  workspace: 1024-byte aligned,
+ *   ktb200_latent_attn_workspace bytes (which also gives 0 for arguments that the call refuses).
+ * ------------------------------------------------------------------------------------------ */
+typedef struct ktb200_latent_append_params {
+    const void* q; long q_stride; int heads, nope_dim;
+    const void* kva; long kva_stride; int kv_rank, rot_dim;
+    const void* norm_weight; float eps;
+    int rot_dims, rot_layout, rot_split; float rot_gain; const double* inv_freq;
+    const int *angle_pos, *pos, *slot, *seqs; int seqs_stride, n_seqs;
+    const int* page_table; int n_slots, max_pages, page_size, n_pages;
+    void *cache, *q_rot;
+} ktb200_latent_append_params;
+int ktb200_latent_append(const ktb200_latent_append_params* p, int n_tokens, void* stream);
+typedef struct ktb200_latent_attn_params {
+    const void* q; long q_stride; const void* q_rot; int heads, nope_dim, vdim;
+    const void* w; float scale; int form;
+    const int *pos, *slot, *seqs; int seqs_stride, n_seqs;
+    const int* page_table; int n_slots, max_pages, page_size, n_pages;
+    const void* cache; void* out; long out_stride;
+} ktb200_latent_attn_params;
+int ktb200_latent_attn_form(const ktb200_latent_attn_params* p, int n_tokens);
+size_t ktb200_latent_attn_workspace(const ktb200_latent_attn_params* p, int n_tokens, int max_kv);
+int ktb200_latent_attn(const ktb200_latent_attn_params* p, int n_tokens, int max_kv, void* workspace, size_t workspace_bytes, void* stream);
+
 /* paged latent KV write: StaticCache.update (archive/ktransformers/models/custom_cache.py:147-200)
  * kv_cache[page_idx[t]][page_offset[t]][0:512] = ckv[t], [512:576] = k_pe[t] */
 int ktb200_mla_kv_write(void* kv_cache, int page_size, const void* ckv, const void* k_pe, const int* page_idx,

@@ -1,0 +1,454 @@
+// Latent attention of any number of new tokens a sequence over the paged latent cache (ktb200_latent_attn), bf16, latents of 512 + 64 rotated columns.
+// Two forms of one sum:
+//   expanded (portions)   latent_plan_kernel: where each portion's keys and query tiles go; latent_gather_kernel: its cache rows side by side; latent_expand_kernel: keys and values of them
+//                         (2 x 512 (N + V) operations a key and head); latent_prompt_kernel: attention with 2 (N + 64 + V) operations a pair and head
+//   absorbed (few tokens) absorb_kernel: the queries to the latents; the latent decode kernel (mla.cu), 2 (2 x 512 + 64) operations a pair and head; absorb_kernel: sums of latents to values
+// Keys and values of one call take up to kLxBytes; with more the heads go in passes.
+#include <algorithm>
+#include <type_traits>
+
+#include "latent_expand.cuh"
+#include "latent_prompt.cuh"
+#include "mla_ragged.h"
+#include "mma_tile.cuh"
+
+namespace ktb {
+
+constexpr size_t kLxBytes = (size_t)2 << 30;
+constexpr int kLatentFew = 64;      // tokens a sequence on average from which the expanded form takes less
+constexpr int kLatentStep = 4096;   // tokens that the absorbed form takes at once (their partial sums are 263 KB each with 128 heads)
+
+// ------------------------------------------------------------------------------------------------ plan and rows
+// one warp: portions in order, 32 side by side
+__global__ void __launch_bounds__(32) latent_plan_kernel(const ktb200_latent_attn_params p, int n_tokens, int row_cap, int tile_cap, long rows_of_heads, int* plan) {
+    griddep_wait();
+    griddep_launch_dependents();      // (as absorb_kernel: behind the wait)
+    const int lane = threadIdx.x;
+    int* off = plan + kPlanSeqs;
+    int4* tiles = reinterpret_cast<int4*>(plan + plan_tiles_at(p.n_seqs));
+    int rows = 0, nt = 0;
+    for (int s0 = 0; s0 < p.n_seqs; s0 += 32) {
+        const int s = s0 + lane;
+        int first = 0, count = 0, pos = 0, keys = 0;
+        if (s < p.n_seqs) {
+            first = p.seqs[s];
+            count = p.seqs[p.seqs_stride + s];
+            if (count > 0 && first >= 0 && first <= n_tokens - count) pos = p.pos[first];
+            else count = 0;
+            if (count > 0 && (pos < 0 || (unsigned)p.slot[first] >= (unsigned)p.n_slots)) count = 0;
+            keys = count > 0 ? (int)min((long)pos + count, (long)row_cap) : 0;
+        }
+        const int r = (keys + kLatentTile - 1) / kLatentTile * kLatentTile, q = (count + kPlanTokens - 1) / kPlanTokens;
+        int rs = r, qs = q;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int a = __shfl_up_sync(0xffffffffu, rs, o), b = __shfl_up_sync(0xffffffffu, qs, o);
+            if (lane >= o) { rs += a; qs += b; }
+        }
+        if (s < p.n_seqs) {
+            off[s] = rows + rs - r;
+            off[p.n_seqs + 1 + s] = keys;
+            for (int i = 0; i < q; i++) {      // the last tokens, which see most keys, first
+                const int at = nt + qs - q + i, o = (q - 1 - i) * kPlanTokens;
+                if (at < tile_cap) tiles[at] = make_int4(first + o, min(kPlanTokens, count - o), pos + o, s);
+            }
+        }
+        rows += __shfl_sync(0xffffffffu, rs, 31);
+        nt += __shfl_sync(0xffffffffu, qs, 31);
+    }
+    if (lane == 0) {
+        off[p.n_seqs] = rows;
+        plan[kPlanRows] = rows;
+        plan[kPlanHeads] = rows > 0 ? (int)min((long)p.heads, rows_of_heads / rows) : p.heads;
+        plan[kPlanTiles] = min(nt, tile_cap);
+        plan[kPlanBad] = 0;
+    }
+}
+
+// Rows side by side: 32 a CTA and step, a warp four of them.  Rows behind a portion's last key, and rows that are not there, are zeros.  A latent that holds a number that is not finite
+// becomes zeros too, and its bit is set: the rows of queries that see it are NaN, those that do not are not touched (0 x NaN).  (Without `bad` rows are copied as they are: the latent
+// decode kernel never multiplies what a token does not see)
+__global__ void __launch_bounds__(256) latent_gather_kernel(const ktb200_latent_attn_params p, int* plan, __nv_bfloat16* lat, uint32_t* bad) {
+    griddep_launch_dependents();
+    griddep_wait();
+    const int rows = plan[kPlanRows], lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int* off = plan + kPlanSeqs;
+    __shared__ uint32_t odd[8];
+    for (int r0 = blockIdx.x * 32; r0 < rows; r0 += gridDim.x * 32) {
+        int seq = -1;      // the last portion that begins at or before this row and has one
+        for (int s0 = 0; s0 < p.n_seqs; s0 += 32) {
+            const unsigned in = __ballot_sync(0xffffffffu, s0 + lane < p.n_seqs && off[s0 + lane] <= r0 && off[s0 + lane + 1] > r0);
+            if (in) { seq = s0 + __ffs(in) - 1; break; }
+        }
+        uint32_t mine = 0;
+        if (seq >= 0) {
+            const int key0 = r0 - off[seq], keys = off[p.n_seqs + 1 + seq], slot = p.slot[p.seqs[seq]];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int key = key0 + 4 * warp + i;
+                int page = -1;
+                if (key < keys) page = p.page_table[(long)slot * p.max_pages + (key / p.page_size) % p.max_pages];
+                const bool there = (unsigned)page < (unsigned)p.n_pages;
+                const uint4* src = reinterpret_cast<const uint4*>((const __nv_bfloat16*)p.cache + ((long)page * p.page_size + key % p.page_size) * kLatentRow);
+                uint4 v[3];
+                bool finite = true;
+#pragma unroll
+                for (int c = 0; c < 3; c++) {
+                    v[c] = there && lane + 32 * c < kLatentRow / 8 ? src[lane + 32 * c] : make_uint4(0, 0, 0, 0);
+                    const uint32_t w[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
+#pragma unroll
+                    for (int k = 0; k < 4; k++) finite &= c == 2 || ((w[k] & 0x7f800000u) != 0x7f800000u && (w[k] & 0x7f80u) != 0x7f80u);      // (the last are the rotated part: what it holds reaches the scores alone)
+                }
+                const bool whole = __all_sync(0xffffffffu, finite) || !bad;
+                if (!whole) mine |= 1u << (4 * warp + i);
+                uint4* dst = reinterpret_cast<uint4*>(lat + (long)(r0 + 4 * warp + i) * kLatentRow);
+#pragma unroll
+                for (int c = 0; c < 3; c++)
+                    if (lane + 32 * c < kLatentRow / 8) dst[lane + 32 * c] = whole || c == 2 ? v[c] : make_uint4(0, 0, 0, 0);
+            }
+        }
+        if (!bad) continue;
+        if (lane == 0) odd[warp] = mine;
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            uint32_t all = 0;
+#pragma unroll
+            for (int i = 0; i < 8; i++) all |= odd[i];
+            bad[r0 / 32] = all;
+            if (all) atomicOr(plan + kPlanBad, 1);
+        }
+        __syncthreads();
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ absorbed form
+// C[t][h][:] = A[t][h][:] B_h on mma tiles, fp32 sums, one rounding: a CTA has 16 or 64 tokens of one head and a block of columns, and all of its K in shared memory at once: the product is
+// bound by the weights' bytes (16.8 MB each with 128 heads), and with several CTAs an SM all of them are on their way at the start.
+//   VALUES = false: A = q_nope (K = N), B_h = W_K,h [N][512], blocks of 128 columns;  VALUES = true: A = sums of latents (K = 512), B_h = W_V,h^T, W_V,h [V][512], blocks of 32 columns
+// The first also writes where each token's keys are (`where`: position, or -1 in no portion or slot; page-table row); the second leaves rows of tokens without a position as they are.
+template <int MT, int K, bool VALUES> struct AbsorbShape {
+    static constexpr int NB = VALUES ? 32 : 128, KP = K + 8, BP = VALUES ? 512 + 8 : NB + 8;      // padded rows: neighbouring rows meet in no bank
+    static constexpr int WM = MT / 16, WN = VALUES ? (MT == 16 ? 4 : 2) : 8 / WM, WK = 8 / (WM * WN), NT = NB / 8 / WN;      // warps along tokens, columns and K; runs of 8 columns a warp
+    static constexpr int A_BYTES = MT * KP * 2, B_BYTES = (VALUES ? NB : K) * BP * 2, SMEM = A_BYTES + B_BYTES;
+    static_assert(WM * WN * WK == 8 && NT >= 1, "8 warps");
+};
+template <int MT, int K, bool VALUES> __global__ void __launch_bounds__(256) absorb_kernel(const ktb200_latent_attn_params p, const __nv_bfloat16* A, long a_stride, int a_head, int width, __nv_bfloat16* out,
+                                                                                            long out_stride, int t0, int n_tokens, int* where) {
+    using S = AbsorbShape<MT, K, VALUES>;
+    extern __shared__ __align__(16) uint8_t ab_smem[];
+    __nv_bfloat16* As = reinterpret_cast<__nv_bfloat16*>(ab_smem);
+    __nv_bfloat16* Bs = reinterpret_cast<__nv_bfloat16*>(ab_smem + S::A_BYTES);
+    const int h = blockIdx.y, n0 = blockIdx.x * S::NB, m0 = blockIdx.z * MT, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const __nv_bfloat16* B = (const __nv_bfloat16*)p.w + ((long)h * (p.nope_dim + p.vdim) + (VALUES ? p.nope_dim + n0 : 0)) * kLatent + (VALUES ? 0 : n0);
+    // the call's first kernel lets the next ones start behind its own wait, so that what was ahead of the call is complete for all of them: the last one's weights wait for nothing
+    if (VALUES) {
+        griddep_launch_dependents();
+    } else {
+        griddep_wait();
+        griddep_launch_dependents();
+    }
+    constexpr int BR = VALUES ? S::NB : K, BC = (VALUES ? kLatent : S::NB) / 8;
+    for (int i = tid; i < BR * BC; i += 256) cp_async16(Bs + (i / BC) * S::BP + (i % BC) * 8, B + (long)(i / BC) * kLatent + (i % BC) * 8, true);
+    if (VALUES) griddep_wait();
+    constexpr int AC = K / 8;
+    for (int i = tid; i < MT * AC; i += 256) {
+        const int m = i / AC;
+        const bool in = m0 + m < n_tokens;
+        cp_async16(As + m * S::KP + (i % AC) * 8, A + (long)(in ? m0 + m : 0) * a_stride + (long)h * a_head + (i % AC) * 8, in);
+    }
+    if (!VALUES && h == 0 && blockIdx.x == 0) {
+        for (int m = warp; m < MT; m += 8) {
+            const int t = t0 + m0 + m;
+            if (m0 + m >= n_tokens) break;
+            bool in = false;
+            for (int s = lane; s < p.n_seqs; s += 32) in |= t >= p.seqs[s] && t - p.seqs[s] < p.seqs[p.seqs_stride + s];
+            in = __any_sync(0xffffffffu, in) && (unsigned)p.slot[t] < (unsigned)p.n_slots && p.pos[t] >= 0;
+            if (lane == 0) {
+                where[m0 + m] = in ? p.pos[t] : -1;
+                where[kLatentStep + m0 + m] = in ? p.slot[t] : 0;
+            }
+        }
+    }
+    cp_async_wait_all();
+    __syncthreads();
+    const int wm = warp % S::WM, wn = warp / S::WM % S::WN, wk = warp / (S::WM * S::WN);
+    float acc[S::NT][4];
+#pragma unroll
+    for (int i = 0; i < S::NT; i++)
+#pragma unroll
+        for (int c = 0; c < 4; c++) acc[i][c] = 0.f;
+    constexpr int KW = K / S::WK;
+#pragma unroll 4
+    for (int k = wk * KW; k < (wk + 1) * KW; k += 16) {
+        uint32_t a[4];
+        ldmatrix_x4(a, As + (wm * 16 + (lane & 15)) * S::KP + k + (lane >> 4) * 8);
+        if (S::NT == 1) {      // (two K steps' columns in one load would need an even number of them: K is a multiple of 64)
+            uint32_t b[4];
+            ldmatrix_x4(b, Bs + (wn * 8 + (lane & 7)) * S::BP + k + (lane >> 3 & 1) * 8);
+            mma_bf16_16816(acc[0], a, b[0], b[1]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < S::NT; i += 2) {      // 16 columns at a time
+                uint32_t b[4];
+                const int c = (wn * S::NT + i) * 8;
+                if (VALUES) ldmatrix_x4(b, Bs + (c + (lane & 7) + (lane >> 4) * 8) * S::BP + k + (lane >> 3 & 1) * 8);
+                else ldmatrix_x4_trans(b, Bs + (k + (lane & 15)) * S::BP + c + (lane >> 4) * 8);
+                mma_bf16_16816(acc[i], a, b[0], b[1]);
+                mma_bf16_16816(acc[(i + 1) % S::NT], a, b[2], b[3]);
+            }
+        }
+    }
+    if (S::WK > 1) {
+        float* part = reinterpret_cast<float*>(ab_smem);      // (over the operands)
+        __syncthreads();
+        if (wk > 0)
+#pragma unroll
+            for (int i = 0; i < S::NT * 4; i++) part[((warp - S::WM * S::WN) * S::NT * 4 + i) * 32 + lane] = acc[i / 4][i % 4];
+        __syncthreads();
+        if (wk > 0) return;
+#pragma unroll
+        for (int k = 1; k < S::WK; k++)
+#pragma unroll
+            for (int i = 0; i < S::NT * 4; i++) acc[i / 4][i % 4] += part[((warp + (k - 1) * S::WM * S::WN) * S::NT * 4 + i) * 32 + lane];
+    }
+#pragma unroll
+    for (int r = 0; r < 2; r++) {
+        const int m = m0 + wm * 16 + (lane >> 2) + 8 * r;
+        if (m >= n_tokens || (VALUES && where[m] < 0)) continue;
+        __nv_bfloat16* row = out + (long)m * out_stride + (long)h * width + n0 + wn * S::NT * 8 + 2 * (lane & 3);
+#pragma unroll
+        for (int i = 0; i < S::NT; i++) {
+            if ((uintptr_t)row % 4 == 0) {
+                *reinterpret_cast<uint32_t*>(row + 8 * i) = latent_pack(acc[i][2 * r], acc[i][2 * r + 1]);
+            } else {
+                row[8 * i] = __float2bfloat16_rn(acc[i][2 * r]);
+                row[8 * i + 1] = __float2bfloat16_rn(acc[i][2 * r + 1]);
+            }
+        }
+    }
+}
+template <int MT, int K, bool VALUES> static int absorb_launch(const ktb200_latent_attn_params* p, const __nv_bfloat16* A, long a_stride, int a_head, int width, __nv_bfloat16* out, long out_stride, int t0, int n,
+                                                              int* where, cudaStream_t s) {
+    using S = AbsorbShape<MT, K, VALUES>;
+    KTB_CUDA_CHECK(raise_smem_limit((const void*)absorb_kernel<MT, K, VALUES>, S::SMEM));
+    KTB_CUDA_CHECK(launch_pdl(absorb_kernel<MT, K, VALUES>, dim3((VALUES ? p->vdim : kLatent) / S::NB, p->heads, (n + MT - 1) / MT), dim3(256), (size_t)S::SMEM, s, *p, A, a_stride, a_head, width, out, out_stride, t0,
+                              n, where));
+    count_launch();
+    return KTB200_OK;
+}
+
+// ------------------------------------------------------------------------------------------------ host
+static size_t la_up(size_t n) { return (n + 1023) / 1024 * 1024; }
+struct LatentLayout {      // of the workspace: byte offsets, and what the sizes follow from
+    int form, rows, tiles, passes, parts, part;
+    bool gathered;      // absorbed: pages that are not whole 32 rows are laid side by side first
+    size_t plan, lat, bad, kv, o_part, ml_part, where, table, q_abs, sums, partial, partial_bytes, total;
+    long rows_of_heads;      // expanded rows, one a head, that there is room for
+};
+static int latent_form(const ktb200_latent_attn_params* p, int n_tokens) {
+    if (p->form) return p->form;
+    return (long)n_tokens >= (long)kLatentFew * p->n_seqs ? 2 : 1;
+}
+static int latent_layout(LatentLayout& y, const ktb200_latent_attn_params* p, int n_tokens, int max_kv) {
+    y = LatentLayout{};
+    y.form = latent_form(p, n_tokens);
+    int device = 0;
+    KTB_CUDA_CHECK(cudaGetDevice(&device));
+    size_t at = 0;
+    auto take = [&](size_t n) { const size_t o = at; at += la_up(n); return o; };
+    const size_t H = p->heads, bn = p->nope_dim + p->vdim;
+    const long tiled = ((long)max_kv + kLatentTile - 1) / kLatentTile * kLatentTile, rows = tiled * p->n_seqs;
+    if (rows > (1L << 30)) { set_error("latent_attn: %d sequences of up to %d keys", p->n_seqs, max_kv); return KTB200_EINVAL; }
+    y.rows = (int)rows;
+    y.gathered = y.form == 1 && p->page_size % 32 != 0;
+    if (y.form == 2 || y.gathered) {
+        y.tiles = n_tokens / kPlanTokens + p->n_seqs;
+        y.plan = take((plan_tiles_at(p->n_seqs) + 4L * y.tiles) * 4);
+        y.lat = take((size_t)rows * kLatentRow * 2);
+        y.bad = take((size_t)rows / 32 * 4);
+    }
+    if (y.form == 2) {
+        const long room = (long)std::max<size_t>((size_t)rows, std::min(H * (size_t)rows, kLxBytes / (bn * 2)));
+        y.rows_of_heads = std::min(room, 0x7fffffffL);
+        const long per = y.rows_of_heads / rows;
+        y.passes = (int)((H + per - 1) / per);
+        y.kv = take((size_t)y.rows_of_heads * bn * 2);
+        // few query tiles and heads: the keys in parts of 512 and more, as many as fill the SMs
+        const long ctas = (long)y.tiles * std::min((long)H, per), sms = num_sms(device);
+        y.parts = 1;
+        if (2 * ctas <= sms && tiled > 1024) {
+            y.part = (int)std::max(512L, (tiled / (sms / ctas) + kLatentTile - 1) / kLatentTile * kLatentTile);
+            y.parts = (int)((tiled + y.part - 1) / y.part);
+            if (y.parts == 1) y.part = 0;
+        }
+        if (y.parts > 1) {
+            y.o_part = take((size_t)n_tokens * H * y.parts * p->vdim * 4);
+            y.ml_part = take((size_t)n_tokens * H * y.parts * 8);
+        }
+    } else {
+        const size_t n = std::min(n_tokens, kLatentStep);
+        y.where = take(2 * kLatentStep * 4);
+        if (y.gathered) y.table = take((size_t)p->n_seqs * (tiled / 32) * 4);
+        y.q_abs = take(n * H * kLatent * 2);
+        y.sums = take(n * H * kLatent * 2);
+        y.partial_bytes = mla_ragged_workspace((int)n, p->heads, max_kv);
+        y.partial = take(y.partial_bytes);
+    }
+    y.total = at;
+    return KTB200_OK;
+}
+static int latent_check(const ktb200_latent_attn_params* p, int max_kv) {
+    if (!p || p->heads <= 0 || p->page_size <= 0 || p->max_pages <= 0 || p->n_slots <= 0 || p->n_pages <= 0 || p->n_seqs < 0 || max_kv <= 0) { set_error("latent_attn: bad sizes"); return KTB200_EINVAL; }
+    if ((p->nope_dim != 64 && p->nope_dim != 128) || (p->vdim != 64 && p->vdim != 128)) { set_error("latent_attn: heads of %d + 64 and values of %d: 64 or 128 of each", p->nope_dim, p->vdim); return KTB200_EINVAL; }
+    if (p->form < 0 || p->form > 2) { set_error("latent_attn: form %d", p->form); return KTB200_EINVAL; }
+    if (!(p->scale > 0.f) || p->scale > 1e30f) { set_error("latent_attn: the scale has to be above zero"); return KTB200_EINVAL; }
+    if (p->q_stride < (long)p->heads * (p->nope_dim + kLatentRot) || p->out_stride < (long)p->heads * p->vdim) { set_error("latent_attn: rows overlap"); return KTB200_EINVAL; }
+    if (p->q_stride % 8) { set_error("latent_attn: rows of q have to begin at multiples of 16 bytes"); return KTB200_EINVAL; }
+    if ((long)p->n_pages * p->page_size > 0x7fffffffL) { set_error("latent_attn: %d pages of %d tokens", p->n_pages, p->page_size); return KTB200_EINVAL; }
+    return KTB200_OK;
+}
+static int latent_map(CUtensorMap* map, const void* ptr, long width, long rows, long stride, int box_rows) {      // boxes of 64 columns x box_rows, 128-byte swizzled; what is outside comes as zeros
+    const umma::EncodeTiledFn enc = umma::encode_tiled();
+    if (!enc) { set_error("latent_attn: cuTensorMapEncodeTiled is not available from this driver"); return KTB200_ECUDA; }
+    const cuuint64_t dims[2] = {(cuuint64_t)width, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)stride * 2};
+    const cuuint32_t box[2] = {64, (cuuint32_t)box_rows}, estr[2] = {1, 1};
+    const CUresult cr = enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (cr != CUDA_SUCCESS) { set_error("latent_attn: cuTensorMapEncodeTiled failed (%d)", (int)cr); return KTB200_ECUDA; }
+    return KTB200_OK;
+}
+// the plan and the rows of all portions
+static int latent_rows(const ktb200_latent_attn_params* p, const LatentLayout& y, int n_tokens, uint8_t* ws, int sms, cudaStream_t s) {
+    int* plan = (int*)(ws + y.plan);
+    KTB_CUDA_CHECK(launch_pdl(latent_plan_kernel, dim3(1), dim3(32), (size_t)0, s, *p, n_tokens, (int)(y.rows / p->n_seqs), y.tiles, y.rows_of_heads, plan));
+    KTB_CUDA_CHECK(launch_pdl(latent_gather_kernel, dim3(std::min(y.rows / 32, 8 * sms)), dim3(256), (size_t)0, s, *p, plan, (__nv_bfloat16*)(ws + y.lat), y.form == 2 ? (uint32_t*)(ws + y.bad) : nullptr));
+    count_launch(2);
+    return KTB200_OK;
+}
+template <int N, int V> static int latent_expanded(const ktb200_latent_attn_params* p, const LatentLayout& y, int n_tokens, uint8_t* ws, int sms, cudaStream_t s) {
+    constexpr int BN = N + V;
+    const int rc = latent_rows(p, y, n_tokens, ws, sms, s);
+    if (rc) return rc;
+    CUtensorMap lat, w;
+    LpMaps m;
+    const __nv_bfloat16 *rows = (const __nv_bfloat16*)(ws + y.lat), *kv = (const __nv_bfloat16*)(ws + y.kv);
+    int e = latent_map(&lat, rows, kLatentRow, y.rows, kLatentRow, 128);
+    if (!e) e = latent_map(&w, p->w, kLatent, (long)p->heads * BN, kLatent, BN / 2);
+    if (!e) e = latent_map(&m.q, p->q, (long)p->heads * (N + kLatentRot), n_tokens, p->q_stride, 128);
+    if (!e) e = latent_map(&m.q_rot, p->q_rot, (long)p->heads * kLatentRot, n_tokens, (long)p->heads * kLatentRot, 128);
+    if (!e) e = latent_map(&m.k, kv, BN, y.rows_of_heads, BN, 128);
+    if (!e) e = latent_map(&m.v, kv, BN, y.rows_of_heads, BN, 64);
+    if (e) return e;
+    m.k_rot = lat;
+    KTB_CUDA_CHECK(raise_smem_limit((const void*)latent_expand_kernel, kLxSmem));
+    KTB_CUDA_CHECK(raise_smem_limit((const void*)latent_prompt_kernel<N, V>, kLpSmem));
+    const int pairs = sms / 2, mt = (y.rows + 255) / 256;
+    const int ctas = (int)std::min<long>((long)y.tiles * p->heads, 0x7fffffffL);
+    LatentPrompt a{(const int*)(ws + y.plan), (const uint32_t*)(ws + y.bad), p->n_seqs, p->heads, 0, y.parts > 1 ? y.part : 0, y.parts, p->scale * 1.4426950408889634f, (__nv_bfloat16*)p->out, p->out_stride,
+                   (float*)(ws + y.o_part), (float*)(ws + y.ml_part)};
+    for (a.pass = 0; a.pass < y.passes; a.pass++) {
+        KTB_CUDA_CHECK(launch_pdl(latent_expand_kernel, dim3((unsigned)(2 * std::min<long>((long)mt * p->heads, pairs))), dim3(kLxThreads), (size_t)kLxSmem, s, lat, w, a.plan, (__nv_bfloat16*)(ws + y.kv), BN,
+                                  p->heads, a.pass));
+        KTB_CUDA_CHECK(launch_pdl(latent_prompt_kernel<N, V>, dim3(ctas, 1, y.parts), dim3(kLpThreads), (size_t)kLpSmem, s, m, a));
+        count_launch(2);
+        if (y.parts > 1) {
+            KTB_CUDA_CHECK(launch_pdl(latent_merge_kernel<V>, dim3(y.tiles, p->heads, 4), dim3(256), (size_t)0, s, a));
+            count_launch();
+        }
+    }
+    return KTB200_OK;
+}
+// the page table of rows laid side by side: pages of 32
+__global__ void __launch_bounds__(256) latent_table_kernel(const int* plan, int n_seqs, int width, int* table) {
+    griddep_launch_dependents();
+    griddep_wait();
+    const int s = blockIdx.y, i = blockIdx.x * 256 + threadIdx.x, first = plan[kPlanSeqs + s] / 32;
+    if (i < width) table[(long)s * width + i] = first + min(i, max(0, (plan[kPlanSeqs + s + 1] / 32 - first) - 1));
+}
+// a token's row in that table: its portion
+__global__ void __launch_bounds__(256) latent_portion_kernel(const ktb200_latent_attn_params p, int t0, int n, int* where) {
+    griddep_launch_dependents();
+    griddep_wait();
+    const int m = blockIdx.x * 256 + threadIdx.x, t = t0 + m;
+    if (m >= n) return;
+    int row = 0;
+    for (int s = 0; s < p.n_seqs; s++)
+        if (t >= p.seqs[s] && t - p.seqs[s] < p.seqs[p.seqs_stride + s]) { row = s; break; }
+    where[kLatentStep + m] = row;
+}
+template <int N, int V> static int latent_absorbed(const ktb200_latent_attn_params* p, const LatentLayout& y, int n_tokens, int max_kv, uint8_t* ws, int sms, cudaStream_t s) {
+    int* where = (int*)(ws + y.where);      // positions, then page-table rows
+    __nv_bfloat16 *q_abs = (__nv_bfloat16*)(ws + y.q_abs), *sums = (__nv_bfloat16*)(ws + y.sums);
+    const void* cache = p->cache;
+    long cache_rows = (long)p->n_pages * p->page_size;
+    const int* table = p->page_table;
+    int max_pages = p->max_pages, page_size = p->page_size;
+    if (y.gathered) {
+        int rc = latent_rows(p, y, n_tokens, ws, sms, s);
+        if (rc) return rc;
+        max_pages = y.rows / p->n_seqs / 32;
+        KTB_CUDA_CHECK(launch_pdl(latent_table_kernel, dim3((max_pages + 255) / 256, p->n_seqs), dim3(256), (size_t)0, s, (const int*)(ws + y.plan), p->n_seqs, max_pages, (int*)(ws + y.table)));
+        count_launch();
+        cache = ws + y.lat; cache_rows = y.rows; table = (const int*)(ws + y.table); page_size = 32;
+    }
+    for (int t0 = 0; t0 < n_tokens; t0 += kLatentStep) {
+        const int n = std::min(kLatentStep, n_tokens - t0);
+        const __nv_bfloat16* q = (const __nv_bfloat16*)p->q + (long)t0 * p->q_stride;
+        const __nv_bfloat16* q_rot = (const __nv_bfloat16*)p->q_rot + (long)t0 * p->heads * kLatentRot;
+        __nv_bfloat16* out = (__nv_bfloat16*)p->out + (long)t0 * p->out_stride;
+        const long wide = (long)p->heads * kLatent;
+        int rc = n <= 16 ? absorb_launch<16, N, false>(p, q, p->q_stride, N + kLatentRot, kLatent, q_abs, wide, t0, n, where, s)
+                         : absorb_launch<64, N, false>(p, q, p->q_stride, N + kLatentRot, kLatent, q_abs, wide, t0, n, where, s);
+        if (rc) return rc;
+        if (y.gathered) {
+            KTB_CUDA_CHECK(launch_pdl(latent_portion_kernel, dim3((n + 255) / 256), dim3(256), (size_t)0, s, *p, t0, n, where));
+            count_launch();
+        }
+        rc = mla_ragged(q_abs, q_rot, p->heads, p->scale, where, where + kLatentStep, table, max_pages, page_size, cache, cache_rows, sums, n, max_kv, ws + y.partial, y.partial_bytes, s);
+        if (rc) return rc;
+        rc = n <= 16 ? absorb_launch<16, kLatent, true>(p, sums, wide, kLatent, V, out, p->out_stride, t0, n, where, s)
+                     : absorb_launch<64, kLatent, true>(p, sums, wide, kLatent, V, out, p->out_stride, t0, n, where, s);
+        if (rc) return rc;
+    }
+    return KTB200_OK;
+}
+
+}  // namespace ktb
+
+using namespace ktb;
+
+extern "C" {
+
+int ktb200_latent_attn_form(const ktb200_latent_attn_params* p, int n_tokens) { return p ? latent_form(p, n_tokens) : 0; }
+
+size_t ktb200_latent_attn_workspace(const ktb200_latent_attn_params* p, int n_tokens, int max_kv) {
+    LatentLayout y;
+    if (latent_check(p, max_kv) || n_tokens <= 0 || p->n_seqs == 0 || latent_layout(y, p, n_tokens, max_kv)) return 0;
+    return y.total;
+}
+
+int ktb200_latent_attn(const ktb200_latent_attn_params* p, int n_tokens, int max_kv, void* workspace, size_t workspace_bytes, void* stream) {
+    int rc = latent_check(p, max_kv);
+    if (rc) return rc;
+    if (n_tokens <= 0 || p->n_seqs == 0) return KTB200_OK;
+    if (!p->q || !p->q_rot || !p->w || !p->pos || !p->slot || !p->seqs || !p->page_table || !p->cache || !p->out) { set_error("latent_attn: null pointer"); return KTB200_EINVAL; }
+    if (((uintptr_t)p->q | (uintptr_t)p->q_rot | (uintptr_t)p->w | (uintptr_t)p->cache) & 15) { set_error("latent_attn: q, q_rot, w and the cache have to be 16-byte aligned"); return KTB200_EINVAL; }
+    LatentLayout y;
+    if ((rc = latent_layout(y, p, n_tokens, max_kv))) return rc;
+    if (!workspace || ((uintptr_t)workspace & 1023) || workspace_bytes < y.total) { set_error("latent_attn: workspace of %zu bytes, 1024-byte aligned; %zu are needed", workspace_bytes, y.total); return KTB200_EINVAL; }
+    int device = 0;
+    KTB_CUDA_CHECK(cudaGetDevice(&device));
+    const int sms = num_sms(device);
+    uint8_t* ws = (uint8_t*)workspace;
+    const cudaStream_t s = (cudaStream_t)stream;
+    auto call = [&](auto n, auto v) {
+        constexpr int N = decltype(n)::value, V = decltype(v)::value;
+        return y.form == 2 ? latent_expanded<N, V>(p, y, n_tokens, ws, sms, s) : latent_absorbed<N, V>(p, y, n_tokens, max_kv, ws, sms, s);
+    };
+    using C64 = std::integral_constant<int, 64>;
+    using C128 = std::integral_constant<int, 128>;
+    if (p->nope_dim == 128) return p->vdim == 128 ? call(C128(), C128()) : call(C128(), C64());
+    return p->vdim == 128 ? call(C64(), C128()) : call(C64(), C64());
+}
+
+}  // extern "C"

@@ -127,6 +127,25 @@ def _fields(text):
     return [(n, kinds[k]) for k, names in (part.split(":") for part in text.split()) for n in names.split(",")]
 
 
+class LatentAppendParams(C.Structure):
+    """ktb200_latent_append_params (include/ktb200.h)"""
+    _fields_ = _fields("p:q l:q_stride i:heads,nope_dim p:kva l:kva_stride i:kv_rank,rot_dim p:norm_weight f:eps i:rot_dims,rot_layout,rot_split f:rot_gain p:inv_freq,angle_pos,pos,slot,seqs "
+                       "i:seqs_stride,n_seqs p:page_table i:n_slots,max_pages,page_size,n_pages p:cache,q_rot")
+
+
+class LatentAttnParams(C.Structure):
+    """ktb200_latent_attn_params (include/ktb200.h)"""
+    _fields_ = _fields("p:q l:q_stride p:q_rot i:heads,nope_dim,vdim p:w f:scale i:form p:pos,slot,seqs i:seqs_stride,n_seqs p:page_table i:n_slots,max_pages,page_size,n_pages p:cache,out l:out_stride")
+
+
+SYMBOLS |= {
+    "ktb200_latent_append": (_I, [C.POINTER(LatentAppendParams), _I, _VP]),
+    "ktb200_latent_attn_form": (_I, [C.POINTER(LatentAttnParams), _I]),
+    "ktb200_latent_attn_workspace": (C.c_size_t, [C.POINTER(LatentAttnParams), _I, _I]),
+    "ktb200_latent_attn": (_I, [C.POINTER(LatentAttnParams), _I, _I, _VP, C.c_size_t, _VP]),
+}
+
+
 class QkvPrepParams(C.Structure):
     """ktb200_qkv_prep_params (include/ktb200.h)"""
     _fields_ = _fields("p:proj l:proj_stride i:q_off,k_off,v_off,heads,kv_heads,maps,dim,vdim,rot_dims,rot_layout p:inv_freq i:qk_norm p:q_weight,k_weight i:v_unit_rms f:eps "
