@@ -2,21 +2,21 @@
 // Two forms of one sum:
 //   expanded (portions)   latent_plan_kernel: where each portion's keys and query tiles go; latent_gather_kernel: its cache rows side by side; latent_expand_kernel: keys and values of them
 //                         (2 x 512 (N + V) operations a key and head); latent_prompt_kernel: attention with 2 (N + 64 + V) operations a pair and head
-//   absorbed (few tokens) absorb_kernel: the queries to the latents; the latent decode kernel (mla.cu), 2 (2 x 512 + 64) operations a pair and head; absorb_kernel: sums of latents to values
+//   absorbed (few tokens) latent_few_prep_kernel: blocks of rows and their keys in one line; absorb_kernel: the queries to the latents; latent_few_kernel: attention with 2 (2 x 512 + 64)
+//                         operations a pair and head, latent_few_merge_kernel; absorb_kernel: sums of latents to values
 // Keys and values of one call take up to kLxBytes; with more the heads go in passes.
 #include <algorithm>
 #include <type_traits>
 
 #include "latent_expand.cuh"
+#include "latent_few.cuh"
 #include "latent_prompt.cuh"
-#include "mla_ragged.h"
 #include "mma_tile.cuh"
 
 namespace ktb {
 
 constexpr size_t kLxBytes = (size_t)2 << 30;
 constexpr int kLatentFew = 64;      // tokens a sequence on average from which the expanded form takes less
-constexpr int kLatentStep = 4096;   // tokens that the absorbed form takes at once (their partial sums are 263 KB each with 128 heads)
 
 // ------------------------------------------------------------------------------------------------ plan and rows
 // one warp: portions in order, 32 side by side
@@ -65,9 +65,7 @@ __global__ void __launch_bounds__(32) latent_plan_kernel(const ktb200_latent_att
     }
 }
 
-// Rows side by side: 32 a CTA and step, a warp four of them.  Rows behind a portion's last key, and rows that are not there, are zeros.  A latent that holds a number that is not finite
-// becomes zeros too, and its bit is set: the rows of queries that see it are NaN, those that do not are not touched (0 x NaN).  (Without `bad` rows are copied as they are: the latent
-// decode kernel never multiplies what a token does not see)
+// Rows side by side: 32 a CTA and step, a warp four of them.  Rows behind a portion's last key, and rows that are not there, are zeros, and latents that are not finite (latent_copy_row)
 __global__ void __launch_bounds__(256) latent_gather_kernel(const ktb200_latent_attn_params p, int* plan, __nv_bfloat16* lat, uint32_t* bad) {
     griddep_launch_dependents();
     griddep_wait();
@@ -89,25 +87,9 @@ __global__ void __launch_bounds__(256) latent_gather_kernel(const ktb200_latent_
                 int page = -1;
                 if (key < keys) page = p.page_table[(long)slot * p.max_pages + (key / p.page_size) % p.max_pages];
                 const bool there = (unsigned)page < (unsigned)p.n_pages;
-                const uint4* src = reinterpret_cast<const uint4*>((const __nv_bfloat16*)p.cache + ((long)page * p.page_size + key % p.page_size) * kLatentRow);
-                uint4 v[3];
-                bool finite = true;
-#pragma unroll
-                for (int c = 0; c < 3; c++) {
-                    v[c] = there && lane + 32 * c < kLatentRow / 8 ? src[lane + 32 * c] : make_uint4(0, 0, 0, 0);
-                    const uint32_t w[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
-#pragma unroll
-                    for (int k = 0; k < 4; k++) finite &= c == 2 || ((w[k] & 0x7f800000u) != 0x7f800000u && (w[k] & 0x7f80u) != 0x7f80u);      // (the last are the rotated part: what it holds reaches the scores alone)
-                }
-                const bool whole = __all_sync(0xffffffffu, finite) || !bad;
-                if (!whole) mine |= 1u << (4 * warp + i);
-                uint4* dst = reinterpret_cast<uint4*>(lat + (long)(r0 + 4 * warp + i) * kLatentRow);
-#pragma unroll
-                for (int c = 0; c < 3; c++)
-                    if (lane + 32 * c < kLatentRow / 8) dst[lane + 32 * c] = whole || c == 2 ? v[c] : make_uint4(0, 0, 0, 0);
+                if (latent_copy_row((const __nv_bfloat16*)p.cache + ((long)page * p.page_size + key % p.page_size) * kLatentRow, there, lat + (long)(r0 + 4 * warp + i) * kLatentRow, true)) mine |= 1u << (4 * warp + i);
             }
         }
-        if (!bad) continue;
         if (lane == 0) odd[warp] = mine;
         __syncthreads();
         if (threadIdx.x == 0) {
@@ -125,7 +107,7 @@ __global__ void __launch_bounds__(256) latent_gather_kernel(const ktb200_latent_
 // C[t][h][:] = A[t][h][:] B_h on mma tiles, fp32 sums, one rounding: a CTA has 16 or 64 tokens of one head and a block of columns, and all of its K in shared memory at once: the product is
 // bound by the weights' bytes (16.8 MB each with 128 heads), and with several CTAs an SM all of them are on their way at the start.
 //   VALUES = false: A = q_nope (K = N), B_h = W_K,h [N][512], blocks of 128 columns;  VALUES = true: A = sums of latents (K = 512), B_h = W_V,h^T, W_V,h [V][512], blocks of 32 columns
-// The first also writes where each token's keys are (`where`: position, or -1 in no portion or slot; page-table row); the second leaves rows of tokens without a position as they are.
+// The first also writes which tokens there are (`there`: in a portion, with a position and a slot); the second leaves the rows of others as they are.
 template <int MT, int K, bool VALUES> struct AbsorbShape {
     static constexpr int NB = VALUES ? 32 : 128, KP = K + 8, BP = VALUES ? 512 + 8 : NB + 8;      // padded rows: neighbouring rows meet in no bank
     static constexpr int WM = MT / 16, WN = VALUES ? (MT == 16 ? 4 : 2) : 8 / WM, WK = 8 / (WM * WN), NT = NB / 8 / WN;      // warps along tokens, columns and K; runs of 8 columns a warp
@@ -133,23 +115,17 @@ template <int MT, int K, bool VALUES> struct AbsorbShape {
     static_assert(WM * WN * WK == 8 && NT >= 1, "8 warps");
 };
 template <int MT, int K, bool VALUES> __global__ void __launch_bounds__(256) absorb_kernel(const ktb200_latent_attn_params p, const __nv_bfloat16* A, long a_stride, int a_head, int width, __nv_bfloat16* out,
-                                                                                            long out_stride, int t0, int n_tokens, int* where) {
+                                                                                            long out_stride, int n_tokens, int* there) {
     using S = AbsorbShape<MT, K, VALUES>;
     extern __shared__ __align__(16) uint8_t ab_smem[];
     __nv_bfloat16* As = reinterpret_cast<__nv_bfloat16*>(ab_smem);
     __nv_bfloat16* Bs = reinterpret_cast<__nv_bfloat16*>(ab_smem + S::A_BYTES);
     const int h = blockIdx.y, n0 = blockIdx.x * S::NB, m0 = blockIdx.z * MT, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const __nv_bfloat16* B = (const __nv_bfloat16*)p.w + ((long)h * (p.nope_dim + p.vdim) + (VALUES ? p.nope_dim + n0 : 0)) * kLatent + (VALUES ? 0 : n0);
-    // the call's first kernel lets the next ones start behind its own wait, so that what was ahead of the call is complete for all of them: the last one's weights wait for nothing
-    if (VALUES) {
-        griddep_launch_dependents();
-    } else {
-        griddep_wait();
-        griddep_launch_dependents();
-    }
+    griddep_launch_dependents();
     constexpr int BR = VALUES ? S::NB : K, BC = (VALUES ? kLatent : S::NB) / 8;
-    for (int i = tid; i < BR * BC; i += 256) cp_async16(Bs + (i / BC) * S::BP + (i % BC) * 8, B + (long)(i / BC) * kLatent + (i % BC) * 8, true);
-    if (VALUES) griddep_wait();
+    for (int i = tid; i < BR * BC; i += 256) cp_async16(Bs + (i / BC) * S::BP + (i % BC) * 8, B + (long)(i / BC) * kLatent + (i % BC) * 8, true);      // (the call's first kernel lets the next ones start behind its own wait: what was ahead of the call is complete)
+    griddep_wait();
     constexpr int AC = K / 8;
     for (int i = tid; i < MT * AC; i += 256) {
         const int m = i / AC;
@@ -158,15 +134,12 @@ template <int MT, int K, bool VALUES> __global__ void __launch_bounds__(256) abs
     }
     if (!VALUES && h == 0 && blockIdx.x == 0) {
         for (int m = warp; m < MT; m += 8) {
-            const int t = t0 + m0 + m;
-            if (m0 + m >= n_tokens) break;
+            const int t = m0 + m;
+            if (t >= n_tokens) break;
             bool in = false;
             for (int s = lane; s < p.n_seqs; s += 32) in |= t >= p.seqs[s] && t - p.seqs[s] < p.seqs[p.seqs_stride + s];
             in = __any_sync(0xffffffffu, in) && (unsigned)p.slot[t] < (unsigned)p.n_slots && p.pos[t] >= 0;
-            if (lane == 0) {
-                where[m0 + m] = in ? p.pos[t] : -1;
-                where[kLatentStep + m0 + m] = in ? p.slot[t] : 0;
-            }
+            if (lane == 0) there[t] = in;
         }
     }
     cp_async_wait_all();
@@ -214,7 +187,7 @@ template <int MT, int K, bool VALUES> __global__ void __launch_bounds__(256) abs
 #pragma unroll
     for (int r = 0; r < 2; r++) {
         const int m = m0 + wm * 16 + (lane >> 2) + 8 * r;
-        if (m >= n_tokens || (VALUES && where[m] < 0)) continue;
+        if (m >= n_tokens || (VALUES && !there[m])) continue;
         __nv_bfloat16* row = out + (long)m * out_stride + (long)h * width + n0 + wn * S::NT * 8 + 2 * (lane & 3);
 #pragma unroll
         for (int i = 0; i < S::NT; i++) {
@@ -227,12 +200,10 @@ template <int MT, int K, bool VALUES> __global__ void __launch_bounds__(256) abs
         }
     }
 }
-template <int MT, int K, bool VALUES> static int absorb_launch(const ktb200_latent_attn_params* p, const __nv_bfloat16* A, long a_stride, int a_head, int width, __nv_bfloat16* out, long out_stride, int t0, int n,
-                                                              int* where, cudaStream_t s) {
+template <int MT, int K, bool VALUES> static int absorb_launch(const ktb200_latent_attn_params* p, const __nv_bfloat16* A, long a_stride, int a_head, int width, __nv_bfloat16* out, long out_stride, int n, int* there, cudaStream_t s) {
     using S = AbsorbShape<MT, K, VALUES>;
     KTB_CUDA_CHECK(raise_smem_limit((const void*)absorb_kernel<MT, K, VALUES>, S::SMEM));
-    KTB_CUDA_CHECK(launch_pdl(absorb_kernel<MT, K, VALUES>, dim3((VALUES ? p->vdim : kLatent) / S::NB, p->heads, (n + MT - 1) / MT), dim3(256), (size_t)S::SMEM, s, *p, A, a_stride, a_head, width, out, out_stride, t0,
-                              n, where));
+    KTB_CUDA_CHECK(launch_pdl(absorb_kernel<MT, K, VALUES>, dim3((VALUES ? p->vdim : kLatent) / S::NB, p->heads, (n + MT - 1) / MT), dim3(256), (size_t)S::SMEM, s, *p, A, a_stride, a_head, width, out, out_stride, n, there));
     count_launch();
     return KTB200_OK;
 }
@@ -240,9 +211,9 @@ template <int MT, int K, bool VALUES> static int absorb_launch(const ktb200_late
 // ------------------------------------------------------------------------------------------------ host
 static size_t la_up(size_t n) { return (n + 1023) / 1024 * 1024; }
 struct LatentLayout {      // of the workspace: byte offsets, and what the sizes follow from
-    int form, rows, tiles, passes, parts, part;
+    int form, rows, tiles, passes, parts, part, pairs, blocks, tail_tiles;
     bool gathered;      // absorbed: pages that are not whole 32 rows are laid side by side first
-    size_t plan, lat, bad, kv, o_part, ml_part, where, table, q_abs, sums, partial, partial_bytes, total;
+    size_t plan, lat, bad, kv, o_part, ml_part, few, there, tails, tail_bad, q_abs, sums, total;
     long rows_of_heads;      // expanded rows, one a head, that there is room for
 };
 static int latent_form(const ktb200_latent_attn_params* p, int n_tokens) {
@@ -286,13 +257,20 @@ static int latent_layout(LatentLayout& y, const ktb200_latent_attn_params* p, in
             y.ml_part = take((size_t)n_tokens * H * y.parts * 8);
         }
     } else {
-        const size_t n = std::min(n_tokens, kLatentStep);
-        y.where = take(2 * kLatentStep * 4);
-        if (y.gathered) y.table = take((size_t)p->n_seqs * (tiled / 32) * 4);
-        y.q_abs = take(n * H * kLatent * 2);
-        y.sums = take(n * H * kLatent * 2);
-        y.partial_bytes = mla_ragged_workspace((int)n, p->heads, max_kv);
-        y.partial = take(y.partial_bytes);
+        if ((long)n_tokens * p->heads > (1L << 30)) { set_error("latent_attn: %d tokens of %d heads", n_tokens, p->heads); return KTB200_EINVAL; }
+        y.pairs = num_sms(device) / 2;
+        y.blocks = (int)((long)n_tokens * p->heads / kFewRows + p->n_seqs);
+        y.few = take((few_blocks_at(y.pairs) + (long)y.blocks * (sizeof(FewBlock) / 4)) * 4);
+        y.there = take((size_t)n_tokens * 4);
+        if (!y.gathered) {
+            y.tail_tiles = n_tokens / kFewTile + 2 * p->n_seqs;
+            y.tails = take((size_t)y.tail_tiles * kFewTile * kLatentRow * 2);
+            y.tail_bad = take((size_t)y.tail_tiles * kFewTile / 8);
+        }
+        y.q_abs = take((size_t)n_tokens * H * kLatent * 2);
+        y.sums = take((size_t)n_tokens * H * kLatent * 2);
+        y.o_part = take((size_t)2 * y.pairs * kFewRows * kLatent * 4);
+        y.ml_part = take((size_t)2 * y.pairs * kFewRows * 8);
     }
     y.total = at;
     return KTB200_OK;
@@ -321,7 +299,7 @@ static int latent_map(CUtensorMap* map, const void* ptr, long width, long rows, 
 static int latent_rows(const ktb200_latent_attn_params* p, const LatentLayout& y, int n_tokens, uint8_t* ws, int sms, cudaStream_t s) {
     int* plan = (int*)(ws + y.plan);
     KTB_CUDA_CHECK(launch_pdl(latent_plan_kernel, dim3(1), dim3(32), (size_t)0, s, *p, n_tokens, (int)(y.rows / p->n_seqs), y.tiles, y.rows_of_heads, plan));
-    KTB_CUDA_CHECK(launch_pdl(latent_gather_kernel, dim3(std::min(y.rows / 32, 8 * sms)), dim3(256), (size_t)0, s, *p, plan, (__nv_bfloat16*)(ws + y.lat), y.form == 2 ? (uint32_t*)(ws + y.bad) : nullptr));
+    KTB_CUDA_CHECK(launch_pdl(latent_gather_kernel, dim3(std::min(y.rows / 32, 8 * sms)), dim3(256), (size_t)0, s, *p, plan, (__nv_bfloat16*)(ws + y.lat), (uint32_t*)(ws + y.bad)));
     count_launch(2);
     return KTB200_OK;
 }
@@ -358,59 +336,35 @@ template <int N, int V> static int latent_expanded(const ktb200_latent_attn_para
     }
     return KTB200_OK;
 }
-// the page table of rows laid side by side: pages of 32
-__global__ void __launch_bounds__(256) latent_table_kernel(const int* plan, int n_seqs, int width, int* table) {
-    griddep_launch_dependents();
-    griddep_wait();
-    const int s = blockIdx.y, i = blockIdx.x * 256 + threadIdx.x, first = plan[kPlanSeqs + s] / 32;
-    if (i < width) table[(long)s * width + i] = first + min(i, max(0, (plan[kPlanSeqs + s + 1] / 32 - first) - 1));
-}
-// a token's row in that table: its portion
-__global__ void __launch_bounds__(256) latent_portion_kernel(const ktb200_latent_attn_params p, int t0, int n, int* where) {
-    griddep_launch_dependents();
-    griddep_wait();
-    const int m = blockIdx.x * 256 + threadIdx.x, t = t0 + m;
-    if (m >= n) return;
-    int row = 0;
-    for (int s = 0; s < p.n_seqs; s++)
-        if (t >= p.seqs[s] && t - p.seqs[s] < p.seqs[p.seqs_stride + s]) { row = s; break; }
-    where[kLatentStep + m] = row;
-}
-template <int N, int V> static int latent_absorbed(const ktb200_latent_attn_params* p, const LatentLayout& y, int n_tokens, int max_kv, uint8_t* ws, int sms, cudaStream_t s) {
-    int* where = (int*)(ws + y.where);      // positions, then page-table rows
-    __nv_bfloat16 *q_abs = (__nv_bfloat16*)(ws + y.q_abs), *sums = (__nv_bfloat16*)(ws + y.sums);
-    const void* cache = p->cache;
-    long cache_rows = (long)p->n_pages * p->page_size;
-    const int* table = p->page_table;
-    int max_pages = p->max_pages, page_size = p->page_size;
+template <int N, int V> static int latent_absorbed(const ktb200_latent_attn_params* p, const LatentLayout& y, int n_tokens, uint8_t* ws, int sms, cudaStream_t s) {
     if (y.gathered) {
-        int rc = latent_rows(p, y, n_tokens, ws, sms, s);
-        if (rc) return rc;
-        max_pages = y.rows / p->n_seqs / 32;
-        KTB_CUDA_CHECK(launch_pdl(latent_table_kernel, dim3((max_pages + 255) / 256, p->n_seqs), dim3(256), (size_t)0, s, (const int*)(ws + y.plan), p->n_seqs, max_pages, (int*)(ws + y.table)));
-        count_launch();
-        cache = ws + y.lat; cache_rows = y.rows; table = (const int*)(ws + y.table); page_size = 32;
-    }
-    for (int t0 = 0; t0 < n_tokens; t0 += kLatentStep) {
-        const int n = std::min(kLatentStep, n_tokens - t0);
-        const __nv_bfloat16* q = (const __nv_bfloat16*)p->q + (long)t0 * p->q_stride;
-        const __nv_bfloat16* q_rot = (const __nv_bfloat16*)p->q_rot + (long)t0 * p->heads * kLatentRot;
-        __nv_bfloat16* out = (__nv_bfloat16*)p->out + (long)t0 * p->out_stride;
-        const long wide = (long)p->heads * kLatent;
-        int rc = n <= 16 ? absorb_launch<16, N, false>(p, q, p->q_stride, N + kLatentRot, kLatent, q_abs, wide, t0, n, where, s)
-                         : absorb_launch<64, N, false>(p, q, p->q_stride, N + kLatentRot, kLatent, q_abs, wide, t0, n, where, s);
-        if (rc) return rc;
-        if (y.gathered) {
-            KTB_CUDA_CHECK(launch_pdl(latent_portion_kernel, dim3((n + 255) / 256), dim3(256), (size_t)0, s, *p, t0, n, where));
-            count_launch();
-        }
-        rc = mla_ragged(q_abs, q_rot, p->heads, p->scale, where, where + kLatentStep, table, max_pages, page_size, cache, cache_rows, sums, n, max_kv, ws + y.partial, y.partial_bytes, s);
-        if (rc) return rc;
-        rc = n <= 16 ? absorb_launch<16, kLatent, true>(p, sums, wide, kLatent, V, out, p->out_stride, t0, n, where, s)
-                     : absorb_launch<64, kLatent, true>(p, sums, wide, kLatent, V, out, p->out_stride, t0, n, where, s);
+        const int rc = latent_rows(p, y, n_tokens, ws, sms, s);
         if (rc) return rc;
     }
-    return KTB200_OK;
+    __nv_bfloat16 *q_abs = (__nv_bfloat16*)(ws + y.q_abs), *tails = (__nv_bfloat16*)(ws + y.tails);
+    int* there = (int*)(ws + y.there);
+    const long rows = (long)n_tokens * p->heads, wide = (long)p->heads * kLatent;
+    LatentFew a{*p, (int*)(ws + y.few), n_tokens, y.blocks, y.gathered ? 0x7fffffff : y.tail_tiles, y.pairs, p->page_size % 64 && !y.gathered ? 32 : 64, y.gathered ? (const int*)(ws + y.plan) : nullptr,
+                (const uint32_t*)(ws + y.bad), (const uint32_t*)(ws + y.tail_bad), p->scale * 1.4426950408889634f, (__nv_bfloat16*)(ws + y.sums), (float*)(ws + y.o_part), (float*)(ws + y.ml_part)};
+    FewMaps m;
+    int e = latent_map(&m.q, q_abs, kLatent, rows, kLatent, 64);
+    if (!e) e = latent_map(&m.q_rot, p->q_rot, kLatentRot, rows, kLatentRot, 64);
+    if (!e) e = y.gathered ? latent_map(&m.rows, ws + y.lat, kLatentRow, y.rows, kLatentRow, a.box) : latent_map(&m.rows, p->cache, kLatentRow, (long)p->n_pages * p->page_size, kLatentRow, a.box);
+    if (!e) e = y.gathered ? latent_map(&m.tails, ws + y.lat, kLatentRow, y.rows, kLatentRow, a.box) : latent_map(&m.tails, tails, kLatentRow, (long)y.tail_tiles * kFewTile, kLatentRow, a.box);
+    if (e) return e;
+    KTB_CUDA_CHECK(launch_pdl(latent_few_prep_kernel, dim3(1 + (y.gathered ? 0 : 4 * y.tail_tiles)), dim3(256), (size_t)0, s, a, tails, (uint32_t*)(ws + y.tail_bad)));
+    count_launch();
+    const __nv_bfloat16* q = (const __nv_bfloat16*)p->q;
+    int rc = n_tokens <= 16 ? absorb_launch<16, N, false>(p, q, p->q_stride, N + kLatentRot, kLatent, q_abs, wide, n_tokens, there, s)
+                            : absorb_launch<64, N, false>(p, q, p->q_stride, N + kLatentRot, kLatent, q_abs, wide, n_tokens, there, s);
+    if (rc) return rc;
+    KTB_CUDA_CHECK(raise_smem_limit((const void*)latent_few_kernel, kFewSmem));
+    KTB_CUDA_CHECK(launch_pdl(latent_few_kernel, dim3(2 * y.pairs), dim3(kFewThreads), (size_t)kFewSmem, s, m, a));
+    KTB_CUDA_CHECK(launch_pdl(latent_few_merge_kernel, dim3(y.blocks, kFewRows / 8), dim3(256), (size_t)0, s, a));
+    count_launch(2);
+    __nv_bfloat16* out = (__nv_bfloat16*)p->out;
+    return n_tokens <= 16 ? absorb_launch<16, kLatent, true>(p, a.sums, wide, kLatent, V, out, p->out_stride, n_tokens, there, s)
+                          : absorb_launch<64, kLatent, true>(p, a.sums, wide, kLatent, V, out, p->out_stride, n_tokens, there, s);
 }
 
 }  // namespace ktb
@@ -443,7 +397,7 @@ int ktb200_latent_attn(const ktb200_latent_attn_params* p, int n_tokens, int max
     const cudaStream_t s = (cudaStream_t)stream;
     auto call = [&](auto n, auto v) {
         constexpr int N = decltype(n)::value, V = decltype(v)::value;
-        return y.form == 2 ? latent_expanded<N, V>(p, y, n_tokens, ws, sms, s) : latent_absorbed<N, V>(p, y, n_tokens, max_kv, ws, sms, s);
+        return y.form == 2 ? latent_expanded<N, V>(p, y, n_tokens, ws, sms, s) : latent_absorbed<N, V>(p, y, n_tokens, ws, sms, s);
     };
     using C64 = std::integral_constant<int, 64>;
     using C128 = std::integral_constant<int, 128>;

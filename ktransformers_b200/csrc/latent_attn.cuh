@@ -18,6 +18,29 @@ __device__ __forceinline__ uint32_t latent_pack(float lo, float hi) {
     const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&v);
 }
+// A warp copies one cache row, or zeros where it is not there.  With `clean` a latent that holds a number that is not finite becomes zeros, and the answer is true: whoever sees the row is to be
+// NaN, and whoever does not must not meet it (0 x NaN).  The rotated part stays: what it holds reaches the scores alone
+__device__ __forceinline__ bool latent_copy_row(const __nv_bfloat16* src, bool there, __nv_bfloat16* dst, bool clean) {
+    const int lane = threadIdx.x & 31;
+    uint4 v[3];
+    bool finite = true;
+#pragma unroll
+    for (int c = 0; c < 3; c++) {
+        v[c] = there && lane + 32 * c < kLatentRow / 8 ? reinterpret_cast<const uint4*>(src)[lane + 32 * c] : make_uint4(0, 0, 0, 0);
+        const uint32_t w[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
+#pragma unroll
+        for (int k = 0; k < 4; k++) finite &= c == 2 || ((w[k] & 0x7f800000u) != 0x7f800000u && (w[k] & 0x7f80u) != 0x7f80u);
+    }
+    const bool whole = __all_sync(0xffffffffu, finite) || !clean;
+#pragma unroll
+    for (int c = 0; c < 3; c++)
+        if (lane + 32 * c < kLatentRow / 8) reinterpret_cast<uint4*>(dst)[lane + 32 * c] = whole || c == 2 ? v[c] : make_uint4(0, 0, 0, 0);
+    return !whole;
+}
+// a sector of 32 bytes, from a thread
+template <typename T> __device__ __forceinline__ void latent_store32(T* to, const uint32_t* w) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
+}
 __device__ __forceinline__ float latent_exp2(float x) {      // one instruction; 2^-inf = 0
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

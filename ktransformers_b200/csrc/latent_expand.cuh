@@ -148,7 +148,7 @@ __global__ void __launch_bounds__(kLxThreads, 1) __cluster_dims__(2, 1, 1)
                     uint32_t w[8];
 #pragma unroll
                     for (int i = 0; i < 8; i++) w[i] = latent_pack(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
-                    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(row + c), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
+                    latent_store32(row + c, w);
                 }
             }
             tc_fence_before();

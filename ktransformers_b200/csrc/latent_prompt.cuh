@@ -254,9 +254,7 @@ template <int N, int V> __global__ void __launch_bounds__(kLpThreads, 1) latent_
                 for (int i = 0; i < 16; i++) o[i] = latent_pack(__uint_as_float(v[2 * i]) * k, __uint_as_float(v[2 * i + 1]) * k);
                 if (vec) {
 #pragma unroll
-                    for (int i = 0; i < 2; i++)
-                        asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(out + 32 * q + 16 * i), "r"(o[8 * i]), "r"(o[8 * i + 1]), "r"(o[8 * i + 2]), "r"(o[8 * i + 3]),
-                                     "r"(o[8 * i + 4]), "r"(o[8 * i + 5]), "r"(o[8 * i + 6]), "r"(o[8 * i + 7]) : "memory");
+                    for (int i = 0; i < 2; i++) latent_store32(out + 32 * q + 16 * i, o + 8 * i);
                 } else {
 #pragma unroll
                     for (int i = 0; i < 32; i++) reinterpret_cast<uint16_t*>(out)[32 * q + i] = (uint16_t)(o[i >> 1] >> (16 * (i & 1)));

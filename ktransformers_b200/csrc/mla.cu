@@ -34,7 +34,6 @@
 #include <cuda_bf16.h>
 
 #include "common.cuh"
-#include "mla_ragged.h"
 #include "umma.cuh"
 
 namespace ktb {
@@ -401,13 +400,12 @@ __global__ void __launch_bounds__(kMlaThreads, 1) mla_decode_tc_kernel(const __g
 }
 
 // out[b][h][:] = sum_s w_s * o_part[b][s][h][:],  w_s = 2^(lse_s - max) / sum ; lse (natural log) optional
-// keep_nan: rows whose every part is NaN stay that (else zeros)
 // sink (optional, [num_heads], natural-log units): one more term exp(sink_h) in the denominator that carries no value
 // A CTA per head and sequence, a thread per four columns and part of the splits (128 threads each, kMergeLoads splits a part and round): bound by rounds of loads, 10 of 8 for 74 splits
 // in one part, two of 10 in four parts.
 constexpr int kMergeLoads = 10, kMergeParts = 4;
 __global__ void __launch_bounds__(128 * kMergeParts) mla_merge_kernel(const float* o_part, const float* lse_part, int num_splits, int num_heads,
-                                                                      __nv_bfloat16* out, float* lse_out, const float* sink, int keep_nan) {
+                                                                      __nv_bfloat16* out, float* lse_out, const float* sink) {
     __shared__ float ws[kMaxSplits];
     __shared__ float red[8];
     __shared__ float4 sums[kMergeParts - 1][128];
@@ -433,11 +431,9 @@ __global__ void __launch_bounds__(128 * kMergeParts) mla_merge_kernel(const floa
     mx = fmaxf(mx, snk);
     __nv_bfloat162* o2 = reinterpret_cast<__nv_bfloat162*>(out + ((long)b * num_heads + h) * kDV + c);
     if (mx == -INFINITY) {   // kv_len == 0 (e.g. a padded CUDA-graph batch slot): zeros, lse = -inf
-        float none = 0.f;
-        if (keep_nan && __syncthreads_or(my != my)) none = __int_as_float(0x7fffffff);      // (no number among the maxima, which is not the same as no key)
         if (part) return;
-        o2[0] = __floats2bfloat162_rn(none, none);
-        o2[1] = __floats2bfloat162_rn(none, none);
+        o2[0] = __floats2bfloat162_rn(0.f, 0.f);
+        o2[1] = __floats2bfloat162_rn(0.f, 0.f);
         if (lse_out && tid == 0) lse_out[(long)b * num_heads + h] = -INFINITY;
         return;
     }
@@ -509,7 +505,7 @@ size_t ktb200_mla_workspace_bytes(int batch, int num_heads, int max_splits) {
 
 // shared launch path of plain MLA decode and the windowed / ragged form
 static int mla_launch(const ktb::MlaKParams& in, const void* kv_cache, long kv_cache_rows, int batch, int num_kv_splits, int max_tiles, void* workspace,
-                      size_t workspace_bytes, void* out, float* lse_out, const float* sink, bool split_p, void* stream, int keep_nan = 0) {
+                      size_t workspace_bytes, void* out, float* lse_out, const float* sink, bool split_p, void* stream) {
     using namespace ktb;
     int dev = 0;
     KTB_CUDA_CHECK(cudaGetDevice(&dev));
@@ -559,7 +555,7 @@ static int mla_launch(const ktb::MlaKParams& in, const void* kv_cache, long kv_c
     else KTB_CUDA_CHECK(launch_pdl(mla_decode_tc_kernel<false>, dim3(splits, head_groups, batch), dim3(kMlaThreads), (size_t)kMlaSmem, s, map, q_map, pe_map, p));
     count_launch();
     KTB_CUDA_CHECK(launch_pdl(mla_merge_kernel, dim3(batch * p.num_heads), dim3(128 * std::min(kMergeParts, (splits + kMergeLoads - 1) / kMergeLoads)), 0, s, (const float*)p.o_part, (const float*)p.lse_part, splits, p.num_heads,
-                              (__nv_bfloat16*)out, lse_out, sink, keep_nan));
+                              (__nv_bfloat16*)out, lse_out, sink));
     count_launch();
     return KTB200_OK;
 }
@@ -612,25 +608,6 @@ int ktb200_latent_window_attn_tc(const void* q_abs, const void* q_rot, int num_h
     const int span = window > 0 && window < max_kv ? window : max_kv;
     return mla_launch(p, cache, cache_rows, n_tokens, 0, (span + kLT - 1) / kLT + 1, workspace, workspace_bytes, out, nullptr, sink, true, stream);
 }
-
-}  // extern "C"
-
-size_t ktb::mla_ragged_workspace(int n_tokens, int num_heads, int max_kv) {
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess) return 0;
-    const int max_tiles = (max_kv + kLT - 1) / kLT;
-    return (size_t)n_tokens * std::max(1, std::min(pick_splits(n_tokens, num_heads, max_tiles, dev), max_tiles)) * num_heads * (kDV + 1) * sizeof(float);
-}
-int ktb::mla_ragged(const void* q_abs, const void* q_rot, int num_heads, float scale, const int* pos, const int* row, const int* page_table, int max_pages, int page_size, const void* cache,
-                    long cache_rows, void* out, int n_tokens, int max_kv, void* workspace, size_t workspace_bytes, cudaStream_t stream) {
-    MlaKParams p{};
-    p.q_nope = (const __nv_bfloat16*)q_abs; p.q_pe = (const __nv_bfloat16*)q_rot;
-    p.page_table = page_table; p.pos = pos; p.seq_row = row; p.ring = 1;
-    p.num_heads = num_heads; p.page_size = page_size; p.max_pages = max_pages; p.scale_log2 = scale * 1.4426950408889634f;
-    return mla_launch(p, cache, cache_rows, n_tokens, 0, (max_kv + kLT - 1) / kLT, workspace, workspace_bytes, out, nullptr, nullptr, false, stream, 1);
-}
-
-extern "C" {
 
 // Diagnostics: while set, CTA (split 0, head group 0, sequence 0) of ktb200_mla_decode writes the raw fp32 scores of its
 // first tile (S[64 heads][32 tokens], before scaling) to debug_dev[0..2048) and %globaltimer stamps (uint64) to
