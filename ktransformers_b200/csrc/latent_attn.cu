@@ -104,36 +104,40 @@ __global__ void __launch_bounds__(256) latent_gather_kernel(const ktb200_latent_
 }
 
 // ------------------------------------------------------------------------------------------------ absorbed form
-// C[t][h][:] = A[t][h][:] B_h on mma tiles, fp32 sums, one rounding: a CTA has 16 or 64 tokens of one head and a block of columns, and all of its K in shared memory at once: the product is
-// bound by the weights' bytes (16.8 MB each with 128 heads), and with several CTAs an SM all of them are on their way at the start.
-//   VALUES = false: A = q_nope (K = N), B_h = W_K,h [N][512], blocks of 128 columns;  VALUES = true: A = sums of latents (K = 512), B_h = W_V,h^T, W_V,h [V][512], blocks of 32 columns
+// C[t][h][:] = A[t][h][:] B_h on mma tiles, fp32 sums, one rounding: a CTA has MT tokens of one head and NB columns, and all of its K in shared memory at once: the product is bound by the
+// weights' bytes (16.8 MB each with 128 heads), and all of them are on their way at the start.
+//   VALUES = false: A = q_nope (K = N), B_h = W_K,h [N][512];  VALUES = true: A = sums of latents (K = 512), B_h = W_V,h^T, W_V,h [V][512]
+// All columns of a head in a CTA where there are heads and token tiles for half of the SMs, blocks of 128 (or 32) where there are not.
 // The first also writes which tokens there are (`there`: in a portion, with a position and a slot); the second leaves the rows of others as they are.
-template <int MT, int K, bool VALUES> struct AbsorbShape {
-    static constexpr int NB = VALUES ? 32 : 128, KP = K + 8, BP = VALUES ? 512 + 8 : NB + 8;      // padded rows: neighbouring rows meet in no bank
-    static constexpr int WM = MT / 16, WN = VALUES ? (MT == 16 ? 4 : 2) : 8 / WM, WK = 8 / (WM * WN), NT = NB / 8 / WN;      // warps along tokens, columns and K; runs of 8 columns a warp
+template <int MT, int K, bool VALUES, int NB> struct AbsorbShape {
+    static constexpr int WARPS = NB > 128 || (VALUES && NB > 32) ? 16 : 8, KP = K + 8, BP = VALUES ? kLatent + 8 : NB + 8, CP = NB + 8;      // padded rows: neighbouring rows meet in no bank
+    static constexpr int WM = MT / 16, COLS = NB / 8, WN = WARPS / WM < COLS ? WARPS / WM : COLS, WK = WARPS / (WM * WN), NT = COLS / WN;      // warps along tokens, columns and K; runs of 8 columns a warp
     static constexpr int A_BYTES = MT * KP * 2, B_BYTES = (VALUES ? NB : K) * BP * 2, SMEM = A_BYTES + B_BYTES;
-    static_assert(WM * WN * WK == 8 && NT >= 1, "8 warps");
+    static_assert(WM * WN * WK == WARPS && NT >= 1 && (NT == 1 || NT % 2 == 0) && K % (16 * WK) == 0 && MT * CP * 2 <= B_BYTES, "shape");
 };
-template <int MT, int K, bool VALUES> __global__ void __launch_bounds__(256) absorb_kernel(const ktb200_latent_attn_params p, const __nv_bfloat16* A, long a_stride, int a_head, int width, __nv_bfloat16* out,
-                                                                                            long out_stride, int n_tokens, int* there) {
-    using S = AbsorbShape<MT, K, VALUES>;
+template <int MT, int K, bool VALUES, int NB> __global__ void __launch_bounds__(AbsorbShape<MT, K, VALUES, NB>::WARPS * 32) absorb_kernel(const ktb200_latent_attn_params p, const __nv_bfloat16* A, long a_stride, int a_head,
+                                                                                                                                         int width, __nv_bfloat16* out, long out_stride, int n_tokens, int* there) {
+    using S = AbsorbShape<MT, K, VALUES, NB>;
+    constexpr int THREADS = S::WARPS * 32;
     extern __shared__ __align__(16) uint8_t ab_smem[];
     __nv_bfloat16* As = reinterpret_cast<__nv_bfloat16*>(ab_smem);
     __nv_bfloat16* Bs = reinterpret_cast<__nv_bfloat16*>(ab_smem + S::A_BYTES);
-    const int h = blockIdx.y, n0 = blockIdx.x * S::NB, m0 = blockIdx.z * MT, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int h = blockIdx.y, n0 = blockIdx.x * NB, m0 = blockIdx.z * MT, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const __nv_bfloat16* B = (const __nv_bfloat16*)p.w + ((long)h * (p.nope_dim + p.vdim) + (VALUES ? p.nope_dim + n0 : 0)) * kLatent + (VALUES ? 0 : n0);
     griddep_launch_dependents();
-    constexpr int BR = VALUES ? S::NB : K, BC = (VALUES ? kLatent : S::NB) / 8;
-    for (int i = tid; i < BR * BC; i += 256) cp_async16(Bs + (i / BC) * S::BP + (i % BC) * 8, B + (long)(i / BC) * kLatent + (i % BC) * 8, true);      // (the call's first kernel lets the next ones start behind its own wait: what was ahead of the call is complete)
+    constexpr int BR = VALUES ? NB : K, BC = (VALUES ? kLatent : NB) / 8;
+#pragma unroll 8
+    for (int i = tid; i < BR * BC; i += THREADS) cp_async16(Bs + (i / BC) * S::BP + (i % BC) * 8, B + (long)(i / BC) * kLatent + (i % BC) * 8, true);      // (the call's first kernel lets the next ones start behind its own wait: what was ahead of the call is complete)
     griddep_wait();
     constexpr int AC = K / 8;
-    for (int i = tid; i < MT * AC; i += 256) {
+#pragma unroll 4
+    for (int i = tid; i < MT * AC; i += THREADS) {
         const int m = i / AC;
         const bool in = m0 + m < n_tokens;
         cp_async16(As + m * S::KP + (i % AC) * 8, A + (long)(in ? m0 + m : 0) * a_stride + (long)h * a_head + (i % AC) * 8, in);
     }
     if (!VALUES && h == 0 && blockIdx.x == 0) {
-        for (int m = warp; m < MT; m += 8) {
+        for (int m = warp; m < MT; m += S::WARPS) {
             const int t = m0 + m;
             if (t >= n_tokens) break;
             bool in = false;
@@ -155,7 +159,7 @@ template <int MT, int K, bool VALUES> __global__ void __launch_bounds__(256) abs
     for (int k = wk * KW; k < (wk + 1) * KW; k += 16) {
         uint32_t a[4];
         ldmatrix_x4(a, As + (wm * 16 + (lane & 15)) * S::KP + k + (lane >> 4) * 8);
-        if (S::NT == 1) {      // (two K steps' columns in one load would need an even number of them: K is a multiple of 64)
+        if (S::NT == 1) {
             uint32_t b[4];
             ldmatrix_x4(b, Bs + (wn * 8 + (lane & 7)) * S::BP + k + (lane >> 3 & 1) * 8);
             mma_bf16_16816(acc[0], a, b[0], b[1]);
@@ -171,41 +175,65 @@ template <int MT, int K, bool VALUES> __global__ void __launch_bounds__(256) abs
             }
         }
     }
+    __syncthreads();      // (the operands are done with)
     if (S::WK > 1) {
-        float* part = reinterpret_cast<float*>(ab_smem);      // (over the operands)
-        __syncthreads();
+        float* part = reinterpret_cast<float*>(ab_smem);
         if (wk > 0)
 #pragma unroll
             for (int i = 0; i < S::NT * 4; i++) part[((warp - S::WM * S::WN) * S::NT * 4 + i) * 32 + lane] = acc[i / 4][i % 4];
         __syncthreads();
-        if (wk > 0) return;
+        if (wk == 0)
 #pragma unroll
-        for (int k = 1; k < S::WK; k++)
+            for (int k = 1; k < S::WK; k++)
 #pragma unroll
-            for (int i = 0; i < S::NT * 4; i++) acc[i / 4][i % 4] += part[((warp + (k - 1) * S::WM * S::WN) * S::NT * 4 + i) * 32 + lane];
+                for (int i = 0; i < S::NT * 4; i++) acc[i / 4][i % 4] += part[((warp + (k - 1) * S::WM * S::WN) * S::NT * 4 + i) * 32 + lane];
     }
+    // results through shared memory, so that whole lines are written
+    __nv_bfloat16* Cs = Bs;
+    if (wk == 0) {
 #pragma unroll
-    for (int r = 0; r < 2; r++) {
-        const int m = m0 + wm * 16 + (lane >> 2) + 8 * r;
-        if (m >= n_tokens || (VALUES && !there[m])) continue;
-        __nv_bfloat16* row = out + (long)m * out_stride + (long)h * width + n0 + wn * S::NT * 8 + 2 * (lane & 3);
+        for (int r = 0; r < 2; r++)
 #pragma unroll
-        for (int i = 0; i < S::NT; i++) {
-            if ((uintptr_t)row % 4 == 0) {
-                *reinterpret_cast<uint32_t*>(row + 8 * i) = latent_pack(acc[i][2 * r], acc[i][2 * r + 1]);
-            } else {
-                row[8 * i] = __float2bfloat16_rn(acc[i][2 * r]);
-                row[8 * i + 1] = __float2bfloat16_rn(acc[i][2 * r + 1]);
-            }
+            for (int i = 0; i < S::NT; i++)
+                *reinterpret_cast<uint32_t*>(Cs + (wm * 16 + (lane >> 2) + 8 * r) * S::CP + (wn * S::NT + i) * 8 + 2 * (lane & 3)) = latent_pack(acc[i][2 * r], acc[i][2 * r + 1]);
+    }
+    __syncthreads();
+#pragma unroll 4
+    for (int i = tid; i < MT * (NB / 8); i += THREADS) {
+        const int m = i / (NB / 8), c = i % (NB / 8) * 8;
+        if (m0 + m >= n_tokens || (VALUES && !there[m0 + m])) continue;
+        __nv_bfloat16* to = out + (long)(m0 + m) * out_stride + (long)h * width + n0 + c;
+        const uint4 v = *reinterpret_cast<const uint4*>(Cs + m * S::CP + c);
+        if ((uintptr_t)to % 16 == 0) {
+            *reinterpret_cast<uint4*>(to) = v;
+        } else {
+            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int x = 0; x < 8; x++) reinterpret_cast<uint16_t*>(to)[x] = (uint16_t)(w[x >> 1] >> (16 * (x & 1)));
         }
     }
 }
-template <int MT, int K, bool VALUES> static int absorb_launch(const ktb200_latent_attn_params* p, const __nv_bfloat16* A, long a_stride, int a_head, int width, __nv_bfloat16* out, long out_stride, int n, int* there, cudaStream_t s) {
-    using S = AbsorbShape<MT, K, VALUES>;
-    KTB_CUDA_CHECK(raise_smem_limit((const void*)absorb_kernel<MT, K, VALUES>, S::SMEM));
-    KTB_CUDA_CHECK(launch_pdl(absorb_kernel<MT, K, VALUES>, dim3((VALUES ? p->vdim : kLatent) / S::NB, p->heads, (n + MT - 1) / MT), dim3(256), (size_t)S::SMEM, s, *p, A, a_stride, a_head, width, out, out_stride, n, there));
-    count_launch();
-    return KTB200_OK;
+template <int K, int WIDTH, bool VALUES> static int absorb_launch(const ktb200_latent_attn_params* p, const __nv_bfloat16* A, long a_stride, int a_head, __nv_bfloat16* out, long out_stride, int n, int* there, int sms,
+                                                                  cudaStream_t s) {
+    auto go = [&](auto mt, auto nb) {
+        constexpr int MT = decltype(mt)::value, NB = decltype(nb)::value;
+        using S = AbsorbShape<MT, K, VALUES, NB>;
+        const auto kernel = absorb_kernel<MT, K, VALUES, NB>;
+        KTB_CUDA_CHECK(raise_smem_limit((const void*)kernel, S::SMEM));
+        KTB_CUDA_CHECK(launch_pdl(kernel, dim3(WIDTH / NB, p->heads, (n + MT - 1) / MT), dim3(S::WARPS * 32), (size_t)S::SMEM, s, *p, A, a_stride, a_head, WIDTH, out, out_stride, n, there));
+        count_launch();
+        return KTB200_OK;
+    };
+    using C16 = std::integral_constant<int, 16>;
+    using C32 = std::integral_constant<int, 32>;
+    using C64 = std::integral_constant<int, 64>;
+    using Part = std::integral_constant<int, VALUES ? 32 : 128>;
+    using All = std::integral_constant<int, WIDTH>;
+    const int mt = n <= 16 ? 16 : n <= 32 ? 32 : 64;
+    const bool all = (long)p->heads * ((n + mt - 1) / mt) * 2 >= sms;
+    if (mt == 16) return all ? go(C16(), All()) : go(C16(), Part());
+    if (mt == 32) return all ? go(C32(), All()) : go(C32(), Part());
+    return all ? go(C64(), All()) : go(C64(), Part());
 }
 
 // ------------------------------------------------------------------------------------------------ host
@@ -354,17 +382,13 @@ template <int N, int V> static int latent_absorbed(const ktb200_latent_attn_para
     if (e) return e;
     KTB_CUDA_CHECK(launch_pdl(latent_few_prep_kernel, dim3(1 + (y.gathered ? 0 : 4 * y.tail_tiles)), dim3(256), (size_t)0, s, a, tails, (uint32_t*)(ws + y.tail_bad)));
     count_launch();
-    const __nv_bfloat16* q = (const __nv_bfloat16*)p->q;
-    int rc = n_tokens <= 16 ? absorb_launch<16, N, false>(p, q, p->q_stride, N + kLatentRot, kLatent, q_abs, wide, n_tokens, there, s)
-                            : absorb_launch<64, N, false>(p, q, p->q_stride, N + kLatentRot, kLatent, q_abs, wide, n_tokens, there, s);
+    const int rc = absorb_launch<N, kLatent, false>(p, (const __nv_bfloat16*)p->q, p->q_stride, N + kLatentRot, q_abs, wide, n_tokens, there, sms, s);
     if (rc) return rc;
     KTB_CUDA_CHECK(raise_smem_limit((const void*)latent_few_kernel, kFewSmem));
     KTB_CUDA_CHECK(launch_pdl(latent_few_kernel, dim3(2 * y.pairs), dim3(kFewThreads), (size_t)kFewSmem, s, m, a));
     KTB_CUDA_CHECK(launch_pdl(latent_few_merge_kernel, dim3(y.blocks, kFewRows / 8), dim3(256), (size_t)0, s, a));
     count_launch(2);
-    __nv_bfloat16* out = (__nv_bfloat16*)p->out;
-    return n_tokens <= 16 ? absorb_launch<16, kLatent, true>(p, a.sums, wide, kLatent, V, out, p->out_stride, n_tokens, there, s)
-                          : absorb_launch<64, kLatent, true>(p, a.sums, wide, kLatent, V, out, p->out_stride, n_tokens, there, s);
+    return absorb_launch<kLatent, V, true>(p, a.sums, wide, kLatent, (__nv_bfloat16*)p->out, p->out_stride, n_tokens, there, sms, s);
 }
 
 }  // namespace ktb

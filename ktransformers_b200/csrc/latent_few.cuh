@@ -27,12 +27,21 @@ struct FewMisc {
 constexpr int kFewSmem = kFewRoom + (int)sizeof(FewMisc) + 1024;
 static_assert(kFewSmem <= 232448, "shared memory budget");
 
-struct FewBlock { int row0, rows, lead, seq, pos0, tile0, tiles, tail; };      // first row of q'; rows; rows of the portion ahead of it; its portion and that one's first position; its first tile in the line, its tiles, the first of its portion's that comes from the tails
+struct __align__(16) FewBlock {
+    int row0, rows, lead, seq;      // first row of q'; rows; rows of the portion ahead of it; its portion
+    int pos0, tile0, tiles, tail;   // that one's first position; its first tile in the line, its tiles, its portion's first among the tails
+    int run0, parts, late, spare;   // the run that has its first tile, the runs that have one; whether that run has tiles of another block before them
+};
 // what latent_few_prep_kernel leaves: ints tiles of the line, blocks, pairs that have a run (of kFewRun tiles and more), then (from 4 on) for each its first block and tile in it, then FewBlock
 // from few_blocks_at
 constexpr int kFewLine = 0, kFewBlocks = 1, kFewRuns = 2, kFewPairs = 4, kFewRun = 2;
-__host__ __device__ inline long few_blocks_at(int pairs) { return (kFewPairs + 2L * pairs + 7) / 8 * 8; }
-__host__ __device__ __forceinline__ int few_run(long line, int runs, int i) { return (int)(line * i / runs); }      // the first tile of run i
+__host__ __device__ inline long few_blocks_at(int pairs) { return (kFewPairs + 2L * pairs + 3) / 4 * 4; }
+__host__ // the first tile of run i, of runs that differ by one tile at most, and the run that has tile x
+__device__ __forceinline__ int few_run(int line, int runs, int i) { return line / runs * i + min(i, line % runs); }
+__device__ __forceinline__ int few_run_of(int line, int runs, int x) {
+    const int n = line / runs, more = line % runs, long_ones = more * (n + 1);
+    return x < long_ones ? x / (n + 1) : more + (x - long_ones) / n;
+}
 
 struct LatentFew {
     ktb200_latent_attn_params p;
@@ -141,7 +150,7 @@ __global__ void __launch_bounds__(256) latent_few_prep_kernel(const LatentFew a,
         const bool room = b0 + nb <= a.block_cap && t0 + nt <= a.tail_cap;      // (portions that share tokens may not have it)
         for (int b = 0; b < nb && b0 + b < a.block_cap; b++) {
             const int lead = b * kFewRows, n = (int)min((long)kFewRows, rows - lead), keys = q.pos + (lead + n - 1) / H + 1;
-            blocks[b0 + b] = FewBlock{q.first * H + lead, n, lead, s, q.pos, 0, room ? (keys + kFewTile - 1) / kFewTile : 0, t0};
+            blocks[b0 + b] = FewBlock{q.first * H + lead, n, lead, s, q.pos, 0, room ? (keys + kFewTile - 1) / kFewTile : 0, t0, 0, 0, 0, 0};
         }
         __syncthreads();
         if (tid == 0) { carry[0] += all_b; carry[1] += all_t; }
@@ -156,19 +165,21 @@ __global__ void __launch_bounds__(256) latent_few_prep_kernel(const LatentFew a,
         if (tid == 0) carry[2] += all;
         __syncthreads();
     }
-    const int line = carry[2];
-    const int runs = min(a.pairs, (line + kFewRun - 1) / kFewRun);
+    const int line = carry[2], runs = min(a.pairs, (line + kFewRun - 1) / kFewRun);
     if (tid == 0) { a.plan[kFewLine] = line; a.plan[kFewBlocks] = nb; a.plan[kFewRuns] = runs; }
-    for (int i = tid; i < runs; i += 256) {
-        const int x = few_run(line, runs, i);
-        int lo = 0, hi = nb;      // the last block that begins at or before x (one without tiles is none)
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) / 2;
-            if (blocks[mid].tile0 <= x) lo = mid;
-            else hi = mid;
+    for (int b = tid; b < nb; b += 256) {      // each block finds its runs, and is the first of those that begin in it
+        const int x = blocks[b].tile0, n = blocks[b].tiles;
+        if (n == 0) continue;
+        const int first = few_run_of(line, runs, x), last = few_run_of(line, runs, x + n - 1);
+        blocks[b].run0 = first;
+        blocks[b].parts = last - first + 1;
+        blocks[b].late = few_run(line, runs, first) < x;
+        for (int i = first; i <= last; i++) {
+            const int at = few_run(line, runs, i);
+            if (at < x) continue;
+            a.plan[kFewPairs + 2 * i] = b;
+            a.plan[kFewPairs + 2 * i + 1] = at - x;
         }
-        a.plan[kFewPairs + 2 * i] = lo;
-        a.plan[kFewPairs + 2 * i + 1] = x - blocks[lo].tile0;
     }
 }
 
@@ -509,18 +520,12 @@ __global__ void __launch_bounds__(kFewThreads, 1) __cluster_dims__(2, 1, 1) late
 __global__ void __launch_bounds__(256) latent_few_merge_kernel(const LatentFew a) {
     griddep_launch_dependents();
     griddep_wait();
-    const int line = a.plan[kFewLine], nb = a.plan[kFewBlocks], runs = a.plan[kFewRuns], lane = threadIdx.x & 31, in = blockIdx.y * 8 + (threadIdx.x >> 5);
-    if ((int)blockIdx.x >= nb) return;
+    const int lane = threadIdx.x & 31, in = blockIdx.y * 8 + (threadIdx.x >> 5);
+    if ((int)blockIdx.x >= a.plan[kFewBlocks]) return;
     const FewBlock k = reinterpret_cast<const FewBlock*>(a.plan + few_blocks_at(a.pairs))[blockIdx.x];
-    if (in >= k.rows || k.tiles == 0) return;
-    int first = (int)min((long)runs - 1, (long)k.tile0 * runs / line);      // the run that has the block's first tile
-    while (first + 1 < runs && few_run(line, runs, first + 1) <= k.tile0) first++;
-    while (first > 0 && few_run(line, runs, first) > k.tile0) first--;
-    int parts = 1;
-    while (first + parts < runs && few_run(line, runs, first + parts) < k.tile0 + k.tiles) parts++;
-    if (parts == 1) return;
-    const int lead = few_run(line, runs, first) < k.tile0;      // the first part is that run's second segment or a later one
-    auto at = [&](int i) { return (2L * (first + i) + (i == 0 ? lead : 0)) * kFewRows + in; };
+    if (in >= k.rows || k.tiles == 0 || k.parts == 1) return;
+    const int parts = k.parts;
+    auto at = [&](int i) { return (2L * (k.run0 + i) + (i == 0 ? k.late : 0)) * kFewRows + in; };
     float m = -INFINITY, l = 0.f, o[16];
     bool nan = false;
 #pragma unroll
