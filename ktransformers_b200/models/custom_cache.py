@@ -92,6 +92,14 @@ class ForwardBatch:
         self.seq_of = meta[9] if meta.shape[0] >= 10 else None
         self.turns: Dict[Any, torch.Tensor] = {}
 
+    @classmethod
+    def portions(cls, pos: torch.Tensor, slot: torch.Tensor, seqs: torch.Tensor, max_kv: int) -> "ForwardBatch":
+        """A batch of index rows alone, for operators that take nothing but them: pos, slot [T] and seqs [2, n_seqs] (first token's row, tokens), int32 on the device."""
+        b = cls.__new__(cls)
+        b.pos, b.slot, b.seqs, b.max_kv, b.n_tokens, b.n_seqs, b.turns = pos, slot, seqs, max_kv, int(pos.shape[0]), int(seqs.shape[1]), {}
+        b.tokens = b.want = b.prev_idx = b.rd_row = b.wr_row = b.seq_of = None
+        return b
+
     def turn_table(self, rot, inv_freq: torch.Tensor) -> torch.Tensor:
         """(cos, sin) of position * frequency for every token, [T, rot.dims / 2, 2] fp32 (angles fp64): one `ktb200_turn_table` launch per
         step for all layers of the same rotation `rot`; `inv_freq`: its fp64 frequencies on the device"""

@@ -25,7 +25,7 @@ class DeepseekV3Config(PretrainedConfig):
                  norm_topk_prob=True, scoring_func="sigmoid", topk_method="noaux_tc", hidden_act="silu",
                  num_hidden_layers=61, first_k_dense_replace=3, moe_layer_freq=1, num_attention_heads=128,
                  q_lora_rank=1536, kv_lora_rank=512, qk_rope_head_dim=64, qk_nope_head_dim=128, v_head_dim=128,
-                 vocab_size=129280, rms_norm_eps=1e-6, ep_size=1, **kwargs):
+                 vocab_size=129280, rms_norm_eps=1e-6, ep_size=1, rope_scaling=None, **kwargs):
         self.hidden_size = hidden_size
         self.intermediate_size = intermediate_size
         self.moe_intermediate_size = moe_intermediate_size
@@ -52,6 +52,7 @@ class DeepseekV3Config(PretrainedConfig):
         self.rms_norm_eps = rms_norm_eps
         self.ep_size = ep_size
         super().__init__(**kwargs)
+        self.rope_scaling = rope_scaling      # {"type": "yarn", "factor", ...} or None
 
 
 class DeepseekV3MLP(nn.Module):
@@ -178,6 +179,40 @@ class DeepseekV3RotaryEmbedding(nn.Module):
         return emb.cos().to(x.dtype), emb.sin().to(x.dtype)
 
 
+def yarn_inv_freq(dims: int, base: float, factor: float, original: int, beta_fast: float = 32.0, beta_slow: float = 1.0) -> torch.Tensor:
+    """Frequencies of a rotation scaled for contexts of `factor` times the `original` length (YaRN; modeling_deepseek_v3.py:233-334), float64: those that turn more than beta_fast times in the
+    original length stay, those that turn less than beta_slow times are divided by the factor, and between the two the share moves in a straight line over the column."""
+    i = torch.arange(dims // 2, dtype=torch.float64)
+    freq = float(base) ** (-2.0 * i / dims)
+    column = lambda turns: dims * math.log(original / (turns * 2 * math.pi)) / (2 * math.log(base))
+    lo, hi = max(math.floor(column(beta_fast)), 0), min(math.ceil(column(beta_slow)), dims - 1)
+    share = ((i - lo) / ((hi - lo) or 0.001)).clamp(0.0, 1.0)
+    return freq * (1 - share) + freq / float(factor) * share
+
+
+class DeepseekV3YarnRotaryEmbedding(nn.Module):
+    """RoPE tables scaled for long contexts (modeling_deepseek_v3.py:233-334, injected as operators/RoPE.py:222-326): cosines and sines of position * inv_freq, angles in float64 (no buffers: a
+    cast of the model leaves the frequencies as they are), times `gain` = mscale over mscale_all_dim's part of it, which DeepseekV3Attention has in its soft-max scale."""
+
+    def __init__(self, dim, max_position_embeddings=163840, base=10000.0, scaling_factor=1.0, original_max_position_embeddings=4096, beta_fast=32, beta_slow=1, mscale=1.0, mscale_all_dim=0.0):
+        super().__init__()
+        self.dim, self.base = dim, base
+        self.gain = yarn_get_mscale(scaling_factor, mscale) / yarn_get_mscale(scaling_factor, mscale_all_dim)
+        self._inv_freq = {torch.device("cpu"): yarn_inv_freq(dim, base, scaling_factor, original_max_position_embeddings, beta_fast, beta_slow)}
+
+    def inv_freq_on(self, device) -> torch.Tensor:
+        device = torch.device(device)
+        if device not in self._inv_freq:
+            self._inv_freq[device] = self._inv_freq[torch.device("cpu")].to(device)
+        return self._inv_freq[device]
+
+    @torch.no_grad()
+    def forward(self, x, position_ids):
+        freqs = position_ids[:, :, None].double() * self.inv_freq_on(position_ids.device)[None, None, :]
+        emb = torch.cat((freqs, freqs), dim=-1)
+        return (emb.cos() * self.gain).to(x.dtype), (emb.sin() * self.gain).to(x.dtype)
+
+
 def rotate_half(x):
     x1, x2 = x[..., : x.shape[-1] // 2], x[..., x.shape[-1] // 2:]
     return torch.cat((-x2, x1), dim=-1)
@@ -215,9 +250,14 @@ class DeepseekV3Attention(nn.Module):
         self.kv_a_layernorm = DeepseekV3RMSNorm(self.kv_lora_rank, config.rms_norm_eps)
         self.kv_b_proj = nn.Linear(self.kv_lora_rank, self.num_heads * (self.qk_nope_head_dim + self.v_head_dim), bias=False)
         self.o_proj = nn.Linear(self.num_heads * self.v_head_dim, self.hidden_size, bias=False)
-        self.rotary_emb = DeepseekV3RotaryEmbedding(self.qk_rope_head_dim, base=getattr(config, "rope_theta", 10000.0))
-        self.softmax_scale = self.q_head_dim ** (-0.5)
         rs = getattr(config, "rope_scaling", None)
+        base = getattr(config, "rope_theta", 10000.0)
+        if rs is not None and rs.get("type", rs.get("rope_type")) == "yarn":
+            names = ("original_max_position_embeddings", "beta_fast", "beta_slow", "mscale", "mscale_all_dim")
+            self.rotary_emb = DeepseekV3YarnRotaryEmbedding(self.qk_rope_head_dim, base=base, scaling_factor=rs["factor"], **{n: rs[n] for n in names if n in rs})
+        else:
+            self.rotary_emb = DeepseekV3RotaryEmbedding(self.qk_rope_head_dim, base=base)
+        self.softmax_scale = self.q_head_dim ** (-0.5)
         if rs is not None and rs.get("mscale_all_dim", 0):
             m = yarn_get_mscale(rs["factor"], rs["mscale_all_dim"])
             self.softmax_scale = self.softmax_scale * m * m

@@ -5,21 +5,24 @@ decode branch): q projections -> RoPE -> paged latent-cache update -> q_nope . W
 over the 576-wide latents -> . W_UV^T -> o_proj.  The attention itself is `MLAWrapper.run` = ktb200_mla_decode (tcgen05 +
 TMEM + TMA, csrc/mla.cu); the cache write is ktb200_mla_kv_write; the projections are whatever modules the rules injected
 (KLinearB200 on raw GGUF blocks, or nn.Linear); the two absorb products are ktb200_mla_absorb_q / _o (HBM-bound batched
-GEMVs over the bf16 halves of kv_b_proj; torch.matmul for other dtypes).  Prefill (q_len > 1 without absorb) is outside this path and raises."""
+GEMVs over the bf16 halves of kv_b_proj; torch.matmul for other dtypes).  Several tokens a sequence (q_len > 1: prompt portions, drafts) and scaled rotations run on
+`latent_append` and `latent_attention` (operators/latent_attention.py) between the projections."""
 from __future__ import annotations
 
 import ctypes as C
 import math
+from types import SimpleNamespace
 from typing import Optional, Tuple
 
 import torch
 
 from .. import native
-from ..models.custom_cache import Fp8CacheLayer, StaticCache
-from ..models.modeling_deepseek_v3 import DeepseekV3Attention, DeepseekV3RMSNorm, DeepseekV3RotaryEmbedding, apply_rotary_pos_emb
+from ..models.custom_cache import Fp8CacheLayer, ForwardBatch, StaticCache
+from ..models.modeling_deepseek_v3 import DeepseekV3Attention, DeepseekV3RMSNorm, DeepseekV3RotaryEmbedding, DeepseekV3YarnRotaryEmbedding, apply_rotary_pos_emb
 from ..util.utils import InferenceState
 from .base_operator import BaseInjectedModule, device_of, stream_of
 from .flashinfer_wrapper import MLAWrapper, MLAWrapperSingleton
+from .latent_attention import LatentRotation, latent_append, latent_attention
 
 
 def _is_plain(module, cls) -> bool:
@@ -164,17 +167,52 @@ class KDeepseekV2Attention(BaseInjectedModule, DeepseekV3Attention):
         native.check(lib.ktb200_mla_absorb_o(lat.data_ptr(), out_absorb.data_ptr(), heads, self.v_head_dim, 512, o.data_ptr(), bsz, stream))
         return self.o_proj(o)
 
+    def _portion(self, hidden_states, position_ids, cache, cache_position):
+        """New tokens of every sequence at consecutive cache positions, each of which sees its sequence's tokens up to itself: projections, `latent_append`, `latent_attention`, projection.
+        None for what these do not take.  (The reference's prefill branches: archive/ktransformers/operators/attention.py:140-344, 349-478; its `attention_mask` is not read there either.)"""
+        get = self._quick()
+        rot, norm, x, bf16 = get("rotary_emb"), get("kv_a_layernorm"), hidden_states, torch.bfloat16
+        yarn = _is_plain(rot, DeepseekV3YarnRotaryEmbedding)
+        if not (x.dtype is bf16 and x.is_cuda and (yarn or _is_plain(rot, DeepseekV3RotaryEmbedding)) and _is_plain(norm, DeepseekV3RMSNorm) and type(cache) is StaticCache):
+            return None
+        bsz, q_len, heads, nope, vdim, w = x.shape[0], x.shape[1], get("num_heads"), get("qk_nope_head_dim"), get("v_head_dim"), get("kv_b_proj").weight
+        if w.dtype is not bf16 or get("kv_lora_rank") != 512 or get("qk_rope_head_dim") != 64 or nope not in (64, 128) or vdim not in (64, 128) or position_ids is None or cache_position is None:
+            return None
+        if bsz > cache.max_batch_size or q_len > cache.max_pages * cache.page_size or cache_position.numel() != q_len or position_ids.numel() not in (q_len, bsz * q_len):
+            raise ValueError(f"KDeepseekV2Attention: {bsz} x {q_len} tokens, {position_ids.numel()} positions, {cache_position.numel()} cache positions for a cache of {cache.max_batch_size} sequences of "
+                             f"{cache.max_pages * cache.page_size}")
+        layer, dev, T = get("layer_idx"), x.device, bsz * q_len
+        q = get("q_proj")(x) if get("q_lora_rank") is None else get("q_b_proj")(get("q_a_layernorm")(get("q_a_proj")(x)))
+        q, kva = q.reshape(T, -1), get("kv_a_proj_with_mqa")(x).reshape(T, -1)
+        if not (q.dtype is bf16 is kva.dtype):
+            return None
+        i = torch.arange(bsz, dtype=torch.int32, device=dev)
+        batch = ForwardBatch.portions(cache_position.reshape(-1).to(torch.int32).repeat(bsz), i.repeat_interleave(q_len), torch.stack((i * q_len, torch.full_like(i, q_len))), cache.max_pages * cache.page_size)
+        pages = SimpleNamespace(page_table=cache.page_table_list[layer], max_pages_per_seq=cache.max_pages, page_size=cache.page_size)
+        kv, angles = cache.key_cache[layer], position_ids.to(torch.int32).expand(bsz, q_len).reshape(-1)
+        turn = LatentRotation(rot.inv_freq_on(dev) if yarn else rot.inv_freq.to(dev), gain=rot.gain if yarn else 1.0)
+        q_rot = latent_append(q, kva, norm.weight, norm.variance_epsilon, batch, pages, kv, heads, nope, rot=turn, positions=angles)
+        o = latent_attention(q, q_rot, kv, w, batch, pages, heads, nope, vdim, get("softmax_scale"), form="absorbed" if get("absorb_for_prefill") else None)
+        if not torch.cuda.is_current_stream_capturing():
+            cache.past_tokens[layer] += q_len
+        return get("o_proj")(o.view(bsz, q_len, heads * vdim))
+
     def forward(self, hidden_states: torch.Tensor, attention_mask: Optional[torch.Tensor] = None,
                 position_ids: Optional[torch.Tensor] = None, past_key_value=None, output_attentions: bool = False,
                 use_cache: bool = False, cache_position: Optional[torch.Tensor] = None, **kwargs):
         bsz, q_len, _ = hidden_states.size()
-        if q_len != 1 and not self.absorb_for_prefill:
-            raise NotImplementedError("KDeepseekV2Attention: the B200 path covers absorbed decode (q_len == 1)")
+        if q_len != 1:
+            out = self._portion(hidden_states, position_ids, past_key_value, cache_position)
+            if out is None:
+                raise NotImplementedError("KDeepseekV2Attention: several tokens a sequence need bf16, the static latent cache of 512 + 64, heads and values of 64 or 128, DeepseekV3's norms and rotations, "
+                                          "position_ids and cache_position")
+            return out, None, past_key_value
         assert past_key_value is not None, "decode needs the paged latent cache (models/custom_cache.StaticCache)"
-        if q_len == 1:
-            out = self._step(hidden_states, position_ids, past_key_value, cache_position)
-            if out is not None:
-                return out, None, past_key_value
+        out = self._step(hidden_states, position_ids, past_key_value, cache_position)
+        if out is None and type(self._quick()("rotary_emb")) is DeepseekV3YarnRotaryEmbedding:
+            out = self._portion(hidden_states, position_ids, past_key_value, cache_position)
+        if out is not None:
+            return out, None, past_key_value
         q = self.q_proj(hidden_states) if self.q_lora_rank is None else self.q_b_proj(self.q_a_layernorm(self.q_a_proj(hidden_states)))
         q = q.view(bsz, q_len, self.num_heads, self.q_head_dim)
         q_nope, q_pe = torch.split(q, [self.qk_nope_head_dim, self.qk_rope_head_dim], dim=-1)

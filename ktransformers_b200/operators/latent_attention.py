@@ -8,12 +8,12 @@ The reference has both in its attention operator (archive/ktransformers/operator
 from __future__ import annotations
 
 import ctypes as C
-import math
 from typing import Optional
 
 import torch
 
 from .. import native
+from ..models.modeling_deepseek_v3 import yarn_inv_freq  # noqa: F401  (the frequencies of a scaled LatentRotation)
 from .base_operator import device_of, stream_of
 
 FORMS = {None: 0, "absorbed": 1, "expanded": 2}
@@ -29,17 +29,6 @@ class LatentRotation:
     def __init__(self, inv_freq: torch.Tensor, layout: str = "interleaved", split: bool = True, gain: float = 1.0):
         self.dims, self.layout_code = 2 * int(inv_freq.numel()), {"interleaved": 0, "halves": 1}[layout]
         self.split, self.gain, self.inv_freq = bool(split), float(gain), inv_freq.to(torch.float64).contiguous()
-
-
-def yarn_inv_freq(dims: int, base: float, factor: float, original: int, beta_fast: float = 32.0, beta_slow: float = 1.0) -> torch.Tensor:
-    """Frequencies of a rotation scaled for contexts of `factor` times the `original` length (YaRN), float64: those that turn more than beta_fast times in the original length stay, those that
-    turn less than beta_slow times are divided by the factor, and between the two the share moves in a straight line over the column."""
-    i = torch.arange(dims // 2, dtype=torch.float64)
-    freq = float(base) ** (-2.0 * i / dims)
-    column = lambda turns: dims * math.log(original / (turns * 2 * math.pi)) / (2 * math.log(base))
-    lo, hi = max(math.floor(column(beta_fast)), 0), min(math.ceil(column(beta_slow)), dims - 1)
-    share = ((i - lo) / ((hi - lo) or 0.001)).clamp(0.0, 1.0)
-    return freq * (1 - share) + freq / float(factor) * share
 
 
 def _latent_batch(what: str, T: int, dev, kv: torch.Tensor, width: int, batch, cache):
