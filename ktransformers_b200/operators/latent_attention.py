@@ -7,6 +7,7 @@
 The reference has both in its attention operator (archive/ktransformers/operators/attention.py:140-344 for prompts, :349-478) and the scaled rotation in operators/RoPE.py:222-326."""
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 from typing import Optional
 
@@ -14,10 +15,10 @@ import torch
 
 from .. import native
 from ..models.modeling_deepseek_v3 import yarn_inv_freq  # noqa: F401  (the frequencies of a scaled LatentRotation)
-from .base_operator import device_of, stream_of
 
 FORMS = {None: 0, "absorbed": 1, "expanded": 2}
 LATENT, LATENT_ROT = 512, 64
+_HERE, _stream = contextlib.nullcontext(), torch._C._cuda_getCurrentRawStream      # (the current stream of a device as the C-ABI takes it)
 
 
 class LatentRotation:
@@ -31,29 +32,43 @@ class LatentRotation:
         self.split, self.gain, self.inv_freq = bool(split), float(gain), inv_freq.to(torch.float64).contiguous()
 
 
-def _latent_batch(what: str, T: int, dev, kv: torch.Tensor, width: int, batch, cache):
-    """Checks what both calls share; their arguments from `pos` to the number of pages"""
-    pos, slot, seqs, table, ps, n_seqs = batch.pos, batch.slot, batch.seqs, cache.page_table, cache.page_size, batch.n_seqs
-    if kv.dtype is not torch.bfloat16 or dev.type != "cuda":
-        raise ValueError(f"{what}: CUDA tensors and a bfloat16 cache only; got {kv.dtype} on {dev}")
-    if not kv.is_contiguous() or kv.dim() not in (3, 4) or kv.shape[1] != ps or kv.shape[-1] != width or kv.numel() != kv.shape[0] * ps * width:
-        raise ValueError(f"{what}: the cache layer has to be contiguous [pages, {ps}, {width}], got {tuple(kv.shape)}")
-    if seqs is None or not (seqs.dtype is pos.dtype is slot.dtype is table.dtype is torch.int32):
+_BF16, _I32, _F64 = torch.bfloat16, torch.int32, torch.float64
+
+
+def _latent_batch(what: str, T: int, dev: int, kv: torch.Tensor, width: int, batch, cache):
+    """Checks what both calls share; their arguments from `pos` to the number of pages.  (A decode step's calls are bound by their host work: each tensor is asked for its sizes once.)"""
+    pos, slot, seqs, table, ps, n_seqs, columns = batch.pos, batch.slot, batch.seqs, cache.page_table, cache.page_size, batch.n_seqs, cache.max_pages_per_seq
+    shape = kv.shape
+    if kv.dtype is not _BF16 or dev < 0:
+        raise ValueError(f"{what}: CUDA tensors and a bfloat16 cache only; got {kv.dtype} on {kv.device}")
+    if len(shape) not in (3, 4) or shape[1] != ps or shape[-1] != width or (len(shape) == 4 and shape[2] != 1) or not kv.is_contiguous():
+        raise ValueError(f"{what}: the cache layer has to be contiguous [pages, {ps}, {width}], got {tuple(shape)}")
+    if seqs is None or not (seqs.dtype is pos.dtype is slot.dtype is table.dtype is _I32):
         raise ValueError(f"{what}: needs int32 pos, slot, seqs and page table")
-    if pos.shape[0] < T or slot.shape[0] < T or seqs.shape[0] < 2 or n_seqs > seqs.shape[1]:
-        raise ValueError(f"{what}: {T} tokens, but {pos.shape[0]} positions, {slot.shape[0]} slots; {n_seqs} portions of {tuple(seqs.shape)}")
-    if pos.stride(0) != 1 or slot.stride(0) != 1 or seqs.stride(1) != 1 or table.dim() != 2 or not table.is_contiguous() or table.shape[1] != cache.max_pages_per_seq:
-        raise ValueError(f"{what}: index rows and page table rows have to be contiguous, max_pages_per_seq = {cache.max_pages_per_seq} of them")
-    if not (kv.device == pos.device == slot.device == seqs.device == table.device == dev):
+    (rows, portions), (seqs_stride, step), slots = seqs.shape, seqs.stride(), table.shape
+    if pos.numel() < T or slot.numel() < T or rows < 2 or n_seqs > portions:
+        raise ValueError(f"{what}: {T} tokens, but {pos.numel()} positions, {slot.numel()} slots; {n_seqs} portions of {tuple(seqs.shape)}")
+    if not (pos.is_contiguous() and slot.is_contiguous() and table.is_contiguous()) or (step != 1 and portions > 1) or len(slots) != 2 or slots[1] != columns:
+        raise ValueError(f"{what}: index rows and page table rows have to be contiguous, max_pages_per_seq = {columns} of them")
+    if not (kv.get_device() == pos.get_device() == slot.get_device() == seqs.get_device() == table.get_device() == dev):
         raise ValueError(f"{what}: all tensors have to be on one device")
-    return pos.data_ptr(), slot.data_ptr(), seqs.data_ptr(), seqs.stride(0), n_seqs, table.data_ptr(), table.shape[0], table.shape[1], ps, kv.shape[0]
+    return pos.data_ptr(), slot.data_ptr(), seqs.data_ptr(), seqs_stride, n_seqs, table.data_ptr(), slots[0], columns, ps, shape[0]
 
 
-def _rows(what: str, name: str, t: torch.Tensor, T: Optional[int], width: int, dev):
+def _rows(what: str, name: str, t: torch.Tensor, T: int, width: int, dev: int):
     """rows of bf16 with their columns side by side: (pointer, stride)"""
-    if t.dim() != 2 or t.dtype is not torch.bfloat16 or t.device != dev or (T is not None and t.shape[0] != T) or t.shape[1] < width or (t.stride(1) != 1 and t.shape[1] > 1):
-        raise ValueError(f"{what}: {name} has to be rows of {width} bfloat16 values side by side on {dev}, got {tuple(t.shape)} of {t.dtype} on {t.device}")
-    return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+    shape = t.shape
+    if t.dtype is not _BF16 or len(shape) != 2 or shape[0] != T or shape[1] < width or t.get_device() != dev:
+        raise ValueError(f"{what}: {name} has to be {T} rows of {width} bfloat16 values or more, got {tuple(shape)} of {t.dtype} on {t.device}")
+    stride, step = t.stride()
+    if step != 1 and shape[1] > 1:
+        raise ValueError(f"{what}: {name} has to have its columns side by side")
+    return t.data_ptr(), stride if T > 1 else shape[1]
+
+
+def _on(dev: int):
+    """`dev` as the current device: kernels are launched on the current one, whatever their stream's"""
+    return _HERE if dev == torch.cuda.current_device() else torch.cuda.device(dev)
 
 
 def latent_append(q: torch.Tensor, kva: torch.Tensor, weight: torch.Tensor, eps: float, batch, cache, kv: torch.Tensor, heads: int, nope: int, rot=None, inv_freq: Optional[torch.Tensor] = None,
@@ -63,31 +78,30 @@ def latent_append(q: torch.Tensor, kva: torch.Tensor, weight: torch.Tensor, eps:
     gain (None: no rotation), with float64 frequencies in inv_freq (or rot.inv_freq).  batch: pos, slot [T], seqs [2, portions], n_seqs; `positions` [T] int32: the angles' where they are not
     batch.pos.  Rows of tokens in none of the batch's portions are left as they were (in the new tensor: as they came)."""
     what = "latent_append"
-    T, dev, rank = q.shape[0], q.device, weight.numel()
-    width = kv.shape[-1]
+    T, dev, rank, width = q.shape[0], q.get_device(), weight.numel(), kv.shape[-1]
     rot_dim = width - rank
     if heads <= 0 or nope < 0 or rank <= 0 or rot_dim < 0:
         raise ValueError(f"{what}: {heads} heads of {nope} + {rot_dim}, cache rows of {width} for latents of {rank}")
     index = _latent_batch(what, T, dev, kv, width, batch, cache)
     q_ptr, q_stride = _rows(what, "q", q, T, heads * (nope + rot_dim), dev)
     kva_ptr, kva_stride = _rows(what, "kva", kva, T, width, dev)
-    if weight.dtype is not torch.bfloat16 or weight.device != dev or not weight.is_contiguous():
-        raise ValueError(f"{what}: weight has to be contiguous bfloat16 on {dev}")
+    if weight.dtype is not _BF16 or weight.get_device() != dev or not weight.is_contiguous():
+        raise ValueError(f"{what}: weight has to be contiguous bfloat16 on the queries' device, got {weight.dtype} on {weight.device}")
     dims = layout = split = 0
     gain, freq, at = 1.0, None, None
     if rot is not None and rot.dims:
-        f = rot.inv_freq if inv_freq is None and hasattr(rot, "inv_freq") else inv_freq
-        if f is None or torch.is_tensor(f) is False or f.numel() != rot.dims // 2 or f.dtype is not torch.float64 or f.device != dev or not f.is_contiguous():
-            raise ValueError(f"{what}: a rotation needs {rot.dims // 2} contiguous float64 frequencies on {dev}")
-        dims, layout, split, gain, freq = rot.dims, rot.layout_code, int(getattr(rot, "split", False)), float(getattr(rot, "gain", 1.0)), f.data_ptr()
+        f, dims = getattr(rot, "inv_freq", None) if inv_freq is None else inv_freq, rot.dims
+        if not isinstance(f, torch.Tensor) or f.numel() != dims // 2 or f.dtype is not _F64 or f.get_device() != dev or not f.is_contiguous():
+            raise ValueError(f"{what}: a rotation needs {dims // 2} contiguous float64 frequencies on the queries' device")
+        layout, split, gain, freq = rot.layout_code, int(getattr(rot, "split", False)), getattr(rot, "gain", 1.0), f.data_ptr()
     if positions is not None:
-        if positions.dtype is not torch.int32 or positions.device != dev or positions.shape[0] < T or positions.stride(0) != 1:
-            raise ValueError(f"{what}: positions have to be {T} contiguous int32 values on {dev}")
+        if positions.dtype is not _I32 or positions.get_device() != dev or positions.numel() < T or not positions.is_contiguous():
+            raise ValueError(f"{what}: positions have to be {T} contiguous int32 values on the queries' device")
         at = positions.data_ptr()
     out = q.new_empty((T, heads, rot_dim))
     a = native.LatentAppendParams(q_ptr, q_stride, heads, nope, kva_ptr, kva_stride, rank, rot_dim, weight.data_ptr(), eps, dims, layout, split, gain, freq, at, *index, kv.data_ptr(), out.data_ptr())
-    with device_of(dev):
-        native.check(native.lib().ktb200_latent_append(C.byref(a), T, stream_of(dev)))
+    with _on(dev):
+        native.check(native.lib().ktb200_latent_append(C.byref(a), T, _stream(dev)))
     return out
 
 
@@ -99,24 +113,24 @@ def latent_attention(q: torch.Tensor, q_rot: torch.Tensor, kv: torch.Tensor, w: 
     the tokens a sequence has on average.  batch.max_kv: no position is max_kv or more.  To `out` (a view of any row stride) or a new tensor; rows of tokens in none of the batch's portions are
     left as they were (in a new tensor: as they came)."""
     what = "latent_attention"
-    T, dev = q.shape[0], q.device
+    T, dev = q.shape[0], q.get_device()
     index = _latent_batch(what, T, dev, kv, LATENT + LATENT_ROT, batch, cache)
     q_ptr, q_stride = _rows(what, "q", q, T, heads * (nope + LATENT_ROT), dev)
-    if q_rot.numel() != T * heads * LATENT_ROT or not q_rot.is_contiguous() or q_rot.dtype is not torch.bfloat16 or q_rot.device != dev:
-        raise ValueError(f"{what}: q_rot has to be contiguous [{T}, {heads}, {LATENT_ROT}] of bfloat16 on {dev}, got {tuple(q_rot.shape)} of {q_rot.dtype} on {q_rot.device}")
-    if tuple(w.shape) != (heads * (nope + vdim), LATENT) or not w.is_contiguous() or w.dtype is not torch.bfloat16 or w.device != dev:
-        raise ValueError(f"{what}: w has to be contiguous [{heads * (nope + vdim)}, {LATENT}] of bfloat16 on {dev}, got {tuple(w.shape)} of {w.dtype} on {w.device}")
+    if q_rot.numel() != T * heads * LATENT_ROT or not q_rot.is_contiguous() or q_rot.dtype is not _BF16 or q_rot.get_device() != dev:
+        raise ValueError(f"{what}: q_rot has to be contiguous [{T}, {heads}, {LATENT_ROT}] of bfloat16 on the queries' device, got {tuple(q_rot.shape)} of {q_rot.dtype} on {q_rot.device}")
+    if w.shape != (heads * (nope + vdim), LATENT) or not w.is_contiguous() or w.dtype is not _BF16 or w.get_device() != dev:
+        raise ValueError(f"{what}: w has to be contiguous [{heads * (nope + vdim)}, {LATENT}] of bfloat16 on the queries' device, got {tuple(w.shape)} of {w.dtype} on {w.device}")
     if form not in FORMS:
         raise ValueError(f"{what}: form {form!r}: one of {', '.join(map(repr, FORMS))}")
     if out is None:
         out = q.new_empty((T, heads * vdim))
-    elif out.shape[0] != T or out.dim() != 2 or out.shape[1] != heads * vdim:
+    elif out.shape != (T, heads * vdim):
         raise ValueError(f"{what}: out has to be [{T}, {heads * vdim}], got {tuple(out.shape)}")
     out_ptr, out_stride = _rows(what, "out", out, T, heads * vdim, dev)
     a = native.LatentAttnParams(q_ptr, q_stride, q_rot.data_ptr(), heads, nope, vdim, w.data_ptr(), scale, FORMS[form], *index, kv.data_ptr(), out_ptr, out_stride)
     lib, ref, keys = native.lib(), C.byref(a), batch.max_kv
-    with device_of(dev):
+    with _on(dev):
         nbytes = lib.ktb200_latent_attn_workspace(ref, T, keys)
         ws = q.new_empty(nbytes + 512, dtype=torch.uint8) if nbytes else None      # (the allocator's blocks begin at multiples of 512 bytes)
-        native.check(lib.ktb200_latent_attn(ref, T, keys, (ws.data_ptr() + 1023) // 1024 * 1024 if nbytes else None, nbytes, stream_of(dev)))
+        native.check(lib.ktb200_latent_attn(ref, T, keys, (ws.data_ptr() + 1023) // 1024 * 1024 if nbytes else None, nbytes, _stream(dev)))
     return out
