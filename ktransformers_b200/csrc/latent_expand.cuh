@@ -1,25 +1,31 @@
 // Keys and values of the expanded form: [k | v] of row r and head h = W_h c_r for the rows that latent_gather_kernel laid side by side (bf16, K = 512).
 // Persistent pairs of CTAs (cta_group::2): a pair's tile is 256 rows x one head (bn = nope_dim + vdim columns), each CTA has 128 of the rows and brings half of the head's weight rows, which
 // both tensor cores read.
-//     warp 0 TMA ring (192 KB) of its own half, whose bytes are counted by the first CTA's barriers; warp 1 of the first CTA the pair's products; warps 4-19 results (a thread one row, every
-//     fourth run of 16 columns).  Two accumulators of bn columns.
-// Tiles run row tile fastest inside groups of kLxGroup, so that the CTAs of a wave share the weight rows and the latents through L2.
+// A head's weights (64 KB to 128 KB a CTA) stay in shared memory while the pair walks the rows: brought again for each tile they were two of four operand bytes, and at 43 bytes a cycle and SM
+// from L2 the copies bound the kernel (4049 rows, 128 heads: 120 us).
+//     warp 0 TMA: weights of a new head run by run of 64 columns as the last products of the old one are done with them, rows through a ring; a pair's bytes are counted by the first CTA's barriers
+//     warp 1 of the first CTA the pair's products; warps 4-19 results (a thread one row, every fourth run of 16 columns).  Two accumulators of bn columns.
+// Tiles stand in one line, rows fastest, cut into equal runs, one a pair.
 // Results: [head of the pass][row][bn], rows of the plan (a multiple of 128: a CTA's rows are all there or not at all), one rounding.
 #pragma once
 #include "latent_attn.cuh"
 
 namespace ktb {
 
-constexpr int kLxThreads = 640, kLxGroup = 8, kLxRing = 192 * 1024;
+constexpr int kLxThreads = 640, kLxBlocks = kLatent / 64, kLxBox = 128 * 128, kLxStages = 6;      // runs of 64 columns; 128 rows of one; the ring of rows
 struct LxMisc {
-    unsigned long long full[8], free[8], d_full[2], d_free[2];
+    unsigned long long w_full[kLxBlocks], w_free[kLxBlocks], full[kLxStages], free[kLxStages], d_full[2], d_free[2];
     uint32_t tmem_base;
 };
-constexpr int kLxSmem = kLxRing + (int)sizeof(LxMisc) + 1024;
+constexpr int kLxRing = kLxBlocks * kLxBox, kLxRoom = kLxRing + kLxStages * kLxBox, kLxSmem = kLxRoom + (int)sizeof(LxMisc) + 1024;
 static_assert(kLxSmem <= 232448, "shared memory budget");
-__host__ __device__ constexpr int lx_stage(int bn) { return 128 * 128 + bn / 2 * 128; }
-__host__ __device__ constexpr int lx_stages(int bn) { return kLxRing / lx_stage(bn) < 8 ? kLxRing / lx_stage(bn) : 8; }
 
+// a line of `line` tiles in `runs` runs that differ by one tile at most: the first tile of run i, and the run that has tile x
+__device__ __forceinline__ int latent_run(int line, int runs, int i) { return line / runs * i + min(i, line % runs); }
+__device__ __forceinline__ int latent_run_of(int line, int runs, int x) {
+    const int n = line / runs, more = line % runs, long_ones = more * (n + 1);
+    return x < long_ones ? x / (n + 1) : more + (x - long_ones) / n;
+}
 __device__ __forceinline__ void lx_cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void lx_cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ uint32_t lx_cluster_at(uint32_t addr, uint32_t rank) {
@@ -60,19 +66,31 @@ __device__ __forceinline__ void lx_mma_pair_x4(uint32_t tmem_d, uint64_t desc_a,
         "}\n" ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate), "r"(bar0), "r"(bar1) : "memory");
 }
 
+__device__ __forceinline__ void lx_commit_pair(uint32_t bar) {      // both CTAs' barrier completes when all products so far have
+    asm volatile(
+        "{\n"
+        ".reg .pred q;\n"
+        ".reg .b32 r;\n"
+        ".reg .b16 both;\n"
+        "mov.b16 both, 3;\n"
+        "elect.sync r|q, 0xffffffff;\n"
+        "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], both;\n"
+        "}\n" ::"r"(bar)
+        : "memory");
+}
+
 // lat: rows of [512 | 64] (the first 512 columns are read); wmap: rows of w
 __global__ void __launch_bounds__(kLxThreads, 1) __cluster_dims__(2, 1, 1)
     latent_expand_kernel(const __grid_constant__ CUtensorMap lat, const __grid_constant__ CUtensorMap wmap, const int* plan, __nv_bfloat16* out, int bn, int heads, int pass) {
     using namespace umma;
     extern __shared__ __align__(16) uint8_t lx_smem_raw[];
     const uint32_t raw = smem_u32(lx_smem_raw), base = (raw + 1023u) & ~1023u;
-    LxMisc& misc = *reinterpret_cast<LxMisc*>(lx_smem_raw + (base - raw) + kLxRing);
+    LxMisc& misc = *reinterpret_cast<LxMisc*>(lx_smem_raw + (base - raw) + kLxRoom);
     const int tid = threadIdx.x, lane = tid & 31, warp = uniform(tid >> 5), rank = blockIdx.x & 1, pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
-    const int stage = lx_stage(bn), stages = lx_stages(bn);
-    constexpr int kBlocks = kLatent / 64;
     griddep_launch_dependents();
     if (tid == 0) {
-        for (int s = 0; s < 8; s++) { bar_init(smem_u32(&misc.full[s]), 1); bar_init(smem_u32(&misc.free[s]), 1); }
+        for (int s = 0; s < kLxBlocks; s++) { bar_init(smem_u32(&misc.w_full[s]), 1); bar_init(smem_u32(&misc.w_free[s]), 1); }
+        for (int s = 0; s < kLxStages; s++) { bar_init(smem_u32(&misc.full[s]), 1); bar_init(smem_u32(&misc.free[s]), 1); }
         for (int b = 0; b < 2; b++) { bar_init(smem_u32(&misc.d_full[b]), 1); bar_init(smem_u32(&misc.d_free[b]), 32); }
         bar_fence_init();
         tma_prefetch_desc(&lat);
@@ -89,56 +107,60 @@ __global__ void __launch_bounds__(kLxThreads, 1) __cluster_dims__(2, 1, 1)
     tc_fence_after();
     const uint32_t tmem = uniform(misc.tmem_base);
     griddep_wait();
-    const int rows = plan[kPlanRows], h0 = pass * plan[kPlanHeads], nt = min(plan[kPlanHeads], heads - h0), mt = (rows + 255) / 256, tiles = nt > 0 ? mt * nt : 0;
-    auto place = [&](int tile, int& m0, int& h) {
-        const int per = kLxGroup * nt, g = tile / per, r = tile - g * per, gm = min(kLxGroup, mt - g * kLxGroup);
-        h = r / gm;
-        m0 = (g * kLxGroup + r % gm) * 256 + rank * 128;
-    };
+    const int rows = plan[kPlanRows], h0 = pass * plan[kPlanHeads], nt = min(plan[kPlanHeads], heads - h0), mt = (rows + 255) / 256, line = nt > 0 ? mt * nt : 0;
+    const int first = latent_run(line, pairs, pair), end = latent_run(line, pairs, pair + 1);
     if (warp == 0) {
-        if (lane == 0) {
-            int s = 0, ph = 1;
-            for (int tile = pair; tile < tiles; tile += pairs) {
-                int m0, h;
-                place(tile, m0, h);
-                for (int kb = 0; kb < kBlocks; kb++) {
+        if (lane == 0 && first < end) {
+            int s = 0, ph = 1, h = first / mt, m = first - h * mt, wph = 1;
+            for (int tile = first; tile < end; tile++) {
+                const bool fresh = tile == first || m == 0;
+                for (int kb = 0; kb < kLxBlocks; kb++) {
+                    if (fresh) {
+                        bar_wait(smem_u32(&misc.w_free[kb]), wph);
+                        if (rank == 0) bar_expect_tx(smem_u32(&misc.w_full[kb]), bn * 128);
+                        lx_load_pair(base + kb * kLxBox, &wmap, lx_cluster_at(smem_u32(&misc.w_full[kb]), 0), kb * 64, (h0 + h) * bn + rank * (bn / 2));
+                    }
                     bar_wait(smem_u32(&misc.free[s]), ph);
-                    const uint32_t dst = base + s * stage, bar = lx_cluster_at(smem_u32(&misc.full[s]), 0);
-                    if (rank == 0) bar_expect_tx(smem_u32(&misc.full[s]), 2 * stage);
-                    lx_load_pair(dst, &lat, bar, kb * 64, m0);
-                    lx_load_pair(dst + 128 * 128, &wmap, bar, kb * 64, (h0 + h) * bn + rank * (bn / 2));
-                    if (++s == stages) { s = 0; ph ^= 1; }
+                    if (rank == 0) bar_expect_tx(smem_u32(&misc.full[s]), 2 * kLxBox);
+                    lx_load_pair(base + kLxRing + s * kLxBox, &lat, lx_cluster_at(smem_u32(&misc.full[s]), 0), kb * 64, m * 256 + rank * 128);
+                    if (++s == kLxStages) { s = 0; ph ^= 1; }
                 }
+                if (fresh) wph ^= 1;
+                if (++m == mt) { m = 0; h++; }
             }
         }
         __syncwarp();
     } else if (warp == 1 && rank == 0) {
         const uint32_t idesc = instr_desc(1, 1, 1, 0, 0, 256, 0) | ((uint32_t)(bn >> 3) << 17);
-        int s = 0, ph = 0, it = 0;
-        for (int tile = pair; tile < tiles; tile += pairs, it++) {
+        int s = 0, ph = 0, it = 0, m = first < end ? first % mt : 0, wph = 0;
+        for (int tile = first; tile < end; tile++, it++) {
             const int buf = it & 1;
+            const bool fresh = tile == first || m == 0, last = tile + 1 == end || m + 1 == mt;      // of this head's
             bar_wait(smem_u32(&misc.d_free[buf]), ((it >> 1) & 1) ^ 1);
             tc_fence_after();
-            for (int kb = 0; kb < kBlocks; kb++) {
+            for (int kb = 0; kb < kLxBlocks; kb++) {
+                if (fresh) bar_wait(smem_u32(&misc.w_full[kb]), wph);
                 bar_wait(smem_u32(&misc.full[s]), ph);
                 tc_fence_after();
-                const uint32_t a = base + s * stage, b = a + 128 * 128;
-                lx_mma_pair_x4(tmem + buf * 256, smem_desc(a, 16, 1024, kLayoutSw128), smem_desc(b, 16, 1024, kLayoutSw128), idesc, kb > 0, smem_u32(&misc.free[s]),
-                               kb + 1 == kBlocks ? smem_u32(&misc.d_full[buf]) : 0);
-                if (++s == stages) { s = 0; ph ^= 1; }
+                lx_mma_pair_x4(tmem + buf * 256, smem_desc(base + kLxRing + s * kLxBox, 16, 1024, kLayoutSw128), smem_desc(base + kb * kLxBox, 16, 1024, kLayoutSw128), idesc, kb > 0, smem_u32(&misc.free[s]),
+                               last ? smem_u32(&misc.w_free[kb]) : 0);
+                if (++s == kLxStages) { s = 0; ph ^= 1; }
             }
+            lx_commit_pair(smem_u32(&misc.d_full[buf]));
+            if (fresh) wph ^= 1;
+            if (++m == mt) m = 0;
         }
     } else if (warp >= 4) {
         const int sp = warp & 3, ch = (warp - 4) >> 2;
-        int it = 0;
-        for (int tile = pair; tile < tiles; tile += pairs, it++) {
-            int m0, h;
-            place(tile, m0, h);
+        int it = 0, h = first < end ? first / mt : 0, m = first < end ? first - h * mt : 0;
+        for (int tile = first; tile < end; tile++, it++) {
+            const int m0 = m * 256 + rank * 128;
             const int buf = it & 1, r = m0 + 32 * sp + lane;
             const uint32_t tcol = tmem + ((uint32_t)(32 * sp) << 16) + buf * 256;
             bar_wait(smem_u32(&misc.d_full[buf]), (it >> 1) & 1);
             tc_fence_after();
             __nv_bfloat16* row = out + ((long)h * rows + r) * bn;
+            if (++m == mt) { m = 0; h++; }
 #pragma unroll 1
             for (int c = 16 * ch; c < bn; c += 64) {
                 uint32_t v[16];

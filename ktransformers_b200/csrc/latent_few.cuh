@@ -36,13 +36,7 @@ struct __align__(16) FewBlock {
 // from few_blocks_at
 constexpr int kFewLine = 0, kFewBlocks = 1, kFewRuns = 2, kFewPairs = 4, kFewRun = 2;
 __host__ __device__ inline long few_blocks_at(int pairs) { return (kFewPairs + 2L * pairs + 3) / 4 * 4; }
-__host__ // the first tile of run i, of runs that differ by one tile at most, and the run that has tile x
-__device__ __forceinline__ int few_run(int line, int runs, int i) { return line / runs * i + min(i, line % runs); }
-__device__ __forceinline__ int few_run_of(int line, int runs, int x) {
-    const int n = line / runs, more = line % runs, long_ones = more * (n + 1);
-    return x < long_ones ? x / (n + 1) : more + (x - long_ones) / n;
-}
-
+__host__ 
 struct LatentFew {
     ktb200_latent_attn_params p;
     int* plan;
@@ -170,12 +164,12 @@ __global__ void __launch_bounds__(256) latent_few_prep_kernel(const LatentFew a,
     for (int b = tid; b < nb; b += 256) {      // each block finds its runs, and is the first of those that begin in it
         const int x = blocks[b].tile0, n = blocks[b].tiles;
         if (n == 0) continue;
-        const int first = few_run_of(line, runs, x), last = few_run_of(line, runs, x + n - 1);
+        const int first = latent_run_of(line, runs, x), last = latent_run_of(line, runs, x + n - 1);
         blocks[b].run0 = first;
         blocks[b].parts = last - first + 1;
-        blocks[b].late = few_run(line, runs, first) < x;
+        blocks[b].late = latent_run(line, runs, first) < x;
         for (int i = first; i <= last; i++) {
-            const int at = few_run(line, runs, i);
+            const int at = latent_run(line, runs, i);
             if (at < x) continue;
             a.plan[kFewPairs + 2 * i] = b;
             a.plan[kFewPairs + 2 * i + 1] = at - x;
@@ -185,18 +179,6 @@ __global__ void __launch_bounds__(256) latent_few_prep_kernel(const LatentFew a,
 
 struct FewMaps { CUtensorMap q, q_rot, rows, tails; };
 
-__device__ __forceinline__ void few_commit_pair(uint32_t bar) {      // both CTAs' barrier completes when all products so far have
-    asm volatile(
-        "{\n"
-        ".reg .pred q;\n"
-        ".reg .b32 r;\n"
-        ".reg .b16 both;\n"
-        "mov.b16 both, 3;\n"
-        "elect.sync r|q, 0xffffffff;\n"
-        "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], both;\n"
-        "}\n" ::"r"(bar)
-        : "memory");
-}
 // Four products of the pair, O += P V: operands of consecutive K-steps 32 bytes of P's rows and 16 rows of V apart
 __device__ __forceinline__ void few_mma_pv_x4(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
@@ -256,7 +238,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) __cluster_dims__(2, 1, 1) late
     griddep_wait();
     const int line = a.plan[kFewLine], runs = a.plan[kFewRuns], H = a.p.heads;
     const FewBlock* blocks = reinterpret_cast<const FewBlock*>(a.plan + few_blocks_at(a.pairs));
-    const int b_first = a.plan[kFewPairs + 2 * pair], t_first = a.plan[kFewPairs + 2 * pair + 1], total = pair < runs ? few_run(line, runs, pair + 1) - few_run(line, runs, pair) : 0;
+    const int b_first = a.plan[kFewPairs + 2 * pair], t_first = a.plan[kFewPairs + 2 * pair + 1], total = pair < runs ? latent_run(line, runs, pair + 1) - latent_run(line, runs, pair) : 0;
     // every role walks the pair's run the same way: segment by segment (a block's tiles t .. t + n - 1)
     if (warp == 0) {
         // ================================================================ copies
@@ -342,7 +324,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) __cluster_dims__(2, 1, 1) late
                     lx_mma_pair_x4(tmem + 256 + (i & 1) * 64, smem_desc(base + c * kFewBox, 16, 1024, kLayoutSw128), smem_desc(base + kFewOffK + c * kFewBox, 16, 1024, kLayoutSw128), idesc_qk, c > 0,
                                    smem_u32(&misc.k_free[c]), c == kFewK - 1 ? smem_u32(&misc.s_full[i & 1]) : 0);
                 }
-                if (last) few_commit_pair(smem_u32(&misc.q_free));
+                if (last) lx_commit_pair(smem_u32(&misc.q_free));
             };
             bar_wait(smem_u32(&misc.q_full), seg & 1);
             scores(it, n == 1);
@@ -357,9 +339,9 @@ __global__ void __launch_bounds__(kFewThreads, 1) __cluster_dims__(2, 1, 1) late
                     tc_fence_after();
                     few_mma_pv_x4(tmem + (g & 1) * 128, smem_desc(base + kFewOffP + (g >> 1) * kFewBox, 16, 1024, kLayoutSw128), smem_desc(base + kFewOffV + 2 * g * kFewBox, kFewBox, 1024, kLayoutSw128), idesc_pv,
                                   j > 0 || g > 1);
-                    few_commit_pair(smem_u32(&misc.v_free[g]));
+                    lx_commit_pair(smem_u32(&misc.v_free[g]));
                 }
-                few_commit_pair(smem_u32(&misc.pv_done));
+                lx_commit_pair(smem_u32(&misc.pv_done));
             }
             it += n;
             left -= n;
