@@ -353,7 +353,7 @@ template <int N, int V> static int latent_expanded(const ktb200_latent_attn_para
     LatentPrompt a{(const int*)(ws + y.plan), (const uint32_t*)(ws + y.bad), p->n_seqs, p->heads, 0, y.parts > 1 ? y.part : 0, y.parts, p->scale * 1.4426950408889634f, (__nv_bfloat16*)p->out, p->out_stride,
                    (float*)(ws + y.o_part), (float*)(ws + y.ml_part)};
     for (a.pass = 0; a.pass < y.passes; a.pass++) {
-        KTB_CUDA_CHECK(launch_pdl(latent_expand_kernel, dim3((unsigned)(2 * std::min<long>((long)mt * p->heads, pairs))), dim3(kLxThreads), (size_t)kLxSmem, s, lat, w, a.plan, (__nv_bfloat16*)(ws + y.kv), BN,
+        KTB_CUDA_CHECK(launch_pdl(latent_expand_kernel, dim3((unsigned)(2 * std::min<long>((long)mt * p->heads, pairs))), dim3(kLxThreads), (size_t)kLxSmem, s, lat, w, m.k, a.plan, BN,
                                   p->heads, a.pass));
         KTB_CUDA_CHECK(launch_pdl(latent_prompt_kernel<N, V>, dim3(ctas, 1, y.parts), dim3(kLpThreads), (size_t)kLpSmem, s, m, a));
         count_launch(2);

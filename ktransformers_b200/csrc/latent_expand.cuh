@@ -4,7 +4,8 @@
 // A head's weights (64 KB to 128 KB a CTA) stay in shared memory while the pair walks the rows: brought again for each tile they were two of four operand bytes, and at 43 bytes a cycle and SM
 // from L2 the copies bound the kernel (4049 rows, 128 heads: 120 us).
 //     warp 0 TMA: weights of a new head run by run of 64 columns as the last products of the old one are done with them, rows through a ring; a pair's bytes are counted by the first CTA's barriers
-//     warp 1 of the first CTA the pair's products; warps 4-19 results (a thread one row, every fourth run of 16 columns).  Two accumulators of bn columns.
+//     warp 1 of the first CTA the pair's products; warps 4-7 and 8-11 results, 64 columns at a time through shared memory and out by TMA.  Two accumulators of bn columns.  (Sectors of 32 bytes
+//     stored by the threads took 120 us for 4049 rows and 128 heads, 86 without the stores: a tile has only 512 columns of products to hide its 64 KB of results behind)
 // Tiles stand in one line, rows fastest, cut into equal runs, one a pair.
 // Results: [head of the pass][row][bn], rows of the plan (a multiple of 128: a CTA's rows are all there or not at all), one rounding.
 #pragma once
@@ -12,12 +13,12 @@
 
 namespace ktb {
 
-constexpr int kLxThreads = 640, kLxBlocks = kLatent / 64, kLxBox = 128 * 128, kLxStages = 6;      // runs of 64 columns; 128 rows of one; the ring of rows
+constexpr int kLxThreads = 384, kLxBlocks = kLatent / 64, kLxBox = 128 * 128, kLxStages = 4;      // runs of 64 columns; 128 rows of one; the ring of rows
 struct LxMisc {
     unsigned long long w_full[kLxBlocks], w_free[kLxBlocks], full[kLxStages], free[kLxStages], d_full[2], d_free[2];
     uint32_t tmem_base;
 };
-constexpr int kLxRing = kLxBlocks * kLxBox, kLxRoom = kLxRing + kLxStages * kLxBox, kLxSmem = kLxRoom + (int)sizeof(LxMisc) + 1024;
+constexpr int kLxRing = kLxBlocks * kLxBox, kLxOut = kLxRing + kLxStages * kLxBox, kLxRoom = kLxOut + 2 * kLxBox, kLxSmem = kLxRoom + (int)sizeof(LxMisc) + 1024;
 static_assert(kLxSmem <= 232448, "shared memory budget");
 
 // a line of `line` tiles in `runs` runs that differ by one tile at most: the first tile of run i, and the run that has tile x
@@ -79,9 +80,9 @@ __device__ __forceinline__ void lx_commit_pair(uint32_t bar) {      // both CTAs
         : "memory");
 }
 
-// lat: rows of [512 | 64] (the first 512 columns are read); wmap: rows of w
+// lat: rows of [512 | 64] (the first 512 columns are read); wmap: rows of w; out: rows of bn columns, boxes of 128 x 64
 __global__ void __launch_bounds__(kLxThreads, 1) __cluster_dims__(2, 1, 1)
-    latent_expand_kernel(const __grid_constant__ CUtensorMap lat, const __grid_constant__ CUtensorMap wmap, const int* plan, __nv_bfloat16* out, int bn, int heads, int pass) {
+    latent_expand_kernel(const __grid_constant__ CUtensorMap lat, const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap out, const int* plan, int bn, int heads, int pass) {
     using namespace umma;
     extern __shared__ __align__(16) uint8_t lx_smem_raw[];
     const uint32_t raw = smem_u32(lx_smem_raw), base = (raw + 1023u) & ~1023u;
@@ -91,7 +92,7 @@ __global__ void __launch_bounds__(kLxThreads, 1) __cluster_dims__(2, 1, 1)
     if (tid == 0) {
         for (int s = 0; s < kLxBlocks; s++) { bar_init(smem_u32(&misc.w_full[s]), 1); bar_init(smem_u32(&misc.w_free[s]), 1); }
         for (int s = 0; s < kLxStages; s++) { bar_init(smem_u32(&misc.full[s]), 1); bar_init(smem_u32(&misc.free[s]), 1); }
-        for (int b = 0; b < 2; b++) { bar_init(smem_u32(&misc.d_full[b]), 1); bar_init(smem_u32(&misc.d_free[b]), 32); }
+        for (int b = 0; b < 2; b++) { bar_init(smem_u32(&misc.d_full[b]), 1); bar_init(smem_u32(&misc.d_free[b]), 16); }
         bar_fence_init();
         tma_prefetch_desc(&lat);
         tma_prefetch_desc(&wmap);
@@ -151,32 +152,45 @@ __global__ void __launch_bounds__(kLxThreads, 1) __cluster_dims__(2, 1, 1)
             if (++m == mt) m = 0;
         }
     } else if (warp >= 4) {
-        const int sp = warp & 3, ch = (warp - 4) >> 2;
+        const int sp = warp & 3, half = (warp - 4) >> 2, r = 32 * sp + lane;
+        const bool lead = warp == 4 + 4 * half && lane == 0;      // of the four warps that share a box
+        const uint32_t box = base + kLxOut + half * kLxBox;
         int it = 0, h = first < end ? first / mt : 0, m = first < end ? first - h * mt : 0;
         for (int tile = first; tile < end; tile++, it++) {
-            const int m0 = m * 256 + rank * 128;
-            const int buf = it & 1, r = m0 + 32 * sp + lane;
+            const int m0 = m * 256 + rank * 128, row0 = h * rows + m0, buf = it & 1;
             const uint32_t tcol = tmem + ((uint32_t)(32 * sp) << 16) + buf * 256;
+            if (++m == mt) { m = 0; h++; }
             bar_wait(smem_u32(&misc.d_full[buf]), (it >> 1) & 1);
             tc_fence_after();
-            __nv_bfloat16* row = out + ((long)h * rows + r) * bn;
-            if (++m == mt) { m = 0; h++; }
 #pragma unroll 1
-            for (int c = 16 * ch; c < bn; c += 64) {
-                uint32_t v[16];
-                tmem_ld16(tcol + c, v);
-                tmem_wait_ld();
-                if (m0 < rows) {      // (whole sectors of the thread's own row)
-                    uint32_t w[8];
+            for (int c = 64 * half; c < bn; c += 128) {
+                uint32_t w[32];
 #pragma unroll
-                    for (int i = 0; i < 8; i++) w[i] = latent_pack(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
-                    latent_store32(row + c, w);
+                for (int q = 0; q < 2; q++) {
+                    uint32_t v[32];
+                    tmem_ld32(tcol + c + 32 * q, v);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int i = 0; i < 16; i++) w[16 * q + i] = latent_pack(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
+                }
+                if (lead) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");      // (the box before has left)
+                asm volatile("barrier.cta.sync %0, 128;" ::"r"(1 + half) : "memory");
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+                    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(box + r * 128 + ((i ^ (r & 7)) << 4)), "r"(w[4 * i]), "r"(w[4 * i + 1]), "r"(w[4 * i + 2]), "r"(w[4 * i + 3]) : "memory");
+                fence_async_smem();
+                asm volatile("barrier.cta.sync %0, 128;" ::"r"(1 + half) : "memory");
+                if (lead && m0 < rows) {
+                    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(&out), "r"(box), "r"(c), "r"(row0) : "memory");
+                    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
                 }
             }
             tc_fence_before();
             __syncwarp();
             if (lane == 0) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(lx_cluster_at(smem_u32(&misc.d_free[buf]), 0)) : "memory");
         }
+        if (lead) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+        __syncwarp();
     }
     tc_fence_before();
     __syncthreads();
