@@ -437,7 +437,7 @@ typedef struct ktb200_latent_attn_params {
     const int* page_table; int n_slots, max_pages, page_size, n_pages;
     const void* cache; void* out; long out_stride;
 } ktb200_latent_attn_params;
-int ktb200_latent_attn_form(const ktb200_latent_attn_params* p, int n_tokens);
+int ktb200_latent_attn_form(const ktb200_latent_attn_params* p, int n_tokens, int max_kv);
 size_t ktb200_latent_attn_workspace(const ktb200_latent_attn_params* p, int n_tokens, int max_kv);
 int ktb200_latent_attn(const ktb200_latent_attn_params* p, int n_tokens, int max_kv, void* workspace, size_t workspace_bytes, void* stream);
 

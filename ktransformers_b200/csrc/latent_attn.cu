@@ -16,16 +16,21 @@
 namespace ktb {
 
 constexpr size_t kLxBytes = (size_t)2 << 30;
-constexpr int kLatentFew = 64;      // tokens a sequence on average from which the expanded form takes less
+// Tokens a sequence on average from which the expanded form takes less, by the call's keys.  128 heads, absorbed / expanded: 64 tokens behind 1000 66 / 68 us, 96 95 / 68; behind 8000 96 241 / 325,
+// 128 303 / 327; behind 30000 128 1032 / 1331; 8 x 128 behind 4000 818 / 953.  16 heads: 128 behind 1000 42 / 44, behind 30000 146 / 206.  (What the expanded form makes of the keys is the same for
+// all numbers of tokens, but with few keys its launches and first tiles are most of it)
+constexpr int kLatentFew = 144, kLatentFewShort = 64, kLatentShort = 2048;
 
 // ------------------------------------------------------------------------------------------------ plan and rows
 // one warp: portions in order, 32 side by side
+constexpr int kPlanSort = 256;      // query tiles that are sorted
 __global__ void __launch_bounds__(32) latent_plan_kernel(const ktb200_latent_attn_params p, int n_tokens, int row_cap, int tile_cap, long rows_of_heads, int* plan) {
     griddep_wait();
     griddep_launch_dependents();      // (as absorb_kernel: behind the wait)
     const int lane = threadIdx.x;
     int* off = plan + kPlanSeqs;
     int4* tiles = reinterpret_cast<int4*>(plan + plan_tiles_at(p.n_seqs));
+    __shared__ int4 held[kPlanSort];
     int rows = 0, nt = 0;
     for (int s0 = 0; s0 < p.n_seqs; s0 += 32) {
         const int s = s0 + lane;
@@ -50,17 +55,34 @@ __global__ void __launch_bounds__(32) latent_plan_kernel(const ktb200_latent_att
             off[p.n_seqs + 1 + s] = keys;
             for (int i = 0; i < q; i++) {      // the last tokens, which see most keys, first
                 const int at = nt + qs - q + i, o = (q - 1 - i) * kPlanTokens;
-                if (at < tile_cap) tiles[at] = make_int4(first + o, min(kPlanTokens, count - o), pos + o, s);
+                const int4 tile = make_int4(first + o, min(kPlanTokens, count - o), pos + o, s);
+                if (at < tile_cap) tiles[at] = tile;
+                if (at < kPlanSort) held[at] = tile;
             }
         }
         rows += __shfl_sync(0xffffffffu, rs, 31);
         nt += __shfl_sync(0xffffffffu, qs, 31);
     }
+    // tiles that see most keys first, so that the last CTAs to start have least to do
+    nt = min(nt, tile_cap);
+    if (nt <= kPlanSort) {
+        __syncwarp();
+        for (int i = lane; i < nt; i += 32) {
+            const int4 tile = held[i];
+            const int keys = tile.z + tile.y;
+            int before = 0;
+            for (int k = 0; k < nt; k++) {
+                const int other = held[k].z + held[k].y;
+                before += other > keys || (other == keys && k < i);
+            }
+            tiles[before] = tile;
+        }
+    }
     if (lane == 0) {
         off[p.n_seqs] = rows;
         plan[kPlanRows] = rows;
         plan[kPlanHeads] = rows > 0 ? (int)min((long)p.heads, rows_of_heads / rows) : p.heads;
-        plan[kPlanTiles] = min(nt, tile_cap);
+        plan[kPlanTiles] = nt;
         plan[kPlanBad] = 0;
     }
 }
@@ -244,13 +266,13 @@ struct LatentLayout {      // of the workspace: byte offsets, and what the sizes
     size_t plan, lat, bad, kv, o_part, ml_part, few, there, tails, tail_bad, q_abs, sums, total;
     long rows_of_heads;      // expanded rows, one a head, that there is room for
 };
-static int latent_form(const ktb200_latent_attn_params* p, int n_tokens) {
+static int latent_form(const ktb200_latent_attn_params* p, int n_tokens, int max_kv) {
     if (p->form) return p->form;
-    return (long)n_tokens >= (long)kLatentFew * p->n_seqs ? 2 : 1;
+    return (long)n_tokens >= (long)(max_kv <= kLatentShort ? kLatentFewShort : kLatentFew) * p->n_seqs ? 2 : 1;
 }
 static int latent_layout(LatentLayout& y, const ktb200_latent_attn_params* p, int n_tokens, int max_kv) {
     y = LatentLayout{};
-    y.form = latent_form(p, n_tokens);
+    y.form = latent_form(p, n_tokens, max_kv);
     int device = 0;
     KTB_CUDA_CHECK(cudaGetDevice(&device));
     size_t at = 0;
@@ -397,7 +419,7 @@ using namespace ktb;
 
 extern "C" {
 
-int ktb200_latent_attn_form(const ktb200_latent_attn_params* p, int n_tokens) { return p ? latent_form(p, n_tokens) : 0; }
+int ktb200_latent_attn_form(const ktb200_latent_attn_params* p, int n_tokens, int max_kv) { return p ? latent_form(p, n_tokens, max_kv) : 0; }
 
 size_t ktb200_latent_attn_workspace(const ktb200_latent_attn_params* p, int n_tokens, int max_kv) {
     LatentLayout y;

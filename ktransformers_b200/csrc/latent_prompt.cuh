@@ -13,6 +13,7 @@
 namespace ktb {
 
 constexpr int kLpThreads = 384, kLpBlock = 16384, kLpRoom = 229376;      // bytes of a ring block; of queries and ring
+constexpr long kLpFits = 96l << 20;
 struct LpMaps { CUtensorMap q, q_rot, k, k_rot, v; };
 struct LpMisc {
     unsigned long long q_full, full[12], free[12], s_full[2], p_full[2][2], o_done[2];
@@ -52,9 +53,11 @@ template <int N, int V> __global__ void __launch_bounds__(kLpThreads, 1) latent_
     griddep_wait();
     const int rows = a.plan[kPlanRows], nqt = a.plan[kPlanTiles], h0 = a.pass * a.plan[kPlanHeads], nh = min(a.plan[kPlanHeads], a.heads - h0);
     if (nh <= 0 || (long)blockIdx.x >= (long)nh * nqt) return;
-    // a head's query tiles are neighbours: those that run together share its keys and values through L2
-    const int hl = blockIdx.x / nqt, h = h0 + hl;
-    const int4 item = reinterpret_cast<const int4*>(a.plan + plan_tiles_at(a.n_seqs))[blockIdx.x % nqt];
+    // keys and values that all fit in L2: the tiles that see most keys first, of all heads; else a head's tiles are neighbours, so that those that run together share its keys and values
+    // (1000 tokens: 108 us in heads' order, 104 so; 2048 behind 2001: 535, and 564 so)
+    const bool by_tile = (long)rows * nh * (N + V) * 2 <= kLpFits;
+    const int hl = by_tile ? blockIdx.x % nh : blockIdx.x / nqt, h = h0 + hl;
+    const int4 item = reinterpret_cast<const int4*>(a.plan + plan_tiles_at(a.n_seqs))[by_tile ? blockIdx.x / nh : blockIdx.x % nqt];
     const int tok0 = item.x, ntok = item.y, pos0 = item.z, row0 = a.plan[kPlanSeqs + item.w], keys = min(pos0 + ntok, a.plan[kPlanSeqs + a.n_seqs + 1 + item.w]);
     const bool cut = a.part > 0;
     const int k_lo = cut ? blockIdx.z * a.part : 0, k_hi = cut ? min(keys, k_lo + a.part) : keys, n = (k_hi - k_lo + kLatentTile - 1) / kLatentTile, tiles = ntok > 128 ? 2 : 1;

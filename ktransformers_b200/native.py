@@ -140,7 +140,7 @@ class LatentAttnParams(C.Structure):
 
 SYMBOLS |= {
     "ktb200_latent_append": (_I, [C.POINTER(LatentAppendParams), _I, _VP]),
-    "ktb200_latent_attn_form": (_I, [C.POINTER(LatentAttnParams), _I]),
+    "ktb200_latent_attn_form": (_I, [C.POINTER(LatentAttnParams), _I, _I]),
     "ktb200_latent_attn_workspace": (C.c_size_t, [C.POINTER(LatentAttnParams), _I, _I]),
     "ktb200_latent_attn": (_I, [C.POINTER(LatentAttnParams), _I, _I, _VP, C.c_size_t, _VP]),
 }

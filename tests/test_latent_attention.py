@@ -307,8 +307,9 @@ def test_attention_refuses_on_the_host(wrong):
 
 
 def test_form_follows_the_tokens_a_sequence():
-    form = lambda T, n, f=0: native.lib().ktb200_latent_attn_form(C.byref(attn_params(n_seqs=n, form=f)), T)
-    assert form(1, 1) == 1 and form(2000, 1) == 2 and form(40, 40) == 1 and form(4000, 4) == 2 and form(1, 1, 2) == 2 and form(4000, 1, 1) == 1
+    form = lambda T, n, keys=9000, f=0: native.lib().ktb200_latent_attn_form(C.byref(attn_params(n_seqs=n, form=f)), T, keys)
+    assert form(1, 1) == 1 and form(2000, 1) == 2 and form(40, 40) == 1 and form(4000, 4) == 2 and form(1, 1, f=2) == 2 and form(4000, 1, f=1) == 1
+    assert form(100, 1, keys=1000) == 2 and form(100, 1) == 1 and form(63, 1, keys=1000) == 1
 
 
 @pytest.mark.parametrize("wrong", [dict(heads=0), dict(kv_rank=0), dict(rot_dims=66), dict(rot_dims=7), dict(rot_layout=2), dict(inv_freq=0), dict(q_stride=1), dict(kva_stride=575), dict(page_size=0),
