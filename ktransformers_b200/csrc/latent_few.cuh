@@ -10,6 +10,8 @@
 //     tile's outgrows it by 2^8
 // All tiles of all blocks stand in one line that is cut into equal runs, one a pair; blocks that are cut leave fp32 parts for latent_few_merge_kernel, whole ones are done.
 // Tiles that not all rows see whole, or whose last rows are not there, come from `tails`: copies with zeros for what is not there or not finite (latent_few_prep_kernel).
+// Bound by the copies: 278 KB a pair and tile from L2 at 12 TB/s, 3900 cycles of which products take 2518 (45 tokens behind 30000 keys: 334 us, 180 with the copies left out, 250 with the products
+// left out); keys' tiles in L2 ahead of their use did not help (358).
 // Shared memory: queries 72 KB, keys 72, values 64, weights 16.  TMEM: O 256 columns, S two buffers of 64.
 #pragma once
 #include "latent_attn.cuh"
@@ -143,7 +145,8 @@ __global__ void __launch_bounds__(256) latent_few_prep_kernel(const LatentFew a,
         const int b0 = carry[0] + scan(nb, all_b), t0 = carry[1] + scan(nt, all_t);
         const bool room = b0 + nb <= a.block_cap && t0 + nt <= a.tail_cap;      // (portions that share tokens may not have it)
         for (int b = 0; b < nb && b0 + b < a.block_cap; b++) {
-            const int lead = b * kFewRows, n = (int)min((long)kFewRows, rows - lead), keys = q.pos + (lead + n - 1) / H + 1;
+            // (rows side by side hold the call's max_kv of a portion and no more: what a call says of more is not there)
+            const int lead = b * kFewRows, n = (int)min((long)kFewRows, rows - lead), all = q.pos + (lead + n - 1) / H + 1, keys = a.rows_plan ? min(all, a.rows_plan[kPlanSeqs + p.n_seqs + 1 + s]) : all;
             blocks[b0 + b] = FewBlock{q.first * H + lead, n, lead, s, q.pos, 0, room ? (keys + kFewTile - 1) / kFewTile : 0, t0, 0, 0, 0, 0};
         }
         __syncthreads();

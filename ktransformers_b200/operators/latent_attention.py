@@ -63,7 +63,7 @@ def _rows(what: str, name: str, t: torch.Tensor, T: int, width: int, dev: int):
     stride, step = t.stride()
     if step != 1 and shape[1] > 1:
         raise ValueError(f"{what}: {name} has to have its columns side by side")
-    return t.data_ptr(), stride if T > 1 else shape[1]
+    return t.data_ptr(), stride if T > 1 else width      # (one row has no other)
 
 
 def _on(dev: int):

@@ -103,6 +103,30 @@ def test_attention_large_scores_and_one_key_with_all_the_weight(form):
 
 
 @gpu
+@pytest.mark.parametrize("form,page", [("expanded", 64), ("absorbed", 64), ("absorbed", 16)])
+def test_attention_with_fewer_keys_than_there_are(form, page):
+    """A max_kv that a portion's positions pass: that portion's rows are whatever they are, nothing else is touched, and the portion that keeps to it is right."""
+    d = draw([(3000, 40), (50, 60)], heads=2, page=page, seed=21)
+    want, bound = attention(d)
+    d.batch.max_kv = 128
+    got = torch.full((109, 256), 7.0, dtype=torch.bfloat16, device="cuda")
+    call(d, form, out=got[:100])
+    near(got[40:100], want[40:], bound[40:])
+    assert (got[100:] == 7).all()
+
+
+@gpu
+def test_one_row_of_any_width():
+    d = draw([(130, 1)], heads=3, seed=22)
+    want, bound = attention(d)
+    wide = torch.full((1, 3 * 192 + 5), math.nan, dtype=torch.bfloat16, device="cuda")
+    wide[:, :576] = d.q
+    d.q = wide
+    for form in ("expanded", "absorbed"):
+        near(call(d, form), want, bound)
+
+
+@gpu
 def test_attention_in_passes_over_the_heads():
     """More keys and values than one pass holds (40,000 keys of 128 heads are 2.6 GB); with a bound far above the keys there are, the passes behind the first find nothing to do."""
     d = draw([(39936, 64)], heads=128, seed=9)
