@@ -18,7 +18,7 @@ from ..models.modeling_deepseek_v3 import yarn_inv_freq  # noqa: F401  (the freq
 
 FORMS = {None: 0, "absorbed": 1, "expanded": 2}
 LATENT, LATENT_ROT = 512, 64
-_HERE, _stream = contextlib.nullcontext(), torch._C._cuda_getCurrentRawStream      # (the current stream of a device as the C-ABI takes it)
+_HERE, _stream = contextlib.nullcontext(), getattr(torch._C, "_cuda_getCurrentRawStream", None)      # (the current stream of a device as the C-ABI takes it)
 
 
 class LatentRotation:
