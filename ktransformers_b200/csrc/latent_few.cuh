@@ -357,6 +357,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) __cluster_dims__(2, 1, 1) late
         const int sp = warp & 3, half = sp >> 1, r = 32 * (sp & 1) + lane;      // TMEM lane 32 sp + lane: the row r and the tile's keys (or O's columns) of this half
         const uint32_t tl = tmem + ((uint32_t)(32 * sp) << 16);
         const float c = a.scale_log2;
+        const bool any_bad = a.rows_plan && a.rows_plan[kPlanBad] != 0;      // (rows side by side are copies, all of them; other tiles ahead of the tails are as the cache holds them)
         int left = total, b = b_first, t = t_first, it = 0, seg = 0;
         while (left > 0) {
             const FewBlock k = blocks[b];
@@ -381,7 +382,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) __cluster_dims__(2, 1, 1) late
                 // (the loads above are in registers only now)
 #pragma unroll
                 for (int x = 0; x < 64; x++) asm volatile("" : "+f"(s[x]));
-                if (t + j >= tail) {      // (a tile that not all rows see whole, or one of the portion's last)
+                if (any_bad || t + j >= tail) {
                     const uint32_t* bits = a.rows_plan ? a.bad + (a.rows_plan[kPlanSeqs + k.seq] + k0) / 32 : a.tail_bad + ((k.tail + t + j - tail) * kFewTile + 64 * half) / 32;
                     const uint2 w = *reinterpret_cast<const uint2*>(bits);
                     if (w.x | w.y) {
@@ -389,6 +390,8 @@ __global__ void __launch_bounds__(kFewThreads, 1) __cluster_dims__(2, 1, 1) late
                         for (int x = 0; x < 64; x++)
                             if ((x < 32 ? w.x : w.y) >> (x & 31) & 1) s[x] = __int_as_float(0x7fffffff);
                     }
+                }
+                if (t + j >= tail) {      // (a tile that not all rows see whole, or one of the portion's last)
                     const int i1 = p - k0;
 #pragma unroll
                     for (int x = 0; x < 64; x++)
