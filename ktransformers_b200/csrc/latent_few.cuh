@@ -528,8 +528,7 @@ __global__ void __launch_bounds__(256) latent_few_merge_kernel(const LatentFew a
 #pragma unroll
         for (int x = 0; x < 4; x++) v[x] = *reinterpret_cast<const float4*>(a.o_part + at(i) * kLatent + x * 128 + lane * 4);
         nan |= ml.y != ml.y;
-        const float w = ml.x == -INFINITY ? 0.f : latent_exp2(ml.x - m);
-        if (w == 0.f) continue;
+        const float w = ml.x == -INFINITY ? 0.f : latent_exp2(ml.x - m);      // (0: what is not finite in the part's sum still makes the row NaN)
         l = fmaf(ml.y, w, l);
 #pragma unroll
         for (int x = 0; x < 4; x++) { o[4 * x] = fmaf(v[x].x, w, o[4 * x]); o[4 * x + 1] = fmaf(v[x].y, w, o[4 * x + 1]); o[4 * x + 2] = fmaf(v[x].z, w, o[4 * x + 2]); o[4 * x + 3] = fmaf(v[x].w, w, o[4 * x + 3]); }
