@@ -104,8 +104,9 @@ template <bool VEC, int ITEMS, int LAYOUT> __global__ void __launch_bounds__(kLa
             for (int i = 0; i < 2; i++) held[i] = lane + 32 * i < pieces ? reinterpret_cast<const uint4*>(row)[lane + 32 * i] : make_uint4(0, 0, 0, 0);
         const int pos = p.pos[t], slot = p.slot[t];
         for (int i = lane; i < half; i += 32) cs[warp][i] = latent_turn(p, t, i);
-        if (!latent_in_portion(p.seqs, p.seqs_stride, p.n_seqs, t) || pos < 0 || (unsigned)slot >= (unsigned)p.n_slots) return;
-        const int page = p.page_table[(long)slot * p.max_pages + (pos / p.page_size) % p.max_pages];
+        const int column = pos / p.page_size;      // (a position behind the last column has no row: nothing to write to)
+        if (!latent_in_portion(p.seqs, p.seqs_stride, p.n_seqs, t) || pos < 0 || column >= p.max_pages || (unsigned)slot >= (unsigned)p.n_slots) return;
+        const int page = p.page_table[(long)slot * p.max_pages + column];
         if ((unsigned)page >= (unsigned)p.n_pages) return;
         __nv_bfloat16* dst = (__nv_bfloat16*)p.cache + ((long)page * p.page_size + pos % p.page_size) * width;
         float sum = 0.f;

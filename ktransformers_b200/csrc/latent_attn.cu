@@ -27,7 +27,7 @@ constexpr int kPlanSort = 256;      // query tiles that are sorted
 __global__ void __launch_bounds__(32) latent_plan_kernel(const ktb200_latent_attn_params p, int n_tokens, int row_cap, int tile_cap, long rows_of_heads, int* plan) {
     griddep_wait();
     griddep_launch_dependents();      // (as absorb_kernel: behind the wait)
-    const int lane = threadIdx.x;
+    const int lane = threadIdx.x, room = latent_room(p);
     int* off = plan + kPlanSeqs;
     int4* tiles = reinterpret_cast<int4*>(plan + plan_tiles_at(p.n_seqs));
     __shared__ int4 held[kPlanSort];
@@ -41,7 +41,7 @@ __global__ void __launch_bounds__(32) latent_plan_kernel(const ktb200_latent_att
             if (count > 0 && first >= 0 && first <= n_tokens - count) pos = p.pos[first];
             else count = 0;
             if (count > 0 && (pos < 0 || (unsigned)p.slot[first] >= (unsigned)p.n_slots)) count = 0;
-            keys = count > 0 ? (int)min((long)pos + count, (long)row_cap) : 0;
+            keys = count > 0 ? (int)min((long)pos + count, (long)min(row_cap, room)) : 0;
         }
         const int r = (keys + kLatentTile - 1) / kLatentTile * kLatentTile, q = (count + kPlanTokens - 1) / kPlanTokens;
         int rs = r, qs = q;
@@ -107,7 +107,7 @@ __global__ void __launch_bounds__(256) latent_gather_kernel(const ktb200_latent_
             for (int i = 0; i < 4; i++) {
                 const int key = key0 + 4 * warp + i;
                 int page = -1;
-                if (key < keys) page = p.page_table[(long)slot * p.max_pages + (key / p.page_size) % p.max_pages];
+                if (key < keys) page = p.page_table[(long)slot * p.max_pages + key / p.page_size];
                 const bool there = (unsigned)page < (unsigned)p.n_pages;
                 if (latent_copy_row((const __nv_bfloat16*)p.cache + ((long)page * p.page_size + key % p.page_size) * kLatentRow, there, lat + (long)(r0 + 4 * warp + i) * kLatentRow, true)) mine |= 1u << (4 * warp + i);
             }

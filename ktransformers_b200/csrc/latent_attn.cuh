@@ -14,6 +14,11 @@ constexpr int kLatent = 512, kLatentRot = 64, kLatentRow = kLatent + kLatentRot,
 constexpr int kPlanRows = 0, kPlanHeads = 1, kPlanTiles = 2, kPlanBad = 3, kPlanSeqs = 4, kPlanTokens = 256;      // kPlanTokens: of a query tile
 __host__ __device__ inline long plan_tiles_at(int n_seqs) { return ((long)kPlanSeqs + 2 * n_seqs + 1 + 3) / 4 * 4; }
 
+// positions that have a column of the page table: keys from there on are not there, and tokens at such positions see those that are
+__host__ __device__ inline int latent_room(const ktb200_latent_attn_params& p) {
+    const long n = (long)p.max_pages * p.page_size;
+    return n < 0x7fffff00L ? (int)n : 0x7fffff00;
+}
 __device__ __forceinline__ uint32_t latent_pack(float lo, float hi) {
     const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&v);

@@ -32,7 +32,7 @@ static_assert(kFewSmem <= 232448, "shared memory budget");
 struct __align__(16) FewBlock {
     int row0, rows, lead, seq;      // first row of q'; rows; rows of the portion ahead of it; its portion
     int pos0, tile0, tiles, tail;   // that one's first position; its first tile in the line, its tiles, its portion's first among the tails
-    int run0, parts, late, spare;   // the run that has its first tile, the runs that have one; whether that run has tiles of another block before them
+    int run0, parts, late, whole;   // the run that has its first tile, the runs that have one; whether that run has tiles of another block before them; its portion's tiles that all rows see whole
 };
 // what latent_few_prep_kernel leaves: ints tiles of the line, blocks, pairs that have a run (of kFewRun tiles and more), then (from 4 on) for each its first block and tile in it, then FewBlock
 // from few_blocks_at
@@ -51,16 +51,18 @@ struct LatentFew {
 };
 
 // a portion as every kernel of the form sees it
-struct FewPortion { int first, count, pos, slot; };
+struct FewPortion { int first, count, pos, slot, end; };      // end: keys that its last token sees
 __device__ __forceinline__ FewPortion few_portion(const ktb200_latent_attn_params& p, int n_tokens, int s) {
-    FewPortion q{p.seqs[s], p.seqs[p.seqs_stride + s], 0, 0};
+    FewPortion q{p.seqs[s], p.seqs[p.seqs_stride + s], 0, 0, 0};
     if (q.count <= 0 || q.first < 0 || q.first > n_tokens - q.count) { q.count = 0; return q; }
     q.pos = p.pos[q.first];
     q.slot = p.slot[q.first];
     if (q.pos < 0 || q.pos > 0x7fffff00 - q.count || (unsigned)q.slot >= (unsigned)p.n_slots) q.count = 0;
+    q.end = min(q.pos + q.count, latent_room(p));
     return q;
 }
-__device__ __forceinline__ int few_tails(const FewPortion& q) { return q.count > 0 ? (q.pos + q.count - 1) / kFewTile - q.pos / kFewTile + 1 : 0; }
+__device__ __forceinline__ int few_whole(const FewPortion& q) { return min(q.pos, q.end) / kFewTile; }
+__device__ __forceinline__ int few_tails(const FewPortion& q) { return q.count > 0 ? (q.end + kFewTile - 1) / kFewTile - few_whole(q) : 0; }
 
 // CTA 0: blocks, the line, its cuts.  The others: 32 rows of the tails each
 __global__ void __launch_bounds__(256) latent_few_prep_kernel(const LatentFew a, __nv_bfloat16* tails, uint32_t* tail_bad) {
@@ -88,19 +90,19 @@ __global__ void __launch_bounds__(256) latent_few_prep_kernel(const LatentFew a,
                 const int l = __ffs(has) - 1;
                 seq = s0 + l;
                 at = tile - (before + __shfl_sync(0xffffffffu, sum - n, l));
-                q = FewPortion{__shfl_sync(0xffffffffu, mine.first, l), __shfl_sync(0xffffffffu, mine.count, l), __shfl_sync(0xffffffffu, mine.pos, l), __shfl_sync(0xffffffffu, mine.slot, l)};
+                q = FewPortion{__shfl_sync(0xffffffffu, mine.first, l), __shfl_sync(0xffffffffu, mine.count, l), __shfl_sync(0xffffffffu, mine.pos, l), __shfl_sync(0xffffffffu, mine.slot, l), __shfl_sync(0xffffffffu, mine.end, l)};
                 break;
             }
             before += __shfl_sync(0xffffffffu, sum, 31);
         }
         if (seq < 0) return;
-        const int key0 = (q.pos / kFewTile + at) * kFewTile + (g & 3) * 32, keys = q.pos + q.count;
+        const int key0 = (few_whole(q) + at) * kFewTile + (g & 3) * 32, keys = q.end;
         uint32_t mine = 0;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const int key = key0 + 4 * warp + i;
             int page = -1;
-            if (key < keys) page = p.page_table[(long)q.slot * p.max_pages + (key / p.page_size) % p.max_pages];
+            if (key < keys) page = p.page_table[(long)q.slot * p.max_pages + key / p.page_size];
             const bool there = (unsigned)page < (unsigned)p.n_pages;
             if (latent_copy_row((const __nv_bfloat16*)p.cache + ((long)page * p.page_size + key % p.page_size) * kLatentRow, there, tails + ((long)g * 32 + 4 * warp + i) * kLatentRow, true)) mine |= 1u << (4 * warp + i);
         }
@@ -146,8 +148,8 @@ __global__ void __launch_bounds__(256) latent_few_prep_kernel(const LatentFew a,
         const bool room = b0 + nb <= a.block_cap && t0 + nt <= a.tail_cap;      // (portions that share tokens may not have it)
         for (int b = 0; b < nb && b0 + b < a.block_cap; b++) {
             // (rows side by side hold the call's max_kv of a portion and no more: what a call says of more is not there)
-            const int lead = b * kFewRows, n = (int)min((long)kFewRows, rows - lead), all = q.pos + (lead + n - 1) / H + 1, keys = a.rows_plan ? min(all, a.rows_plan[kPlanSeqs + p.n_seqs + 1 + s]) : all;
-            blocks[b0 + b] = FewBlock{q.first * H + lead, n, lead, s, q.pos, 0, room ? (keys + kFewTile - 1) / kFewTile : 0, t0, 0, 0, 0, 0};
+            const int lead = b * kFewRows, n = (int)min((long)kFewRows, rows - lead), all = min(q.pos + (lead + n - 1) / H + 1, q.end), keys = a.rows_plan ? min(all, a.rows_plan[kPlanSeqs + p.n_seqs + 1 + s]) : all;
+            blocks[b0 + b] = FewBlock{q.first * H + lead, n, lead, s, q.pos, 0, room ? (keys + kFewTile - 1) / kFewTile : 0, t0, 0, 0, 0, few_whole(q)};
         }
         __syncthreads();
         if (tid == 0) { carry[0] += all_b; carry[1] += all_t; }
@@ -250,13 +252,13 @@ __global__ void __launch_bounds__(kFewThreads, 1) __cluster_dims__(2, 1, 1) late
         while (left > 0) {
             const FewBlock k = blocks[b];
             if (k.tiles == 0) { b++; continue; }
-            const int n = min(left, k.tiles - t), slot = a.rows_plan ? 0 : a.p.slot[a.p.seqs[k.seq]], off = a.rows_plan ? a.rows_plan[kPlanSeqs + k.seq] : 0, tail = k.pos0 / kFewTile;
+            const int n = min(left, k.tiles - t), slot = a.rows_plan ? 0 : a.p.slot[a.p.seqs[k.seq]], off = a.rows_plan ? a.rows_plan[kPlanSeqs + k.seq] : 0, tail = k.whole;
             const int* table = a.p.page_table + (long)slot * a.p.max_pages;
             // lane i: the row of the tile's keys from 32 i on (four of them), of the tile after the one being loaded
             auto row_of = [&](int tile) {
                 if (a.rows_plan) return off + tile * kFewTile + 32 * (lane & 3);
                 if (tile >= tail) return (k.tail + tile - tail) * kFewTile + 32 * (lane & 3);
-                const int key = tile * kFewTile + 32 * (lane & 3), page = table[(key / a.p.page_size) % a.p.max_pages];
+                const int key = tile * kFewTile + 32 * (lane & 3), page = table[key / a.p.page_size];
                 return (unsigned)page < (unsigned)a.p.n_pages ? page * a.p.page_size + key % a.p.page_size : none;
             };
             int row = row_of(t);
@@ -357,14 +359,15 @@ __global__ void __launch_bounds__(kFewThreads, 1) __cluster_dims__(2, 1, 1) late
         const int sp = warp & 3, half = sp >> 1, r = 32 * (sp & 1) + lane;      // TMEM lane 32 sp + lane: the row r and the tile's keys (or O's columns) of this half
         const uint32_t tl = tmem + ((uint32_t)(32 * sp) << 16);
         const float c = a.scale_log2;
+        const int room = latent_room(a.p);
         const bool any_bad = a.rows_plan && a.rows_plan[kPlanBad] != 0;      // (rows side by side are copies, all of them; other tiles ahead of the tails are as the cache holds them)
         int left = total, b = b_first, t = t_first, it = 0, seg = 0;
         while (left > 0) {
             const FewBlock k = blocks[b];
             if (k.tiles == 0) { b++; continue; }
-            const int n = min(left, k.tiles - t), in = 64 * rank + r, tail = k.pos0 / kFewTile;
+            const int n = min(left, k.tiles - t), in = 64 * rank + r, tail = k.whole;
             const bool valid = in < k.rows;
-            const int p = valid ? k.pos0 + (k.lead + in) / H : -1;
+            const int p = valid ? min(k.pos0 + (k.lead + in) / H, room - 1) : -1;      // the last key that the row sees
             float m_ref = -INFINITY, l = 0.f;
             for (int j = 0; j < n; j++) {
                 const int i = it + j, k0 = (t + j) * kFewTile + 64 * half;

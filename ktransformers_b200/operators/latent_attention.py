@@ -76,7 +76,8 @@ def latent_append(q: torch.Tensor, kva: torch.Tensor, weight: torch.Tensor, eps:
     """From the projections' rows to the turned queries [T, heads, rot_dim] and the tokens' rows of cache layer `kv` [pages, page_size, rank + rot_dim], one `ktb200_latent_append` launch.
     q [T, heads * (nope + rot_dim)]; kva [T, rank + rot_dim or more]: latent, key part; weight [rank]: the latent's norm.  rot: `LatentRotation` or anything with its dims, layout_code, split and
     gain (None: no rotation), with float64 frequencies in inv_freq (or rot.inv_freq).  batch: pos, slot [T], seqs [2, portions], n_seqs; `positions` [T] int32: the angles' where they are not
-    batch.pos.  Rows of tokens in none of the batch's portions are left as they were (in the new tensor: as they came)."""
+    batch.pos.  Tokens at positions behind the page table's last column are turned and written nowhere.  Rows of tokens in none of the batch's portions are left as they were (in the new
+    tensor: as they came)."""
     what = "latent_append"
     T, dev, rank, width = q.shape[0], q.get_device(), weight.numel(), kv.shape[-1]
     rot_dim = width - rank
@@ -110,7 +111,8 @@ def latent_attention(q: torch.Tensor, q_rot: torch.Tensor, kv: torch.Tensor, w: 
     """o [T, heads * vdim] = soft-max attention of the queries [q_nope | q_rot] over the latents of cache layer `kv` [pages, page_size, 512 + 64] up to each token's position, `ktb200_latent_attn`:
     keys [W_K,h c | k_rot], values W_V,h c with w [heads * (nope + vdim), 512] (kv_b_proj's weight: every head's W_K above its W_V); q [T, heads * (nope + 64)] of any row stride, of which the
     first `nope` columns of a head are read; q_rot [T, heads, 64] as `latent_append` gives them.  nope, vdim: 64 or 128.  form: "expanded", "absorbed" (module docstring) or None, by
-    the tokens a sequence has on average and batch.max_kv.  batch.max_kv: no position is max_kv or more.  To `out` (a view of any row stride) or a new tensor; rows of tokens in none of the batch's portions are
+    the tokens a sequence has on average and batch.max_kv.  batch.max_kv: no position is max_kv or more.  Keys behind the
+    page table's last column are not there: tokens at such positions see the others.  To `out` (a view of any row stride) or a new tensor; rows of tokens in none of the batch's portions are
     left as they were (in a new tensor: as they came)."""
     what = "latent_attention"
     T, dev = q.shape[0], q.get_device()

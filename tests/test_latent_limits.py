@@ -1,11 +1,13 @@
-"""latent_append and latent_attention at the limits of a call: latents that are not finite far ahead of the new tokens."""
+"""latent_append, latent_attention and the layer on them at the limits of a call: latents that are not finite far ahead of the new tokens, positions behind the page table."""
 import math
+from types import SimpleNamespace
 
 import pytest
 import torch
 
-from latent_util import RANK, draw
-from ktransformers_b200.operators.latent_attention import latent_attention
+from latent_util import HALF, RANK, ROT, draw, near
+from test_latent_portions import YARN, Exact, layer
+from ktransformers_b200.operators.latent_attention import LatentRotation, latent_append, latent_attention
 
 gpu = pytest.mark.gpu
 FORMS = pytest.mark.parametrize("form", ["expanded", "absorbed"])
@@ -13,6 +15,36 @@ FORMS = pytest.mark.parametrize("form", ["expanded", "absorbed"])
 
 def call(d, form, **kw):
     return latent_attention(d.q, d.q_rot, d.kv, d.w, d.batch, d.cache, d.heads, d.nope, d.vdim, d.scale, form=form, **kw)
+
+
+def definition(d):
+    """(out, bound) in 64 bits with latent_util.attention's bound, over the keys that are there: up to the token's position, in a column of the page table, in a page of the pool.  A row without any is zero"""
+    outs, bounds, at = [], [], 0
+    w = d.w.view(d.heads, d.nope + d.vdim, RANK).double()
+    room = d.cache.page_table.shape[1] * d.page
+    for i, (b, n) in enumerate(d.lens):
+        key = torch.arange(min(b + n, room), device=d.kv.device)
+        page = d.cache.page_table[i].long()[key // d.page]
+        there = (page >= 0) & (page < d.kv.shape[0])
+        rows = d.kv[page.clamp(0, d.kv.shape[0] - 1), key % d.page].double().masked_fill(~there[:, None], 0.0)
+        lat, rot = rows[:, :RANK], rows[:, RANK:]
+        q = d.q.view(-1, d.heads, d.nope + ROT)[at:at + n, :, :d.nope].double()
+        see = (key[None, :] <= torch.arange(b, b + n, device=rows.device)[:, None]) & there[None, :]
+        some = see.any(1, keepdim=True)
+        o, e = [], []
+        for h in range(d.heads):
+            wk, wv = w[h, :d.nope], w[h, d.nope:]
+            s = (q[:, h] @ wk @ lat.t() + d.q_rot[at:at + n, h].double() @ rot.t()) * d.scale
+            p = torch.where(some, torch.softmax(s.masked_fill(~see, -math.inf), 1), torch.zeros_like(s))
+            k, v = lat @ wk.t(), lat @ wv.t()
+            off = torch.maximum(q[:, h].abs() @ k.abs().t(), (q[:, h] @ wk).abs() @ lat.abs().t()).masked_fill(~see, 0.0).amax(1) * (HALF * d.scale)
+            mass = torch.maximum(p @ v.abs(), (p @ lat).abs() @ wv.abs().t() + (p @ lat.abs()) @ wv.abs().t() * HALF)
+            o.append(p @ v)
+            e.append(mass * (torch.expm1(2 * off)[:, None] * (1 + 4 * HALF) + 4 * HALF) + o[-1].abs() * HALF)
+        outs.append(torch.stack(o, 1).flatten(1))
+        bounds.append(torch.stack(e, 1).flatten(1))
+        at += n
+    return torch.cat(outs), torch.cat(bounds)
 
 
 # ------------------------------------------------------------------------------------------------ latents that are not finite
@@ -41,3 +73,108 @@ def test_a_latent_that_is_not_finite_beside_one_key_with_all_the_weight(form):
     assert torch.isfinite(call(d, form)).all()
     d.kv[d.cache.page_table[0, 0].long(), 5, 300] = math.inf
     assert not torch.isfinite(call(d, form)).any()
+
+
+# ------------------------------------------------------------------------------------------------ positions behind the page table
+def short_table(page, before, tokens, shift, heads=2, seed=0, **kw):
+    """A portion whose positions go on behind the last column of its page table"""
+    d = draw([(before, tokens)], heads=heads, page=page, seed=seed, **kw)
+    columns = (before + tokens + page - 1) // page
+    d.cache = SimpleNamespace(page_table=d.cache.page_table[:, :columns].contiguous(), max_pages_per_seq=columns, page_size=page)
+    d.batch.pos += shift
+    d.lens = [(before + shift, tokens)]
+    d.batch.max_kv = before + shift + tokens
+    return d
+
+
+SHORT = pytest.mark.parametrize("page,before,tokens,shift", [
+    (16, 34, 30, 16),        # 64 positions, the portion at 50 .. 79
+    (64, 290, 30, 20),       # 320 positions, two and a half key tiles; 310 .. 339
+    (64, 98, 30, 200),       # 128 positions, all tokens behind them
+    (48, 250, 134, 10),      # 384 positions, three key tiles; 260 .. 393
+    (64, 500, 140, 1000),    # 640 positions, all tokens far behind them
+    (16, 79, 1, 1),          # 80 positions, a decoded token at the first that is not there
+])
+
+
+@gpu
+@FORMS
+@SHORT
+def test_attention_behind_the_page_table(form, page, before, tokens, shift):
+    """Tokens at positions that have no column see the keys that have one, as the one-token step of the layer does."""
+    d = short_table(page, before, tokens, shift, seed=41)
+    want, bound = definition(d)
+    near(call(d, form), want, bound)
+    d.batch.max_kv = 4 * d.batch.max_kv
+    near(call(d, form), want, bound)
+
+
+def append(d, rot):
+    kva = torch.randn((d.batch.n_tokens, RANK + ROT), device="cuda", generator=torch.Generator(device="cuda").manual_seed(5)).bfloat16()
+    weight = torch.linspace(0.5, 1.5, RANK, device="cuda").bfloat16()
+    return latent_append(d.q, kva, weight, 1e-6, d.batch, d.cache, d.kv, d.heads, d.nope, rot=rot)
+
+
+@gpu
+@SHORT
+def test_append_behind_the_page_table(page, before, tokens, shift):
+    """Tokens at positions that have no column are turned and written nowhere."""
+    d = short_table(page, before, tokens, shift, seed=42)
+    rot = LatentRotation(10000.0 ** (-torch.arange(0, 64, 2, dtype=torch.float64) / 64).cuda())
+    start, room = d.kv.clone(), d.cache.page_table.shape[1] * page
+    got = append(d, rot)
+    after, d.kv = d.kv, start.clone()
+    stay = max(0, room - before - shift)      # tokens that have a column
+    d.batch.seqs[1, 0] = stay
+    first = append(d, rot)
+    assert torch.equal(after.view(torch.int16), d.kv.view(torch.int16)) and torch.equal(got[:stay], first[:stay])
+    key = torch.arange(before + shift, before + shift + stay, device="cuda")
+    at = d.cache.page_table[0].long()[key // page], key % page
+    start[at] = after[at]
+    assert torch.equal(after.view(torch.int16), start.view(torch.int16))
+
+
+@gpu
+def test_append_of_a_portion_longer_than_its_table():
+    """More tokens than the table has positions: the first ones are written, each once, whatever the order of the warps."""
+    d = draw([(0, 1000)], heads=2, page=16, seed=43)
+    rot = LatentRotation(10000.0 ** (-torch.arange(0, 64, 2, dtype=torch.float64) / 64).cuda())
+    whole, start = d.kv.clone(), d.kv.clone()
+    d.kv = whole
+    append(d, rot)
+    table = d.cache.page_table
+    d.cache, d.kv = SimpleNamespace(page_table=table[:, :5].contiguous(), max_pages_per_seq=5, page_size=16), start.clone()
+    append(d, rot)
+    used = table[0, :5].long()
+    start[used] = whole[used]
+    assert torch.equal(d.kv.view(torch.int16), start.view(torch.int16))
+
+
+@gpu
+@pytest.mark.parametrize("scaling", [None, YARN])
+def test_layer_at_the_end_of_its_cache(scaling):
+    """A portion that crosses the end of the static cache, and a decoded token behind it: what the cache holds stays, tokens that fit are right, those that do not see what is there."""
+    from ktransformers_b200.models.custom_cache import StaticCache
+    from ktransformers_b200.operators.attention import KDeepseekV2Attention
+    from ktransformers_b200.operators.flashinfer_wrapper import MLAWrapper
+    cfg, plain = layer(16, 128, scaling, seed=6)
+    exact = Exact(cfg, plain)
+    op = KDeepseekV2Attention("blk.0.self_attn", None, cfg, plain, "cuda", "cuda")
+    cache = StaticCache(cfg, max_batch_size=3, max_cache_len=200, device="cuda")      # 256 positions
+    op.mla_wrapper = MLAWrapper(2, cache.max_pages * 2)
+    rows = cache.key_cache[0].view(3, 256, 576)
+    where = lambda at, n: torch.arange(at, at + n, device="cuda")
+    x = torch.randn(2, 263, 512, device="cuda").bfloat16()
+    run = lambda at, n: op(x[:, at:at + n], position_ids=where(at, n)[None].expand(2, n), past_key_value=cache, cache_position=where(at, n))[0]
+    with torch.no_grad():
+        run(0, 250)
+        before = rows.clone()
+        y = run(250, 12)
+        want = exact(x[:, :256], where(0, 256)[None].expand(2, 256))[:, 250:]
+        # some ten roundings of 1.65e-3 (root of mean square) one behind the other are 5.2e-3, three times that
+        assert (y[:, :6].float() - want).norm() <= 1.6e-2 * want.norm() and torch.isfinite(y).all()
+        assert torch.equal(rows[:, :250], before[:, :250]) and (rows[2] == 0).all() and (rows[:2, 250:] != 0).any(-1).all()
+        full = rows.clone()
+        token = run(262, 1)
+        again = op._portion(x[:, 262:], where(262, 1)[None].expand(2, 1), cache, where(262, 1))
+        assert torch.equal(rows, full) and (token.float() - again.float()).norm() <= 2 * 1.6e-2 * again.float().norm()      # (both are that far off at most)
