@@ -21,12 +21,12 @@ struct LatentAppend {
     int n_tokens, latent_ctas, slices, per, toks;      // CTAs of latent rows; CTAs a token's heads are cut into, the heads of one, the tokens of one
 };
 
-// whether token t is in one of the portions (called by a whole warp)
-__device__ __forceinline__ bool latent_in_portion(const int* seqs, int stride, int n_seqs, int t) {
+// whether token t is in one of the portions that are there, as one is not that reaches past the call's tokens (called by a whole warp)
+__device__ __forceinline__ bool latent_in_portion(const ktb200_latent_append_params& p, int n_tokens, int t) {
     bool in = false;
-    for (int s = threadIdx.x & 31; s < n_seqs; s += 32) {
-        const int first = seqs[s];
-        in |= t >= first && t - first < seqs[stride + s];
+    for (int s = threadIdx.x & 31; s < p.n_seqs; s += 32) {
+        const int first = p.seqs[s], count = p.seqs[p.seqs_stride + s];
+        in |= first >= 0 && t >= first && t - first < count && count <= n_tokens - first;
     }
     return __any_sync(0xffffffffu, in);
 }
@@ -105,7 +105,7 @@ template <bool VEC, int ITEMS, int LAYOUT> __global__ void __launch_bounds__(kLa
         const int pos = p.pos[t], slot = p.slot[t];
         for (int i = lane; i < half; i += 32) cs[warp][i] = latent_turn(p, t, i);
         const int column = pos / p.page_size;      // (a position behind the last column has no row: nothing to write to)
-        if (!latent_in_portion(p.seqs, p.seqs_stride, p.n_seqs, t) || pos < 0 || column >= p.max_pages || (unsigned)slot >= (unsigned)p.n_slots) return;
+        if (!latent_in_portion(p, a.n_tokens, t) || pos < 0 || column >= p.max_pages || (unsigned)slot >= (unsigned)p.n_slots) return;
         const int page = p.page_table[(long)slot * p.max_pages + column];
         if ((unsigned)page >= (unsigned)p.n_pages) return;
         __nv_bfloat16* dst = (__nv_bfloat16*)p.cache + ((long)page * p.page_size + pos % p.page_size) * width;
@@ -176,7 +176,7 @@ template <bool VEC, int ITEMS, int LAYOUT> __global__ void __launch_bounds__(kLa
     if (VEC) load(0);      // (on their way while the angles are made)
     for (int i = threadIdx.x; i < toks * half; i += kLaThreads) cs[i / half][i % half] = latent_turn(p, t0 + i / half, i % half);
     for (int k = warp; k < toks; k += kLaThreads / 32) {
-        const bool mine = latent_in_portion(p.seqs, p.seqs_stride, p.n_seqs, t0 + k);
+        const bool mine = latent_in_portion(p, a.n_tokens, t0 + k);
         if (lane == 0) there[k] = mine;
     }
     __syncthreads();

@@ -27,22 +27,15 @@ constexpr int kPlanSort = 256;      // query tiles that are sorted
 __global__ void __launch_bounds__(32) latent_plan_kernel(const ktb200_latent_attn_params p, int n_tokens, int row_cap, int tile_cap, long rows_of_heads, int* plan) {
     griddep_wait();
     griddep_launch_dependents();      // (as absorb_kernel: behind the wait)
-    const int lane = threadIdx.x, room = latent_room(p);
+    const int lane = threadIdx.x;
     int* off = plan + kPlanSeqs;
     int4* tiles = reinterpret_cast<int4*>(plan + plan_tiles_at(p.n_seqs));
     __shared__ int4 held[kPlanSort];
     int rows = 0, nt = 0;
     for (int s0 = 0; s0 < p.n_seqs; s0 += 32) {
         const int s = s0 + lane;
-        int first = 0, count = 0, pos = 0, keys = 0;
-        if (s < p.n_seqs) {
-            first = p.seqs[s];
-            count = p.seqs[p.seqs_stride + s];
-            if (count > 0 && first >= 0 && first <= n_tokens - count) pos = p.pos[first];
-            else count = 0;
-            if (count > 0 && (pos < 0 || (unsigned)p.slot[first] >= (unsigned)p.n_slots)) count = 0;
-            keys = count > 0 ? (int)min((long)pos + count, (long)min(row_cap, room)) : 0;
-        }
+        const LatentPortion portion = s < p.n_seqs ? latent_portion(p, n_tokens, s) : LatentPortion{};
+        const int first = portion.first, count = portion.count, pos = portion.pos, keys = min(portion.end, row_cap);
         const int r = (keys + kLatentTile - 1) / kLatentTile * kLatentTile, q = (count + kPlanTokens - 1) / kPlanTokens;
         int rs = r, qs = q;
 #pragma unroll
@@ -130,7 +123,7 @@ __global__ void __launch_bounds__(256) latent_gather_kernel(const ktb200_latent_
 // weights' bytes (16.8 MB each with 128 heads), and all of them are on their way at the start.
 //   VALUES = false: A = q_nope (K = N), B_h = W_K,h [N][512];  VALUES = true: A = sums of latents (K = 512), B_h = W_V,h^T, W_V,h [V][512]
 // All columns of a head in a CTA where there are heads and token tiles for half of the SMs, blocks of 128 (or 32) where there are not.
-// The first also writes which tokens there are (`there`: in a portion, with a position and a slot); the second leaves the rows of others as they are.
+// The first also writes which tokens there are (`there`: in a portion that is there); the second leaves the rows of others as they are.
 template <int MT, int K, bool VALUES, int NB> struct AbsorbShape {
     static constexpr int WARPS = NB > 128 || (VALUES && NB > 32) ? 16 : 8, KP = K + 8, BP = VALUES ? kLatent + 8 : NB + 8, CP = NB + 8;      // padded rows: neighbouring rows meet in no bank
     static constexpr int WM = MT / 16, COLS = NB / 8, WN = WARPS / WM < COLS ? WARPS / WM : COLS, WK = WARPS / (WM * WN), NT = COLS / WN;      // warps along tokens, columns and K; runs of 8 columns a warp
@@ -163,8 +156,9 @@ template <int MT, int K, bool VALUES, int NB> __global__ void __launch_bounds__(
             const int t = m0 + m;
             if (t >= n_tokens) break;
             bool in = false;
-            for (int s = lane; s < p.n_seqs; s += 32) in |= t >= p.seqs[s] && t - p.seqs[s] < p.seqs[p.seqs_stride + s];
-            in = __any_sync(0xffffffffu, in) && (unsigned)p.slot[t] < (unsigned)p.n_slots && p.pos[t] >= 0;
+            for (int s = lane; s < p.n_seqs; s += 32)
+                if (t >= p.seqs[s] && t - p.seqs[s] < p.seqs[p.seqs_stride + s]) in |= latent_portion(p, n_tokens, s).count > 0;
+            in = __any_sync(0xffffffffu, in);
             if (lane == 0) there[t] = in;
         }
     }

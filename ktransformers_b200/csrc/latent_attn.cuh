@@ -19,6 +19,17 @@ __host__ __device__ inline int latent_room(const ktb200_latent_attn_params& p) {
     const long n = (long)p.max_pages * p.page_size;
     return n < 0x7fffff00L ? (int)n : 0x7fffff00;
 }
+// A portion as all kernels of both forms see it; count 0: not there, as one is that reaches past the call's tokens or whose first token's position or slot is not there
+struct LatentPortion { int first, count, pos, slot, end; };      // end: keys that its last token sees
+__device__ __forceinline__ LatentPortion latent_portion(const ktb200_latent_attn_params& p, int n_tokens, int s) {
+    LatentPortion q{p.seqs[s], p.seqs[p.seqs_stride + s], 0, 0, 0};
+    if (q.count <= 0 || q.first < 0 || q.first > n_tokens - q.count) { q.count = 0; return q; }
+    q.pos = p.pos[q.first];
+    q.slot = p.slot[q.first];
+    if (q.pos < 0 || q.pos > 0x7fffff00 - q.count || (unsigned)q.slot >= (unsigned)p.n_slots) { q.count = 0; return q; }
+    q.end = min(q.pos + q.count, latent_room(p));
+    return q;
+}
 __device__ __forceinline__ uint32_t latent_pack(float lo, float hi) {
     const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&v);

@@ -50,19 +50,8 @@ struct LatentFew {
     float *o_part, *ml_part;                              // [2 pairs][128][512], [2 pairs][128][2]
 };
 
-// a portion as every kernel of the form sees it
-struct FewPortion { int first, count, pos, slot, end; };      // end: keys that its last token sees
-__device__ __forceinline__ FewPortion few_portion(const ktb200_latent_attn_params& p, int n_tokens, int s) {
-    FewPortion q{p.seqs[s], p.seqs[p.seqs_stride + s], 0, 0, 0};
-    if (q.count <= 0 || q.first < 0 || q.first > n_tokens - q.count) { q.count = 0; return q; }
-    q.pos = p.pos[q.first];
-    q.slot = p.slot[q.first];
-    if (q.pos < 0 || q.pos > 0x7fffff00 - q.count || (unsigned)q.slot >= (unsigned)p.n_slots) q.count = 0;
-    q.end = min(q.pos + q.count, latent_room(p));
-    return q;
-}
-__device__ __forceinline__ int few_whole(const FewPortion& q) { return min(q.pos, q.end) / kFewTile; }
-__device__ __forceinline__ int few_tails(const FewPortion& q) { return q.count > 0 ? (q.end + kFewTile - 1) / kFewTile - few_whole(q) : 0; }
+__device__ __forceinline__ int few_whole(const LatentPortion& q) { return min(q.pos, q.end) / kFewTile; }
+__device__ __forceinline__ int few_tails(const LatentPortion& q) { return q.count > 0 ? (q.end + kFewTile - 1) / kFewTile - few_whole(q) : 0; }
 
 // CTA 0: blocks, the line, its cuts.  The others: 32 rows of the tails each
 __global__ void __launch_bounds__(256) latent_few_prep_kernel(const LatentFew a, __nv_bfloat16* tails, uint32_t* tail_bad) {
@@ -75,9 +64,9 @@ __global__ void __launch_bounds__(256) latent_few_prep_kernel(const LatentFew a,
     if (blockIdx.x > 0) {
         const int g = blockIdx.x - 1, tile = g / 4;
         int seq = -1, at = 0, before = 0;
-        FewPortion q{};
+        LatentPortion q{};
         for (int s0 = 0; s0 < p.n_seqs; s0 += 32) {
-            const FewPortion mine = s0 + lane < p.n_seqs ? few_portion(p, a.n_tokens, s0 + lane) : FewPortion{};
+            const LatentPortion mine = s0 + lane < p.n_seqs ? latent_portion(p, a.n_tokens, s0 + lane) : LatentPortion{};
             const int n = few_tails(mine);
             int sum = n;
 #pragma unroll
@@ -90,7 +79,7 @@ __global__ void __launch_bounds__(256) latent_few_prep_kernel(const LatentFew a,
                 const int l = __ffs(has) - 1;
                 seq = s0 + l;
                 at = tile - (before + __shfl_sync(0xffffffffu, sum - n, l));
-                q = FewPortion{__shfl_sync(0xffffffffu, mine.first, l), __shfl_sync(0xffffffffu, mine.count, l), __shfl_sync(0xffffffffu, mine.pos, l), __shfl_sync(0xffffffffu, mine.slot, l), __shfl_sync(0xffffffffu, mine.end, l)};
+                q = LatentPortion{__shfl_sync(0xffffffffu, mine.first, l), __shfl_sync(0xffffffffu, mine.count, l), __shfl_sync(0xffffffffu, mine.pos, l), __shfl_sync(0xffffffffu, mine.slot, l), __shfl_sync(0xffffffffu, mine.end, l)};
                 break;
             }
             before += __shfl_sync(0xffffffffu, sum, 31);
@@ -140,7 +129,7 @@ __global__ void __launch_bounds__(256) latent_few_prep_kernel(const LatentFew a,
     __syncthreads();
     for (int s0 = 0; s0 < p.n_seqs; s0 += 256) {
         const int s = s0 + tid;
-        const FewPortion q = s < p.n_seqs ? few_portion(p, a.n_tokens, s) : FewPortion{};
+        const LatentPortion q = s < p.n_seqs ? latent_portion(p, a.n_tokens, s) : LatentPortion{};
         const long rows = (long)q.count * H;
         const int nb = (int)((rows + kFewRows - 1) / kFewRows), nt = few_tails(q);
         int all_b, all_t;

@@ -1,4 +1,4 @@
-"""latent_append, latent_attention and the layer on them at the limits of a call: latents that are not finite far ahead of the new tokens, positions behind the page table."""
+"""latent_append, latent_attention and the layer on them at the limits of a call: latents that are not finite far ahead of the new tokens, positions behind the page table, portions that are not there."""
 import math
 from types import SimpleNamespace
 
@@ -150,6 +150,43 @@ def test_append_of_a_portion_longer_than_its_table():
     assert torch.equal(d.kv.view(torch.int16), start.view(torch.int16))
 
 
+# ------------------------------------------------------------------------------------------------ portions that are not there
+@gpu
+@FORMS
+@pytest.mark.parametrize("first,count", [(5, 100), (5, 36), (-1, 20), (2000000000, 2000000000)])
+def test_portions_that_reach_past_the_call(form, first, count):
+    """A portion with tokens that the call does not have is not there: its rows stay, and nothing is appended for it."""
+    d = draw([(90, 5), (10, 35)], heads=3, seed=51)
+    want, bound = definition(d)
+    d.batch.seqs[:, 1] = torch.tensor([first, count], dtype=torch.int32, device="cuda")
+    got = call(d, form, out=torch.full((40, 384), 7.0, dtype=torch.bfloat16, device="cuda"))
+    near(got[:5], want[:5], bound[:5])
+    assert (got[5:] == 7).all()
+    start = d.kv.clone()
+    append(d, None)
+    page, row = d.cache.page_table[0, 1].long(), slice(90 - 64, 95 - 64)
+    assert not torch.equal(d.kv[page, row], start[page, row])
+    start[page, row] = d.kv[page, row]
+    assert torch.equal(d.kv.view(torch.int16), start.view(torch.int16))
+
+
+@gpu
+@FORMS
+def test_portions_whose_first_token_is_not_there(form):
+    """The first token's slot and position are the portion's: where they are not there, none of its rows is written, in either form."""
+    d = draw([(90, 5), (10, 35)], heads=3, seed=52)
+    want, bound = definition(d)
+    for name, what in (("slot", 9), ("pos", -1), ("pos", 0x7ffffff0)):
+        held = getattr(d.batch, name)[5].clone()
+        getattr(d.batch, name)[5] = what
+        got = call(d, form, out=torch.full((40, 384), 7.0, dtype=torch.bfloat16, device="cuda"))
+        near(got[:5], want[:5], bound[:5])
+        assert (got[5:] == 7).all()
+        getattr(d.batch, name)[5] = held
+    near(call(d, form), want, bound)
+
+
+# ------------------------------------------------------------------------------------------------ the layer
 @gpu
 @pytest.mark.parametrize("scaling", [None, YARN])
 def test_layer_at_the_end_of_its_cache(scaling):
