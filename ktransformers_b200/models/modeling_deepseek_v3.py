@@ -179,10 +179,10 @@ class DeepseekV3RotaryEmbedding(nn.Module):
         return emb.cos().to(x.dtype), emb.sin().to(x.dtype)
 
 
-def yarn_inv_freq(dims: int, base: float, factor: float, original: int, beta_fast: float = 32.0, beta_slow: float = 1.0) -> torch.Tensor:
+def yarn_inv_freq(dims: int, base: float, factor: float, original: int, beta_fast: float = 32.0, beta_slow: float = 1.0, device="cpu") -> torch.Tensor:
     """Frequencies of a rotation scaled for contexts of `factor` times the `original` length (YaRN; modeling_deepseek_v3.py:233-334), float64: those that turn more than beta_fast times in the
     original length stay, those that turn less than beta_slow times are divided by the factor, and between the two the share moves in a straight line over the column."""
-    i = torch.arange(dims // 2, dtype=torch.float64)
+    i = torch.arange(dims // 2, dtype=torch.float64, device=device)
     freq = float(base) ** (-2.0 * i / dims)
     column = lambda turns: dims * math.log(original / (turns * 2 * math.pi)) / (2 * math.log(base))
     lo, hi = max(math.floor(column(beta_fast)), 0), min(math.ceil(column(beta_slow)), dims - 1)
@@ -198,13 +198,20 @@ class DeepseekV3YarnRotaryEmbedding(nn.Module):
         super().__init__()
         self.dim, self.base = dim, base
         self.gain = yarn_get_mscale(scaling_factor, mscale) / yarn_get_mscale(scaling_factor, mscale_all_dim)
-        self._inv_freq = {torch.device("cpu"): yarn_inv_freq(dim, base, scaling_factor, original_max_position_embeddings, beta_fast, beta_slow)}
+        self._scaled, self._inv_freq = (dim, base, scaling_factor, original_max_position_embeddings, beta_fast, beta_slow), {}
 
     def inv_freq_on(self, device) -> torch.Tensor:
+        """The frequencies, made on the device that asks first (the module may have been built on the meta device, and a captured call may copy nothing from the host) and kept there."""
         device = torch.device(device)
-        if device not in self._inv_freq:
-            self._inv_freq[device] = self._inv_freq[torch.device("cpu")].to(device)
-        return self._inv_freq[device]
+        held = self._inv_freq.get(device)
+        if held is None:
+            held = yarn_inv_freq(*self._scaled, device=device)
+            if device.type == "cuda":
+                if torch.cuda.is_current_stream_capturing():
+                    return held      # (its memory is the graph's)
+                torch.cuda.current_stream(device).synchronize()      # (the next call may be on another stream)
+            self._inv_freq[device] = held
+        return held
 
     @torch.no_grad()
     def forward(self, x, position_ids):

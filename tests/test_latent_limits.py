@@ -1,4 +1,5 @@
-"""latent_append, latent_attention and the layer on them at the limits of a call: latents that are not finite far ahead of the new tokens, positions behind the page table, portions that are not there."""
+"""latent_append, latent_attention and the layer on them at the limits of a call: latents that are not finite far ahead of the new tokens, positions behind the page table, portions that are not there, layers that
+were built without memory or are captured before their first call."""
 import math
 from types import SimpleNamespace
 
@@ -7,6 +8,8 @@ import torch
 
 from latent_util import HALF, RANK, ROT, draw, near
 from test_latent_portions import YARN, Exact, layer
+from ktransformers_b200.models.modeling_deepseek_v3 import DeepseekV3Attention, DeepseekV3Config, DeepseekV3YarnRotaryEmbedding, yarn_inv_freq
+from ktransformers_b200.operators.attention import KDeepseekV2Attention
 from ktransformers_b200.operators.latent_attention import LatentRotation, latent_append, latent_attention
 
 gpu = pytest.mark.gpu
@@ -192,7 +195,6 @@ def test_portions_whose_first_token_is_not_there(form):
 def test_layer_at_the_end_of_its_cache(scaling):
     """A portion that crosses the end of the static cache, and a decoded token behind it: what the cache holds stays, tokens that fit are right, those that do not see what is there."""
     from ktransformers_b200.models.custom_cache import StaticCache
-    from ktransformers_b200.operators.attention import KDeepseekV2Attention
     from ktransformers_b200.operators.flashinfer_wrapper import MLAWrapper
     cfg, plain = layer(16, 128, scaling, seed=6)
     exact = Exact(cfg, plain)
@@ -215,3 +217,37 @@ def test_layer_at_the_end_of_its_cache(scaling):
         token = run(262, 1)
         again = op._portion(x[:, 262:], where(262, 1)[None].expand(2, 1), cache, where(262, 1))
         assert torch.equal(rows, full) and (token.float() - again.float()).norm() <= 2 * 1.6e-2 * again.float().norm()      # (both are that far off at most)
+
+
+def test_scaled_rotation_of_a_layer_built_without_memory():
+    """Models are built on the meta device before their weights are loaded: the frequencies are there all the same."""
+    cfg = DeepseekV3Config(hidden_size=64, num_attention_heads=2, q_lora_rank=None, num_hidden_layers=1, rope_scaling=dict(YARN))
+    with torch.device("meta"):
+        rot = DeepseekV3Attention(cfg).rotary_emb
+        f = rot.inv_freq_on("cpu")
+    assert f.device.type == "cpu" and torch.equal(f, yarn_inv_freq(64, 10000.0, 40, 4096))
+    cos, _ = rot(torch.zeros(1), torch.tensor([[0, 7]]))
+    assert cos.device.type == "cpu" and torch.equal(cos[0, 1, :32], ((7 * f).cos() * rot.gain).float())
+
+
+@gpu
+def test_scaled_layer_captured_before_its_first_call():
+    """Nothing of a scaled rotation is copied from the host by the first call: it may be a captured one.  The same bits as eagerly."""
+    from ktransformers_b200.models.custom_cache import StaticCache
+    cfg, plain = layer(4, 64, YARN, seed=8)
+    op = KDeepseekV2Attention("blk.0.self_attn", None, cfg, plain, "cuda", "cuda")
+    x, at = torch.randn(2, 1, 512, device="cuda").bfloat16(), torch.full((1,), 3000, device="cuda")
+    run = lambda cache: op(x, position_ids=at[None].expand(2, 1), past_key_value=cache, cache_position=at)[0]
+    make = lambda: StaticCache(cfg, max_batch_size=2, max_cache_len=3010, device="cuda")
+    with torch.no_grad():
+        eager = make()
+        want = run(eager)
+        plain.rotary_emb = DeepseekV3YarnRotaryEmbedding(64, scaling_factor=40, mscale=1.0, mscale_all_dim=1.0)
+        cache, g = make(), torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(g):
+            y = run(cache)
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, want) and torch.equal(cache.key_cache[0], eager.key_cache[0])
+        assert torch.equal(run(cache), want)      # and eagerly behind the captured call
