@@ -25,7 +25,8 @@ class DeepseekV3Config(PretrainedConfig):
                  norm_topk_prob=True, scoring_func="sigmoid", topk_method="noaux_tc", hidden_act="silu",
                  num_hidden_layers=61, first_k_dense_replace=3, moe_layer_freq=1, num_attention_heads=128,
                  q_lora_rank=1536, kv_lora_rank=512, qk_rope_head_dim=64, qk_nope_head_dim=128, v_head_dim=128,
-                 vocab_size=129280, rms_norm_eps=1e-6, ep_size=1, rope_scaling=None, **kwargs):
+                 vocab_size=129280, rms_norm_eps=1e-6, ep_size=1, rope_scaling=None, rope_parameters=None, max_position_embeddings=163840,
+                 **kwargs):
         self.hidden_size = hidden_size
         self.intermediate_size = intermediate_size
         self.moe_intermediate_size = moe_intermediate_size
@@ -52,7 +53,14 @@ class DeepseekV3Config(PretrainedConfig):
         self.rms_norm_eps = rms_norm_eps
         self.ep_size = ep_size
         super().__init__(**kwargs)
-        self.rope_scaling = rope_scaling      # {"type": "yarn", "factor", ...} or None
+        self.max_position_embeddings = max_position_embeddings
+        # {"type" or "rope_type": "yarn", "factor", ...} or None; newer checkpoints have it as rope_parameters, the base among them.  (The attribute has both names, and a configuration is saved under the newer)
+        scaling = rope_scaling if rope_scaling is not None else rope_parameters
+        if scaling is not None:
+            scaling = dict(scaling)
+            self.rope_theta = scaling["rope_theta"] = kwargs.get("rope_theta", scaling.get("rope_theta", 10000.0))
+            scaling["rope_type"] = scaling.get("rope_type", scaling.get("type", "default"))
+        self.rope_scaling = scaling
 
 
 class DeepseekV3MLP(nn.Module):

@@ -1,5 +1,5 @@
 """latent_append, latent_attention and the layer on them at the limits of a call: latents that are not finite far ahead of the new tokens, positions behind the page table, portions that are not there, layers that
-were built without memory or are captured before their first call."""
+were built without memory or are captured before their first call, configurations that come back from a file."""
 import math
 from types import SimpleNamespace
 
@@ -8,7 +8,7 @@ import torch
 
 from latent_util import HALF, RANK, ROT, draw, near
 from test_latent_portions import YARN, Exact, layer
-from ktransformers_b200.models.modeling_deepseek_v3 import DeepseekV3Attention, DeepseekV3Config, DeepseekV3YarnRotaryEmbedding, yarn_inv_freq
+from ktransformers_b200.models.modeling_deepseek_v3 import DeepseekV3Attention, DeepseekV3Config, DeepseekV3RotaryEmbedding, DeepseekV3YarnRotaryEmbedding, yarn_get_mscale, yarn_inv_freq
 from ktransformers_b200.operators.attention import KDeepseekV2Attention
 from ktransformers_b200.operators.latent_attention import LatentRotation, latent_append, latent_attention
 
@@ -251,3 +251,22 @@ def test_scaled_layer_captured_before_its_first_call():
         torch.cuda.synchronize()
         assert torch.equal(y, want) and torch.equal(cache.key_cache[0], eager.key_cache[0])
         assert torch.equal(run(cache), want)      # and eagerly behind the captured call
+
+
+@pytest.mark.parametrize("given", [dict(rope_scaling=YARN), dict(rope_scaling=YARN, rope_theta=50000.0), dict(rope_parameters={**YARN, "rope_type": "yarn", "rope_theta": 50000.0}),
+                                   dict(rope_parameters={"rope_type": "default", "rope_theta": 50000.0}), dict()])
+def test_a_scaled_configuration_comes_back(given, tmp_path):
+    """A configuration whose rotation is scaled is the same after to_dict and after a file, and has the same layer, under either name that checkpoints give the scaling; the caller's dict stays."""
+    held = {k: dict(v) if isinstance(v, dict) else v for k, v in given.items()}
+    first = DeepseekV3Config(hidden_size=64, num_attention_heads=2, q_lora_rank=None, num_hidden_layers=1, **given)
+    assert given == held
+    first.save_pretrained(tmp_path)
+    base = 50000.0 if "rope_parameters" in given or "rope_theta" in given else 10000.0
+    for cfg in (first, DeepseekV3Config.from_dict(first.to_dict()), DeepseekV3Config.from_pretrained(tmp_path)):
+        rot, wanted = DeepseekV3Attention(cfg).rotary_emb, next((v for v in given.values() if isinstance(v, dict)), None)
+        if wanted is None or wanted.get("rope_type") == "default":
+            assert type(rot) is DeepseekV3RotaryEmbedding and rot.base == base
+        else:
+            assert {k: cfg.rope_scaling[k] for k in YARN} == YARN
+            assert torch.equal(rot.inv_freq_on("cpu"), yarn_inv_freq(64, base, 40, 4096))
+            assert math.isclose(DeepseekV3Attention(cfg).softmax_scale, 192 ** -0.5 * yarn_get_mscale(40, 1.0) ** 2)
