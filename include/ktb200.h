@@ -408,9 +408,11 @@ int ktb200_latent_step(const ktb200_latent_step_params* p, void* stream);
 /* ------------------------------------------------------------------------------------------
  * Latent attention beyond one decoded token (bf16): the append to the paged latent cache and the attention of any number of new tokens a sequence over it
  * (archive/ktransformers/operators/attention.py:140-344, the prefill branches; operators/RoPE.py:222-326, the scaled rotation).
- * Token t of a call belongs to sequence slot[t] (a row of page_table, n_slots x max_pages: position p has row p % page_size of the page in column p / page_size) at position pos[t]; portion s is
- * the tokens seqs[s] .. seqs[s] + seqs[seqs_stride + s] - 1, at consecutive positions, not there where it reaches past the call's tokens; portions share no tokens.  Tokens at positions behind the last column are written nowhere and see the keys that have one.  cache: [n_pages][page_size][kv_rank + rot_dim], [latent | rotated key part].  What slots, pages or portions that are not
- * there would hold is neither read nor written, and rows of tokens in no portion stay as they were.
+ * Token t of a call belongs to sequence slot[t] (a row of page_table, n_slots x max_pages: position p has row p % page_size of the page in column p / page_size) at position
+ * pos[t]; portion s is the tokens seqs[s] .. seqs[s] + seqs[seqs_stride + s] - 1, at consecutive positions, not there where it reaches past the call's tokens; portions share no
+ * tokens.  Tokens at positions behind the last column are written nowhere and see the keys that have one.  cache: [n_pages][page_size][kv_rank + rot_dim], [latent | rotated key
+ * part].  What slots, pages or portions that are not there would hold is neither read nor written, and rows of tokens in no portion stay as they were.  Keys in pages outside the
+ * pool are not seen; a row that sees no key becomes zero.
  *
  * ktb200_latent_append: q row = heads x [nope_dim | rot_dim], kva row = [latent | key part | ...].  q_rot[t][h][:] and the cache row's key part: pairs of the first rot_dims columns turned
  *   by pos * inv_freq[i] (fp64; angle_pos[t] in pos's place where given), cosines and sines times rot_gain.  rot_layout 0: columns 2 i and 2 i + 1 are a pair, 1: i and i + rot_dims / 2;

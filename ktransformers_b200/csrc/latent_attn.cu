@@ -76,24 +76,25 @@ __global__ void __launch_bounds__(32) latent_plan_kernel(const ktb200_latent_att
         plan[kPlanRows] = rows;
         plan[kPlanHeads] = rows > 0 ? (int)min((long)p.heads, rows_of_heads / rows) : p.heads;
         plan[kPlanTiles] = nt;
-        plan[kPlanBad] = 0;
+        plan[kPlanOdd] = 0;
     }
 }
 
-// Rows side by side: 32 a CTA and step, a warp four of them.  Rows behind a portion's last key, and rows that are not there, are zeros, and latents that are not finite (latent_copy_row)
-__global__ void __launch_bounds__(256) latent_gather_kernel(const ktb200_latent_attn_params p, int* plan, __nv_bfloat16* lat, uint32_t* bad) {
+// Rows side by side: 32 a CTA and step, a warp four of them.  Rows behind a portion's last key, and rows that are not there, are zeros, and latents that are not finite (latent_copy_row): a bit a row of
+// which of these it is
+__global__ void __launch_bounds__(256) latent_gather_kernel(const ktb200_latent_attn_params p, int* plan, __nv_bfloat16* lat, uint32_t* bad, uint32_t* gone) {
     griddep_launch_dependents();
     griddep_wait();
     const int rows = plan[kPlanRows], lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int* off = plan + kPlanSeqs;
-    __shared__ uint32_t odd[8];
+    __shared__ uint32_t odd[8][2];
     for (int r0 = blockIdx.x * 32; r0 < rows; r0 += gridDim.x * 32) {
         int seq = -1;      // the last portion that begins at or before this row and has one
         for (int s0 = 0; s0 < p.n_seqs; s0 += 32) {
             const unsigned in = __ballot_sync(0xffffffffu, s0 + lane < p.n_seqs && off[s0 + lane] <= r0 && off[s0 + lane + 1] > r0);
             if (in) { seq = s0 + __ffs(in) - 1; break; }
         }
-        uint32_t mine = 0;
+        uint32_t mine = 0, lost = 0;
         if (seq >= 0) {
             const int key0 = r0 - off[seq], keys = off[p.n_seqs + 1 + seq], slot = p.slot[p.seqs[seq]];
 #pragma unroll
@@ -102,17 +103,19 @@ __global__ void __launch_bounds__(256) latent_gather_kernel(const ktb200_latent_
                 int page = -1;
                 if (key < keys) page = p.page_table[(long)slot * p.max_pages + key / p.page_size];
                 const bool there = (unsigned)page < (unsigned)p.n_pages;
+                if (key < keys && !there) lost |= 1u << (4 * warp + i);
                 if (latent_copy_row((const __nv_bfloat16*)p.cache + ((long)page * p.page_size + key % p.page_size) * kLatentRow, there, lat + (long)(r0 + 4 * warp + i) * kLatentRow, true)) mine |= 1u << (4 * warp + i);
             }
         }
-        if (lane == 0) odd[warp] = mine;
+        if (lane == 0) { odd[warp][0] = mine; odd[warp][1] = lost; }
         __syncthreads();
         if (threadIdx.x == 0) {
-            uint32_t all = 0;
+            uint32_t all[2] = {0, 0};
 #pragma unroll
-            for (int i = 0; i < 8; i++) all |= odd[i];
-            bad[r0 / 32] = all;
-            if (all) atomicOr(plan + kPlanBad, 1);
+            for (int i = 0; i < 8; i++) { all[0] |= odd[i][0]; all[1] |= odd[i][1]; }
+            bad[r0 / 32] = all[0];
+            gone[r0 / 32] = all[1];
+            if (all[0] | all[1]) atomicOr(plan + kPlanOdd, (all[0] ? kOddBad : 0) | (all[1] ? kOddGone : 0));
         }
         __syncthreads();
     }
@@ -257,7 +260,7 @@ static size_t la_up(size_t n) { return (n + 1023) / 1024 * 1024; }
 struct LatentLayout {      // of the workspace: byte offsets, and what the sizes follow from
     int form, rows, tiles, passes, parts, part, pairs, blocks, tail_tiles;
     bool gathered;      // absorbed: pages that are not whole 32 rows are laid side by side first
-    size_t plan, lat, bad, kv, o_part, ml_part, few, there, tails, tail_bad, q_abs, sums, total;
+    size_t plan, lat, bad, gone, kv, o_part, ml_part, few, there, tails, tail_bad, tail_gone, q_abs, sums, total;
     long rows_of_heads;      // expanded rows, one a head, that there is room for
 };
 static int latent_form(const ktb200_latent_attn_params* p, int n_tokens, int max_kv) {
@@ -281,6 +284,7 @@ static int latent_layout(LatentLayout& y, const ktb200_latent_attn_params* p, in
         y.plan = take((plan_tiles_at(p->n_seqs) + 4L * y.tiles) * 4);
         y.lat = take((size_t)rows * kLatentRow * 2);
         y.bad = take((size_t)rows / 32 * 4);
+        y.gone = take((size_t)rows / 32 * 4);
     }
     if (y.form == 2) {
         const long room = (long)std::max<size_t>((size_t)rows, std::min(H * (size_t)rows, kLxBytes / (bn * 2)));
@@ -310,6 +314,7 @@ static int latent_layout(LatentLayout& y, const ktb200_latent_attn_params* p, in
             y.tail_tiles = n_tokens / kFewTile + 2 * p->n_seqs;
             y.tails = take((size_t)y.tail_tiles * kFewTile * kLatentRow * 2);
             y.tail_bad = take((size_t)y.tail_tiles * kFewTile / 8);
+            y.tail_gone = take((size_t)y.tail_tiles * kFewTile / 8);
         }
         y.q_abs = take((size_t)n_tokens * H * kLatent * 2);
         y.sums = take((size_t)n_tokens * H * kLatent * 2);
@@ -343,7 +348,7 @@ static int latent_map(CUtensorMap* map, const void* ptr, long width, long rows, 
 static int latent_rows(const ktb200_latent_attn_params* p, const LatentLayout& y, int n_tokens, uint8_t* ws, int sms, cudaStream_t s) {
     int* plan = (int*)(ws + y.plan);
     KTB_CUDA_CHECK(launch_pdl(latent_plan_kernel, dim3(1), dim3(32), (size_t)0, s, *p, n_tokens, (int)(y.rows / p->n_seqs), y.tiles, y.rows_of_heads, plan));
-    KTB_CUDA_CHECK(launch_pdl(latent_gather_kernel, dim3(std::min(y.rows / 32, 8 * sms)), dim3(256), (size_t)0, s, *p, plan, (__nv_bfloat16*)(ws + y.lat), (uint32_t*)(ws + y.bad)));
+    KTB_CUDA_CHECK(launch_pdl(latent_gather_kernel, dim3(std::min(y.rows / 32, 8 * sms)), dim3(256), (size_t)0, s, *p, plan, (__nv_bfloat16*)(ws + y.lat), (uint32_t*)(ws + y.bad), (uint32_t*)(ws + y.gone)));
     count_launch(2);
     return KTB200_OK;
 }
@@ -366,7 +371,7 @@ template <int N, int V> static int latent_expanded(const ktb200_latent_attn_para
     KTB_CUDA_CHECK(raise_smem_limit((const void*)latent_prompt_kernel<N, V>, kLpSmem));
     const int pairs = sms / 2, mt = (y.rows + 255) / 256;
     const int ctas = (int)std::min<long>((long)y.tiles * p->heads, 0x7fffffffL);
-    LatentPrompt a{(const int*)(ws + y.plan), (const uint32_t*)(ws + y.bad), p->n_seqs, p->heads, 0, y.parts > 1 ? y.part : 0, y.parts, p->scale * 1.4426950408889634f, (__nv_bfloat16*)p->out, p->out_stride,
+    LatentPrompt a{(const int*)(ws + y.plan), (const uint32_t*)(ws + y.bad), (const uint32_t*)(ws + y.gone), p->n_seqs, p->heads, 0, y.parts > 1 ? y.part : 0, y.parts, p->scale * 1.4426950408889634f, (__nv_bfloat16*)p->out, p->out_stride,
                    (float*)(ws + y.o_part), (float*)(ws + y.ml_part)};
     for (a.pass = 0; a.pass < y.passes; a.pass++) {
         KTB_CUDA_CHECK(launch_pdl(latent_expand_kernel, dim3((unsigned)(2 * std::min<long>((long)mt * p->heads, pairs))), dim3(kLxThreads), (size_t)kLxSmem, s, lat, w, m.k, a.plan, BN,
@@ -389,14 +394,14 @@ template <int N, int V> static int latent_absorbed(const ktb200_latent_attn_para
     int* there = (int*)(ws + y.there);
     const long rows = (long)n_tokens * p->heads, wide = (long)p->heads * kLatent;
     LatentFew a{*p, (int*)(ws + y.few), n_tokens, y.blocks, y.gathered ? 0x7fffffff : y.tail_tiles, y.pairs, p->page_size % 64 && !y.gathered ? 32 : 64, y.gathered ? (const int*)(ws + y.plan) : nullptr,
-                (const uint32_t*)(ws + y.bad), (const uint32_t*)(ws + y.tail_bad), p->scale * 1.4426950408889634f, (__nv_bfloat16*)(ws + y.sums), (float*)(ws + y.o_part), (float*)(ws + y.ml_part)};
+                (const uint32_t*)(ws + (y.gathered ? y.bad : y.tail_bad)), (const uint32_t*)(ws + (y.gathered ? y.gone : y.tail_gone)), p->scale * 1.4426950408889634f, (__nv_bfloat16*)(ws + y.sums), (float*)(ws + y.o_part), (float*)(ws + y.ml_part)};
     FewMaps m;
     int e = latent_map(&m.q, q_abs, kLatent, rows, kLatent, 64);
     if (!e) e = latent_map(&m.q_rot, p->q_rot, kLatentRot, rows, kLatentRot, 64);
     if (!e) e = y.gathered ? latent_map(&m.rows, ws + y.lat, kLatentRow, y.rows, kLatentRow, a.box) : latent_map(&m.rows, p->cache, kLatentRow, (long)p->n_pages * p->page_size, kLatentRow, a.box);
     if (!e) e = y.gathered ? latent_map(&m.tails, ws + y.lat, kLatentRow, y.rows, kLatentRow, a.box) : latent_map(&m.tails, tails, kLatentRow, (long)y.tail_tiles * kFewTile, kLatentRow, a.box);
     if (e) return e;
-    KTB_CUDA_CHECK(launch_pdl(latent_few_prep_kernel, dim3(1 + (y.gathered ? 0 : 4 * y.tail_tiles)), dim3(256), (size_t)0, s, a, tails, (uint32_t*)(ws + y.tail_bad)));
+    KTB_CUDA_CHECK(launch_pdl(latent_few_prep_kernel, dim3(1 + (y.gathered ? 0 : 4 * y.tail_tiles)), dim3(256), (size_t)0, s, a, tails, (uint32_t*)(ws + y.tail_bad), (uint32_t*)(ws + y.tail_gone)));
     count_launch();
     const int rc = absorb_launch<N, kLatent, false>(p, (const __nv_bfloat16*)p->q, p->q_stride, N + kLatentRot, q_abs, wide, n_tokens, there, sms, s);
     if (rc) return rc;

@@ -9,9 +9,11 @@
 namespace ktb {
 
 constexpr int kLatent = 512, kLatentRot = 64, kLatentRow = kLatent + kLatentRot, kLatentTile = 128;      // rows of a sequence begin at multiples of kLatentTile
-// the plan, ints: the rows of all sequences, the heads of a pass, query tiles, whether a row holds what is not finite; from kPlanSeqs on the first row of each portion and one more, then its keys (0: none, or not there), then the
+// the plan, ints: the rows of all sequences, the heads of a pass, query tiles, what rows are odd (kOddBad: one holds what is not finite, kOddGone: the page of a key is not
+// there); from kPlanSeqs on the first row of each portion and one more, then its keys (0: none, or not there), then the
 // tiles (int4, 16-byte aligned: first token, tokens, position of the first, portion)
-constexpr int kPlanRows = 0, kPlanHeads = 1, kPlanTiles = 2, kPlanBad = 3, kPlanSeqs = 4, kPlanTokens = 256;      // kPlanTokens: of a query tile
+constexpr int kPlanRows = 0, kPlanHeads = 1, kPlanTiles = 2, kPlanOdd = 3, kPlanSeqs = 4, kPlanTokens = 256;      // kPlanTokens: of a query tile
+constexpr int kOddBad = 1, kOddGone = 2;
 __host__ __device__ inline long plan_tiles_at(int n_seqs) { return ((long)kPlanSeqs + 2 * n_seqs + 1 + 3) / 4 * 4; }
 
 // positions that have a column of the page table: keys from there on are not there, and tokens at such positions see those that are
@@ -53,6 +55,10 @@ __device__ __forceinline__ bool latent_copy_row(const __nv_bfloat16* src, bool t
         if (lane + 32 * c < kLatentRow / 8) reinterpret_cast<uint4*>(dst)[lane + 32 * c] = whole || c == 2 ? v[c] : make_uint4(0, 0, 0, 0);
     return !whole;
 }
+// A sum of weights that is zero where keys are not there: the row sees none and becomes zero.  (Elsewhere all of its scores are -inf, and it is NaN.)  The parts of a row hand it on as -0
+constexpr uint32_t kNoKeys = 0x80000000u;
+__device__ __forceinline__ float latent_sum(float l, bool gone) { return gone && l == 0.f ? __uint_as_float(kNoKeys) : l; }
+__device__ __forceinline__ float latent_inverse(float l) { return __float_as_uint(l) == kNoKeys ? 0.f : 1.f / l; }
 // a sector of 32 bytes, from a thread
 template <typename T> __device__ __forceinline__ void latent_store32(T* to, const uint32_t* w) {
     asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");

@@ -44,7 +44,7 @@ struct LatentFew {
     int* plan;
     int n_tokens, block_cap, tail_cap, pairs, box;        // room for blocks and tails; rows of a copy: 64 or 32
     const int* rows_plan;                                 // rows side by side (latent_plan_kernel): no tails
-    const uint32_t *bad, *tail_bad;                       // a bit a row of those, or of the tails
+    const uint32_t *bad, *gone;                           // a bit a row of those, or of the tails: who sees it is NaN; nobody sees it
     float scale_log2;
     __nv_bfloat16* sums;                                  // [T][heads][512]
     float *o_part, *ml_part;                              // [2 pairs][128][512], [2 pairs][128][2]
@@ -54,13 +54,13 @@ __device__ __forceinline__ int few_whole(const LatentPortion& q) { return min(q.
 __device__ __forceinline__ int few_tails(const LatentPortion& q) { return q.count > 0 ? (q.end + kFewTile - 1) / kFewTile - few_whole(q) : 0; }
 
 // CTA 0: blocks, the line, its cuts.  The others: 32 rows of the tails each
-__global__ void __launch_bounds__(256) latent_few_prep_kernel(const LatentFew a, __nv_bfloat16* tails, uint32_t* tail_bad) {
+__global__ void __launch_bounds__(256) latent_few_prep_kernel(const LatentFew a, __nv_bfloat16* tails, uint32_t* tail_bad, uint32_t* tail_gone) {
     const ktb200_latent_attn_params& p = a.p;
     griddep_wait();
     griddep_launch_dependents();      // (behind the wait: the next kernels' weights then wait for nothing)
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, H = p.heads;
     __shared__ int sums[8], carry[3];
-    __shared__ uint32_t odd[8];
+    __shared__ uint32_t odd[8][2];
     if (blockIdx.x > 0) {
         const int g = blockIdx.x - 1, tile = g / 4;
         int seq = -1, at = 0, before = 0;
@@ -86,22 +86,24 @@ __global__ void __launch_bounds__(256) latent_few_prep_kernel(const LatentFew a,
         }
         if (seq < 0) return;
         const int key0 = (few_whole(q) + at) * kFewTile + (g & 3) * 32, keys = q.end;
-        uint32_t mine = 0;
+        uint32_t mine = 0, lost = 0;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const int key = key0 + 4 * warp + i;
             int page = -1;
             if (key < keys) page = p.page_table[(long)q.slot * p.max_pages + key / p.page_size];
             const bool there = (unsigned)page < (unsigned)p.n_pages;
+            if (key < keys && !there) lost |= 1u << (4 * warp + i);
             if (latent_copy_row((const __nv_bfloat16*)p.cache + ((long)page * p.page_size + key % p.page_size) * kLatentRow, there, tails + ((long)g * 32 + 4 * warp + i) * kLatentRow, true)) mine |= 1u << (4 * warp + i);
         }
-        if (lane == 0) odd[warp] = mine;
+        if (lane == 0) { odd[warp][0] = mine; odd[warp][1] = lost; }
         __syncthreads();
         if (tid == 0) {
-            uint32_t all = 0;
+            uint32_t all[2] = {0, 0};
 #pragma unroll
-            for (int i = 0; i < 8; i++) all |= odd[i];
-            tail_bad[g] = all;
+            for (int i = 0; i < 8; i++) { all[0] |= odd[i][0]; all[1] |= odd[i][1]; }
+            tail_bad[g] = all[0];
+            tail_gone[g] = all[1];
         }
         return;
     }
@@ -349,7 +351,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) __cluster_dims__(2, 1, 1) late
         const uint32_t tl = tmem + ((uint32_t)(32 * sp) << 16);
         const float c = a.scale_log2;
         const int room = latent_room(a.p);
-        const bool any_bad = a.rows_plan && a.rows_plan[kPlanBad] != 0;      // (rows side by side are copies, all of them; other tiles ahead of the tails are as the cache holds them)
+        const bool odd = a.rows_plan && a.rows_plan[kPlanOdd] != 0;      // (rows side by side are copies, all of them; other tiles ahead of the tails are as the cache holds them)
         int left = total, b = b_first, t = t_first, it = 0, seg = 0;
         while (left > 0) {
             const FewBlock k = blocks[b];
@@ -357,9 +359,18 @@ __global__ void __launch_bounds__(kFewThreads, 1) __cluster_dims__(2, 1, 1) late
             const int n = min(left, k.tiles - t), in = 64 * rank + r, tail = k.whole;
             const bool valid = in < k.rows;
             const int p = valid ? min(k.pos0 + (k.lead + in) / H, room - 1) : -1;      // the last key that the row sees
+            const int* table = a.p.page_table + (a.rows_plan ? 0 : (long)a.p.slot[a.p.seqs[k.seq]] * a.p.max_pages);
             float m_ref = -INFINITY, l = 0.f;
+            bool lost = false;      // keys of this half were not there
             for (int j = 0; j < n; j++) {
                 const int i = it + j, k0 = (t + j) * kFewTile + 64 * half;
+                uint2 gone = make_uint2(0, 0);      // (looked up while the scores are made)
+                if (t + j >= tail || a.rows_plan) {
+                    if (t + j >= tail || odd) gone = *reinterpret_cast<const uint2*>(a.gone + (a.rows_plan ? a.rows_plan[kPlanSeqs + k.seq] + k0 : (k.tail + t + j - tail) * kFewTile + 64 * half) / 32);
+                } else {
+                    gone.x = (unsigned)table[k0 / a.p.page_size] < (unsigned)a.p.n_pages ? 0 : 0xffffffffu;
+                    gone.y = a.box == 64 ? gone.x : (unsigned)table[(k0 + 32) / a.p.page_size] < (unsigned)a.p.n_pages ? 0 : 0xffffffffu;
+                }
                 bar_wait(smem_u32(&misc.s_full[i & 1]), (i >> 1) & 1);
                 tc_fence_after();
                 float s[64];
@@ -374,14 +385,19 @@ __global__ void __launch_bounds__(kFewThreads, 1) __cluster_dims__(2, 1, 1) late
                 // (the loads above are in registers only now)
 #pragma unroll
                 for (int x = 0; x < 64; x++) asm volatile("" : "+f"(s[x]));
-                if (any_bad || t + j >= tail) {
-                    const uint32_t* bits = a.rows_plan ? a.bad + (a.rows_plan[kPlanSeqs + k.seq] + k0) / 32 : a.tail_bad + ((k.tail + t + j - tail) * kFewTile + 64 * half) / 32;
-                    const uint2 w = *reinterpret_cast<const uint2*>(bits);
+                if (odd || t + j >= tail) {
+                    const uint2 w = *reinterpret_cast<const uint2*>(a.bad + (a.rows_plan ? a.rows_plan[kPlanSeqs + k.seq] + k0 : (k.tail + t + j - tail) * kFewTile + 64 * half) / 32);
                     if (w.x | w.y) {
 #pragma unroll
                         for (int x = 0; x < 64; x++)
                             if ((x < 32 ? w.x : w.y) >> (x & 31) & 1) s[x] = __int_as_float(0x7fffffff);
                     }
+                }
+                if (gone.x | gone.y) {
+                    lost = true;
+#pragma unroll
+                    for (int x = 0; x < 64; x++)
+                        if ((x < 32 ? gone.x : gone.y) >> (x & 31) & 1) s[x] = -INFINITY;
                 }
                 if (t + j >= tail) {      // (a tile that not all rows see whole, or one of the portion's last)
                     const int i1 = p - k0;
@@ -449,13 +465,15 @@ __global__ void __launch_bounds__(kFewThreads, 1) __cluster_dims__(2, 1, 1) late
             bar_wait(smem_u32(&misc.pv_done), (it - 1) & 1);
             tc_fence_after();
             asm volatile("barrier.cta.sync 1, 128;" ::: "memory");      // (the maxima are read)
+            l = latent_sum(l, lost);
             misc.top[0][half][r] = l;
             asm volatile("barrier.cta.sync 1, 128;" ::: "memory");
-            l += misc.top[0][half ^ 1][r];
+            const float other = misc.top[0][half ^ 1][r];
+            l = latent_sum(l + other, __float_as_uint(l) == kNoKeys || __float_as_uint(other) == kNoKeys);
             asm volatile("barrier.cta.sync 1, 128;" ::: "memory");
             const bool whole = n == k.tiles;
             const long row = (long)k.row0 + in, part = 2L * pair + (seg > 0);
-            const float inv = 1.f / l;      // (a row sees itself: without any weight its scores are all -inf, and it is NaN)
+            const float inv = latent_inverse(l);
             if (!whole && valid && half == 0) *reinterpret_cast<float2*>(a.ml_part + (part * kFewRows + in) * 2) = make_float2(m_ref, l);
 #pragma unroll 1
             for (int q = 0; q < 8; q++) {      // 128 columns from 128 half on of each 256
@@ -507,7 +525,7 @@ __global__ void __launch_bounds__(256) latent_few_merge_kernel(const LatentFew a
     const int parts = k.parts;
     auto at = [&](int i) { return (2L * (k.run0 + i) + (i == 0 ? k.late : 0)) * kFewRows + in; };
     float m = -INFINITY, l = 0.f, o[16];
-    bool nan = false;
+    bool nan = false, gone = false;
 #pragma unroll
     for (int x = 0; x < 16; x++) o[x] = 0.f;
     for (int i = lane; i < parts; i += 32) m = fmaxf(m, a.ml_part[at(i) * 2]);
@@ -520,12 +538,13 @@ __global__ void __launch_bounds__(256) latent_few_merge_kernel(const LatentFew a
 #pragma unroll
         for (int x = 0; x < 4; x++) v[x] = *reinterpret_cast<const float4*>(a.o_part + at(i) * kLatent + x * 128 + lane * 4);
         nan |= ml.y != ml.y;
+        gone |= __float_as_uint(ml.y) == kNoKeys;
         const float w = ml.x == -INFINITY ? 0.f : latent_exp2(ml.x - m);      // (0: what is not finite in the part's sum still makes the row NaN)
         l = fmaf(ml.y, w, l);
 #pragma unroll
         for (int x = 0; x < 4; x++) { o[4 * x] = fmaf(v[x].x, w, o[4 * x]); o[4 * x + 1] = fmaf(v[x].y, w, o[4 * x + 1]); o[4 * x + 2] = fmaf(v[x].z, w, o[4 * x + 2]); o[4 * x + 3] = fmaf(v[x].w, w, o[4 * x + 3]); }
     }
-    const float inv = nan ? __int_as_float(0x7fffffff) : 1.f / l;
+    const float inv = nan ? __int_as_float(0x7fffffff) : latent_inverse(latent_sum(l, gone));
     __nv_bfloat16* to = a.sums + ((long)k.row0 + in) * kLatent;
 #pragma unroll
     for (int x = 0; x < 4; x++) *reinterpret_cast<uint2*>(to + x * 128 + lane * 4) = make_uint2(latent_pack(o[4 * x] * inv, o[4 * x + 1] * inv), latent_pack(o[4 * x + 2] * inv, o[4 * x + 3] * inv));

@@ -24,7 +24,7 @@ static_assert(sizeof(LpMisc) <= 2048 && kLpSmem <= 232448, "shared memory budget
 
 struct LatentPrompt {
     const int* plan;
-    const uint32_t* bad;      // a bit a gathered row: its query rows are NaN
+    const uint32_t *bad, *gone;      // a bit a gathered row: who sees it is NaN; nobody sees it
     int n_seqs, heads, pass, part, parts;      // keys of a part (a multiple of 128; 0: one part)
     float scale_log2;
     __nv_bfloat16* out;
@@ -153,7 +153,7 @@ template <int N, int V> __global__ void __launch_bounds__(kLpThreads, 1) latent_
             const int p = pos0 + tok, w_first = pos0 + t * 128 + 32 * sp;      // the row's position and the warp's first
             const bool valid = tok < ntok;
             const float c = a.scale_log2;
-            const bool any_bad = a.plan[kPlanBad] != 0;
+            const int odd = a.plan[kPlanOdd];
             float m_ref = -INFINITY, l = 0.f;
             for (int j = 0; j < n; j++) {
                 const int k0 = k_lo + j * kLatentTile;
@@ -171,12 +171,14 @@ template <int N, int V> __global__ void __launch_bounds__(kLpThreads, 1) latent_
                 // (the loads above are in registers only now)
 #pragma unroll
                 for (int i = 0; i < 128; i++) asm volatile("" : "+f"(s[i]));
-                if (any_bad) {
-                    const uint4 b = *reinterpret_cast<const uint4*>(a.bad + (row0 + k0) / 32);
-                    const uint32_t w[4] = {b.x, b.y, b.z, b.w};
+                if (odd) {
+                    const uint4 b = *reinterpret_cast<const uint4*>(a.bad + (row0 + k0) / 32), g = *reinterpret_cast<const uint4*>(a.gone + (row0 + k0) / 32);
+                    const uint32_t w[4] = {b.x, b.y, b.z, b.w}, none[4] = {g.x, g.y, g.z, g.w};
 #pragma unroll
-                    for (int i = 0; i < 128; i++)
+                    for (int i = 0; i < 128; i++) {
                         if (w[i / 32] >> (i & 31) & 1) s[i] = __int_as_float(0x7fffffff);
+                        if (none[i / 32] >> (i & 31) & 1) s[i] = -INFINITY;
+                    }
                 }
                 if (!(k0 + kLatentTile - 1 <= w_first && k0 + kLatentTile <= k_hi)) {
                     const int i1 = min(p, k_hi - 1) - k0;
@@ -236,7 +238,8 @@ template <int N, int V> __global__ void __launch_bounds__(kLpThreads, 1) latent_
             tc_fence_after();
             const long row = (long)(tok0 + tok) * a.heads + h;
             float k = 1.f;
-            if (!cut) k = 1.f / l;      // (a row sees itself: without any weight its scores are all -inf, and it is NaN)
+            l = latent_sum(l, odd & kOddGone);
+            if (!cut) k = latent_inverse(l);
             else if (valid) *reinterpret_cast<float2*>(a.ml_part + (row * a.parts + blockIdx.z) * 2) = make_float2(m_ref, l);
             __nv_bfloat16* out = a.out + (long)(tok0 + tok) * a.out_stride + (long)h * V;
             const bool vec = (reinterpret_cast<uintptr_t>(out) & 31) == 0;
@@ -287,6 +290,7 @@ template <int V> __global__ void __launch_bounds__(256) latent_merge_kernel(cons
         float m = -INFINITY, l = 0.f, o[C];
 #pragma unroll
         for (int c = 0; c < C; c++) o[c] = 0.f;
+        bool gone = false;
         for (int p = 0; p < parts; p++) m = fmaxf(m, a.ml_part[(row * a.parts + p) * 2]);
 #pragma unroll 4
         for (int p = 0; p < parts; p++) {
@@ -301,11 +305,12 @@ template <int V> __global__ void __launch_bounds__(256) latent_merge_kernel(cons
                 const float2 u = *reinterpret_cast<const float2*>(src);
                 v[0] = u.x; v[1] = u.y;
             }
+            gone |= __float_as_uint(ml.y) == kNoKeys;
             l += ml.x == -INFINITY && ml.y == 0.f ? 0.f : ml.y * w;
 #pragma unroll
             for (int c = 0; c < C; c++) o[c] += w == 0.f ? 0.f : v[c] * w;
         }
-        const float k = 1.f / l;
+        const float k = latent_inverse(latent_sum(l, gone));
         __nv_bfloat16* out = a.out + (long)(item.x + i) * a.out_stride + (long)h * V + lane * C;
 #pragma unroll
         for (int c = 0; c < C; c++) out[c] = __float2bfloat16_rn(o[c] * k);

@@ -112,7 +112,7 @@ def latent_attention(q: torch.Tensor, q_rot: torch.Tensor, kv: torch.Tensor, w: 
     keys [W_K,h c | k_rot], values W_V,h c with w [heads * (nope + vdim), 512] (kv_b_proj's weight: every head's W_K above its W_V); q [T, heads * (nope + 64)] of any row stride, of which the
     first `nope` columns of a head are read; q_rot [T, heads, 64] as `latent_append` gives them.  nope, vdim: 64 or 128.  form: "expanded", "absorbed" (module docstring) or None, by
     the tokens a sequence has on average and batch.max_kv.  batch.max_kv: no position is max_kv or more.  Keys behind the
-    page table's last column are not there: tokens at such positions see the others.  To `out` (a view of any row stride) or a new tensor; rows of tokens in none of the batch's portions are
+    page table's last column and in pages outside the pool are not seen (tokens at such positions see the others; a row that sees no key becomes zero).  To `out` (a view of any row stride) or a new tensor; rows of tokens in none of the batch's portions are
     left as they were (in a new tensor: as they came)."""
     what = "latent_attention"
     T, dev = q.shape[0], q.get_device()

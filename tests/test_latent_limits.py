@@ -1,4 +1,4 @@
-"""latent_append, latent_attention and the layer on them at the limits of a call: latents that are not finite far ahead of the new tokens, positions behind the page table, portions that are not there, layers that
+"""latent_append, latent_attention and the layer on them at the limits of a call: latents that are not finite far ahead of the new tokens, positions behind the page table, portions and pages that are not there, layers that
 were built without memory or are captured before their first call, configurations that come back from a file."""
 import math
 from types import SimpleNamespace
@@ -187,6 +187,32 @@ def test_portions_whose_first_token_is_not_there(form):
         assert (got[5:] == 7).all()
         getattr(d.batch, name)[5] = held
     near(call(d, form), want, bound)
+
+
+# ------------------------------------------------------------------------------------------------ pages that are not there
+@gpu
+@FORMS
+@pytest.mark.parametrize("lens,heads,page,gone", [
+    ([(400, 70), (30, 60)], 2, 64, [(0, 0), (0, 3), (1, 1)]),
+    ([(400, 70), (30, 60)], 2, 16, [(0, 0), (0, 7), (0, 8), (0, 26), (1, 2)]),
+    ([(400, 70), (30, 60)], 3, 48, [(0, 2), (0, 8), (1, 0)]),
+    ([(1000, 3), (0, 1)], 16, 32, [(0, i) for i in range(8, 20)] + [(0, 31)]),
+    ([(4000, 5)], 128, 64, [(0, i) for i in range(0, 40)]),      # whole runs of tiles without a key
+    ([(3000, 2)], 4, 64, [(0, i) for i in range(47)]),            # no key at all, in several parts
+    ([(0, 5), (100, 20)], 2, 64, [(0, 0)]),                       # no key at all
+    ([(0, 5), (100, 20)], 2, 16, [(0, 0)]),
+    ([(5000, 70)], 4, 64, [(0, i) for i in range(0, 79)]),        # parts of the keys, most of them empty
+])
+def test_keys_of_pages_that_are_not_there(form, lens, heads, page, gone):
+    """Keys in pages outside the pool are not seen; a row that sees no key becomes zero."""
+    d = draw(lens, heads=heads, page=page, seed=61)
+    for k, (i, column) in enumerate(gone):
+        d.cache.page_table[i, column] = -1 if k % 2 else d.kv.shape[0] + k
+    want, bound = definition(d)
+    got = call(d, form)
+    empty = (bound == 0).all(1)
+    assert (got[empty] == 0).all()
+    near(got[~empty], want[~empty], bound[~empty])
 
 
 # ------------------------------------------------------------------------------------------------ the layer
