@@ -275,10 +275,10 @@ static int latent_layout(LatentLayout& y, const ktb200_latent_attn_params* p, in
     size_t at = 0;
     auto take = [&](size_t n) { const size_t o = at; at += la_up(n); return o; };
     const size_t H = p->heads, bn = p->nope_dim + p->vdim;
-    const long tiled = ((long)max_kv + kLatentTile - 1) / kLatentTile * kLatentTile, rows = tiled * p->n_seqs;
+    y.gathered = y.form == 1 && p->page_size % 32 != 0;
+    const long tiled = ((long)max_kv + kLatentTile - 1) / kLatentTile * kLatentTile, rows = y.form == 2 || y.gathered ? tiled * p->n_seqs : 0;
     if (rows > (1L << 30)) { set_error("latent_attn: %d sequences of up to %d keys", p->n_seqs, max_kv); return KTB200_EINVAL; }
     y.rows = (int)rows;
-    y.gathered = y.form == 1 && p->page_size % 32 != 0;
     if (y.form == 2 || y.gathered) {
         y.tiles = n_tokens / kPlanTokens + p->n_seqs;
         y.plan = take((plan_tiles_at(p->n_seqs) + 4L * y.tiles) * 4);

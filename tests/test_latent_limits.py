@@ -215,6 +215,16 @@ def test_keys_of_pages_that_are_not_there(form, lens, heads, page, gone):
     near(got[~empty], want[~empty], bound[~empty])
 
 
+# ------------------------------------------------------------------------------------------------ calls without tokens, and very many sequences
+@gpu
+def test_decoded_tokens_of_very_many_sequences():
+    """Sequences times max_kv above 2^30: the absorbed form has no rows of all keys to make room for."""
+    d = draw([(5, 1)] * 9000, heads=1, seed=72)
+    near_keys = call(d, "absorbed")
+    d.batch.max_kv = 131072
+    assert torch.equal(call(d, None), near_keys) and torch.isfinite(near_keys).all()
+
+
 # ------------------------------------------------------------------------------------------------ the layer
 @gpu
 @pytest.mark.parametrize("scaling", [None, YARN])
