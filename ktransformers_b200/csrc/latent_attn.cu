@@ -260,7 +260,7 @@ static size_t la_up(size_t n) { return (n + 1023) / 1024 * 1024; }
 struct LatentLayout {      // of the workspace: byte offsets, and what the sizes follow from
     int form, rows, tiles, passes, parts, part, pairs, blocks, tail_tiles;
     bool gathered;      // absorbed: pages that are not whole 32 rows are laid side by side first
-    size_t plan, lat, bad, gone, kv, o_part, ml_part, few, there, tails, tail_bad, tail_gone, q_abs, sums, total;
+    size_t plan, lat, bad, gone, kv, o_part, ml_part, few, there, tails, tail_bad, tail_gone, tail_holes, q_abs, sums, total;
     long rows_of_heads;      // expanded rows, one a head, that there is room for
 };
 static int latent_form(const ktb200_latent_attn_params* p, int n_tokens, int max_kv) {
@@ -315,6 +315,7 @@ static int latent_layout(LatentLayout& y, const ktb200_latent_attn_params* p, in
             y.tails = take((size_t)y.tail_tiles * kFewTile * kLatentRow * 2);
             y.tail_bad = take((size_t)y.tail_tiles * kFewTile / 8);
             y.tail_gone = take((size_t)y.tail_tiles * kFewTile / 8);
+            y.tail_holes = take((size_t)y.tail_tiles * 16);
         }
         y.q_abs = take((size_t)n_tokens * H * kLatent * 2);
         y.sums = take((size_t)n_tokens * H * kLatent * 2);
@@ -394,14 +395,14 @@ template <int N, int V> static int latent_absorbed(const ktb200_latent_attn_para
     int* there = (int*)(ws + y.there);
     const long rows = (long)n_tokens * p->heads, wide = (long)p->heads * kLatent;
     LatentFew a{*p, (int*)(ws + y.few), n_tokens, y.blocks, y.gathered ? 0x7fffffff : y.tail_tiles, y.pairs, p->page_size % 64 && !y.gathered ? 32 : 64, y.gathered ? (const int*)(ws + y.plan) : nullptr,
-                (const uint32_t*)(ws + (y.gathered ? y.bad : y.tail_bad)), (const uint32_t*)(ws + (y.gathered ? y.gone : y.tail_gone)), p->scale * 1.4426950408889634f, (__nv_bfloat16*)(ws + y.sums), (float*)(ws + y.o_part), (float*)(ws + y.ml_part)};
+                (const uint32_t*)(ws + (y.gathered ? y.bad : y.tail_bad)), (const uint32_t*)(ws + (y.gathered ? y.gone : y.tail_gone)), (const uint4*)(ws + y.tail_holes), p->scale * 1.4426950408889634f, (__nv_bfloat16*)(ws + y.sums), (float*)(ws + y.o_part), (float*)(ws + y.ml_part)};
     FewMaps m;
     int e = latent_map(&m.q, q_abs, kLatent, rows, kLatent, 64);
     if (!e) e = latent_map(&m.q_rot, p->q_rot, kLatentRot, rows, kLatentRot, 64);
     if (!e) e = y.gathered ? latent_map(&m.rows, ws + y.lat, kLatentRow, y.rows, kLatentRow, a.box) : latent_map(&m.rows, p->cache, kLatentRow, (long)p->n_pages * p->page_size, kLatentRow, a.box);
     if (!e) e = y.gathered ? latent_map(&m.tails, ws + y.lat, kLatentRow, y.rows, kLatentRow, a.box) : latent_map(&m.tails, tails, kLatentRow, (long)y.tail_tiles * kFewTile, kLatentRow, a.box);
     if (e) return e;
-    KTB_CUDA_CHECK(launch_pdl(latent_few_prep_kernel, dim3(1 + (y.gathered ? 0 : 4 * y.tail_tiles)), dim3(256), (size_t)0, s, a, tails, (uint32_t*)(ws + y.tail_bad), (uint32_t*)(ws + y.tail_gone)));
+    KTB_CUDA_CHECK(launch_pdl(latent_few_prep_kernel, dim3(1 + (y.gathered ? 0 : 4 * y.tail_tiles)), dim3(256), (size_t)0, s, a, tails, (uint32_t*)(ws + y.tail_bad), (uint32_t*)(ws + y.tail_gone), (uint32_t*)(ws + y.tail_holes)));
     count_launch();
     const int rc = absorb_launch<N, kLatent, false>(p, (const __nv_bfloat16*)p->q, p->q_stride, N + kLatentRot, q_abs, wide, n_tokens, there, sms, s);
     if (rc) return rc;

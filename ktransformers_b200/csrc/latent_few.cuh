@@ -45,16 +45,17 @@ struct LatentFew {
     int n_tokens, block_cap, tail_cap, pairs, box;        // room for blocks and tails; rows of a copy: 64 or 32
     const int* rows_plan;                                 // rows side by side (latent_plan_kernel): no tails
     const uint32_t *bad, *gone;                           // a bit a row of those, or of the tails: who sees it is NaN; nobody sees it
+    const uint4* holes;                                   // for each tile of the tails: of its portion's first, whether pages ahead of it are not there
     float scale_log2;
     __nv_bfloat16* sums;                                  // [T][heads][512]
     float *o_part, *ml_part;                              // [2 pairs][128][512], [2 pairs][128][2]
 };
 
-__device__ __forceinline__ int few_whole(const LatentPortion& q) { return min(q.pos, q.end) / kFewTile; }
+__device__ __forceinline__ int few_whole(const LatentPortion& q) { return min(q.pos, q.end - 1) / kFewTile; }      // (at least one tile is behind them)
 __device__ __forceinline__ int few_tails(const LatentPortion& q) { return q.count > 0 ? (q.end + kFewTile - 1) / kFewTile - few_whole(q) : 0; }
 
 // CTA 0: blocks, the line, its cuts.  The others: 32 rows of the tails each
-__global__ void __launch_bounds__(256) latent_few_prep_kernel(const LatentFew a, __nv_bfloat16* tails, uint32_t* tail_bad, uint32_t* tail_gone) {
+__global__ void __launch_bounds__(256) latent_few_prep_kernel(const LatentFew a, __nv_bfloat16* tails, uint32_t* tail_bad, uint32_t* tail_gone, uint32_t* tail_holes) {
     const ktb200_latent_attn_params& p = a.p;
     griddep_wait();
     griddep_launch_dependents();      // (behind the wait: the next kernels' weights then wait for nothing)
@@ -97,13 +98,17 @@ __global__ void __launch_bounds__(256) latent_few_prep_kernel(const LatentFew a,
             if (latent_copy_row((const __nv_bfloat16*)p.cache + ((long)page * p.page_size + key % p.page_size) * kLatentRow, there, tails + ((long)g * 32 + 4 * warp + i) * kLatentRow, true)) mine |= 1u << (4 * warp + i);
         }
         if (lane == 0) { odd[warp][0] = mine; odd[warp][1] = lost; }
-        __syncthreads();
+        bool hole = false;
+        if (at == 0)      // (a quarter of them each)
+            for (int c = (g & 3) * 256 + tid; c < (few_whole(q) * kFewTile + p.page_size - 1) / p.page_size; c += 1024) hole |= (unsigned)p.page_table[(long)q.slot * p.max_pages + c] >= (unsigned)p.n_pages;
+        hole = __syncthreads_or(hole);
         if (tid == 0) {
             uint32_t all[2] = {0, 0};
 #pragma unroll
             for (int i = 0; i < 8; i++) { all[0] |= odd[i][0]; all[1] |= odd[i][1]; }
             tail_bad[g] = all[0];
             tail_gone[g] = all[1];
+            tail_holes[g] = hole;
         }
         return;
     }
@@ -361,13 +366,17 @@ __global__ void __launch_bounds__(kFewThreads, 1) __cluster_dims__(2, 1, 1) late
             const int p = valid ? min(k.pos0 + (k.lead + in) / H, room - 1) : -1;      // the last key that the row sees
             const int* table = a.p.page_table + (a.rows_plan ? 0 : (long)a.p.slot[a.p.seqs[k.seq]] * a.p.max_pages);
             float m_ref = -INFINITY, l = 0.f;
-            bool lost = false;      // keys of this half were not there
+            bool lost = false, holes = false;      // keys of this half were not there; there may be such
+            if (!a.rows_plan && t < tail) {
+                const uint4 h = a.holes[k.tail];
+                holes = h.x | h.y | h.z | h.w;
+            }
             for (int j = 0; j < n; j++) {
                 const int i = it + j, k0 = (t + j) * kFewTile + 64 * half;
-                uint2 gone = make_uint2(0, 0);      // (looked up while the scores are made)
+                uint2 gone = make_uint2(0, 0);
                 if (t + j >= tail || a.rows_plan) {
                     if (t + j >= tail || odd) gone = *reinterpret_cast<const uint2*>(a.gone + (a.rows_plan ? a.rows_plan[kPlanSeqs + k.seq] + k0 : (k.tail + t + j - tail) * kFewTile + 64 * half) / 32);
-                } else {
+                } else if (holes) {
                     gone.x = (unsigned)table[k0 / a.p.page_size] < (unsigned)a.p.n_pages ? 0 : 0xffffffffu;
                     gone.y = a.box == 64 ? gone.x : (unsigned)table[(k0 + 32) / a.p.page_size] < (unsigned)a.p.n_pages ? 0 : 0xffffffffu;
                 }

@@ -202,6 +202,7 @@ def test_portions_whose_first_token_is_not_there(form):
     ([(0, 5), (100, 20)], 2, 64, [(0, 0)]),                       # no key at all
     ([(0, 5), (100, 20)], 2, 16, [(0, 0)]),
     ([(5000, 70)], 4, 64, [(0, i) for i in range(0, 79)]),        # parts of the keys, most of them empty
+    ([(200, 5), (700, 9)], 4, 256, [(0, 0), (1, 1)]),             # pages of several tiles, of which the first tokens see some whole
 ])
 def test_keys_of_pages_that_are_not_there(form, lens, heads, page, gone):
     """Keys in pages outside the pool are not seen; a row that sees no key becomes zero."""
