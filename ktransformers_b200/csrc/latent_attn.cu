@@ -326,7 +326,7 @@ static int latent_layout(LatentLayout& y, const ktb200_latent_attn_params* p, in
     return KTB200_OK;
 }
 static int latent_check(const ktb200_latent_attn_params* p, int max_kv) {
-    if (!p || p->heads <= 0 || p->page_size <= 0 || p->max_pages <= 0 || p->n_slots <= 0 || p->n_pages <= 0 || p->n_seqs < 0 || max_kv <= 0) { set_error("latent_attn: bad sizes"); return KTB200_EINVAL; }
+    if (!p || p->heads <= 0 || p->page_size <= 0 || p->max_pages <= 0 || p->n_slots <= 0 || p->n_pages <= 0 || p->n_seqs < 0 || max_kv < 0) { set_error("latent_attn: bad sizes"); return KTB200_EINVAL; }
     if ((p->nope_dim != 64 && p->nope_dim != 128) || (p->vdim != 64 && p->vdim != 128)) { set_error("latent_attn: heads of %d + 64 and values of %d: 64 or 128 of each", p->nope_dim, p->vdim); return KTB200_EINVAL; }
     if (p->form < 0 || p->form > 2) { set_error("latent_attn: form %d", p->form); return KTB200_EINVAL; }
     if (!(p->scale > 0.f) || p->scale > 1e30f) { set_error("latent_attn: the scale has to be above zero"); return KTB200_EINVAL; }
@@ -423,7 +423,7 @@ int ktb200_latent_attn_form(const ktb200_latent_attn_params* p, int n_tokens, in
 
 size_t ktb200_latent_attn_workspace(const ktb200_latent_attn_params* p, int n_tokens, int max_kv) {
     LatentLayout y;
-    if (latent_check(p, max_kv) || n_tokens <= 0 || p->n_seqs == 0 || latent_layout(y, p, n_tokens, max_kv)) return 0;
+    if (latent_check(p, max_kv) || n_tokens <= 0 || p->n_seqs == 0 || max_kv == 0 || latent_layout(y, p, n_tokens, max_kv)) return 0;
     return y.total;
 }
 
@@ -431,6 +431,7 @@ int ktb200_latent_attn(const ktb200_latent_attn_params* p, int n_tokens, int max
     int rc = latent_check(p, max_kv);
     if (rc) return rc;
     if (n_tokens <= 0 || p->n_seqs == 0) return KTB200_OK;
+    if (max_kv == 0) { set_error("latent_attn: %d tokens and no keys", n_tokens); return KTB200_EINVAL; }
     if (!p->q || !p->q_rot || !p->w || !p->pos || !p->slot || !p->seqs || !p->page_table || !p->cache || !p->out) { set_error("latent_attn: null pointer"); return KTB200_EINVAL; }
     if (((uintptr_t)p->q | (uintptr_t)p->q_rot | (uintptr_t)p->w | (uintptr_t)p->cache) & 15) { set_error("latent_attn: q, q_rot, w and the cache have to be 16-byte aligned"); return KTB200_EINVAL; }
     LatentLayout y;

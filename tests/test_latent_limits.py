@@ -1,5 +1,6 @@
 """latent_append, latent_attention and the layer on them at the limits of a call: latents that are not finite far ahead of the new tokens, positions behind the page table, portions and pages that are not there, layers that
 were built without memory or are captured before their first call, configurations that come back from a file."""
+import ctypes as C
 import math
 from types import SimpleNamespace
 
@@ -8,6 +9,7 @@ import torch
 
 from latent_util import HALF, RANK, ROT, draw, near
 from test_latent_portions import YARN, Exact, layer
+from ktransformers_b200 import native
 from ktransformers_b200.models.modeling_deepseek_v3 import DeepseekV3Attention, DeepseekV3Config, DeepseekV3RotaryEmbedding, DeepseekV3YarnRotaryEmbedding, yarn_get_mscale, yarn_inv_freq
 from ktransformers_b200.operators.attention import KDeepseekV2Attention
 from ktransformers_b200.operators.latent_attention import LatentRotation, latent_append, latent_attention
@@ -217,6 +219,24 @@ def test_keys_of_pages_that_are_not_there(form, lens, heads, page, gone):
 
 
 # ------------------------------------------------------------------------------------------------ calls without tokens, and very many sequences
+def test_calls_without_tokens_or_portions_need_no_keys():
+    """(host code only)"""
+    base = dict(q=64, q_stride=2 * 192, q_rot=64, heads=2, nope_dim=128, vdim=128, w=64, scale=0.1, form=0, pos=64, slot=64, seqs=64, seqs_stride=1, n_seqs=1, page_table=64, n_slots=1, max_pages=4,
+                page_size=64, n_pages=9, cache=64, out=64, out_stride=256)
+    lib, p = native.lib(), native.LatentAttnParams(**base)
+    assert lib.ktb200_latent_attn(C.byref(p), 0, 0, None, 0, None) == native.OK
+    assert lib.ktb200_latent_attn(C.byref(native.LatentAttnParams(**{**base, "n_seqs": 0})), 4, 0, None, 0, None) == native.OK
+    assert lib.ktb200_latent_attn(C.byref(p), 4, 0, None, 0, None) == native.EINVAL
+    assert lib.ktb200_latent_attn(C.byref(p), 0, -1, None, 0, None) == native.EINVAL
+
+
+@gpu
+def test_a_call_without_tokens():
+    d = draw([(30, 0)], heads=2, seed=71)
+    d.batch.max_kv = 0
+    assert call(d, None).shape == (0, 256)
+
+
 @gpu
 def test_decoded_tokens_of_very_many_sequences():
     """Sequences times max_kv above 2^30: the absorbed form has no rows of all keys to make room for."""
