@@ -28,6 +28,8 @@ class StaticCache:
         self.value_cache = [None] * config.num_hidden_layers
         table = torch.arange(self.max_pages * max_batch_size, dtype=torch.int32, device=device).reshape(max_batch_size, self.max_pages)
         self.page_table_list = [table] * config.num_hidden_layers
+        # a batch of one token a sequence: the tokens' slots (and their portions' first rows), the portions' sizes
+        self.token_rows = torch.stack((torch.arange(max_batch_size, dtype=torch.int32, device=device), torch.ones(max_batch_size, dtype=torch.int32, device=device)))
         self.past_tokens = [0] * config.num_hidden_layers
         self.is_MLA = self.is_page = True
 

@@ -186,10 +186,12 @@ class KDeepseekV2Attention(BaseInjectedModule, DeepseekV3Attention):
         q, kva = q.reshape(T, -1), get("kv_a_proj_with_mqa")(x).reshape(T, -1)
         if not (q.dtype is bf16 is kva.dtype):
             return None
-        i = torch.arange(bsz, dtype=torch.int32, device=dev)
-        batch = ForwardBatch.portions(cache_position.reshape(-1).to(torch.int32).repeat(bsz), i.repeat_interleave(q_len), torch.stack((i * q_len, torch.full_like(i, q_len))), cache.max_pages * cache.page_size)
+        # index rows: a decoded token's slots and portions lie in the cache, so that a step makes its positions alone (made anew in each layer they were nine small launches of the step's 26)
+        one, here = cache.token_rows[:, :bsz], cache_position.reshape(1, q_len).expand(bsz, q_len).to(torch.int32).reshape(-1).contiguous()
+        slot, seqs = (one[0], one) if q_len == 1 else (one[0, :, None].expand(bsz, q_len).reshape(-1).contiguous(), one * q_len)
+        batch = ForwardBatch.portions(here, slot, seqs, cache.max_pages * cache.page_size)
         pages = SimpleNamespace(page_table=cache.page_table_list[layer], max_pages_per_seq=cache.max_pages, page_size=cache.page_size)
-        kv, angles = cache.key_cache[layer], position_ids.to(torch.int32).expand(bsz, q_len).reshape(-1)
+        kv, angles = cache.key_cache[layer], position_ids.expand(bsz, q_len).to(torch.int32).reshape(-1).contiguous()
         turn = LatentRotation(rot.inv_freq_on(dev) if yarn else rot.inv_freq.to(dev), gain=rot.gain if yarn else 1.0)
         q_rot = latent_append(q, kva, norm.weight, norm.variance_epsilon, batch, pages, kv, heads, nope, rot=turn, positions=angles)
         o = latent_attention(q, q_rot, kv, w, batch, pages, heads, nope, vdim, get("softmax_scale"), form="absorbed" if get("absorb_for_prefill") else None)
