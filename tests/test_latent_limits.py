@@ -246,6 +246,25 @@ def test_decoded_tokens_of_very_many_sequences():
     assert torch.equal(call(d, None), near_keys) and torch.isfinite(near_keys).all()
 
 
+# ------------------------------------------------------------------------------------------------ a scheduler's step
+@gpu
+@pytest.mark.parametrize("form", ["expanded", "absorbed", None])
+@pytest.mark.parametrize("page", [64, 16])
+def test_portions_and_decoded_tokens_in_one_call(form, page):
+    """A long portion beside decoded tokens and drafts over contexts of very different lengths, an empty portion among them: one form for all of them, each right."""
+    d = draw([(900, 1), (0, 700), (3000, 1), (17, 0), (40, 3), (0, 1), (500, 130)], heads=4, page=page, seed=81)
+    want, bound = definition(d)
+    near(call(d, form), want, bound)
+    start = d.kv.clone()
+    rot = LatentRotation(10000.0 ** (-torch.arange(0, 64, 2, dtype=torch.float64) / 64).cuda())
+    append(d, rot)
+    key = torch.cat([torch.arange(b, b + n, device="cuda") for b, n in d.lens])
+    at = d.cache.page_table[d.batch.slot.long(), key // page].long(), key % page
+    assert (d.kv[at] != start[at]).any(-1).all()
+    start[at] = d.kv[at]
+    assert torch.equal(d.kv.view(torch.int16), start.view(torch.int16))
+
+
 # ------------------------------------------------------------------------------------------------ the layer
 @gpu
 @pytest.mark.parametrize("scaling", [None, YARN])
@@ -274,6 +293,23 @@ def test_layer_at_the_end_of_its_cache(scaling):
         token = run(262, 1)
         again = op._portion(x[:, 262:], where(262, 1)[None].expand(2, 1), cache, where(262, 1))
         assert torch.equal(rows, full) and (token.float() - again.float()).norm() <= 2 * 1.6e-2 * again.float().norm()      # (both are that far off at most)
+
+
+@gpu
+@pytest.mark.parametrize("heads", [4, 128])
+def test_layer_with_a_cache_much_longer_than_its_context(heads):
+    """Parts of the keys, passes over the heads and workspaces follow the cache's size; results do not."""
+    from ktransformers_b200.models.custom_cache import StaticCache
+    cfg, plain = layer(heads, 128, YARN, seed=9)
+    exact = Exact(cfg, plain)
+    op = KDeepseekV2Attention("blk.0.self_attn", None, cfg, plain, "cuda", "cuda")
+    cache, at = StaticCache(cfg, max_batch_size=2, max_cache_len=100000, device="cuda"), 0
+    for n in (200, 1, 100, 3):
+        x, where = torch.randn(2, n, 512, device="cuda").bfloat16(), torch.arange(at, at + n, device="cuda")[None].expand(2, n)
+        with torch.no_grad():
+            y, want = op(x, position_ids=where, past_key_value=cache, cache_position=where[0])[0], exact(x, where)
+        at += n
+        assert (y.float() - want).norm() <= 1.6e-2 * want.norm()      # (some ten roundings of 1.65e-3 one behind the other are 5.2e-3, three times that)
 
 
 def test_scaled_rotation_of_a_layer_built_without_memory():
