@@ -419,8 +419,9 @@ int ktb200_latent_step(const ktb200_latent_step_params* p, void* stream);
  *   rot_split: pairs of layout 0 come out in layout 1, as DeepSeek's caches hold them.  Latent: x / sqrt(mean x^2 + eps) * norm_weight, rounded once.
  * ktb200_latent_attn: out[t][h][:] = soft-max attention of [q_nope | q_rot] over the sequence's keys [W_K,h c_j | k_j], values W_V,h c_j, j <= pos[t]; w [heads][nope_dim + vdim][512] holds
  *   W_K,h above W_V,h (kv_b_proj).  Latents of 512 + 64, nope_dim and vdim 64 or 128, scale > 0.  form 1 (absorbed): the queries go to the latents and sums of latents to the values; 2 (expanded):
- *   keys and values are made of the latents once a call; 0: the one that takes less (ktb200_latent_attn_form).  max_kv: no position of the call is max_kv or more.  workspace: 1024-byte aligned,
- *   ktb200_latent_attn_workspace bytes (which also gives 0 for arguments that the call refuses).
+ *   keys and values are made of the latents once a call; 0: the one that takes less (ktb200_latent_attn_form).  max_kv: no position of the call is max_kv or more.  q: rows at
+ *   multiples of 16 bytes.  workspace: 1024-byte aligned, ktb200_latent_attn_workspace bytes (which also gives 0 for arguments that the call refuses); in form 2, and in form 1 over pages that are no
+ *   whole 32 rows, whose rows are laid side by side first, it follows max_kv times the portions.
  * ------------------------------------------------------------------------------------------ */
 typedef struct ktb200_latent_append_params {
     const void* q; long q_stride; int heads, nope_dim;

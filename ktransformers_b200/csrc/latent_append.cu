@@ -1,10 +1,10 @@
 // The append to the paged latent cache (ktb200_latent_append): rotation of all heads' rotated query columns and of the key's, the norm of the latent, the row of the token's page.
 //     (a, b) -> gain (a cos x - b sin x, b cos x + a sin x), x = position * frequency;  c / sqrt(mean c^2 + eps) * weight;  one rounding each
 // Angles are fp64 up to their remainder of whole turns (in 32 bits a position of 100,000 loses 2^-8 of a radian), everything else fp32.
-// Bound by instructions (110 a warp and run of 8 columns) and, for its bytes, by the rotated query columns (16 KB a token each way with 128 heads of 64: 2000 tokens 15.9 us, 4.4 TB/s); a decode step
-// by the chain launch, position, angle, store (3.6 us).
+// Bound by instructions (2000 tokens of 128 heads: 10.6 M of warps, 165 for 32 runs of 8 columns, issue slots 67 % busy; 12 portions of 16 heads: 25.3 M, 72 %) and, for its bytes, by the rotated query
+// columns (16 KB a token each way with 128 heads of 64: 2000 tokens 16.0 us, 4.4 TB/s); a decode step by the chain launch, position, angle, store (3.6 us).
 // Split: the first CTAs take a latent row a warp; the others some heads of a token, or all heads of up to eight, four runs of 8 columns a thread (a load and a store of 16 bytes each), which are
-// loaded ahead of the angles.  (A token a CTA, its loads behind the angles and layouts chosen at run time: 2000 tokens 21 us, 12 portions of 16 heads 75, now 35.)
+// loaded ahead of the angles.  (A token a CTA, its loads behind the angles and layouts chosen at run time: 2000 tokens 21 us, 12 portions of 16 heads 75, now 34.)
 #include <algorithm>
 #include <type_traits>
 

@@ -16,9 +16,10 @@
 namespace ktb {
 
 constexpr size_t kLxBytes = (size_t)2 << 30;
-// Tokens a sequence on average from which the expanded form takes less, by the call's keys.  128 heads, absorbed / expanded: 64 tokens behind 1000 66 / 68 us, 96 95 / 68; behind 8000 96 241 / 325,
-// 128 303 / 327; behind 30000 128 1032 / 1331; 8 x 128 behind 4000 818 / 953.  16 heads: 128 behind 1000 42 / 44, behind 30000 146 / 206.  (What the expanded form makes of the keys is the same for
-// all numbers of tokens, but with few keys its launches and first tiles are most of it)
+// Tokens a sequence on average from which the expanded form takes less, by the call's keys.  128 heads, absorbed / expanded: 64 tokens behind 1000 66 / 67 us, 96 90 / 68; behind 8000 96 228 / 325,
+// 128 292 / 328; behind 30000 128 953 / 1339; 8 x 128 behind 4000 1319 / 1609.  16 heads: 128 behind 1000 51 / 58, behind 30000 146 / 209.  (What the expanded form makes of the keys is the same for
+// all numbers of tokens, but with few keys its launches and first tiles are most of it.)  One form for a whole call: portions far from the average take the wrong one (2000 tokens beside 63 decoded
+// ones behind 4000 keys 2050 us, in two calls 373)
 constexpr int kLatentFew = 144, kLatentFewShort = 64, kLatentShort = 2048;
 
 // ------------------------------------------------------------------------------------------------ plan and rows

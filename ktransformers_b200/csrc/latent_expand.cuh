@@ -5,7 +5,7 @@
 // from L2 the copies bound the kernel (4049 rows, 128 heads: 120 us).
 //     warp 0 TMA: weights of a new head run by run of 64 columns as the last products of the old one are done with them, rows through a ring; a pair's bytes are counted by the first CTA's barriers
 //     warp 1 of the first CTA the pair's products; warps 4-7 and 8-11 results, 64 columns at a time through shared memory and out by TMA.  Two accumulators of bn columns.  (Sectors of 32 bytes
-//     stored by the threads took 120 us for 4049 rows and 128 heads, 86 without the stores: a tile has only 512 columns of products to hide its 64 KB of results behind)
+//     stored by the threads took 120 us for 4049 rows and 128 heads, so 112: a tile has only 512 columns of products to hide its 64 KB of results behind)
 // Tiles stand in one line, rows fastest, cut into equal runs, one a pair.
 // Results: [head of the pass][row][bn], rows of the plan (a multiple of 128: a CTA's rows are all there or not at all), one rounding.
 #pragma once

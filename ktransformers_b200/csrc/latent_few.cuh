@@ -9,9 +9,10 @@
 //     warps 2-5 soft-max: a thread owns a row and half of the tile's keys; P (bf16, each weight 2^-9 of itself off) goes to shared memory.  The running maximum is raised, and O scaled, only when a
 //     tile's outgrows it by 2^8
 // All tiles of all blocks stand in one line that is cut into equal runs, one a pair; blocks that are cut leave fp32 parts for latent_few_merge_kernel, whole ones are done.
-// Tiles that not all rows see whole, or whose last rows are not there, come from `tails`: copies with zeros for what is not there or not finite (latent_few_prep_kernel).
-// Bound by the copies: 278 KB a pair and tile from L2 at 12 TB/s, 3900 cycles of which products take 2518 (45 tokens behind 30000 keys: 334 us, 180 with the copies left out, 250 with the products
-// left out); keys' tiles in L2 ahead of their use did not help (358).
+// Tiles that not all rows see whole, or whose last rows are not there, come from `tails`: copies with zeros for what is not there or not finite, and bits that say so (latent_few_prep_kernel).
+// Pages of whole tiles that are not there are zeros too; a tile's are looked up only where prep found a portion with some (always: 32 decoded tokens 104 us, now 101).
+// Bound by its copies beside the products: 278 KB a pair and tile (45 tokens behind 30000 keys: 2.96 GB from L2 in 325 us, 9.1 TB/s, tensor pipe 59 % active; 32 decoded tokens: 457 MB in 81 us with
+// 242 MB of them from memory, 34 %).  Keys' tiles in L2 ahead of their use did not help (341 -> 358).
 // Shared memory: queries 72 KB, keys 72, values 64, weights 16.  TMEM: O 256 columns, S two buffers of 64.
 #pragma once
 #include "latent_attn.cuh"
@@ -38,7 +39,6 @@ struct __align__(16) FewBlock {
 // from few_blocks_at
 constexpr int kFewLine = 0, kFewBlocks = 1, kFewRuns = 2, kFewPairs = 4, kFewRun = 2;
 __host__ __device__ inline long few_blocks_at(int pairs) { return (kFewPairs + 2L * pairs + 3) / 4 * 4; }
-__host__ 
 struct LatentFew {
     ktb200_latent_attn_params p;
     int* plan;

@@ -109,11 +109,12 @@ def latent_append(q: torch.Tensor, kva: torch.Tensor, weight: torch.Tensor, eps:
 def latent_attention(q: torch.Tensor, q_rot: torch.Tensor, kv: torch.Tensor, w: torch.Tensor, batch, cache, heads: int, nope: int, vdim: int, scale: float, form: Optional[str] = None,
                      out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """o [T, heads * vdim] = soft-max attention of the queries [q_nope | q_rot] over the latents of cache layer `kv` [pages, page_size, 512 + 64] up to each token's position, `ktb200_latent_attn`:
-    keys [W_K,h c | k_rot], values W_V,h c with w [heads * (nope + vdim), 512] (kv_b_proj's weight: every head's W_K above its W_V); q [T, heads * (nope + 64)] of any row stride, of which the
-    first `nope` columns of a head are read; q_rot [T, heads, 64] as `latent_append` gives them.  nope, vdim: 64 or 128.  form: "expanded", "absorbed" (module docstring) or None, by
-    the tokens a sequence has on average and batch.max_kv.  batch.max_kv: no position is max_kv or more.  Keys behind the
-    page table's last column and in pages outside the pool are not seen (tokens at such positions see the others; a row that sees no key becomes zero).  To `out` (a view of any row stride) or a new tensor; rows of tokens in none of the batch's portions are
-    left as they were (in a new tensor: as they came)."""
+    keys [W_K,h c | k_rot], values W_V,h c with w [heads * (nope + vdim), 512] (kv_b_proj's weight: every head's W_K above its W_V); q [T, heads * (nope + 64)], rows at multiples of 16 bytes, of which
+    the first `nope` columns of a head are read; q_rot [T, heads, 64] as `latent_append` gives them.  nope, vdim: 64 or 128.  form: "expanded", "absorbed" (module docstring) or None, by the tokens a
+    sequence has on average and batch.max_kv: one form for all portions, so that long ones and decoded tokens are better given in two calls.  batch.max_kv: no position is max_kv or more; the workspace
+    of the expanded form, and of pages that are no whole 32 rows, follows max_kv times the portions.  Keys behind the page table's last column and in pages outside the pool are not seen (tokens at
+    such positions see the others; a row that sees no key becomes zero).  To `out` (a view of any row stride) or a new tensor; rows of tokens in none of the batch's portions are left as they were (in
+    a new tensor: as they came)."""
     what = "latent_attention"
     T, dev = q.shape[0], q.get_device()
     index = _latent_batch(what, T, dev, kv, LATENT + LATENT_ROT, batch, cache)
