@@ -445,7 +445,7 @@ size_t ktb200_latent_attn_workspace(const ktb200_latent_attn_params* p, int n_to
 int ktb200_latent_attn(const ktb200_latent_attn_params* p, int n_tokens, int max_kv, void* workspace, size_t workspace_bytes, void* stream);
 
 /* paged latent KV write: StaticCache.update (archive/ktransformers/models/custom_cache.py:147-200)
- * kv_cache[page_idx[t]][page_offset[t]][0:512] = ckv[t], [512:576] = k_pe[t] */
+ * kv_cache[page_idx[t]][page_offset[t]][0:512] = ckv[t], [512:576] = k_pe[t]; nothing where page_idx[t] < 0 */
 int ktb200_mla_kv_write(void* kv_cache, int page_size, const void* ckv, const void* k_pe, const int* page_idx,
                         const int* page_offset, int n_tokens, void* stream);
 

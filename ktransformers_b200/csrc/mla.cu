@@ -477,6 +477,7 @@ __global__ void __launch_bounds__(128 * kMergeParts) mla_merge_kernel(const floa
 __global__ void __launch_bounds__(72) mla_kv_write_kernel(__nv_bfloat16* kv, int page_size, const __nv_bfloat16* ckv,
                                                           const __nv_bfloat16* k_pe, const int* page_idx, const int* page_off) {
     const int t = blockIdx.x, i = threadIdx.x;   // 72 x 16 B = 1152 B
+    if (page_idx[t] < 0) return;
     __nv_bfloat16* dst = kv + ((long)page_idx[t] * page_size + page_off[t]) * kDK;
     const uint4 v = (i < 64) ? reinterpret_cast<const uint4*>(ckv + (long)t * kDV)[i] : reinterpret_cast<const uint4*>(k_pe + (long)t * 64)[i - 64];
     reinterpret_cast<uint4*>(dst)[i] = v;

@@ -55,7 +55,9 @@ class StaticCache:
         k_out = self.key_cache[layer_idx]
         bsz, q_len = key_states.shape[0], key_states.shape[1]
         pos = cache_position.to(torch.int32).reshape(1, -1).expand(bsz, q_len)
-        page_idx = (pos // self.page_size + torch.arange(bsz, device=pos.device, dtype=torch.int32).reshape(bsz, 1) * self.max_pages).reshape(-1).contiguous()
+        # (a position that the cache does not have is written nowhere: its row would lie in the next sequence's pages, or behind the last one's)
+        there = (pos >= 0) & (pos < self.max_pages * self.page_size)
+        page_idx = (pos // self.page_size + torch.arange(bsz, device=pos.device, dtype=torch.int32).reshape(bsz, 1) * self.max_pages).masked_fill(~there, -1).reshape(-1).contiguous()
         page_off = (pos % self.page_size).reshape(-1).contiguous()
         ckv = key_states.reshape(-1, self.kv_lora_rank).contiguous()
         kpe = value_states.reshape(-1, self.qk_rope_head_dim).contiguous()

@@ -247,14 +247,14 @@ class KDeepseekV2Attention(BaseInjectedModule, DeepseekV3Attention):
         w = self.mla_wrapper
         if w.need_plan:
             # decode: one query per sequence, kv length = position + 1, identity page table of the static cache
-            kv_len = (position_ids.reshape(bsz, -1)[:, -1] + 1).to(torch.int32)
+            kv_len = (position_ids.reshape(bsz, -1)[:, -1] + 1).clamp(max=past_key_value.max_pages * past_key_value.page_size).to(torch.int32)      # (no row lies behind the cache's last)
             pages = past_key_value.max_pages
             indptr = torch.arange(0, bsz + 1, dtype=torch.int32, device=hidden_states.device) * pages
             w.plan(None, indptr, page_table.reshape(-1), kv_len, None, self.num_heads, self.kv_lora_rank, self.qk_rope_head_dim,
                    past_key_value.page_size, self.softmax_scale, q_nope.dtype, ckv_pages.dtype)
             w.max_pages_per_seq = pages
         else:   # the plan is static (identity page table); only the lengths move from step to step (a captured device copy)
-            w.kv_len_arr_buf[:bsz].copy_((position_ids.reshape(bsz, -1)[:, -1] + 1).to(torch.int32))
+            w.kv_len_arr_buf[:bsz].copy_((position_ids.reshape(bsz, -1)[:, -1] + 1).clamp(max=past_key_value.max_pages * past_key_value.page_size).to(torch.int32))
         attn = w.run(q_nope, q_pe.contiguous(), ckv_pages, kpe_pages).view(bsz, q_len, self.num_heads, self.kv_lora_rank)
         if fused:
             o = torch.empty((bsz, q_len, self.num_heads, self.v_head_dim), dtype=attn.dtype, device=attn.device)

@@ -296,6 +296,31 @@ def test_layer_at_the_end_of_its_cache(scaling):
 
 
 @gpu
+def test_one_token_step_behind_the_end_of_its_cache():
+    """A decoded token behind the static cache, by the layer's fused step and module by module (a rotation of another class): neither writes it anywhere, and both see what is there."""
+    from ktransformers_b200.models.custom_cache import StaticCache
+    from ktransformers_b200.operators.flashinfer_wrapper import MLAWrapper
+
+    class OtherRotary(DeepseekV3RotaryEmbedding):
+        pass
+
+    cfg, plain = layer(16, 128, None, seed=10)
+    x, past, outs = torch.randn(2, 3, 1, 512, device="cuda").bfloat16(), torch.randn(3, 128, 576, device="cuda").bfloat16(), []
+    for rot in (DeepseekV3RotaryEmbedding(64), OtherRotary(64)):
+        plain.rotary_emb = rot.to("cuda")
+        op = KDeepseekV2Attention("blk.0.self_attn", None, cfg, plain, "cuda", "cuda")
+        cache = StaticCache(cfg, max_batch_size=3, max_cache_len=128, device="cuda")
+        cache.key_cache[0].view(3, 128, 576).copy_(past)
+        op.mla_wrapper = MLAWrapper(2, cache.max_pages * 2)
+        with torch.no_grad():      # (the first call plans, the second does not)
+            for i, pos in enumerate((128, 150)):
+                outs.append(op(x[:, i], position_ids=torch.full((2, 1), pos, device="cuda"), past_key_value=cache, cache_position=torch.tensor([pos], device="cuda"))[0].float())
+        assert torch.equal(cache.key_cache[0].view(3, 128, 576), past)
+    for a, b in zip(outs[:2], outs[2:]):
+        assert torch.isfinite(a).all() and (a - b).norm() <= 2 * 1.6e-2 * b.norm()      # (some ten roundings of 1.65e-3 in each, three times that)
+
+
+@gpu
 @pytest.mark.parametrize("heads", [4, 128])
 def test_layer_with_a_cache_much_longer_than_its_context(heads):
     """Parts of the keys, passes over the heads and workspaces follow the cache's size; results do not."""
